@@ -9,6 +9,7 @@ from . import params, series
 from .layer import COMBINE_KINDS, EWS, BToSignature, LogEWS, configure
 from .logsig import log_level_sizes, log_signature_dim
 from .params import AParamBlockDiag, AParamConstant, AParamDiag, AParamEFM, AParamGeneral, AParamJordanRepeated, B
+from .token_ops import decayed_attention, decayed_attention_step, token_embedding, vocab_loss
 from .series import check_series_q, series_error_bound, suggest_series_q
 
 __all__ = [
@@ -27,6 +28,10 @@ __all__ = [
     "check_series_q",
     "series_error_bound",
     "suggest_series_q",
+    "decayed_attention",
+    "decayed_attention_step",
+    "token_embedding",
+    "vocab_loss",
     "log_level_sizes",
     "log_signature_dim",
     "params",

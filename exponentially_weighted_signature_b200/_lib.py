@@ -16,6 +16,9 @@ LIB_PATH = os.path.join(HERE, "libews_b200.so")
 EWS_OK = 0
 EWS_ERR_WORKSPACE = 3
 EWS_ERR_LOOKBACK_TIMEOUT = 5
+EWS_ERR_INDEX = 6
+EWS_DTYPE_F32 = 0
+EWS_DTYPE_BF16 = 1
 EWS_NOALLOC_SCRATCH_BYTES = 16 << 20
 
 EWS_F_UNIFORM = 1
@@ -56,6 +59,16 @@ EXPORTED = (
     "ews_gated_clock_work_size",
     "ews_gated_clock_fwd",
     "ews_gated_clock_bwd",
+    "ews_embed_fwd",
+    "ews_embed_work_size",
+    "ews_embed_bwd",
+    "ews_decay_work_size",
+    "ews_decay_fwd",
+    "ews_decay_bwd",
+    "ews_decay_step",
+    "ews_vocab_work_size",
+    "ews_vocab_fwd",
+    "ews_vocab_bwd",
     "ews_read_device_status",
     "ews_status_fold",
     "ews_error_string",
@@ -167,6 +180,67 @@ class DenseArgs(ctypes.Structure):
     ]
 
 
+class DecayArgs(ctypes.Structure):
+    """Mirror of ``ews_decay_args``."""
+
+    _fields_ = [
+        ("batch", _c_int),
+        ("steps", _c_int),
+        ("heads", _c_int),
+        ("kv_heads", _c_int),
+        ("dk", _c_int),
+        ("dv", _c_int),
+        ("dtype", _c_int),
+        ("scale", ctypes.c_float),
+        ("q", _vp),
+        ("k", _vp),
+        ("v", _vp),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("rate", _vp),
+        ("lengths", _vp),
+        ("initial", _vp),
+        ("out", _vp),
+        ("final_state", _vp),
+        ("dout", _vp),
+        ("dout_stride", ctypes.c_int64 * 3),
+        ("dfinal", _vp),
+        ("dq", _vp),
+        ("dk_out", _vp),
+        ("dv_out", _vp),
+        ("dinitial", _vp),
+        ("work", _vp),
+        ("work_bytes", _c_size),
+    ]
+
+
+class VocabArgs(ctypes.Structure):
+    """Mirror of ``ews_vocab_args``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("dtype", _c_int),
+        ("targets_wide", _c_int),
+        ("hidden", _vp),
+        ("weight", _vp),
+        ("targets", _vp),
+        ("hidden_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("ignore", ctypes.c_int64),
+        ("loss", _vp),
+        ("lse", _vp),
+        ("dloss", _vp),
+        ("dhidden", _vp),
+        ("dweight", _vp),
+        ("work", _vp),
+        ("work_bytes", _c_size),
+        ("status", _vp),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -245,6 +319,27 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.ews_gated_clock_bwd.argtypes = [_vp, _vp, _vp, _f, _f, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp,
                                             _c_size, _vp]
         lib.ews_gated_clock_bwd.restype = _c_int
+        _i64 = ctypes.c_int64
+        lib.ews_embed_fwd.argtypes = [_vp, _c_int, _vp, _c_int, _i64, _i64, _i64, _i64, _f, _vp, _vp, _vp]
+        lib.ews_embed_fwd.restype = _c_int
+        lib.ews_embed_work_size.argtypes = [_i64, _i64, _i64]
+        lib.ews_embed_work_size.restype = _c_size
+        lib.ews_embed_bwd.argtypes = [_vp, _c_int, _vp, _c_int, _i64, _i64, _i64, _i64, _f, _i64, _vp, _vp, _c_size, _vp, _vp]
+        lib.ews_embed_bwd.restype = _c_int
+        lib.ews_decay_work_size.argtypes = [ctypes.POINTER(DecayArgs), _c_int]
+        lib.ews_decay_work_size.restype = _c_size
+        for name in ("ews_decay_fwd", "ews_decay_bwd"):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(DecayArgs), _vp]
+            fn.restype = _c_int
+        lib.ews_decay_step.argtypes = [ctypes.POINTER(DecayArgs), _vp, _c_int, _vp, _vp, _vp]
+        lib.ews_decay_step.restype = _c_int
+        lib.ews_vocab_work_size.argtypes = [ctypes.POINTER(VocabArgs), _c_int]
+        lib.ews_vocab_work_size.restype = _c_size
+        for name in ("ews_vocab_fwd", "ews_vocab_bwd"):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(VocabArgs), _vp]
+            fn.restype = _c_int
         lib.ews_read_device_status.argtypes = [_vp, _vp, ctypes.POINTER(_c_int)]
         lib.ews_read_device_status.restype = _c_int
         lib.ews_diag_fwd_noalloc_status.argtypes = [_vp, ctypes.POINTER(_c_int)]
@@ -264,6 +359,8 @@ def check(rc: int, what: str) -> None:
         msg = load().ews_error_string(rc).decode()
         if rc == EWS_ERR_LOOKBACK_TIMEOUT:
             raise EWSLookbackTimeout(f"{what}: {msg} (code {rc})")
+        if rc == EWS_ERR_INDEX:
+            raise IndexError(f"{what}: {msg} (code {rc})")
         if rc == 1:
             raise ValueError(f"{what}: {msg} (code {rc})")
         if rc == 2:

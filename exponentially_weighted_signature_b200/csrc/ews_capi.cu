@@ -33,6 +33,7 @@ extern "C" const char* ews_error_string(int code) {
         case EWS_ERR_WORKSPACE: return "workspace missing or too small";
         case EWS_ERR_LAUNCH: return "CUDA launch failed";
         case EWS_ERR_LOOKBACK_TIMEOUT: return "look-back wait timed out";
+        case EWS_ERR_INDEX: return "token id, target or state slot out of range";
     }
     return "unknown error";
 }

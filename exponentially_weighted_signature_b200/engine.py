@@ -88,6 +88,29 @@ def _status_slot(device):
     return slot
 
 
+# Token ids, targets and state slots out of range: the kernel itself stores the code in this pinned word, so a
+# call adds no launch and no copy; the next call on the device raises IndexError.
+_INDEX = {}
+
+
+def index_word(device):
+    """(address of the device's pinned index status, the same word as a ctypes int)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    slot = _INDEX.get(idx)
+    if slot is None:
+        host = torch.zeros(1, dtype=torch.int32).pin_memory()
+        slot = _INDEX[idx] = (ctypes.c_void_p(host.data_ptr()), ctypes.c_int.from_address(host.data_ptr()), host)
+    return slot
+
+
+def raise_index(device) -> None:
+    """Raises (once) IndexError if an earlier token operator on ``device`` met an index out of range."""
+    word = index_word(device)[1]
+    if word.value != _lib.EWS_OK:
+        code, word.value = word.value, _lib.EWS_OK
+        _lib.check(code, "an earlier token operator on this device")
+
+
 def raise_pending(device) -> None:
     """Raises (once) the first look-back timeout that an earlier call on ``device`` reported."""
     sticky, host = _status_slot(device)

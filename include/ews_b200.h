@@ -41,6 +41,13 @@ typedef struct CUstream_st* ews_stream_t; /* = cudaStream_t */
 #define EWS_ERR_LOOKBACK_TIMEOUT 5   /* a device-side wait for a neighbouring chunk ran out (read
                                         with ews_read_device_status; the outputs are then invalid) */
 
+#define EWS_ERR_INDEX 6              /* a token id, a target or a state's slot out of range (set on the device
+                                        in the caller's status word; that entry counted as absent) */
+
+/* ---- element types of the token operators ------------------------------------------------------ */
+#define EWS_DTYPE_F32 0
+#define EWS_DTYPE_BF16 1
+
 /* ---- flags ----------------------------------------------------------------------------------- */
 #define EWS_F_UNIFORM 1u        /* uniform clock: per-sample constant flow/local tables (cached flows,
                                    ews/core/chen_scan.py:155-168 cached=True) */
@@ -325,6 +332,83 @@ int ews_gated_clock_fwd(const float* x, const float* w, const float* b, float in
 int ews_gated_clock_bwd(const float* x, const float* w, const float* b, float in_scale, float norm_constant,
                         const float* dtheta, int batch, int steps, int dim, float* dx, float* dw, float* db, void* work,
                         size_t work_bytes, ews_stream_t stream);
+
+/* ---- token embedding ------------------------------------------------------------------------------
+ * out (n, dim) = scale * table[ids] with ids (n) int64 (ids_wide) or int32, table (vocab, dim) of `dtype` with rows
+ * `table_stride` elements apart; arithmetic in float32, rounded once.
+ *   ews_embed_bwd: dtable (vocab, dim) of `dtype`, every row written: scale times the float32 sum of the rows of
+ *   dout (n, dim; rows `dout_stride` apart) whose id it is, in the order of the positions (bit-reproducible); rows
+ *   of the id `skip` (-1: none) stay zero. `work`: ews_embed_work_size bytes of device memory.
+ * An id out of range gives a zero row (no gradient) and sets *status (device or pinned host memory, may be NULL)
+ * to EWS_ERR_INDEX. */
+int ews_embed_fwd(const void* ids, int ids_wide, const void* table, int dtype, int64_t n, int64_t vocab, int64_t dim,
+                  int64_t table_stride, float scale, void* out, int* status, ews_stream_t stream);
+size_t ews_embed_work_size(int64_t n, int64_t vocab, int64_t dim);
+int ews_embed_bwd(const void* ids, int ids_wide, const void* dout, int dtype, int64_t n, int64_t vocab, int64_t dim,
+                  int64_t dout_stride, float scale, int64_t skip, void* dtable, void* work, size_t work_bytes, int* status,
+                  ews_stream_t stream);
+
+/* ---- decayed linear attention ---------------------------------------------------------------------
+ * S_t = exp(-rate_h) S_{t-1} + k_t v_t^T, out_t = scale q_t S_t for every sample and query head h; key/value head
+ * h / (heads / kv_heads). q (batch, steps, heads, dk), k (.., kv_heads, dk), v (.., kv_heads, dv) of `dtype` with
+ * contiguous last axes and element strides {batch, step, head}; rate (heads) float32; lengths (batch) int32 or NULL:
+ * positions at or beyond a sample's length are not read, give zeros and leave the state; initial (batch, heads, dk,
+ * dv) float32 or NULL (zero). Outputs are contiguous: out (batch, steps, heads, dv) of `dtype`, final_state like
+ * initial (may be NULL). dk, dv <= 128.
+ *   ews_decay_bwd: from dout (strides like q) and dfinal (may be NULL) the gradients dq, dk_out, dv_out (contiguous,
+ *   of `dtype`; shared heads summed in float32 in head order) and dinitial (float32, may be NULL). scale != 0.
+ *   ews_decay_step: one token per row on the states `state` (pool, heads, dk, dv), updated in place: q, k, v, out
+ *   without the step axis (its stride is not read), row b on state slots[b] (int32; NULL: b). A negative slot is an
+ *   idle row: zero output, no state touched; one >= pool likewise, with *status = EWS_ERR_INDEX. Two rows must not
+ *   share a slot.
+ * `work`: ews_decay_work_size(args, backward) bytes. */
+typedef struct {
+    int batch, steps, heads, kv_heads, dk, dv, dtype;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const float* rate;
+    const int* lengths;
+    const float* initial;
+    void* out;
+    float* final_state;
+    const void* dout;
+    int64_t dout_stride[3];
+    const float* dfinal;
+    void *dq, *dk_out, *dv_out;
+    float* dinitial;
+    void* work;
+    size_t work_bytes;
+} ews_decay_args;
+size_t ews_decay_work_size(const ews_decay_args* args, int backward);
+int ews_decay_fwd(const ews_decay_args* args, ews_stream_t stream);
+int ews_decay_bwd(const ews_decay_args* args, ews_stream_t stream);
+int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float* state, int* status,
+                   ews_stream_t stream);
+
+/* ---- vocabulary loss ------------------------------------------------------------------------------
+ * loss_n = logsumexp_v <hidden_n, weight_v> - <hidden_n, weight_{t_n}> for hidden (rows, dim) and weight (vocab, dim)
+ * of `dtype` (rows `hidden_stride` / `weight_stride` elements apart), targets (rows) int64 (targets_wide) or int32;
+ * 0 where the target is `ignore`. loss and lse (the row's logsumexp, kept for the backward) are float32.
+ *   ews_vocab_bwd: from dloss (rows) the gradients dhidden (rows, dim) and dweight (vocab, dim), contiguous, either
+ *   may be NULL. The logits are formed again in pieces of the vocabulary and never kept whole.
+ * A target out of range counts as ignored and sets *status to EWS_ERR_INDEX. `work`: ews_vocab_work_size(args,
+ * backward) bytes; it begins with a status block (see ews_read_device_status). */
+typedef struct {
+    int64_t rows, vocab, dim;
+    int dtype, targets_wide;
+    const void *hidden, *weight, *targets;
+    int64_t hidden_stride, weight_stride, ignore;
+    float *loss, *lse;
+    const float* dloss;
+    void *dhidden, *dweight;
+    void* work;
+    size_t work_bytes;
+    int* status;
+} ews_vocab_args;
+size_t ews_vocab_work_size(const ews_vocab_args* args, int backward);
+int ews_vocab_fwd(const ews_vocab_args* args, ews_stream_t stream);
+int ews_vocab_bwd(const ews_vocab_args* args, ews_stream_t stream);
 
 /* ---- utilities --------------------------------------------------------------------------------- */
 /* Every forward and backward workspace begins with a status block whose error word the call clears and
