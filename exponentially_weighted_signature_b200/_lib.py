@@ -212,6 +212,7 @@ class DecayArgs(ctypes.Structure):
         ("dinitial", _vp),
         ("work", _vp),
         ("work_bytes", _c_size),
+        ("status", _vp),
     ]
 
 
@@ -332,7 +333,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(DecayArgs), _vp]
             fn.restype = _c_int
-        lib.ews_decay_step.argtypes = [ctypes.POINTER(DecayArgs), _vp, _c_int, _vp, _vp, _vp]
+        lib.ews_decay_step.argtypes = [ctypes.POINTER(DecayArgs), _vp, _c_int, _vp, _vp]
         lib.ews_decay_step.restype = _c_int
         lib.ews_vocab_work_size.argtypes = [ctypes.POINTER(VocabArgs), _c_int]
         lib.ews_vocab_work_size.restype = _c_size

@@ -21,39 +21,14 @@
 // When (sample, head, slice) alone cannot fill the GPU, the axis is split: a state-only pass gives each
 // segment's own state, join_kernel chains them, and the segments run side by side from their states.
 // Rows at or beyond a sample's length are neither loaded nor multiplied; their outputs are zero.
-#include "ews_token.cuh"
+#include "ews_decay.cuh"
 
 namespace ews {
 namespace decay {
 
-using namespace token;
-
 constexpr int C = 64;      // tokens of a chunk
 constexpr int NT = 128;    // threads: four warps of 16 rows
 constexpr int MAXD = 128;  // widest head
-
-// One stream (batch, steps, heads, width): element strides, and the query heads that share one of its heads.
-template <typename T>
-struct Stream {
-    const T* p;
-    long sb, st, sh;
-    int group, width, vec;
-};
-
-template <typename T>
-struct Chain {
-    Stream<T> x, y, z;
-    T* out;          // (batch, steps, heads, dz), or
-    float* out32;    // the same in float32 (shared heads: summed afterwards)
-    const float* rate;
-    const int* lengths;
-    const float* init;  // state the chain starts from (may be null); element (i, j) of a head at i * init_r + j * init_c
-    float* fin;         // state it ends with (may be null)
-    long init_r, init_c, fin_r, fin_c;
-    float oscale, init_scale, fin_scale;
-    float* seg;      // (batch * heads, segments, dx, dz): the segments' own states, then their starting states
-    int batch, steps, heads, rev, segs, seg_chunks, slices;
-};
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -288,7 +263,7 @@ __global__ void __launch_bounds__(NT) chain_kernel(const __grid_constant__ Chain
     const int c0 = slice * DV;
     if (STATE && !a.fin && seg == a.segs - 1) return;  // no segment starts from it
     const long len = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
-    const long p0 = (long)seg * a.seg_chunks * C, p1 = min(p0 + (long)a.seg_chunks * C, (long)a.steps);
+    const long p0 = (long)seg * a.span, p1 = min(p0 + (long)a.span, (long)a.steps);
     const int dx = a.y.width, dz = a.z.width;
     const T* xb = STATE ? nullptr : a.x.p + b * a.x.sb + (h / a.x.group) * a.x.sh;
     const T* yb = a.y.p + b * a.y.sb + (h / a.y.group) * a.y.sh;
@@ -460,10 +435,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chain
     const long bh = e / per, i = (e - bh * per) / dz, j = e % dz;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
     const long len = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
-    const long span = (long)a.seg_chunks * C;
+    const long span = a.span;
     const float rate = a.rate[h];
     float s = a.init ? a.init[bh * per + i * a.init_r + j * a.init_c] * a.init_scale : 0.f;
-    for (int g = 0; g < a.segs; ++g) {
+    for (int k = 0; k < a.segs; ++k) {
+        const int g = a.down ? a.segs - 1 - k : k;
         float* p = a.seg + (bh * a.segs + g) * per + i * dz + j;
         const float own = *p;
         *p = s;
@@ -566,21 +542,30 @@ int pad_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 // Segments of the axis: as many as two CTAs on each of 148 SMs, but none shorter than four chunks, since each
 // costs a second reading of y and z and a state.
-void plan(int batch, int steps, int heads, int dz, int* slices, int* segs, int* seg_chunks) {
+void plan(int batch, int steps, int heads, int dz, int* slices, int* segs, int* span) {
     *slices = (dz + 63) / 64;
     const long ctas = (long)batch * heads * *slices;
     const int chunks = steps > 0 ? (steps + C - 1) / C : 1;
     long want = ctas >= 148 ? 1 : (296 + ctas - 1) / ctas;
     if (want > chunks / 4) want = chunks / 4;
     if (want < 1) want = 1;
-    *seg_chunks = (int)((chunks + want - 1) / want);
-    *segs = (chunks + *seg_chunks - 1) / *seg_chunks;
+    const int per = (int)((chunks + want - 1) / want);
+    *span = per * C;
+    *segs = (chunks + per - 1) / per;
 }
 
-size_t seg_bytes(int batch, int steps, int heads, int dx, int dz) {
-    int slices, segs, sc;
-    plan(batch, steps, heads, dz, &slices, &segs, &sc);
-    return segs > 1 ? sizeof(float) * (size_t)batch * heads * segs * dx * dz : 0;
+// The segments' states, for whichever form runs (a state in full precision needs its pass even over one segment).
+size_t seg_bytes(const ews_decay_args* a, int dx, int dz) {
+    int slices, segs, span;
+    plan(a->batch, a->steps, a->heads, dz, &slices, &segs, &span);
+    if (segs == 1) segs = 0;
+    if (a->dtype == EWS_DTYPE_BF16) {
+        const int t = tc_segments(a->batch, a->steps, a->heads, true, &span);
+        if (t > segs) segs = t;
+        const int f = tc_segments(a->batch, a->steps, a->heads, false, &span);
+        if (f > segs) segs = f;
+    }
+    return sizeof(float) * (size_t)a->batch * a->heads * segs * dx * dz;
 }
 
 template <typename T, int DK, int DV, int NS, bool STATE>
@@ -608,19 +593,43 @@ int launch_d(const Chain<T>& a, cudaStream_t s) {
     return launch<T, 128, 64, NS, STATE>(a, s);
 }
 
+template <typename T>
+int join(const Chain<T>& a, cudaStream_t s) {
+    const long total = (long)a.batch * a.heads * a.y.width * a.z.width;
+    join_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
+}
+
+// bfloat16 streams that TMA can read run on the tensor core's 5th-generation form. There a state that leaves in
+// float32 takes the state pass (three pieces of the weighted operand) whatever the split.
+int run_tc(Chain<bf16> a, cudaStream_t s) {
+    a.segs = tc_segments(a.batch, a.steps, a.heads, a.fin != nullptr, &a.span);
+    if (a.segs > 1 || a.fin) {
+        if (!a.seg) return EWS_ERR_WORKSPACE;
+        int rc = tc_chain(a, true, a.fin != nullptr, s);
+        if (rc != EWS_OK) return rc;
+        Chain<bf16> j = a;
+        j.down = a.rev;
+        if ((rc = join<bf16>(j, s)) != EWS_OK) return rc;
+        a.fin = nullptr;
+    }
+    return tc_chain(a, false, false, s);
+}
+
 // NS for a state that leaves the kernel in float32 is three, for one that only feeds rounded outputs two.
 template <typename T>
 int run_chain(Chain<T> a, cudaStream_t s) {
-    plan(a.batch, a.steps, a.heads, a.z.width, &a.slices, &a.segs, &a.seg_chunks);
     constexpr bool f32 = sizeof(T) == 4;
+    if constexpr (!f32) {
+        if (tc_fits(a)) return run_tc(a, s);
+    }
+    plan(a.batch, a.steps, a.heads, a.z.width, &a.slices, &a.segs, &a.span);
     const bool exact = a.fin != nullptr && !f32;
     int rc;
     if (a.segs > 1) {
         if (!a.seg) return EWS_ERR_WORKSPACE;
         rc = exact ? launch_d<T, f32 ? 1 : 3, true>(a, s) : launch_d<T, f32 ? 1 : 2, true>(a, s);
-        if (rc != EWS_OK) return rc;
-        const long total = (long)a.batch * a.heads * a.y.width * a.z.width;
-        join_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, s>>>(a);
+        if (rc != EWS_OK || (rc = join<T>(a, s)) != EWS_OK) return rc;
         return launch_d<T, f32 ? 1 : 2, false>(a, s);
     }
     return exact ? launch_d<T, f32 ? 1 : 3, false>(a, s) : launch_d<T, f32 ? 1 : 2, false>(a, s);
@@ -654,9 +663,9 @@ struct Sizes {
 
 Sizes sizes(const ews_decay_args* a, bool bwd) {
     Sizes z{};
-    z.seg = up(seg_bytes(a->batch, a->steps, a->heads, a->dk, a->dv));
+    z.seg = up(seg_bytes(a, a->dk, a->dv));
     if (bwd) {
-        const size_t t = up(seg_bytes(a->batch, a->steps, a->heads, a->dv, a->dk));
+        const size_t t = up(seg_bytes(a, a->dv, a->dk));
         if (t > z.seg) z.seg = t;
         const int d = a->dk > a->dv ? a->dk : a->dv;
         if (a->heads != a->kv_heads) z.part = up(sizeof(float) * (size_t)a->batch * a->steps * a->heads * d);
@@ -671,7 +680,7 @@ Chain<T> base(const ews_decay_args* a) {
     c.rate = a->rate, c.lengths = a->lengths;
     c.batch = a->batch, c.steps = a->steps, c.heads = a->heads;
     c.oscale = a->scale, c.init_scale = c.fin_scale = 1.f;
-    c.seg = static_cast<float*>(a->work);
+    c.seg = static_cast<float*>(a->work), c.status = a->status;
     return c;
 }
 
@@ -724,14 +733,14 @@ int backward(const ews_decay_args* a, const Sizes& z, cudaStream_t s) {
 }
 
 template <typename T>
-int step(const ews_decay_args* a, const int* slots, int pool, float* state, int* status, cudaStream_t s) {
+int step(const ews_decay_args* a, const int* slots, int pool, float* state, cudaStream_t s) {
     Step<T> p{};
     p.q = static_cast<const T*>(a->q), p.k = static_cast<const T*>(a->k), p.v = static_cast<const T*>(a->v);
     p.qb = a->q_stride[0], p.qh = a->q_stride[2], p.kb = a->k_stride[0], p.kh = a->k_stride[2];
     p.vb = a->v_stride[0], p.vh = a->v_stride[2];
     p.rate = a->rate, p.slots = slots, p.state = state, p.out = static_cast<T*>(a->out);
     p.batch = a->batch, p.heads = a->heads, p.group = a->heads / a->kv_heads, p.dk = a->dk, p.dv = a->dv;
-    p.pool = pool, p.scale = a->scale, p.status = status;
+    p.pool = pool, p.scale = a->scale, p.status = a->status;
     p.slices = (a->dv + STEP_COLS - 1) / STEP_COLS;
     const long ctas = (long)a->batch * a->heads * p.slices;
     if (ctas > 0x7FFFFFFFl) return EWS_ERR_UNSUPPORTED;
@@ -773,14 +782,13 @@ extern "C" int ews_decay_bwd(const ews_decay_args* a, ews_stream_t stream) {
     return a->dtype == EWS_DTYPE_BF16 ? backward<bf16>(a, z, s) : backward<float>(a, z, s);
 }
 
-extern "C" int ews_decay_step(const ews_decay_args* a, const int* slots, int pool, float* state, int* status,
-                              ews_stream_t stream) {
+extern "C" int ews_decay_step(const ews_decay_args* a, const int* slots, int pool, float* state, ews_stream_t stream) {
     const int rc = check(a);
     if (rc != EWS_OK) return rc;
     if (a->batch == 0) return EWS_OK;
     if (!a->rate || !a->q || !a->k || !a->v || !a->out || !state || pool < 0 || (!slots && pool < a->batch))
         return EWS_ERR_INVALID_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
-    return a->dtype == EWS_DTYPE_BF16 ? step<bf16>(a, slots, pool, state, status, s)
-                                      : step<float>(a, slots, pool, state, status, s);
+    return a->dtype == EWS_DTYPE_BF16 ? step<bf16>(a, slots, pool, state, s)
+                                      : step<float>(a, slots, pool, state, s);
 }

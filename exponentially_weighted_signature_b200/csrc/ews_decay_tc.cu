@@ -1,0 +1,510 @@
+// The decayed attention's chain on the 5th-generation tensor core (bfloat16 streams; the mathematics is in
+// ews_decay.cu). Chunks of 128 tokens, four products a chunk, all 128 rows of an accumulator in tensor memory:
+//
+//     P  = X Y^T            (tokens x tokens)      -> * decay, causal, to bfloat16 in tensor memory
+//     O1 = X State          (tokens x dz)
+//     U  = (w Y)^T Z        (dx x dz)              -> State = g^n State + U, float32 in registers
+//     O2 = P Z              (tokens x dz)          -> out = g^(i+1) O1 + O2
+//
+// One persistent CTA per SM walks (sample, head, segment) items. Warp 0 fetches tiles by TMA, warp 1 issues the
+// products, warps 2-5 (A) turn P into an operand and write the output (staged in the chunk's X tile, stored by
+// TMA), warps 6-13 (B) weight Y (in place, and its rounding residue beside it: the weighted operand is inexact, two
+// bfloat16 pieces carry it to 2^-16, three to 2^-24), keep the state and write its bfloat16 copy. The only chain
+// from chunk to chunk is U -> State -> O1; the loads, P and the output of neighbouring chunks run beside it.
+// Why 128 tokens: the accumulator has 128 rows; the waste of the upper half of P is 1/10 of a chunk's products.
+//
+// Reversed chains keep the rows' order and walk the chunks down: decays are then g^(j-i) for j >= i, a row's weight of
+// the carry g^(n-1-i), an update's g^(j+1).
+#include "ews_decay.cuh"
+#include "ews_tc.cuh"
+
+namespace ews {
+namespace decay {
+
+using namespace tc5;
+
+namespace {
+
+constexpr int TC = 128;                  // tokens of a chunk
+constexpr int BOX = TC * 128;            // bytes of 64 columns of a tile
+constexpr int TILE = 2 * BOX;
+constexpr int NTHR = 32 * 14;
+constexpr uint32_t TP = 0, TO1 = 128, TO2 = 256, TU = 384;  // tensor-memory columns
+
+struct Maps {
+    CUtensorMap x, y, z, out;
+};
+
+template <bool STATE, int NS>
+struct Lay {
+    static constexpr int ZST = STATE ? 2 : 1;
+    static constexpr int X = 0, Y = X + (STATE ? 0 : 2 * TILE), Z = Y + 2 * TILE, S = Z + ZST * TILE, LO = S + (STATE ? 0 : TILE),
+                         BARS = LO + (NS - 1) * TILE, PWA = BARS + 256, PWB = PWA + 4 * (TC + 4), END = PWB + 4 * (TC + 4);
+    static constexpr size_t bytes = END + 1024;
+};
+
+__device__ __forceinline__ void tma_load4(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int t, int h, int b) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store4(const CUtensorMap* map, const void* src, int x, int t, int h, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(smem_u32(src)),
+                 "r"(x), "r"(t), "r"(h), "r"(b)
+                 : "memory");
+}
+// A from tensor memory (two bfloat16 a column).
+__device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d),
+        "r"(a), "l"(bd), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t r[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// A group's own barrier, as an mbarrier: when a wait ran out somewhere the group gets false instead of waiting for
+// warps that have left.
+__device__ __forceinline__ bool group_sync(uint64_t* bar, uint32_t& phase, volatile int* fail) {
+    mbar_arrive(bar);
+    const bool ok = __all_sync(kFull, mbar_wait(bar, phase, fail));
+    phase ^= 1u;
+    return ok;
+}
+
+// An item's place: sample, head, its tokens [t0, t1), of which [t0, end) exist, and its chunks.
+struct Item {
+    int b, h, seg;
+    long bh;
+    int t0, t1, end, chunks;
+};
+
+template <bool STATE, int NS>
+__global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Chain<bf16> a, const __grid_constant__ Maps maps, int items) {
+    using L = Lay<STATE, NS>;
+    extern __shared__ unsigned char raw[];
+    unsigned char* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
+    uint64_t *x_full = bars, *y_full = bars + 2, *z_full = bars + 4, *x_empty = bars + 6, *y_empty = bars + 8, *z_empty = bars + 10;
+    uint64_t *p_full = bars + 12, *p_ready = bars + 13, *o_full = bars + 14, *o_free = bars + 15, *s_ready = bars + 16,
+             *yw_ready = bars + 17, *u_full = bars + 18, *xs_done = bars + 19, *drained = bars + 20, *sync_a = bars + 21, *sync_b = bars + 22;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 23);
+    volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int dx = a.y.width, dz = a.z.width;
+    const int dx16 = (dx + 15) & ~15, dz16 = (dz + 15) & ~15;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 12; ++i) mbar_init(bars + i, 1);
+        mbar_init(p_full, 1), mbar_init(o_full, 1), mbar_init(u_full, 1), mbar_init(xs_done, 1), mbar_init(drained, 1);
+        mbar_init(p_ready, 128), mbar_init(o_free, 128), mbar_init(s_ready, 256), mbar_init(yw_ready, 256);
+        mbar_init(sync_a, 128), mbar_init(sync_b, 256);
+        *fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_at;
+
+    auto place = [&](int w) {
+        Item it;
+        it.seg = w % a.segs;
+        it.bh = w / a.segs;
+        it.b = (int)(it.bh / a.heads), it.h = (int)(it.bh - (long)it.b * a.heads);
+        const int len = a.lengths ? min(max(a.lengths[it.b], 0), a.steps) : a.steps;
+        it.t0 = it.seg * a.span;
+        it.t1 = (int)min((long)it.t0 + a.span, (long)a.steps);
+        it.end = max(it.t0, min(it.t1, len));
+        it.chunks = (it.end - it.t0 + TC - 1) / TC;
+        return it;
+    };
+    auto skip = [&](const Item& it) {  // a state that no segment starts from
+        return STATE && !a.fin && it.seg == (a.rev ? 0 : a.segs - 1);
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            long n = 0;
+            bool ok = true;
+            for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
+                const Item it = place(w);
+                if (skip(it)) continue;
+                for (int c = 0; c < it.chunks; ++c, ++n) {
+                    const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, s = (int)(n & 1), zs = STATE ? s : 0;
+                    const uint32_t two = (uint32_t)((n >> 1) & 1) ^ 1u, zp = STATE ? two : (uint32_t)(n & 1) ^ 1u;
+                    if (!(ok = mbar_wait(y_empty + s, two, fail))) break;
+                    const int bx = dx > 64 ? 2 : 1, bz = dz > 64 ? 2 : 1;
+                    mbar_expect(y_full + s, bx * BOX);
+                    for (int j = 0; j < bx; ++j)
+                        tma_load4(&maps.y, y_full + s, sm + L::Y + s * TILE + j * BOX, j * 64, t, it.h / a.y.group, it.b);
+                    if (!STATE) {
+                        if (!(ok = mbar_wait(x_empty + s, two, fail))) break;
+                        mbar_expect(x_full + s, bx * BOX);
+                        for (int j = 0; j < bx; ++j)
+                            tma_load4(&maps.x, x_full + s, sm + L::X + s * TILE + j * BOX, j * 64, t, it.h / a.x.group, it.b);
+                    }
+                    if (!(ok = mbar_wait(z_empty + zs, zp, fail))) break;
+                    mbar_expect(z_full + zs, bz * BOX);
+                    for (int j = 0; j < bz; ++j)
+                        tma_load4(&maps.z, z_full + zs, sm + L::Z + zs * TILE + j * BOX, j * 64, t, it.h / a.z.group, it.b);
+                }
+            }
+            if (!ok) {  // what was asked for lands before the CTA leaves: at most the last two chunks' loads
+                for (long j = n > 1 ? n - 2 : 0; j <= n; ++j) {
+                    const uint32_t two = (uint32_t)((j >> 1) & 1);
+                    mbar_drain(y_full + (j & 1), two);
+                    if (!STATE) mbar_drain(x_full + (j & 1), two);
+                    mbar_drain(z_full + (STATE ? (j & 1) : 0), STATE ? two : (uint32_t)(j & 1));
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC >> 4) << 24);
+            constexpr uint32_t amn = 1u << 15, bmn = 1u << 16;
+            const uint32_t nz = (uint32_t)(dz16 >> 3) << 17, np = (uint32_t)(TC >> 3) << 17;
+            const int kx = dx16 / 16;
+            long n = 0;
+            bool ok = true;
+            for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
+                const Item it = place(w);
+                if (skip(it)) continue;
+                for (int c = 0; ok && c < it.chunks; ++c, ++n) {
+                    const int s = (int)(n & 1), zs = STATE ? s : 0;
+                    const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
+                    const uint32_t X = smem_u32(sm + L::X + s * TILE), Y = smem_u32(sm + L::Y + s * TILE),
+                                   Z = smem_u32(sm + L::Z + zs * TILE), SB = smem_u32(sm + L::S);
+                    if (!STATE) {
+                        if (!(ok = mbar_wait(x_full + s, two, fail) && mbar_wait(y_full + s, two, fail))) break;
+                        fence_after();
+                        for (int q = 0; q < kx; ++q) {
+                            const uint32_t off = (q >> 2) * BOX + (q & 3) * 32;
+                            mma_bf16(tmem + TP, desc(X + off, false), desc(Y + off, false), base | np, q > 0);
+                        }
+                        mma_commit(p_full);
+                        if (!(ok = mbar_wait(s_ready, ph, fail) && mbar_wait(o_free, ph ^ 1u, fail))) break;
+                        fence_after();
+                        for (int q = 0; q < kx; ++q)
+                            mma_bf16(tmem + TO1, desc(X + (q >> 2) * BOX + (q & 3) * 32, false), desc(SB + q * 2048, true, BOX),
+                                     base | bmn | nz, q > 0);
+                        mma_commit(xs_done);
+                    }
+                    if (!(ok = mbar_wait(yw_ready, ph, fail) && mbar_wait(z_full + zs, STATE ? two : ph, fail))) break;
+                    fence_after();
+                    for (int p = NS - 1; p >= 0; --p) {  // the smallest piece first
+                        const uint32_t W = p == 0 ? Y : smem_u32(sm + L::LO + (p - 1) * TILE);
+                        for (int q = 0; q < TC / 16; ++q)
+                            mma_bf16(tmem + TU, desc(W + q * 2048, true, BOX), desc(Z + q * 2048, true, BOX), base | amn | bmn | nz,
+                                     p < NS - 1 || q > 0);
+                    }
+                    mma_commit(u_full);
+                    if (!STATE) {
+                        if (!(ok = mbar_wait(p_ready, ph, fail))) break;
+                        fence_after();
+                        for (int q = 0; q < TC / 16; ++q)
+                            mma_bf16_ta(tmem + TO2, tmem + TP + q * 8, desc(Z + q * 2048, true, BOX), base | bmn | nz, q > 0);
+                        mma_commit(o_full);
+                    }
+                    mma_commit(y_empty + s);
+                    mma_commit(z_empty + zs);
+                }
+            }
+            if (!ok) {
+                mma_commit(drained);
+                mbar_drain(drained, 0);
+            }
+        }
+    } else if (warp < 6) {
+        if (!STATE) {  // group A
+            float* pw = reinterpret_cast<float*>(sm + L::PWA);
+            const int quarter = warp & 3, i = quarter * 32 + lane, tid = threadIdx.x - 64;
+            const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+            long n = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
+                const Item it = place(w);
+                if (!(ok = group_sync(sync_a, phase, fail))) break;
+                const float rate = a.rate[it.h];
+                pw[tid] = tid == 0 ? 1.f : expf(-rate * (float)tid);
+                if (tid == 0) pw[TC] = expf(-rate * (float)TC);
+                if (!(ok = group_sync(sync_a, phase, fail))) break;
+                for (int c = 0; c < it.chunks; ++c, ++n) {
+                    const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, m = min(TC, it.end - t);
+                    const uint32_t ph = (uint32_t)(n & 1);
+                    unsigned char* stage = sm + L::X + (int)(n & 1) * TILE;
+                    if (!(ok = __all_sync(kFull, mbar_wait(p_full, ph, fail)))) break;
+                    fence_after();
+                    for (int cb = 0; cb < 4; ++cb) {
+                        uint32_t packed[16];
+                        if (a.rev ? cb >= quarter : cb <= quarter) {
+                            float v[32];
+                            tmem_ld32(tmem + TP + lanes + cb * 32, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const int col = cb * 32 + j, gap = a.rev ? col - i : i - col;
+                                v[j] = gap >= 0 && col < m ? v[j] * pw[max(gap, 0)] : 0.f;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) packed[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) packed[j] = 0u;
+                        }
+                        tmem_st16(tmem + TP + lanes + cb * 16, packed);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    fence_before();
+                    mbar_arrive(p_ready);
+
+                    if (!(ok = __all_sync(kFull, mbar_wait(o_full, ph, fail)))) break;
+                    fence_after();
+                    const bool in = i < m;
+                    const float wi = a.rev ? pw[max(m - 1 - i, 0)] : pw[i + 1];
+                    for (int cb = 0; cb * 32 < dz; ++cb) {
+                        float u[32], v[32];
+                        tmem_ld32(tmem + TO1 + lanes + cb * 32, u);
+                        tmem_ld32(tmem + TO2 + lanes + cb * 32, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = in ? fmaf(wi, u[j], v[j]) * a.oscale : 0.f;
+                        if (a.out32) {
+                            if (t + i < it.t1) {
+                                float* o = a.out32 + (((long)it.b * a.steps + t + i) * a.heads + it.h) * dz + cb * 32;
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4)
+                                    if (cb * 32 + j < dz) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            }
+                        } else {
+                            unsigned char* row = stage + (cb >> 1) * BOX + i * 128;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int chunk = ((cb & 1) * 4 + j) ^ (i & 7);
+                                Vec<bf16, true>::store(reinterpret_cast<bf16*>(row + chunk * 16), v + 8 * j);
+                            }
+                        }
+                    }
+                    fence_before();
+                    mbar_arrive(o_free);
+                    if (!a.out32) {
+                        fence_async_smem();
+                        if (!(ok = group_sync(sync_a, phase, fail))) break;
+                        if (tid == 0) {
+                            for (int j = 0; j * 64 < dz; ++j) tma_store4(&maps.out, stage + j * BOX, j * 64, t, it.h, it.b);
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        }
+                    } else if (!(ok = group_sync(sync_a, phase, fail))) {
+                        break;
+                    }
+                    if (tid == 0) mbar_arrive(x_empty + (int)(n & 1));
+                }
+                if (!ok) break;
+                // positions without a token beyond the last chunk
+                const long first = it.t0 + (long)it.chunks * TC;
+                for (long e = tid; e < (it.t1 - first) * dz; e += 128) {
+                    const long at = (((long)it.b * a.steps + first + e / dz) * a.heads + it.h) * dz + e % dz;
+                    if (a.out32) a.out32[at] = 0.f;
+                    else a.out[at] = from_f<bf16>(0.f);
+                }
+            }
+            if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
+    } else {  // group B
+        float* pw = reinterpret_cast<float*>(sm + L::PWB);
+        const int quarter = warp & 3, half = (warp - 6) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 192;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        long n = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
+            const Item it = place(w);
+            if (skip(it)) continue;
+            if (!(ok = group_sync(sync_b, phase, fail))) break;
+            const float rate = a.rate[it.h];
+            if (tid <= TC) pw[tid] = tid == 0 ? 1.f : expf(-rate * (float)tid);
+            if (!(ok = group_sync(sync_b, phase, fail))) break;
+            float s[64];
+            const long per = (long)dx * dz;
+            const float* init = nullptr;
+            long ir = 0, ic = 0;
+            float scale = 1.f;
+            if (!STATE) {
+                if (a.segs > 1) init = a.seg + (it.bh * a.segs + it.seg) * per, ir = dz, ic = 1;
+                else if (a.init) init = a.init + it.bh * per, ir = a.init_r, ic = a.init_c, scale = a.init_scale;
+            }
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+                const int col = half * 64 + j;
+                s[j] = init && row < dx && col < dz ? init[row * ir + col * ic] * scale : 0.f;
+            }
+            for (int c = 0; c < it.chunks; ++c, ++n) {
+                const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, m = min(TC, it.end - t);
+                const int st = (int)(n & 1), zs = STATE ? st : 0;
+                const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
+                if (!STATE) {
+                    if (!(ok = __all_sync(kFull, mbar_wait(xs_done, ph ^ 1u, fail)))) break;
+                    if (half * 64 < dz) {
+                        unsigned char* p = sm + L::S + half * BOX + row * 128;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) Vec<bf16, true>::store(reinterpret_cast<bf16*>(p + ((j ^ (row & 7)) * 16)), s + 8 * j);
+                    }
+                    fence_async_smem();
+                    mbar_arrive(s_ready);
+                }
+                if (!(ok = __all_sync(kFull, mbar_wait(y_full + st, two, fail) && mbar_wait(z_full + zs, STATE ? two : ph, fail) &&
+                                                 (STATE || mbar_wait(p_full, ph, fail)))))
+                    break;
+                unsigned char* Y = sm + L::Y + st * TILE;
+                const int vecs = dx > 64 ? TILE / 16 : BOX / 16;
+                for (int e = tid; e < vecs; e += 256) {
+                    const int tok = (e >> 3) & (TC - 1);
+                    const float wt = tok < m ? pw[a.rev ? tok + 1 : m - 1 - tok] : 0.f;
+                    uint4* at = reinterpret_cast<uint4*>(Y + e * 16);
+                    const uint4 q = *at;
+                    const uint32_t in[4] = {q.x, q.y, q.z, q.w};
+                    uint32_t piece[NS][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float f0 = tok < m ? bf16_lo(in[j]) * wt : 0.f, f1 = tok < m ? bf16_hi(in[j]) * wt : 0.f;
+#pragma unroll
+                        for (int p = 0; p < NS; ++p) {
+                            const uint32_t u = pack_bf16(f0, f1);
+                            piece[p][j] = u;
+                            f0 -= bf16_lo(u), f1 -= bf16_hi(u);
+                        }
+                    }
+                    *at = make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]);
+#pragma unroll
+                    for (int p = 1; p < NS; ++p)
+                        *reinterpret_cast<uint4*>(sm + L::LO + (p - 1) * TILE + e * 16) =
+                            make_uint4(piece[p][0], piece[p][1], piece[p][2], piece[p][3]);
+                }
+                if (m < TC) {  // a short chunk: rows of Z that are no tokens must not reach a product
+                    unsigned char* Z = sm + L::Z + zs * TILE;
+                    for (int e = tid; e < TILE / 16; e += 256)
+                        if (((e >> 3) & (TC - 1)) >= m) *reinterpret_cast<uint4*>(Z + e * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+                mbar_arrive(yw_ready);
+                if (!(ok = __all_sync(kFull, mbar_wait(u_full, ph, fail)))) break;
+                fence_after();
+                const float gn = pw[m];
+                if (half * 64 < dz) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        float v[32];
+                        tmem_ld32(tmem + TU + lanes + half * 64 + q * 32, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) s[q * 32 + j] = fmaf(gn, s[q * 32 + j], v[j]);
+                    }
+                }
+                fence_before();
+            }
+            if (!ok) break;
+            float* fin = nullptr;
+            long fr = 0, fc = 0;
+            float fscale = 1.f;
+            if (STATE) fin = a.seg + (it.bh * a.segs + it.seg) * per, fr = dz, fc = 1;
+            else if (a.segs == 1 && a.fin) fin = a.fin + it.bh * per, fr = a.fin_r, fc = a.fin_c, fscale = a.fin_scale;
+            if (fin && row < dx)
+#pragma unroll
+                for (int j = 0; j < 64; ++j)
+                    if (half * 64 + j < dz) fin[row * fr + (half * 64 + j) * fc] = s[j] * fscale;
+        }
+    }
+    __syncthreads();
+    fence_after();
+    if (threadIdx.x == 0 && *fail) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+bool map_of(CUtensorMap* m, const bf16* p, int width, int steps, int heads, int batch, long st, long sh, long sb) {
+    EncodeFn enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)steps, (cuuint64_t)heads, (cuuint64_t)batch};
+    // an axis of one has no stride to speak of
+    const cuuint64_t strides[3] = {(cuuint64_t)(steps > 1 ? st * 2 : 16), (cuuint64_t)(heads > 1 ? sh * 2 : 16),
+                                   (cuuint64_t)(batch > 1 ? sb * 2 : 16)};
+    const cuuint32_t box[4] = {64, TC, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<bf16*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool mappable(const Stream<bf16>& s, int steps, int heads, int batch) {
+    const long most = 1l << 38;
+    return s.vec && (steps == 1 || (s.st > 0 && s.st < most)) && (heads == 1 || (s.sh > 0 && s.sh < most)) &&
+           (batch == 1 || (s.sb > 0 && s.sb < most));
+}
+
+template <bool STATE, int NS>
+int go(const Chain<bf16>& a, const Maps& m, cudaStream_t s) {
+    auto* kern = tc_kernel<STATE, NS>;
+    using L = Lay<STATE, NS>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
+    const long items = (long)a.batch * a.heads * a.segs;
+    if (items > 0x7FFFFFFFl) return EWS_ERR_UNSUPPORTED;
+    kern<<<(unsigned)(items < 148 ? items : 148), NTHR, L::bytes, s>>>(a, m, (int)items);
+    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
+}
+
+}  // namespace
+
+// The split of the axis that the cost model prefers, in chunks walked by the busiest CTA: a split walks each
+// chunk once more for the states alone, at about 0.6 of a chunk's time, and costs two launches (about two chunks).
+int tc_segments(int batch, int steps, int heads, bool state, int* span) {
+    const int chunks = (steps + TC - 1) / TC < 1 ? 1 : (steps + TC - 1) / TC;
+    const long rows = (long)batch * heads;
+    double best = 0;
+    int pick = 1;
+    for (int s = 1; s <= 64 && (s == 1 || s * 2 <= chunks); ++s) {
+        const int per = (chunks + s - 1) / s;
+        const double waves = (double)((rows * s + 147) / 148);
+        const double cost = waves * per * (s > 1 || state ? 1.6 : 1.0) + (s > 1 ? 2.0 : 0.0);
+        if (s == 1 || cost < best) best = cost, pick = s;
+    }
+    const int per = (chunks + pick - 1) / pick;
+    *span = per * TC;
+    return (chunks + per - 1) / per;
+}
+
+bool tc_fits(const Chain<bf16>& a) {
+    const int batch = a.batch, steps = a.steps;
+    return steps > 0 && a.z.width % 8 == 0 && mappable(a.x, steps, a.heads / a.x.group, batch) &&
+           mappable(a.y, steps, a.heads / a.y.group, batch) && mappable(a.z, steps, a.heads / a.z.group, batch) &&
+           (a.out32 || aligned16(a.out));
+}
+
+int tc_chain(const Chain<bf16>& a, bool state_only, bool exact, cudaStream_t s) {
+    Maps m{};
+    auto in = [&](CUtensorMap* map, const Stream<bf16>& t) {
+        return map_of(map, t.p, t.width, a.steps, a.heads / t.group, a.batch, t.st, t.sh, t.sb);
+    };
+    if (!in(&m.y, a.y) || !in(&m.z, a.z)) return EWS_ERR_LAUNCH;
+    if (state_only) return exact ? go<true, 3>(a, m, s) : go<true, 2>(a, m, s);
+    if (!in(&m.x, a.x)) return EWS_ERR_LAUNCH;
+    const int dz = a.z.width;
+    if (!a.out32 && !map_of(&m.out, a.out, dz, a.steps, a.heads, a.batch, (long)a.heads * dz, dz, (long)a.steps * a.heads * dz))
+        return EWS_ERR_LAUNCH;
+    return go<false, 2>(a, m, s);
+}
+
+}  // namespace decay
+}  // namespace ews

@@ -17,107 +17,19 @@
 // Operands are bfloat16. float32 inputs are split into three bfloat16 planes (8 bits each) and each product runs
 // over the six pairs of planes that matter (2^-24), smallest first, with the same kernel.
 // Rows whose target is ignored are packed as zeros, so nothing in them reaches a sum.
-#include <cuda.h>
-
-#include "ews_token.cuh"
+#include "ews_tc.cuh"
 
 namespace ews {
 namespace vocab {
 
 using namespace token;
+using namespace tc5;
 
 constexpr int BM = 128, BK = 64;
 constexpr int NTH = 192;               // warps: TMA, MMA, four of the epilogue
 constexpr int SMS = 148;
 constexpr long kPieceElems = 1l << 26; // entries of G (times planes) at a time: 128 MB
 constexpr float kLog2e = 1.4426950408889634f;
-
-// ---- tensor-core plumbing ------------------------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, P;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded: false when the wait ran out (the CTA's fail word is then set) or another role gave up before.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
-    for (int it = 0; it < kDefaultSpinLimit; ++it) {
-        if (mbar_try(bar, parity)) return true;
-        if ((it & 63) == 63 && *fail) return false;
-    }
-    *fail = 1;
-    return false;
-}
-// After a failure: lets what is in flight land, as far as it does.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
-    for (int it = 0; it < kDefaultSpinLimit; ++it)
-        if (mbar_try(bar, parity)) return;
-}
-__device__ __forceinline__ void tma_load(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
-
-// 128-byte-swizzled operand tile. K-major: rows of 64 k (128 bytes), 8 rows an atom, atoms 1024 bytes apart; a
-// k-step of 16 is 32 bytes on. MN-major: boxes of 64 mn (128 bytes) x 64 k rows, 8192 bytes each; 8 k rows an atom,
-// atoms 1024 bytes apart; a k-step of 16 is 2048 bytes on.
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, bool mn) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(mn ? (8192u >> 4) : 1u) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-__device__ __forceinline__ void mma_bf16(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-        "}\n" ::"r"(tmem),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float v[32]) {
-    uint32_t r[32];
-    __syncwarp();
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-        "%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // ---- the GEMM --------------------------------------------------------------------------------------------------
 
@@ -129,7 +41,7 @@ struct Gemm {
     int n_fast;           // consecutive tiles walk n
     int pairs;
     signed char ia[6], ib[6];
-    DeviceStatus* st;
+    int* status;          // the caller's word: a bounded wait that ran out
     // LSE, GRAD (m = rows, n = the piece's part of the vocabulary from v0 on)
     const int* target;    // -1: ignored
     int v0;
@@ -390,7 +302,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
     }
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (threadIdx.x == 0 && *fail) a.st->error = EWS_ERR_LOOKBACK_TIMEOUT;
+    if (threadIdx.x == 0 && *fail) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
 }
 
@@ -398,9 +310,8 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
 
 // Targets as vocabulary positions, -1 where there is no loss.
 __global__ void __launch_bounds__(256) target_kernel(const void* __restrict__ targets, int wide, long rows, long vocab, long ignore,
-                                                     int* __restrict__ out, float* __restrict__ picked, DeviceStatus* st, int* status) {
+                                                     int* __restrict__ out, float* __restrict__ picked, int* status) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i == 0) *st = DeviceStatus{0, 0, 0, 0};
     if (i >= rows) return;
     const long t = wide ? reinterpret_cast<const long long*>(targets)[i] : (long)reinterpret_cast<const int*>(targets)[i];
     int v = -1;
@@ -486,21 +397,6 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ a
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encoder() {
-    static EncodeFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
 
 // (planes, rows, cols) bfloat16 with rows `ld` apart; a box of 64 columns by `box_rows` rows.
 struct Operand {
@@ -589,7 +485,7 @@ Plan plan(const ews_vocab_args* a, bool bwd) {
     p.pieces = (v + most - 1) / most;
     p.piece = p.pieces == 1 ? v : ((v + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     p.pieces = (v + p.piece - 1) / p.piece;
-    size_t at = 256;
+    size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;
@@ -650,7 +546,7 @@ template <typename T>
 int begin(const ews_vocab_args* a, const Plan& p, char* w, float* picked, Operand* h, cudaStream_t s) {
     int* target = reinterpret_cast<int*>(w + p.target);
     target_kernel<<<(unsigned)((a->rows + 255) / 256), 256, 0, s>>>(a->targets, a->targets_wide, a->rows, a->vocab, a->ignore, target, picked,
-                                                                   reinterpret_cast<DeviceStatus*>(w), a->status);
+                                                                   a->status);
     bf16* at = reinterpret_cast<bf16*>(w + p.h);
     h->p = at, h->rows = a->rows, h->cols = p.ldd, h->ld = p.ldd, h->planes = p.planes, h->plane = a->rows * p.ldd;
     return pack<T>(a->hidden, a->hidden_stride, a->rows, (int)a->dim, target, at, p, h->plane, s);
@@ -663,7 +559,7 @@ int forward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     Operand h{}, wt{};
     int rc = begin<T>(a, p, w, picked, &h, s);
     Gemm g{};
-    g.st = reinterpret_cast<DeviceStatus*>(w);
+    g.status = a->status;
     g.target = reinterpret_cast<const int*>(w + p.target);
     g.part = reinterpret_cast<float2*>(w + p.part);
     g.picked = picked;
@@ -693,14 +589,14 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
         const long n = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
         if ((rc = weight_piece<T>(a, p, w, v0, n, &wt, s)) != EWS_OK) break;
         Gemm g{};
-        g.st = reinterpret_cast<DeviceStatus*>(w);
+        g.status = a->status;
         g.target = target, g.lse = a->lse, g.dloss = a->dloss;
         g.m = (int)a->rows, g.n = (int)n, g.k = (int)a->dim, g.v0 = (int)v0;
         g.g = G, g.ldg = (n + 7) / 8 * 8, g.g_plane = a->rows * g.ldg, g.planes = p.planes;
         if ((rc = gemm<GRAD, false, false>(g, h, wt, p.planes, s)) != EWS_OK) break;
         go.p = G, go.rows = a->rows, go.cols = n, go.ld = g.ldg, go.plane = g.g_plane, go.planes = p.planes;
         Gemm o{};
-        o.st = g.st, o.f32 = sizeof(T) == 4, o.ldo = a->dim, o.n = (int)a->dim, o.n_fast = 1;
+        o.status = a->status, o.f32 = sizeof(T) == 4, o.ldo = a->dim, o.n = (int)a->dim, o.n_fast = 1;
         if (a->dhidden) {  // dH += G W: K is the piece of the vocabulary
             Gemm d = o;
             d.m = (int)a->rows, d.k = (int)n, d.splits = p.split_h;

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib, engine
-from .engine import _fold_status, _ptr, _require_cuda, _stream_ptr, _timed
+from .engine import _ptr, _require_cuda, _stream_ptr, _timed
 
 _DTYPES = {torch.float32: _lib.EWS_DTYPE_F32, torch.bfloat16: _lib.EWS_DTYPE_BF16}
 MAX_HEAD = 128
@@ -142,6 +142,7 @@ class _Decayed(torch.autograd.Function):
         a.q, a.k, a.v = _ptr(q), _ptr(k), _ptr(v)
         a.q_stride, a.k_stride, a.v_stride = _strides(q), _strides(k), _strides(v)
         a.rate, a.lengths = _ptr(rate), _ptr(lengths)
+        a.status = engine.index_word(q.device)[0]
         return a
 
     @staticmethod
@@ -160,6 +161,7 @@ class _Decayed(torch.autograd.Function):
         a.work, a.work_bytes = _ptr(work), size
         with torch.cuda.device(dev), _timed("ews_decay_fwd", dev, B * T):
             _lib.check(lib.ews_decay_fwd(ctypes.byref(a), _stream_ptr(dev)), "ews_decay_fwd")
+        _after(dev)
         ctx.scale = scale
         ctx.save_for_backward(q, k, v, rate, initial, lengths)
         ctx.set_materialize_grads(False)
@@ -185,6 +187,7 @@ class _Decayed(torch.autograd.Function):
         a.work, a.work_bytes = _ptr(work), size
         with torch.cuda.device(dev), _timed("ews_decay_bwd", dev, B * T):
             _lib.check(lib.ews_decay_bwd(ctypes.byref(a), _stream_ptr(dev)), "ews_decay_bwd")
+        _after(dev)
         return (*grads, None, d0, None, None, None)
 
 
@@ -238,7 +241,7 @@ def decayed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: t
         if lengths.shape != (B,) or lengths.dtype != torch.int32:
             raise ValueError(f"lengths must be int32 ({B},), got {lengths.dtype} {tuple(lengths.shape)}")
         lengths = lengths.contiguous()
-    _same_device(q, k, v, rate, initial_state, lengths)
+    engine.raise_index(_same_device(q, k, v, rate, initial_state, lengths))
     out, end = _Decayed.apply(q, k, v, rate, initial_state, lengths, _scale(scale, dk), bool(return_state))
     return (out, end) if return_state else out
 
@@ -270,11 +273,12 @@ def decayed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ra
     a.batch, a.steps, a.heads, a.kv_heads, a.dk, a.dv = B, 1, H, k.shape[1], dk, dv
     a.dtype, a.scale = _DTYPES[q.dtype], _scale(scale, dk)
     a.q, a.k, a.v, a.rate, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), rate.data_ptr(), out.data_ptr()
+    a.status = engine.index_word(dev)[0]
     (a.q_stride[0], a.q_stride[2], _), (a.k_stride[0], a.k_stride[2], _), (a.v_stride[0], a.v_stride[2], _) = (
         q.stride(), k.stride(), v.stride())
     with torch.cuda.device(dev), _timed("ews_decay_step", dev, B, 1):
         _lib.check(_lib.load().ews_decay_step(ctypes.byref(a), _ptr(slots), state.shape[0], _ptr(state),
-                                              engine.index_word(dev)[0], _stream_ptr(dev)), "ews_decay_step")
+                                              _stream_ptr(dev)), "ews_decay_step")
     _after(dev)
     return out
 
@@ -305,11 +309,8 @@ class _VocabLoss(torch.autograd.Function):
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         a.loss, a.lse, a.work, a.work_bytes = _ptr(loss), _ptr(lse), _ptr(work), size
         a.status = engine.index_word(dev)[0]
-        with torch.cuda.device(dev):
-            with _timed("ews_vocab_fwd", dev, a.rows):
-                _lib.check(lib.ews_vocab_fwd(ctypes.byref(a), _stream_ptr(dev)), "ews_vocab_fwd")
-            if a.rows:
-                _fold_status(work, dev)
+        with torch.cuda.device(dev), _timed("ews_vocab_fwd", dev, a.rows):
+            _lib.check(lib.ews_vocab_fwd(ctypes.byref(a), _stream_ptr(dev)), "ews_vocab_fwd")
         ctx.ignore = ignore
         ctx.save_for_backward(hidden, weight, targets, lse)
         _after(dev)
@@ -328,12 +329,10 @@ class _VocabLoss(torch.autograd.Function):
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         a.lse, a.dloss, a.dhidden, a.dweight = _ptr(lse), _ptr(dloss), _ptr(dh), _ptr(dw)
         a.work, a.work_bytes = _ptr(work), size
-        with torch.cuda.device(dev):
-            with _timed("ews_vocab_bwd", dev, a.rows):
-                _lib.check(lib.ews_vocab_bwd(ctypes.byref(a), _stream_ptr(dev)), "ews_vocab_bwd")
-            if a.rows and (dh is not None or dw is not None):
-                _fold_status(work, dev)
-                engine.raise_pending(dev)
+        a.status = engine.index_word(dev)[0]
+        with torch.cuda.device(dev), _timed("ews_vocab_bwd", dev, a.rows):
+            _lib.check(lib.ews_vocab_bwd(ctypes.byref(a), _stream_ptr(dev)), "ews_vocab_bwd")
+        _after(dev)
         return dh, dw, None, None
 
 
@@ -355,6 +354,5 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
         raise ValueError(f"targets {tuple(targets.shape)} must have the shape {tuple(hidden.shape[:-1])}")
     dev = _same_device(hidden, weight, targets)
     engine.raise_index(dev)
-    engine.raise_pending(dev)
     loss = _VocabLoss.apply(hidden.reshape(-1, hidden.shape[-1]), weight, targets.reshape(-1), int(ignore_index))
     return loss.reshape(targets.shape)

@@ -361,7 +361,8 @@ int ews_embed_bwd(const void* ids, int ids_wide, const void* dout, int dtype, in
  *   without the step axis (its stride is not read), row b on state slots[b] (int32; NULL: b). A negative slot is an
  *   idle row: zero output, no state touched; one >= pool likewise, with *status = EWS_ERR_INDEX. Two rows must not
  *   share a slot.
- * `work`: ews_decay_work_size(args, backward) bytes. */
+ * status: device or pinned host memory, may be NULL; a bounded device wait that ran out sets
+ * EWS_ERR_LOOKBACK_TIMEOUT (the outputs are then invalid). `work`: ews_decay_work_size(args, backward) bytes. */
 typedef struct {
     int batch, steps, heads, kv_heads, dk, dv, dtype;
     float scale;
@@ -379,12 +380,12 @@ typedef struct {
     float* dinitial;
     void* work;
     size_t work_bytes;
+    int* status;
 } ews_decay_args;
 size_t ews_decay_work_size(const ews_decay_args* args, int backward);
 int ews_decay_fwd(const ews_decay_args* args, ews_stream_t stream);
 int ews_decay_bwd(const ews_decay_args* args, ews_stream_t stream);
-int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float* state, int* status,
-                   ews_stream_t stream);
+int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float* state, ews_stream_t stream);
 
 /* ---- vocabulary loss ------------------------------------------------------------------------------
  * loss_n = logsumexp_v <hidden_n, weight_v> - <hidden_n, weight_{t_n}> for hidden (rows, dim) and weight (vocab, dim)
@@ -392,8 +393,9 @@ int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float
  * 0 where the target is `ignore`. loss and lse (the row's logsumexp, kept for the backward) are float32.
  *   ews_vocab_bwd: from dloss (rows) the gradients dhidden (rows, dim) and dweight (vocab, dim), contiguous, either
  *   may be NULL. The logits are formed again in pieces of the vocabulary and never kept whole.
- * A target out of range counts as ignored and sets *status to EWS_ERR_INDEX. `work`: ews_vocab_work_size(args,
- * backward) bytes; it begins with a status block (see ews_read_device_status). */
+ * A target out of range counts as ignored and sets *status (device or pinned host memory, may be NULL) to
+ * EWS_ERR_INDEX; a bounded device wait that ran out sets EWS_ERR_LOOKBACK_TIMEOUT (the outputs are then invalid).
+ * `work`: ews_vocab_work_size(args, backward) bytes. */
 typedef struct {
     int64_t rows, vocab, dim;
     int dtype, targets_wide;
