@@ -755,7 +755,7 @@ int step(const ews_decay_args* a, const int* slots, int pool, float* state, cuda
 using namespace ews::decay;
 
 extern "C" size_t ews_decay_work_size(const ews_decay_args* a, int backward_pass) {
-    return check(a) == EWS_OK ? sizes(a, backward_pass != 0).total : 0;
+    return check(a) == EWS_OK && a->batch > 0 ? sizes(a, backward_pass != 0).total : 0;
 }
 
 extern "C" int ews_decay_fwd(const ews_decay_args* a, ews_stream_t stream) {

@@ -622,7 +622,7 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
 using namespace ews::vocab;
 
 extern "C" size_t ews_vocab_work_size(const ews_vocab_args* a, int backward_pass) {
-    return check(a) == EWS_OK ? plan(a, backward_pass != 0).bytes : 0;
+    return check(a) == EWS_OK && a->rows > 0 ? plan(a, backward_pass != 0).bytes : 0;
 }
 
 extern "C" int ews_vocab_fwd(const ews_vocab_args* a, ews_stream_t stream) {
