@@ -180,68 +180,6 @@ class DenseArgs(ctypes.Structure):
     ]
 
 
-class DecayArgs(ctypes.Structure):
-    """Mirror of ``ews_decay_args``."""
-
-    _fields_ = [
-        ("batch", _c_int),
-        ("steps", _c_int),
-        ("heads", _c_int),
-        ("kv_heads", _c_int),
-        ("dk", _c_int),
-        ("dv", _c_int),
-        ("dtype", _c_int),
-        ("scale", ctypes.c_float),
-        ("q", _vp),
-        ("k", _vp),
-        ("v", _vp),
-        ("q_stride", ctypes.c_int64 * 3),
-        ("k_stride", ctypes.c_int64 * 3),
-        ("v_stride", ctypes.c_int64 * 3),
-        ("rate", _vp),
-        ("lengths", _vp),
-        ("initial", _vp),
-        ("out", _vp),
-        ("final_state", _vp),
-        ("dout", _vp),
-        ("dout_stride", ctypes.c_int64 * 3),
-        ("dfinal", _vp),
-        ("dq", _vp),
-        ("dk_out", _vp),
-        ("dv_out", _vp),
-        ("dinitial", _vp),
-        ("work", _vp),
-        ("work_bytes", _c_size),
-        ("status", _vp),
-    ]
-
-
-class VocabArgs(ctypes.Structure):
-    """Mirror of ``ews_vocab_args``."""
-
-    _fields_ = [
-        ("rows", ctypes.c_int64),
-        ("vocab", ctypes.c_int64),
-        ("dim", ctypes.c_int64),
-        ("dtype", _c_int),
-        ("targets_wide", _c_int),
-        ("hidden", _vp),
-        ("weight", _vp),
-        ("targets", _vp),
-        ("hidden_stride", ctypes.c_int64),
-        ("weight_stride", ctypes.c_int64),
-        ("ignore", ctypes.c_int64),
-        ("loss", _vp),
-        ("lse", _vp),
-        ("dloss", _vp),
-        ("dhidden", _vp),
-        ("dweight", _vp),
-        ("work", _vp),
-        ("work_bytes", _c_size),
-        ("status", _vp),
-    ]
-
-
 _lock = threading.Lock()
 _lib = None
 
@@ -327,19 +265,20 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.ews_embed_work_size.restype = _c_size
         lib.ews_embed_bwd.argtypes = [_vp, _c_int, _vp, _c_int, _i64, _i64, _i64, _i64, _f, _i64, _vp, _vp, _c_size, _vp, _vp]
         lib.ews_embed_bwd.restype = _c_int
-        lib.ews_decay_work_size.argtypes = [ctypes.POINTER(DecayArgs), _c_int]
+        # the argument structs come packed as bytes (token_ops)
+        lib.ews_decay_work_size.argtypes = [ctypes.c_char_p, _c_int]
         lib.ews_decay_work_size.restype = _c_size
         for name in ("ews_decay_fwd", "ews_decay_bwd"):
             fn = getattr(lib, name)
-            fn.argtypes = [ctypes.POINTER(DecayArgs), _vp]
+            fn.argtypes = [ctypes.c_char_p, _vp]
             fn.restype = _c_int
-        lib.ews_decay_step.argtypes = [ctypes.POINTER(DecayArgs), _vp, _c_int, _vp, _vp]
+        lib.ews_decay_step.argtypes = [ctypes.c_char_p, _vp, _c_int, _vp, _vp]
         lib.ews_decay_step.restype = _c_int
-        lib.ews_vocab_work_size.argtypes = [ctypes.POINTER(VocabArgs), _c_int]
+        lib.ews_vocab_work_size.argtypes = [ctypes.c_char_p, _c_int]
         lib.ews_vocab_work_size.restype = _c_size
         for name in ("ews_vocab_fwd", "ews_vocab_bwd"):
             fn = getattr(lib, name)
-            fn.argtypes = [ctypes.POINTER(VocabArgs), _vp]
+            fn.argtypes = [ctypes.c_char_p, _vp]
             fn.restype = _c_int
         lib.ews_read_device_status.argtypes = [_vp, _vp, ctypes.POINTER(_c_int)]
         lib.ews_read_device_status.restype = _c_int

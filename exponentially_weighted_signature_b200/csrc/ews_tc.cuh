@@ -52,6 +52,11 @@ __device__ __forceinline__ void tma_load(const CUtensorMap* map, uint64_t* bar, 
         "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)),
+                 "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
 
 // 128-byte-swizzled operand tile. K-major: rows of 64 k (128 bytes), 8 rows an atom, atoms 1024 bytes apart; a
 // k-step of 16 is 32 bytes on. MN-major: boxes of 64 mn (128 bytes) by the k rows, `box` bytes each; 8 k rows an atom,

@@ -26,55 +26,65 @@ using namespace token;
 using namespace tc5;
 
 constexpr int BM = 128, BK = 64;
-constexpr int NTH = 192;               // warps: TMA, MMA, four of the epilogue
+constexpr int EPW = 8;                 // epilogue warps
+constexpr int NTH = 64 + EPW * 32;     // and one each for TMA and MMA
 constexpr int SMS = 148;
-constexpr long kPieceElems = 1l << 26; // entries of G (times planes) at a time: 128 MB
+constexpr long kPieceElems = 1l << 27; // entries of G (times planes) at a time: 256 MB
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- the GEMM --------------------------------------------------------------------------------------------------
 
 enum Epilogue { LSE, GRAD, OUT };
 
-struct Gemm {
-    int m, n, k;          // extents; C (m, n) = sum over plane pairs of A_ia (m, k) B_ib (n, k)^T
+// C (m, n) = sum over plane pairs of A_ia (m, k) B_ib (n, k)^T, in tiles and K splits.
+struct Job {
+    int m, n, k;
     int tiles_m, tiles_n, splits, blocks;  // k blocks of 64 a split, of every pair
-    int n_fast;           // consecutive tiles walk n
+    long units;
+    void* out;            // OUT: of the type of the inputs, rows n apart, or
+    float* acc;           // (splits, m, n) float32 partials:
+    int add;              // add to them (a later piece) rather than store
+};
+
+struct Gemm {
+    Job job[2];           // OUT: dH (A = G, K-major) and dW (A = G, MN-major) in one launch; else job[0]
     int pairs;
     signed char ia[6], ib[6];
     int* status;          // the caller's word: a bounded wait that ran out
+    int f32;              // the inputs are float32
     // LSE, GRAD (m = rows, n = the piece's part of the vocabulary from v0 on)
     const int* target;    // -1: ignored
     int v0;
-    float2* part;         // (tiles_n of the whole vocabulary, rows): maximum, sum
+    float2* part;         // (2 tiles_n of the whole vocabulary, rows): maximum, sum
     int part_tile0;
     float* picked;        // the target's logit
     const float *lse, *dloss;
     bf16* g;              // (planes, rows, ldg)
     long ldg, g_plane;
     int planes;
-    // OUT
-    void* out;            // of the type of the inputs, or null:
-    long ldo;
-    float* acc;           // (splits, m, n) float32 partials
-    int add;              // add to them (a later piece) rather than store
-    int f32;
 };
 
-template <int BN>
+struct Maps {
+    CUtensorMap a[2], b[2], g;
+};
+
+// GRAD gives a stage of operands for the epilogue's output tile: a warp's 32 rows by half the columns.
+template <int EPI, int BN>
 struct Tile {
     static constexpr int A = BM * BK * 2, B = BN * BK * 2, STAGE = A + B;
-    static constexpr int STAGES = BN == 256 ? 4 : 6;
-    static constexpr size_t bytes = (size_t)STAGES * STAGE + 1024 + 256;
+    static constexpr int OUTW = EPI == GRAD ? 32 * BN : 0;  // bytes a warp
+    static constexpr int STAGES = EPI == GRAD ? (BN == 256 ? 3 : 5) : BN == 256 ? 4 : 6;
+    static constexpr size_t bytes = (size_t)STAGES * STAGE + EPW * OUTW + 1024 + 256;
 };
 
-template <int EPI, int BN, bool AMN, bool BMN>
-__global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                                                   const __grid_constant__ Gemm a) {
-    using TL = Tile<BN>;
-    constexpr int S = TL::STAGES;
+template <int EPI, int BN>
+__global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Gemm a) {
+    using TL = Tile<EPI, BN>;
+    constexpr int S = TL::STAGES, HALF = BN / 2;
+    constexpr bool BMN = EPI == OUT;
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S * TL::STAGE);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S * TL::STAGE + EPW * TL::OUTW);
     uint64_t* empty = full + S;
     uint64_t* acc_full = empty + S;   // 2
     uint64_t* acc_empty = acc_full + 2;
@@ -85,7 +95,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, 128);
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, EPW * 32);
         mbar_init(drained, 1);
         *fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -98,18 +108,25 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_at;
-    const long units = (long)a.tiles_m * a.tiles_n * a.splits;
-    const int kblocks = (a.k + BK - 1) / BK;
+    const long units = a.job[0].units + (EPI == OUT ? a.job[1].units : 0);
 
-    // a unit's tile and k range
-    auto unit = [&](long u, int& tm, int& tn, int& sp, int& k0, int& k1) {
-        const long per = (long)a.tiles_m * a.tiles_n;
-        sp = (int)(u / per);
-        const long t = u - sp * per;
-        if (a.n_fast) tn = (int)(t % a.tiles_n), tm = (int)(t / a.tiles_n);
-        else tm = (int)(t % a.tiles_m), tn = (int)(t / a.tiles_m);
-        k0 = sp * a.blocks;
-        k1 = min(k0 + a.blocks, kblocks);
+    struct Unit {
+        int job, tm, tn, sp, k0, k1;
+    };
+    auto unit = [&](long u) {
+        Unit r;
+        r.job = EPI == OUT && u >= a.job[0].units ? 1 : 0;
+        if (r.job) u -= a.job[0].units;
+        const Job& j = a.job[r.job];
+        const long per = (long)j.tiles_m * j.tiles_n;
+        r.sp = (int)(u / per);
+        const long t = u - r.sp * per;
+        // neighbours share the larger operand's rows: a gradient's G, the logits' piece of the weight
+        if (EPI == OUT) r.tn = (int)(t % j.tiles_n), r.tm = (int)(t / j.tiles_n);
+        else r.tm = (int)(t % j.tiles_m), r.tn = (int)(t / j.tiles_m);
+        r.k0 = r.sp * j.blocks;
+        r.k1 = min(r.k0 + j.blocks, (j.k + BK - 1) / BK);
+        return r;
     };
 
     if (warp == 0) {
@@ -117,25 +134,26 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
             long it = 0;
             bool ok = true;
             for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                int tm, tn, sp, k0, k1;
-                unit(u, tm, tn, sp, k0, k1);
+                const Unit r = unit(u);
+                const CUtensorMap *ta = &maps.a[r.job], *tb = &maps.b[r.job];
+                const bool amn = EPI == OUT && r.job == 1;
                 for (int p = 0; ok && p < a.pairs; ++p)
-                    for (int kb = k0; kb < k1; ++kb, ++it) {
+                    for (int kb = r.k0; kb < r.k1; ++kb, ++it) {
                         const int s = (int)(it % S);
                         if (!(ok = mbar_wait(empty + s, (uint32_t)((it / S) & 1) ^ 1u, fail))) break;
                         unsigned char* at = tiles + s * TL::STAGE;
                         mbar_expect(full + s, TL::STAGE);
-                        if (AMN) {
+                        if (amn) {
                             for (int j = 0; j < BM / 64; ++j)
-                                tma_load(&ta, full + s, at + j * 8192, tm * BM + j * 64, kb * BK, a.ia[p]);
+                                tma_load(ta, full + s, at + j * 8192, r.tm * BM + j * 64, kb * BK, a.ia[p]);
                         } else {
-                            tma_load(&ta, full + s, at, kb * BK, tm * BM, a.ia[p]);
+                            tma_load(ta, full + s, at, kb * BK, r.tm * BM, a.ia[p]);
                         }
                         if (BMN) {
                             for (int j = 0; j < BN / 64; ++j)
-                                tma_load(&tb, full + s, at + TL::A + j * 8192, tn * BN + j * 64, kb * BK, a.ib[p]);
+                                tma_load(tb, full + s, at + TL::A + j * 8192, r.tn * BN + j * 64, kb * BK, a.ib[p]);
                         } else {
-                            tma_load(&tb, full + s, at + TL::A, kb * BK, tn * BN, a.ib[p]);
+                            tma_load(tb, full + s, at + TL::A, kb * BK, r.tn * BN, a.ib[p]);
                         }
                     }
             }
@@ -144,24 +162,24 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((AMN ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
-                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-            constexpr uint32_t astep = AMN ? 2048 >> 4 : 32 >> 4, bstep = BMN ? 2048 >> 4 : 32 >> 4;
             long it = 0, tile = 0;
             bool ok = true;
             for (long u = blockIdx.x; ok && u < units; u += gridDim.x, ++tile) {
-                int tm, tn, sp, k0, k1;
-                unit(u, tm, tn, sp, k0, k1);
+                const Unit r = unit(u);
+                const bool amn = EPI == OUT && r.job == 1;
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((amn ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
+                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+                const uint32_t astep = amn ? 2048 >> 4 : 32 >> 4, bstep = BMN ? 2048 >> 4 : 32 >> 4;
                 const int buf = (int)(tile & 1);
                 if (!(ok = mbar_wait(acc_empty + buf, (uint32_t)((tile >> 1) & 1) ^ 1u, fail))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const long steps = (long)a.pairs * (k1 - k0);
+                const long steps = (long)a.pairs * max(r.k1 - r.k0, 0);
                 for (long i = 0; i < steps; ++i, ++it) {
                     const int s = (int)(it % S);
                     if (!(ok = mbar_wait(full + s, (uint32_t)((it / S) & 1), fail))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t at = smem_u32(tiles + s * TL::STAGE);
-                    const uint64_t ad = desc(at, AMN), bd = desc(at + TL::A, BMN);
+                    const uint64_t ad = desc(at, amn), bd = desc(at + TL::A, BMN);
 #pragma unroll
                     for (int q = 0; q < BK / 16; ++q)
                         mma_bf16(tmem + buf * BN, ad + q * astep, bd + q * bstep, idesc, i > 0 || q > 0);
@@ -175,22 +193,23 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
             }
         }
     } else {
-        const int quarter = warp & 3;
+        // two warps share a quarter of the rows, each has half of the tile's columns
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
         long tile = 0;
         for (long u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
-            int tm, tn, sp, k0, k1;
-            unit(u, tm, tn, sp, k0, k1);
+            const Unit r = unit(u);
+            const Job& job = a.job[r.job];
             const int buf = (int)(tile & 1);
             if (!__all_sync(kFull, mbar_wait(acc_full + buf, (uint32_t)((tile >> 1) & 1), fail))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
-            const int row = tm * BM + quarter * 32 + lane;
-            const bool in = row < a.m;
-            const int cols = min(BN, a.n - tn * BN);
+            const int row = r.tm * BM + quarter * 32 + lane;
+            const bool in = row < job.m;
+            const int cols = min(half * HALF + HALF, job.n - r.tn * BN);
             if (EPI == LSE) {
-                const int pick = in ? a.target[row] - a.v0 - tn * BN : -1;
+                const int pick = in ? a.target[row] - a.v0 - r.tn * BN : -1;
                 float mx = -INFINITY, sum = 0.f;
-                for (int c = 0; c < cols; c += 32) {
+                for (int c = half * HALF; c < cols; c += 32) {
                     float v[32];
                     tmem_ld32(src + c, v);
                     if (c + 32 > cols) {
@@ -215,24 +234,52 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
                         a.picked[row] = z;
                     }
                 }
-                if (in) a.part[(long)(a.part_tile0 + tn) * a.m + row] = make_float2(mx, sum);
+                if (in) a.part[(long)((a.part_tile0 + r.tn) * 2 + half) * job.m + row] = make_float2(mx, sum);
             } else if (EPI == GRAD) {
                 const int t = in ? a.target[row] : -1;
-                const int pick = t < 0 ? -1 : t - a.v0 - tn * BN;
+                const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
                 const float w = t < 0 ? 0.f : a.dloss[row];
                 const float shift = in ? -a.lse[row] * kLog2e : 0.f;
-                for (int c = 0; c < cols; c += 32) {
+                for (int c = half * HALF; c < cols; c += 32) {
                     float v[32];
                     tmem_ld32(src + c, v);
-                    const bool here = (unsigned)(pick - c) < 32u;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float p = exp2f(fmaf(v[j], kLog2e, shift));
-                        if (here && pick - c == j) p -= 1.f;
-                        v[j] = t >= 0 && c + j < cols ? p * w : 0.f;
+                    for (int j = 0; j < 32; ++j) v[j] = exp2f(fmaf(v[j], kLog2e, shift));
+                    if ((unsigned)(pick - c) < 32u) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] -= pick - c == j ? 1.f : 0.f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = t >= 0 ? v[j] * w : 0.f;
+                    if (c + 32 > cols) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j >= cols) v[j] = 0.f;
+                    }
+                    if (a.planes == 1) {
+                        // through shared memory (rows of 64 columns, swizzled) and out by TMA, which drops what lies
+                        // beyond the matrix: stored from the registers, a warp's 32 rows at 16 bytes each took
+                        // the logits' pass from 1.46 to 1.09 PFLOP/s
+                        unsigned char* box = tiles + S * TL::STAGE + (warp - 2) * TL::OUTW + ((c >> 6) & (TL::OUTW / 4096 - 1)) * 4096;
+                        if ((c & 32) == 0) {
+                            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(TL::OUTW / 4096 - 1) : "memory");
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            Vec<bf16, true>::store(reinterpret_cast<bf16*>(box + lane * 128 + (((c & 32) / 8 + j) ^ (lane & 7)) * 16), v + 8 * j);
+                        if ((c & 32) || c + 32 >= cols) {
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) {
+                                tma_store(&maps.g, box, r.tn * BN + (c & ~63), r.tm * BM + quarter * 32, 0);
+                                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                            }
+                        }
+                        continue;
                     }
                     for (int s = 0; in && s < a.planes; ++s) {
-                        bf16* g = a.g + s * a.g_plane + (long)row * a.ldg + tn * BN + c;
+                        bf16* g = a.g + s * a.g_plane + (long)row * a.ldg + r.tn * BN + c;
 #pragma unroll
                         for (int j = 0; j < 32; j += 8) {
                             uint32_t q[4];
@@ -241,28 +288,31 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
                                 q[e] = pack_bf16(v[j + 2 * e], v[j + 2 * e + 1]);
                                 v[j + 2 * e] -= bf16_lo(q[e]), v[j + 2 * e + 1] -= bf16_hi(q[e]);
                             }
-                            if (tn * BN + c + j < a.ldg) *reinterpret_cast<uint4*>(g + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                            if (r.tn * BN + c + j < a.ldg) *reinterpret_cast<uint4*>(g + j) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
                     }
                 }
+                if (a.planes == 1 && lane == 0)  // a box that this tile lacks counts too: the waits above go by number
+                    for (int c = max(half * HALF, (cols + 63) & ~63); c < half * HALF + HALF; c += 64)
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             } else {
-                for (int c = 0; c < cols; c += 32) {
+                for (int c = half * HALF; c < cols; c += 32) {
                     float v[32];
                     tmem_ld32(src + c, v);
-                    if (k0 >= k1) {
+                    if (r.k0 >= r.k1) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = 0.f;
                     }
-                    const int col = tn * BN + c;
+                    const int col = r.tn * BN + c;
                     const int w = min(32, cols - c);
                     if (!in) {
-                    } else if (a.acc) {
-                        float* p = a.acc + ((long)sp * a.m + row) * a.n + col;
-                        if (w == 32 && (a.n & 3) == 0) {
+                    } else if (job.acc) {
+                        float* p = job.acc + ((long)r.sp * job.m + row) * job.n + col;
+                        if (w == 32 && (job.n & 3) == 0) {
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) {
                                 float4 q = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                                if (a.add) {
+                                if (job.add) {
                                     const float4 o = *reinterpret_cast<const float4*>(p + j);
                                     q.x += o.x, q.y += o.y, q.z += o.z, q.w += o.w;
                                 }
@@ -271,11 +321,11 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (j < w) p[j] = a.add ? p[j] + v[j] : v[j];
+                                if (j < w) p[j] = job.add ? p[j] + v[j] : v[j];
                         }
                     } else if (a.f32) {
-                        float* p = static_cast<float*>(a.out) + (long)row * a.ldo + col;
-                        if (w == 32 && (a.ldo & 3) == 0 && aligned16_dev(a.out)) {
+                        float* p = static_cast<float*>(job.out) + (long)row * job.n + col;
+                        if (w == 32 && (job.n & 3) == 0 && aligned16_dev(job.out)) {
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                         } else {
@@ -284,8 +334,8 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
                                 if (j < w) p[j] = v[j];
                         }
                     } else {
-                        bf16* p = static_cast<bf16*>(a.out) + (long)row * a.ldo + col;
-                        if (w == 32 && (a.ldo & 7) == 0 && aligned16_dev(a.out)) {
+                        bf16* p = static_cast<bf16*>(job.out) + (long)row * job.n + col;
+                        if (w == 32 && (job.n & 7) == 0 && aligned16_dev(job.out)) {
 #pragma unroll
                             for (int j = 0; j < 32; j += 8) Vec<bf16, true>::store(p + j, v + j);
                         } else {
@@ -299,6 +349,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(acc_empty + buf);
         }
+        if (EPI == GRAD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -308,48 +359,58 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ CUten
 
 // ---- the passes around it ------------------------------------------------------------------------------------
 
-// Targets as vocabulary positions, -1 where there is no loss.
-__global__ void __launch_bounds__(256) target_kernel(const void* __restrict__ targets, int wide, long rows, long vocab, long ignore,
-                                                     int* __restrict__ out, float* __restrict__ picked, int* status) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows) return;
-    const long t = wide ? reinterpret_cast<const long long*>(targets)[i] : (long)reinterpret_cast<const int*>(targets)[i];
-    int v = -1;
-    if (t != ignore) {
-        if (t >= 0 && t < vocab) v = (int)t;
-        else report(status, EWS_ERR_INDEX);
-    }
-    out[i] = v;
-    if (picked) picked[i] = 0.f;
-}
-
-// Rows as bfloat16 planes of `ld` columns, zero beyond `dim`; rows without a target (`target` given) are zero.
+// Rows as bfloat16 planes of `ld` columns, zero beyond `dim`.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ in, long stride, long rows, int dim, const int* __restrict__ target,
-                                                   bf16* __restrict__ out, int ld, long plane, int planes) {
+struct Pack {
+    const T* in;
+    long stride, rows;
+    bf16* out;
+    long plane;
+};
+
+// Packs the hidden rows (a row without a target as zeros) with the targets as vocabulary positions (-1: no loss),
+// and behind them the rows of a piece of the weight.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Pack<T> h, const __grid_constant__ Pack<T> w, int dim, int ld,
+                                                   int planes, const void* __restrict__ targets, int wide, long vocab, long ignore,
+                                                   int* __restrict__ target, int* status) {
     const int per = ld / 8;
-    const long total = rows * per;
-    const bool vec = stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(in);
+    const long total = (h.rows + w.rows) * per;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        const long row = e / per;
+        long row = e / per;
         const int col = (int)(e - row * per) * 8;
+        const bool hidden = row < h.rows;
+        bool live = true;
+        if (hidden) {
+            const long t = wide ? reinterpret_cast<const long long*>(targets)[row] : (long)reinterpret_cast<const int*>(targets)[row];
+            live = t != ignore && t >= 0 && t < vocab;
+            if (col == 0) {
+                target[row] = live ? (int)t : -1;
+                if (!live && t != ignore) report(status, EWS_ERR_INDEX);
+            }
+        } else {
+            row -= h.rows;
+        }
+        const T* in = hidden ? h.in : w.in;
+        const long stride = hidden ? h.stride : w.stride;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        if (!target || target[row] >= 0) {
+        if (live) {
             const T* p = in + row * stride + col;
-            if (vec) {
+            if (stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(in)) {
 #pragma unroll
-                for (int j = 0; j < 8; j += Vec<T, true>::N)
-                    if (col < dim) Vec<T, true>::load(p + j, v + j);
+                for (int j = 0; j < 8; j += Vec<T, true>::N) Vec<T, true>::load(p + j, v + j);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (col + j < dim) v[j] = to_f(p[j]);
             }
         }
+        bf16* out = (hidden ? h.out : w.out) + row * ld + col;
+        const long plane = hidden ? h.plane : w.plane;
         for (int s = 0; s < planes; ++s) {
-            Vec<bf16, true>::store(out + s * plane + row * ld + col, v);
+            Vec<bf16, true>::store(out + s * plane, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] -= to_f(from_f<bf16>(v[j]));
         }
@@ -415,39 +476,50 @@ bool make_map(CUtensorMap* map, const Operand& o, int box_rows) {
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int EPI, int BN, bool AMN, bool BMN>
-int gemm_bn(Gemm g, const Operand& oa, const Operand& ob, cudaStream_t s) {
-    CUtensorMap ta, tb;
-    if (!make_map(&ta, oa, AMN ? 64 : BM) || !make_map(&tb, ob, BMN ? 64 : BN)) return EWS_ERR_LAUNCH;
-    auto* kern = gemm_kernel<EPI, BN, AMN, BMN>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
-    g.tiles_m = (g.m + BM - 1) / BM, g.tiles_n = (g.n + BN - 1) / BN;
-    const long units = (long)g.tiles_m * g.tiles_n * g.splits;
-    kern<<<(unsigned)(units < SMS ? units : SMS), NTH, Tile<BN>::bytes, s>>>(ta, tb, g);
-    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
-}
-
 // Column tiles of 256, or of 128 where a narrow output leaves half of a wide one empty.
 int tile_n(long n) { return n <= 128 ? 128 : 256; }
 
-template <int EPI, bool AMN, bool BMN>
-int gemm(Gemm g, const Operand& oa, const Operand& ob, int planes, cudaStream_t s) {
-    static const signed char pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
-    g.pairs = planes == 1 ? 1 : 6;
-    for (int i = 0; i < g.pairs; ++i) g.ia[i] = planes == 1 ? 0 : pa[i], g.ib[i] = planes == 1 ? 0 : pb[i];
-    const int kblocks = (g.k + BK - 1) / BK;
-    if (g.splits < 1) g.splits = 1;
-    g.blocks = (kblocks + g.splits - 1) / g.splits;
-    return tile_n(g.n) == 128 ? gemm_bn<EPI, 128, AMN, BMN>(g, oa, ob, s) : gemm_bn<EPI, 256, AMN, BMN>(g, oa, ob, s);
-}
-
-// Splits of a gradient's K axis: enough units for every SM, none below eight k blocks.
-int splits_of(long m, long n, long k) {
+// K splits of a gradient of (m, n): as many as leave no SM without a tile, none below eight k blocks.
+int splits_of(long m, long n, long k, long other) {
     const long tiles = ((m + BM - 1) / BM) * ((n + tile_n(n) - 1) / tile_n(n));
-    long want = SMS / tiles;
+    long want = (SMS - other > tiles ? SMS - other : tiles) / tiles;
     const long most = (k + BK * 8 - 1) / (BK * 8);
     if (want > most) want = most;
     return want < 1 ? 1 : (int)want;
+}
+
+Job job_of(long m, long n, long k, int splits) {
+    Job j{};
+    j.m = (int)m, j.n = (int)n, j.k = (int)k, j.splits = splits;
+    j.tiles_m = (int)((m + BM - 1) / BM), j.tiles_n = (int)((n + tile_n(n) - 1) / tile_n(n));
+    j.blocks = (int)(((k + BK - 1) / BK + splits - 1) / splits);
+    j.units = (long)j.tiles_m * j.tiles_n * splits;
+    return j;
+}
+
+template <int EPI, int BN>
+int gemm_bn(const Maps& maps, const Gemm& g, cudaStream_t s) {
+    auto* kern = gemm_kernel<EPI, BN>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<EPI, BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
+    const long units = g.job[0].units + g.job[1].units;
+    kern<<<(unsigned)(units < SMS ? units : SMS), NTH, Tile<EPI, BN>::bytes, s>>>(maps, g);
+    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
+}
+
+// Operands of job[0], and of job[1] where it has units (OUT). Both jobs' n is the model's width, so they share BN.
+template <int EPI>
+int gemm(Gemm g, const Operand& a0, const Operand& b0, const Operand& a1, const Operand& b1, int planes, cudaStream_t s) {
+    static const signed char pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
+    g.pairs = planes == 1 ? 1 : 6;
+    for (int i = 0; i < g.pairs; ++i) g.ia[i] = planes == 1 ? 0 : pa[i], g.ib[i] = planes == 1 ? 0 : pb[i];
+    Maps m{};
+    if (EPI == GRAD && planes == 1 &&
+        !make_map(&m.g, Operand{g.g, g.job[0].m, g.job[0].n, g.ldg, 0, 1}, 32))
+        return EWS_ERR_LAUNCH;
+    const int bn = tile_n(g.job[0].units ? g.job[0].n : g.job[1].n);
+    if (g.job[0].units && (!make_map(&m.a[0], a0, BM) || !make_map(&m.b[0], b0, EPI == OUT ? 64 : bn))) return EWS_ERR_LAUNCH;
+    if (g.job[1].units && (!make_map(&m.a[1], a1, 64) || !make_map(&m.b[1], b1, 64))) return EWS_ERR_LAUNCH;
+    return bn == 128 ? gemm_bn<EPI, 128>(m, g, s) : gemm_bn<EPI, 256>(m, g, s);
 }
 
 struct Plan {
@@ -467,24 +539,41 @@ int check(const ews_vocab_args* a) {
     return EWS_OK;
 }
 
+long up(long n, long to) { return (n + to - 1) / to * to; }
+
+// Pieces of the vocabulary: the fewest that keep G (and a packed weight) within kPieceElems, or up to four more
+// where that fills the SMs' waves of tiles better (a launch whose last wave has a few tiles idles the rest).
+void pick_pieces(Plan* p, long n, long v, long d, bool bwd) {
+    long most = v;
+    if (bwd) most = kPieceElems / (n * p->planes);
+    if (p->pack_w && kPieceElems / ((long)p->ldd * p->planes) < most) most = kPieceElems / ((long)p->ldd * p->planes);
+    if (most < 1024) most = 1024;
+    const long least = (v + most - 1) / most;
+    p->pieces = least;
+    p->piece = least == 1 ? v : up((v + least - 1) / least, 256);
+    if (!bwd || least == 1) {
+        p->pieces = (v + p->piece - 1) / p->piece;
+        return;
+    }
+    const long tm = (n + BM - 1) / BM, td = (d + tile_n(d) - 1) / tile_n(d);
+    double best = 0;
+    for (long c = least; c <= least + 4; ++c) {
+        const long piece = up((v + c - 1) / c, 256), count = (v + piece - 1) / piece;
+        auto waves = [](long tiles) { return (double)((tiles + SMS - 1) / SMS); };
+        // a tile's time goes with its K: the width for the logits, the piece and the rows for the gradients
+        const double kgrad = (piece * (double)(tm * td) + n * (double)(piece / BM * td)) / (tm * td + piece / BM * td);
+        const double cost = count * (waves(tm * (piece / 256)) * d + waves(tm * td + piece / BM * td) * kgrad + 2000.0);
+        if (c == least || cost < best) best = cost, p->piece = piece, p->pieces = count;
+    }
+}
+
 Plan plan(const ews_vocab_args* a, bool bwd) {
     Plan p{};
     p.planes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
-    p.ldd = (int)((a->dim + 7) / 8 * 8);
+    p.ldd = (int)up(a->dim, 8);
     p.pack_w = p.planes > 1 || a->weight_stride % 8 || a->dim % 8 || !aligned16(a->weight);
     const long n = a->rows, v = a->vocab;
-    // a piece: G of at most kPieceElems entries (and a packed weight of as many)
-    long most = v;
-    if (bwd) most = kPieceElems / ((n > 0 ? n : 1) * p.planes);
-    if (p.pack_w) {
-        const long w = kPieceElems / ((long)p.ldd * p.planes);
-        if (w < most) most = w;
-    }
-    most = most / 256 * 256;
-    if (most < 1024) most = 1024;
-    p.pieces = (v + most - 1) / most;
-    p.piece = p.pieces == 1 ? v : ((v + p.pieces - 1) / p.pieces + 255) / 256 * 256;
-    p.pieces = (v + p.piece - 1) / p.piece;
+    pick_pieces(&p, n, v, a->dim, bwd);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -497,11 +586,13 @@ Plan plan(const ews_vocab_args* a, bool bwd) {
     if (!bwd) {
         p.picked = take(sizeof(float) * n);
         const long tiles = p.pieces * ((p.piece + tile_n(p.piece) - 1) / tile_n(p.piece));
-        p.part = take(sizeof(float2) * tiles * n);
+        p.part = take(sizeof(float2) * 2 * tiles * n);
     } else {
-        p.g = take(sizeof(bf16) * (size_t)p.planes * n * ((p.piece + 7) / 8 * 8));
-        p.split_h = splits_of(n, a->dim, p.piece);
-        p.split_w = splits_of(p.piece, a->dim, n);
+        p.g = take(sizeof(bf16) * (size_t)p.planes * n * up(p.piece, 8));
+        const long th = ((n + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
+        const long tw = ((p.piece + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
+        p.split_h = splits_of(n, a->dim, p.piece, tw);
+        p.split_w = splits_of(p.piece, a->dim, n, th * p.split_h);
         p.acc_h = p.split_h > 1 || p.pieces > 1;
         p.acc_w = p.split_w > 1;
         if (p.acc_h) p.ah = take(sizeof(float) * (size_t)p.split_h * n * a->dim);
@@ -517,100 +608,89 @@ unsigned grid_of(long total) {
 }
 
 template <typename T>
-int pack(const void* in, long stride, long rows, int dim, const int* target, bf16* out, const Plan& p, long plane, cudaStream_t s) {
-    pack_kernel<T><<<grid_of(rows * (p.ldd / 8)), 256, 0, s>>>(static_cast<const T*>(in), stride, rows, dim, target, out, p.ldd, plane, p.planes);
-    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
-}
-
-template <typename T>
 int reduce(const float* acc, int splits, long total, T* out, cudaStream_t s) {
     reduce_kernel<T><<<grid_of(total), 256, 0, s>>>(acc, splits, total, out);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
-// The weight's rows [v0, v0 + n) as an operand, packed where they cannot be read as they lie.
+// The operands of the piece [v0, v0 + n) of the vocabulary, packed where they cannot be read as they lie (hidden:
+// with the first piece).
 template <typename T>
-int weight_piece(const ews_vocab_args* a, const Plan& p, char* w, long v0, long n, Operand* o, cudaStream_t s) {
+int operands(const ews_vocab_args* a, const Plan& p, char* w, long v0, long n, Operand* h, Operand* o, cudaStream_t s) {
+    Pack<T> ph{}, pw{};
+    if (v0 == 0) {
+        bf16* at = reinterpret_cast<bf16*>(w + p.h);
+        h->p = at, h->rows = a->rows, h->cols = h->ld = p.ldd, h->planes = p.planes, h->plane = a->rows * p.ldd;
+        ph.in = static_cast<const T*>(a->hidden), ph.stride = a->hidden_stride, ph.rows = a->rows, ph.out = at, ph.plane = h->plane;
+    }
     const T* rows = static_cast<const T*>(a->weight) + v0 * a->weight_stride;
     o->rows = n, o->planes = p.planes;
-    if (!p.pack_w) {
+    if (p.pack_w) {
+        bf16* at = reinterpret_cast<bf16*>(w + p.w);
+        o->p = at, o->cols = o->ld = p.ldd, o->plane = n * p.ldd;
+        pw.in = rows, pw.stride = a->weight_stride, pw.rows = n, pw.out = at, pw.plane = o->plane;
+    } else {
         o->p = reinterpret_cast<const bf16*>(rows), o->cols = a->dim, o->ld = a->weight_stride, o->plane = 0;
-        return EWS_OK;
     }
-    bf16* at = reinterpret_cast<bf16*>(w + p.w);
-    o->p = at, o->cols = p.ldd, o->ld = p.ldd, o->plane = n * p.ldd;
-    return pack<T>(rows, a->weight_stride, n, (int)a->dim, nullptr, at, p, o->plane, s);
-}
-
-template <typename T>
-int begin(const ews_vocab_args* a, const Plan& p, char* w, float* picked, Operand* h, cudaStream_t s) {
-    int* target = reinterpret_cast<int*>(w + p.target);
-    target_kernel<<<(unsigned)((a->rows + 255) / 256), 256, 0, s>>>(a->targets, a->targets_wide, a->rows, a->vocab, a->ignore, target, picked,
-                                                                   a->status);
-    bf16* at = reinterpret_cast<bf16*>(w + p.h);
-    h->p = at, h->rows = a->rows, h->cols = p.ldd, h->ld = p.ldd, h->planes = p.planes, h->plane = a->rows * p.ldd;
-    return pack<T>(a->hidden, a->hidden_stride, a->rows, (int)a->dim, target, at, p, h->plane, s);
+    if (ph.rows + pw.rows == 0) return EWS_OK;
+    pack_kernel<T><<<grid_of((ph.rows + pw.rows) * (p.ldd / 8)), 256, 0, s>>>(ph, pw, (int)a->dim, p.ldd, p.planes, a->targets, a->targets_wide,
+                                                                              a->vocab, a->ignore, reinterpret_cast<int*>(w + p.target), a->status);
+    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
 template <typename T>
 int forward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
-    float* picked = reinterpret_cast<float*>(w + p.picked);
-    Operand h{}, wt{};
-    int rc = begin<T>(a, p, w, picked, &h, s);
+    Operand h{}, wt{}, none{};
+    int rc = EWS_OK;
     Gemm g{};
     g.status = a->status;
     g.target = reinterpret_cast<const int*>(w + p.target);
     g.part = reinterpret_cast<float2*>(w + p.part);
-    g.picked = picked;
-    g.m = (int)a->rows, g.k = (int)a->dim;
+    g.picked = reinterpret_cast<float*>(w + p.picked);
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
         const long n = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
-        if ((rc = weight_piece<T>(a, p, w, v0, n, &wt, s)) != EWS_OK) break;
-        g.n = (int)n, g.v0 = (int)v0;
-        rc = gemm<LSE, false, false>(g, h, wt, p.planes, s);
-        g.part_tile0 += (int)((n + tile_n(n) - 1) / tile_n(n));
+        if ((rc = operands<T>(a, p, w, v0, n, &h, &wt, s)) != EWS_OK) break;
+        g.job[0] = job_of(a->rows, n, a->dim, 1), g.v0 = (int)v0;
+        rc = gemm<LSE>(g, h, wt, none, none, p.planes, s);
+        g.part_tile0 += g.job[0].tiles_n;
     }
     if (rc != EWS_OK) return rc;
-    lse_kernel<<<(unsigned)((a->rows + 31) / 32), 256, 0, s>>>(g.part, g.part_tile0, a->rows, g.target, picked, a->loss, a->lse);
+    lse_kernel<<<(unsigned)((a->rows + 31) / 32), 256, 0, s>>>(g.part, 2 * g.part_tile0, a->rows, g.target, g.picked, a->loss, a->lse);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
 template <typename T>
 int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
-    Operand h{}, wt{}, go{};
-    int rc = begin<T>(a, p, w, nullptr, &h, s);
-    const int* target = reinterpret_cast<const int*>(w + p.target);
+    Operand h{}, wt{}, go{}, none{};
+    int rc = EWS_OK;
     float* acc_h = p.acc_h ? reinterpret_cast<float*>(w + p.ah) : nullptr;
     float* acc_w = p.acc_w ? reinterpret_cast<float*>(w + p.aw) : nullptr;
-    bf16* G = reinterpret_cast<bf16*>(w + p.g);
+    Gemm base{};
+    base.status = a->status, base.f32 = sizeof(T) == 4;
+    base.target = reinterpret_cast<const int*>(w + p.target), base.lse = a->lse, base.dloss = a->dloss;
+    base.g = reinterpret_cast<bf16*>(w + p.g), base.planes = p.planes;
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
         const long n = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
-        if ((rc = weight_piece<T>(a, p, w, v0, n, &wt, s)) != EWS_OK) break;
-        Gemm g{};
-        g.status = a->status;
-        g.target = target, g.lse = a->lse, g.dloss = a->dloss;
-        g.m = (int)a->rows, g.n = (int)n, g.k = (int)a->dim, g.v0 = (int)v0;
-        g.g = G, g.ldg = (n + 7) / 8 * 8, g.g_plane = a->rows * g.ldg, g.planes = p.planes;
-        if ((rc = gemm<GRAD, false, false>(g, h, wt, p.planes, s)) != EWS_OK) break;
-        go.p = G, go.rows = a->rows, go.cols = n, go.ld = g.ldg, go.plane = g.g_plane, go.planes = p.planes;
-        Gemm o{};
-        o.status = a->status, o.f32 = sizeof(T) == 4, o.ldo = a->dim, o.n = (int)a->dim, o.n_fast = 1;
+        if ((rc = operands<T>(a, p, w, v0, n, &h, &wt, s)) != EWS_OK) break;
+        Gemm g = base;
+        g.job[0] = job_of(a->rows, n, a->dim, 1), g.v0 = (int)v0;
+        g.ldg = up(n, 8), g.g_plane = a->rows * g.ldg;
+        if ((rc = gemm<GRAD>(g, h, wt, none, none, p.planes, s)) != EWS_OK) break;
+        go.p = g.g, go.rows = a->rows, go.cols = n, go.ld = g.ldg, go.plane = g.g_plane, go.planes = p.planes;
+        Gemm o = base;
+        T* out = static_cast<T*>(a->dweight) + (a->dweight ? v0 * a->dim : 0);
         if (a->dhidden) {  // dH += G W: K is the piece of the vocabulary
-            Gemm d = o;
-            d.m = (int)a->rows, d.k = (int)n, d.splits = p.split_h;
-            d.out = a->dhidden, d.acc = acc_h, d.add = v0 > 0;
-            if ((rc = gemm<OUT, false, true>(d, go, wt, p.planes, s)) != EWS_OK) break;
+            o.job[0] = job_of(a->rows, a->dim, n, p.split_h);
+            o.job[0].out = a->dhidden, o.job[0].acc = acc_h, o.job[0].add = v0 > 0;
         }
         if (a->dweight) {  // dW = G^T H: K is the rows
-            Gemm d = o;
-            T* out = static_cast<T*>(a->dweight) + v0 * a->dim;
-            d.m = (int)n, d.k = (int)a->rows, d.splits = p.split_w;
-            d.out = out, d.acc = acc_w;
-            if ((rc = gemm<OUT, true, true>(d, go, h, p.planes, s)) != EWS_OK) break;
-            if (acc_w && (rc = reduce<T>(acc_w, p.split_w, n * a->dim, out, s)) != EWS_OK) break;
+            o.job[1] = job_of(n, a->dim, a->rows, p.split_w);
+            o.job[1].out = out, o.job[1].acc = acc_w;
         }
+        if ((rc = gemm<OUT>(o, go, wt, go, h, p.planes, s)) != EWS_OK) break;
+        if (a->dweight && acc_w) rc = reduce<T>(acc_w, p.split_w, n * a->dim, out, s);
     }
     if (rc == EWS_OK && a->dhidden && acc_h) rc = reduce<T>(acc_h, p.split_h, a->rows * a->dim, static_cast<T*>(a->dhidden), s);
     return rc;

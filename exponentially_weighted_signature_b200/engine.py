@@ -88,24 +88,24 @@ def _status_slot(device):
     return slot
 
 
-# Token ids, targets and state slots out of range: the kernel itself stores the code in this pinned word, so a
-# call adds no launch and no copy; the next call on the device raises IndexError.
+# Token ids, targets and state slots out of range, and the token operators' bounded waits that ran out: the kernel
+# itself stores the code in this pinned word, so a call adds no launch and no copy; the next call raises.
 _INDEX = {}
 
 
-def index_word(device):
-    """(address of the device's pinned index status, the same word as a ctypes int)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+def index_word(idx: int):
+    """(address, ctypes view, owner) of the pinned status word of device ``idx``."""
     slot = _INDEX.get(idx)
     if slot is None:
         host = torch.zeros(1, dtype=torch.int32).pin_memory()
-        slot = _INDEX[idx] = (ctypes.c_void_p(host.data_ptr()), ctypes.c_int.from_address(host.data_ptr()), host)
+        slot = _INDEX[idx] = (host.data_ptr(), ctypes.c_int.from_address(host.data_ptr()), host)
     return slot
 
 
-def raise_index(device) -> None:
-    """Raises (once) IndexError if an earlier token operator on ``device`` met an index out of range."""
-    word = index_word(device)[1]
+def raise_index(idx: int) -> None:
+    """Raises (once) what an earlier token operator on device ``idx`` reported: IndexError for an index out of range,
+    EWSLookbackTimeout for a bounded wait that ran out."""
+    word = index_word(idx)[1]
     if word.value != _lib.EWS_OK:
         code, word.value = word.value, _lib.EWS_OK
         _lib.check(code, "an earlier token operator on this device")

@@ -10,17 +10,24 @@ next token operator on the device raises IndexError (at once under ``configure(c
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib, engine
-from .engine import _ptr, _require_cuda, _stream_ptr, _timed
+from .engine import _require_cuda, _timed
 
 _DTYPES = {torch.float32: _lib.EWS_DTYPE_F32, torch.bfloat16: _lib.EWS_DTYPE_BF16}
+_WIDE = {torch.int64: 1, torch.int32: 0}
 MAX_HEAD = 128
+
+# ews_decay_args and ews_vocab_args, packed in one call (native alignment; the fields in the header's order).
+_DECAY = struct.Struct("@7if3P9q6P3q6PNP").pack
+_VOCAB = struct.Struct("@3q2i3P3q6PNP").pack
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without building a Stream
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -30,23 +37,51 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _indices(t: torch.Tensor, what: str) -> int:
-    if t.dtype not in (torch.int64, torch.int32):
+def _wide(t: torch.Tensor, what: str) -> int:
+    wide = _WIDE.get(t.dtype)
+    if wide is None:
         raise TypeError(f"{what} must be int64 or int32, got {t.dtype}")
-    return 1 if t.dtype == torch.int64 else 0
+    return wide
 
 
-def _same_device(*tensors) -> torch.device:
-    _require_cuda(*tensors)
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t is not None and t.device != dev:
-            raise ValueError(f"all tensors must be on one device, got {dev} and {t.device}")
-    return dev
+def _device(*tensors) -> int:
+    """The index of the one CUDA device that all tensors are on, pending index errors on it raised."""
+    idx = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (idx < 0 or t.get_device() != idx):
+            _require_cuda(*tensors)
+            raise ValueError(f"all tensors must be on one device, got {tensors[0].device} and {t.device}")
+    if engine.index_word(idx)[1].value:
+        engine.raise_index(idx)
+    return idx
+
+
+def _launch(idx: int, name: str, units: int, fn, *args) -> None:
+    """One library call on the device's current stream."""
+    if engine.PROFILE is None and idx == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx), _timed(name, torch.device("cuda", idx), units):
+            rc = fn(*args, _raw_stream(idx))
+    if rc:
+        _lib.check(rc, name)
+    if engine.CHECK_SYNC:
+        torch.cuda.current_stream(idx).synchronize()
+        engine.raise_index(idx)
+
+
+def _work(size: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    return torch.empty(size, dtype=torch.uint8, device=like.device) if size else None
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-d tensor whose rows are contiguous and do not overlap (a view where it already is one)."""
+    if t.is_contiguous():
+        return t
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         return t.contiguous()
     return t
@@ -56,48 +91,38 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _after(dev) -> None:
-    if engine.CHECK_SYNC:
-        torch.cuda.current_stream(dev).synchronize()
-        engine.raise_index(dev)
-
-
 # ----------------------------------------------------------------------------------------- token embedding
+
+
+def _embed(flat, table, scale, shape):
+    idx, (vocab, dim), n = table.get_device(), table.shape, flat.numel()
+    out = torch.empty((*shape, dim), dtype=table.dtype, device=table.device)
+    _launch(idx, "ews_embed_fwd", n, _lib.load().ews_embed_fwd, flat.data_ptr(), _WIDE[flat.dtype], table.data_ptr(),
+            _DTYPES[table.dtype], n, vocab, dim, _row_stride(table), scale, out.data_ptr(), engine.index_word(idx)[0])
+    return out
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale, padding_index):
-        lib = _lib.load()
-        dev = table.device
-        code, wide = _DTYPES[table.dtype], _indices(ids, "ids")
-        flat, rows = ids.reshape(-1), _rows(table)
-        flat = flat.contiguous()
-        n, (vocab, dim) = flat.numel(), table.shape
-        out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=dev)
-        with torch.cuda.device(dev), _timed("ews_embed_fwd", dev, n, 1):
-            _lib.check(lib.ews_embed_fwd(_ptr(flat), wide, _ptr(rows), code, n, vocab, dim, _row_stride(rows), scale,
-                                         _ptr(out), engine.index_word(dev)[0], _stream_ptr(dev)), "ews_embed_fwd")
-        ctx.meta = (code, wide, vocab, dim, scale, padding_index)
+    def forward(ctx, flat, table, scale, padding_index, shape):
+        rows = _rows(table)
+        ctx.meta = (rows.shape, scale, padding_index)
         ctx.save_for_backward(flat)
-        _after(dev)
-        return out
+        return _embed(flat, rows, scale, shape)
 
     @staticmethod
     def backward(ctx, dout):
-        code, wide, vocab, dim, scale, padding_index = ctx.meta
+        (vocab, dim), scale, padding_index = ctx.meta
         (flat,) = ctx.saved_tensors
         lib = _lib.load()
-        dev = dout.device
         n = flat.numel()
         g = _rows(dout.reshape(n, dim))
-        grad = torch.empty((vocab, dim), dtype=dout.dtype, device=dev)
-        work = torch.empty(int(lib.ews_embed_work_size(n, vocab, dim)), dtype=torch.uint8, device=dev)
-        skip = -1 if padding_index is None else padding_index
-        with torch.cuda.device(dev), _timed("ews_embed_bwd", dev, n, 3):
-            _lib.check(lib.ews_embed_bwd(_ptr(flat), wide, _ptr(g), code, n, vocab, dim, _row_stride(g), scale, skip,
-                                         _ptr(grad), _ptr(work), work.numel(), None, _stream_ptr(dev)), "ews_embed_bwd")
-        return None, grad, None, None
+        grad = torch.empty((vocab, dim), dtype=dout.dtype, device=dout.device)
+        work = _work(lib.ews_embed_work_size(n, vocab, dim), dout)
+        _launch(dout.get_device(), "ews_embed_bwd", n, lib.ews_embed_bwd, flat.data_ptr(), _WIDE[flat.dtype], g.data_ptr(),
+                _DTYPES[dout.dtype], n, vocab, dim, _row_stride(g), scale, padding_index, grad.data_ptr(), work.data_ptr(),
+                work.numel(), None)
+        return None, grad, None, None, None
 
 
 def token_embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
@@ -108,86 +133,71 @@ def token_embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     positions, rounded once and bit-reproducible; rows of ``padding_index`` (their token is looked up as any
     other) and of tokens that do not occur are zero. An id out of range gives a zero row and IndexError on the next
     call."""
-    if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+    if table.dim() != 2 or 0 in table.shape:
         raise ValueError(f"table must be (V, D) with V, D > 0, got {tuple(table.shape)}")
     _dtype(table, "table")
-    _indices(ids, "ids")
-    dev = _same_device(table, ids)
-    if padding_index is not None:
-        if not -table.shape[0] <= padding_index < table.shape[0]:
-            raise ValueError(f"padding_index {padding_index} is out of range for {table.shape[0]} rows")
-        padding_index %= table.shape[0]
-    engine.raise_index(dev)
-    return _Embedding.apply(ids, table, float(scale), padding_index)
+    _wide(ids, "ids")
+    if padding_index is not None and not -table.shape[0] <= padding_index < table.shape[0]:
+        raise ValueError(f"padding_index {padding_index} is out of range for {table.shape[0]} rows")
+    _device(table, ids)
+    flat = ids.reshape(-1).contiguous()
+    if table.requires_grad and torch.is_grad_enabled():
+        skip = -1 if padding_index is None else padding_index % table.shape[0]
+        return _Embedding.apply(flat, table, float(scale), skip, ids.shape)
+    return _embed(flat, _rows(table.detach()), float(scale), ids.shape)
 
 
 # ---------------------------------------------------------------------------------------- decayed attention
 
 
-def _strides(t: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
-
-
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _decay_args(q, k, v, rate, lengths, initial, scale, out=None, end=None, dout=None, dend=None, grads=(None, None, None),
+                d0=None, work=None):
+    B, T, H, dk = q.shape
+    return _DECAY(B, T, H, k.shape[2], dk, v.shape[3], _DTYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], rate.data_ptr(), _addr(lengths), _addr(initial),
+                  _addr(out), _addr(end), _addr(dout), *((0, 0, 0) if dout is None else dout.stride()[:3]), _addr(dend),
+                  _addr(grads[0]), _addr(grads[1]), _addr(grads[2]), _addr(d0), _addr(work), 0 if work is None else work.numel(),
+                  engine.index_word(q.get_device())[0])
+
+
+def _decayed(q, k, v, rate, initial, lengths, scale, want_state):
+    lib = _lib.load()
+    B, T, H, dk = q.shape
+    dv = v.shape[3]
+    out = torch.empty((B, T, H, dv), dtype=q.dtype, device=q.device)
+    end = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if want_state else None
+    work = _work(lib.ews_decay_work_size(_decay_args(q, k, v, rate, lengths, initial, scale, out, end), 0), q)
+    args = _decay_args(q, k, v, rate, lengths, initial, scale, out, end, work=work)
+    _launch(q.get_device(), "ews_decay_fwd", B * T, lib.ews_decay_fwd, args)
+    return out, end
 
 
 class _Decayed(torch.autograd.Function):
     @staticmethod
-    def _args(q, k, v, rate, lengths, scale):
-        a = _lib.DecayArgs()
-        a.batch, a.steps, a.heads, a.dk = q.shape
-        a.kv_heads, a.dv = k.shape[2], v.shape[3]
-        a.dtype, a.scale = _DTYPES[q.dtype], scale
-        a.q, a.k, a.v = _ptr(q), _ptr(k), _ptr(v)
-        a.q_stride, a.k_stride, a.v_stride = _strides(q), _strides(k), _strides(v)
-        a.rate, a.lengths = _ptr(rate), _ptr(lengths)
-        a.status = engine.index_word(q.device)[0]
-        return a
-
-    @staticmethod
     def forward(ctx, q, k, v, rate, initial, lengths, scale, want_state):
-        lib = _lib.load()
-        dev = q.device
-        q, k, v = (_last_contiguous(t) for t in (q, k, v))
-        B, T, H, dk = q.shape
-        dv = v.shape[3]
-        a = _Decayed._args(q, k, v, rate, lengths, scale)
-        out = torch.empty((B, T, H, dv), dtype=q.dtype, device=dev)
-        end = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev) if want_state else None
-        a.initial, a.out, a.final_state = _ptr(initial), _ptr(out), _ptr(end)
-        size = lib.ews_decay_work_size(ctypes.byref(a), 0)
-        work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        a.work, a.work_bytes = _ptr(work), size
-        with torch.cuda.device(dev), _timed("ews_decay_fwd", dev, B * T):
-            _lib.check(lib.ews_decay_fwd(ctypes.byref(a), _stream_ptr(dev)), "ews_decay_fwd")
-        _after(dev)
+        q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
         ctx.scale = scale
         ctx.save_for_backward(q, k, v, rate, initial, lengths)
         ctx.set_materialize_grads(False)
-        return out, end
+        return _decayed(q, k, v, rate, initial, lengths, scale, want_state)
 
     @staticmethod
     def backward(ctx, dout, dend):
         q, k, v, rate, initial, lengths = ctx.saved_tensors
         lib = _lib.load()
-        dev = q.device
         B, T, H, dk = q.shape
         dv = v.shape[3]
-        dout = torch.zeros((B, T, H, dv), dtype=q.dtype, device=dev) if dout is None else _last_contiguous(dout)
+        dout = torch.zeros((B, T, H, dv), dtype=q.dtype, device=q.device) if dout is None else _last_contiguous(dout)
         dend = None if dend is None else dend.contiguous()
-        a = _Decayed._args(q, k, v, rate, lengths, ctx.scale)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
-        d0 = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev) if ctx.needs_input_grad[4] else None
-        a.initial, a.dout, a.dout_stride, a.dfinal = _ptr(initial), _ptr(dout), _strides(dout), _ptr(dend)
-        a.dq, a.dk_out, a.dv_out = (_ptr(g) for g in grads)
-        a.dinitial = _ptr(d0)
-        size = lib.ews_decay_work_size(ctypes.byref(a), 1)
-        work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        a.work, a.work_bytes = _ptr(work), size
-        with torch.cuda.device(dev), _timed("ews_decay_bwd", dev, B * T):
-            _lib.check(lib.ews_decay_bwd(ctypes.byref(a), _stream_ptr(dev)), "ews_decay_bwd")
-        _after(dev)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v)]
+        d0 = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if ctx.needs_input_grad[4] else None
+        work = _work(lib.ews_decay_work_size(_decay_args(q, k, v, rate, lengths, initial, ctx.scale), 1), q)
+        args = _decay_args(q, k, v, rate, lengths, initial, ctx.scale, None, None, dout, dend, grads, d0, work)
+        _launch(q.get_device(), "ews_decay_bwd", B * T, lib.ews_decay_bwd, args)
         return (*grads, None, d0, None, None, None)
 
 
@@ -231,8 +241,8 @@ def decayed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: t
 
     Returns o (B, T, H, dv), with ``return_state`` also the state after the last token (B, H, dk, dv) float32, for
     ``decayed_attention_step`` or the next piece of a long sequence. Differentiable in q, k, v and initial_state."""
-    _, dk, dv = H_dk_dv = _check_heads(q, k, v, rate, 4)
-    B, H = q.shape[0], H_dk_dv[0]
+    H, dk, dv = _check_heads(q, k, v, rate, 4)
+    B = q.shape[0]
     if initial_state is not None:
         if initial_state.shape != (B, H, dk, dv) or initial_state.dtype != torch.float32:
             raise ValueError(f"initial_state must be float32 {(B, H, dk, dv)}, got {initial_state.dtype} {tuple(initial_state.shape)}")
@@ -241,9 +251,15 @@ def decayed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: t
         if lengths.shape != (B,) or lengths.dtype != torch.int32:
             raise ValueError(f"lengths must be int32 ({B},), got {lengths.dtype} {tuple(lengths.shape)}")
         lengths = lengths.contiguous()
-    engine.raise_index(_same_device(q, k, v, rate, initial_state, lengths))
-    out, end = _Decayed.apply(q, k, v, rate, initial_state, lengths, _scale(scale, dk), bool(return_state))
-    return (out, end) if return_state else out
+    _device(q, k, v, rate, initial_state, lengths)
+    scale, want = _scale(scale, dk), bool(return_state)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or initial_state is not None and initial_state.requires_grad):
+        out, end = _Decayed.apply(q, k, v, rate, initial_state, lengths, scale, want)
+    else:
+        q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
+        out, end = _decayed(q, k, v, rate, initial_state, lengths, scale, want)
+    return (out, end) if want else out
 
 
 def decayed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: torch.Tensor, state: torch.Tensor, *,
@@ -265,74 +281,56 @@ def decayed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ra
         raise ValueError(f"slots must be contiguous int32 ({B},), got {slots.dtype} {tuple(slots.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError("decayed_attention_step has no gradient: call it under torch.no_grad()")
-    dev = _same_device(q, k, v, rate, state, slots)
-    engine.raise_index(dev)
-    q, k, v = (_last_contiguous(t) for t in (q, k, v))
-    out = torch.empty((B, H, dv), dtype=q.dtype, device=dev)
-    a = _lib.DecayArgs()
-    a.batch, a.steps, a.heads, a.kv_heads, a.dk, a.dv = B, 1, H, k.shape[1], dk, dv
-    a.dtype, a.scale = _DTYPES[q.dtype], _scale(scale, dk)
-    a.q, a.k, a.v, a.rate, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), rate.data_ptr(), out.data_ptr()
-    a.status = engine.index_word(dev)[0]
-    (a.q_stride[0], a.q_stride[2], _), (a.k_stride[0], a.k_stride[2], _), (a.v_stride[0], a.v_stride[2], _) = (
-        q.stride(), k.stride(), v.stride())
-    with torch.cuda.device(dev), _timed("ews_decay_step", dev, B, 1):
-        _lib.check(_lib.load().ews_decay_step(ctypes.byref(a), _ptr(slots), state.shape[0], _ptr(state),
-                                              _stream_ptr(dev)), "ews_decay_step")
-    _after(dev)
+    idx = _device(q, k, v, rate, state, slots)
+    q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
+    out = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    args = _DECAY(B, 1, H, k.shape[1], dk, dv, _DTYPES[q.dtype], _scale(scale, dk), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  qb, 0, qh, kb, 0, kh, vb, 0, vh, rate.data_ptr(), 0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                  engine.index_word(idx)[0])
+    _launch(idx, "ews_decay_step", B, _lib.load().ews_decay_step, args, _addr(slots), state.shape[0], state.data_ptr())
     return out
 
 
 # --------------------------------------------------------------------------------------------- vocabulary loss
 
 
+def _vocab_args(hidden, weight, targets, ignore, loss=None, lse=None, dloss=None, dh=None, dw=None, work=None):
+    rows, dim = hidden.shape
+    return _VOCAB(rows, weight.shape[0], dim, _DTYPES[hidden.dtype], _WIDE[targets.dtype], hidden.data_ptr(), weight.data_ptr(),
+                  targets.data_ptr(), _row_stride(hidden), _row_stride(weight), ignore, _addr(loss), _addr(lse), _addr(dloss),
+                  _addr(dh), _addr(dw), _addr(work), 0 if work is None else work.numel(), engine.index_word(hidden.get_device())[0])
+
+
+def _vocab(hidden, weight, targets, ignore):
+    lib = _lib.load()
+    rows = hidden.shape[0]
+    loss, lse = torch.empty((2, rows), dtype=torch.float32, device=hidden.device).unbind(0)
+    work = _work(lib.ews_vocab_work_size(_vocab_args(hidden, weight, targets, ignore), 0), hidden)
+    args = _vocab_args(hidden, weight, targets, ignore, loss, lse, work=work)
+    _launch(hidden.get_device(), "ews_vocab_fwd", rows, lib.ews_vocab_fwd, args)
+    return loss, lse
+
+
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
-    def _args(hidden, weight, targets, ignore):
-        a = _lib.VocabArgs()
-        a.rows, a.dim = hidden.shape
-        a.vocab = weight.shape[0]
-        a.dtype, a.targets_wide = _DTYPES[hidden.dtype], _indices(targets, "targets")
-        a.hidden, a.weight, a.targets = _ptr(hidden), _ptr(weight), _ptr(targets)
-        a.hidden_stride, a.weight_stride, a.ignore = _row_stride(hidden), _row_stride(weight), ignore
-        return a
-
-    @staticmethod
     def forward(ctx, hidden, weight, targets, ignore):
-        lib = _lib.load()
-        dev = hidden.device
-        hidden, weight, targets = _rows(hidden), _rows(weight), targets.contiguous()
-        a = _VocabLoss._args(hidden, weight, targets, ignore)
-        loss = torch.empty(a.rows, dtype=torch.float32, device=dev)
-        lse = torch.empty(a.rows, dtype=torch.float32, device=dev)
-        size = int(lib.ews_vocab_work_size(ctypes.byref(a), 0))
-        work = torch.empty(size, dtype=torch.uint8, device=dev)
-        a.loss, a.lse, a.work, a.work_bytes = _ptr(loss), _ptr(lse), _ptr(work), size
-        a.status = engine.index_word(dev)[0]
-        with torch.cuda.device(dev), _timed("ews_vocab_fwd", dev, a.rows):
-            _lib.check(lib.ews_vocab_fwd(ctypes.byref(a), _stream_ptr(dev)), "ews_vocab_fwd")
+        hidden, weight = _rows(hidden), _rows(weight)
+        loss, lse = _vocab(hidden, weight, targets, ignore)
         ctx.ignore = ignore
         ctx.save_for_backward(hidden, weight, targets, lse)
-        _after(dev)
         return loss
 
     @staticmethod
     def backward(ctx, dloss):
         hidden, weight, targets, lse = ctx.saved_tensors
         lib = _lib.load()
-        dev = hidden.device
         dloss = dloss.contiguous()
-        a = _VocabLoss._args(hidden, weight, targets, ctx.ignore)
-        dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+        dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
                   for t, need in ((hidden, ctx.needs_input_grad[0]), (weight, ctx.needs_input_grad[1])))
-        size = int(lib.ews_vocab_work_size(ctypes.byref(a), 1))
-        work = torch.empty(size, dtype=torch.uint8, device=dev)
-        a.lse, a.dloss, a.dhidden, a.dweight = _ptr(lse), _ptr(dloss), _ptr(dh), _ptr(dw)
-        a.work, a.work_bytes = _ptr(work), size
-        a.status = engine.index_word(dev)[0]
-        with torch.cuda.device(dev), _timed("ews_vocab_bwd", dev, a.rows):
-            _lib.check(lib.ews_vocab_bwd(ctypes.byref(a), _stream_ptr(dev)), "ews_vocab_bwd")
-        _after(dev)
+        work = _work(lib.ews_vocab_work_size(_vocab_args(hidden, weight, targets, ctx.ignore), 1), hidden)
+        args = _vocab_args(hidden, weight, targets, ctx.ignore, None, lse, dloss, dh, dw, work)
+        _launch(hidden.get_device(), "ews_vocab_bwd", hidden.shape[0], lib.ews_vocab_bwd, args)
         return dh, dw, None, None
 
 
@@ -349,10 +347,13 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
     if hidden.dtype != weight.dtype:
         raise TypeError(f"hidden and weight must share a type, got {hidden.dtype} and {weight.dtype}")
     _dtype(hidden, "hidden and weight")
-    _indices(targets, "targets")
+    _wide(targets, "targets")
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} must have the shape {tuple(hidden.shape[:-1])}")
-    dev = _same_device(hidden, weight, targets)
-    engine.raise_index(dev)
-    loss = _VocabLoss.apply(hidden.reshape(-1, hidden.shape[-1]), weight, targets.reshape(-1), int(ignore_index))
-    return loss.reshape(targets.shape)
+    _device(hidden, weight, targets)
+    flat, t = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        loss = _VocabLoss.apply(flat, weight, t, int(ignore_index))
+    else:
+        loss = _vocab(_rows(flat), _rows(weight), t, int(ignore_index))[0]
+    return loss if targets.dim() == 1 else loss.reshape(targets.shape)
