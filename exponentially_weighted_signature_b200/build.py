@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libews_b200.so")
 SOURCES = ["ews_capi.cu", "ews_diag.cu", "ews_dense.cu", "ews_block.cu", "ews_tables.cu", "ews_diag_term.cu",
-           "ews_graded.cu", "ews_clock.cu", "ews_embed.cu", "ews_decay.cu", "ews_decay_tc.cu",
+           "ews_graded.cu", "ews_clock.cu", "ews_embed.cu", "ews_decay.cu", "ews_decay_tc.cu", "ews_decay_f32.cu",
            "ews_vocab.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [

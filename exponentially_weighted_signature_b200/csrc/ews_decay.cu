@@ -564,6 +564,9 @@ size_t seg_bytes(const ews_decay_args* a, int dx, int dz) {
         if (t > segs) segs = t;
         const int f = tc_segments(a->batch, a->steps, a->heads, false, &span);
         if (f > segs) segs = f;
+    } else if (dx <= 64) {
+        const int f = tc_segments(a->batch, a->steps, a->heads * slices, false, &span);
+        if (f > segs && f > 1) segs = f;
     }
     return sizeof(float) * (size_t)a->batch * a->heads * segs * dx * dz;
 }
@@ -616,12 +619,28 @@ int run_tc(Chain<bf16> a, cudaStream_t s) {
     return tc_chain(a, false, false, s);
 }
 
+int run_f32(Chain<float> a, cudaStream_t s) {
+    a.slices = (a.z.width + 63) / 64;
+    a.segs = tc_segments(a.batch, a.steps, a.heads * a.slices, false, &a.span);
+    if (a.segs > 1) {
+        if (!a.seg) return EWS_ERR_WORKSPACE;
+        int rc = f32_chain(a, true, s);
+        if (rc != EWS_OK) return rc;
+        Chain<float> j = a;
+        j.down = a.rev;
+        if ((rc = join<float>(j, s)) != EWS_OK) return rc;
+    }
+    return f32_chain(a, false, s);
+}
+
 // NS for a state that leaves the kernel in float32 is three, for one that only feeds rounded outputs two.
 template <typename T>
 int run_chain(Chain<T> a, cudaStream_t s) {
     constexpr bool f32 = sizeof(T) == 4;
     if constexpr (!f32) {
         if (tc_fits(a)) return run_tc(a, s);
+    } else {
+        if (f32_fits(a)) return run_f32(a, s);
     }
     plan(a.batch, a.steps, a.heads, a.z.width, &a.slices, &a.segs, &a.span);
     const bool exact = a.fin != nullptr && !f32;
