@@ -21,10 +21,10 @@ namespace {
 constexpr int FC = 128, FW = 64;       // tokens of a chunk, columns of a tile
 constexpr int PLANE = FC * 128;        // bytes of a plane of a stream, 128-byte rows
 constexpr int SPLANE = FW * 128;       // of the state
-constexpr int FTHR = 32 * 13;          // warps: MMA, four of group A, eight of group B
+constexpr int FTHR = 32 * 13;          // warps: MMA, four of group A, eight of group B (at most 16: 128 registers)
 constexpr uint32_t TP = 0, TPP = 128, TO1 = 320, TO2 = 384, TU = 448;  // tensor-memory columns
 constexpr int LX = 0, LY = LX + 3 * PLANE, LW = LY + 3 * PLANE, LZ = LW + 3 * PLANE, LS = LZ + 3 * PLANE, LBAR = LS + 3 * SPLANE,
-              LPA = LBAR + 128, LPB = LPA + 4 * (FC + 4), LEND = LPB + 4 * (FC + 4);
+              LTAB = LBAR + 128, LEND = LTAB + DECAY_BYTES;
 
 struct Place {
     int b, h, seg, c0, dz;
@@ -32,14 +32,21 @@ struct Place {
     int t0, t1, end, chunks;
 };
 
+__device__ __forceinline__ void prefetch_l2(const float* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// Up to four values of a row that 16-byte loads cannot read.
+__device__ __noinline__ float4 load_ragged(const float* p, int left) {
+    return make_float4(p[0], left > 1 ? p[1] : 0.f, left > 2 ? p[2] : 0.f, left > 3 ? p[3] : 0.f);
+}
+
 // Four neighbouring values into the three planes of a tile, at (row, 4 col4).
-__device__ __forceinline__ void put4(unsigned char* tile, int plane, int row, int col4, float4 v) {
+__device__ __forceinline__ void put4(unsigned char* tile, int plane, int row, int col4, uint64_t a, uint64_t b) {
     unsigned char* p = tile + row * 128 + (((col4 >> 1) ^ (row & 7)) << 4) + (col4 & 1) * 8;
+    const uint64_t minus_one = pair(-1.f, -1.f);
 #pragma unroll
     for (int s = 0; s < 3; ++s) {
-        const uint32_t a = pack_bf16(v.x, v.y), b = pack_bf16(v.z, v.w);
-        *reinterpret_cast<uint2*>(p + s * plane) = make_uint2(a, b);
-        v.x -= bf16_lo(a), v.y -= bf16_hi(a), v.z -= bf16_lo(b), v.w -= bf16_hi(b);
+        const uint32_t u = s == 2 ? round2(a) : round2(a, minus_one), w = s == 2 ? round2(b) : round2(b, minus_one);
+        *reinterpret_cast<uint2*>(p + s * plane) = make_uint2(u, w);
     }
 }
 
@@ -49,16 +56,16 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
     unsigned char* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + LBAR);
     uint64_t *xy_ready = bars, *z_ready = bars + 1, *p_full = bars + 2, *p_ready = bars + 3, *u_full = bars + 4, *o_full = bars + 5,
-             *o_free = bars + 6, *drained = bars + 7, *sync_a = bars + 8, *sync_b = bars + 9;
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 10);
+             *o_free = bars + 6, *drained = bars + 7, *sync_a = bars + 8;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 9);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int dx = a.y.width;
 
     if (threadIdx.x == 0) {
         mbar_init(p_full, 1), mbar_init(u_full, 1), mbar_init(o_full, 1), mbar_init(drained, 1);
         mbar_init(xy_ready, 256), mbar_init(z_ready, 256), mbar_init(p_ready, 128), mbar_init(o_free, 128);
-        mbar_init(sync_a, 128), mbar_init(sync_b, 256);
+        mbar_init(sync_a, 128);
         *fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -69,7 +76,7 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
 
     auto place = [&](int w) {
         Place it;
@@ -90,71 +97,90 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
     auto chunk_at = [&](const Place& it, int c) { return it.t0 + (a.rev ? it.chunks - 1 - c : c) * FC; };
 
     if (warp == 0) {
-        if (lane == 0) {
-            constexpr uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(FC >> 4) << 24);
-            constexpr uint32_t amn = 1u << 15, bmn = 1u << 16, np = (uint32_t)(FC >> 3) << 17;
-            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
-            const int kx = (dx + 15) / 16;
-            const uint32_t S = smem_u32(sm);
-            long n = 0;
-            bool ok = true;
-            for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
-                const Place it = place(w);
-                if (skip(it)) continue;
-                const uint32_t nz = (uint32_t)((it.dz + 15) / 16 * 2) << 17;
-                for (int c = 0; ok && c < it.chunks; ++c, ++n) {
-                    const uint32_t ph = (uint32_t)(n & 1);
-                    if (!(ok = mbar_wait(xy_ready, ph, fail))) break;
-                    fence_after();
-                    if (!STATE) {
+        constexpr uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(FC >> 4) << 24);
+        constexpr uint32_t amn = 1u << 15, bmn = 1u << 16, np = (uint32_t)(FC >> 3) << 17;
+        // planes of the six products, a nibble each, smallest products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+        constexpr int PA = 0x001102, PB = 0x010120;
+        // descriptors of the first planes' first k-step (columns of x and y beyond their width are zero)
+        const uint32_t S = smem_u32(sm);
+        const uint64_t dX = desc(S + LX, false), dY = desc(S + LY, false), dS = desc(S + LS, true), dW = desc(S + LW, true, 0),
+                       dZ = desc(S + LZ, true);
+        long n = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
+            const Place it = place(w);
+            if (skip(it)) continue;
+            const uint32_t nz = (uint32_t)((it.dz + 15) / 16 * 2) << 17;
+            for (int c = 0; ok && c < it.chunks; ++c, ++n) {
+                const uint32_t ph = (uint32_t)(n & 1);
+                if (!(ok = warp_wait(xy_ready, ph, fail))) break;
+                fence_after();
+                if (!STATE) {
+                    if (elect_one()) {
+#pragma unroll 1
+                        for (int p = 0; p < 6; ++p) {
+                            const uint64_t da = dX + ((PA >> (4 * p)) & 3) * (PLANE / 16), db = dY + ((PB >> (4 * p)) & 3) * (PLANE / 16);
 #pragma unroll
-                        for (int p = 0; p < 6; ++p)
-                            for (int q = 0; q < kx; ++q)
-                                mma_bf16(tmem + TP, desc(S + LX + PA[p] * PLANE + q * 32, false), desc(S + LY + PB[p] * PLANE + q * 32, false),
-                                         base | np, p > 0 || q > 0);
+                            for (int q = 0; q < FW / 16; ++q) mma_bf16(tmem + TP, da + q * 2, db + q * 2, base | np, p > 0 || q > 0);
+                        }
                         mma_commit(p_full);
-                        if (!(ok = mbar_wait(o_free, ph ^ 1u, fail))) break;
-                        fence_after();
-#pragma unroll
-                        for (int p = 0; p < 6; ++p)
-                            for (int q = 0; q < kx; ++q)
-                                mma_bf16(tmem + TO1, desc(S + LX + PA[p] * PLANE + q * 32, false), desc(S + LS + PB[p] * SPLANE + q * 2048, true),
-                                         base | bmn | nz, p > 0 || q > 0);
                     }
-                    if (!(ok = mbar_wait(z_ready, ph, fail))) break;
+                    __syncwarp();
+                    if (!(ok = warp_wait(o_free, ph ^ 1u, fail))) break;
                     fence_after();
-                    // the weighted y is one box of 64 columns; the accumulator's upper 64 rows repeat it and are not read
+                    if (elect_one()) {
+#pragma unroll 1
+                        for (int p = 0; p < 6; ++p) {
+                            const uint64_t da = dX + ((PA >> (4 * p)) & 3) * (PLANE / 16), db = dS + ((PB >> (4 * p)) & 3) * (SPLANE / 16);
 #pragma unroll
-                    for (int p = 0; p < 6; ++p)
-                        for (int q = 0; q < FC / 16; ++q)
-                            mma_bf16(tmem + TU, desc(S + LW + PA[p] * PLANE + q * 2048, true, 0), desc(S + LZ + PB[p] * PLANE + q * 2048, true),
-                                     base | amn | bmn | nz, p > 0 || q > 0);
+                            for (int q = 0; q < FW / 16; ++q) mma_bf16(tmem + TO1, da + q * 2, db + q * 128, base | bmn | nz, p > 0 || q > 0);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!(ok = warp_wait(z_ready, ph, fail))) break;
+                fence_after();
+                // the weighted y is one box of 64 columns; the accumulator's upper 64 rows repeat it and are not read
+                if (elect_one()) {
+#pragma unroll 1
+                    for (int p = 0; p < 6; ++p) {
+                        const uint64_t da = dW + ((PA >> (4 * p)) & 3) * (PLANE / 16), db = dZ + ((PB >> (4 * p)) & 3) * (PLANE / 16);
+#pragma unroll
+                        for (int q = 0; q < FC / 16; ++q) mma_bf16(tmem + TU, da + q * 128, db + q * 128, base | amn | bmn | nz, p > 0 || q > 0);
+                    }
                     mma_commit(u_full);
-                    if (!STATE) {
-                        if (!(ok = mbar_wait(p_ready, ph, fail))) break;
-                        fence_after();
+                }
+                __syncwarp();
+                if (!STATE) {
+                    if (!(ok = warp_wait(p_ready, ph, fail))) break;
+                    fence_after();
+                    if (elect_one()) {
+#pragma unroll 1
+                        for (int p = 0; p < 6; ++p) {
+                            const uint32_t ta = tmem + TPP + ((PA >> (4 * p)) & 3) * 64;
+                            const uint64_t db = dZ + ((PB >> (4 * p)) & 3) * (PLANE / 16);
 #pragma unroll
-                        for (int p = 0; p < 6; ++p)
-                            for (int q = 0; q < FC / 16; ++q)
-                                mma_bf16_ta(tmem + TO2, tmem + TPP + PA[p] * 64 + q * 8, desc(S + LZ + PB[p] * PLANE + q * 2048, true),
-                                            base | bmn | nz, p > 0 || q > 0);
+                            for (int q = 0; q < FC / 16; ++q) mma_bf16_ta(tmem + TO2, ta + q * 8, db + q * 128, base | bmn | nz, p > 0 || q > 0);
+                        }
                         mma_commit(o_full);
                     }
+                    __syncwarp();
                 }
             }
-            if (!ok) {
-                mma_commit(drained);
-                mbar_drain(drained, 0);
-            }
+        }
+        if (!ok) {
+            if (elect_one()) mma_commit(drained);
+            __syncwarp();
+            mbar_drain(drained, 0);
         }
     } else if (warp < 5) {
-        if (!STATE) {  // group A
-            float* pw = reinterpret_cast<float*>(sm + LPA);
+        if (!STATE) {  // group A: a thread a row
             const int quarter = warp & 3, i = quarter * 32 + lane, tid = threadIdx.x - 32;
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
             float* out = a.out32 ? a.out32 : a.out;
             const int dz = a.z.width;
             const bool vec = dz % 4 == 0 && aligned16_dev(out);
+            const uint64_t minus_one = pair(-1.f, -1.f);
             long n = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -162,36 +188,38 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                 const Place it = place(w);
                 if (!(ok = group_sync(sync_a, phase, fail))) break;
                 const float rate = a.rate[it.h];
-                pw[tid] = tid == 0 ? 1.f : expf(-rate * (float)tid);
-                if (tid == 0) pw[FC] = expf(-rate * (float)FC);
+                put_decay(sm + LTAB, tid, 128, rate, a.rev);
+                const float wfull = decay_of(rate, a.rev ? FC - 1 - i : i + 1) * a.oscale;  // the carry's weight, of a full chunk
+                const uint32_t row_tab = smem_u32(sm + LTAB) + (i + 127) * 8;
                 if (!(ok = group_sync(sync_a, phase, fail))) break;
                 for (int c = 0; c < it.chunks; ++c, ++n) {
                     const int t = chunk_at(it, c), m = min(FC, it.end - t);
                     const uint32_t ph = (uint32_t)(n & 1);
                     if (!(ok = __all_sync(kFull, mbar_wait(p_full, ph, fail)))) break;
                     fence_after();
+#pragma unroll 1
                     for (int cb = 0; cb < 4; ++cb) {
-                        float v[32];
-                        const bool on = a.rev ? cb >= quarter : cb <= quarter;
-                        if (on) {
-                            tmem_ld32(tmem + TP + lanes + cb * 32, v);
+                        uint64_t v[16];
+                        if (a.rev ? cb >= quarter : cb <= quarter) {
+                            float e[32];
+                            tmem_ld32(tmem + TP + lanes + cb * 32, e);
+                            if (m < FC) {  // a score with no token behind it may be anything
+                                const int left = m - cb * 32;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int col = cb * 32 + j, gap = a.rev ? col - i : i - col;
-                                v[j] = gap >= 0 && col < m ? v[j] * pw[max(gap, 0)] : 0.f;
+                                for (int j = 0; j < 32; ++j) e[j] = j < left ? e[j] : 0.f;
                             }
+                            const uint32_t g = row_tab - cb * 256;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[j] = mul2(pair(e[2 * j], e[2 * j + 1]), lds64(g - 16 * j));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[j] = 0ull;
                         }
-                        uint32_t packed[16];
-#pragma unroll
+#pragma unroll 1
                         for (int s = 0; s < 3; ++s) {
+                            uint32_t packed[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                packed[j] = 0u;
-                                if (on) {
-                                    packed[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-                                    v[2 * j] -= bf16_lo(packed[j]), v[2 * j + 1] -= bf16_hi(packed[j]);
-                                }
-                            }
+                            for (int j = 0; j < 16; ++j) packed[j] = round2(v[j], minus_one);
                             tmem_st16(tmem + TPP + lanes + s * 64 + cb * 16, packed);
                         }
                     }
@@ -202,28 +230,40 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                     if (!(ok = __all_sync(kFull, mbar_wait(o_full, ph, fail)))) break;
                     fence_after();
                     const bool in = i < m;
-                    const float wi = a.rev ? pw[max(m - 1 - i, 0)] : pw[i + 1];
+                    const float wi = m == FC ? wfull : (a.rev ? decay_of(rate, m - 1 - i) * a.oscale : wfull);
+                    const uint64_t wi2 = pair(wi, wi), os2 = pair(a.oscale, a.oscale);
                     float* o = out + (((long)it.b * a.steps + t + i) * a.heads + it.h) * dz + it.c0;
-                    for (int cb = 0; cb * 32 < it.dz; ++cb) {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < FW; c0 += 32) {
+                        const int width = it.dz - c0;
                         float u[32], v[32];
-                        tmem_ld32(tmem + TO1 + lanes + cb * 32, u);
-                        tmem_ld32(tmem + TO2 + lanes + cb * 32, v);
-                        if (cb * 32 + 32 >= it.dz) {  // the accumulators are read: the next chunk's products may have them
+                        if (width > 0) {
+                            tmem_ld32(tmem + TO1 + lanes + c0, u);
+                            tmem_ld32(tmem + TO2 + lanes + c0, v);
+                        }
+                        if (c0 + 32 == FW) {  // the accumulators are read
                             fence_before();
                             mbar_arrive(o_free);
                         }
-                        if (t + i < it.t1) {
+                        if (width <= 0 || t + i >= it.t1) continue;
+                        uint64_t r[16];
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = in ? fmaf(wi, u[j], v[j]) * a.oscale : 0.f;
-                            const int width = it.dz - cb * 32;
-                            if (vec && width >= 32) {
+                        for (int j = 0; j < 16; ++j)
+                            r[j] = fma2(wi2, pair(u[2 * j], u[2 * j + 1]), mul2(os2, pair(v[2 * j], v[2 * j + 1])));
+                        if (!in) {
 #pragma unroll
-                                for (int j = 0; j < 32; j += 4)
-                                    *reinterpret_cast<float4*>(o + cb * 32 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                            } else {
+                            for (int j = 0; j < 16; ++j) r[j] = 0ull;
+                        }
+                        if (vec && width >= 32) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j < width) o[cb * 32 + j] = v[j];
+                            for (int j = 0; j < 16; j += 2) *reinterpret_cast<ulonglong2*>(o + c0 + 2 * j) = make_ulonglong2(r[j], r[j + 1]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                float e0, e1;
+                                unpair(r[j], e0, e1);
+                                if (2 * j < width) o[c0 + 2 * j] = e0;
+                                if (2 * j + 1 < width) o[c0 + 2 * j + 1] = e1;
                             }
                         }
                     }
@@ -235,46 +275,21 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
             }
         }
     } else {  // group B
-        float* pw = reinterpret_cast<float*>(sm + LPB);
         const int tid = threadIdx.x - 160, quarter = warp & 3, half = (warp - 5) >> 2, row = quarter * 32 + lane;
         const bool keeper = quarter < 2;  // the state has at most 64 rows: four warps keep it, 32 columns each
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         long n = 0;
-        uint32_t phase = 0;
         bool ok = true;
 
-        // a thread's eight groups of four values of a tile: rows tid / 16 + 16 k, columns 4 (tid % 16) on
-        auto load = [&](const Stream<float>& s, const float* p, int t, int m, int c0, float4 v[8]) {
-            const int col = c0 + (tid & 15) * 4;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int r = (tid >> 4) + 16 * k;
-                float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < m) {
-                    const float* at = p + (long)(t + r) * s.st + col;
-                    if (s.vec) {
-                        if (col < s.width) q = __ldg(reinterpret_cast<const float4*>(at));
-                    } else {
-                        if (col < s.width) q.x = at[0];
-                        if (col + 1 < s.width) q.y = at[1];
-                        if (col + 2 < s.width) q.z = at[2];
-                        if (col + 3 < s.width) q.w = at[3];
-                    }
-                }
-                v[k] = q;
-            }
-        };
         for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
             const Place it = place(w);
             if (skip(it)) continue;
             const float* xb = STATE ? nullptr : a.x.p + it.b * a.x.sb + (it.h / a.x.group) * a.x.sh;
             const float* yb = a.y.p + it.b * a.y.sb + (it.h / a.y.group) * a.y.sh;
             const float* zb = a.z.p + it.b * a.z.sb + (it.h / a.z.group) * a.z.sh;
-            if (!(ok = group_sync(sync_b, phase, fail))) break;
             const float rate = a.rate[it.h];
-            if (tid <= FC) pw[tid] = tid == 0 ? 1.f : expf(-rate * (float)tid);
-            if (!(ok = group_sync(sync_b, phase, fail))) break;
-            float s[32];
+            const float gfull = decay_of(rate, FC);
+            uint64_t s[16];
             const long per = (long)dx * a.z.width;
             const float* init = nullptr;
             long ir = 0, ic = 0;
@@ -285,50 +300,82 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
             }
             if (keeper) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const int col = half * 32 + j;
-                    s[j] = init && row < dx && col < it.dz ? init[row * ir + (it.c0 + col) * ic] * scale : 0.f;
+                for (int j = 0; j < 16; ++j) {
+                    float e[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int col = half * 32 + 2 * j + k;
+                        e[k] = init && row < dx && col < it.dz ? init[row * ir + (it.c0 + col) * ic] * scale : 0.f;
+                    }
+                    s[j] = pair(e[0], e[1]);
                 }
             }
             for (int c = 0; c < it.chunks; ++c, ++n) {
                 const int t = chunk_at(it, c), m = min(FC, it.end - t);
                 const uint32_t ph = (uint32_t)(n & 1);
-                float4 y[8], x[8];
-                load(a.y, yb, t, m, 0, y);
-                if (!STATE) load(a.x, xb, t, m, 0, x);
                 // the products of the chunk before that read these tiles are done (n > 0: its state update waited)
                 if (!STATE && keeper) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        put4(sm + LS, SPLANE, row, half * 8 + j / 4, make_float4(s[j], s[j + 1], s[j + 2], s[j + 3]));
+                    for (int j = 0; j < 16; j += 2) put4(sm + LS, SPLANE, row, half * 8 + j / 2, s[j], s[j + 1]);
                 }
+                // y, x, z: a thread has rows tid / 16 + 16 k, columns 4 (tid % 16) on
+#pragma unroll 1
+                for (int part = 0; part < 3; ++part) {
+                    if (STATE && part == 1) part = 2;
+                    const Stream<float>& st = part == 0 ? a.y : part == 1 ? a.x : a.z;
+                    const float* p = part == 0 ? yb : part == 1 ? xb : zb;
+                    const int col = (part == 2 ? it.c0 : 0) + (tid & 15) * 4, left = st.width - col;
+                    float4 v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = (tid >> 4) + 16 * k;
-                    const float wt = r < m ? pw[a.rev ? r + 1 : m - 1 - r] : 0.f;
-                    if (!STATE) {
-                        put4(sm + LY, PLANE, r, tid & 15, y[k]);
-                        put4(sm + LX, PLANE, r, tid & 15, x[k]);
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = (tid >> 4) + 16 * k;
+                        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (r < m && left > 0) {
+                            const float* at = p + (long)(t + r) * st.st + col;
+                            if (st.vec) v[k] = __ldg(reinterpret_cast<const float4*>(at));
+                            else v[k] = load_ragged(at, left);
+                        }
                     }
-                    if (r < m) y[k].x *= wt, y[k].y *= wt, y[k].z *= wt, y[k].w *= wt;
-                    put4(sm + LW, PLANE, r, tid & 15, y[k]);
-                }
-                fence_async_smem();
-                mbar_arrive(xy_ready);
-                load(a.z, zb, t, m, it.c0, x);
-                if (!STATE && !(ok = __all_sync(kFull, mbar_wait(o_full, ph ^ 1u, fail)))) break;
+                    if (part == 2) {
+                        if (!STATE && !(ok = __all_sync(kFull, mbar_wait(o_full, ph ^ 1u, fail)))) break;
+                    }
+                    unsigned char* tile = sm + (part == 0 ? LY : part == 1 ? LX : LZ);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) put4(sm + LZ, PLANE, (tid >> 4) + 16 * k, tid & 15, x[k]);
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = (tid >> 4) + 16 * k;
+                        const uint64_t lo = pair(v[k].x, v[k].y), hi = pair(v[k].z, v[k].w);
+                        if (!(STATE && part == 0)) put4(tile, PLANE, r, tid & 15, lo, hi);
+                        if (part == 0) {
+                            const float wt = decay_of(rate, a.rev ? r + 1 : m - 1 - r);  // a row that is no token is zero
+                            const uint64_t wt2 = pair(wt, wt);
+                            put4(sm + LW, PLANE, r, tid & 15, mul2(lo, wt2), mul2(hi, wt2));
+                        }
+                    }
+                    if (part == (STATE ? 0 : 1)) {
+                        fence_async_smem();
+                        mbar_arrive(xy_ready);
+                    }
+                }
+                if (!ok) break;
                 fence_async_smem();
                 mbar_arrive(z_ready);
+                if (c + 1 < it.chunks) {  // the next chunk's rows on their way to L2: two threads a row
+                    const int t2 = chunk_at(it, c + 1), r = tid >> 1, half_row = (tid & 1) * 32;
+                    if (t2 + r < it.end) {
+                        if (!STATE && half_row < a.x.width) prefetch_l2(xb + (long)(t2 + r) * a.x.st + half_row);
+                        if (half_row < a.y.width) prefetch_l2(yb + (long)(t2 + r) * a.y.st + half_row);
+                        if (it.c0 + half_row < a.z.width) prefetch_l2(zb + (long)(t2 + r) * a.z.st + it.c0 + half_row);
+                    }
+                }
                 if (!(ok = __all_sync(kFull, mbar_wait(u_full, ph, fail)))) break;
                 fence_after();
                 if (keeper && half * 32 < it.dz) {
-                    const float gn = pw[m];
+                    const float gn = m == FC ? gfull : decay_of(rate, m);
+                    const uint64_t gn2 = pair(gn, gn);
                     float v[32];
                     tmem_ld32(tmem + TU + lanes + half * 32, v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j] = fmaf(gn, s[j], v[j]);
+                    for (int j = 0; j < 16; ++j) s[j] = fma2(gn2, s[j], pair(v[2 * j], v[2 * j + 1]));
                 }
                 fence_before();
             }
@@ -338,10 +385,18 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
             float fscale = 1.f;
             if (STATE) fin = a.seg + (it.bh * a.segs + it.seg) * per, fr = a.z.width, fc = 1;
             else if (a.segs == 1 && a.fin) fin = a.fin + it.bh * per, fr = a.fin_r, fc = a.fin_c, fscale = a.fin_scale;
-            if (fin && keeper && row < dx)
+            if (fin && keeper && row < dx) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (half * 32 + j < it.dz) fin[row * fr + (it.c0 + half * 32 + j) * fc] = s[j] * fscale;
+                for (int j = 0; j < 16; ++j) {
+                    float e[2];
+                    unpair(s[j], e[0], e[1]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int col = half * 32 + 2 * j + k;
+                        if (col < it.dz) fin[row * fr + (it.c0 + col) * fc] = e[k] * fscale;
+                    }
+                }
+            }
         }
     }
     __syncthreads();

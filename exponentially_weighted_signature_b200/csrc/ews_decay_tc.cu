@@ -7,10 +7,11 @@
 //     O2 = P Z              (tokens x dz)          -> out = g^(i+1) O1 + O2
 //
 // One persistent CTA per SM walks (sample, head, segment) items. Warp 0 fetches tiles by TMA, warp 1 issues the
-// products, warps 2-5 (A) turn P into an operand and write the output (staged in the chunk's X tile, stored by
-// TMA), warps 6-13 (B) weight Y (in place, and its rounding residue beside it: the weighted operand is inexact, two
-// bfloat16 pieces carry it to 2^-16, three to 2^-24), keep the state and write its bfloat16 copy. The only chain
-// from chunk to chunk is U -> State -> O1; the loads, P and the output of neighbouring chunks run beside it.
+// products, warps 2-5 (A) turn P into an operand, warps 6-13 (B) weight Y (in place, and its rounding residue
+// beside it: the weighted operand is inexact, two bfloat16 pieces carry it to 2^-16, three to 2^-24), write the
+// output of the chunk before, keep the state and write its bfloat16 copy. The only chain from chunk to chunk is
+// U -> State -> O1; the loads, P and the output of neighbouring chunks run beside it.
+// X and Y, which a chunk needs first, have two buffers, Z (with the state's passes of their own: two) one.
 // Why 128 tokens: the accumulator has 128 rows; the waste of the upper half of P is 1/10 of a chunk's products.
 //
 // Reversed chains keep the rows' order and walk the chunks down: decays are then g^(j-i) for j >= i, a row's weight of
@@ -28,19 +29,18 @@ namespace {
 constexpr int TC = 128;                  // tokens of a chunk
 constexpr int BOX = TC * 128;            // bytes of 64 columns of a tile
 constexpr int TILE = 2 * BOX;
-constexpr int NTHR = 32 * 14;
+constexpr int NTHR = 32 * 14;  // at most 16 warps: 128 registers a thread
 constexpr uint32_t TP = 0, TO1 = 128, TO2 = 256, TU = 384;  // tensor-memory columns
 
 struct Maps {
-    CUtensorMap x, y, z, out;
+    CUtensorMap x, y, z;
 };
 
 template <bool STATE, int NS>
 struct Lay {
-    static constexpr int ZST = STATE ? 2 : 1;
-    static constexpr int X = 0, Y = X + (STATE ? 0 : 2 * TILE), Z = Y + 2 * TILE, S = Z + ZST * TILE, LO = S + (STATE ? 0 : TILE),
-                         BARS = LO + (NS - 1) * TILE, PWA = BARS + 256, PWB = PWA + 4 * (TC + 4), END = PWB + 4 * (TC + 4);
-    static constexpr size_t bytes = END + 1024;
+    static constexpr int X = 0, Y = X + (STATE ? 0 : 2 * TILE), Z = Y + 2 * TILE, S = Z + (STATE ? 2 : 1) * TILE, LO = S + (STATE ? 0 : TILE),
+                         BARS = LO + (NS - 1) * TILE, TAB = BARS + 256, END = TAB + DECAY_BYTES;
+    static constexpr size_t bytes = END;
 };
 
 __device__ __forceinline__ void tma_load4(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int t, int h, int b) {
@@ -49,11 +49,6 @@ __device__ __forceinline__ void tma_load4(const CUtensorMap* map, uint64_t* bar,
             smem_u32(dst)),
         "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
         : "memory");
-}
-__device__ __forceinline__ void tma_store4(const CUtensorMap* map, const void* src, int x, int t, int h, int b) {
-    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(smem_u32(src)),
-                 "r"(x), "r"(t), "r"(h), "r"(b)
-                 : "memory");
 }
 // An item's place: sample, head, its tokens [t0, t1), of which [t0, end) exist, and its chunks.
 struct Item {
@@ -65,15 +60,19 @@ struct Item {
 template <bool STATE, int NS>
 __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Chain<bf16> a, const __grid_constant__ Maps maps, int items) {
     using L = Lay<STATE, NS>;
-    extern __shared__ unsigned char raw[];
-    unsigned char* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    // the tiles' swizzle wants 1,024-byte boundaries; there is no room to round up
+    extern __shared__ __align__(1024) unsigned char sm[];
+    if (smem_u32(sm) & 1023) {
+        report(a.status, EWS_ERR_LAUNCH);
+        return;
+    }
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
     uint64_t *x_full = bars, *y_full = bars + 2, *z_full = bars + 4, *x_empty = bars + 6, *y_empty = bars + 8, *z_empty = bars + 10;
     uint64_t *p_full = bars + 12, *p_ready = bars + 13, *o_full = bars + 14, *o_free = bars + 15, *s_ready = bars + 16,
-             *yw_ready = bars + 17, *u_full = bars + 18, *xs_done = bars + 19, *drained = bars + 20, *sync_a = bars + 21, *sync_b = bars + 22;
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 23);
+             *yw_ready = bars + 17, *u_full = bars + 18, *xs_done = bars + 19, *drained = bars + 20, *sync_a = bars + 21;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int dx = a.y.width, dz = a.z.width;
     const int dx16 = (dx + 15) & ~15, dz16 = (dz + 15) & ~15;
 
@@ -81,7 +80,7 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
         for (int i = 0; i < 12; ++i) mbar_init(bars + i, 1);
         mbar_init(p_full, 1), mbar_init(o_full, 1), mbar_init(u_full, 1), mbar_init(xs_done, 1), mbar_init(drained, 1);
         mbar_init(p_ready, 128), mbar_init(o_free, 128), mbar_init(s_ready, 256), mbar_init(yw_ready, 256);
-        mbar_init(sync_a, 128), mbar_init(sync_b, 256);
+        mbar_init(sync_a, 128);
         *fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -92,7 +91,7 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
 
     auto place = [&](int w) {
         Item it;
@@ -118,8 +117,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 const Item it = place(w);
                 if (skip(it)) continue;
                 for (int c = 0; c < it.chunks; ++c, ++n) {
-                    const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, s = (int)(n & 1), zs = STATE ? s : 0;
-                    const uint32_t two = (uint32_t)((n >> 1) & 1) ^ 1u, zp = STATE ? two : (uint32_t)(n & 1) ^ 1u;
+                    const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, s = (int)(n & 1);
+                    const uint32_t two = (uint32_t)((n >> 1) & 1) ^ 1u;
                     if (!(ok = mbar_wait(y_empty + s, two, fail))) break;
                     const int bx = dx > 64 ? 2 : 1, bz = dz > 64 ? 2 : 1;
                     mbar_expect(y_full + s, bx * BOX);
@@ -131,7 +130,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                         for (int j = 0; j < bx; ++j)
                             tma_load4(&maps.x, x_full + s, sm + L::X + s * TILE + j * BOX, j * 64, t, it.h / a.x.group, it.b);
                     }
-                    if (!(ok = mbar_wait(z_empty + zs, zp, fail))) break;
+                    const int zs = STATE ? s : 0;
+                    if (!(ok = mbar_wait(z_empty + zs, STATE ? two : (uint32_t)(n & 1) ^ 1u, fail))) break;
                     mbar_expect(z_full + zs, bz * BOX);
                     for (int j = 0; j < bz; ++j)
                         tma_load4(&maps.z, z_full + zs, sm + L::Z + zs * TILE + j * BOX, j * 64, t, it.h / a.z.group, it.b);
@@ -147,66 +147,96 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC >> 4) << 24);
-            constexpr uint32_t amn = 1u << 15, bmn = 1u << 16;
-            const uint32_t nz = (uint32_t)(dz16 >> 3) << 17, np = (uint32_t)(TC >> 3) << 17;
-            const int kx = dx16 / 16;
-            long n = 0;
-            bool ok = true;
-            for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
-                const Item it = place(w);
-                if (skip(it)) continue;
-                for (int c = 0; ok && c < it.chunks; ++c, ++n) {
-                    const int s = (int)(n & 1), zs = STATE ? s : 0;
-                    const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
-                    const uint32_t X = smem_u32(sm + L::X + s * TILE), Y = smem_u32(sm + L::Y + s * TILE),
-                                   Z = smem_u32(sm + L::Z + zs * TILE), SB = smem_u32(sm + L::S);
-                    if (!STATE) {
-                        if (!(ok = mbar_wait(x_full + s, two, fail) && mbar_wait(y_full + s, two, fail))) break;
-                        fence_after();
-                        for (int q = 0; q < kx; ++q) {
-                            const uint32_t off = (q >> 2) * BOX + (q & 3) * 32;
-                            mma_bf16(tmem + TP, desc(X + off, false), desc(Y + off, false), base | np, q > 0);
-                        }
-                        mma_commit(p_full);
-                        if (!(ok = mbar_wait(s_ready, ph, fail) && mbar_wait(o_free, ph ^ 1u, fail))) break;
-                        fence_after();
-                        for (int q = 0; q < kx; ++q)
-                            mma_bf16(tmem + TO1, desc(X + (q >> 2) * BOX + (q & 3) * 32, false), desc(SB + q * 2048, true, BOX),
-                                     base | bmn | nz, q > 0);
-                        mma_commit(xs_done);
-                    }
-                    if (!(ok = mbar_wait(yw_ready, ph, fail) && mbar_wait(z_full + zs, STATE ? two : ph, fail))) break;
-                    fence_after();
-                    for (int p = NS - 1; p >= 0; --p) {  // the smallest piece first
-                        const uint32_t W = p == 0 ? Y : smem_u32(sm + L::LO + (p - 1) * TILE);
-                        for (int q = 0; q < TC / 16; ++q)
-                            mma_bf16(tmem + TU, desc(W + q * 2048, true, BOX), desc(Z + q * 2048, true, BOX), base | amn | bmn | nz,
-                                     p < NS - 1 || q > 0);
-                    }
-                    mma_commit(u_full);
-                    if (!STATE) {
-                        if (!(ok = mbar_wait(p_ready, ph, fail))) break;
-                        fence_after();
-                        for (int q = 0; q < TC / 16; ++q)
-                            mma_bf16_ta(tmem + TO2, tmem + TP + q * 8, desc(Z + q * 2048, true, BOX), base | bmn | nz, q > 0);
-                        mma_commit(o_full);
-                    }
-                    mma_commit(y_empty + s);
-                    mma_commit(z_empty + zs);
+        constexpr uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC >> 4) << 24);
+        constexpr uint32_t amn = 1u << 15, bmn = 1u << 16;
+        const uint32_t nz = (uint32_t)(dz16 >> 3) << 17, np = (uint32_t)(TC >> 3) << 17;
+        const int kx = dx16 / 16;
+        // descriptors of the tiles' first k-step
+        const uint64_t dS = desc(smem_u32(sm + L::S), true, BOX);
+        const uint64_t dLO = desc(smem_u32(sm + L::LO), true, BOX);
+        long total = 0;  // chunks of this CTA, whichever items they belong to
+        for (int w = blockIdx.x; w < items; w += gridDim.x) {
+            const Item it = place(w);
+            if (!skip(it)) total += it.chunks;
+        }
+        auto scores = [&](long n) {  // P of chunk n
+            const int s = (int)(n & 1);
+            const uint32_t two = (uint32_t)((n >> 1) & 1);
+            if (!(warp_wait(x_full + s, two, fail) && warp_wait(y_full + s, two, fail))) return false;
+            fence_after();
+            if (elect_one()) {
+                const uint64_t dX = desc(smem_u32(sm + L::X + s * TILE), false), dY = desc(smem_u32(sm + L::Y + s * TILE), false);
+                for (int q = 0; q < kx; ++q) {
+                    const int off = (q >> 2) * (BOX >> 4) + (q & 3) * 2;
+                    mma_bf16(tmem + TP, dX + off, dY + off, base | np, q > 0);
                 }
+                mma_commit(p_full);
             }
-            if (!ok) {
-                mma_commit(drained);
-                mbar_drain(drained, 0);
+            __syncwarp();
+            return true;
+        };
+        auto carried = [&](long n) {  // O1 of chunk n
+            const int s = (int)(n & 1);
+            const uint32_t ph = (uint32_t)(n & 1);
+            if (!(warp_wait(s_ready, ph, fail) && warp_wait(o_free, ph ^ 1u, fail))) return false;
+            fence_after();
+            if (elect_one()) {
+                const uint64_t dX = desc(smem_u32(sm + L::X + s * TILE), false);
+                for (int q = 0; q < kx; ++q)
+                    mma_bf16(tmem + TO1, dX + (q >> 2) * (BOX >> 4) + (q & 3) * 2, dS + q * 128, base | bmn | nz, q > 0);
+                mma_commit(xs_done);
+                mma_commit(x_empty + s);
             }
+            __syncwarp();
+            return true;
+        };
+        // In the order in which the others' parts come free: this chunk's scores are an operand first, so O2, then the
+        // next chunk's P for group A, then U for group B's state, then the next chunk's O1 from it.
+        bool ok = STATE || total == 0 || (scores(0) && carried(0));
+        for (long n = 0; ok && n < total; ++n) {
+            const int s = (int)(n & 1);
+            const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
+            const uint64_t dYw = desc(smem_u32(sm + L::Y + s * TILE), true, BOX), dZ = desc(smem_u32(sm + L::Z + (STATE ? s : 0) * TILE), true, BOX);
+            if (!(ok = warp_wait(z_full + (STATE ? s : 0), STATE ? two : ph, fail))) break;
+            if (!STATE) {
+                if (!(ok = warp_wait(p_ready, ph, fail))) break;
+                fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int q = 0; q < TC / 16; ++q)
+                        mma_bf16_ta(tmem + TO2, tmem + TP + q * 8, dZ + q * 128, base | bmn | nz, q > 0);
+                    mma_commit(o_full);
+                }
+                __syncwarp();
+                if (n + 1 < total && !(ok = scores(n + 1))) break;
+            }
+            if (!(ok = warp_wait(yw_ready, ph, fail))) break;
+            fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int p = NS - 1; p >= 0; --p) {  // the smallest piece first
+                    const uint64_t dW = p == 0 ? dYw : dLO + (p > 0 ? p - 1 : 0) * (TILE >> 4);
+#pragma unroll
+                    for (int q = 0; q < TC / 16; ++q)
+                        mma_bf16(tmem + TU, dW + q * 128, dZ + q * 128, base | amn | bmn | nz, p < NS - 1 || q > 0);
+                }
+                mma_commit(u_full);
+                mma_commit(y_empty + s);
+                mma_commit(z_empty + (STATE ? s : 0));
+            }
+            __syncwarp();
+            if (!STATE && n + 1 < total) ok = carried(n + 1);
+        }
+        if (!ok) {
+            if (elect_one()) mma_commit(drained);
+            __syncwarp();
+            mbar_drain(drained, 0);
         }
     } else if (warp < 6) {
-        if (!STATE) {  // group A
-            float* pw = reinterpret_cast<float*>(sm + L::PWA);
+        if (!STATE) {  // group A: a thread a row
             const int quarter = warp & 3, i = quarter * 32 + lane, tid = threadIdx.x - 64;
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+            const bool wide = a.out && dz % 16 == 0 && ((uintptr_t)a.out & 31u) == 0;  // every row starts on a sector
             long n = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -214,27 +244,30 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 const Item it = place(w);
                 if (!(ok = group_sync(sync_a, phase, fail))) break;
                 const float rate = a.rate[it.h];
-                pw[tid] = tid == 0 ? 1.f : expf(-rate * (float)tid);
-                if (tid == 0) pw[TC] = expf(-rate * (float)TC);
+                put_decay(sm + L::TAB, tid, 128, rate, a.rev);
+                const float ofull = decay_of(rate, a.rev ? TC - 1 - i : i + 1) * a.oscale;  // the carry's weight here, of a full chunk
+                const uint32_t row_tab = smem_u32(sm + L::TAB) + (i + 127) * 8;
                 if (!(ok = group_sync(sync_a, phase, fail))) break;
                 for (int c = 0; c < it.chunks; ++c, ++n) {
                     const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, m = min(TC, it.end - t);
                     const uint32_t ph = (uint32_t)(n & 1);
-                    unsigned char* stage = sm + L::X + (int)(n & 1) * TILE;
                     if (!(ok = __all_sync(kFull, mbar_wait(p_full, ph, fail)))) break;
                     fence_after();
+                    // 32 columns at a time; their 16 packed columns go where scores have been read already
+#pragma unroll 1
                     for (int cb = 0; cb < 4; ++cb) {
                         uint32_t packed[16];
                         if (a.rev ? cb >= quarter : cb <= quarter) {
                             float v[32];
                             tmem_ld32(tmem + TP + lanes + cb * 32, v);
+                            if (m < TC) {  // a score with no token behind it may be anything
+                                const int left = m - cb * 32;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int col = cb * 32 + j, gap = a.rev ? col - i : i - col;
-                                v[j] = gap >= 0 && col < m ? v[j] * pw[max(gap, 0)] : 0.f;
+                                for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : 0.f;
                             }
+                            const uint32_t g = row_tab - cb * 256;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) packed[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                            for (int j = 0; j < 16; ++j) packed[j] = round2(mul2(pair(v[2 * j], v[2 * j + 1]), lds64(g - 16 * j)));
                         } else {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) packed[j] = 0u;
@@ -247,44 +280,41 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
 
                     if (!(ok = __all_sync(kFull, mbar_wait(o_full, ph, fail)))) break;
                     fence_after();
-                    const bool in = i < m;
-                    const float wi = a.rev ? pw[max(m - 1 - i, 0)] : pw[i + 1];
-                    for (int cb = 0; cb * 32 < dz; ++cb) {
-                        float u[32], v[32];
-                        tmem_ld32(tmem + TO1 + lanes + cb * 32, u);
-                        tmem_ld32(tmem + TO2 + lanes + cb * 32, v);
+                    const float wi = m == TC || !a.rev ? ofull : decay_of(rate, m - 1 - i) * a.oscale;
+                    const uint64_t wi2 = pair(wi, wi), os2 = pair(a.oscale, a.oscale);
+                    const long at = (((long)it.b * a.steps + t + i) * a.heads + it.h) * dz;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < dz; c0 += 16) {
+                        uint32_t u[16], v[16];
+                        tmem_ld16x2(tmem + TO1 + lanes + c0, tmem + TO2 + lanes + c0, u, v);
+                        uint64_t o[8];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = in ? fmaf(wi, u[j], v[j]) * a.oscale : 0.f;
-                        if (a.out32) {
-                            if (t + i < it.t1) {
-                                float* o = a.out32 + (((long)it.b * a.steps + t + i) * a.heads + it.h) * dz + cb * 32;
+                        for (int j = 0; j < 8; ++j) {
+                            o[j] = fma2(wi2, pair(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])),
+                                        mul2(os2, pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]))));
+                            if (i >= m) o[j] = 0ull;
+                        }
+                        if (t + i >= it.t1) {
+                        } else if (a.out32) {
+                            float* to = a.out32 + at + c0;
 #pragma unroll
-                                for (int j = 0; j < 32; j += 4)
-                                    if (cb * 32 + j < dz) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                            }
+                            for (int j = 0; j < 8; j += 2)
+                                if (c0 + 2 * j < dz) *reinterpret_cast<ulonglong2*>(to + 2 * j) = make_ulonglong2(o[j], o[j + 1]);
                         } else {
-                            unsigned char* row = stage + (cb >> 1) * BOX + i * 128;
+                            uint32_t q[8];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int chunk = ((cb & 1) * 4 + j) ^ (i & 7);
-                                Vec<bf16, true>::store(reinterpret_cast<bf16*>(row + chunk * 16), v + 8 * j);
+                            for (int j = 0; j < 8; ++j) q[j] = round2(o[j]);
+                            bf16* to = a.out + at + c0;
+                            if (wide) {
+                                store32(to, q);
+                            } else {
+                                *reinterpret_cast<uint4*>(to) = make_uint4(q[0], q[1], q[2], q[3]);
+                                if (c0 + 8 < dz) *reinterpret_cast<uint4*>(to + 8) = make_uint4(q[4], q[5], q[6], q[7]);
                             }
                         }
                     }
                     fence_before();
                     mbar_arrive(o_free);
-                    if (!a.out32) {
-                        fence_async_smem();
-                        if (!(ok = group_sync(sync_a, phase, fail))) break;
-                        if (tid == 0) {
-                            for (int j = 0; j * 64 < dz; ++j) tma_store4(&maps.out, stage + j * BOX, j * 64, t, it.h, it.b);
-                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        }
-                    } else if (!(ok = group_sync(sync_a, phase, fail))) {
-                        break;
-                    }
-                    if (tid == 0) mbar_arrive(x_empty + (int)(n & 1));
                 }
                 if (!ok) break;
                 // positions without a token beyond the last chunk
@@ -295,23 +325,22 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                     else a.out[at] = from_f<bf16>(0.f);
                 }
             }
-            if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
     } else {  // group B
-        float* pw = reinterpret_cast<float*>(sm + L::PWB);
         const int quarter = warp & 3, half = (warp - 6) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 192;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         long n = 0;
-        uint32_t phase = 0;
         bool ok = true;
         for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
             const Item it = place(w);
             if (skip(it)) continue;
-            if (!(ok = group_sync(sync_b, phase, fail))) break;
             const float rate = a.rate[it.h];
-            if (tid <= TC) pw[tid] = tid == 0 ? 1.f : expf(-rate * (float)tid);
-            if (!(ok = group_sync(sync_b, phase, fail))) break;
-            float s[64];
+            // a full chunk's weights of the four tokens that this thread weights, and of the carry
+            const float gfull = decay_of(rate, TC);
+            float wfull[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) wfull[k] = decay_of(rate, a.rev ? (tid >> 3) + 32 * k + 1 : TC - 1 - (tid >> 3) - 32 * k);
+            uint64_t s[32];
             const long per = (long)dx * dz;
             const float* init = nullptr;
             long ir = 0, ic = 0;
@@ -321,54 +350,65 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 else if (a.init) init = a.init + it.bh * per, ir = a.init_r, ic = a.init_c, scale = a.init_scale;
             }
 #pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                const int col = half * 64 + j;
-                s[j] = init && row < dx && col < dz ? init[row * ir + col * ic] * scale : 0.f;
+            for (int j = 0; j < 32; ++j) {
+                const int col = half * 64 + 2 * j;
+                float e[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) e[k] = init && row < dx && col + k < dz ? init[row * ir + (col + k) * ic] * scale : 0.f;
+                s[j] = pair(e[0], e[1]);
             }
+#pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++n) {
                 const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, m = min(TC, it.end - t);
-                const int st = (int)(n & 1), zs = STATE ? st : 0;
+                const int st = (int)(n & 1);
                 const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
                 if (!STATE) {
                     if (!(ok = __all_sync(kFull, mbar_wait(xs_done, ph ^ 1u, fail)))) break;
                     if (half * 64 < dz) {
                         unsigned char* p = sm + L::S + half * BOX + row * 128;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) Vec<bf16, true>::store(reinterpret_cast<bf16*>(p + ((j ^ (row & 7)) * 16)), s + 8 * j);
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<uint4*>(p + ((j ^ (row & 7)) * 16)) =
+                                make_uint4(round2(s[4 * j]), round2(s[4 * j + 1]), round2(s[4 * j + 2]), round2(s[4 * j + 3]));
                     }
                     fence_async_smem();
                     mbar_arrive(s_ready);
                 }
-                if (!(ok = __all_sync(kFull, mbar_wait(y_full + st, two, fail) && mbar_wait(z_full + zs, STATE ? two : ph, fail) &&
+                if (!(ok = __all_sync(kFull, mbar_wait(y_full + st, two, fail) && mbar_wait(z_full + (STATE ? st : 0), STATE ? two : ph, fail) &&
                                                  (STATE || mbar_wait(p_full, ph, fail)))))
                     break;
                 unsigned char* Y = sm + L::Y + st * TILE;
-                const int vecs = dx > 64 ? TILE / 16 : BOX / 16;
-                for (int e = tid; e < vecs; e += 256) {
-                    const int tok = (e >> 3) & (TC - 1);
-                    const float wt = tok < m ? pw[a.rev ? tok + 1 : m - 1 - tok] : 0.f;
-                    uint4* at = reinterpret_cast<uint4*>(Y + e * 16);
-                    const uint4 q = *at;
-                    const uint32_t in[4] = {q.x, q.y, q.z, q.w};
-                    uint32_t piece[NS][4];
+                const uint64_t minus_one = pair(-1.f, -1.f);
+                const int rounds = dx > 64 ? 2 : 1;
+#pragma unroll 1
+                for (int r = 0; r < rounds; ++r) {  // a box of 64 columns: 1,024 vectors of 16 bytes, four a thread
+                    uint4 q[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float f0 = tok < m ? bf16_lo(in[j]) * wt : 0.f, f1 = tok < m ? bf16_hi(in[j]) * wt : 0.f;
+                    for (int k = 0; k < 4; ++k) q[k] = *reinterpret_cast<const uint4*>(Y + r * BOX + (tid + 256 * k) * 16);
 #pragma unroll
-                        for (int p = 0; p < NS; ++p) {
-                            const uint32_t u = pack_bf16(f0, f1);
-                            piece[p][j] = u;
-                            f0 -= bf16_lo(u), f1 -= bf16_hi(u);
+                    for (int k = 0; k < 4; ++k) {
+                        const int e = tid + 256 * k, tok = e >> 3;
+                        const bool live = tok < m;
+                        const float wt = m == TC ? wfull[k] : decay_of(rate, a.rev ? tok + 1 : m - 1 - tok);
+                        const uint64_t wt2 = pair(wt, wt);
+                        const uint32_t in[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+                        uint32_t piece[NS][4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint64_t f = mul2(pair(bf16_lo(in[j]), bf16_hi(in[j])), wt2);
+                            if (!live) f = 0ull;
+#pragma unroll
+                            for (int p = 0; p < NS; ++p) piece[p][j] = p == NS - 1 ? round2(f) : round2(f, minus_one);
                         }
-                    }
-                    *at = make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]);
+                        *reinterpret_cast<uint4*>(Y + r * BOX + e * 16) = make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]);
 #pragma unroll
-                    for (int p = 1; p < NS; ++p)
-                        *reinterpret_cast<uint4*>(sm + L::LO + (p - 1) * TILE + e * 16) =
-                            make_uint4(piece[p][0], piece[p][1], piece[p][2], piece[p][3]);
+                        for (int p = 1; p < NS; ++p)
+                            *reinterpret_cast<uint4*>(sm + L::LO + (p - 1) * TILE + r * BOX + e * 16) =
+                                make_uint4(piece[p][0], piece[p][1], piece[p][2], piece[p][3]);
+                    }
                 }
                 if (m < TC) {  // a short chunk: rows of Z that are no tokens must not reach a product
-                    unsigned char* Z = sm + L::Z + zs * TILE;
+                    unsigned char* Z = sm + L::Z + (STATE ? st : 0) * TILE;
                     for (int e = tid; e < TILE / 16; e += 256)
                         if (((e >> 3) & (TC - 1)) >= m) *reinterpret_cast<uint4*>(Z + e * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -376,14 +416,15 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 mbar_arrive(yw_ready);
                 if (!(ok = __all_sync(kFull, mbar_wait(u_full, ph, fail)))) break;
                 fence_after();
-                const float gn = pw[m];
+                const float gn = m == TC ? gfull : decay_of(rate, m);
+                const uint64_t gn2 = pair(gn, gn);
                 if (half * 64 < dz) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         float v[32];
                         tmem_ld32(tmem + TU + lanes + half * 64 + q * 32, v);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) s[q * 32 + j] = fmaf(gn, s[q * 32 + j], v[j]);
+                        for (int j = 0; j < 16; ++j) s[q * 16 + j] = fma2(gn2, s[q * 16 + j], pair(v[2 * j], v[2 * j + 1]));
                     }
                 }
                 fence_before();
@@ -394,10 +435,17 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
             float fscale = 1.f;
             if (STATE) fin = a.seg + (it.bh * a.segs + it.seg) * per, fr = dz, fc = 1;
             else if (a.segs == 1 && a.fin) fin = a.fin + it.bh * per, fr = a.fin_r, fc = a.fin_c, fscale = a.fin_scale;
-            if (fin && row < dx)
+            if (fin && row < dx) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j)
-                    if (half * 64 + j < dz) fin[row * fr + (half * 64 + j) * fc] = s[j] * fscale;
+                for (int j = 0; j < 32; ++j) {
+                    const int col = half * 64 + 2 * j;
+                    float e[2];
+                    unpair(s[j], e[0], e[1]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (col + k < dz) fin[row * fr + (col + k) * fc] = e[k] * fscale;
+                }
+            }
         }
     }
     __syncthreads();
@@ -459,7 +507,7 @@ bool tc_fits(const Chain<bf16>& a) {
     const int batch = a.batch, steps = a.steps;
     return steps > 0 && a.z.width % 8 == 0 && mappable(a.x, steps, a.heads / a.x.group, batch) &&
            mappable(a.y, steps, a.heads / a.y.group, batch) && mappable(a.z, steps, a.heads / a.z.group, batch) &&
-           (a.out32 || aligned16(a.out));
+           (a.out32 ? aligned16(a.out32) : aligned16(a.out));
 }
 
 int tc_chain(const Chain<bf16>& a, bool state_only, bool exact, cudaStream_t s) {
@@ -470,9 +518,6 @@ int tc_chain(const Chain<bf16>& a, bool state_only, bool exact, cudaStream_t s) 
     if (!in(&m.y, a.y) || !in(&m.z, a.z)) return EWS_ERR_LAUNCH;
     if (state_only) return exact ? go<true, 3>(a, m, s) : go<true, 2>(a, m, s);
     if (!in(&m.x, a.x)) return EWS_ERR_LAUNCH;
-    const int dz = a.z.width;
-    if (!a.out32 && !map_of(&m.out, a.out, dz, a.steps, a.heads, a.batch, (long)a.heads * dz, dz, (long)a.steps * a.heads * dz))
-        return EWS_ERR_LAUNCH;
     return go<false, 2>(a, m, s);
 }
 

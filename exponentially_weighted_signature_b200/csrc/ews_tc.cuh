@@ -9,6 +9,8 @@
 namespace ews {
 namespace tc5 {
 
+using namespace token;
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
@@ -31,14 +33,36 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded: false when the wait ran out (the CTA's fail word is then set) or another role gave up before.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
+// One lane of a converged warp. The products' issue is written for the whole warp with this in front of each batch, not
+// for a lane of its own: the operands are then uniform values, where a divergent lane had to move each of them to
+// the uniform registers, about 100 cycles a product.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "elect.sync _|P, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
+}
+// Bounded: false when the wait ran out (the CTA's fail word is then set) or another role gave up before. The first
+// look is inline, the loop is not: a role's steps run once a chunk, and what they share of the instruction cache is
+// what bounds them.
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile int* fail) {
+#pragma unroll 1
     for (int it = 0; it < kDefaultSpinLimit; ++it) {
         if (mbar_try(bar, parity)) return true;
         if ((it & 63) == 63 && *fail) return false;
     }
     *fail = 1;
     return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
+    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, fail);
+}
+// The same for a converged warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
+    return __all_sync(kFull, mbar_wait(bar, parity, fail));
 }
 // After a failure: lets what is in flight land, as far as it does.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
@@ -82,24 +106,92 @@ __device__ __forceinline__ void mma_bf16(uint32_t tmem, uint64_t ad, uint64_t bd
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// The load and its wait are one statement: nothing may read the registers in between.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float v[32]) {
     uint32_t r[32];
     __syncwarp();
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-        "%28,%29,%30,%31}, [%32];"
+        "%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        : "r"(taddr)
+        : "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 
+// Pairs of floats: one instruction for two values (the epilogues are bound by their instructions).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t lds64(uint32_t a) {
+    uint64_t r;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(a));
+    return r;
+}
+// A pair rounded to bfloat16, and what the rounding left.
+__device__ __forceinline__ uint32_t round2(uint64_t p) {
+    float a, b;
+    unpair(p, a, b);
+    return pack_bf16(a, b);
+}
+__device__ __forceinline__ uint32_t round2(uint64_t& p, uint64_t minus_one) {
+    const uint32_t u = round2(p);
+    p = fma2(pair(bf16_lo(u), bf16_hi(u)), minus_one, p);
+    return u;
+}
+// The decays between a chunk's tokens as a table of pairs in shared memory: entry x (from -127 to 127) holds the weights of
+// a score x behind its row's token and of its right neighbour, (w(x), w(x - 1)), w(x) = g^x from 0 on (reversed: g^-x up
+// to 0), else zero. A row's 32 scores read 16 pairs at constant distances.
+constexpr int DECAY_BYTES = 255 * 8;
+__device__ __forceinline__ void put_decay(unsigned char* tab, int tid, int threads, float rate, bool rev) {
+    auto w = [&](int x) {
+        if (rev) x = -x;
+        return x < 0 ? 0.f : x == 0 ? 1.f : expf(-rate * (float)x);
+    };
+    for (int x = tid - 127; x <= 127; x += threads) *reinterpret_cast<float2*>(tab + (x + 127) * 8) = make_float2(w(x), w(x - 1));
+}
+__device__ __forceinline__ float decay_of(float rate, int n) { return n <= 0 ? 1.f : expf(-rate * (float)n); }
+
+// 32 bytes, a whole sector, from one lane.
+__device__ __forceinline__ void store32(void* p, const uint32_t r[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// Sixteen columns each from two places.
+__device__ __forceinline__ void tmem_ld16x2(uint32_t ta, uint32_t tb, uint32_t u[16], uint32_t v[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]),
+          "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15])
+        : "r"(ta), "r"(tb)
+        : "memory");
+}
 // A from tensor memory (two bfloat16 a column).
 __device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
     asm volatile(

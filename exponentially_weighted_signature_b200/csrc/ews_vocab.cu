@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     uint64_t* drained = acc_empty + 2;
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
     const long units = a.job[0].units + (EPI == OUT ? a.job[1].units : 0);
 
     struct Unit {
@@ -161,36 +161,44 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 for (long j = it > S ? it - S : 0; j < it; ++j) mbar_drain(full + j % S, (uint32_t)((j / S) & 1));
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            long it = 0, tile = 0;
-            bool ok = true;
-            for (long u = blockIdx.x; ok && u < units; u += gridDim.x, ++tile) {
-                const Unit r = unit(u);
-                const bool amn = EPI == OUT && r.job == 1;
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((amn ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
-                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-                const uint32_t astep = amn ? 2048 >> 4 : 32 >> 4, bstep = BMN ? 2048 >> 4 : 32 >> 4;
-                const int buf = (int)(tile & 1);
-                if (!(ok = mbar_wait(acc_empty + buf, (uint32_t)((tile >> 1) & 1) ^ 1u, fail))) break;
+        int s = 0;
+        uint32_t ph = 0;
+        long tile = 0;
+        bool ok = true;
+        for (long u = blockIdx.x; ok && u < units; u += gridDim.x, ++tile) {
+            const Unit r = unit(u);
+            const bool amn = EPI == OUT && r.job == 1;
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((amn ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
+                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            const uint32_t astep = amn ? 2048 >> 4 : 32 >> 4, bstep = BMN ? 2048 >> 4 : 32 >> 4;
+            const int buf = (int)(tile & 1);
+            if (!(ok = warp_wait(acc_empty + buf, (uint32_t)((tile >> 1) & 1) ^ 1u, fail))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int steps = a.pairs * max(r.k1 - r.k0, 0);
+            const uint64_t ad0 = desc(smem_u32(tiles), amn), bd0 = desc(smem_u32(tiles) + TL::A, BMN);
+            for (int i = 0; i < steps; ++i) {
+                if (!(ok = warp_wait(full + s, ph, fail))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const long steps = (long)a.pairs * max(r.k1 - r.k0, 0);
-                for (long i = 0; i < steps; ++i, ++it) {
-                    const int s = (int)(it % S);
-                    if (!(ok = mbar_wait(full + s, (uint32_t)((it / S) & 1), fail))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = smem_u32(tiles + s * TL::STAGE);
-                    const uint64_t ad = desc(at, amn), bd = desc(at + TL::A, BMN);
+                if (elect_one()) {
+                    const uint64_t ad = ad0 + s * (TL::STAGE >> 4), bd = bd0 + s * (TL::STAGE >> 4);
 #pragma unroll
                     for (int q = 0; q < BK / 16; ++q)
                         mma_bf16(tmem + buf * BN, ad + q * astep, bd + q * bstep, idesc, i > 0 || q > 0);
                     mma_commit(empty + s);
+                    if (i == steps - 1) mma_commit(acc_full + buf);
                 }
-                if (ok) mma_commit(acc_full + buf);
+                __syncwarp();
+                if (++s == S) s = 0, ph ^= 1u;
             }
-            if (!ok) {
-                mma_commit(drained);
-                mbar_drain(drained, 0);
+            if (ok && steps == 0) {
+                if (elect_one()) mma_commit(acc_full + buf);
+                __syncwarp();
             }
+        }
+        if (!ok) {
+            if (elect_one()) mma_commit(drained);
+            __syncwarp();
+            mbar_drain(drained, 0);
         }
     } else {
         // two warps share a quarter of the rows, each has half of the tile's columns
