@@ -438,11 +438,15 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chain
     const long span = a.span;
     const float rate = a.rate[h];
     float s = a.init ? a.init[bh * per + i * a.init_r + j * a.init_c] * a.init_scale : 0.f;
-    for (int k = 0; k < a.segs; ++k) {
-        const int g = a.down ? a.segs - 1 - k : k;
-        float* p = a.seg + (bh * a.segs + g) * per + i * dz + j;
-        const float own = *p;
+    float* p = a.seg + bh * a.segs * per + i * dz + j;
+    const long step = a.down ? -per : per;
+    p += a.down ? (a.segs - 1) * per : 0;
+    float next = *p;
+    for (int k = 0; k < a.segs; ++k, p += step) {
+        const float own = next;
+        if (k + 1 < a.segs) next = p[step];  // on its way while this one is chained
         *p = s;
+        const int g = a.down ? a.segs - 1 - k : k;
         const long n = min(max(len - g * span, 0l), span);
         if (n > 0) s = fmaf(expf(-rate * (float)n), s, own);
     }

@@ -34,9 +34,9 @@ struct Place {
 
 __device__ __forceinline__ void prefetch_l2(const float* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// Up to four values of a row that 16-byte loads cannot read.
-__device__ __noinline__ float4 load_ragged(const float* p, int left) {
-    return make_float4(p[0], left > 1 ? p[1] : 0.f, left > 2 ? p[2] : 0.f, left > 3 ? p[3] : 0.f);
+// Up to four values, from column `col` on, of a row that 16-byte loads cannot read.
+__device__ __noinline__ float4 load_ragged(const float* row, int col, int left) {
+    return make_float4(left > 0 ? row[col] : 0.f, left > 1 ? row[col + 1] : 0.f, left > 2 ? row[col + 2] : 0.f, left > 3 ? row[col + 3] : 0.f);
 }
 
 // Four neighbouring values into the three planes of a tile, at (row, 4 col4).
@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
             const uint32_t nz = (uint32_t)((it.dz + 15) / 16 * 2) << 17;
             for (int c = 0; ok && c < it.chunks; ++c, ++n) {
                 const uint32_t ph = (uint32_t)(n & 1);
+                const int ksteps = (min(FC, it.end - chunk_at(it, c)) + 15) / 16;  // the tokens' steps: the rest holds none
                 if (!(ok = warp_wait(xy_ready, ph, fail))) break;
                 fence_after();
                 if (!STATE) {
@@ -145,8 +146,8 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
 #pragma unroll 1
                     for (int p = 0; p < 6; ++p) {
                         const uint64_t da = dW + ((PA >> (4 * p)) & 3) * (PLANE / 16), db = dZ + ((PB >> (4 * p)) & 3) * (PLANE / 16);
-#pragma unroll
-                        for (int q = 0; q < FC / 16; ++q) mma_bf16(tmem + TU, da + q * 128, db + q * 128, base | amn | bmn | nz, p > 0 || q > 0);
+#pragma unroll 2
+                        for (int q = 0; q < ksteps; ++q) mma_bf16(tmem + TU, da + q * 128, db + q * 128, base | amn | bmn | nz, p > 0 || q > 0);
                     }
                     mma_commit(u_full);
                 }
@@ -159,8 +160,8 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                         for (int p = 0; p < 6; ++p) {
                             const uint32_t ta = tmem + TPP + ((PA >> (4 * p)) & 3) * 64;
                             const uint64_t db = dZ + ((PB >> (4 * p)) & 3) * (PLANE / 16);
-#pragma unroll
-                            for (int q = 0; q < FC / 16; ++q) mma_bf16_ta(tmem + TO2, ta + q * 8, db + q * 128, base | bmn | nz, p > 0 || q > 0);
+#pragma unroll 2
+                            for (int q = 0; q < ksteps; ++q) mma_bf16_ta(tmem + TO2, ta + q * 8, db + q * 128, base | bmn | nz, p > 0 || q > 0);
                         }
                         mma_commit(o_full);
                     }
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                     if (!(ok = __all_sync(kFull, mbar_wait(p_full, ph, fail)))) break;
                     fence_after();
 #pragma unroll 1
-                    for (int cb = 0; cb < 4; ++cb) {
+                    for (int cb = 0; cb * 32 < m; ++cb) {
                         uint64_t v[16];
                         if (a.rev ? cb >= quarter : cb <= quarter) {
                             float e[32];
@@ -300,14 +301,20 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
             }
             if (keeper) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float e[2];
+                for (int j = 0; j < 16; ++j) s[j] = 0ull;
+                if (init) {
+                    const float* from = init + min(row, dx - 1) * ir;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int col = half * 32 + 2 * j + k;
-                        e[k] = init && row < dx && col < it.dz ? init[row * ir + (it.c0 + col) * ic] * scale : 0.f;
+                    for (int j = 0; j < 16; ++j) {
+                        float e[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {  // from places that exist, all in flight at once
+                            const int col = half * 32 + 2 * j + k;
+                            e[k] = from[(it.c0 + min(col, it.dz - 1)) * ic] * scale;
+                            if (row >= dx || col >= it.dz) e[k] = 0.f;
+                        }
+                        s[j] = pair(e[0], e[1]);
                     }
-                    s[j] = pair(e[0], e[1]);
                 }
             }
             for (int c = 0; c < it.chunks; ++c, ++n) {
@@ -326,15 +333,16 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                     const float* p = part == 0 ? yb : part == 1 ? xb : zb;
                     const int col = (part == 2 ? it.c0 : 0) + (tid & 15) * 4, left = st.width - col;
                     float4 v[8];
+                    // every load is issued, from a row and a column that exist, and what does not count is dropped after: under
+                    // a condition each, the loads would come one by one
+                    if (st.vec) {
+                        const float* from = p + (left > 0 ? col : 0);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int r = (tid >> 4) + 16 * k;
-                        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (r < m && left > 0) {
-                            const float* at = p + (long)(t + r) * st.st + col;
-                            if (st.vec) v[k] = __ldg(reinterpret_cast<const float4*>(at));
-                            else v[k] = load_ragged(at, left);
-                        }
+                        for (int k = 0; k < 8; ++k)
+                            v[k] = __ldg(reinterpret_cast<const float4*>(from + (long)(t + min((tid >> 4) + 16 * k, m - 1)) * st.st));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = load_ragged(p + (long)(t + min((tid >> 4) + 16 * k, m - 1)) * st.st, col, left);
                     }
                     if (part == 2) {
                         if (!STATE && !(ok = __all_sync(kFull, mbar_wait(o_full, ph ^ 1u, fail)))) break;
@@ -343,10 +351,12 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int r = (tid >> 4) + 16 * k;
-                        const uint64_t lo = pair(v[k].x, v[k].y), hi = pair(v[k].z, v[k].w);
+                        if (16 * k >= m) continue;
+                        uint64_t lo = pair(v[k].x, v[k].y), hi = pair(v[k].z, v[k].w);
+                        if (r >= m || left <= 0) lo = hi = 0ull;
                         if (!(STATE && part == 0)) put4(tile, PLANE, r, tid & 15, lo, hi);
                         if (part == 0) {
-                            const float wt = decay_of(rate, a.rev ? r + 1 : m - 1 - r);  // a row that is no token is zero
+                            const float wt = decay_of(rate, a.rev ? r + 1 : m - 1 - r);
                             const uint64_t wt2 = pair(wt, wt);
                             put4(sm + LW, PLANE, r, tid & 15, mul2(lo, wt2), mul2(hi, wt2));
                         }

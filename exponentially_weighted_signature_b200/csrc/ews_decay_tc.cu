@@ -350,18 +350,32 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 else if (a.init) init = a.init + it.bh * per, ir = a.init_r, ic = a.init_c, scale = a.init_scale;
             }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const int col = half * 64 + 2 * j;
-                float e[2];
+            for (int j = 0; j < 32; ++j) s[j] = 0ull;
+            if (init) {
+                const float* from = init + min(row, dx - 1) * ir;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) e[k] = init && row < dx && col + k < dz ? init[row * ir + (col + k) * ic] * scale : 0.f;
-                s[j] = pair(e[0], e[1]);
+                for (int j = 0; j < 32; ++j) {
+                    float e[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {  // from places that exist, all in flight at once
+                        const int col = half * 64 + 2 * j + k;
+                        e[k] = from[min(col, dz - 1) * ic] * scale;
+                        if (row >= dx || col >= dz) e[k] = 0.f;
+                    }
+                    s[j] = pair(e[0], e[1]);
+                }
             }
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++n) {
                 const int t = it.t0 + (a.rev ? it.chunks - 1 - c : c) * TC, m = min(TC, it.end - t);
                 const int st = (int)(n & 1);
                 const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
+                if (m < TC) {  // a short chunk: rows of Z that are no tokens must not reach a product, the first of which follows O1
+                    if (!(ok = __all_sync(kFull, mbar_wait(z_full + (STATE ? st : 0), STATE ? two : ph, fail)))) break;
+                    unsigned char* Z = sm + L::Z + (STATE ? st : 0) * TILE;
+                    for (int e = tid; e < TILE / 16; e += 256)
+                        if (((e >> 3) & (TC - 1)) >= m) *reinterpret_cast<uint4*>(Z + e * 16) = make_uint4(0, 0, 0, 0);
+                }
                 if (!STATE) {
                     if (!(ok = __all_sync(kFull, mbar_wait(xs_done, ph ^ 1u, fail)))) break;
                     if (half * 64 < dz) {
@@ -406,11 +420,6 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                             *reinterpret_cast<uint4*>(sm + L::LO + (p - 1) * TILE + r * BOX + e * 16) =
                                 make_uint4(piece[p][0], piece[p][1], piece[p][2], piece[p][3]);
                     }
-                }
-                if (m < TC) {  // a short chunk: rows of Z that are no tokens must not reach a product
-                    unsigned char* Z = sm + L::Z + (STATE ? st : 0) * TILE;
-                    for (int e = tid; e < TILE / 16; e += 256)
-                        if (((e >> 3) & (TC - 1)) >= m) *reinterpret_cast<uint4*>(Z + e * 16) = make_uint4(0, 0, 0, 0);
                 }
                 fence_async_smem();
                 mbar_arrive(yw_ready);
