@@ -468,10 +468,10 @@ __global__ void __launch_bounds__(256) group_kernel(const float* __restrict__ in
 }
 
 // ---- one token per row ----------------------------------------------------------------------------------------
-// A CTA owns 32 columns of one (row, head) state: 8 lanes of four columns by 32 groups of state rows; each thread
+// A CTA owns 64 columns of one (row, head) state: 16 lanes of four columns by 16 groups of state rows; each thread
 // reads, decays, updates and writes its part of the state once and sums its rows of q S; the groups' sums meet in
 // shared memory. Bound by HBM (8 bytes a state entry) for full batches and by one trip to memory for few rows.
-constexpr int STEP_T = 256, STEP_COLS = 32;
+constexpr int STEP_T = 256, STEP_COLS = 64;
 
 template <typename T>
 struct Step {

@@ -7,7 +7,7 @@
 // Gradient: the ids are sorted (stably, so every sum has one order and the result is bit-reproducible; no
 // float atomics), then every row of the table is written exactly once: zero where its token does not occur,
 // else the float32 sum of its rows, rounded once. Three launches:
-//   sort_kernel     least-significant-digit radix sort of (id, position), up to 8 bits a pass, in ONE cluster of
+//   sort_kernel     least-significant-digit radix sort of (id, position), up to 9 bits a pass, in ONE cluster of
 //                   eight CTAs: the passes' steps are separated by the cluster's hardware barrier, where a
 //                   grid-wide sort would pay three launches a pass. It also marks each token's run.
 //   partial_kernel  natural tokens are skewed: one row may take a tenth of all positions. The sorted axis is cut
@@ -26,7 +26,7 @@ using namespace token;
 constexpr int ST = 1024;   // threads of a sort CTA
 constexpr int SW = ST / 32;
 constexpr int SCL = 8;     // CTAs of the sort's cluster
-constexpr int SBITS = 8;   // most bits of a digit
+constexpr int SBITS = 9;   // most bits of a digit: two passes for vocabularies below 2^18
 constexpr int SD = 1 << SBITS;
 constexpr int SI = 8;      // items of a lane that are in flight together
 constexpr int RROWS = 4;   // table rows of one warp
@@ -78,22 +78,28 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // Stable: the CTAs, their warps and a warp's rounds of 32 items take the items in order, a lane's rank within a
-// round counts the lower lanes of the same digit.
+// round counts the lower lanes of the same digit. A warp whose items fit its registers (up to 65,536 in all) reads
+// them once a pass.
 __global__ void __launch_bounds__(ST) sort_kernel(SortArgs a, int ctas) {
-    __shared__ uint32_t hist[SW][SD];
-    __shared__ uint32_t base[SD];
+    extern __shared__ uint32_t shared[];
+    uint32_t* hist = shared;                 // SW x digits
+    uint32_t* base = hist + SW * SD;         // digits
+    uint32_t* group = base + SD;             // 4 x digits / 2: sums over groups of warps
     __shared__ uint32_t warp_tot[SW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
     for (long r = (long)cta * ST + tid; r < a.vocab; r += (long)ctas * ST) a.runs[r] = make_int2(0, 0);
     const int per_warp = ((a.n + ctas * SW - 1) / (ctas * SW) + 31) / 32 * 32;
     const long first = (long)(cta * SW + warp) * per_warp;
     const long last = first + per_warp < a.n ? first + per_warp : a.n;
+    const bool held = per_warp <= 32 * SI;
     const uint32_t *kin = a.key0, *pin = a.pos0;
     uint32_t *kout = a.key1, *pout = a.pos1;
+    const int digits = 1 << a.bits;
+    const uint32_t mask = digits - 1;
+    uint32_t* mine = hist + warp * digits;
     for (int p = 0; p < a.passes; ++p) {
-        const int shift = p * a.bits, digits = 1 << a.bits;
-        const uint32_t mask = digits - 1;
-        for (int d = lane; d < digits; d += 32) hist[warp][d] = 0;
+        const int shift = p * a.bits;
+        for (int d = lane; d < digits; d += 32) mine[d] = 0;
         __syncwarp();
         auto key_of = [&](long i) -> uint32_t {
             if (p > 0) return __ldcg(kin + i);
@@ -104,35 +110,55 @@ __global__ void __launch_bounds__(ST) sort_kernel(SortArgs a, int ctas) {
             }
             return id == a.skip ? (uint32_t)a.vocab : (uint32_t)id;
         };
-        for (long i0 = first; i0 < last; i0 += 32 * SI) {
-            uint32_t key[SI];
+        uint32_t key[SI], pos[SI];
+        auto load = [&](long i0) {
 #pragma unroll
             for (int k = 0; k < SI; ++k) {
                 const long i = i0 + 32 * k + lane;
                 key[k] = i < last ? key_of(i) : 0u;
+                pos[k] = i < last ? (p > 0 ? __ldcg(pin + i) : (uint32_t)i) : 0u;
             }
+        };
+        for (long i0 = first; i0 < last; i0 += 32 * SI) {
+            load(i0);
 #pragma unroll
             for (int k = 0; k < SI; ++k)
-                if (i0 + 32 * k + lane < last) atomicAdd(&hist[warp][(key[k] >> shift) & mask], 1u);
+                if (i0 + 32 * k + lane < last) atomicAdd(&mine[(key[k] >> shift) & mask], 1u);
         }
         __syncthreads();
-        uint32_t mine = 0;
-        if (tid < digits) {
-            for (int w = 0; w < SW; ++w) {
-                const uint32_t c = hist[w][tid];
-                hist[w][tid] = mine;
-                mine += c;
+        // over the warps, exclusively, for each digit: two halves of the CTA take half of the warps each
+        const int d = tid & (digits - 1), part = tid / digits, parts = ST / digits < 4 ? ST / digits : 4, span = SW / parts;
+        uint32_t sum = 0;
+        if (part < parts) {
+            for (int w = part * span; w < (part + 1) * span; ++w) {
+                const uint32_t c = hist[w * digits + d];
+                hist[w * digits + d] = sum;
+                sum += c;
             }
-            __stcg(a.totals + cta * SD + tid, mine);
+            group[part * digits + d] = sum;
+        }
+        __syncthreads();
+        if (part < parts) {
+            uint32_t before = 0, all = 0;
+            for (int g = 0; g < parts; ++g) {
+                if (g == part) before = all;
+                all += group[g * digits + d];
+            }
+            if (before)
+                for (int w = part * span; w < (part + 1) * span; ++w) hist[w * digits + d] += before;
+            if (part == 0) __stcg(a.totals + cta * SD + d, all);
         }
         cluster_sync();
         // the digit's base: all lower digits everywhere, and this digit in the lower CTAs
         uint32_t before = 0, all = 0;
         if (tid < digits) {
-            for (int c = 0; c < ctas; ++c) {
-                const uint32_t t = __ldcg(a.totals + c * SD + tid);
-                all += t;
-                if (c < cta) before += t;
+            uint32_t t[SCL];
+#pragma unroll
+            for (int c = 0; c < SCL; ++c) t[c] = c < ctas ? __ldcg(a.totals + c * SD + tid) : 0u;
+#pragma unroll
+            for (int c = 0; c < SCL; ++c) {
+                all += t[c];
+                if (c < cta) before += t[c];
             }
         }
         uint32_t incl = all;
@@ -149,26 +175,20 @@ __global__ void __launch_bounds__(ST) sort_kernel(SortArgs a, int ctas) {
             base[tid] = s;
         }
         __syncthreads();
-        for (int d = lane; d < digits; d += 32) hist[warp][d] += base[d];
+        for (int e = lane; e < digits; e += 32) mine[e] += base[e];
         __syncwarp();
         for (long i0 = first; i0 < last; i0 += 32 * SI) {
-            uint32_t key[SI], pos[SI];
-#pragma unroll
-            for (int k = 0; k < SI; ++k) {
-                const long i = i0 + 32 * k + lane;
-                key[k] = i < last ? key_of(i) : 0xFFFFFFFFu;
-                pos[k] = i < last ? (p > 0 ? __ldcg(pin + i) : (uint32_t)i) : 0u;
-            }
+            if (!held) load(i0);
 #pragma unroll
             for (int k = 0; k < SI; ++k) {
                 const bool in = i0 + 32 * k + lane < last;
-                const uint32_t d = in ? (key[k] >> shift) & mask : 0xFFFFFFFFu;
-                const uint32_t same = __match_any_sync(kFull, d);
+                const uint32_t dg = in ? (key[k] >> shift) & mask : 0xFFFFFFFFu;
+                const uint32_t same = __match_any_sync(kFull, dg);
                 const int rank = __popc(same & ((1u << lane) - 1u));
                 uint32_t at = 0;
-                if (in) at = hist[warp][d];
+                if (in) at = mine[dg];
                 __syncwarp();
-                if (in && rank == 0) hist[warp][d] = at + __popc(same);
+                if (in && rank == 0) mine[dg] = at + __popc(same);
                 __syncwarp();
                 if (in) {
                     __stcg(kout + at + rank, key[k]);
@@ -183,36 +203,48 @@ __global__ void __launch_bounds__(ST) sort_kernel(SortArgs a, int ctas) {
     }
     for (long i = (long)cta * ST + tid; i < a.n; i += (long)ctas * ST) {
         const uint32_t k = __ldcg(kin + i);
+        const uint32_t before = i > 0 ? __ldcg(kin + i - 1) : 0xFFFFFFFFu, after = i < a.n - 1 ? __ldcg(kin + i + 1) : 0xFFFFFFFFu;
         if (k >= a.vocab) continue;
-        if (i == 0 || __ldcg(kin + i - 1) != k) a.runs[k].x = (int)i;
-        if (i == a.n - 1 || __ldcg(kin + i + 1) != k) a.runs[k].y = (int)i + 1;
+        if (before != k) a.runs[k].x = (int)i;
+        if (after != k) a.runs[k].y = (int)i + 1;
     }
 }
+constexpr size_t SORT_BYTES = sizeof(uint32_t) * (SW * SD + SD + 4 * SD);
 
-// Sum of the rows at sorted positions [from, to), one vector of columns per lane, in order.
+// Sum of the rows at sorted positions [from, to), one vector of columns per lane, in order; eight rows in flight.
 template <typename T, bool VEC>
 __device__ __forceinline__ void sum_rows(const T* __restrict__ dout, long stride, const uint32_t* __restrict__ pos, int from,
                                          int to, int col, bool live, float acc[Vec<T, VEC>::N]) {
-    constexpr int W = Vec<T, VEC>::N;
-    constexpr int U = 4;  // rows in flight
+    constexpr int W = Vec<T, VEC>::N, U = 8;
     const int lane = threadIdx.x & 31;
+    if (!live) col = 0;  // a lane beyond the width reads what another one reads
     for (int s = from; s < to; s += 32) {
         const int m = min(32, to - s);
-        const uint32_t mine = lane < m ? __ldg(pos + s + lane) : 0u;
+        const uint32_t mine = __ldg(pos + s + min(lane, m - 1));
         for (int j = 0; j < m; j += U) {
-            float v[U][W];
+            const T* at[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const long r = __shfl_sync(kFull, mine, (j + u) & 31);
-                if (live && j + u < m) Vec<T, VEC>::load(dout + r * stride + col, v[u]);
-                else
+            for (int u = 0; u < U; ++u) at[u] = dout + (long)__shfl_sync(kFull, mine, min(j + u, m - 1)) * stride + col;
+            if (VEC) {
+                uint4 raw[U];
 #pragma unroll
-                    for (int k = 0; k < W; ++k) v[u][k] = 0.f;
+                for (int u = 0; u < U; ++u) raw[u] = __ldg(reinterpret_cast<const uint4*>(at[u]));
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (j + u < m) {
+                        float v[W];
+                        Vec<T, VEC>::load(reinterpret_cast<const T*>(&raw[u]), v);
+#pragma unroll
+                        for (int k = 0; k < W; ++k) acc[k] += v[k];
+                    }
+            } else {
+                float v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = to_f(*at[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (j + u < m) acc[0] += v[u];
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int k = 0; k < W; ++k) acc[k] += v[u][k];
         }
     }
 }
@@ -281,6 +313,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const T* __restrict__ dout, l
                 const float* p = part + ((long)s0 * 2 + 1) * dim + col;
 #pragma unroll
                 for (int j = 0; j < W; ++j) acc[j] = p[j];
+#pragma unroll 4
                 for (int s = s0 + 1; s <= s1; ++s) {
                     p = part + (long)s * 2 * dim + col;
 #pragma unroll
@@ -296,10 +329,10 @@ __global__ void __launch_bounds__(128) rows_kernel(const T* __restrict__ dout, l
     }
 }
 
-// Segment length: 64 positions, and at least a quarter of sqrt(n), so that neither a segment nor the partials of
+// Segment length: 32 positions, and at least a quarter of sqrt(n), so that neither a segment nor the partials of
 // one run make a long chain.
 int seg_of(long n) {
-    int seg = 64;
+    int seg = 32;
     while ((long)seg * seg * 16 < n) seg <<= 1;
     return seg;
 }
@@ -331,7 +364,8 @@ int backward(const SortArgs& sa, int ctas, const T* dout, long stride, int dim, 
     constexpr int W = Vec<T, VEC>::N;
     if (sa.n > 0) {
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(ST), cfg.stream = s;
+        if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SORT_BYTES) != cudaSuccess) return EWS_ERR_LAUNCH;
+        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(ST), cfg.stream = s, cfg.dynamicSmemBytes = SORT_BYTES;
         cudaLaunchAttribute at{};
         at.id = cudaLaunchAttributeClusterDimension;
         at.val.clusterDim.x = ctas, at.val.clusterDim.y = at.val.clusterDim.z = 1;
