@@ -9,8 +9,9 @@ from . import params, series
 from .layer import COMBINE_KINDS, EWS, BToSignature, LogEWS, configure
 from .logsig import log_level_sizes, log_signature_dim
 from .params import AParamBlockDiag, AParamConstant, AParamDiag, AParamEFM, AParamGeneral, AParamJordanRepeated, B
-from .token_ops import decayed_attention, decayed_attention_step, token_embedding, vocab_loss
 from .series import check_series_q, series_error_bound, suggest_series_q
+from .token_model import DecayBlock, TokenModel
+from .token_ops import decayed_attention, decayed_attention_step, token_embedding, vocab_loss
 
 __all__ = [
     "COMBINE_KINDS",
@@ -28,6 +29,8 @@ __all__ = [
     "check_series_q",
     "series_error_bound",
     "suggest_series_q",
+    "DecayBlock",
+    "TokenModel",
     "decayed_attention",
     "decayed_attention_step",
     "token_embedding",
