@@ -11,7 +11,7 @@
 // beside it: the weighted operand is inexact, two bfloat16 pieces carry it to 2^-16, three to 2^-24), write the
 // output of the chunk before, keep the state and write its bfloat16 copy. The only chain from chunk to chunk is
 // U -> State -> O1; the loads, P and the output of neighbouring chunks run beside it.
-// X and Y, which a chunk needs first, have two buffers, Z (with the state's passes of their own: two) one.
+// X, whose last product of a chunk (O1) is issued a chunk ahead, has one buffer, Y and Z two.
 // Why 128 tokens: the accumulator has 128 rows; the waste of the upper half of P is 1/10 of a chunk's products.
 //
 // Reversed chains keep the rows' order and walk the chunks down: decays are then g^(j-i) for j >= i, a row's weight of
@@ -38,11 +38,12 @@ struct Maps {
 
 template <bool STATE, int NS>
 struct Lay {
-    static constexpr int X = 0, Y = X + (STATE ? 0 : 2 * TILE), Z = Y + 2 * TILE, S = Z + (STATE ? 2 : 1) * TILE, LO = S + (STATE ? 0 : TILE),
+    static constexpr int X = 0, Y = X + (STATE ? 0 : TILE), Z = Y + 2 * TILE, S = Z + 2 * TILE, LO = S + (STATE ? 0 : TILE),
                          BARS = LO + (NS - 1) * TILE, TAB = BARS + 256, END = TAB + DECAY_BYTES;
     static constexpr size_t bytes = END;
 };
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 __device__ __forceinline__ void tma_load4(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int t, int h, int b) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
@@ -83,6 +84,10 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
         mbar_init(sync_a, 128);
         *fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 0) {  // the maps on their way before their first use
+        prefetch_map(&maps.y), prefetch_map(&maps.z);
+        if (!STATE) prefetch_map(&maps.x);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "r"(512));
@@ -125,24 +130,23 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                     for (int j = 0; j < bx; ++j)
                         tma_load4(&maps.y, y_full + s, sm + L::Y + s * TILE + j * BOX, j * 64, t, it.h / a.y.group, it.b);
                     if (!STATE) {
-                        if (!(ok = mbar_wait(x_empty + s, two, fail))) break;
-                        mbar_expect(x_full + s, bx * BOX);
+                        if (!(ok = mbar_wait(x_empty, (uint32_t)(n & 1) ^ 1u, fail))) break;
+                        mbar_expect(x_full, bx * BOX);
                         for (int j = 0; j < bx; ++j)
-                            tma_load4(&maps.x, x_full + s, sm + L::X + s * TILE + j * BOX, j * 64, t, it.h / a.x.group, it.b);
+                            tma_load4(&maps.x, x_full, sm + L::X + j * BOX, j * 64, t, it.h / a.x.group, it.b);
                     }
-                    const int zs = STATE ? s : 0;
-                    if (!(ok = mbar_wait(z_empty + zs, STATE ? two : (uint32_t)(n & 1) ^ 1u, fail))) break;
-                    mbar_expect(z_full + zs, bz * BOX);
+                    if (!(ok = mbar_wait(z_empty + s, two, fail))) break;
+                    mbar_expect(z_full + s, bz * BOX);
                     for (int j = 0; j < bz; ++j)
-                        tma_load4(&maps.z, z_full + zs, sm + L::Z + zs * TILE + j * BOX, j * 64, t, it.h / a.z.group, it.b);
+                        tma_load4(&maps.z, z_full + s, sm + L::Z + s * TILE + j * BOX, j * 64, t, it.h / a.z.group, it.b);
                 }
             }
             if (!ok) {  // what was asked for lands before the CTA leaves: at most the last two chunks' loads
                 for (long j = n > 1 ? n - 2 : 0; j <= n; ++j) {
                     const uint32_t two = (uint32_t)((j >> 1) & 1);
                     mbar_drain(y_full + (j & 1), two);
-                    if (!STATE) mbar_drain(x_full + (j & 1), two);
-                    mbar_drain(z_full + (STATE ? (j & 1) : 0), STATE ? two : (uint32_t)(j & 1));
+                    if (!STATE) mbar_drain(x_full, (uint32_t)(j & 1));
+                    mbar_drain(z_full + (j & 1), two);
                 }
             }
         }
@@ -162,10 +166,10 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
         auto scores = [&](long n) {  // P of chunk n
             const int s = (int)(n & 1);
             const uint32_t two = (uint32_t)((n >> 1) & 1);
-            if (!(warp_wait(x_full + s, two, fail) && warp_wait(y_full + s, two, fail))) return false;
+            if (!(warp_wait(x_full, (uint32_t)(n & 1), fail) && warp_wait(y_full + s, two, fail))) return false;
             fence_after();
             if (elect_one()) {
-                const uint64_t dX = desc(smem_u32(sm + L::X + s * TILE), false), dY = desc(smem_u32(sm + L::Y + s * TILE), false);
+                const uint64_t dX = desc(smem_u32(sm + L::X), false), dY = desc(smem_u32(sm + L::Y + s * TILE), false);
                 for (int q = 0; q < kx; ++q) {
                     const int off = (q >> 2) * (BOX >> 4) + (q & 3) * 2;
                     mma_bf16(tmem + TP, dX + off, dY + off, base | np, q > 0);
@@ -176,28 +180,27 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
             return true;
         };
         auto carried = [&](long n) {  // O1 of chunk n
-            const int s = (int)(n & 1);
             const uint32_t ph = (uint32_t)(n & 1);
             if (!(warp_wait(s_ready, ph, fail) && warp_wait(o_free, ph ^ 1u, fail))) return false;
             fence_after();
             if (elect_one()) {
-                const uint64_t dX = desc(smem_u32(sm + L::X + s * TILE), false);
+                const uint64_t dX = desc(smem_u32(sm + L::X), false);
                 for (int q = 0; q < kx; ++q)
                     mma_bf16(tmem + TO1, dX + (q >> 2) * (BOX >> 4) + (q & 3) * 2, dS + q * 128, base | bmn | nz, q > 0);
                 mma_commit(xs_done);
-                mma_commit(x_empty + s);
+                mma_commit(x_empty);
             }
             __syncwarp();
             return true;
         };
-        // In the order in which the others' parts come free: this chunk's scores are an operand first, so O2, then the
-        // next chunk's P for group A, then U for group B's state, then the next chunk's O1 from it.
+        // In the order in which the others' parts come free: O2 for group A's output, U for group B's state, then, while
+        // they work, the next chunk's P, and O1 from the new state.
         bool ok = STATE || total == 0 || (scores(0) && carried(0));
         for (long n = 0; ok && n < total; ++n) {
             const int s = (int)(n & 1);
             const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
-            const uint64_t dYw = desc(smem_u32(sm + L::Y + s * TILE), true, BOX), dZ = desc(smem_u32(sm + L::Z + (STATE ? s : 0) * TILE), true, BOX);
-            if (!(ok = warp_wait(z_full + (STATE ? s : 0), STATE ? two : ph, fail))) break;
+            const uint64_t dYw = desc(smem_u32(sm + L::Y + s * TILE), true, BOX), dZ = desc(smem_u32(sm + L::Z + s * TILE), true, BOX);
+            if (!(ok = warp_wait(z_full + s, two, fail))) break;
             if (!STATE) {
                 if (!(ok = warp_wait(p_ready, ph, fail))) break;
                 fence_after();
@@ -208,7 +211,6 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                     mma_commit(o_full);
                 }
                 __syncwarp();
-                if (n + 1 < total && !(ok = scores(n + 1))) break;
             }
             if (!(ok = warp_wait(yw_ready, ph, fail))) break;
             fence_after();
@@ -222,10 +224,10 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 }
                 mma_commit(u_full);
                 mma_commit(y_empty + s);
-                mma_commit(z_empty + (STATE ? s : 0));
+                mma_commit(z_empty + s);
             }
             __syncwarp();
-            if (!STATE && n + 1 < total) ok = carried(n + 1);
+            if (!STATE && n + 1 < total) ok = scores(n + 1) && carried(n + 1);
         }
         if (!ok) {
             if (elect_one()) mma_commit(drained);
@@ -284,32 +286,36 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                     const uint64_t wi2 = pair(wi, wi), os2 = pair(a.oscale, a.oscale);
                     const long at = (((long)it.b * a.steps + t + i) * a.heads + it.h) * dz;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < dz; c0 += 16) {
-                        uint32_t u[16], v[16];
-                        tmem_ld16x2(tmem + TO1 + lanes + c0, tmem + TO2 + lanes + c0, u, v);
-                        uint64_t o[8];
+                    for (int c0 = 0; c0 < dz; c0 += 32) {
+                        uint32_t u[32], v[32];
+                        tmem_ld32x2(tmem + TO1 + lanes + c0, tmem + TO2 + lanes + c0, u, v);
+                        uint64_t o[16];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
+                        for (int j = 0; j < 16; ++j)
                             o[j] = fma2(wi2, pair(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])),
                                         mul2(os2, pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]))));
-                            if (i >= m) o[j] = 0ull;
+                        if (m < TC && i >= m) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = 0ull;
                         }
                         if (t + i >= it.t1) {
                         } else if (a.out32) {
                             float* to = a.out32 + at + c0;
 #pragma unroll
-                            for (int j = 0; j < 8; j += 2)
+                            for (int j = 0; j < 16; j += 2)
                                 if (c0 + 2 * j < dz) *reinterpret_cast<ulonglong2*>(to + 2 * j) = make_ulonglong2(o[j], o[j + 1]);
                         } else {
-                            uint32_t q[8];
+                            uint32_t q[16];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) q[j] = round2(o[j]);
+                            for (int j = 0; j < 16; ++j) q[j] = round2(o[j]);
                             bf16* to = a.out + at + c0;
                             if (wide) {
                                 store32(to, q);
+                                if (c0 + 16 < dz) store32(to + 16, q + 8);
                             } else {
-                                *reinterpret_cast<uint4*>(to) = make_uint4(q[0], q[1], q[2], q[3]);
-                                if (c0 + 8 < dz) *reinterpret_cast<uint4*>(to + 8) = make_uint4(q[4], q[5], q[6], q[7]);
+#pragma unroll
+                                for (int j = 0; j < 16; j += 4)
+                                    if (c0 + 2 * j < dz) *reinterpret_cast<uint4*>(to + 2 * j) = make_uint4(q[j], q[j + 1], q[j + 2], q[j + 3]);
                             }
                         }
                     }
@@ -371,8 +377,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                 const int st = (int)(n & 1);
                 const uint32_t ph = (uint32_t)(n & 1), two = (uint32_t)((n >> 1) & 1);
                 if (m < TC) {  // a short chunk: rows of Z that are no tokens must not reach a product, the first of which follows O1
-                    if (!(ok = __all_sync(kFull, mbar_wait(z_full + (STATE ? st : 0), STATE ? two : ph, fail)))) break;
-                    unsigned char* Z = sm + L::Z + (STATE ? st : 0) * TILE;
+                    if (!(ok = __all_sync(kFull, mbar_wait(z_full + st, two, fail)))) break;
+                    unsigned char* Z = sm + L::Z + st * TILE;
                     for (int e = tid; e < TILE / 16; e += 256)
                         if (((e >> 3) & (TC - 1)) >= m) *reinterpret_cast<uint4*>(Z + e * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                     fence_async_smem();
                     mbar_arrive(s_ready);
                 }
-                if (!(ok = __all_sync(kFull, mbar_wait(y_full + st, two, fail) && mbar_wait(z_full + (STATE ? st : 0), STATE ? two : ph, fail) &&
+                if (!(ok = __all_sync(kFull, mbar_wait(y_full + st, two, fail) && mbar_wait(z_full + st, two, fail) &&
                                                  (STATE || mbar_wait(p_full, ph, fail)))))
                     break;
                 unsigned char* Y = sm + L::Y + st * TILE;
