@@ -32,6 +32,13 @@ constexpr int SMS = 148;
 constexpr long kPieceElems = 1l << 27; // entries of G (times planes) at a time: 256 MB
 constexpr float kLog2e = 1.4426950408889634f;
 
+// 2^x: the exponent unit's own instruction, results below the normal range to zero.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // ---- the GEMM --------------------------------------------------------------------------------------------------
 
 enum Epilogue { LSE, GRAD, OUT };
@@ -68,12 +75,12 @@ struct Maps {
     CUtensorMap a[2], b[2], g;
 };
 
-// GRAD gives a stage of operands for the epilogue's output tile: a warp's 32 rows by half the columns.
+// GRAD's epilogue stages its output, a box of 64 columns a warp at a time.
 template <int EPI, int BN>
 struct Tile {
     static constexpr int A = BM * BK * 2, B = BN * BK * 2, STAGE = A + B;
-    static constexpr int OUTW = EPI == GRAD ? 32 * BN : 0;  // bytes a warp
-    static constexpr int STAGES = EPI == GRAD ? (BN == 256 ? 3 : 5) : BN == 256 ? 4 : 6;
+    static constexpr int OUTW = EPI == GRAD ? 4096 : 0;  // bytes a warp: 32 rows of 64 columns
+    static constexpr int STAGES = BN == 256 ? 4 : EPI == GRAD ? 5 : 6;
     static constexpr size_t bytes = (size_t)STAGES * STAGE + EPW * OUTW + 1024 + 256;
 };
 
@@ -231,9 +238,14 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                     const float was = mx;
                     mx = fmaxf(mx, top);
                     const float shift = mx == -INFINITY ? 0.f : -mx * kLog2e;
+                    const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
                     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) part[j & 3] += exp2f(fmaf(v[j], kLog2e, shift));
+                    for (int j = 0; j < 32; j += 2) {
+                        float e0, e1;
+                        unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
+                        part[j & 3] += ex2(e0), part[(j & 3) + 1] += ex2(e1);
+                    }
                     sum = sum * exp2f(fmaf(was, kLog2e, shift)) + ((part[0] + part[1]) + (part[2] + part[3]));
                     if ((unsigned)(pick - c) < 32u) {
                         float z = 0.f;
@@ -248,17 +260,27 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
                 const float w = t < 0 ? 0.f : a.dloss[row];
                 const float shift = in ? -a.lse[row] * kLog2e : 0.f;
+                const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
                 for (int c = half * HALF; c < cols; c += 32) {
                     float v[32];
                     tmem_ld32(src + c, v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = exp2f(fmaf(v[j], kLog2e, shift));
+                    for (int j = 0; j < 32; j += 2) {
+                        float e0, e1;
+                        unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
+                        v[j] = ex2(e0), v[j + 1] = ex2(e1);
+                    }
                     if ((unsigned)(pick - c) < 32u) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] -= pick - c == j ? 1.f : 0.f;
                     }
+                    if (t >= 0) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = t >= 0 ? v[j] * w : 0.f;
+                        for (int j = 0; j < 32; ++j) v[j] *= w;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                    }
                     if (c + 32 > cols) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
@@ -268,9 +290,9 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                         // through shared memory (rows of 64 columns, swizzled) and out by TMA, which drops what lies
                         // beyond the matrix: stored from the registers, a warp's 32 rows at 16 bytes each took
                         // the logits' pass from 1.46 to 1.09 PFLOP/s
-                        unsigned char* box = tiles + S * TL::STAGE + (warp - 2) * TL::OUTW + ((c >> 6) & (TL::OUTW / 4096 - 1)) * 4096;
+                        unsigned char* box = tiles + S * TL::STAGE + (warp - 2) * TL::OUTW;
                         if ((c & 32) == 0) {
-                            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(TL::OUTW / 4096 - 1) : "memory");
+                            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                             __syncwarp();
                         }
 #pragma unroll
@@ -300,9 +322,6 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                         }
                     }
                 }
-                if (a.planes == 1 && lane == 0)  // a box that this tile lacks counts too: the waits above go by number
-                    for (int c = max(half * HALF, (cols + 63) & ~63); c < half * HALF + HALF; c += 64)
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             } else {
                 for (int c = half * HALF; c < cols; c += 32) {
                     float v[32];
