@@ -16,7 +16,8 @@
 //
 // Operands are bfloat16. float32 inputs are split into three bfloat16 planes (8 bits each) and each product runs
 // over the six pairs of planes that matter (2^-24), smallest first, with the same kernel.
-// Rows whose target is ignored are packed as zeros, so nothing in them reaches a sum.
+// Rows without a target cost nothing: a first kernel lists the rows that have one, and everything after works on those
+// rows alone, packed (their number stays on the device: the kernels read it).
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -58,9 +59,10 @@ struct Gemm {
     int pairs;
     signed char ia[6], ib[6];
     int* status;          // the caller's word: a bounded wait that ran out
+    const int* live;      // rows that have a target: the logits' m, dH's m, dW's k
     int f32;              // the inputs are float32
     // LSE, GRAD (m = rows, n = the piece's part of the vocabulary from v0 on)
-    const int* target;    // -1: ignored
+    const int *target, *row;  // of the packed rows: the target, and which row it was
     int v0;
     float2* part;         // (2 tiles_n of the whole vocabulary, rows): maximum, sum
     int part_tile0;
@@ -115,24 +117,30 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
-    const long units = a.job[0].units + (EPI == OUT ? a.job[1].units : 0);
+    const int live = __shfl_sync(kFull, *a.live, 0);
+    const int m0 = min(a.job[0].m, live), tiles0 = (m0 + BM - 1) / BM;
+    const int kb1 = (min(a.job[1].k, live) + BK - 1) / BK, blocks1 = EPI == OUT ? (kb1 + max(a.job[1].splits, 1) - 1) / max(a.job[1].splits, 1) : 0;
+    const long units0 = (long)tiles0 * a.job[0].tiles_n * a.job[0].splits;
+    const long units = units0 + (EPI == OUT ? a.job[1].units : 0);
 
     struct Unit {
         int job, tm, tn, sp, k0, k1;
     };
     auto unit = [&](long u) {
         Unit r;
-        r.job = EPI == OUT && u >= a.job[0].units ? 1 : 0;
-        if (r.job) u -= a.job[0].units;
+        r.job = EPI == OUT && u >= units0 ? 1 : 0;
+        if (r.job) u -= units0;
         const Job& j = a.job[r.job];
-        const long per = (long)j.tiles_m * j.tiles_n;
+        const int tiles_m = r.job ? j.tiles_m : tiles0;
+        const long per = (long)tiles_m * j.tiles_n;
         r.sp = (int)(u / per);
         const long t = u - r.sp * per;
         // neighbours share the larger operand's rows: a gradient's G, the logits' piece of the weight
         if (EPI == OUT) r.tn = (int)(t % j.tiles_n), r.tm = (int)(t / j.tiles_n);
-        else r.tm = (int)(t % j.tiles_m), r.tn = (int)(t / j.tiles_m);
-        r.k0 = r.sp * j.blocks;
-        r.k1 = min(r.k0 + j.blocks, (j.k + BK - 1) / BK);
+        else r.tm = (int)(t % tiles_m), r.tn = (int)(t / tiles_m);
+        const int blocks = r.job ? blocks1 : j.blocks;
+        r.k0 = r.sp * blocks;
+        r.k1 = min(r.k0 + blocks, r.job ? kb1 : (j.k + BK - 1) / BK);
         return r;
     };
 
@@ -219,7 +227,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
             const int row = r.tm * BM + quarter * 32 + lane;
-            const bool in = row < job.m;
+            const bool in = row < (r.job ? job.m : m0);
             const int cols = min(half * HALF + HALF, job.n - r.tn * BN);
             if (EPI == LSE) {
                 const int pick = in ? a.target[row] - a.v0 - r.tn * BN : -1;
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
             } else if (EPI == GRAD) {
                 const int t = in ? a.target[row] : -1;
                 const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
-                const float w = t < 0 ? 0.f : a.dloss[row];
+                const float w = t < 0 ? 0.f : a.dloss[a.row[row]];
                 const float shift = in ? -a.lse[row] * kLog2e : 0.f;
                 const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
                 for (int c = half * HALF; c < cols; c += 32) {
@@ -308,7 +316,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                         }
                         continue;
                     }
-                    for (int s = 0; in && s < a.planes; ++s) {
+                    for (int s = 0; row < job.m && s < a.planes; ++s) {  // rows that are none: zeros
                         bf16* g = a.g + s * a.g_plane + (long)row * a.ldg + r.tn * BN + c;
 #pragma unroll
                         for (int j = 0; j < 32; j += 8) {
@@ -395,36 +403,76 @@ struct Pack {
     long plane;
 };
 
-// Packs the hidden rows (a row without a target as zeros) with the targets as vocabulary positions (-1: no loss),
-// and behind them the rows of a piece of the weight.
+// What the rows' targets say, for the forward and its backward: how many rows have one, which rows those are and their
+// targets (by packed position), and each row's packed position (-1: no target).
+struct RowPlan {
+    int *live, *row, *target, *slot;
+};
+
+__host__ __device__ inline RowPlan row_plan(int* p, long rows) { return RowPlan{p, p + 4, p + 4 + rows, p + 4 + 2 * rows}; }
+
+// One CTA: every thread counts its share of the rows, the CTA scans the counts, every thread lists its share.
+__global__ void __launch_bounds__(1024) plan_kernel(const void* __restrict__ targets, int wide, long rows, long vocab, long ignore, RowPlan p,
+                                                    float* __restrict__ loss, int* status) {
+    __shared__ int warp_sum[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long per = (rows + 1023) / 1024, first = tid * per, last = first + per < rows ? first + per : rows;
+    auto target = [&](long i) {
+        const long t = wide ? __ldg(reinterpret_cast<const long long*>(targets) + i) : (long)__ldg(reinterpret_cast<const int*>(targets) + i);
+        if (t == ignore) return -1;
+        if (t >= 0 && t < vocab) return (int)t;
+        report(status, EWS_ERR_INDEX);
+        return -1;
+    };
+    int count = 0;
+#pragma unroll 8
+    for (long i = first; i < last; ++i) count += target(i) >= 0;
+    int incl = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int at = incl - count;
+    for (int w = 0; w < warp; ++w) at += warp_sum[w];
+    if (tid == 1023) *p.live = at + count;
+#pragma unroll 4
+    for (long i = first; i < last; ++i) {
+        const int t = target(i);
+        p.slot[i] = t >= 0 ? at : -1;
+        if (t >= 0) {
+            p.row[at] = (int)i;
+            p.target[at] = t;
+            ++at;
+        } else {
+            loss[i] = 0.f;
+        }
+    }
+}
+
+// Packs the hidden rows that have a target (zeros up to the end of their last tile), and behind them the rows of a piece
+// of the weight.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Pack<T> h, const __grid_constant__ Pack<T> w, int dim, int ld,
-                                                   int planes, const void* __restrict__ targets, int wide, long vocab, long ignore,
-                                                   int* __restrict__ target, int* status) {
+                                                   int planes, const int* __restrict__ live_rows, const int* __restrict__ rows) {
     const int per = ld / 8;
-    const long total = (h.rows + w.rows) * per;
+    const int live = *live_rows;
+    const long hidden_rows = h.rows ? min(h.rows, ((long)live + BM - 1) / BM * BM) : 0;
+    const long total = (hidden_rows + w.rows) * per;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
         long row = e / per;
         const int col = (int)(e - row * per) * 8;
-        const bool hidden = row < h.rows;
-        bool live = true;
-        if (hidden) {
-            const long t = wide ? reinterpret_cast<const long long*>(targets)[row] : (long)reinterpret_cast<const int*>(targets)[row];
-            live = t != ignore && t >= 0 && t < vocab;
-            if (col == 0) {
-                target[row] = live ? (int)t : -1;
-                if (!live && t != ignore) report(status, EWS_ERR_INDEX);
-            }
-        } else {
-            row -= h.rows;
-        }
+        const bool hidden = row < hidden_rows;
+        if (!hidden) row -= hidden_rows;
         const T* in = hidden ? h.in : w.in;
         const long stride = hidden ? h.stride : w.stride;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        if (live) {
-            const T* p = in + row * stride + col;
+        if (!hidden || row < live) {
+            const T* p = in + (hidden ? rows[row] : row) * stride + col;
             if (stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(in)) {
 #pragma unroll
                 for (int j = 0; j < 8; j += Vec<T, true>::N) Vec<T, true>::load(p + j, v + j);
@@ -445,13 +493,14 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Pack<
 }
 
 // The row's logsumexp from the tiles' maxima and sums: 32 rows by 8 groups of tiles a CTA.
-__global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ part, int tiles, long rows, const int* __restrict__ target,
+__global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ part, int tiles, long rows, RowPlan plan,
                                                   const float* __restrict__ picked, float* __restrict__ loss, float* __restrict__ lse) {
     __shared__ float2 red[8][32];
     const int l = threadIdx.x & 31, g = threadIdx.x >> 5;
     const long row = (long)blockIdx.x * 32 + l;
+    const int live = *plan.live;
     float m = -INFINITY, s = 0.f;
-    if (row < rows)
+    if (row < live)
         for (int t = g; t < tiles; t += 8) {
             const float2 p = part[(long)t * rows + row];
             const float n = fmaxf(m, p.x);
@@ -461,7 +510,7 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
         }
     red[g][l] = make_float2(m, s);
     __syncthreads();
-    if (g > 0 || row >= rows) return;
+    if (g > 0 || row >= live) return;
     for (int j = 1; j < 8; ++j) {
         const float2 p = red[j][l];
         const float n = fmaxf(m, p.x);
@@ -471,15 +520,27 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
     }
     const float z = m + logf(s);
     lse[row] = z;
-    loss[row] = target[row] >= 0 ? z - picked[row] : 0.f;
+    loss[plan.row[row]] = z - picked[row];
 }
 
-// A gradient from its float32 partials, summed in order and rounded once.
+// A gradient from its float32 partials, summed in order and rounded once; with `slot` the rows of the result are taken
+// from their packed positions, and a row without one is zero.
 template <typename T>
-__global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ acc, int splits, long total, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ acc, int splits, long rows, int n, const int* __restrict__ slot,
+                                                     T* __restrict__ out) {
+    const long total = rows * n;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        float s = acc[e];
-        for (int k = 1; k < splits; ++k) s += acc[k * total + e];
+        long from = e;
+        if (slot) {
+            const long row = e / n;
+            const int at = slot[row];
+            from = at < 0 ? -1 : (long)at * n + (e - row * n);
+        }
+        float s = 0.f;
+        if (from >= 0) {
+            s = acc[from];
+            for (int k = 1; k < splits; ++k) s += acc[k * total + from];
+        }
         out[e] = from_f<T>(s);
     }
 }
@@ -554,8 +615,8 @@ struct Plan {
     bool pack_w;           // the weight is packed piece by piece
     long piece, pieces;    // vocabulary entries a piece
     int split_h, split_w;  // K splits of dhidden, dweight
-    bool acc_h, acc_w;
-    size_t target, picked, part, h, w, g, ah, aw, bytes;
+    bool acc_w;
+    size_t picked, part, h, w, g, ah, aw, bytes;
 };
 
 int check(const ews_vocab_args* a) {
@@ -607,7 +668,6 @@ Plan plan(const ews_vocab_args* a, bool bwd) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.target = take(sizeof(int) * n);
     p.h = take(sizeof(bf16) * (size_t)p.planes * n * p.ldd);
     if (p.pack_w) p.w = take(sizeof(bf16) * (size_t)p.planes * p.piece * p.ldd);
     if (!bwd) {
@@ -620,9 +680,8 @@ Plan plan(const ews_vocab_args* a, bool bwd) {
         const long tw = ((p.piece + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
         p.split_h = splits_of(n, a->dim, p.piece, tw);
         p.split_w = splits_of(p.piece, a->dim, n, th * p.split_h);
-        p.acc_h = p.split_h > 1 || p.pieces > 1;
         p.acc_w = p.split_w > 1;
-        if (p.acc_h) p.ah = take(sizeof(float) * (size_t)p.split_h * n * a->dim);
+        p.ah = take(sizeof(float) * (size_t)p.split_h * n * a->dim);
         if (p.acc_w) p.aw = take(sizeof(float) * (size_t)p.split_w * p.piece * a->dim);
     }
     p.bytes = at;
@@ -635,8 +694,8 @@ unsigned grid_of(long total) {
 }
 
 template <typename T>
-int reduce(const float* acc, int splits, long total, T* out, cudaStream_t s) {
-    reduce_kernel<T><<<grid_of(total), 256, 0, s>>>(acc, splits, total, out);
+int reduce(const float* acc, int splits, long rows, long n, const int* slot, T* out, cudaStream_t s) {
+    reduce_kernel<T><<<grid_of(rows * n), 256, 0, s>>>(acc, splits, rows, (int)n, slot, out);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -660,8 +719,8 @@ int operands(const ews_vocab_args* a, const Plan& p, char* w, long v0, long n, O
         o->p = reinterpret_cast<const bf16*>(rows), o->cols = a->dim, o->ld = a->weight_stride, o->plane = 0;
     }
     if (ph.rows + pw.rows == 0) return EWS_OK;
-    pack_kernel<T><<<grid_of((ph.rows + pw.rows) * (p.ldd / 8)), 256, 0, s>>>(ph, pw, (int)a->dim, p.ldd, p.planes, a->targets, a->targets_wide,
-                                                                              a->vocab, a->ignore, reinterpret_cast<int*>(w + p.target), a->status);
+    const RowPlan plan = row_plan(a->plan, a->rows);
+    pack_kernel<T><<<grid_of((ph.rows + pw.rows) * (p.ldd / 8)), 256, 0, s>>>(ph, pw, (int)a->dim, p.ldd, p.planes, plan.live, plan.row);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -671,8 +730,10 @@ int forward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     Operand h{}, wt{}, none{};
     int rc = EWS_OK;
     Gemm g{};
+    const RowPlan plan = row_plan(a->plan, a->rows);
+    plan_kernel<<<1, 1024, 0, s>>>(a->targets, a->targets_wide, a->rows, a->vocab, a->ignore, plan, a->loss, a->status);
     g.status = a->status;
-    g.target = reinterpret_cast<const int*>(w + p.target);
+    g.live = plan.live, g.target = plan.target, g.row = plan.row;
     g.part = reinterpret_cast<float2*>(w + p.part);
     g.picked = reinterpret_cast<float*>(w + p.picked);
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
@@ -683,7 +744,7 @@ int forward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
         g.part_tile0 += g.job[0].tiles_n;
     }
     if (rc != EWS_OK) return rc;
-    lse_kernel<<<(unsigned)((a->rows + 31) / 32), 256, 0, s>>>(g.part, 2 * g.part_tile0, a->rows, g.target, g.picked, a->loss, a->lse);
+    lse_kernel<<<(unsigned)((a->rows + 31) / 32), 256, 0, s>>>(g.part, 2 * g.part_tile0, a->rows, plan, g.picked, a->loss, a->lse);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -692,11 +753,12 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     Operand h{}, wt{}, go{}, none{};
     int rc = EWS_OK;
-    float* acc_h = p.acc_h ? reinterpret_cast<float*>(w + p.ah) : nullptr;
+    float* acc_h = reinterpret_cast<float*>(w + p.ah);
+    const RowPlan plan = row_plan(a->plan, a->rows);
     float* acc_w = p.acc_w ? reinterpret_cast<float*>(w + p.aw) : nullptr;
     Gemm base{};
     base.status = a->status, base.f32 = sizeof(T) == 4;
-    base.target = reinterpret_cast<const int*>(w + p.target), base.lse = a->lse, base.dloss = a->dloss;
+    base.live = plan.live, base.target = plan.target, base.row = plan.row, base.lse = a->lse, base.dloss = a->dloss;
     base.g = reinterpret_cast<bf16*>(w + p.g), base.planes = p.planes;
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
         const long n = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
@@ -710,16 +772,16 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
         T* out = static_cast<T*>(a->dweight) + (a->dweight ? v0 * a->dim : 0);
         if (a->dhidden) {  // dH += G W: K is the piece of the vocabulary
             o.job[0] = job_of(a->rows, a->dim, n, p.split_h);
-            o.job[0].out = a->dhidden, o.job[0].acc = acc_h, o.job[0].add = v0 > 0;
+            o.job[0].acc = acc_h, o.job[0].add = v0 > 0;
         }
         if (a->dweight) {  // dW = G^T H: K is the rows
             o.job[1] = job_of(n, a->dim, a->rows, p.split_w);
             o.job[1].out = out, o.job[1].acc = acc_w;
         }
         if ((rc = gemm<OUT>(o, go, wt, go, h, p.planes, s)) != EWS_OK) break;
-        if (a->dweight && acc_w) rc = reduce<T>(acc_w, p.split_w, n * a->dim, out, s);
+        if (a->dweight && acc_w) rc = reduce<T>(acc_w, p.split_w, n, a->dim, nullptr, out, s);
     }
-    if (rc == EWS_OK && a->dhidden && acc_h) rc = reduce<T>(acc_h, p.split_h, a->rows * a->dim, static_cast<T*>(a->dhidden), s);
+    if (rc == EWS_OK && a->dhidden) rc = reduce<T>(acc_h, p.split_h, a->rows, a->dim, plan.slot, static_cast<T*>(a->dhidden), s);
     return rc;
 }
 
@@ -736,7 +798,7 @@ extern "C" int ews_vocab_fwd(const ews_vocab_args* a, ews_stream_t stream) {
     const int rc = check(a);
     if (rc != EWS_OK) return rc;
     if (a->rows == 0) return EWS_OK;
-    if (!a->hidden || !a->weight || !a->targets || !a->loss || !a->lse) return EWS_ERR_INVALID_ARGUMENT;
+    if (!a->hidden || !a->weight || !a->targets || !a->loss || !a->lse || !a->plan) return EWS_ERR_INVALID_ARGUMENT;
     const Plan p = plan(a, false);
     if (!a->work || !aligned16(a->work) || a->work_bytes < p.bytes) return EWS_ERR_WORKSPACE;
     return a->dtype == EWS_DTYPE_BF16 ? forward<bf16>(a, p, (cudaStream_t)stream) : forward<float>(a, p, (cudaStream_t)stream);
@@ -751,7 +813,7 @@ extern "C" int ews_vocab_bwd(const ews_vocab_args* a, ews_stream_t stream) {
         if (a->dweight && cudaMemsetAsync(a->dweight, 0, e * a->vocab * a->dim, s) != cudaSuccess) return EWS_ERR_LAUNCH;
         return EWS_OK;
     }
-    if (!a->hidden || !a->weight || !a->targets || !a->dloss || !a->lse) return EWS_ERR_INVALID_ARGUMENT;
+    if (!a->hidden || !a->weight || !a->dloss || !a->lse || !a->plan) return EWS_ERR_INVALID_ARGUMENT;
     if (!a->dhidden && !a->dweight) return EWS_OK;
     const Plan p = plan(a, true);
     if (!a->work || !aligned16(a->work) || a->work_bytes < p.bytes) return EWS_ERR_WORKSPACE;

@@ -25,7 +25,7 @@ MAX_HEAD = 128
 
 # ews_decay_args and ews_vocab_args, packed in one call (native alignment; the fields in the header's order).
 _DECAY = struct.Struct("@7if3P9q6P3q6PNP").pack
-_VOCAB = struct.Struct("@3q2i3P3q6PNP").pack
+_VOCAB = struct.Struct("@3q2i3P3q7PNP").pack
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without building a Stream
 
@@ -295,11 +295,11 @@ def decayed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ra
 # --------------------------------------------------------------------------------------------- vocabulary loss
 
 
-def _vocab_args(hidden, weight, targets, ignore, loss=None, lse=None, dloss=None, dh=None, dw=None, work=None):
+def _vocab_args(hidden, weight, targets, ignore, loss=None, lse=None, plan=None, dloss=None, dh=None, dw=None, work=None):
     rows, dim = hidden.shape
     return _VOCAB(rows, weight.shape[0], dim, _DTYPES[hidden.dtype], _WIDE[targets.dtype], hidden.data_ptr(), weight.data_ptr(),
-                  targets.data_ptr(), _row_stride(hidden), _row_stride(weight), ignore, _addr(loss), _addr(lse), _addr(dloss),
-                  _addr(dh), _addr(dw), _addr(work), 0 if work is None else work.numel(), engine.index_word(hidden.get_device())[0])
+                  targets.data_ptr(), _row_stride(hidden), _row_stride(weight), ignore, _addr(loss), _addr(lse), _addr(plan),
+                  _addr(dloss), _addr(dh), _addr(dw), _addr(work), 0 if work is None else work.numel(), engine.index_word(hidden.get_device())[0])
 
 
 def _vocab(hidden, weight, targets, ignore):
@@ -307,29 +307,30 @@ def _vocab(hidden, weight, targets, ignore):
     rows = hidden.shape[0]
     loss, lse = torch.empty((2, rows), dtype=torch.float32, device=hidden.device).unbind(0)
     work = _work(lib.ews_vocab_work_size(_vocab_args(hidden, weight, targets, ignore), 0), hidden)
-    args = _vocab_args(hidden, weight, targets, ignore, loss, lse, work=work)
+    plan = torch.empty(3 * rows + 4, dtype=torch.int32, device=hidden.device)
+    args = _vocab_args(hidden, weight, targets, ignore, loss, lse, plan, work=work)
     _launch(hidden.get_device(), "ews_vocab_fwd", rows, lib.ews_vocab_fwd, args)
-    return loss, lse
+    return loss, lse, plan
 
 
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore):
         hidden, weight = _rows(hidden), _rows(weight)
-        loss, lse = _vocab(hidden, weight, targets, ignore)
+        loss, lse, plan = _vocab(hidden, weight, targets, ignore)
         ctx.ignore = ignore
-        ctx.save_for_backward(hidden, weight, targets, lse)
+        ctx.save_for_backward(hidden, weight, targets, lse, plan)
         return loss
 
     @staticmethod
     def backward(ctx, dloss):
-        hidden, weight, targets, lse = ctx.saved_tensors
+        hidden, weight, targets, lse, plan = ctx.saved_tensors
         lib = _lib.load()
         dloss = dloss.contiguous()
         dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
                   for t, need in ((hidden, ctx.needs_input_grad[0]), (weight, ctx.needs_input_grad[1])))
         work = _work(lib.ews_vocab_work_size(_vocab_args(hidden, weight, targets, ctx.ignore), 1), hidden)
-        args = _vocab_args(hidden, weight, targets, ctx.ignore, None, lse, dloss, dh, dw, work)
+        args = _vocab_args(hidden, weight, targets, ctx.ignore, None, lse, plan, dloss, dh, dw, work)
         _launch(hidden.get_device(), "ews_vocab_bwd", hidden.shape[0], lib.ews_vocab_bwd, args)
         return dh, dw, None, None
 
@@ -338,7 +339,7 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
     """Softmax cross entropy of ``hidden @ weight.T`` against ``targets``, per position, in float32.
 
     hidden (..., D) and weight (V, D), both float32 or both bfloat16; targets (...) int64 or int32. Positions whose
-    target is ``ignore_index`` have loss 0, no gradient, and their hidden rows do not enter the others'. Returns the
+    target is ``ignore_index`` have loss 0 and no gradient, and cost nothing (only the other rows are computed). Returns the
     losses with the shape of ``targets``; the logits (N, V) are formed in tiles and pieces and never kept.
     Differentiable in hidden and weight. A target out of range counts as ignored and raises IndexError on the next
     call."""

@@ -390,8 +390,9 @@ int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float
 /* ---- vocabulary loss ------------------------------------------------------------------------------
  * loss_n = logsumexp_v <hidden_n, weight_v> - <hidden_n, weight_{t_n}> for hidden (rows, dim) and weight (vocab, dim)
  * of `dtype` (rows `hidden_stride` / `weight_stride` elements apart), targets (rows) int64 (targets_wide) or int32;
- * 0 where the target is `ignore`. loss and lse (the row's logsumexp, kept for the backward) are float32.
- *   ews_vocab_bwd: from dloss (rows) the gradients dhidden (rows, dim) and dweight (vocab, dim), contiguous, either
+ * 0 where the target is `ignore`. loss is float32. The forward also writes lse (rows float32: the logsumexps) and plan
+ * (3 rows + 4 int32: the rows that have a target, which alone are computed), both for the backward.
+ *   ews_vocab_bwd: from dloss (rows), lse and plan the gradients dhidden (rows, dim) and dweight (vocab, dim), contiguous, either
  *   may be NULL. The logits are formed again in pieces of the vocabulary and never kept whole.
  * A target out of range counts as ignored and sets *status (device or pinned host memory, may be NULL) to
  * EWS_ERR_INDEX; a bounded device wait that ran out sets EWS_ERR_LOOKBACK_TIMEOUT (the outputs are then invalid).
@@ -402,6 +403,7 @@ typedef struct {
     const void *hidden, *weight, *targets;
     int64_t hidden_stride, weight_stride, ignore;
     float *loss, *lse;
+    int* plan;
     const float* dloss;
     void *dhidden, *dweight;
     void* work;

@@ -19,7 +19,7 @@ def _decay(batch=2, steps=100, heads=4, kv=2, dk=64, dv=64, dtype=1, scale=0.125
 
 
 def _vocab(rows=10, vocab=100, dim=16, dtype=1, hs=16, ws=16):
-    return token_ops._VOCAB(rows, vocab, dim, dtype, 1, 16, 16, 16, hs, ws, -100, 16, 16, 16, 16, 16, 0, 0, 0)
+    return token_ops._VOCAB(rows, vocab, dim, dtype, 1, 16, 16, 16, hs, ws, -100, 16, 16, 16, 16, 16, 16, 0, 0, 0)
 
 
 def test_packed_arguments_have_the_structs_sizes(tmp_path):
