@@ -501,11 +501,17 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
     const int live = *plan.live;
     float m = -INFINITY, s = 0.f;
     if (row < live)
-        for (int t = g; t < tiles; t += 8) {
-            const float2 p = part[(long)t * rows + row];
-            const float n = fmaxf(m, p.x);
+        for (int t0 = g; t0 < tiles; t0 += 64) {
+            float2 p[8];  // eight tiles in flight
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = t0 + 8 * k < tiles ? part[(long)(t0 + 8 * k) * rows + row] : make_float2(-INFINITY, 0.f);
+            float n = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) n = fmaxf(n, p[k].x);
             const float base = n == -INFINITY ? 0.f : n;
-            s = s * exp2f((m - base) * kLog2e) + p.y * exp2f((p.x - base) * kLog2e);
+            s *= exp2f((m - base) * kLog2e);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += p[k].y * exp2f((p[k].x - base) * kLog2e);
             m = n;
         }
     red[g][l] = make_float2(m, s);
@@ -525,23 +531,35 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
 
 // A gradient from its float32 partials, summed in order and rounded once; with `slot` the rows of the result are taken
 // from their packed positions, and a row without one is zero.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ acc, int splits, long rows, int n, const int* __restrict__ slot,
                                                      T* __restrict__ out) {
+    constexpr int W = VEC ? 4 : 1;
+    const int per = n / W;
     const long total = rows * n;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        long from = e;
-        if (slot) {
-            const long row = e / n;
-            const int at = slot[row];
-            from = at < 0 ? -1 : (long)at * n + (e - row * n);
+    // a row's vectors to consecutive threads
+    const int lanes = per < 256 ? per : 256, group = 256 / lanes, l = threadIdx.x % lanes, g = threadIdx.x / lanes;
+    if (g >= group) return;
+    for (long row = (long)blockIdx.x * group + g; row < rows; row += (long)gridDim.x * group) {
+        const long at = slot ? slot[row] : row;
+        for (int c = l; c < per; c += lanes) {
+            float s[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) s[j] = 0.f;
+            if (at >= 0) {
+                const float* p = acc + at * n + c * W;
+                Vec<float, VEC>::load(p, s);
+                for (int k = 1; k < splits; ++k) {
+                    float v[W];
+                    Vec<float, VEC>::load(p + k * total, v);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) s[j] += v[j];
+                }
+            }
+            T* o = out + row * n + c * W;
+            if constexpr (VEC && sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+            else Vec<T, VEC>::store(o, s);
         }
-        float s = 0.f;
-        if (from >= 0) {
-            s = acc[from];
-            for (int k = 1; k < splits; ++k) s += acc[k * total + from];
-        }
-        out[e] = from_f<T>(s);
     }
 }
 
@@ -695,7 +713,9 @@ unsigned grid_of(long total) {
 
 template <typename T>
 int reduce(const float* acc, int splits, long rows, long n, const int* slot, T* out, cudaStream_t s) {
-    reduce_kernel<T><<<grid_of(rows * n), 256, 0, s>>>(acc, splits, rows, (int)n, slot, out);
+    const unsigned grid = grid_of(rows * n / 4 + 1);
+    if (n % 4 == 0 && aligned16(out)) reduce_kernel<T, true><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, out);
+    else reduce_kernel<T, false><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, out);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 

@@ -409,6 +409,31 @@ def test_vocab_loss_pieces(ews):
         assert ((got.double() - exact).abs() <= 1.05 * err + F32 * form + U * exact.abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n,kept", [(700, 3), (700, 130), (300, 300), (257, 1)])
+def test_vocab_loss_with_few_targets(ews, dtype, n, kept):
+    """Only the rows that have a target are computed: none of the others' values matter, wherever they lie."""
+    V, D = 1030, 72
+    g = _gen(n + kept)
+    h = torch.full((n, D), float("nan"), device="cuda").to(dtype)
+    t = torch.full((n,), -100, device="cuda")
+    rows = torch.randperm(n, device="cuda", generator=g)[:kept]
+    h[rows] = torch.randn((kept, D), device="cuda", generator=g).to(dtype)
+    t[rows] = torch.randint(0, V, (kept,), device="cuda", generator=g)
+    w = (torch.randn((V, D), device="cuda", generator=g) / 4).to(dtype)
+    dl = torch.rand((n,), device="cuda", generator=g) + 0.1
+    hl, wl = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ews.vocab_loss(hl, wl, t)
+    dh, dw = torch.autograd.grad(loss, (hl, wl), dl)
+    want, wh, ww, ab, p, gg, hz = _loss_ref(h, w, t, dl)
+    worst = F32 * ab.amax(1)
+    assert ((loss.double() - want).abs() <= 2 * worst + 1e-6 * (want.abs() + 20)).all()
+    eg = p * (2 * worst + 2e-6)[:, None] + (U if dtype == BF16 else 2.0**-21) * gg.abs()
+    for got, exact, err, form in ((dh, wh, eg @ w.double().abs(), gg.abs() @ w.double().abs()), (dw, ww, eg.T @ hz.abs(), gg.abs().T @ hz.abs())):
+        bound = 1.05 * err + F32 * form + (U if dtype == BF16 else 2.0**-23) * exact.abs() + 1e-30
+        assert ((got.double() - exact).abs() <= bound).all(), float(((got.double() - exact).abs() / bound).max())
+
+
 def test_vocab_loss_gradient_against_differences(ews):
     n, V, D = 40, 300, 24
     g = _gen(8)
