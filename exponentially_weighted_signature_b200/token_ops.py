@@ -10,6 +10,7 @@ next token operator on the device raises IndexError (at once under ``configure(c
 
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import Optional
@@ -74,6 +75,25 @@ def _work(size: int, like: torch.Tensor) -> Optional[torch.Tensor]:
     return torch.empty(size, dtype=torch.uint8, device=like.device) if size else None
 
 
+@functools.lru_cache(maxsize=256)
+def _embed_size(n: int, vocab: int, dim: int) -> int:
+    """Workspace bytes are a function of the sizes alone, so each set of sizes asks the library once."""
+    return _lib.load().ews_embed_work_size(n, vocab, dim)
+
+
+@functools.lru_cache(maxsize=256)
+def _decay_size(B: int, T: int, H: int, Hk: int, dk: int, dv: int, code: int, backward: int) -> int:
+    args = _DECAY(B, T, H, Hk, dk, dv, code, 1.0, *([0] * 27), 0, 0)
+    return _lib.load().ews_decay_work_size(args, backward)
+
+
+@functools.lru_cache(maxsize=256)
+def _vocab_size(rows: int, vocab: int, dim: int, code: int, hidden_stride: int, weight_stride: int, weight_at: int, backward: int) -> int:
+    """weight_at: the weight's address modulo 16."""
+    args = _VOCAB(rows, vocab, dim, code, 1, 0, weight_at, 0, hidden_stride, weight_stride, 0, *([0] * 7), 0, 0)
+    return _lib.load().ews_vocab_work_size(args, backward)
+
+
 def _addr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -118,7 +138,7 @@ class _Embedding(torch.autograd.Function):
         n = flat.numel()
         g = _rows(dout.reshape(n, dim))
         grad = torch.empty((vocab, dim), dtype=dout.dtype, device=dout.device)
-        work = _work(lib.ews_embed_work_size(n, vocab, dim), dout)
+        work = _work(_embed_size(n, vocab, dim), dout)
         _launch(dout.get_device(), "ews_embed_bwd", n, lib.ews_embed_bwd, flat.data_ptr(), _WIDE[flat.dtype], g.data_ptr(),
                 _DTYPES[dout.dtype], n, vocab, dim, _row_stride(g), scale, padding_index, grad.data_ptr(), work.data_ptr(),
                 work.numel(), None)
@@ -170,7 +190,7 @@ def _decayed(q, k, v, rate, initial, lengths, scale, want_state):
     dv = v.shape[3]
     out = torch.empty((B, T, H, dv), dtype=q.dtype, device=q.device)
     end = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if want_state else None
-    work = _work(lib.ews_decay_work_size(_decay_args(q, k, v, rate, lengths, initial, scale, out, end), 0), q)
+    work = _work(_decay_size(B, T, H, k.shape[2], dk, dv, _DTYPES[q.dtype], 0), q)
     args = _decay_args(q, k, v, rate, lengths, initial, scale, out, end, work=work)
     _launch(q.get_device(), "ews_decay_fwd", B * T, lib.ews_decay_fwd, args)
     return out, end
@@ -195,7 +215,7 @@ class _Decayed(torch.autograd.Function):
         dend = None if dend is None else dend.contiguous()
         grads = [torch.empty(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v)]
         d0 = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if ctx.needs_input_grad[4] else None
-        work = _work(lib.ews_decay_work_size(_decay_args(q, k, v, rate, lengths, initial, ctx.scale), 1), q)
+        work = _work(_decay_size(B, T, H, k.shape[2], dk, dv, _DTYPES[q.dtype], 1), q)
         args = _decay_args(q, k, v, rate, lengths, initial, ctx.scale, None, None, dout, dend, grads, d0, work)
         _launch(q.get_device(), "ews_decay_bwd", B * T, lib.ews_decay_bwd, args)
         return (*grads, None, d0, None, None, None)
@@ -302,11 +322,16 @@ def _vocab_args(hidden, weight, targets, ignore, loss=None, lse=None, plan=None,
                   _addr(dloss), _addr(dh), _addr(dw), _addr(work), 0 if work is None else work.numel(), engine.index_word(hidden.get_device())[0])
 
 
+def _vocab_work(hidden, weight, backward):
+    return _work(_vocab_size(*hidden.shape[:1], *weight.shape, _DTYPES[hidden.dtype], _row_stride(hidden), _row_stride(weight),
+                             weight.data_ptr() % 16, backward), hidden)
+
+
 def _vocab(hidden, weight, targets, ignore):
     lib = _lib.load()
     rows = hidden.shape[0]
     loss, lse = torch.empty((2, rows), dtype=torch.float32, device=hidden.device).unbind(0)
-    work = _work(lib.ews_vocab_work_size(_vocab_args(hidden, weight, targets, ignore), 0), hidden)
+    work = _vocab_work(hidden, weight, 0)
     plan = torch.empty(3 * rows + 4, dtype=torch.int32, device=hidden.device)
     args = _vocab_args(hidden, weight, targets, ignore, loss, lse, plan, work=work)
     _launch(hidden.get_device(), "ews_vocab_fwd", rows, lib.ews_vocab_fwd, args)
@@ -329,7 +354,7 @@ class _VocabLoss(torch.autograd.Function):
         dloss = dloss.contiguous()
         dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
                   for t, need in ((hidden, ctx.needs_input_grad[0]), (weight, ctx.needs_input_grad[1])))
-        work = _work(lib.ews_vocab_work_size(_vocab_args(hidden, weight, targets, ctx.ignore), 1), hidden)
+        work = _vocab_work(hidden, weight, 1)
         args = _vocab_args(hidden, weight, targets, ctx.ignore, None, lse, plan, dloss, dh, dw, work)
         _launch(hidden.get_device(), "ews_vocab_bwd", hidden.shape[0], lib.ews_vocab_bwd, args)
         return dh, dw, None, None

@@ -81,3 +81,13 @@ def test_index_error_code():
     with pytest.raises(IndexError):
         _lib.check(_lib.EWS_ERR_INDEX, "x")
     assert struct.calcsize("@N") == ctypes.sizeof(ctypes.c_size_t)
+
+
+def test_cached_workspace_sizes_are_the_librarys():
+    lib = _lib.load()
+    for backward in (0, 1):
+        assert token_ops._decay_size(2, 5000, 4, 2, 64, 64, 1, backward) == lib.ews_decay_work_size(_decay(steps=5000), backward) > 0
+        assert token_ops._vocab_size(10, 100, 16, 1, 16, 16, 0, backward) == lib.ews_vocab_work_size(_vocab(), backward) > 0
+        # a weight that TMA cannot read as it lies is packed in the workspace
+        assert token_ops._vocab_size(10, 100, 16, 1, 16, 16, 2, backward) > token_ops._vocab_size(10, 100, 16, 1, 16, 16, 0, backward)
+    assert token_ops._embed_size(100, 10, 8) == lib.ews_embed_work_size(100, 10, 8)
