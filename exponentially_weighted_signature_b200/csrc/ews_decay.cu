@@ -128,12 +128,13 @@ struct Tc<bf16> {
         }
         return a;
     }
-    __device__ static __forceinline__ void mma2(float d0[4], float d1[4], const A& a, const B& b) {
+    static constexpr bool SMALL = false;
+    __device__ static __forceinline__ void mma2(float d0[4], float d1[4], float*, float*, const A& a, const B& b) {
         mma_bf16(d0, a.r, b.r[0], b.r[1]);
         mma_bf16(d1, a.r, b.r[2], b.r[3]);
     }
     template <int NS>
-    __device__ static __forceinline__ void mma2w(float d0[4], float d1[4], const AW<NS>& a, const B& b) {
+    __device__ static __forceinline__ void mma2w(float d0[4], float d1[4], float*, float*, const AW<NS>& a, const B& b) {
 #pragma unroll
         for (int s = NS - 1; s >= 0; --s) {
             mma_bf16(d0, a.r[s], b.r[0], b.r[1]);
@@ -193,17 +194,19 @@ struct Tc<float> {
         const float w0 = wt[k0 + 2 * c], w1 = wt[k0 + 2 * c + 1];
         return of(a[0] * w0, a[8] * w0, a[ld] * w1, a[ld + 8] * w1);
     }
-    __device__ static __forceinline__ void mma2(float d0[4], float d1[4], const A& a, const B& b) {
-        mma_tf32(d0, a.l, b.h[0], b.h[1]);
-        mma_tf32(d1, a.l, b.h[2], b.h[3]);
-        mma_tf32(d0, a.h, b.l[0], b.l[1]);
-        mma_tf32(d1, a.h, b.l[2], b.l[3]);
+    // The small products have an accumulator of their own: every addition to the large one truncates.
+    static constexpr bool SMALL = true;
+    __device__ static __forceinline__ void mma2(float d0[4], float d1[4], float c0[4], float c1[4], const A& a, const B& b) {
+        mma_tf32(c0, a.l, b.h[0], b.h[1]);
+        mma_tf32(c1, a.l, b.h[2], b.h[3]);
+        mma_tf32(c0, a.h, b.l[0], b.l[1]);
+        mma_tf32(c1, a.h, b.l[2], b.l[3]);
         mma_tf32(d0, a.h, b.h[0], b.h[1]);
         mma_tf32(d1, a.h, b.h[2], b.h[3]);
     }
     template <int NS>
-    __device__ static __forceinline__ void mma2w(float d0[4], float d1[4], const A& a, const B& b) {
-        mma2(d0, d1, a, b);
+    __device__ static __forceinline__ void mma2w(float d0[4], float d1[4], float c0[4], float c1[4], const A& a, const B& b) {
+        mma2(d0, d1, c0, c1, a, b);
     }
 };
 
@@ -330,24 +333,31 @@ __global__ void __launch_bounds__(NT) chain_kernel(const __grid_constant__ Chain
             float pr[C / 8][4];
 #pragma unroll
             for (int j = 0; j < C / 8; ++j) pr[j][0] = pr[j][1] = pr[j][2] = pr[j][3] = 0.f;
+            float os[M::SMALL ? DV / 8 : 2][4] = {}, ps[M::SMALL ? C / 8 : 2][4] = {};  // the small products' sums
+            constexpr int O1 = M::SMALL ? 1 : 0;
 #pragma unroll
             for (int kk = 0; kk < DK; kk += M::KS) {
                 const typename M::A xa = M::a_mk(X, S::LK, m0, kk);
 #pragma unroll
                 for (int j = 0; j < C / 16; ++j)
-                    if (j <= warp) M::mma2(pr[2 * j], pr[2 * j + 1], xa, M::b_nk(Y, S::LK, 16 * j, kk));
+                    if (j <= warp) M::mma2(pr[2 * j], pr[2 * j + 1], ps[2 * j * O1], ps[2 * j * O1 + 1], xa, M::b_nk(Y, S::LK, 16 * j, kk));
 #pragma unroll
-                for (int j = 0; j < DV / 16; ++j) M::mma2(o[2 * j], o[2 * j + 1], xa, M::b_kn(st, S::LV, kk, 16 * j));
+                for (int j = 0; j < DV / 16; ++j)
+                    M::mma2(o[2 * j], o[2 * j + 1], os[2 * j * O1], os[2 * j * O1 + 1], xa, M::b_kn(st, S::LV, kk, 16 * j));
             }
             const int shift = a.rev ? 0 : 1;
             const float w0 = pw[m0 + r + shift], w1 = pw[m0 + r + 8 + shift];
 #pragma unroll
-            for (int j = 0; j < DV / 8; ++j) o[j][0] *= w0, o[j][1] *= w0, o[j][2] *= w1, o[j][3] *= w1;
+            for (int j = 0; j < DV / 8; ++j) {
+                o[j][0] *= w0, o[j][1] *= w0, o[j][2] *= w1, o[j][3] *= w1;
+                if constexpr (M::SMALL) os[j][0] *= w0, os[j][1] *= w0, os[j][2] *= w1, os[j][3] *= w1;
+            }
 #pragma unroll
             for (int j = 0; j < C / 8; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int gap = m0 + r + (e >> 1) * 8 - (8 * j + 2 * c + (e & 1));
+                    if constexpr (M::SMALL) pr[j][e] += ps[j][e];
                     pr[j][e] = gap >= 0 ? pr[j][e] * pw[gap] : 0.f;
                 }
 #pragma unroll
@@ -355,7 +365,8 @@ __global__ void __launch_bounds__(NT) chain_kernel(const __grid_constant__ Chain
                 if (kk < m0 + 16) {
                     const typename M::A pa = M::a_acc(pr, kk);
 #pragma unroll
-                    for (int j = 0; j < DV / 16; ++j) M::mma2(o[2 * j], o[2 * j + 1], pa, M::b_kn(Z, S::LV, kk, 16 * j));
+                    for (int j = 0; j < DV / 16; ++j)
+                        M::mma2(o[2 * j], o[2 * j + 1], os[2 * j * O1], os[2 * j * O1 + 1], pa, M::b_kn(Z, S::LV, kk, 16 * j));
                 }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -369,7 +380,7 @@ __global__ void __launch_bounds__(NT) chain_kernel(const __grid_constant__ Chain
                     for (int q = 0; q < 2; ++q) {
                         const int col = 8 * j + 2 * c + q;
                         if (c0 + col >= dz) continue;
-                        const float val = o[j][2 * e + q] * a.oscale;
+                        const float val = (M::SMALL ? o[j][2 * e + q] + os[j * O1][2 * e + q] : o[j][2 * e + q]) * a.oscale;
                         if (a.out32) a.out32[at + col] = val;
                         else a.out[at + col] = from_f<T>(val);
                     }
@@ -379,7 +390,8 @@ __global__ void __launch_bounds__(NT) chain_kernel(const __grid_constant__ Chain
         const float gn = pw[n];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            float add[NTL][4];
+            float add[NTL][4], as[M::SMALL ? NTL : 2][4] = {};
+            constexpr int A1 = M::SMALL ? 1 : 0;
 #pragma unroll
             for (int j = 0; j < NTL; ++j) add[j][0] = add[j][1] = add[j][2] = add[j][3] = 0.f;
 #pragma unroll
@@ -387,12 +399,12 @@ __global__ void __launch_bounds__(NT) chain_kernel(const __grid_constant__ Chain
                 const auto ya = M::template a_km<NS>(Y, S::LK, kk, (wm * MT + i) * 16, wt);
 #pragma unroll
                 for (int j = 0; j < NTL; j += 2)
-                    M::template mma2w<NS>(add[j], add[j + 1], ya, M::b_kn(Z, S::LV, kk, (wn * NTL + j) * 8));
+                    M::template mma2w<NS>(add[j], add[j + 1], as[j * A1], as[j * A1 + 1], ya, M::b_kn(Z, S::LV, kk, (wn * NTL + j) * 8));
             }
 #pragma unroll
             for (int j = 0; j < NTL; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][j][e] = fmaf(gn, s[i][j][e], add[j][e]);
+                for (int e = 0; e < 4; ++e) s[i][j][e] = fmaf(gn, s[i][j][e], M::SMALL ? add[j][e] + as[j * A1][e] : add[j][e]);
         }
         if (!STATE) put_state();
     }
@@ -546,8 +558,8 @@ int pad_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 // Segments of the axis: as many as two CTAs on each of 148 SMs, but none shorter than four chunks, since each
 // costs a second reading of y and z and a state.
-void plan(int batch, int steps, int heads, int dz, int* slices, int* segs, int* span) {
-    *slices = (dz + 63) / 64;
+void plan(int batch, int steps, int heads, int dz, int width, int* slices, int* segs, int* span) {
+    *slices = (dz + width - 1) / width;
     const long ctas = (long)batch * heads * *slices;
     const int chunks = steps > 0 ? (steps + C - 1) / C : 1;
     long want = ctas >= 148 ? 1 : (296 + ctas - 1) / ctas;
@@ -558,10 +570,13 @@ void plan(int batch, int steps, int heads, int dz, int* slices, int* segs, int* 
     *segs = (chunks + per - 1) / per;
 }
 
+// Columns of z a CTA takes: the float32 form's two sums of a wide product leave room for 32.
+int slice_width(bool f32, int dx) { return f32 && dx > 64 ? 32 : 64; }
+
 // The segments' states, for whichever form runs (a state in full precision needs its pass even over one segment).
 size_t seg_bytes(const ews_decay_args* a, int dx, int dz) {
     int slices, segs, span;
-    plan(a->batch, a->steps, a->heads, dz, &slices, &segs, &span);
+    plan(a->batch, a->steps, a->heads, dz, slice_width(a->dtype == EWS_DTYPE_F32, dx), &slices, &segs, &span);
     if (segs == 1) segs = 0;
     if (a->dtype == EWS_DTYPE_BF16) {
         const int t = tc_segments(a->batch, a->steps, a->heads, true, &span);
@@ -569,7 +584,7 @@ size_t seg_bytes(const ews_decay_args* a, int dx, int dz) {
         const int f = tc_segments(a->batch, a->steps, a->heads, false, &span);
         if (f > segs) segs = f;
     } else if (dx <= 64) {
-        const int f = tc_segments(a->batch, a->steps, a->heads * slices, false, &span);
+        const int f = tc_segments(a->batch, a->steps, a->heads * ((dz + 63) / 64), false, &span);
         if (f > segs && f > 1) segs = f;
     }
     return sizeof(float) * (size_t)a->batch * a->heads * segs * dx * dz;
@@ -589,15 +604,19 @@ int launch(const Chain<T>& a, cudaStream_t s) {
 
 template <typename T, int NS, bool STATE>
 int launch_d(const Chain<T>& a, cudaStream_t s) {
-    const int dk = pad_width(a.y.width);
-    if (a.z.width <= 32) {
-        if (dk == 32) return launch<T, 32, 32, NS, STATE>(a, s);
-        if (dk == 64) return launch<T, 64, 32, NS, STATE>(a, s);
+    [[maybe_unused]] const int dk = pad_width(a.y.width);
+    if constexpr (sizeof(T) == 4) {  // narrower x and y run in ews_decay_f32.cu
         return launch<T, 128, 32, NS, STATE>(a, s);
+    } else {
+        if (a.z.width <= 32) {
+            if (dk == 32) return launch<T, 32, 32, NS, STATE>(a, s);
+            if (dk == 64) return launch<T, 64, 32, NS, STATE>(a, s);
+            return launch<T, 128, 32, NS, STATE>(a, s);
+        }
+        if (dk == 32) return launch<T, 32, 64, NS, STATE>(a, s);
+        if (dk == 64) return launch<T, 64, 64, NS, STATE>(a, s);
+        return launch<T, 128, 64, NS, STATE>(a, s);
     }
-    if (dk == 32) return launch<T, 32, 64, NS, STATE>(a, s);
-    if (dk == 64) return launch<T, 64, 64, NS, STATE>(a, s);
-    return launch<T, 128, 64, NS, STATE>(a, s);
 }
 
 template <typename T>
@@ -646,7 +665,7 @@ int run_chain(Chain<T> a, cudaStream_t s) {
     } else {
         if (f32_fits(a)) return run_f32(a, s);
     }
-    plan(a.batch, a.steps, a.heads, a.z.width, &a.slices, &a.segs, &a.span);
+    plan(a.batch, a.steps, a.heads, a.z.width, slice_width(f32, a.y.width), &a.slices, &a.segs, &a.span);
     const bool exact = a.fin != nullptr && !f32;
     int rc;
     if (a.segs > 1) {

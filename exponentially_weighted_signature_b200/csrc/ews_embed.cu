@@ -6,7 +6,8 @@
 //
 // Gradient: the ids are sorted (stably, so every sum has one order and the result is bit-reproducible; no
 // float atomics), then every row of the table is written exactly once: zero where its token does not occur,
-// else the float32 sum of its rows, rounded once. Three launches:
+// else the float32 sum of its rows, rounded once. Up to 256 positions are looked through without a sort (few_kernel),
+// more take three launches:
 //   sort_kernel     least-significant-digit radix sort of (id, position), up to 9 bits a pass, in ONE cluster of
 //                   eight CTAs: the passes' steps are separated by the cluster's hardware barrier, where a
 //                   grid-wide sort would pay three launches a pass. It also marks each token's run.
@@ -329,6 +330,64 @@ __global__ void __launch_bounds__(128) rows_kernel(const T* __restrict__ dout, l
     }
 }
 
+// Few positions (a short list of ids): no sort, every warp looks through the ids for its four table rows, 32 at a time, and
+// adds what it finds in their order, four rows of dout in flight.
+constexpr int FEW = 256;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(128) few_kernel(const void* __restrict__ ids, int wide, int n, long vocab, long skip,
+                                                  const T* __restrict__ dout, long stride, int dim, float scale, int blocks,
+                                                  T* __restrict__ dtable) {
+    constexpr int W = Vec<T, VEC>::N, U = 4;
+    const int lane = threadIdx.x & 31;
+    const long unit = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const long group = unit / blocks;
+    const int cb = (int)(unit - group * blocks);
+    const long r0 = group * RROWS;
+    if (r0 >= vocab) return;
+    const int col = (cb * 32 + lane) * W;
+    const bool live = col < dim;
+    const T* from = dout + (live ? col : 0);
+    float acc[RROWS][W];
+#pragma unroll
+    for (int r = 0; r < RROWS; ++r)
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[r][k] = 0.f;
+    for (int s = 0; s < n; s += 32) {
+        const long id = s + lane < n ? load_id(ids, wide, s + lane) : -1;
+        const int rel = id != skip && id >= r0 && id < r0 + RROWS ? (int)(id - r0) : -1;
+        uint32_t found = __ballot_sync(kFull, rel >= 0);
+        while (found) {
+            int at[U];
+            const int many = min(U, __popc(found));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                at[u] = found ? __ffs(found) - 1 : at[0];
+                found &= found - 1;
+            }
+            float v[U][W];
+#pragma unroll
+            for (int u = 0; u < U; ++u) Vec<T, VEC>::load(from + (long)(s + at[u]) * stride, v[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = u < many ? __shfl_sync(kFull, rel, at[u]) : -1;
+#pragma unroll
+                for (int q = 0; q < RROWS; ++q)
+                    if (r == q)
+#pragma unroll
+                        for (int k = 0; k < W; ++k) acc[q][k] += v[u][k];
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RROWS; ++r)
+        if (live && r0 + r < vocab) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) acc[r][k] *= scale;
+            Vec<T, VEC>::store(dtable + (r0 + r) * dim + col, acc[r]);
+        }
+}
+
 // Segment length: 32 positions, and at least a quarter of sqrt(n), so that neither a segment nor the partials of
 // one run make a long chain.
 int seg_of(long n) {
@@ -344,6 +403,7 @@ struct Layout {
 Layout layout(long n, long vocab, long dim) {
     Layout l{};
     size_t at = 0;
+    if (n <= FEW) return l;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;
@@ -362,7 +422,14 @@ template <typename T, bool VEC>
 int backward(const SortArgs& sa, int ctas, const T* dout, long stride, int dim, float scale, const Layout& l, char* work,
              T* dtable, cudaStream_t s) {
     constexpr int W = Vec<T, VEC>::N;
-    if (sa.n > 0) {
+    if (sa.n <= FEW) {
+        const int blocks = (dim + 32 * W - 1) / (32 * W);
+        const long units = (sa.vocab + RROWS - 1) / RROWS * blocks;
+        few_kernel<T, VEC><<<(unsigned)((units + 3) / 4), 128, 0, s>>>(sa.ids, sa.wide, sa.n, sa.vocab, sa.skip, dout, stride, dim, scale,
+                                                                      blocks, dtable);
+        return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
+    }
+    {
         cudaLaunchConfig_t cfg{};
         if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SORT_BYTES) != cudaSuccess) return EWS_ERR_LAUNCH;
         cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(ST), cfg.stream = s, cfg.dynamicSmemBytes = SORT_BYTES;
@@ -371,8 +438,6 @@ int backward(const SortArgs& sa, int ctas, const T* dout, long stride, int dim, 
         at.val.clusterDim.x = ctas, at.val.clusterDim.y = at.val.clusterDim.z = 1;
         cfg.attrs = &at, cfg.numAttrs = 1;
         if (cudaLaunchKernelEx(&cfg, sort_kernel, sa, ctas) != cudaSuccess) return EWS_ERR_LAUNCH;
-    } else if (cudaMemsetAsync(sa.runs, 0, sizeof(int2) * sa.vocab, s) != cudaSuccess) {
-        return EWS_ERR_LAUNCH;
     }
     const bool odd = sa.passes & 1;  // the sorted order is in the second buffers after an odd number of passes
     const uint32_t *key = odd ? sa.key1 : sa.key0, *pos = odd ? sa.pos1 : sa.pos0;
@@ -436,7 +501,7 @@ extern "C" int ews_embed_bwd(const void* ids, int ids_wide, const void* dout, in
     if (dtype != EWS_DTYPE_F32 && dtype != EWS_DTYPE_BF16) return EWS_ERR_UNSUPPORTED;
     if (!dtable || (n > 0 && (!ids || !dout))) return EWS_ERR_INVALID_ARGUMENT;
     const Layout l = layout(n, vocab, dim);
-    if (!work || work_bytes < l.bytes) return EWS_ERR_WORKSPACE;
+    if (l.bytes && (!work || work_bytes < l.bytes)) return EWS_ERR_WORKSPACE;
     char* w = static_cast<char*>(work);
     SortArgs a{};
     a.ids = ids, a.wide = ids_wide, a.n = (int)n, a.vocab = vocab, a.skip = skip, a.status = status;

@@ -140,8 +140,8 @@ class _Embedding(torch.autograd.Function):
         grad = torch.empty((vocab, dim), dtype=dout.dtype, device=dout.device)
         work = _work(_embed_size(n, vocab, dim), dout)
         _launch(dout.get_device(), "ews_embed_bwd", n, lib.ews_embed_bwd, flat.data_ptr(), _WIDE[flat.dtype], g.data_ptr(),
-                _DTYPES[dout.dtype], n, vocab, dim, _row_stride(g), scale, padding_index, grad.data_ptr(), work.data_ptr(),
-                work.numel(), None)
+                _DTYPES[dout.dtype], n, vocab, dim, _row_stride(g), scale, padding_index, grad.data_ptr(), _addr(work),
+                0 if work is None else work.numel(), None)
         return None, grad, None, None, None
 
 
