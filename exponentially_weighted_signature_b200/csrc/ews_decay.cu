@@ -465,17 +465,29 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chain
     if (a.fin) a.fin[bh * per + i * a.fin_r + j * a.fin_c] = s * a.fin_scale;
 }
 
-// Sums the float32 gradients of the query heads that share a key/value head, in head order.
-template <typename T>
+// Sums the float32 gradients of the query heads that share a key/value head, in head order: a thread a vector of one
+// head, the vectors of a row side by side.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) group_kernel(const float* __restrict__ in, long rows, int kv, int group, int d,
                                                     T* __restrict__ out) {
-    const long total = rows * kv * d;
+    constexpr int W = VEC ? 4 : 1;
+    const int per = d / W;
+    const long total = rows * kv * per;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        const long rk = e / d;
-        const float* p = in + rk * group * d + (e - rk * d);
-        float s = 0.f;
-        for (int g = 0; g < group; ++g) s += p[(long)g * d];
-        out[e] = from_f<T>(s);
+        const long rk = e / per;
+        const int c = (int)(e - rk * per) * W;
+        const float* p = in + rk * group * d + c;
+        float s[W];
+        Vec<float, VEC>::load(p, s);
+        for (int g = 1; g < group; ++g) {
+            float v[W];
+            Vec<float, VEC>::load(p + (long)g * d, v);
+#pragma unroll
+            for (int j = 0; j < W; ++j) s[j] += v[j];
+        }
+        T* o = out + rk * d + c;
+        if constexpr (VEC && sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+        else Vec<T, VEC>::store(o, s);
     }
 }
 
@@ -750,9 +762,11 @@ int backward(const ews_decay_args* a, const Sizes& z, cudaStream_t s) {
     const long rows = (long)a->batch * a->steps;
     auto sum = [&](int d, void* out) {
         if (!part) return (int)EWS_OK;
-        const long blocks = (rows * a->kv_heads * d + 255) / 256;
-        group_kernel<T><<<(unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, s>>>(part, rows, a->kv_heads, group, d,
-                                                                                         static_cast<T*>(out));
+        const bool vec = d % 4 == 0 && aligned16(out);
+        const long blocks = (rows * a->kv_heads * d / (vec ? 4 : 1) + 255) / 256;
+        const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks < 148 * 64 ? blocks : 148 * 64);
+        if (vec) group_kernel<T, true><<<grid, 256, 0, s>>>(part, rows, a->kv_heads, group, d, static_cast<T*>(out));
+        else group_kernel<T, false><<<grid, 256, 0, s>>>(part, rows, a->kv_heads, group, d, static_cast<T*>(out));
         return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
     };
     // dq: forwards, the state transposed

@@ -31,6 +31,9 @@ constexpr int EPW = 8;                 // epilogue warps
 constexpr int NTH = 64 + EPW * 32;     // and one each for TMA and MMA
 constexpr int SMS = 148;
 constexpr long kPieceElems = 1l << 27; // entries of G (times planes) at a time: 256 MB
+// Every addition to the tensor core's accumulator truncates (2^-24 of the sum, always towards zero), and a gradient's sum
+// is long: for float32 a tile's sum leaves the accumulator every 256 of K and is added, rounded, to the float32 partial.
+constexpr int kRun = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^x: the exponent unit's own instruction, results below the normal range to zero.
@@ -58,6 +61,7 @@ struct Gemm {
     Job job[2];           // OUT: dH (A = G, K-major) and dW (A = G, MN-major) in one launch; else job[0]
     int pairs;
     signed char ia[6], ib[6];
+    int run;              // k blocks in one accumulator: the whole range, or few (float32 gradients, see kRun)
     int* status;          // the caller's word: a bounded wait that ran out
     const int* live;      // rows that have a target: the logits' m, dH's m, dW's k
     int f32;              // the inputs are float32
@@ -152,25 +156,27 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 const Unit r = unit(u);
                 const CUtensorMap *ta = &maps.a[r.job], *tb = &maps.b[r.job];
                 const bool amn = EPI == OUT && r.job == 1;
-                for (int p = 0; ok && p < a.pairs; ++p)
-                    for (int kb = r.k0; kb < r.k1; ++kb, ++it) {
-                        const int s = (int)(it % S);
-                        if (!(ok = mbar_wait(empty + s, (uint32_t)((it / S) & 1) ^ 1u, fail))) break;
-                        unsigned char* at = tiles + s * TL::STAGE;
-                        mbar_expect(full + s, TL::STAGE);
-                        if (amn) {
-                            for (int j = 0; j < BM / 64; ++j)
-                                tma_load(ta, full + s, at + j * 8192, r.tm * BM + j * 64, kb * BK, a.ia[p]);
-                        } else {
-                            tma_load(ta, full + s, at, kb * BK, r.tm * BM, a.ia[p]);
+                for (int from = r.k0; ok && from < r.k1; from += a.run) {
+                    for (int p = 0; ok && p < a.pairs; ++p)
+                        for (int kb = from; kb < min(from + a.run, r.k1); ++kb, ++it) {
+                            const int s = (int)(it % S);
+                            if (!(ok = mbar_wait(empty + s, (uint32_t)((it / S) & 1) ^ 1u, fail))) break;
+                            unsigned char* at = tiles + s * TL::STAGE;
+                            mbar_expect(full + s, TL::STAGE);
+                            if (amn) {
+                                for (int j = 0; j < BM / 64; ++j)
+                                    tma_load(ta, full + s, at + j * 8192, r.tm * BM + j * 64, kb * BK, a.ia[p]);
+                            } else {
+                                tma_load(ta, full + s, at, kb * BK, r.tm * BM, a.ia[p]);
+                            }
+                            if (BMN) {
+                                for (int j = 0; j < BN / 64; ++j)
+                                    tma_load(tb, full + s, at + TL::A + j * 8192, r.tn * BN + j * 64, kb * BK, a.ib[p]);
+                            } else {
+                                tma_load(tb, full + s, at + TL::A, kb * BK, r.tn * BN, a.ib[p]);
+                            }
                         }
-                        if (BMN) {
-                            for (int j = 0; j < BN / 64; ++j)
-                                tma_load(tb, full + s, at + TL::A + j * 8192, r.tn * BN + j * 64, kb * BK, a.ib[p]);
-                        } else {
-                            tma_load(tb, full + s, at + TL::A, kb * BK, r.tn * BN, a.ib[p]);
-                        }
-                    }
+                }
             }
             if (!ok)
                 for (long j = it > S ? it - S : 0; j < it; ++j) mbar_drain(full + j % S, (uint32_t)((j / S) & 1));
@@ -180,34 +186,37 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
         uint32_t ph = 0;
         long tile = 0;
         bool ok = true;
-        for (long u = blockIdx.x; ok && u < units; u += gridDim.x, ++tile) {
+        for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
             const Unit r = unit(u);
             const bool amn = EPI == OUT && r.job == 1;
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((amn ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
                                    ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
             const uint32_t astep = amn ? 2048 >> 4 : 32 >> 4, bstep = BMN ? 2048 >> 4 : 32 >> 4;
-            const int buf = (int)(tile & 1);
-            if (!(ok = warp_wait(acc_empty + buf, (uint32_t)((tile >> 1) & 1) ^ 1u, fail))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int steps = a.pairs * max(r.k1 - r.k0, 0);
-            const uint64_t ad0 = desc(smem_u32(tiles), amn), bd0 = desc(smem_u32(tiles) + TL::A, BMN);
-            for (int i = 0; i < steps; ++i) {
-                if (!(ok = warp_wait(full + s, ph, fail))) break;
+            // a range of no blocks passes an empty accumulator on, once
+            for (int from = r.k0; ok && (from == r.k0 || from < r.k1); from += a.run, ++tile) {
+                const int buf = (int)(tile & 1);
+                if (!(ok = warp_wait(acc_empty + buf, (uint32_t)((tile >> 1) & 1) ^ 1u, fail))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) {
-                    const uint64_t ad = ad0 + s * (TL::STAGE >> 4), bd = bd0 + s * (TL::STAGE >> 4);
+                const int steps = a.pairs * max(min(from + a.run, r.k1) - from, 0);
+                const uint64_t ad0 = desc(smem_u32(tiles), amn), bd0 = desc(smem_u32(tiles) + TL::A, BMN);
+                for (int i = 0; i < steps; ++i) {
+                    if (!(ok = warp_wait(full + s, ph, fail))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
+                        const uint64_t ad = ad0 + s * (TL::STAGE >> 4), bd = bd0 + s * (TL::STAGE >> 4);
 #pragma unroll
-                    for (int q = 0; q < BK / 16; ++q)
-                        mma_bf16(tmem + buf * BN, ad + q * astep, bd + q * bstep, idesc, i > 0 || q > 0);
-                    mma_commit(empty + s);
-                    if (i == steps - 1) mma_commit(acc_full + buf);
+                        for (int q = 0; q < BK / 16; ++q)
+                            mma_bf16(tmem + buf * BN, ad + q * astep, bd + q * bstep, idesc, i > 0 || q > 0);
+                        mma_commit(empty + s);
+                        if (i == steps - 1) mma_commit(acc_full + buf);
+                    }
+                    __syncwarp();
+                    if (++s == S) s = 0, ph ^= 1u;
                 }
-                __syncwarp();
-                if (++s == S) s = 0, ph ^= 1u;
-            }
-            if (ok && steps == 0) {
-                if (elect_one()) mma_commit(acc_full + buf);
-                __syncwarp();
+                if (ok && steps == 0) {
+                    if (elect_one()) mma_commit(acc_full + buf);
+                    __syncwarp();
+                }
             }
         }
         if (!ok) {
@@ -219,170 +228,179 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
         // two warps share a quarter of the rows, each has half of the tile's columns
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         long tile = 0;
-        for (long u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
+        bool ok = true;
+        for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
             const Unit r = unit(u);
             const Job& job = a.job[r.job];
-            const int buf = (int)(tile & 1);
-            if (!__all_sync(kFull, mbar_wait(acc_full + buf, (uint32_t)((tile >> 1) & 1), fail))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
-            const int row = r.tm * BM + quarter * 32 + lane;
-            const bool in = row < (r.job ? job.m : m0);
-            const int cols = min(half * HALF + HALF, job.n - r.tn * BN);
-            if (EPI == LSE) {
-                const int pick = in ? a.target[row] - a.v0 - r.tn * BN : -1;
-                float mx = -INFINITY, sum = 0.f;
-                for (int c = half * HALF; c < cols; c += 32) {
-                    float v[32];
-                    tmem_ld32(src + c, v);
-                    if (c + 32 > cols) {
+            for (int from = r.k0; from == r.k0 || from < r.k1; from += a.run, ++tile) {
+                const int buf = (int)(tile & 1);
+                if (!(ok = __all_sync(kFull, mbar_wait(acc_full + buf, (uint32_t)((tile >> 1) & 1), fail)))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t src = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
+                const int row = r.tm * BM + quarter * 32 + lane;
+                const bool in = row < (r.job ? job.m : m0);
+                const int cols = min(half * HALF + HALF, job.n - r.tn * BN);
+                const bool add = job.add || from > r.k0;
+                if (EPI == LSE) {
+                    const int pick = in ? a.target[row] - a.v0 - r.tn * BN : -1;
+                    float mx = -INFINITY, sum = 0.f;
+                    for (int c = half * HALF; c < cols; c += 32) {
+                        float v[32];
+                        tmem_ld32(src + c, v);
+                        if (c + 32 > cols) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c + j >= cols) v[j] = -INFINITY;
+                            for (int j = 0; j < 32; ++j)
+                                if (c + j >= cols) v[j] = -INFINITY;
+                        }
+                        float top = v[0];
+#pragma unroll
+                        for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+                        const float was = mx;
+                        mx = fmaxf(mx, top);
+                        const float shift = mx == -INFINITY ? 0.f : -mx * kLog2e;
+                        const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float e0, e1;
+                            unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
+                            part[j & 3] += ex2(e0), part[(j & 3) + 1] += ex2(e1);
+                        }
+                        sum = sum * exp2f(fmaf(was, kLog2e, shift)) + ((part[0] + part[1]) + (part[2] + part[3]));
+                        if ((unsigned)(pick - c) < 32u) {
+                            float z = 0.f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) z = pick - c == j ? v[j] : z;
+                            a.picked[row] = z;
+                        }
                     }
-                    float top = v[0];
-#pragma unroll
-                    for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
-                    const float was = mx;
-                    mx = fmaxf(mx, top);
-                    const float shift = mx == -INFINITY ? 0.f : -mx * kLog2e;
+                    if (in) a.part[(long)((a.part_tile0 + r.tn) * 2 + half) * job.m + row] = make_float2(mx, sum);
+                } else if (EPI == GRAD) {
+                    const int t = in ? a.target[row] : -1;
+                    const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
+                    const float w = t < 0 ? 0.f : a.dloss[a.row[row]];
+                    const float lse = in ? a.lse[row] : 0.f, shift = -lse * kLog2e;
                     const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int c = half * HALF; c < cols; c += 32) {
+                        float v[32];
+                        tmem_ld32(src + c, v);
+                        if (a.planes > 1) {  // float32: the scaled exponent's own rounding (2^-24 of some 15) would be the largest error
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float e0, e1;
-                        unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
-                        part[j & 3] += ex2(e0), part[(j & 3) + 1] += ex2(e1);
-                    }
-                    sum = sum * exp2f(fmaf(was, kLog2e, shift)) + ((part[0] + part[1]) + (part[2] + part[3]));
-                    if ((unsigned)(pick - c) < 32u) {
-                        float z = 0.f;
+                            for (int j = 0; j < 32; ++j) v[j] = expf(v[j] - lse);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) z = pick - c == j ? v[j] : z;
-                        a.picked[row] = z;
-                    }
-                }
-                if (in) a.part[(long)((a.part_tile0 + r.tn) * 2 + half) * job.m + row] = make_float2(mx, sum);
-            } else if (EPI == GRAD) {
-                const int t = in ? a.target[row] : -1;
-                const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
-                const float w = t < 0 ? 0.f : a.dloss[a.row[row]];
-                const float shift = in ? -a.lse[row] * kLog2e : 0.f;
-                const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
-                for (int c = half * HALF; c < cols; c += 32) {
-                    float v[32];
-                    tmem_ld32(src + c, v);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float e0, e1;
-                        unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
-                        v[j] = ex2(e0), v[j + 1] = ex2(e1);
-                    }
-                    if ((unsigned)(pick - c) < 32u) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] -= pick - c == j ? 1.f : 0.f;
-                    }
-                    if (t >= 0) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= w;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0.f;
-                    }
-                    if (c + 32 > cols) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c + j >= cols) v[j] = 0.f;
-                    }
-                    if (a.planes == 1) {
-                        // through shared memory (rows of 64 columns, swizzled) and out by TMA, which drops what lies
-                        // beyond the matrix: stored from the registers, a warp's 32 rows at 16 bytes each took
-                        // the logits' pass from 1.46 to 1.09 PFLOP/s
-                        unsigned char* box = tiles + S * TL::STAGE + (warp - 2) * TL::OUTW;
-                        if ((c & 32) == 0) {
-                            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                            __syncwarp();
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            Vec<bf16, true>::store(reinterpret_cast<bf16*>(box + lane * 128 + (((c & 32) / 8 + j) ^ (lane & 7)) * 16), v + 8 * j);
-                        if ((c & 32) || c + 32 >= cols) {
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) {
-                                tma_store(&maps.g, box, r.tn * BN + (c & ~63), r.tm * BM + quarter * 32, 0);
-                                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                            for (int j = 0; j < 32; j += 2) {
+                                float e0, e1;
+                                unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
+                                v[j] = ex2(e0), v[j + 1] = ex2(e1);
                             }
                         }
-                        continue;
-                    }
-                    for (int s = 0; row < job.m && s < a.planes; ++s) {  // rows that are none: zeros
-                        bf16* g = a.g + s * a.g_plane + (long)row * a.ldg + r.tn * BN + c;
+                        if ((unsigned)(pick - c) < 32u) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            uint32_t q[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                q[e] = pack_bf16(v[j + 2 * e], v[j + 2 * e + 1]);
-                                v[j + 2 * e] -= bf16_lo(q[e]), v[j + 2 * e + 1] -= bf16_hi(q[e]);
-                            }
-                            if (r.tn * BN + c + j < a.ldg) *reinterpret_cast<uint4*>(g + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                            for (int j = 0; j < 32; ++j) v[j] -= pick - c == j ? 1.f : 0.f;
                         }
-                    }
-                }
-            } else {
-                for (int c = half * HALF; c < cols; c += 32) {
-                    float v[32];
-                    tmem_ld32(src + c, v);
-                    if (r.k0 >= r.k1) {
+                        if (t >= 0) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0.f;
-                    }
-                    const int col = r.tn * BN + c;
-                    const int w = min(32, cols - c);
-                    if (!in) {
-                    } else if (job.acc) {
-                        float* p = job.acc + ((long)r.sp * job.m + row) * job.n + col;
-                        if (w == 32 && (job.n & 3) == 0) {
+                            for (int j = 0; j < 32; ++j) v[j] *= w;
+                        } else {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                float4 q = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                                if (job.add) {
-                                    const float4 o = *reinterpret_cast<const float4*>(p + j);
-                                    q.x += o.x, q.y += o.y, q.z += o.z, q.w += o.w;
+                            for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                        }
+                        if (c + 32 > cols) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (c + j >= cols) v[j] = 0.f;
+                        }
+                        if (a.planes == 1) {
+                            // through shared memory (rows of 64 columns, swizzled) and out by TMA, which drops what lies
+                            // beyond the matrix: stored from the registers, a warp's 32 rows at 16 bytes each took
+                            // the logits' pass from 1.46 to 1.09 PFLOP/s
+                            unsigned char* box = tiles + S * TL::STAGE + (warp - 2) * TL::OUTW;
+                            if ((c & 32) == 0) {
+                                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                                __syncwarp();
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                Vec<bf16, true>::store(reinterpret_cast<bf16*>(box + lane * 128 + (((c & 32) / 8 + j) ^ (lane & 7)) * 16), v + 8 * j);
+                            if ((c & 32) || c + 32 >= cols) {
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                                if (lane == 0) {
+                                    tma_store(&maps.g, box, r.tn * BN + (c & ~63), r.tm * BM + quarter * 32, 0);
+                                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                                 }
-                                *reinterpret_cast<float4*>(p + j) = q;
+                            }
+                            continue;
+                        }
+                        for (int s = 0; row < job.m && s < a.planes; ++s) {  // rows that are none: zeros
+                            bf16* g = a.g + s * a.g_plane + (long)row * a.ldg + r.tn * BN + c;
+#pragma unroll
+                            for (int j = 0; j < 32; j += 8) {
+                                uint32_t q[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    q[e] = pack_bf16(v[j + 2 * e], v[j + 2 * e + 1]);
+                                    v[j + 2 * e] -= bf16_lo(q[e]), v[j + 2 * e + 1] -= bf16_hi(q[e]);
+                                }
+                                if (r.tn * BN + c + j < a.ldg) *reinterpret_cast<uint4*>(g + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                            }
+                        }
+                    }
+                } else {
+                    for (int c = half * HALF; c < cols; c += 32) {
+                        float v[32];
+                        tmem_ld32(src + c, v);
+                        if (r.k0 >= r.k1) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                        }
+                        const int col = r.tn * BN + c;
+                        const int w = min(32, cols - c);
+                        if (!in) {
+                        } else if (job.acc) {
+                            float* p = job.acc + ((long)r.sp * job.m + row) * job.n + col;
+                            if (w == 32 && (job.n & 3) == 0) {
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) {
+                                    float4 q = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                                    if (add) {
+                                        const float4 o = *reinterpret_cast<const float4*>(p + j);
+                                        q.x += o.x, q.y += o.y, q.z += o.z, q.w += o.w;
+                                    }
+                                    *reinterpret_cast<float4*>(p + j) = q;
+                                }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j < w) p[j] = add ? p[j] + v[j] : v[j];
+                            }
+                        } else if (a.f32) {
+                            float* p = static_cast<float*>(job.out) + (long)row * job.n + col;
+                            if (w == 32 && (job.n & 3) == 0 && aligned16_dev(job.out)) {
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j < w) p[j] = v[j];
                             }
                         } else {
+                            bf16* p = static_cast<bf16*>(job.out) + (long)row * job.n + col;
+                            if (w == 32 && (job.n & 7) == 0 && aligned16_dev(job.out)) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j < w) p[j] = job.add ? p[j] + v[j] : v[j];
-                        }
-                    } else if (a.f32) {
-                        float* p = static_cast<float*>(job.out) + (long)row * job.n + col;
-                        if (w == 32 && (job.n & 3) == 0 && aligned16_dev(job.out)) {
+                                for (int j = 0; j < 32; j += 8) Vec<bf16, true>::store(p + j, v + j);
+                            } else {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j < w) p[j] = v[j];
-                        }
-                    } else {
-                        bf16* p = static_cast<bf16*>(job.out) + (long)row * job.n + col;
-                        if (w == 32 && (job.n & 7) == 0 && aligned16_dev(job.out)) {
-#pragma unroll
-                            for (int j = 0; j < 32; j += 8) Vec<bf16, true>::store(p + j, v + j);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j < w) p[j] = from_f<bf16>(v[j]);
+                                for (int j = 0; j < 32; ++j)
+                                    if (j < w) p[j] = from_f<bf16>(v[j]);
+                            }
                         }
                     }
                 }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive(acc_empty + buf);
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(acc_empty + buf);
         }
         if (EPI == GRAD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
@@ -622,6 +640,7 @@ int gemm(Gemm g, const Operand& a0, const Operand& b0, const Operand& a1, const 
     if (EPI == GRAD && planes == 1 &&
         !make_map(&m.g, Operand{g.g, g.job[0].m, g.job[0].n, g.ldg, 0, 1}, 32))
         return EWS_ERR_LAUNCH;
+    g.run = EPI == OUT && planes > 1 ? kRun : 1 << 28;
     const int bn = tile_n(g.job[0].units ? g.job[0].n : g.job[1].n);
     if (g.job[0].units && (!make_map(&m.a[0], a0, BM) || !make_map(&m.b[0], b0, EPI == OUT ? 64 : bn))) return EWS_ERR_LAUNCH;
     if (g.job[1].units && (!make_map(&m.a[1], a1, 64) || !make_map(&m.b[1], b1, 64))) return EWS_ERR_LAUNCH;
@@ -698,7 +717,7 @@ Plan plan(const ews_vocab_args* a, bool bwd) {
         const long tw = ((p.piece + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
         p.split_h = splits_of(n, a->dim, p.piece, tw);
         p.split_w = splits_of(p.piece, a->dim, n, th * p.split_h);
-        p.acc_w = p.split_w > 1;
+        p.acc_w = p.split_w > 1 || p.planes > 1;
         p.ah = take(sizeof(float) * (size_t)p.split_h * n * a->dim);
         if (p.acc_w) p.aw = take(sizeof(float) * (size_t)p.split_w * p.piece * a->dim);
     }
