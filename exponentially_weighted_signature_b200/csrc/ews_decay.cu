@@ -12,8 +12,15 @@
 // Backwards the carried value is E = g R of the token behind, so that the last state's gradient enters
 // unweighted: a row's weight of the carry is g^i, not g^(i+1), an update's g^(n-j), not g^(n-1-j).
 //
-// chain_kernel: a CTA of four warps owns a (sample, head, segment of the axis, slice of up to 64 columns of z); it walks its segment
-// in chunks of 64 tokens with the state in registers (float32). Within a chunk out = P Z + diag(g^(i+1)) X State,
+// Which form runs: bfloat16 streams that TMA can read (16-byte-aligned rows and strides) run in ews_decay_tc.cu, float32
+// with x and y up to 64 wide in ews_decay_f32.cu, both on the 5th-generation tensor core; the rest (odd bfloat16 widths and
+// strides, wide float32 heads) here, on warp-level matrix instructions. Both sides of each rule, forward and backward:
+// bfloat16 B = 8, T = 2048, 16 heads of 128: 269 us there, 857 here; float32 B = 16, T = 1440, 8 heads of 64, shared in
+// pairs, ragged: 522 us there, 1,717 here. What bounds this form is the legacy instructions' rate (2,048 operations a
+// cycle and SM) and the splitting of float32 fragments, each of which four warps repeat.
+//
+// chain_kernel: a CTA of four warps owns a (sample, head, segment of the axis, slice of up to 64 columns of z); it walks
+// its segment in chunks of 64 tokens with the state in registers (float32). Within a chunk out = P Z + diag(g^(i+1)) X State,
 // P = (X Y^T) * g^(i-j) for j <= i: warp-level matrix instructions, P straight from the accumulators to operand
 // fragments, the state rounded to the operand type for its product alone. The update (g^(n-1-j) y_j) z_j^T splits
 // the weighted operand into `NS` bfloat16 pieces: the weight makes it inexact, and the state is a float32 result
@@ -494,7 +501,8 @@ __global__ void __launch_bounds__(256) group_kernel(const float* __restrict__ in
 // ---- one token per row ----------------------------------------------------------------------------------------
 // A CTA owns 64 columns of one (row, head) state: 16 lanes of four columns by 16 groups of state rows; each thread
 // reads, decays, updates and writes its part of the state once and sums its rows of q S; the groups' sums meet in
-// shared memory. Bound by HBM (8 bytes a state entry) for full batches and by one trip to memory for few rows.
+// shared memory. Bound by HBM (8 bytes a state entry) for full batches and by one trip to memory for few rows: 256 rows of
+// 16 heads of 128 x 128 (530 MB) take 96 us, 5.5 TB/s (on 32 columns a CTA 110 us); 8 heads of 64 x 64 take 6 us.
 constexpr int STEP_T = 256, STEP_COLS = 64;
 
 template <typename T>
@@ -690,13 +698,15 @@ int run_chain(Chain<T> a, cudaStream_t s) {
 }
 
 template <typename T>
-Stream<T> stream_of(const void* p, const int64_t st[3], int group, int width) {
+Stream<T> stream_of(const ews_decay_args* a, const void* p, const int64_t st[3], int group, int width) {
     Stream<T> s{};
     s.p = static_cast<const T*>(p);
     s.sb = st[0], s.st = st[1], s.sh = st[2];
     s.group = group, s.width = width;
     constexpr int E = 16 / sizeof(T);
-    s.vec = aligned16(p) && width % E == 0 && s.sb % E == 0 && s.st % E == 0 && s.sh % E == 0;
+    // an axis of one has no stride to speak of
+    s.vec = aligned16(p) && width % E == 0 && (a->batch == 1 || s.sb % E == 0) && (a->steps == 1 || s.st % E == 0) &&
+            (a->heads == group || s.sh % E == 0);
     return s;
 }
 
@@ -742,9 +752,9 @@ template <typename T>
 int forward(const ews_decay_args* a, cudaStream_t s) {
     const int group = a->heads / a->kv_heads;
     Chain<T> c = base<T>(a);
-    c.x = stream_of<T>(a->q, a->q_stride, 1, a->dk);
-    c.y = stream_of<T>(a->k, a->k_stride, group, a->dk);
-    c.z = stream_of<T>(a->v, a->v_stride, group, a->dv);
+    c.x = stream_of<T>(a, a->q, a->q_stride, 1, a->dk);
+    c.y = stream_of<T>(a, a->k, a->k_stride, group, a->dk);
+    c.z = stream_of<T>(a, a->v, a->v_stride, group, a->dv);
     c.out = static_cast<T*>(a->out);
     c.init = a->initial, c.fin = a->final_state;
     c.init_r = c.fin_r = a->dv, c.init_c = c.fin_c = 1;
@@ -754,10 +764,10 @@ int forward(const ews_decay_args* a, cudaStream_t s) {
 template <typename T>
 int backward(const ews_decay_args* a, const Sizes& z, cudaStream_t s) {
     const int group = a->heads / a->kv_heads;
-    const auto q = stream_of<T>(a->q, a->q_stride, 1, a->dk);
-    const auto k = stream_of<T>(a->k, a->k_stride, group, a->dk);
-    const auto v = stream_of<T>(a->v, a->v_stride, group, a->dv);
-    const auto g = stream_of<T>(a->dout, a->dout_stride, 1, a->dv);
+    const auto q = stream_of<T>(a, a->q, a->q_stride, 1, a->dk);
+    const auto k = stream_of<T>(a, a->k, a->k_stride, group, a->dk);
+    const auto v = stream_of<T>(a, a->v, a->v_stride, group, a->dv);
+    const auto g = stream_of<T>(a, a->dout, a->dout_stride, 1, a->dv);
     float* part = group > 1 ? reinterpret_cast<float*>(static_cast<char*>(a->work) + z.seg) : nullptr;
     const long rows = (long)a->batch * a->steps;
     auto sum = [&](int d, void* out) {

@@ -7,12 +7,20 @@
 //     O2 = P Z              (tokens x dz)          -> out = g^(i+1) O1 + O2
 //
 // One persistent CTA per SM walks (sample, head, segment) items. Warp 0 fetches tiles by TMA, warp 1 issues the
-// products, warps 2-5 (A) turn P into an operand, warps 6-13 (B) weight Y (in place, and its rounding residue
-// beside it: the weighted operand is inexact, two bfloat16 pieces carry it to 2^-16, three to 2^-24), write the
-// output of the chunk before, keep the state and write its bfloat16 copy. The only chain from chunk to chunk is
-// U -> State -> O1; the loads, P and the output of neighbouring chunks run beside it.
+// products, warps 2-5 (A) turn P into an operand and write the output, warps 6-13 (B) weight Y (in place, and its
+// rounding residue beside it: the weighted operand is inexact, two bfloat16 pieces carry it to 2^-16, three to 2^-24),
+// keep the state and write its bfloat16 copy. The only chain from chunk to chunk is U -> State -> O1; the loads, P and the
+// output of neighbouring chunks run beside it.
 // X, whose last product of a chunk (O1) is issued a chunk ahead, has one buffer, Y and Z two.
 // Why 128 tokens: the accumulator has 128 rows; the waste of the upper half of P is 1/10 of a chunk's products.
+//
+// Measured: one chain over B = 8, T = 2048, 16 heads of 128 (268 MB of streams) 62 us, 4.3 TB/s, two thirds of the copy
+// bandwidth, on 128 of the 148 SMs; a chunk takes 5,400 cycles of a CTA, of which its products are 2,600 and its traffic
+// 4,800 at the copy bandwidth. What bounds it is group A: its scores (1,500), the wait for O2 (1,100) and the output
+// (2,300) follow one another, and a role's instructions come slowly (its code runs once a chunk, and the roles' code
+// together is larger than the inner instruction cache: unrolled loops lost more than they gained). A third group for
+// the output took 96 registers a thread and spilled: 329 us for the training case instead of 290 at the time.
+// The states' pass over 17,984 tokens of 16 heads (three pieces) takes 62 us, the outputs' 74 us.
 //
 // Reversed chains keep the rows' order and walk the chunks down: decays are then g^(j-i) for j >= i, a row's weight of
 // the carry g^(n-1-i), an update's g^(j+1).

@@ -16,7 +16,9 @@
 //                   to a float32 partial row, at most two per segment.
 //   rows_kernel     one warp per 16 x 32 bytes of four table rows: sums a run inside one segment directly, a
 //                   longer one from its partials in order.
-// Bound by HBM: N rows read, V rows written.
+// Bound by HBM: N rows read, V rows written. Measured for N = 65,536, V = 131,072, D = 512, float32: the lookup 37 us
+// (268 MB), the sort 41 us, the partials 17 us, the rows 71 us (402 MB, 5.7 TB/s); the sort is bound by its rounds of
+// rank and scatter on eight SMs (one CTA instead of eight: 23 us for 1,024 positions, 18 with eight).
 #include "ews_token.cuh"
 
 namespace ews {
@@ -81,7 +83,8 @@ __device__ __forceinline__ void cluster_sync() {
 // Stable: the CTAs, their warps and a warp's rounds of 32 items take the items in order, a lane's rank within a
 // round counts the lower lanes of the same digit. A warp whose items fit its registers (up to 65,536 in all) reads
 // them once a pass.
-__global__ void __launch_bounds__(ST) sort_kernel(SortArgs a, int ctas) {
+__global__ void __launch_bounds__(ST) sort_kernel(SortArgs a) {
+    constexpr int ctas = SCL;
     extern __shared__ uint32_t shared[];
     uint32_t* hist = shared;                 // SW x digits
     uint32_t* base = hist + SW * SD;         // digits
@@ -155,7 +158,7 @@ __global__ void __launch_bounds__(ST) sort_kernel(SortArgs a, int ctas) {
         if (tid < digits) {
             uint32_t t[SCL];
 #pragma unroll
-            for (int c = 0; c < SCL; ++c) t[c] = c < ctas ? __ldcg(a.totals + c * SD + tid) : 0u;
+            for (int c = 0; c < SCL; ++c) t[c] = __ldcg(a.totals + c * SD + tid);
 #pragma unroll
             for (int c = 0; c < SCL; ++c) {
                 all += t[c];
@@ -331,7 +334,8 @@ __global__ void __launch_bounds__(128) rows_kernel(const T* __restrict__ dout, l
 }
 
 // Few positions (a short list of ids): no sort, every warp looks through the ids for its four table rows, 32 at a time, and
-// adds what it finds in their order, four rows of dout in flight.
+// adds what it finds in their order, four rows of dout in flight. For V = 50,257, D = 768, bfloat16 against the three
+// kernels of the sorted form: 64 positions 17 and 41 us, 256 positions 30 and 42 us, 1,024 positions 87 and 44 us.
 constexpr int FEW = 256;
 
 template <typename T, bool VEC>
@@ -419,7 +423,7 @@ Layout layout(long n, long vocab, long dim) {
 }
 
 template <typename T, bool VEC>
-int backward(const SortArgs& sa, int ctas, const T* dout, long stride, int dim, float scale, const Layout& l, char* work,
+int backward(const SortArgs& sa, const T* dout, long stride, int dim, float scale, const Layout& l, char* work,
              T* dtable, cudaStream_t s) {
     constexpr int W = Vec<T, VEC>::N;
     if (sa.n <= FEW) {
@@ -432,12 +436,12 @@ int backward(const SortArgs& sa, int ctas, const T* dout, long stride, int dim, 
     {
         cudaLaunchConfig_t cfg{};
         if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SORT_BYTES) != cudaSuccess) return EWS_ERR_LAUNCH;
-        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(ST), cfg.stream = s, cfg.dynamicSmemBytes = SORT_BYTES;
+        cfg.gridDim = dim3(SCL), cfg.blockDim = dim3(ST), cfg.stream = s, cfg.dynamicSmemBytes = SORT_BYTES;
         cudaLaunchAttribute at{};
         at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = ctas, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        at.val.clusterDim.x = SCL, at.val.clusterDim.y = at.val.clusterDim.z = 1;
         cfg.attrs = &at, cfg.numAttrs = 1;
-        if (cudaLaunchKernelEx(&cfg, sort_kernel, sa, ctas) != cudaSuccess) return EWS_ERR_LAUNCH;
+        if (cudaLaunchKernelEx(&cfg, sort_kernel, sa) != cudaSuccess) return EWS_ERR_LAUNCH;
     }
     const bool odd = sa.passes & 1;  // the sorted order is in the second buffers after an odd number of passes
     const uint32_t *key = odd ? sa.key1 : sa.key0, *pos = odd ? sa.pos1 : sa.pos0;
@@ -512,18 +516,17 @@ extern "C" int ews_embed_bwd(const void* ids, int ids_wide, const void* dout, in
     a.key0 = (uint32_t*)(w + l.key0), a.pos0 = (uint32_t*)(w + l.pos0);
     a.key1 = (uint32_t*)(w + l.key1), a.pos1 = (uint32_t*)(w + l.pos1);
     a.totals = (uint32_t*)(w + l.totals), a.runs = (int2*)(w + l.runs);
-    const int ctas = n <= 2048 ? 1 : SCL;
     cudaStream_t s = (cudaStream_t)stream;
     const int vw = dtype == EWS_DTYPE_BF16 ? 8 : 4;
     const bool vec = dim % vw == 0 && dout_stride % vw == 0 && aligned16(dout) && aligned16(dtable);
     if (dtype == EWS_DTYPE_BF16) {
         const auto* g = static_cast<const bf16*>(dout);
         auto* d = static_cast<bf16*>(dtable);
-        return vec ? backward<bf16, true>(a, ctas, g, dout_stride, (int)dim, scale, l, w, d, s)
-                   : backward<bf16, false>(a, ctas, g, dout_stride, (int)dim, scale, l, w, d, s);
+        return vec ? backward<bf16, true>(a, g, dout_stride, (int)dim, scale, l, w, d, s)
+                   : backward<bf16, false>(a, g, dout_stride, (int)dim, scale, l, w, d, s);
     }
     const auto* g = static_cast<const float*>(dout);
     auto* d = static_cast<float*>(dtable);
-    return vec ? backward<float, true>(a, ctas, g, dout_stride, (int)dim, scale, l, w, d, s)
-               : backward<float, false>(a, ctas, g, dout_stride, (int)dim, scale, l, w, d, s);
+    return vec ? backward<float, true>(a, g, dout_stride, (int)dim, scale, l, w, d, s)
+               : backward<float, false>(a, g, dout_stride, (int)dim, scale, l, w, d, s);
 }
