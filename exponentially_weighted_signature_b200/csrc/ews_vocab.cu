@@ -48,6 +48,18 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// G is kept in the inputs' type between the two products. The rows' loss gradients are most often one number, 1 / N,
+// and where the softmax is small beside the target's 1 its rounding is then the same in every row's largest entry, so
+// that it does not average out in the sums. The first row's mantissa, a number in [1, 2), is therefore left out of G and
+// multiplied into the float32 sums: a common loss gradient becomes a power of two, which rounds nothing, and no entry
+// changes its size by more than 2. Without it one random bfloat16 case in four had a gradient 1.5 times as far from
+// the exact one as a float32 G rounded once at the end, with it one in a hundred.
+__device__ __forceinline__ float common_factor(const float* dloss, const int* row, int live) {
+    const float x = live > 0 ? fabsf(dloss[row[0]]) : 0.f;
+    if (!(x > 1e-37f && x < 1e37f)) return 1.f;
+    return __uint_as_float((__float_as_uint(x) & 0x007FFFFFu) | 0x3F800000u);
+}
+
 // ---- the GEMM --------------------------------------------------------------------------------------------------
 
 enum Epilogue { LSE, GRAD, OUT };
@@ -129,6 +141,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     const int live = __shfl_sync(kFull, *a.live, 0);
     const int m0 = min(a.job[0].m, live), tiles0 = (m0 + BM - 1) / BM;
     const int kb1 = (min(a.job[1].k, live) + BK - 1) / BK, blocks1 = EPI == OUT ? (kb1 + max(a.job[1].splits, 1) - 1) / max(a.job[1].splits, 1) : 0;
+    const float factor = EPI == LSE ? 1.f : common_factor(a.dloss, a.row, live);
     const long units0 = (long)tiles0 * a.job[0].tiles_n * a.job[0].splits;
     const long units = units0 + (EPI == OUT ? a.job[1].units : 0);
 
@@ -283,7 +296,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 } else if (EPI == GRAD) {
                     const int t = in ? a.target[row] : -1;
                     const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
-                    const float w = t < 0 ? 0.f : a.dloss[a.row[row]];
+                    const float w = t < 0 ? 0.f : a.dloss[a.row[row]] / factor;
                     const float lse = in ? a.lse[row] : 0.f, shift = -lse * kLog2e;
                     const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
                     for (int c = half * HALF; c < cols; c += 32) {
@@ -362,6 +375,10 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                         }
                         const int col = r.tn * BN + c;
                         const int w = min(32, cols - c);
+                        if (!job.acc) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] *= factor;
+                        }
                         if (!in) {
                         } else if (job.acc) {
                             float* p = job.acc + ((long)r.sp * job.m + row) * job.n + col;
@@ -556,13 +573,15 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
 // from their packed positions, and a row without one is zero.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ acc, int splits, long rows, int n, const int* __restrict__ slot,
-                                                     T* __restrict__ out) {
+                                                     const float* __restrict__ dloss, const int* __restrict__ live_rows,
+                                                     const int* __restrict__ row_of, T* __restrict__ out) {
     constexpr int W = VEC ? 4 : 1;
     const int per = n / W;
     const long total = rows * n;
     // a row's vectors to consecutive threads
     const int lanes = per < 256 ? per : 256, group = 256 / lanes, l = threadIdx.x % lanes, g = threadIdx.x / lanes;
     if (g >= group) return;
+    const float factor = common_factor(dloss, row_of, *live_rows);
     for (long row = (long)blockIdx.x * group + g; row < rows; row += (long)gridDim.x * group) {
         const long at = slot ? slot[row] : row;
         for (int c = l; c < per; c += lanes) {
@@ -579,6 +598,8 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ a
                     for (int j = 0; j < W; ++j) s[j] += v[j];
                 }
             }
+#pragma unroll
+            for (int j = 0; j < W; ++j) s[j] *= factor;
             T* o = out + row * n + c * W;
             if constexpr (VEC && sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
             else Vec<T, VEC>::store(o, s);
@@ -736,10 +757,12 @@ unsigned grid_of(long total) {
 }
 
 template <typename T>
-int reduce(const float* acc, int splits, long rows, long n, const int* slot, T* out, cudaStream_t s) {
+int reduce(const ews_vocab_args* a, const float* acc, int splits, long rows, const int* slot, T* out, cudaStream_t s) {
+    const RowPlan plan = row_plan(a->plan, a->rows);
+    const long n = a->dim;
     const unsigned grid = grid_of(rows * n / 4 + 1);
-    if (n % 4 == 0 && aligned16(out)) reduce_kernel<T, true><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, out);
-    else reduce_kernel<T, false><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, out);
+    if (n % 4 == 0 && aligned16(out)) reduce_kernel<T, true><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, a->dloss, plan.live, plan.row, out);
+    else reduce_kernel<T, false><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, a->dloss, plan.live, plan.row, out);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -823,9 +846,9 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
             o.job[1].out = out, o.job[1].acc = acc_w;
         }
         if ((rc = gemm<OUT>(o, go, wt, go, h, p.planes, s)) != EWS_OK) break;
-        if (a->dweight && acc_w) rc = reduce<T>(acc_w, p.split_w, n, a->dim, nullptr, out, s);
+        if (a->dweight && acc_w) rc = reduce<T>(a, acc_w, p.split_w, n, nullptr, out, s);
     }
-    if (rc == EWS_OK && a->dhidden) rc = reduce<T>(acc_h, p.split_h, a->rows, a->dim, plan.slot, static_cast<T*>(a->dhidden), s);
+    if (rc == EWS_OK && a->dhidden) rc = reduce<T>(a, acc_h, p.split_h, a->rows, plan.slot, static_cast<T*>(a->dhidden), s);
     return rc;
 }
 

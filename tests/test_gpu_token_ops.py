@@ -434,6 +434,27 @@ def test_vocab_loss_with_few_targets(ews, dtype, n, kept):
         assert ((got.double() - exact).abs() <= bound).all(), float(((got.double() - exact).abs() / bound).max())
 
 
+@pytest.mark.parametrize("first", [None, 0.0])
+def test_a_common_loss_gradient_is_not_rounded(ews, first):
+    """1 + 2^-8 lies half way between two bfloat16 numbers: rounded into every row it would put the gradients 2^-8 off.
+    Left out of what is rounded, two independent roundings remain, each of 2^-7 / sqrt(12) at most. A first row whose
+    gradient is another one has the ordinary rounding: 2^-8 of every entry, and that of the result."""
+    n, V, D = 600, 2000, 128
+    g = _gen(61)
+    h = torch.randn((n, D), device="cuda", generator=g).bfloat16()
+    w = (torch.randn((V, D), device="cuda", generator=g) * 0.02).bfloat16()
+    t = torch.randint(0, V, (n,), device="cuda", generator=g)
+    dl = torch.full((n,), (1 + 2.0**-8) / 512, device="cuda")
+    if first is not None:
+        dl[0] = first
+    hl, wl = h.clone().requires_grad_(), w.clone().requires_grad_()
+    got = torch.autograd.grad(ews.vocab_loss(hl, wl, t), (hl, wl), dl)
+    want = _loss_ref(h, w, t, dl)[1:3]
+    bound = 2**0.5 * 2**-7 / 12**0.5 if first is None else 2**-8 + 2**-7 / 12**0.5
+    for a, b in zip(got, want):
+        assert (a.double() - b).norm() <= bound * b.norm()
+
+
 def test_vocab_loss_gradient_against_differences(ews):
     n, V, D = 40, 300, 24
     g = _gen(8)
