@@ -591,21 +591,20 @@ void plan(int batch, int steps, int heads, int dz, int width, int* slices, int* 
 }
 
 // Columns of z a CTA takes: the float32 form's two sums of a wide product leave room for 32.
-int slice_width(bool f32, int dx) { return f32 && dx > 64 ? 32 : 64; }
+constexpr int slice_width(bool f32) { return f32 ? 32 : 64; }
 
 // The segments' states, for whichever form runs (a state in full precision needs its pass even over one segment).
 size_t seg_bytes(const ews_decay_args* a, int dx, int dz) {
+    const bool f32 = a->dtype == EWS_DTYPE_F32;
     int slices, segs, span;
-    plan(a->batch, a->steps, a->heads, dz, slice_width(a->dtype == EWS_DTYPE_F32, dx), &slices, &segs, &span);
+    if (f32 && dx <= F32_WIDE) segs = tc_segments(a->batch, a->steps, a->heads * ((dz + 63) / 64), false, &span);
+    else plan(a->batch, a->steps, a->heads, dz, slice_width(f32), &slices, &segs, &span);
     if (segs == 1) segs = 0;
-    if (a->dtype == EWS_DTYPE_BF16) {
+    if (!f32) {
         const int t = tc_segments(a->batch, a->steps, a->heads, true, &span);
         if (t > segs) segs = t;
         const int f = tc_segments(a->batch, a->steps, a->heads, false, &span);
         if (f > segs) segs = f;
-    } else if (dx <= 64) {
-        const int f = tc_segments(a->batch, a->steps, a->heads * ((dz + 63) / 64), false, &span);
-        if (f > segs && f > 1) segs = f;
     }
     return sizeof(float) * (size_t)a->batch * a->heads * segs * dx * dz;
 }
@@ -613,6 +612,7 @@ size_t seg_bytes(const ews_decay_args* a, int dx, int dz) {
 template <typename T, int DK, int DV, int NS, bool STATE>
 int launch(const Chain<T>& a, cudaStream_t s) {
     using S = Smem<T, DK, DV, STATE>;
+    if (a.y.width > DK || a.z.width > a.slices * DV) return EWS_ERR_UNSUPPORTED;  // the plan's slices and the kernel's
     auto* kern = chain_kernel<T, DK, DV, NS, STATE>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::bytes) != cudaSuccess)
         return EWS_ERR_LAUNCH;
@@ -625,17 +625,17 @@ int launch(const Chain<T>& a, cudaStream_t s) {
 template <typename T, int NS, bool STATE>
 int launch_d(const Chain<T>& a, cudaStream_t s) {
     [[maybe_unused]] const int dk = pad_width(a.y.width);
-    if constexpr (sizeof(T) == 4) {  // narrower x and y run in ews_decay_f32.cu
-        return launch<T, 128, 32, NS, STATE>(a, s);
+    if constexpr (sizeof(T) == 4) {  // narrower x and y run in ews_decay_f32.cu, whatever the axis's length
+        return launch<T, 128, slice_width(true), NS, STATE>(a, s);
     } else {
         if (a.z.width <= 32) {
             if (dk == 32) return launch<T, 32, 32, NS, STATE>(a, s);
             if (dk == 64) return launch<T, 64, 32, NS, STATE>(a, s);
             return launch<T, 128, 32, NS, STATE>(a, s);
         }
-        if (dk == 32) return launch<T, 32, 64, NS, STATE>(a, s);
-        if (dk == 64) return launch<T, 64, 64, NS, STATE>(a, s);
-        return launch<T, 128, 64, NS, STATE>(a, s);
+        if (dk == 32) return launch<T, 32, slice_width(false), NS, STATE>(a, s);
+        if (dk == 64) return launch<T, 64, slice_width(false), NS, STATE>(a, s);
+        return launch<T, 128, slice_width(false), NS, STATE>(a, s);
     }
 }
 
@@ -685,7 +685,7 @@ int run_chain(Chain<T> a, cudaStream_t s) {
     } else {
         if (f32_fits(a)) return run_f32(a, s);
     }
-    plan(a.batch, a.steps, a.heads, a.z.width, slice_width(f32, a.y.width), &a.slices, &a.segs, &a.span);
+    plan(a.batch, a.steps, a.heads, a.z.width, slice_width(f32), &a.slices, &a.segs, &a.span);
     const bool exact = a.fin != nullptr && !f32;
     int rc;
     if (a.segs > 1) {

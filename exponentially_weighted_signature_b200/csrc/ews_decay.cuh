@@ -40,7 +40,9 @@ int tc_segments(int batch, int steps, int heads, bool state, int* span);
 bool tc_fits(const Chain<bf16>& a);
 int tc_chain(const Chain<bf16>& a, bool state_only, bool exact, cudaStream_t s);
 
-// The same for float32 in three bfloat16 planes (x and y up to 64 wide, any alignment): ews_decay_f32.cu.
+// The same for float32 in three bfloat16 planes (x and y up to F32_WIDE wide; any alignment, any length, none included):
+// ews_decay_f32.cu.
+constexpr int F32_WIDE = 64;
 bool f32_fits(const Chain<float>& a);
 int f32_chain(const Chain<float>& a, bool state_only, cudaStream_t s);
 

@@ -21,7 +21,7 @@ using namespace tc5;
 
 namespace {
 
-constexpr int FC = 128, FW = 64;       // tokens of a chunk, columns of a tile
+constexpr int FC = 128, FW = F32_WIDE;  // tokens of a chunk, columns of a tile
 constexpr int PLANE = FC * 128;        // bytes of a plane of a stream, 128-byte rows
 constexpr int SPLANE = FW * 128;       // of the state
 constexpr int FTHR = 32 * 13;          // warps: MMA, four of group A, eight of group B (at most 16: 128 registers)
@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
 
 }  // namespace
 
-bool f32_fits(const Chain<float>& a) { return a.steps > 0 && a.y.width <= FW; }
+// An axis of no tokens is one item without a chunk: its state goes from where it starts to where it ends.
+bool f32_fits(const Chain<float>& a) { return a.y.width <= FW; }
 
 int f32_chain(const Chain<float>& a, bool state_only, cudaStream_t s) {
     const long items = (long)a.batch * a.heads * a.segs * a.slices;

@@ -1,0 +1,47 @@
+"""The token operators at their edges: axes of no tokens, the autograd contract, losses that nearly vanish, values that are
+not finite, long axes of the forms that run on warp-level instructions, and vocabularies in several pieces.
+
+``_check`` and its bounds are those of test_gpu_token_ops.py."""
+
+import torch
+
+import pytest
+from test_gpu_token_ops import BF16, F32, FP32, U, _check, _gen, _inputs, _loss_ref, _ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ews():
+    import exponentially_weighted_signature_b200 as e
+
+    return e
+
+
+# ------------------------------------------------------------------------------------------ no tokens
+
+
+def _leave_nan(*shape):
+    """Freed blocks of NaN of this size: what the operator's next allocations are likely to get."""
+    held = [torch.full(shape, float("nan"), device="cuda") for _ in range(4)]
+    del held
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (33, 80), (16, 33), (48, 100), (1, 40), (65, 64), (128, 128)])
+def test_no_tokens_leave_the_state(ews, dtype, dk, dv):
+    """T = 0: the state is the initial one (or zero), its gradient the state's own (which passes through 1 / scale and
+    scale: three roundings)."""
+    g = _gen(dk * dv)
+    q, k, v = (torch.zeros((2, 0, h, d), dtype=dtype, device="cuda") for h, d in ((4, dk), (2, dk), (2, dv)))
+    rate = torch.tensor([0.5, 0.1, 0.02, 3.0], device="cuda")
+    s0 = torch.randn((2, 4, dk, dv), device="cuda", generator=g).requires_grad_()
+    ds = torch.randn((2, 4, dk, dv), device="cuda", generator=g)
+    _leave_nan(2, 4, dk, dv)
+    out, end = ews.decayed_attention(q, k, v, rate, initial_state=s0, return_state=True)
+    assert out.shape == (2, 0, 4, dv) and torch.equal(end, s0)
+    _leave_nan(2, 4, dk, dv)
+    (d0,) = torch.autograd.grad(end, (s0,), ds)
+    assert ((d0 - ds).abs() <= 2.0**-22 * ds.abs()).all()
+    _leave_nan(2, 4, dk, dv)
+    assert (ews.decayed_attention(q, k, v, rate, return_state=True)[1] == 0).all()
