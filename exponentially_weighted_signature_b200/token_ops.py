@@ -289,7 +289,8 @@ def decayed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ra
     q (B, H, dk), k (B, Hk, dk), v (B, Hk, dv); state (P, H, dk, dv) float32, contiguous. Row b works on state
     ``slots[b]`` (int32 (B,); None: b, with P >= B). A negative slot is a row without a request: its output is zero and
     no state is touched. Two rows must not share a slot; one out of range gives a zero row and IndexError on the
-    next call. Returns o (B, H, dv). For serving: no gradient."""
+    next call. Returns o (B, H, dv). For serving: no gradient; a backward that needs the states as they were raises, as
+    after any operation in place."""
     H, dk, dv = _check_heads(q, k, v, rate, 3)
     B = q.shape[0]
     if state.dim() != 4 or state.shape[1:] != (H, dk, dv) or state.dtype != torch.float32 or not state.is_contiguous():
@@ -309,6 +310,8 @@ def decayed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ra
                   qb, 0, qh, kb, 0, kh, vb, 0, vh, rate.data_ptr(), 0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
                   engine.index_word(idx)[0])
     _launch(idx, "ews_decay_step", B, _lib.load().ews_decay_step, args, _addr(slots), state.shape[0], state.data_ptr())
+    if not state.is_inference():  # autograd cannot see the write: a backward that saved these states must
+        torch.autograd.graph.increment_version(state)
     return out
 
 

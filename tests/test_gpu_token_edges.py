@@ -45,3 +45,20 @@ def test_no_tokens_leave_the_state(ews, dtype, dk, dv):
     assert ((d0 - ds).abs() <= 2.0**-22 * ds.abs()).all()
     _leave_nan(2, 4, dk, dv)
     assert (ews.decayed_attention(q, k, v, rate, return_state=True)[1] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------ the autograd contract
+
+
+def test_a_step_on_a_state_that_a_backward_needs_is_seen(ews):
+    """The step overwrites its states: a backward that saved them raises, as after any operation in place."""
+    q, k, v, rate, s0, _ = _inputs(FP32, 2, 5, 2, 2, 16, 16)
+    leaf = q.clone().requires_grad_()
+    pool = s0.clone()
+    out = ews.decayed_attention(leaf, k, v, rate, initial_state=pool)
+    with torch.no_grad():
+        ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], rate, pool)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    with torch.inference_mode():  # tensors without a version
+        ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], rate, s0.clone())
