@@ -4,8 +4,9 @@
 per head, over prompts and in training) with ``decayed_attention_step`` (one token per row on a pool of states), and
 ``vocab_loss`` (softmax cross entropy over a large vocabulary whose logits are never kept). All run on the caller's
 current stream through the C ABI, on float32 or bfloat16 CUDA tensors; states, sums, softmax statistics and losses
-are float32. There is no CPU fallback. Indices out of range do not stop the GPU: the entry counts as absent and the
-next token operator on the device raises IndexError (at once under ``configure(check_status=True)``).
+are float32. There is no CPU fallback. Derivatives are reverse-mode: a dual tensor is refused. Indices out of range do
+not stop the GPU: the entry counts as absent and the next token operator on the device raises IndexError (at once under
+``configure(check_status=True)``).
 """
 
 from __future__ import annotations
@@ -16,6 +17,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, engine
 from .engine import _require_cuda, _timed
@@ -46,7 +48,12 @@ def _wide(t: torch.Tensor, what: str) -> int:
 
 
 def _device(*tensors) -> int:
-    """The index of the one CUDA device that all tensors are on, pending index errors on it raised."""
+    """The index of the one CUDA device that all tensors are on, pending index errors on it raised. Dual tensors are
+    refused: where no input requires a gradient no autograd function runs, and a tangent would vanish unseen."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the token operators have no forward-mode derivative")
     idx = tensors[0].get_device()
     for t in tensors:
         if t is not None and (idx < 0 or t.get_device() != idx):

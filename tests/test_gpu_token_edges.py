@@ -62,3 +62,29 @@ def test_a_step_on_a_state_that_a_backward_needs_is_seen(ews):
         out.sum().backward()
     with torch.inference_mode():  # tensors without a version
         ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], rate, s0.clone())
+
+
+def test_tangents_are_refused(ews):
+    """No forward-mode derivative is built: a dual tensor raises instead of losing its tangent."""
+    import torch.autograd.forward_ad as fw
+
+    q, k, v, rate, s0, _ = _inputs(FP32, 2, 5, 2, 2, 16, 16)
+    ids = torch.tensor([0, 1], device="cuda")
+    h = torch.randn((2, 16), device="cuda")
+    with fw.dual_level():
+        dual = lambda x: fw.make_dual(x, torch.ones_like(x))  # noqa: E731
+        calls = [lambda: ews.decayed_attention(dual(q), k, v, rate),
+                 lambda: ews.decayed_attention(q, k, v, dual(rate)),
+                 lambda: ews.decayed_attention(q, k, v, rate, initial_state=dual(s0)),
+                 lambda: ews.decayed_attention_step(q[:, 0], k[:, 0], dual(v[:, 0]), rate, s0),
+                 lambda: ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], rate, dual(s0)),
+                 lambda: ews.token_embedding(ids, dual(h)),
+                 lambda: ews.vocab_loss(dual(h), h, ids),
+                 lambda: ews.vocab_loss(h, dual(h), ids)]
+        was = s0.clone()
+        for call in calls:
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError):
+                    call()
+        assert torch.equal(s0, was)
+        assert ews.token_embedding(ids, h).shape == (2, 16)  # and others still run there
