@@ -10,6 +10,7 @@ the tables, of the input increments and of the lift.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 import torch.nn.functional as F
@@ -188,6 +189,38 @@ def _coef_buffer(coef):
 def increments_to_knots_grad(gdx: torch.Tensor) -> torch.Tensor:
     """Adjoint of dx_t = x_{t+1} - x_t: (B, T, d) -> (B, T+1, d)."""
     return F.pad(gdx, (0, 0, 1, 0)) - F.pad(gdx, (0, 0, 0, 1))
+
+
+class _Once(torch.autograd.Function):
+    """Passes gradients on; to differentiate them again raises."""
+
+    @staticmethod
+    def forward(ctx, name, *grads):
+        ctx.name = name
+        return tuple(g.detach() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name}: no second derivative is built for this operator")
+
+
+def first_order(backward):
+    """For a backward that fills buffers through raw pointers: its gradients carry no graph, so under ``create_graph`` a
+    term built on them would lose this operator's part without a word. They are marked instead, whether the cotangent
+    depends on anything or not (``once_differentiable`` marks them only where it does), and a second differentiation
+    that reaches them raises."""
+
+    @functools.wraps(backward)
+    def wrapped(ctx, *cotangents):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *cotangents)
+        with torch.no_grad():
+            out = backward(ctx, *cotangents)
+        out = out if isinstance(out, tuple) else (out,)
+        marked = iter(_Once.apply(type(ctx).__name__, *(g.detach().requires_grad_() for g in out if g is not None)))
+        return tuple(None if g is None else next(marked) for g in out)
+
+    return wrapped
 
 
 class DiagScan(torch.autograd.Function):

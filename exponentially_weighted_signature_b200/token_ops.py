@@ -4,9 +4,9 @@
 per head, over prompts and in training) with ``decayed_attention_step`` (one token per row on a pool of states), and
 ``vocab_loss`` (softmax cross entropy over a large vocabulary whose logits are never kept). All run on the caller's
 current stream through the C ABI, on float32 or bfloat16 CUDA tensors; states, sums, softmax statistics and losses
-are float32. There is no CPU fallback. Derivatives are reverse-mode: a dual tensor is refused. Indices out of range do
-not stop the GPU: the entry counts as absent and the next token operator on the device raises IndexError (at once under
-``configure(check_status=True)``).
+are float32. There is no CPU fallback. Derivatives are reverse-mode and first-order: a dual tensor is refused, and so
+is differentiating a gradient again. Indices out of range do not stop the GPU: the entry counts as absent and the next
+token operator on the device raises IndexError (at once under ``configure(check_status=True)``).
 """
 
 from __future__ import annotations
@@ -20,7 +20,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib, engine
-from .engine import _require_cuda, _timed
+from .engine import _require_cuda, _timed, first_order
 
 _DTYPES = {torch.float32: _lib.EWS_DTYPE_F32, torch.bfloat16: _lib.EWS_DTYPE_BF16}
 _WIDE = {torch.int64: 1, torch.int32: 0}
@@ -138,6 +138,7 @@ class _Embedding(torch.autograd.Function):
         return _embed(flat, rows, scale, shape)
 
     @staticmethod
+    @first_order
     def backward(ctx, dout):
         (vocab, dim), scale, padding_index = ctx.meta
         (flat,) = ctx.saved_tensors
@@ -213,6 +214,7 @@ class _Decayed(torch.autograd.Function):
         return _decayed(q, k, v, rate, initial, lengths, scale, want_state)
 
     @staticmethod
+    @first_order
     def backward(ctx, dout, dend):
         q, k, v, rate, initial, lengths = ctx.saved_tensors
         lib = _lib.load()
@@ -358,6 +360,7 @@ class _VocabLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @first_order
     def backward(ctx, dloss):
         hidden, weight, targets, lse, plan = ctx.saved_tensors
         lib = _lib.load()

@@ -88,3 +88,25 @@ def test_tangents_are_refused(ews):
                     call()
         assert torch.equal(s0, was)
         assert ews.token_embedding(ids, h).shape == (2, 16)  # and others still run there
+
+
+def test_second_derivatives_are_refused(ews):
+    """A gradient taken with create_graph is usable as a number; differentiating it again raises instead of leaving the
+    operator's part out, whether or not the cotangent itself depends on anything."""
+    q, k, v, rate, s0, _ = _inputs(FP32, 2, 5, 2, 2, 16, 16)
+    ids = torch.tensor([0, 1], device="cuda")
+    h, w = (torch.randn((2, 16), device="cuda") for _ in range(2))
+    leaf = lambda x: x.clone().requires_grad_()  # noqa: E731
+    cases = [(lambda a, b: ews.decayed_attention(a, k, v, rate, initial_state=b), (q, s0)),
+             (lambda a, b: ews.token_embedding(ids, a) * b, (w, h)),
+             (lambda a, b: ews.vocab_loss(a, b, ids), (h, w))]
+    for f, args in cases:
+        for power in (1, 2):  # a constant cotangent, and one that depends on the result
+            a, b = (leaf(x) for x in args)
+            plain = torch.autograd.grad((f(a, b) ** power).sum(), (a, b))
+            grads = torch.autograd.grad((f(a, b) ** power).sum(), (a, b), create_graph=True)
+            for x, y in zip(plain, grads):
+                assert torch.equal(x, y.detach())
+            penalty = sum((x**2).sum() for x in grads) + (a**2).sum()
+            with pytest.raises(RuntimeError, match="second derivative"):
+                penalty.backward()
