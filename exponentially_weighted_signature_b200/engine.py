@@ -4,7 +4,8 @@ Each engine is one autograd Function whose forward calls the library's *_fwd ent
 backward calls *_bwd. The per-sample parameter tables (log-flows and series tables) are ordinary
 differentiable torch tensors built from the generator and the clock, so their tiny maps back to the
 generator parameters and the clock run through torch autograd; the kernels return the gradients of
-the tables, of the input increments and of the lift.
+the tables, of the input increments and of the lift. Gradients are first-order: differentiating one
+again raises.
 """
 
 from __future__ import annotations
@@ -263,6 +264,7 @@ class DiagScan(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_out):
         readout, flags, chunk, increments, B, T, d_in, N, bwd_bytes, path_dtype = ctx.meta
         path, x, q1, q2, lift, out, fwd_ws = ctx.saved_tensors
@@ -313,6 +315,7 @@ class Expm(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, G):
         (X,) = ctx.saved_tensors
         Gc = G.to(torch.float64).contiguous()
@@ -353,6 +356,7 @@ class SeriesTables(torch.autograd.Function):
         return F, G, H
 
     @staticmethod
+    @first_order
     def backward(ctx, dF, dG, dH):
         X, Wc, c1, c2 = ctx.saved_tensors
         B, n = X.shape[0], X.shape[-1]
@@ -401,6 +405,7 @@ class DenseLeaf(torch.autograd.Function):
         return Dc, F, G, H
 
     @staticmethod
+    @first_order
     def backward(ctx, dDc, dF, dG, dH):
         A, h, Al, Wc, c1, c2 = ctx.saved_tensors
         B, n = h.shape[0], A.shape[-1]
@@ -447,6 +452,7 @@ class GradedNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         flat, g = ctx.saved_tensors
         d, levels, eps = ctx.meta
@@ -485,6 +491,7 @@ class GatedClock(torch.autograd.Function):
         return theta
 
     @staticmethod
+    @first_order
     def backward(ctx, dtheta):
         xc, wc, bc = ctx.saved_tensors
         s, c = ctx.consts
@@ -539,6 +546,7 @@ class DenseScan(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_out):
         readout, flags, chunk, increments, B, T, d_in, N, QP, bwd_bytes, path_dtype = ctx.meta
         path, M, F, G, H, out, fwd_ws = ctx.saved_tensors
@@ -612,6 +620,7 @@ class DiagScanClock(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_out):
         readout, flags, chunk, increments, series_q, B, T, d_in, N, bwd_bytes, path_dtype, clock_dtype = ctx.meta
         path, clock, rates, lift, out, fwd_ws = ctx.saved_tensors
@@ -683,6 +692,7 @@ class BlockScan(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_out):
         readout, flags, chunk, increments, series_q, B, T, d_in, N, bwd_bytes, path_dtype, clock_dtype = ctx.meta
         path, clock, blocks, lift, out, fwd_ws = ctx.saved_tensors
