@@ -275,16 +275,18 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                         for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
                         const float was = mx;
                         mx = fmaxf(mx, top);
-                        const float shift = mx == -INFINITY ? 0.f : -mx * kLog2e;
-                        const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
+                        // the maximum leaves before the scaling: its own term is 1 and no other one exceeds it, where a rounded
+                        // -mx * log2(e) put every exponent off by up to 2^-24 of the maximum
+                        const float base = mx == -INFINITY ? 0.f : mx;
+                        const uint64_t scale2 = pair(kLog2e, kLog2e), base2 = pair(-base, -base);
                         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             float e0, e1;
-                            unpair(fma2(pair(v[j], v[j + 1]), scale2, shift2), e0, e1);
+                            unpair(mul2(add2(pair(v[j], v[j + 1]), base2), scale2), e0, e1);
                             part[j & 3] += ex2(e0), part[(j & 3) + 1] += ex2(e1);
                         }
-                        sum = sum * exp2f(fmaf(was, kLog2e, shift)) + ((part[0] + part[1]) + (part[2] + part[3]));
+                        sum = sum * exp2f((was - base) * kLog2e) + ((part[0] + part[1]) + (part[2] + part[3]));
                         if ((unsigned)(pick - c) < 32u) {
                             float z = 0.f;
 #pragma unroll
@@ -564,9 +566,11 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
         s = s * exp2f((m - base) * kLog2e) + p.y * exp2f((p.x - base) * kLog2e);
         m = n;
     }
-    const float z = m + logf(s);
-    lse[row] = z;
-    loss[plan.row[row]] = z - picked[row];
+    // The maximum and the target's logit cancel first, exactly where the target is the maximum: a sum rounded at the
+    // logits' size would lose a confident row's loss, or turn it negative. With s >= 1 no loss is.
+    const float rest = logf(s);
+    lse[row] = m + rest;
+    loss[plan.row[row]] = (m - picked[row]) + rest;
 }
 
 // A gradient from its float32 partials, summed in order and rounded once; with `slot` the rows of the result are taken

@@ -110,3 +110,40 @@ def test_second_derivatives_are_refused(ews):
             penalty = sum((x**2).sum() for x in grads) + (a**2).sum()
             with pytest.raises(RuntimeError, match="second derivative"):
                 penalty.backward()
+
+
+# ------------------------------------------------------------------------------------------ losses
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+def test_confident_rows_keep_their_small_losses(ews, dtype, offset):
+    """Logits that are exact (each row picks one column of the weight), the target's 20 to 60 above the others. The
+    exponentials' sum is 1 and a remainder r, of which each of the at most 32 additions on the way rounds by 2^-24 or less,
+    and never by more than what it adds; the exponentials have 2^-20 of their own."""
+    D, V = 64, 700
+    g = _gen(17)
+    w = torch.randn((V, D), device="cuda", generator=g) + offset
+    t = torch.randperm(V, device="cuda", generator=g)[:D]
+    w[t, torch.arange(D, device="cuda")] += torch.linspace(20.0, 60.0, D, device="cuda")
+    w = w.to(dtype)
+    h = torch.eye(D, device="cuda").to(dtype)
+    loss = ews.vocab_loss(h, w, t)
+    z = w.t().double()
+    others = torch.exp(z - z.gather(1, t[:, None])).scatter(1, t[:, None], 0.0)
+    want = torch.log1p(others.sum(1))
+    bound = torch.minimum(torch.full_like(want, 32 * 2.0**-24), 1.01 * want) + 2.0**-20 * want
+    assert (loss >= 0).all()
+    assert ((loss.double() - want).abs() <= bound).all(), float(((loss.double() - want).abs() / bound).max())
+
+
+def test_losses_do_not_lose_the_logits_offset(ews):
+    """Logits near 1,000 and exact: the differences that make the loss are exact too, so its error is that of the
+    exponentials (2^-20) and of 40 additions (2^-24 each), not a rounding of 1,000 (2^-15)."""
+    D, V = 64, 700
+    g = _gen(19)
+    w = 1000.0 + torch.randn((V, D), device="cuda", generator=g)
+    t = torch.randint(0, V, (D,), device="cuda", generator=g)
+    loss = ews.vocab_loss(torch.eye(D, device="cuda"), w, t)
+    want = torch.nn.functional.cross_entropy(w.t().double(), t, reduction="none")
+    assert ((loss.double() - want).abs() <= 2.0**-20 + 40 * 2.0**-24 + 2.0**-22 * want).all()
