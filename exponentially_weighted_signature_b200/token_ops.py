@@ -339,10 +339,12 @@ def _vocab_work(hidden, weight, backward):
                              weight.data_ptr() % 16, backward), hidden)
 
 
-def _vocab(hidden, weight, targets, ignore):
+def _vocab(hidden, weight, targets, ignore, shape):
     lib = _lib.load()
     rows = hidden.shape[0]
-    loss, lse = torch.empty((2, rows), dtype=torch.float32, device=hidden.device).unbind(0)
+    # of its own memory and shape: a loss that is a view cannot be changed in place by the caller
+    loss = torch.empty(shape, dtype=torch.float32, device=hidden.device)
+    lse = torch.empty(rows, dtype=torch.float32, device=hidden.device)
     work = _vocab_work(hidden, weight, 0)
     plan = torch.empty(3 * rows + 4, dtype=torch.int32, device=hidden.device)
     args = _vocab_args(hidden, weight, targets, ignore, loss, lse, plan, work=work)
@@ -352,9 +354,9 @@ def _vocab(hidden, weight, targets, ignore):
 
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore):
+    def forward(ctx, hidden, weight, targets, ignore, shape):
         hidden, weight = _rows(hidden), _rows(weight)
-        loss, lse, plan = _vocab(hidden, weight, targets, ignore)
+        loss, lse, plan = _vocab(hidden, weight, targets, ignore, shape)
         ctx.ignore = ignore
         ctx.save_for_backward(hidden, weight, targets, lse, plan)
         return loss
@@ -370,7 +372,7 @@ class _VocabLoss(torch.autograd.Function):
         work = _vocab_work(hidden, weight, 1)
         args = _vocab_args(hidden, weight, targets, ctx.ignore, None, lse, plan, dloss, dh, dw, work)
         _launch(hidden.get_device(), "ews_vocab_bwd", hidden.shape[0], lib.ews_vocab_bwd, args)
-        return dh, dw, None, None
+        return dh, dw, None, None, None
 
 
 def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100) -> torch.Tensor:
@@ -392,7 +394,5 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
     _device(hidden, weight, targets)
     flat, t = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        loss = _VocabLoss.apply(flat, weight, t, int(ignore_index))
-    else:
-        loss = _vocab(_rows(flat), _rows(weight), t, int(ignore_index))[0]
-    return loss if targets.dim() == 1 else loss.reshape(targets.shape)
+        return _VocabLoss.apply(flat, weight, t, int(ignore_index), targets.shape)
+    return _vocab(_rows(flat), _rows(weight), t, int(ignore_index), targets.shape)[0]

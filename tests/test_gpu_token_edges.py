@@ -147,3 +147,23 @@ def test_losses_do_not_lose_the_logits_offset(ews):
     loss = ews.vocab_loss(torch.eye(D, device="cuda"), w, t)
     want = torch.nn.functional.cross_entropy(w.t().double(), t, reduction="none")
     assert ((loss.double() - want).abs() <= 2.0**-20 + 40 * 2.0**-24 + 2.0**-22 * want).all()
+
+
+@pytest.mark.parametrize("shape", [(6,), (2, 3)])
+def test_losses_may_be_weighted_in_place(ews, shape):
+    g = _gen(23)
+    h, w = torch.randn((*shape, 16), device="cuda", generator=g), torch.randn((30, 16), device="cuda", generator=g)
+    t = torch.randint(0, 30, shape, device="cuda", generator=g)
+    weight = torch.rand(shape, device="cuda", generator=g)
+    hl, wl = h.clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad((ews.vocab_loss(hl, wl, t) * weight).sum(), (hl, wl))
+    loss = ews.vocab_loss(hl, wl, t)
+    loss *= weight
+    for a, b in zip(torch.autograd.grad(loss.sum(), (hl, wl)), want):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        loss = ews.vocab_loss(h, w, t)
+    factor = weight.clone().requires_grad_()
+    loss *= factor  # a result without a gradient, weighted by something that has one
+    loss.sum().backward()
+    assert torch.equal(factor.grad, ews.vocab_loss(h, w, t))
