@@ -34,11 +34,18 @@ class DecayBlock(nn.Module):
         self.out = nn.Linear(self.heads * self.head_dim, hidden_dim, bias=False)
         self.ff1 = nn.Linear(hidden_dim, ff_mult * hidden_dim)
         self.ff2 = nn.Linear(ff_mult * hidden_dim, hidden_dim)
-        self.register_buffer("rate", torch.exp2(-torch.linspace(1.0, 9.0, self.heads)), persistent=False)
+        self.register_buffer("rate", self._rates().to(self.qkv.weight.device), persistent=False)
+
+    def _rates(self):
+        return torch.exp2(-torch.linspace(1.0, 9.0, self.heads, device="cpu"))
 
     def _apply(self, fn, recurse=True):
+        """A change of type, or memory without contents, is for the weights: the rates keep their float32 values and only
+        follow to the device (a model's decays are the same in every type; on the meta device they have no values yet)."""
+        rate = self.rate
         super()._apply(fn, recurse)
-        self.rate = self.rate.float()  # rates stay float32 whatever the model's type
+        device = self.rate.device
+        self.rate = (self._rates() if rate.is_meta else rate).to(device)
         return self
 
     def _heads(self, x):

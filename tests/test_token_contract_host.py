@@ -31,3 +31,37 @@ def test_a_first_order_gradient_is_a_number_and_no_more(power):
     with torch.no_grad():
         grad.mul_(2)
     assert torch.equal(grad.detach(), 2 * plain)
+
+
+def _block(heads=6):
+    from exponentially_weighted_signature_b200 import DecayBlock
+
+    return DecayBlock(heads * 4, heads)
+
+
+def test_rates_are_the_same_in_every_type():
+    want = torch.exp2(-torch.linspace(1.0, 9.0, 6))
+    block = _block()
+    assert torch.equal(block.rate, want)
+    for cast in (lambda m: m.bfloat16(), lambda m: m.float(), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.bfloat16)):
+        cast(block)
+        assert block.rate.dtype == torch.float32 and torch.equal(block.rate, want)
+    assert block.qkv.weight.dtype == torch.bfloat16 and block._buffers["rate"] is block.rate
+    assert torch.equal(torch.nn.Sequential(_block()).bfloat16()[0].rate, want)
+
+
+def test_rates_that_were_set_are_kept():
+    block = _block()
+    block.rate.mul_(0.3)
+    was = block.rate.clone()
+    assert torch.equal(block.bfloat16().rate, was)
+
+
+def test_rates_have_values_after_a_build_without_memory():
+    want = torch.exp2(-torch.linspace(1.0, 9.0, 6))
+    assert torch.equal(_block().to_empty(device="cpu").rate, want)
+    with torch.device("meta"):
+        block = _block()
+    assert block.rate.is_meta
+    assert torch.equal(block.to_empty(device="cpu").rate, want)
+    assert _block().to("meta").rate.is_meta
