@@ -207,10 +207,10 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                         if (a.rev ? cb >= quarter : cb <= quarter) {
                             float e[32];
                             tmem_ld32(tmem + TP + lanes + cb * 32, e);
-                            if (m < FC) {  // a score with no token behind it may be anything
-                                const int left = m - cb * 32;
+                            if (m < FC || cb == quarter) {
+                                const uint32_t live = live_scores(cb, quarter, lane, m, a.rev);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) e[j] = j < left ? e[j] : 0.f;
+                                for (int j = 0; j < 32; ++j) e[j] = live & (1u << j) ? e[j] : 0.f;
                             }
                             const uint32_t g = row_tab - cb * 256;
 #pragma unroll

@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                         if (a.rev ? cb >= quarter : cb <= quarter) {
                             float v[32];
                             tmem_ld32(tmem + TP + lanes + cb * 32, v);
-                            if (m < TC) {  // a score with no token behind it may be anything
-                                const int left = m - cb * 32;
+                            if (m < TC || cb == quarter) {
+                                const uint32_t live = live_scores(cb, quarter, lane, m, a.rev);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : 0.f;
+                                for (int j = 0; j < 32; ++j) v[j] = live & (1u << j) ? v[j] : 0.f;
                             }
                             const uint32_t g = row_tab - cb * 256;
 #pragma unroll

@@ -175,6 +175,14 @@ __device__ __forceinline__ void put_decay(unsigned char* tab, int tid, int threa
     };
     for (int x = tid - 127; x <= 127; x += threads) *reinterpret_cast<float2*>(tab + (x + 127) * 8) = make_float2(w(x), w(x - 1));
 }
+// Which of a row's scores against the 32 tokens from 32 cb on count, row 32 quarter + lane of a chunk of m tokens: the tokens
+// exist, and none lies behind the row (reversed: before it). The others may be anything and are dropped, not weighted with
+// zero: what is not finite in a token must not reach the tokens that come first.
+__device__ __forceinline__ uint32_t live_scores(int cb, int quarter, int lane, int m, bool rev) {
+    const int to = cb == quarter && !rev ? min(m - cb * 32, lane + 1) : m - cb * 32;
+    const uint32_t below = to >= 32 ? kFull : to > 0 ? (1u << to) - 1u : 0u;
+    return cb == quarter && rev ? below & (kFull << lane) : below;
+}
 __device__ __forceinline__ float decay_of(float rate, int n) { return n <= 0 ? 1.f : expf(-rate * (float)n); }
 
 // 32 bytes, a whole sector, from one lane.

@@ -167,3 +167,30 @@ def test_losses_may_be_weighted_in_place(ews, shape):
     loss *= factor  # a result without a gradient, weighted by something that has one
     loss.sum().backward()
     assert torch.equal(factor.grad, ews.vocab_loss(h, w, t))
+
+
+# ------------------------------------------------------------------------------------------ values that are not finite
+
+
+@pytest.mark.parametrize("dtype,dk,dv", [(BF16, 64, 64), (BF16, 128, 48), (BF16, 37, 40), (FP32, 64, 64), (FP32, 40, 72), (FP32, 100, 64)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_key_that_is_not_finite_reaches_no_earlier_token(ews, dtype, dk, dv, value):
+    """Forward: a key enters from its own token on. Backward: a token's cotangent enters dk up to its own token."""
+    T, at = 300, 149  # inside a block of 32 of any chunk
+    q, k, v, rate, s0, g = _inputs(dtype, 2, T, 2, 1, dk, dv, seed=41)
+    do = torch.randn((2, T, 2, dv), device="cuda", generator=g).to(dtype)
+
+    def run(k, do):
+        leaf = k.clone().requires_grad_()
+        out = ews.decayed_attention(q, leaf, v, rate, initial_state=s0)
+        return out.detach(), torch.autograd.grad(out, (leaf,), do)[0]
+
+    clean, dk_clean = run(k, do)
+    bad = k.clone()
+    bad[:, at] = value
+    out = run(bad, do)[0]
+    assert torch.equal(out[:, :at], clean[:, :at]) and not torch.isfinite(out[:, at]).all(-1).any()
+    bad = do.clone()
+    bad[:, at] = value
+    grad = run(k, bad)[1]
+    assert torch.equal(grad[:, at + 1 :], dk_clean[:, at + 1 :]) and not torch.isfinite(grad[:, at]).all(-1).any()
