@@ -245,7 +245,7 @@ def _check_heads(q, k, v, rate, axes):
         raise NotImplementedError(f"head widths are 1 to {MAX_HEAD}, got {dk} and {dv}")
     if rate.shape != (H,) or rate.dtype != torch.float32 or not rate.is_contiguous():
         raise ValueError(f"rate must be a contiguous float32 tensor of {H} values, got {rate.dtype} {tuple(rate.shape)}")
-    if rate.requires_grad:
+    if rate.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("the rates are constants of the heads: no gradient is built for them")
     return H, dk, dv
 

@@ -194,3 +194,17 @@ def test_a_key_that_is_not_finite_reaches_no_earlier_token(ews, dtype, dk, dv, v
     bad[:, at] = value
     grad = run(k, bad)[1]
     assert torch.equal(grad[:, at + 1 :], dk_clean[:, at + 1 :]) and not torch.isfinite(grad[:, at]).all(-1).any()
+
+
+def test_rates_that_are_parameters_serve_without_gradients(ews):
+    """No gradient is built for the rates, so they are refused where one would be lost, and only there."""
+    q, k, v, rate, s0, _ = _inputs(FP32, 2, 5, 2, 2, 16, 16)
+    p = torch.nn.Parameter(rate.clone())
+    want = ews.decayed_attention(q, k, v, rate)
+    step = ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], rate, s0.clone())
+    with torch.no_grad():
+        assert torch.equal(ews.decayed_attention(q, k, v, p), want)
+        assert torch.equal(ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], p, s0.clone()), step)
+    for call in (lambda: ews.decayed_attention(q, k, v, p), lambda: ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], p, s0)):
+        with pytest.raises(NotImplementedError):
+            call()
