@@ -28,6 +28,8 @@
 // When (sample, head, slice) alone cannot fill the GPU, the axis is split: a state-only pass gives each
 // segment's own state, join_kernel chains them, and the segments run side by side from their states.
 // Rows at or beyond a sample's length are neither loaded nor multiplied; their outputs are zero.
+#include <cfloat>
+
 #include "ews_decay.cuh"
 
 namespace ews {
@@ -839,7 +841,7 @@ extern "C" int ews_decay_bwd(const ews_decay_args* a, ews_stream_t stream) {
     const int rc = check(a);
     if (rc != EWS_OK) return rc;
     if (a->batch == 0) return EWS_OK;
-    if (!(a->scale != 0.f)) return EWS_ERR_INVALID_ARGUMENT;
+    if (!(fabsf(a->scale) >= FLT_MIN && fabsf(a->scale) <= FLT_MAX)) return EWS_ERR_INVALID_ARGUMENT;  // 1 / scale is used too
     if (!a->rate || (a->steps > 0 && (!a->q || !a->k || !a->v || !a->dout || !a->dq || !a->dk_out || !a->dv_out)))
         return EWS_ERR_INVALID_ARGUMENT;
     const Sizes z = sizes(a, true);

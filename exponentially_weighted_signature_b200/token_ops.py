@@ -12,7 +12,6 @@ token operator on the device raises IndexError (at once under ``configure(check_
 from __future__ import annotations
 
 import functools
-import math
 import struct
 from typing import Optional
 
@@ -252,8 +251,8 @@ def _check_heads(q, k, v, rate, axes):
 
 def _scale(scale, dk):
     scale = dk**-0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or scale == 0.0:
-        raise ValueError(f"scale must be finite and not zero, got {scale}")
+    if not 2.0**-126 <= abs(scale) < 2.0**128 - 2.0**103:  # the kernels take it, and 1 / scale, in float32
+        raise ValueError(f"scale must be finite, not zero and within float32's normal range, got {scale}")
     return scale
 
 

@@ -356,7 +356,8 @@ int ews_embed_bwd(const void* ids, int ids_wide, const void* dout, int dtype, in
  * dv) float32 or NULL (zero). Outputs are contiguous: out (batch, steps, heads, dv) of `dtype`, final_state like
  * initial (may be NULL). dk, dv <= 128.
  *   ews_decay_bwd: from dout (strides like q) and dfinal (may be NULL) the gradients dq, dk_out, dv_out (contiguous,
- *   of `dtype`; shared heads summed in float32 in head order) and dinitial (float32, may be NULL). scale != 0.
+ *   of `dtype`; shared heads summed in float32 in head order) and dinitial (float32, may be NULL). |scale| within
+ *   float32's normal range (1 / scale is used too).
  *   ews_decay_step: one token per row on the states `state` (pool, heads, dk, dv), updated in place: q, k, v, out
  *   without the step axis (its stride is not read), row b on state slots[b] (int32; NULL: b). A negative slot is an
  *   idle row: zero output, no state touched; one >= pool likewise, with *status = EWS_ERR_INDEX. Two rows must not

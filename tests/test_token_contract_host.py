@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from exponentially_weighted_signature_b200 import engine
+from exponentially_weighted_signature_b200 import _lib, engine, token_ops
 
 
 class _Square(torch.autograd.Function):
@@ -65,3 +65,17 @@ def test_rates_have_values_after_a_build_without_memory():
     assert block.rate.is_meta
     assert torch.equal(block.to_empty(device="cpu").rate, want)
     assert _block().to("meta").rate.is_meta
+
+
+def test_a_scale_has_to_be_a_number_that_float32_holds():
+    """The backward carries a state over 1 / scale: neither may vanish or overflow."""
+    for bad in (0.0, float("inf"), float("nan"), 1e300, -1e39, 1e-46, 1e-39):
+        with pytest.raises(ValueError):
+            token_ops._scale(bad, 64)
+    for good in (-0.5, 2.0**-126, 3.4e38):
+        assert token_ops._scale(good, 64) == good
+    assert token_ops._scale(None, 64) == 0.125
+    lib = _lib.load()
+    for bad in (0.0, float("inf"), float("nan"), 1e-39):
+        args = token_ops._DECAY(2, 100, 4, 2, 64, 64, 1, bad, 16, 16, 16, *([0] * 9), 16, 0, 0, 16, 0, 16, 0, 0, 0, 0, 16, 16, 16, 0, 0, 0, 0)
+        assert lib.ews_decay_bwd(args, None) == 1
