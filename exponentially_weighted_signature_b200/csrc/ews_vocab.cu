@@ -69,7 +69,7 @@ struct Job {
     int m, n, k;
     int tiles_m, tiles_n, splits, blocks;  // k blocks of 64 a split, of every pair
     long units;
-    void* out;            // OUT: of the type of the inputs, rows n apart, or
+    bf16* out;            // OUT: rounded, rows n apart (bfloat16 inputs: dW of one split), or
     float* acc;           // (splits, m, n) float32 partials:
     int add;              // add to them (a later piece) rather than store
 };
@@ -81,7 +81,6 @@ struct Gemm {
     int run;              // k blocks in one accumulator: the whole range, or few (float32 gradients, see kRun)
     int* status;          // the caller's word: a bounded wait that ran out
     const int* live;      // rows that have a target: the logits' m, dH's m, dW's k
-    int f32;              // the inputs are float32
     // LSE, GRAD (m = rows, n = the piece's part of the vocabulary from v0 on)
     const int *target, *row;  // of the packed rows: the target, and which row it was
     int v0;
@@ -399,18 +398,8 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                                 for (int j = 0; j < 32; ++j)
                                     if (j < w) p[j] = add ? p[j] + v[j] : v[j];
                             }
-                        } else if (a.f32) {
-                            float* p = static_cast<float*>(job.out) + (long)row * job.n + col;
-                            if (w == 32 && (job.n & 3) == 0 && aligned16_dev(job.out)) {
-#pragma unroll
-                                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j < w) p[j] = v[j];
-                            }
                         } else {
-                            bf16* p = static_cast<bf16*>(job.out) + (long)row * job.n + col;
+                            bf16* p = job.out + (long)row * job.n + col;
                             if (w == 32 && (job.n & 7) == 0 && aligned16_dev(job.out)) {
 #pragma unroll
                                 for (int j = 0; j < 32; j += 8) Vec<bf16, true>::store(p + j, v + j);
@@ -828,7 +817,7 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     const RowPlan plan = row_plan(a->plan, a->rows);
     float* acc_w = p.acc_w ? reinterpret_cast<float*>(w + p.aw) : nullptr;
     Gemm base{};
-    base.status = a->status, base.f32 = sizeof(T) == 4;
+    base.status = a->status;
     base.live = plan.live, base.target = plan.target, base.row = plan.row, base.lse = a->lse, base.dloss = a->dloss;
     base.g = reinterpret_cast<bf16*>(w + p.g), base.planes = p.planes;
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
@@ -847,7 +836,8 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
         }
         if (a->dweight) {  // dW = G^T H: K is the rows
             o.job[1] = job_of(n, a->dim, a->rows, p.split_w);
-            o.job[1].out = out, o.job[1].acc = acc_w;
+            o.job[1].acc = acc_w;
+            if constexpr (sizeof(T) == 2) o.job[1].out = out;  // read where there are no partials
         }
         if ((rc = gemm<OUT>(o, go, wt, go, h, p.planes, s)) != EWS_OK) break;
         if (a->dweight && acc_w) rc = reduce<T>(a, acc_w, p.split_w, n, nullptr, out, s);
