@@ -208,3 +208,96 @@ def test_rates_that_are_parameters_serve_without_gradients(ews):
     for call in (lambda: ews.decayed_attention(q, k, v, p), lambda: ews.decayed_attention_step(q[:, 0], k[:, 0], v[:, 0], p, s0)):
         with pytest.raises(NotImplementedError):
             call()
+
+
+# ------------------------------------------------------------------------------------------ long axes, many pieces
+
+
+@pytest.mark.parametrize("dtype,B,T,H,Hk,dk,dv,lengths,state", [
+    (BF16, 1, 600, 1, 1, 37, 29, None, True),  # two segments of five chunks
+    (BF16, 2, 1100, 2, 1, 37, 101, [1100, 333], True),  # four, and a length that ends inside the second
+    (BF16, 2, 777, 2, 2, 70, 12, [0, 640], True),  # no token, and a length at a segment's edge
+    (BF16, 1, 901, 2, 2, 101, 90, None, False),
+    (FP32, 1, 700, 2, 1, 100, 40, None, True),
+    (FP32, 2, 1100, 1, 1, 128, 66, [321, 1100], True),
+    (FP32, 1, 520, 2, 2, 72, 128, None, False),
+])
+def test_split_axes_of_the_warp_level_form(ews, dtype, B, T, H, Hk, dk, dv, lengths, state):
+    """Odd bfloat16 widths and wide float32 heads over axes that are split: the segments' states, their join in both
+    directions, and what starts and ends in them."""
+    from test_gpu_token_ops import test_decayed_attention_and_gradients as whole
+
+    whole(ews, dtype, B, T, H, Hk, dk, dv, lengths, state)
+
+
+def _loss_case(ews, h, w, t, dl):
+    """Loss and gradients within the bounds of test_gpu_token_ops.test_vocab_loss_and_gradients."""
+    dtype = w.dtype
+    hl, wl = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ews.vocab_loss(hl, wl, t)
+    dh, dw = torch.autograd.grad(loss, (hl, wl), dl)
+    want, wh, ww, ab, p, gg, hz = _loss_ref(h, w, t, dl)
+    worst = F32 * ab.amax(1)
+    assert ((loss.double() - want).abs() <= 2 * worst + 1e-6 * (want.abs() + 20)).all()
+    eg = p * (2 * worst + 2e-6)[:, None] + (U if dtype == BF16 else 2.0**-21) * gg.abs()
+    for got, exact, err, form in ((dh, wh, eg @ w.double().abs(), gg.abs() @ w.double().abs()), (dw, ww, eg.T @ hz.abs(), gg.abs().T @ hz.abs())):
+        bound = 1.05 * err + F32 * form + (U if dtype == BF16 else 2.0**-23) * exact.abs() + 1e-30
+        assert ((got.double() - exact).abs() <= bound).all(), float(((got.double() - exact).abs() / bound).max())
+
+
+def test_float32_gradients_over_several_pieces(ews):
+    """9,000 rows of three planes by 5,003 entries are more than one piece of the softmax gradient."""
+    n, V, D = 9000, 5003, 24
+    g = _gen(71)
+    h = torch.randn((n, D), device="cuda", generator=g)
+    w = torch.randn((V, D), device="cuda", generator=g) * 2 / D**0.5
+    t = torch.randint(0, V, (n,), device="cuda", generator=g)
+    t[::7] = -100
+    _loss_case(ews, h, w, t, torch.rand((n,), device="cuda", generator=g) + 0.1)
+
+
+@pytest.mark.parametrize("dtype,V,D,planes", [(FP32, 90001, 509, 3), (BF16, 270001, 509, 1)])
+def test_packed_weights_over_several_pieces(ews, dtype, V, D, planes):
+    """A weight that is packed (512 columns after padding) in two pieces: targets on both sides of the pieces' edge."""
+    assert 2**27 < V * 512 * planes < 2**28
+    edge = ((V + 1) // 2 + 255) // 256 * 256
+    g = _gen(73)
+    t = torch.tensor([0, edge - 1, edge, edge + 1, V - 1, 256, -100, V // 3], device="cuda")
+    h = torch.randn((len(t), D), device="cuda", generator=g).to(dtype)
+    w = (torch.randn((V, D), device="cuda", generator=g) / D**0.5).to(dtype)
+    _loss_case(ews, h, w, t, torch.rand((len(t),), device="cuda", generator=g) + 0.1)
+
+
+def test_backwards_in_a_cuda_graph(ews):
+    """Forward and backward captured once and replayed on new contents."""
+    q, k, v, rate, s0, g = _inputs(BF16, 2, 300, 2, 1, 64, 64, seed=83)
+    q, k, v, s0 = (x.requires_grad_() for x in (q, k, v, s0))
+    h, w = (torch.randn((n, 64), device="cuda", generator=g).to(BF16).requires_grad_() for n in (400, 500))
+    t = torch.randint(0, 500, (400,), device="cuda", generator=g)
+    do = torch.randn((2, 300, 2, 64), device="cuda", generator=g).to(BF16)
+    dl = torch.rand((400,), device="cuda", generator=g)
+
+    def run():
+        out, end = ews.decayed_attention(q, k, v, rate, initial_state=s0, return_state=True)
+        x = ews.token_embedding(t, w, scale=2.0)
+        return [*torch.autograd.grad((out, end), (q, k, v, s0), (do, s0.detach())), *torch.autograd.grad(x, (w,), h.detach()),
+                *torch.autograd.grad(ews.vocab_loss(h, w, t), (h, w), dl)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    with torch.no_grad():
+        for x in (q, k, v, s0, h, w, do):
+            x.copy_(torch.randn(x.shape, device="cuda", generator=g))
+        dl.copy_(torch.rand(dl.shape, device="cuda", generator=g))
+        t.copy_(torch.randint(0, 500, (400,), device="cuda", generator=g))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(held, run()):
+        assert torch.equal(a, b)
