@@ -208,9 +208,10 @@ __global__ void __launch_bounds__(FTHR, 1) f32_kernel(const __grid_constant__ Ch
                             float e[32];
                             tmem_ld32(tmem + TP + lanes + cb * 32, e);
                             if (m < FC || cb == quarter) {
-                                const uint32_t live = live_scores(cb, quarter, lane, m, a.rev);
+                                // as two bounds: as bits the training case takes 534 us instead of 520
+                                const Live live = live_scores(cb, quarter, lane, m, a.rev);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) e[j] = live & (1u << j) ? e[j] : 0.f;
+                                for (int j = 0; j < 32; ++j) e[j] = j >= live.from && j < live.to ? e[j] : 0.f;
                             }
                             const uint32_t g = row_tab - cb * 256;
 #pragma unroll

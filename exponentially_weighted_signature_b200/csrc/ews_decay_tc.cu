@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_kernel(const __grid_constant__ Cha
                             float v[32];
                             tmem_ld32(tmem + TP + lanes + cb * 32, v);
                             if (m < TC || cb == quarter) {
-                                const uint32_t live = live_scores(cb, quarter, lane, m, a.rev);
+                                // as bits: as two bounds a score the training case takes 285 us instead of 274
+                                const uint32_t live = live_scores(cb, quarter, lane, m, a.rev).bits();
 #pragma unroll
                                 for (int j = 0; j < 32; ++j) v[j] = live & (1u << j) ? v[j] : 0.f;
                             }

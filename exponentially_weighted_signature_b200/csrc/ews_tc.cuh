@@ -178,10 +178,13 @@ __device__ __forceinline__ void put_decay(unsigned char* tab, int tid, int threa
 // Which of a row's scores against the 32 tokens from 32 cb on count, row 32 quarter + lane of a chunk of m tokens: the tokens
 // exist, and none lies behind the row (reversed: before it). The others may be anything and are dropped, not weighted with
 // zero: what is not finite in a token must not reach the tokens that come first.
-__device__ __forceinline__ uint32_t live_scores(int cb, int quarter, int lane, int m, bool rev) {
-    const int to = cb == quarter && !rev ? min(m - cb * 32, lane + 1) : m - cb * 32;
-    const uint32_t below = to >= 32 ? kFull : to > 0 ? (1u << to) - 1u : 0u;
-    return cb == quarter && rev ? below & (kFull << lane) : below;
+struct Live {
+    int from, to;  // [from, to) of the 32
+    __device__ __forceinline__ uint32_t bits() const { return (to >= 32 ? kFull : to > 0 ? (1u << to) - 1u : 0u) & (kFull << from); }
+};
+__device__ __forceinline__ Live live_scores(int cb, int quarter, int lane, int m, bool rev) {
+    const bool diagonal = cb == quarter;
+    return Live{diagonal && rev ? lane : 0, diagonal && !rev ? min(m - cb * 32, lane + 1) : m - cb * 32};
 }
 __device__ __forceinline__ float decay_of(float rate, int n) { return n <= 0 ? 1.f : expf(-rate * (float)n); }
 
