@@ -15,8 +15,8 @@
 // Which form runs: bfloat16 streams that TMA can read (16-byte-aligned rows and strides) run in ews_decay_tc.cu, float32
 // with x and y up to 64 wide in ews_decay_f32.cu, both on the 5th-generation tensor core; the rest (odd bfloat16 widths and
 // strides, wide float32 heads) here, on warp-level matrix instructions. Both sides of each rule, forward and backward:
-// bfloat16 B = 8, T = 2048, 16 heads of 128: 269 us there, 857 here; float32 B = 16, T = 1440, 8 heads of 64, shared in
-// pairs, ragged: 522 us there, 1,717 here. What bounds this form is the legacy instructions' rate (2,048 operations a
+// bfloat16 B = 8, T = 2048, 16 heads of 128: 274 us there, 857 here; float32 B = 16, T = 1440, 8 heads of 64, shared in
+// pairs, ragged: 517 us there, 1,717 here. What bounds this form is the legacy instructions' rate (2,048 operations a
 // cycle and SM) and the splitting of float32 fragments, each of which four warps repeat.
 //
 // chain_kernel: a CTA of four warps owns a (sample, head, segment of the axis, slice of up to 64 columns of z); it walks

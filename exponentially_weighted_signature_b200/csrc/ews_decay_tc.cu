@@ -20,6 +20,9 @@
 // (2,300) follow one another, and a role's instructions come slowly (its code runs once a chunk, and the roles' code
 // together is larger than the inner instruction cache: unrolled loops lost more than they gained). A third group for
 // the output took 96 registers a thread and spilled: 329 us for the training case instead of 290 at the time.
+// Rounded to bfloat16 on the way are the decayed scores (the operand of O2 comes from tensor memory in that type) and the
+// state's copy for O1; the state itself stays in float32. For random inputs the output is then 2.3e-3 from the exact one
+// (norm over norm) where its own rounding alone leaves 1.7e-3.
 // The states' pass over 17,984 tokens of 16 heads (three pieces) takes 62 us, the outputs' 74 us.
 //
 // Reversed chains keep the rows' order and walk the chunks down: decays are then g^(j-i) for j >= i, a row's weight of

@@ -17,8 +17,10 @@
 //   rows_kernel     one warp per 16 x 32 bytes of four table rows: sums a run inside one segment directly, a
 //                   longer one from its partials in order.
 // Bound by HBM: N rows read, V rows written. Measured for N = 65,536, V = 131,072, D = 512, float32: the lookup 37 us
-// (268 MB), the sort 41 us, the partials 17 us, the rows 71 us (402 MB, 5.7 TB/s); the sort is bound by its rounds of
-// rank and scatter on eight SMs (one CTA instead of eight: 23 us for 1,024 positions, 18 with eight).
+// (268 MB), the sort 41 us, the partials 20 us, the rows 71 us (402 MB, 5.7 TB/s); the sort is bound by its rounds of
+// rank and scatter on eight SMs (one CTA instead of eight: 23 us for 1,024 positions, 18 with eight). It is one cluster
+// whatever the number of positions, which limits it: 23, 41, 123, 433 us for 16 K, 64 K, 256 K, 1 M of them, of 91, 140, 304,
+// 891 us for the whole gradient, whose bytes take 47, 62, 125, 375 us.
 #include "ews_token.cuh"
 
 namespace ews {

@@ -20,7 +20,7 @@
 // burst rate and above its rate under the power cap; for 7,370 rows, D = 1,024 a piece of 10,240 entries takes 122 us for
 // GRAD (1.27 PFLOP/s) and 256 us for both gradients in one launch (1.21 PFLOP/s; as launches of their own, 116 and 119 us
 // for 7,424 entries, each left a fifth of its last wave of tiles idle). What bounds them is the tensor pipe under the
-// power cap. Pieces of 16, 32, 64 M entries of G took 3.95, 3.24, 3.16 ms for a step that takes 3.02 ms with 128 M.
+// power cap. Pieces of 16, 32, 64 M entries of G took 3.95, 3.24, 3.16 ms for a step that took 3.02 ms with 128 M (2.80 now).
 // Rows without a target cost nothing: a first kernel lists the rows that have one, and everything after works on those
 // rows alone, packed (their number stays on the device: the kernels read it).
 #include "ews_tc.cuh"
@@ -53,7 +53,8 @@ __device__ __forceinline__ float ex2(float x) {
 // that it does not average out in the sums. The first row's mantissa, a number in [1, 2), is therefore left out of G and
 // multiplied into the float32 sums: a common loss gradient becomes a power of two, which rounds nothing, and no entry
 // changes its size by more than 2. Without it one random bfloat16 case in four had a gradient 1.5 times as far from
-// the exact one as a float32 G rounded once at the end, with it one in a hundred.
+// the exact one as a float32 G rounded once at the end, with it one in a hundred. Loss gradients that differ from row to row,
+// or a first row that differs from all others, leave the rounding as it is.
 __device__ __forceinline__ float common_factor(const float* dloss, const int* row, int live) {
     const float x = live > 0 ? fabsf(dloss[row[0]]) : 0.f;
     if (!(x > 1e-37f && x < 1e37f)) return 1.f;

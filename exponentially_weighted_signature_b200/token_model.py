@@ -69,7 +69,8 @@ class DecayBlock(nn.Module):
 class TokenModel(nn.Module):
     """Embedding (scaled by sqrt(hidden)), blocks, RMSNorm, and logits on the embedding's table.
 
-    ``mixers``: one entry a block, "decay" (DecayBlock) or "ews" (EWSBlock with ``ews_kwargs``; float32)."""
+    ``mixers``: one entry a block, "decay" (DecayBlock) or "ews" (EWSBlock with ``ews_kwargs``; float32). ``seed`` is for the
+    table and the EWS blocks' generators; linear layers draw from torch's global generator, as in ``StackedEWS``."""
 
     def __init__(self, vocab: int, hidden_dim: int = 128, heads: int = 4, mixers=("decay", "decay"), *,
                  kv_heads: Optional[int] = None, head_dim: Optional[int] = None, ews_kwargs: Optional[dict] = None, seed: int = 0):
