@@ -9,6 +9,7 @@ from . import params, series
 from .layer import COMBINE_KINDS, EWS, BToSignature, LogEWS, configure
 from .logsig import log_level_sizes, log_signature_dim
 from .params import AParamBlockDiag, AParamConstant, AParamDiag, AParamEFM, AParamGeneral, AParamJordanRepeated, B
+from .recur_ops import gated_recurrence, gated_recurrence_step
 from .series import check_series_q, series_error_bound, suggest_series_q
 from .token_model import DecayBlock, TokenModel
 from .token_ops import decayed_attention, decayed_attention_step, token_embedding, vocab_loss
@@ -35,6 +36,8 @@ __all__ = [
     "decayed_attention_step",
     "token_embedding",
     "vocab_loss",
+    "gated_recurrence",
+    "gated_recurrence_step",
     "log_level_sizes",
     "log_signature_dim",
     "params",

@@ -1,0 +1,151 @@
+"""The gated linear recurrence: a mixer whose decays depend on the token, for prompts, training and single tokens.
+
+``gated_recurrence`` over sequences, ``gated_recurrence_step`` (one token per row on a pool of states). Types, streams,
+derivatives and errors are those of the token operators (token_ops.py).
+"""
+
+from __future__ import annotations
+
+import functools
+import struct
+from typing import Optional
+
+import torch
+
+from . import _lib, engine
+from .engine import first_order
+from .token_ops import _DTYPES, _addr, _device, _dtype, _last_contiguous, _launch, _work
+
+_RECUR = struct.Struct("@4i3P6q3P3PP2qP3P2PPNP").pack  # ews_recur_args
+
+
+def _args(x, decay, gate, rate, lengths=None, initial=None, out=None, end=None, carry=None, dout=None, dend=None,
+          grads=(None, None, None), drate=None, d0=None, work=None):
+    B, T, C = x.shape
+    return _RECUR(B, T, C, _DTYPES[x.dtype], x.data_ptr(), decay.data_ptr(), gate.data_ptr(), *x.stride()[:2], *decay.stride()[:2],
+                  *gate.stride()[:2], rate.data_ptr(), _addr(lengths), _addr(initial), _addr(out), _addr(end), _addr(carry),
+                  _addr(dout), *((0, 0) if dout is None else dout.stride()[:2]), _addr(dend), *map(_addr, grads), _addr(drate),
+                  _addr(d0), _addr(work), 0 if work is None else work.numel(), engine.index_word(x.get_device())[0])
+
+
+@functools.lru_cache(maxsize=256)
+def _sizes(B: int, T: int, C: int, code: int):
+    """(carry, forward's and backward's workspace) in bytes: a function of the sizes alone."""
+    lib, args = _lib.load(), _RECUR(B, T, C, code, *([0] * 27))
+    return lib.ews_recur_carry_size(args), lib.ews_recur_work_size(args, 0), lib.ews_recur_work_size(args, 1)
+
+
+def _forward(x, decay, gate, rate, initial, lengths, want_state, want_carry):
+    B, T, C = x.shape
+    carry_bytes, work_bytes, _ = _sizes(B, T, C, _DTYPES[x.dtype])
+    out = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
+    end = torch.empty((B, C), dtype=torch.float32, device=x.device) if want_state else None
+    carry = torch.empty(carry_bytes // 4, dtype=torch.float32, device=x.device) if want_carry else None
+    args = _args(x, decay, gate, rate, lengths, initial, out, end, carry, work=(work := _work(work_bytes, x)))
+    _launch(x.get_device(), "ews_recur_fwd", B * T, _lib.load().ews_recur_fwd, args)
+    return out, end, carry
+
+
+class _Recurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, decay, gate, rate, initial, lengths, want_state):
+        x, decay, gate = _last_contiguous(x), _last_contiguous(decay), _last_contiguous(gate)
+        out, end, carry = _forward(x, decay, gate, rate, initial, lengths, want_state, True)
+        ctx.save_for_backward(x, decay, gate, rate, initial, lengths, carry)
+        ctx.set_materialize_grads(False)
+        return out, end
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dout, dend):
+        x, decay, gate, rate, initial, lengths, carry = ctx.saved_tensors
+        B, T, C = x.shape
+        dout = None if dout is None else _last_contiguous(dout)
+        dend = None if dend is None else dend.contiguous()
+        grads = [torch.empty((B, T, C), dtype=x.dtype, device=x.device) for _ in range(3)]
+        drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
+        d0 = torch.empty((B, C), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[4] else None
+        work = _work(_sizes(B, T, C, _DTYPES[x.dtype])[2], x)
+        args = _args(x, decay, gate, rate, lengths, initial, None, None, carry, dout, dend, grads, drate, d0, work)
+        _launch(x.get_device(), "ews_recur_bwd", B * T, _lib.load().ews_recur_bwd, args)
+        return (*grads, drate, d0, None, None)
+
+
+def _check(x, decay, gate, rate, axes):
+    if not (x.dtype == decay.dtype == gate.dtype):
+        raise TypeError(f"x, decay and gate must share a type, got {x.dtype}, {decay.dtype}, {gate.dtype}")
+    _dtype(x, "x, decay and gate")
+    if x.dim() != axes or x.shape[-1] == 0 or decay.shape != x.shape or gate.shape != x.shape:
+        raise ValueError(f"x, decay and gate must share a shape of {axes} axes with channels, got {tuple(x.shape)}, "
+                         f"{tuple(decay.shape)}, {tuple(gate.shape)}")
+    C = x.shape[-1]
+    if rate.shape != (C,) or rate.dtype != torch.float32 or not rate.is_contiguous():
+        raise ValueError(f"rate must be a contiguous float32 tensor of {C} values, got {rate.dtype} {tuple(rate.shape)}")
+    return C
+
+
+def gated_recurrence(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor, rate: torch.Tensor, *,
+                     initial_state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                     return_state: bool = False):
+    """A linear recurrence a channel whose decay and input the token gates:
+    ``a_t = exp(-rate sigmoid(decay_t))``, ``h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t``.
+
+    x, decay, gate (B, T, C), float32 or bfloat16, any strides (views of one projection, for instance); rate (C,) float32,
+    zero or larger (a negative one gives NaN): a diagonal generator's rates, with ``sigmoid(decay)`` as the clock's step.
+    A decay of -inf, or of its type's lowest value, passes the state on unchanged and takes no input. initial_state (B, C)
+    float32 or None (zero). lengths (B,) int32: positions at or beyond a sample's length are not read, give zeros and
+    leave the state.
+
+    Returns h (B, T, C), with ``return_state`` also the state after the last token (B, C) float32, for
+    ``gated_recurrence_step`` or the next piece of a long sequence; states and the scan are float32 whatever the type.
+    Differentiable in x, decay, gate, rate and initial_state; results do not depend on timing."""
+    C = _check(x, decay, gate, rate, 3)
+    B = x.shape[0]
+    if initial_state is not None:
+        if initial_state.shape != (B, C) or initial_state.dtype != torch.float32:
+            raise ValueError(f"initial_state must be float32 {(B, C)}, got {initial_state.dtype} {tuple(initial_state.shape)}")
+        initial_state = initial_state.contiguous()
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.dtype != torch.int32:
+            raise ValueError(f"lengths must be int32 ({B},), got {lengths.dtype} {tuple(lengths.shape)}")
+        lengths = lengths.contiguous()
+    _device(x, decay, gate, rate, initial_state, lengths)
+    want = bool(return_state)
+    if torch.is_grad_enabled() and (x.requires_grad or decay.requires_grad or gate.requires_grad or rate.requires_grad
+                                    or initial_state is not None and initial_state.requires_grad):
+        out, end = _Recurrence.apply(x, decay, gate, rate, initial_state, lengths, want)
+    else:
+        x, decay, gate = _last_contiguous(x), _last_contiguous(decay), _last_contiguous(gate)
+        out, end, _ = _forward(x, decay, gate, rate, initial_state, lengths, want, False)
+    return (out, end) if want else out
+
+
+def gated_recurrence_step(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor, rate: torch.Tensor, state: torch.Tensor, *,
+                          slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token per row of ``gated_recurrence`` on a pool of states, updated in place.
+
+    x, decay, gate (B, C); state (P, C) float32, contiguous. Row b works on state ``slots[b]`` (int32 (B,); None: b, with
+    P >= B). A negative slot is a row without a request: its output is zero and no state is touched. Two rows must not share
+    a slot; one out of range gives a zero row and IndexError on the next call. Returns h (B, C). For serving: no
+    gradient; a backward that needs the states as they were raises, as after any operation in place."""
+    C = _check(x, decay, gate, rate, 2)
+    B = x.shape[0]
+    if state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous float32 (P, {C}), got {state.dtype} {tuple(state.shape)}")
+    if slots is None:
+        if state.shape[0] < B:
+            raise ValueError(f"{B} rows need as many states or slots, got {state.shape[0]} states")
+    elif slots.shape != (B,) or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise ValueError(f"slots must be contiguous int32 ({B},), got {slots.dtype} {tuple(slots.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or decay.requires_grad or gate.requires_grad or rate.requires_grad
+                                    or state.requires_grad):
+        raise RuntimeError("gated_recurrence_step has no gradient: call it under torch.no_grad()")
+    idx = _device(x, decay, gate, rate, state, slots)
+    x, decay, gate = _last_contiguous(x), _last_contiguous(decay), _last_contiguous(gate)
+    out = torch.empty((B, C), dtype=x.dtype, device=x.device)
+    args = _RECUR(B, 1, C, _DTYPES[x.dtype], x.data_ptr(), decay.data_ptr(), gate.data_ptr(), x.stride(0), 0, decay.stride(0), 0,
+                  gate.stride(0), 0, rate.data_ptr(), 0, 0, out.data_ptr(), *([0] * 13), engine.index_word(idx)[0])
+    _launch(idx, "ews_recur_step", B, _lib.load().ews_recur_step, args, _addr(slots), state.shape[0], state.data_ptr())
+    if not state.is_inference():  # autograd cannot see the write: a backward that saved these states must
+        torch.autograd.graph.increment_version(state)
+    return out

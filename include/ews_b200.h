@@ -388,6 +388,44 @@ int ews_decay_fwd(const ews_decay_args* args, ews_stream_t stream);
 int ews_decay_bwd(const ews_decay_args* args, ews_stream_t stream);
 int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float* state, ews_stream_t stream);
 
+/* ---- gated linear recurrence ----------------------------------------------------------------------
+ * For every sample and channel: a = exp(-rate sigmoid(decay_t)), h_t = a h_{t-1} + sqrt(1 - a^2) sigmoid(gate_t) x_t.
+ * x, decay, gate (batch, steps, channels) of `dtype` with contiguous last axes and element strides {batch, step}; rate
+ * (channels) float32, not negative (a negative one gives NaN); lengths (batch) int32 or NULL: positions at or beyond a
+ * sample's length are not read, give zeros and leave the state; initial (batch, channels) float32 or NULL (zero). out (batch,
+ * steps, channels) of `dtype`, contiguous; final_state like initial, may be NULL. carry: ews_recur_carry_size(args) bytes
+ * for the backward, or NULL.
+ *   ews_recur_bwd: from dout (strides as x; NULL: zero), dfinal (may be NULL) and the forward's carry the gradients dx, ddecay,
+ *   dgate (contiguous, of `dtype`), drate (channels float32, may be NULL) and dinitial (float32, may be NULL).
+ *   ews_recur_step: one token per row on the states `state` (pool, channels) float32, updated in place: x, decay, gate, out
+ *   without the step axis (its stride is not read), row b on state slots[b] (int32; NULL: b). A negative slot is an idle
+ *   row: zero output, no state touched; one >= pool likewise, with *status = EWS_ERR_INDEX. Two rows must not share a slot.
+ * status: device or pinned host memory, may be NULL; a bounded device wait that ran out sets
+ * EWS_ERR_LOOKBACK_TIMEOUT (the outputs are then invalid). `work`: ews_recur_work_size(args, backward) bytes. */
+typedef struct {
+    int batch, steps, channels, dtype;
+    const void *x, *decay, *gate;
+    int64_t x_stride[2], decay_stride[2], gate_stride[2];
+    const float* rate;
+    const int* lengths;
+    const float* initial;
+    void* out;
+    float *final_state, *carry;
+    const void* dout;
+    int64_t dout_stride[2];
+    const float* dfinal;
+    void *dx, *ddecay, *dgate;
+    float *drate, *dinitial;
+    void* work;
+    size_t work_bytes;
+    int* status;
+} ews_recur_args;
+size_t ews_recur_carry_size(const ews_recur_args* args);
+size_t ews_recur_work_size(const ews_recur_args* args, int backward);
+int ews_recur_fwd(const ews_recur_args* args, ews_stream_t stream);
+int ews_recur_bwd(const ews_recur_args* args, ews_stream_t stream);
+int ews_recur_step(const ews_recur_args* args, const int* slots, int pool, float* state, ews_stream_t stream);
+
 /* ---- vocabulary loss ------------------------------------------------------------------------------
  * loss_n = logsumexp_v <hidden_n, weight_v> - <hidden_n, weight_{t_n}> for hidden (rows, dim) and weight (vocab, dim)
  * of `dtype` (rows `hidden_stride` / `weight_stride` elements apart), targets (rows) int64 (targets_wide) or int32;
