@@ -16,17 +16,25 @@
 // and the results do not depend on timing. The backward reads no states: the forward leaves one a tile of the backward
 // (float32, 1 / 64 of the stream), from which the tile runs the recurrence again. So the gradient of the rates, a float32 sum
 // over all tokens, does not see the rounding of the stored states, and a stream less is read.
-#include "ews_token.cuh"
+#include <float.h>
+
+#include "ews_tc.cuh"
 
 namespace ews {
 namespace recur {
 
 using namespace token;
+using tc5::add2;
+using tc5::fma2;
+using tc5::mul2;
+using tc5::pair;
+using tc5::unpair;
 
 constexpr int kMaxWarps = 16;
-constexpr int FL = 16, FW = 8;  // forward: tokens a warp, warps a tile
-constexpr int BL = 8, BW = 8;   // backward
+constexpr int FL = 16, FW = 8, FCTAS = 2;  // forward: tokens a warp, warps a tile, CTAs an SM
+constexpr int BL = 8, BW = 8, BCTAS = 2;   // backward
 constexpr int FT = FL * FW, BT = BL * BW;
+constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 struct Stream {
@@ -50,60 +58,154 @@ struct Params {
     // look-back
     DeviceStatus* st;
     int* flags;    // (batch, blocks, tiles)
-    float2* maps;  // (batch, tiles, channels)
-    float* ends;   // (batch, tiles, channels)
+    float *map_a, *map_h, *ends;  // (batch, tiles, channels)
     int* status;
 };
 
-// V elements of a stream: as floats, zero where there are none.
+// V floats, as one packed operand where there are two: the kernels are bound by their instructions, and one handles a pair.
+template <int V>
+struct F;
+template <>
+struct F<1> {
+    float r;
+    __device__ __forceinline__ F() {}
+    __device__ __forceinline__ F(float x) : r(x) {}
+    __device__ __forceinline__ float get(int) const { return r; }
+    template <typename Fn>
+    __device__ __forceinline__ F each(Fn f) const { return F(f(r)); }
+    template <typename Fn>
+    __device__ __forceinline__ static F make(Fn f) { return F(f(0)); }
+};
+template <>
+struct F<2> {
+    uint64_t r;
+    __device__ __forceinline__ F() {}
+    __device__ __forceinline__ F(float x) : r(pair(x, x)) {}
+    __device__ __forceinline__ F(float x, float y) : r(pair(x, y)) {}
+    __device__ __forceinline__ float get(int j) const {
+        float x, y;
+        unpair(r, x, y);
+        return j ? y : x;
+    }
+    template <typename Fn>
+    __device__ __forceinline__ F each(Fn f) const { return F(f(get(0)), f(get(1))); }
+    template <typename Fn>
+    __device__ __forceinline__ static F make(Fn f) { return F(f(0), f(1)); }
+};
+// rounded as the packed ones are: whether a call's tensors allow pairs does not change its results
+__device__ __forceinline__ F<1> operator*(F<1> a, F<1> b) { return F<1>(__fmul_rn(a.r, b.r)); }
+__device__ __forceinline__ F<1> operator+(F<1> a, F<1> b) { return F<1>(__fadd_rn(a.r, b.r)); }
+__device__ __forceinline__ F<1> fma(F<1> a, F<1> b, F<1> c) { return F<1>(fmaf(a.r, b.r, c.r)); }
+__device__ __forceinline__ F<2> operator*(F<2> a, F<2> b) {
+    F<2> o;
+    o.r = mul2(a.r, b.r);
+    return o;
+}
+__device__ __forceinline__ F<2> operator+(F<2> a, F<2> b) {
+    F<2> o;
+    o.r = add2(a.r, b.r);
+    return o;
+}
+__device__ __forceinline__ F<2> fma(F<2> a, F<2> b, F<2> c) {
+    F<2> o;
+    o.r = fma2(a.r, b.r, c.r);
+    return o;
+}
+
+// V elements of a stream.
 template <typename T, int V>
 struct Word;
 template <>
 struct Word<float, 1> {
     float w;
     __device__ __forceinline__ void load(const float* p) { w = __ldg(p); }
-    __device__ __forceinline__ void zero() { w = 0.f; }
-    __device__ __forceinline__ float get(int) const { return w; }
-    __device__ static __forceinline__ void store(float* p, const float v[1]) { *p = v[0]; }
+    __device__ __forceinline__ void fill(float x) { w = x; }
+    __device__ __forceinline__ F<1> get() const { return F<1>(w); }
+    __device__ static __forceinline__ void store(float* p, F<1> v) { *p = v.r; }
 };
 template <>
 struct Word<bf16, 1> {
     bf16 w;
     __device__ __forceinline__ void load(const bf16* p) { w = __ldg(p); }
-    __device__ __forceinline__ void zero() { w = __float2bfloat16_rn(0.f); }
-    __device__ __forceinline__ float get(int) const { return __bfloat162float(w); }
-    __device__ static __forceinline__ void store(bf16* p, const float v[1]) { *p = __float2bfloat16_rn(v[0]); }
+    __device__ __forceinline__ void fill(float x) { w = __float2bfloat16_rn(x); }
+    __device__ __forceinline__ F<1> get() const { return F<1>(__bfloat162float(w)); }
+    __device__ static __forceinline__ void store(bf16* p, F<1> v) { *p = __float2bfloat16_rn(v.r); }
 };
 template <>
 struct Word<bf16, 2> {
     uint32_t w;
     __device__ __forceinline__ void load(const bf16* p) { w = __ldg(reinterpret_cast<const uint32_t*>(p)); }
-    __device__ __forceinline__ void zero() { w = 0u; }
-    __device__ __forceinline__ float get(int j) const { return j ? bf16_hi(w) : bf16_lo(w); }
-    __device__ static __forceinline__ void store(bf16* p, const float v[2]) { *reinterpret_cast<uint32_t*>(p) = pack_bf16(v[0], v[1]); }
+    __device__ __forceinline__ void fill(float x) { w = pack_bf16(x, x); }
+    __device__ __forceinline__ F<2> get() const { return F<2>(bf16_lo(w), bf16_hi(w)); }
+    __device__ static __forceinline__ void store(bf16* p, F<2> v) { *reinterpret_cast<uint32_t*>(p) = pack_bf16(v.get(0), v.get(1)); }
 };
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// The exponent unit's own instructions; what lies below the normal range counts as zero (a sigmoid of less than -87, say),
+// which spares their corrections, a third of the kernels' instructions.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float root(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float inverse_root(float x) {
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int V>
+__device__ __forceinline__ F<V> sigmoid(F<V> x) {
+    const F<V> e = (x * F<V>(-kLog2e)).each([](float t) { return ex2(t); });
+    return (e + F<V>(1.f)).each([](float t) { return rcp(t); });
+}
 
 // a = exp(-p) and w = 1 - a^2. Up to p = 0.175 from q = 1 - exp(-p) by its series (the first dropped term is 2^-27 of q there):
 // a = 1 - q then has no error but its rounding, where the exponent unit's 2^-22 would add up over the hundreds of tokens such
 // an a remembers, and w = q (2 - q) loses nothing to cancellation. Beyond, a state forgets within some six tokens.
-struct Decay {
-    float a, w;
-};
-__device__ __forceinline__ Decay decay_of(float p) {
-    float q = fmaf(p, -1.f / 720.f, 1.f / 120.f);
-    q = fmaf(p, q, -1.f / 24.f);
-    q = fmaf(p, q, 1.f / 6.f);
-    q = fmaf(p, q, -0.5f);
-    q = fmaf(p * p, q, p);
-    const float e = __expf(-p);
-    return p < 0.175f ? Decay{1.f - q, q * (2.f - q)} : Decay{e, fmaf(-e, e, 1.f)};
+constexpr float kSeries = 0.175f;
+template <int V>
+__device__ __forceinline__ F<V> decay_loss(F<V> p) {
+    F<V> q = fma(p, F<V>(-1.f / 720.f), F<V>(1.f / 120.f));
+    q = fma(p, q, F<V>(-1.f / 24.f));
+    q = fma(p, q, F<V>(1.f / 6.f));
+    q = fma(p, q, F<V>(-0.5f));
+    return fma(p * p, q, p);
 }
-__device__ __forceinline__ float root(float w) {
-    float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(w));
-    return r;
+template <int V>
+struct Decay {
+    F<V> a, w;
+};
+template <int V>
+__device__ __forceinline__ Decay<V> decay_of(F<V> p) {
+    const F<V> q = decay_loss(p), near = fma(q, F<V>(-1.f), F<V>(1.f)), w = fma(q, near, q);
+    const F<V> e = (p * F<V>(-kLog2e)).each([](float t) { return ex2(t); });
+    Decay<V> d;
+    d.a = F<V>::make([&](int j) { return p.get(j) < kSeries ? near.get(j) : e.get(j); });
+    d.w = F<V>::make([&](int j) { return p.get(j) < kSeries ? w.get(j) : fmaf(-e.get(j), e.get(j), 1.f); });
+    return d;
+}
+// w once more where a is at hand.
+template <int V>
+__device__ __forceinline__ F<V> rest_of(F<V> p, F<V> a) {
+    const F<V> q = decay_loss(p), w = fma(q, fma(q, F<V>(-1.f), F<V>(1.f)), q);
+    return F<V>::make([&](int j) { return p.get(j) < kSeries ? w.get(j) : fmaf(-a.get(j), a.get(j), 1.f); });
+}
+template <int V>
+__device__ __forceinline__ F<V> root(F<V> w) { return w.each([](float t) { return root(t); }); }
+
+// A channel's rate; an infinite one as float32's largest, so that a shut gate's product with it is zero.
+__device__ __forceinline__ float rate_at(const float* p) {
+    const float r = __ldg(p);
+    return r > FLT_MAX ? FLT_MAX : r;
 }
 
 struct Tile {
@@ -128,33 +230,41 @@ __device__ __forceinline__ Tile tile_of(const Params<T>& a, long ticket, bool do
 
 template <int V>
 struct Shared {
-    float2 map[kMaxWarps][32 * V];
+    F<V> A[kMaxWarps][32], H[kMaxWarps][32];
     int flag[kMaxWarps];
     int ticket;
 };
 
-// The state that comes into the tile, from the tiles before it (down: behind it): `mine` channels of the lane. Every thread
-// of the CTA calls it, after the tile's own map was published; false when a wait ran out.
+// V consecutive floats of the lane's channels; what lies beyond the last is not touched.
+template <int V>
+__device__ __forceinline__ F<V> load_channels(const float* p, int c, int channels) {
+    return F<V>::make([&](int j) { return c + j < channels ? __ldcg(p + c + j) : 0.f; });
+}
+template <int V>
+__device__ __forceinline__ void store_channels(float* p, int c, int channels, F<V> v) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (c + j < channels) __stcg(p + c + j, v.get(j));
+}
+
+// The state that comes into the tile from the tiles before it (down: behind it). Every thread of the CTA calls it, after the
+// tile's own map was published; false when a wait ran out.
 template <typename T, int V>
-__device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, bool down, Shared<V>& sh, int warp, int lane, int warps, float c[V]) {
+__device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, bool down, Shared<V>& sh, int warp, int lane, int warps, F<V>* state) {
     const int step = down ? 1 : -1;
     const int before = down ? a.tiles - 1 - t.tt : t.tt;  // how many there are
     const int window = before < warps ? before : warps;
-    int flag = kFlagEmpty;
-    const int at = t.tt + step * (1 + warp);
     if (warp < window) {
+        const int at = t.tt + step * (1 + warp);
         // the last of the window has to have its state: nothing further back is folded
-        flag = wait_slot(a.flags + t.slot + at, a.st, kDefaultSpinLimit, t.slot + at, warp == window - 1 ? kFlagIncl : kFlagAgg);
+        const int flag = wait_slot(a.flags + t.slot + at, a.st, kDefaultSpinLimit, t.slot + at, warp == window - 1 ? kFlagIncl : kFlagAgg);
         const long base = ((long)t.b * a.tiles + at) * a.channels;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int ch = t.c0 + lane * V + j;
-            float2 m = make_float2(0.f, 0.f);
-            if (flag > 0 && ch < a.channels) {
-                if (flag == kFlagIncl) m.y = __ldcg(a.ends + base + ch);
-                else m = __ldcg(a.maps + base + ch);
-            }
-            sh.map[warp][lane * V + j] = m;
+        const int c = t.c0 + lane * V;
+        if (flag == kFlagIncl) {
+            sh.H[warp][lane] = load_channels<V>(a.ends + base, c, a.channels);
+        } else if (flag == kFlagAgg) {
+            sh.A[warp][lane] = load_channels<V>(a.map_a + base, c, a.channels);
+            sh.H[warp][lane] = load_channels<V>(a.map_h + base, c, a.channels);
         }
         if (lane == 0) sh.flag[warp] = flag;
     }
@@ -166,31 +276,22 @@ __device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, boo
         if (sh.flag[w] < 0) ok = false;
     }
     if (!ok) return false;
-#pragma unroll
-    for (int j = 0; j < V; ++j) c[j] = sh.map[n][lane * V + j].y;
-    for (int w = n - 1; w >= 0; --w)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 m = sh.map[w][lane * V + j];
-            c[j] = fmaf(m.x, c[j], m.y);
-        }
+    F<V> h = sh.H[n][lane];
+    for (int w = n - 1; w >= 0; --w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
+    *state = h;
     return true;
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void publish_map(const Params<T>& a, const Tile& t, int lane, const float A[V], const float H[V]) {
+__device__ __forceinline__ void publish_map(const Params<T>& a, const Tile& t, int lane, F<V> A, F<V> H) {
     const long base = ((long)t.b * a.tiles + t.tt) * a.channels;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (t.c0 + lane * V + j < a.channels) __stcg(a.maps + base + t.c0 + lane * V + j, make_float2(A[j], H[j]));
+    store_channels<V>(a.map_a + base, t.c0 + lane * V, a.channels, A);
+    store_channels<V>(a.map_h + base, t.c0 + lane * V, a.channels, H);
     publish(a.flags + t.slot + t.tt, kFlagAgg);
 }
 template <typename T, int V>
-__device__ __forceinline__ void publish_end(const Params<T>& a, const Tile& t, int lane, const float h[V]) {
-    const long base = ((long)t.b * a.tiles + t.tt) * a.channels;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (t.c0 + lane * V + j < a.channels) __stcg(a.ends + base + t.c0 + lane * V + j, h[j]);
+__device__ __forceinline__ void publish_end(const Params<T>& a, const Tile& t, int lane, F<V> h) {
+    store_channels<V>(a.ends + ((long)t.b * a.tiles + t.tt) * a.channels, t.c0 + lane * V, a.channels, h);
     publish(a.flags + t.slot + t.tt, kFlagIncl);
 }
 
@@ -206,7 +307,7 @@ __device__ __forceinline__ Tile take_tile(const Params<T>& a, bool down, Shared<
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(FW * 32) forward_kernel(const __grid_constant__ Params<T> a) {
+__global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_constant__ Params<T> a) {
     __shared__ Shared<V> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Tile t = take_tile(a, false, sh);
@@ -223,91 +324,61 @@ __global__ void __launch_bounds__(FW * 32) forward_kernel(const __grid_constant_
         const T* pi = a.gate.p + t.b * a.gate.sb + (long)from * a.gate.st + c;
 #pragma unroll
         for (int l = 0; l < FL; ++l) {
-            wx[l].zero(), wr[l].zero(), wi[l].zero();
-            if (l < live) wx[l].load(px + l * a.x.st), wr[l].load(pr + l * a.decay.st), wi[l].load(pi + l * a.gate.st);
+            wx[l].fill(0.f), wr[l].fill(-INFINITY), wi[l].fill(0.f);  // where there is no token: a = 1, b = 0
+            if (l < live) wx[l].load(px), wr[l].load(pr), wi[l].load(pi);
+            px += a.x.st, pr += a.decay.st, pi += a.gate.st;
         }
     }
-    float rate[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) rate[j] = in ? __ldg(a.rate + c + j) : 0.f;
-    float av[FL][V], bv[FL][V], A[V], H[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) A[j] = 1.f, H[j] = 0.f;
+    const F<V> rate = F<V>::make([&](int j) { return in ? rate_at(a.rate + c + j) : 0.f; });
+    F<V> av[FL], bv[FL], A(1.f), H(0.f);
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float p = rate[j] * sigmoid(wr[l].get(j));
-            const Decay d = decay_of(p);
-            av[l][j] = l < live ? d.a : 1.f;
-            bv[l][j] = l < live ? root(d.w) * sigmoid(wi[l].get(j)) * wx[l].get(j) : 0.f;
-            A[j] *= av[l][j];
-            H[j] = fmaf(av[l][j], H[j], bv[l][j]);
-        }
+        const Decay<V> d = decay_of(rate * sigmoid(wr[l].get()));
+        av[l] = d.a;
+        bv[l] = root(d.w) * sigmoid(wi[l].get()) * wx[l].get();
+        A = A * av[l];
+        H = fma(av[l], H, bv[l]);
     }
     // the warps' maps in front of this one
-    float pa[V], ph[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sh.map[warp][lane * V + j] = make_float2(A[j], H[j]), pa[j] = 1.f, ph[j] = 0.f;
+    F<V> pa(1.f), ph(0.f), h(0.f);
+    sh.A[warp][lane] = A, sh.H[warp][lane] = H;
     __syncthreads();
-    for (int w = 0; w < warp; ++w)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 m = sh.map[w][lane * V + j];
-            pa[j] *= m.x;
-            ph[j] = fmaf(m.x, ph[j], m.y);
-        }
-    float h[V];
+    for (int w = 0; w < warp; ++w) {
+        const F<V> m = sh.A[w][lane];
+        pa = pa * m;
+        ph = fma(m, ph, sh.H[w][lane]);
+    }
     const bool last = warp == warps - 1;
+    const F<V> ta = A * pa, th = fma(A, ph, H);
     if (t.tt == 0) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[j] = a.initial && in ? __ldg(a.initial + (long)t.b * a.channels + c + j) : 0.f;
+        if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
     } else {
-        if (last) {
-            float ta[V], tb[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) ta[j] = A[j] * pa[j], tb[j] = fmaf(A[j], ph[j], H[j]);
-            publish_map<T, V>(a, t, lane, ta, tb);
-        }
+        if (last) publish_map<T, V>(a, t, lane, ta, th);
         __syncthreads();  // every warp has read the maps
-        if (!look_back<T, V>(a, t, false, sh, warp, lane, warps, h)) {
+        if (!look_back<T, V>(a, t, false, sh, warp, lane, warps, &h)) {
             if (threadIdx.x == 0) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
             return;
         }
     }
     if (last) {
-        float end[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) end[j] = fmaf(A[j] * pa[j], h[j], fmaf(A[j], ph[j], H[j]));
-        if (t.tt < a.tiles - 1) {
-            publish_end<T, V>(a, t, lane, end);
-        } else if (a.final_state && in) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) a.final_state[(long)t.b * a.channels + c + j] = end[j];
-        }
+        const F<V> end = fma(ta, h, th);
+        if (t.tt < a.tiles - 1) publish_end<T, V>(a, t, lane, end);
+        else if (a.final_state) store_channels<V>(a.final_state + (long)t.b * a.channels, c, a.channels, end);
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = fmaf(pa[j], h[j], ph[j]);
-    if (a.carry && in && from % BT == 0 && from < a.steps) {
-        const long at = ((long)t.b * ((a.steps + BT - 1) / BT) + from / BT) * a.channels + c;
-#pragma unroll
-        for (int j = 0; j < V; ++j) a.carry[at + j] = h[j];
-    }
+    h = fma(pa, h, ph);
+    if (a.carry && from % BT == 0 && from < a.steps)
+        store_channels<V>(a.carry + ((long)t.b * ((a.steps + BT - 1) / BT) + from / BT) * a.channels, c, a.channels, h);
     T* po = a.out + ((long)t.b * a.steps + from) * a.channels + c;
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
-        float o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            h[j] = fmaf(av[l][j], h[j], bv[l][j]);
-            o[j] = l < live ? h[j] : 0.f;
-        }
-        if (l < rows) Word<T, V>::store(po + (long)l * a.channels, o);
+        h = fma(av[l], h, bv[l]);
+        if (l < rows) Word<T, V>::store(po, l < live ? h : F<V>(0.f));
+        po += a.channels;
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(BW * 32) backward_kernel(const __grid_constant__ Params<T> a) {
+__global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_constant__ Params<T> a) {
     __shared__ Shared<V> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Tile t = take_tile(a, true, sh);
@@ -318,8 +389,9 @@ __global__ void __launch_bounds__(BW * 32) backward_kernel(const __grid_constant
     const int live = in ? min(max(len - from, 0), BL) : 0, rows = in ? min(max(a.steps - from, 0), BL) : 0;
 
     Word<T, V> wx[BL], wg[BL];
-    float av[BL][V], rv[BL][V], iv[BL][V];
-    float rate[V], h[V], A[V], H[V], D[V];
+    F<V> av[BL], rv[BL], iv[BL], hb[BL];  // hb: the state in front of each token, at first from zero at the warp's start
+    F<V> A(1.f), H(0.f), D(0.f), h(0.f);
+    const F<V> rate = F<V>::make([&](int j) { return in ? rate_at(a.rate + c + j) : 0.f; });
     {
         Word<T, V> wr[BL], wi[BL];
         const T* px = a.x.p + t.b * a.x.sb + (long)from * a.x.st + c;
@@ -328,143 +400,92 @@ __global__ void __launch_bounds__(BW * 32) backward_kernel(const __grid_constant
         const T* pg = a.dout.p + t.b * a.dout.sb + (long)from * a.dout.st + c;
 #pragma unroll
         for (int l = 0; l < BL; ++l) {
-            wx[l].zero(), wr[l].zero(), wi[l].zero(), wg[l].zero();
-            if (l < live) {
-                wx[l].load(px + l * a.x.st), wr[l].load(pr + l * a.decay.st), wi[l].load(pi + l * a.gate.st);
-                if (a.dout.p) wg[l].load(pg + l * a.dout.st);
-            }
+            wx[l].fill(0.f), wr[l].fill(-INFINITY), wi[l].fill(0.f), wg[l].fill(0.f);
+            if (l < live) wx[l].load(px), wr[l].load(pr), wi[l].load(pi);
+            if (l < live && a.dout.p) wg[l].load(pg);
+            px += a.x.st, pr += a.decay.st, pi += a.gate.st, pg += a.dout.st;
         }
+        if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels);
+        else if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            rate[j] = in ? __ldg(a.rate + c + j) : 0.f;
-            h[j] = 0.f;  // the state in front of the tile
-            if (t.tt == 0) {
-                if (a.initial && in) h[j] = __ldg(a.initial + (long)t.b * a.channels + c + j);
-            } else if (in) {
-                h[j] = __ldg(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels + c + j);
-            }
-            A[j] = 1.f, H[j] = 0.f, D[j] = 0.f;
+        for (int l = 0; l < BL; ++l) {
+            rv[l] = sigmoid(wr[l].get()), iv[l] = sigmoid(wi[l].get());
+            const Decay<V> d = decay_of(rate * rv[l]);
+            av[l] = d.a;
+            hb[l] = H;
+            H = fma(av[l], H, root(d.w) * iv[l] * wx[l].get());
+            A = A * av[l];
         }
-#pragma unroll
-        for (int l = 0; l < BL; ++l)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                rv[l][j] = sigmoid(wr[l].get(j)), iv[l][j] = sigmoid(wi[l].get(j));
-            }
     }
-    float hb[BL][V];  // within the warp from zero: what is in front of each token
 #pragma unroll
-    for (int l = 0; l < BL; ++l)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const Decay d = decay_of(rate[j] * rv[l][j]);
-            av[l][j] = l < live ? d.a : 1.f;
-            hb[l][j] = H[j];
-            H[j] = fmaf(av[l][j], H[j], l < live ? root(d.w) * iv[l][j] * wx[l].get(j) : 0.f);
-            A[j] *= av[l][j];
-        }
-#pragma unroll
-    for (int l = BL - 1; l >= 0; --l)
-#pragma unroll
-        for (int j = 0; j < V; ++j) D[j] = av[l][j] * (wg[l].get(j) + D[j]);
+    for (int l = BL - 1; l >= 0; --l) D = av[l] * (wg[l].get() + D);
     // the states: maps of the warps in front
-#pragma unroll
-    for (int j = 0; j < V; ++j) sh.map[warp][lane * V + j] = make_float2(A[j], H[j]);
+    sh.A[warp][lane] = A, sh.H[warp][lane] = H;
     __syncthreads();
-    for (int w = 0; w < warp; ++w)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 m = sh.map[w][lane * V + j];
-            h[j] = fmaf(m.x, h[j], m.y);
-        }
+    for (int w = 0; w < warp; ++w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
     __syncthreads();
     // the gradients: maps of the warps behind
-    float pa[V], pd[V], g[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sh.map[warp][lane * V + j] = make_float2(A[j], D[j]), pa[j] = 1.f, pd[j] = 0.f;
+    F<V> pa(1.f), pd(0.f), g(0.f);
+    sh.H[warp][lane] = D;
     __syncthreads();
-    for (int w = warps - 1; w > warp; --w)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 m = sh.map[w][lane * V + j];
-            pa[j] *= m.x;
-            pd[j] = fmaf(m.x, pd[j], m.y);
-        }
+    for (int w = warps - 1; w > warp; --w) {
+        const F<V> m = sh.A[w][lane];
+        pa = pa * m;
+        pd = fma(m, pd, sh.H[w][lane]);
+    }
+    const F<V> ta = A * pa, td = fma(A, pd, D);
     if (t.tt == a.tiles - 1) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) g[j] = a.dfinal && in ? __ldg(a.dfinal + (long)t.b * a.channels + c + j) : 0.f;
+        if (a.dfinal) g = load_channels<V>(a.dfinal + (long)t.b * a.channels, c, a.channels);
     } else {
-        if (warp == 0) {
-            float ta[V], td[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) ta[j] = A[j] * pa[j], td[j] = fmaf(A[j], pd[j], D[j]);
-            publish_map<T, V>(a, t, lane, ta, td);
-        }
+        if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
         __syncthreads();
-        if (!look_back<T, V>(a, t, true, sh, warp, lane, warps, g)) {
+        if (!look_back<T, V>(a, t, true, sh, warp, lane, warps, &g)) {
             if (threadIdx.x == 0) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
             return;
         }
     }
     if (warp == 0) {
-        float end[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) end[j] = fmaf(A[j] * pa[j], g[j], fmaf(A[j], pd[j], D[j]));
-        if (t.tt > 0) {
-            publish_end<T, V>(a, t, lane, end);
-        } else if (a.dinitial && in) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) a.dinitial[(long)t.b * a.channels + c + j] = end[j];
-        }
+        const F<V> end = fma(ta, g, td);
+        if (t.tt > 0) publish_end<T, V>(a, t, lane, end);
+        else if (a.dinitial) store_channels<V>(a.dinitial + (long)t.b * a.channels, c, a.channels, end);
     }
-    float sum[V], prod[V];
+    g = fma(pa, g, pd);
 #pragma unroll
-    for (int j = 0; j < V; ++j) g[j] = fmaf(pa[j], g[j], pd[j]), sum[j] = 0.f, prod[j] = 1.f;
-#pragma unroll
-    for (int l = 0; l < BL; ++l)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            hb[l][j] = fmaf(prod[j], h[j], hb[l][j]);
-            prod[j] *= av[l][j];
-        }
-    const long at = ((long)t.b * a.steps + from) * a.channels + c;
+    for (int l = 0; l < BL; ++l) {
+        hb[l] = hb[l] + h;
+        h = av[l] * h;
+    }
+    F<V> sum(0.f);
+    const F<V> minus(-1.f), one(1.f);
+    const long at = ((long)t.b * a.steps + from + BL - 1) * a.channels + c;
+    T *ox = a.dx + at, *od = a.ddecay + at, *oi = a.dgate + at;
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
-        float ox[V], orr[V], oi[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float e = av[l][j], r = rv[l][j], i = iv[l][j], x = wx[l].get(j);
-            const float w = decay_of(rate[j] * r).w;  // formed again: kept, it would take the registers of another CTA
-            const float inv = rsqrtf(w), m = w == 0.f ? 0.f : w * inv;
-            const float slope = w > 0.f ? e * e * inv : 0.f;  // no step of the clock: the state passes, whatever the input
-            g[j] += wg[l].get(j);
-            const float ix = i * x, gm = g[j] * m;
-            const float dl = g[j] * fmaf(e, hb[l][j], -slope * ix);
-            ox[j] = gm * i;
-            oi[j] = gm * ix * (1.f - i);
-            const float rd = r * dl;
-            orr[j] = -rate[j] * (1.f - r) * rd;
-            if (l < live) sum[j] -= rd, g[j] *= e;
-            else ox[j] = oi[j] = orr[j] = 0.f;
-        }
+        const F<V> e = av[l], r = rv[l], i = iv[l];
+        const F<V> w = rest_of(rate * r, e);  // formed again: kept, it would take too many registers
+        // no step of the clock: the state passes, whatever the input
+        const F<V> inv = w.each([](float x) { return fabsf(x) < FLT_MIN ? 0.f : inverse_root(x); });
+        g = g + wg[l].get();
+        const F<V> ix = i * wx[l].get(), gm = g * (w * inv);
+        const F<V> rd = r * g * fma(e * e * inv * ix, minus, e * hb[l]);
         if (l < rows) {
-            Word<T, V>::store(a.dx + at + (long)l * a.channels, ox);
-            Word<T, V>::store(a.ddecay + at + (long)l * a.channels, orr);
-            Word<T, V>::store(a.dgate + at + (long)l * a.channels, oi);
+            const bool there = l < live;
+            Word<T, V>::store(ox, there ? gm * i : F<V>(0.f));
+            Word<T, V>::store(oi, there ? gm * ix * fma(i, minus, one) : F<V>(0.f));
+            Word<T, V>::store(od, there ? rate * rd * fma(r, one, minus) : F<V>(0.f));
         }
+        ox -= a.channels, od -= a.channels, oi -= a.channels;
+        sum = fma(rd, minus, sum);
+        g = e * g;
     }
     if (a.drate_part) {  // of the tile, the warps in order
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < V; ++j) sh.map[warp][lane * V + j].x = sum[j];
+        sh.H[warp][lane] = sum;
         __syncthreads();
-        if (warp == 0 && in) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float s = 0.f;
-                for (int w = 0; w < warps; ++w) s += sh.map[w][lane * V + j].x;
-                a.drate_part[((long)t.b * a.tiles + t.tt) * a.channels + c + j] = s;
-            }
+        if (warp == 0) {
+            F<V> s(0.f);
+            for (int w = 0; w < warps; ++w) s = s + sh.H[w][lane];
+            store_channels<V>(a.drate_part + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, s);
         }
     }
 }
@@ -530,16 +551,17 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Step<
                 }
             };
             load(a.x + row * a.xb + c, x), load(a.decay + row * a.db + c, r), load(a.gate + row * a.gb + c, i);
-            Vec<float, true>::load(a.rate + c, k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = rate_at(a.rate + c + j);
             Vec<float, true>::load(state, h);
         } else {
             x[0] = to_f(a.x[row * a.xb + c]), r[0] = to_f(a.decay[row * a.db + c]), i[0] = to_f(a.gate[row * a.gb + c]);
-            k[0] = a.rate[c], h[0] = *state;
+            k[0] = rate_at(a.rate + c), h[0] = *state;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const Decay d = decay_of(k[j] * sigmoid(r[j]));
-            o[j] = fmaf(d.a, h[j], root(d.w) * sigmoid(i[j]) * x[j]);
+            const Decay<1> d = decay_of(F<1>(k[j]) * sigmoid(F<1>(r[j])));
+            o[j] = fma(d.a, F<1>(h[j]), root(d.w) * sigmoid(F<1>(i[j])) * F<1>(x[j])).r;
         }
         if constexpr (V == 4) Vec<float, true>::store(state, o);
         else *state = o[0];
@@ -573,7 +595,7 @@ Sizes sizes(const ews_recur_args* a, bool bwd) {
     const size_t tiles = tiles_of(a->steps, bwd), states = (size_t)a->batch * tiles * a->channels;
     if (tiles > 1) {
         z.flags = up(sizeof(DeviceStatus) + sizeof(int) * (size_t)a->batch * tiles * ((a->channels + 31) / 32));
-        z.maps = up(sizeof(float2) * states), z.ends = up(sizeof(float) * states);
+        z.maps = up(2 * sizeof(float) * states), z.ends = up(sizeof(float) * states);
     }
     if (bwd) z.part = up(sizeof(float) * states);
     z.bytes = z.flags + z.maps + z.ends + z.part;
@@ -612,7 +634,8 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     if (p.tiles > 1) {
         p.st = reinterpret_cast<DeviceStatus*>(w);
         p.flags = reinterpret_cast<int*>(w + sizeof(DeviceStatus));
-        p.maps = reinterpret_cast<float2*>(w + z.flags);
+        p.map_a = reinterpret_cast<float*>(w + z.flags);
+        p.map_h = p.map_a + (size_t)a->batch * p.tiles * a->channels;
         p.ends = reinterpret_cast<float*>(w + z.flags + z.maps);
         if (cudaMemsetAsync(w, 0, z.flags, s) != cudaSuccess) return EWS_ERR_LAUNCH;
     }
@@ -655,7 +678,7 @@ int step(const ews_recur_args* a, const int* slots, int pool, float* state, cuda
     constexpr uintptr_t mask = sizeof(T) * 4 - 1;
     auto fits = [&](const void* q, long stride) { return ((uintptr_t)q & mask) == 0 && (a->batch == 1 || stride % 4 == 0); };
     const bool vec = a->channels % 4 == 0 && fits(p.x, p.xb) && fits(p.decay, p.db) && fits(p.gate, p.gb) && fits(p.out, 0) &&
-                     aligned16(state) && aligned16(p.rate);
+                     aligned16(state);
     const long threads = (long)a->batch * (vec ? a->channels / 4 : a->channels), ctas = (threads + 127) / 128;
     if (ctas > 0x7FFFFFFFl) return EWS_ERR_UNSUPPORTED;
     if (vec) step_kernel<T, 4><<<(unsigned)ctas, 128, 0, s>>>(p);
