@@ -6,6 +6,7 @@ the reference's layer API (alexandre-bloch/exponentially-weighted-signature, ews
 """
 
 from . import params, series
+from .gated_ops import gated_linear
 from .layer import COMBINE_KINDS, EWS, BToSignature, LogEWS, configure
 from .logsig import log_level_sizes, log_signature_dim
 from .params import AParamBlockDiag, AParamConstant, AParamDiag, AParamEFM, AParamGeneral, AParamJordanRepeated, B
@@ -36,6 +37,7 @@ __all__ = [
     "decayed_attention_step",
     "token_embedding",
     "vocab_loss",
+    "gated_linear",
     "gated_recurrence",
     "gated_recurrence_step",
     "log_level_sizes",

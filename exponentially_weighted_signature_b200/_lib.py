@@ -290,6 +290,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             fn.restype = _c_int
         lib.ews_recur_step.argtypes = [ctypes.c_char_p, _vp, _c_int, _vp, _vp]
         lib.ews_recur_step.restype = _c_int
+        lib.ews_gated_work_size.argtypes = [ctypes.c_char_p, _c_int]
+        lib.ews_gated_work_size.restype = _c_size
+        for name in ("ews_gated_fwd", "ews_gated_bwd"):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.c_char_p, _vp]
+            fn.restype = _c_int
         lib.ews_read_device_status.argtypes = [_vp, _vp, ctypes.POINTER(_c_int)]
         lib.ews_read_device_status.restype = _c_int
         lib.ews_diag_fwd_noalloc_status.argtypes = [_vp, ctypes.POINTER(_c_int)]

@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libews_b200.so")
 SOURCES = ["ews_capi.cu", "ews_diag.cu", "ews_dense.cu", "ews_block.cu", "ews_tables.cu", "ews_diag_term.cu",
            "ews_graded.cu", "ews_clock.cu", "ews_embed.cu", "ews_decay.cu", "ews_decay_tc.cu", "ews_decay_f32.cu",
-           "ews_vocab.cu", "ews_recur.cu"]
+           "ews_vocab.cu", "ews_recur.cu", "ews_gated.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode",

@@ -1,0 +1,911 @@
+// Gated linear layer: both projections, the activation and their product in one kernel, with its gradients.
+//
+//     G = X Wg^T,  U = X Wu^T,  H = act(G) U,       act(g) = g sigmoid(g)  or  g Phi(g)
+//     dG = dH U act'(G),  dU = dH act(G),  dX = dG Wg + dU Wu,  dWg = dG^T X,  dWu = dU^T X
+//
+// Many rows run on the 5th-generation tensor core, in a persistent kernel of one CTA an SM (gemm_kernel): operands by TMA into
+// 128-byte-swizzled tiles, K-major or MN-major as they lie in memory, tcgen05.mma of 128 x BN x 16, the accumulator in tensor
+// memory, two deep, so that a tile's epilogue runs under the next one's products.
+//   FWD  a tile's B operand is BN / 2 rows of Wg above the same rows of Wu, so that a gate and its partner end in one lane:
+//        the epilogue forms H, and for training also leaves G and U in the inputs' type (rounded once; H is formed from the
+//        float32 sums). Keeping them costs 2 N F values and spares the backward a third of its products.
+//   OUT  all gradients' tiles in one launch: dX (K runs over both pairs), dWg and dWu.
+// dG and dU are formed by one pass over dH, G and U in between.
+// Operands are bfloat16. float32 inputs are split into three bfloat16 planes (8 bits each) and a product runs over the six pairs
+// of planes that matter (2^-24), smallest first; every 256 of K the sum leaves the tensor core's accumulator, which truncates at
+// every addition, and is added in registers.
+//
+// Few rows (a served batch's tokens) are bound by the weights' bytes: few_kernel gives each CTA 16 rows of both weights, its warps
+// shares of K, and multiplies with mma.sync as the bytes arrive, the rows of X as the narrow side.
+#include "ews_tc.cuh"
+
+namespace ews {
+namespace gated {
+
+using namespace token;
+using namespace tc5;
+
+constexpr int BM = 128, BK = 64;
+constexpr int EPW = 8;              // epilogue warps
+constexpr int NTH = 64 + EPW * 32;  // and one each for TMA and MMA
+constexpr int SMS = 148;
+constexpr int kRun = 4;             // float32: k blocks of 64 in one accumulator
+constexpr int kFewBf16 = 64, kFewF32 = 16;  // rows up to which few_kernel / few_f32_kernel run
+enum Activation { SILU = 0, GELU = 1 };
+enum Epilogue { FWD, OUT };
+
+// act(g) and act'(g). bfloat16 results take the exponent unit's forms (2^-22).
+template <bool EXACT>
+__device__ __forceinline__ float logistic(float g) {
+    if (EXACT) return 1.f / (1.f + expf(-g));
+    return __fdividef(1.f, 1.f + __expf(-g));
+}
+// -inf: sigmoid and Phi are zero there, and 0 * inf is not the limit, which is zero.
+template <bool EXACT>
+__device__ __forceinline__ float act_of(float g, int kind) {
+    const float c = kind == SILU ? logistic<EXACT>(g) : EXACT ? 0.5f * erfcf(-0.70710678118654752f * g) : 0.5f + 0.5f * erff(0.70710678118654752f * g);
+    return c == 0.f ? 0.f : g * c;
+}
+template <bool EXACT>
+__device__ __forceinline__ void act_grad(float g, int kind, float* act, float* slope) {
+    if (kind == SILU) {
+        const float c = logistic<EXACT>(g);
+        *act = c == 0.f ? 0.f : g * c;
+        *slope = c == 0.f || c == 1.f ? c : fmaf(*act, 1.f - c, c);
+    } else {
+        const float c = EXACT ? 0.5f * erfcf(-0.70710678118654752f * g) : 0.5f + 0.5f * erff(0.70710678118654752f * g);
+        const float phi = 0.39894228040143268f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
+        *act = c == 0.f ? 0.f : g * c;
+        *slope = phi == 0.f ? c : fmaf(g, phi, c);
+    }
+}
+
+// ---- the GEMM -------------------------------------------------------------------------------------------------
+
+// C (m, n) = the sum over pairs of A (m, k) B (n, k)^T, in tiles and K splits.
+struct Job {
+    int m, n, k;
+    int tiles_m, tiles_n, splits, blocks;  // k blocks of 64 a split, of every pair
+    long units;
+    int pairs;
+    signed char ia[12], ib[12], mb[12];    // A's plane, B's plane, B's map
+    void* out;
+    float* acc;                            // splits > 1: (splits, m, n) float32 partials
+};
+
+struct Gemm {
+    Job job[3];   // FWD: one; OUT: dX (A K-major), dWg, dWu (A MN-major)
+    int run;      // k blocks in one accumulator
+    int act;
+    void *g, *u;  // FWD: the projections, or null
+    int* status;
+};
+
+struct Maps {
+    CUtensorMap a[2], b[3];  // FWD: X; Wg, Wu.  OUT: [dG dU] K-major and MN-major; Wg, Wu, X
+};
+
+template <int BN>
+struct Tile {
+    static constexpr int A = BM * BK * 2, B = BN * BK * 2, STAGE = A + B;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr size_t bytes = (size_t)STAGES * STAGE + 1024 + 256;
+};
+
+// Up to 32 consecutive results of a row, `w` of them there: whole sectors where the rows allow them.
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, const float v[32], int w, bool vec) {
+    if (w == 32 && vec) {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t q[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) q[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+            store32(p, q);
+            store32(p + 16, q + 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+                uint32_t q[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(v[j + e]);
+                store32(p + j, q);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < w) p[j] = from_f<T>(v[j]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ bool whole_rows(const void* p, int n) {
+    return n % (32 / (int)sizeof(T)) == 0 && ((uintptr_t)p & 31u) == 0;
+}
+
+template <typename T, int EPI, int BN>
+__global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Gemm a) {
+    using TL = Tile<BN>;
+    constexpr int S = TL::STAGES;
+    constexpr bool SUM = sizeof(T) == 4, BMN = EPI == OUT;
+    static_assert(!SUM || BN == 128, "the sums of a float32 tile stay in registers");
+    extern __shared__ unsigned char raw[];
+    unsigned char* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S * TL::STAGE);
+    uint64_t* empty = full + S;
+    uint64_t* acc_full = empty + S;   // 2
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drained = acc_empty + 2;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
+    volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, EPW * 32);
+        mbar_init(drained, 1);
+        *fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "r"(2 * BN));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
+    const long units = a.job[0].units + (EPI == OUT ? a.job[1].units + a.job[2].units : 0);
+
+    struct Unit {
+        int job, tm, tn, sp, k0, k1;
+    };
+    auto unit = [&](long u) {
+        Unit r;
+        r.job = 0;
+        if (EPI == OUT)
+            while (u >= a.job[r.job].units) u -= a.job[r.job++].units;
+        const Job& j = a.job[r.job];
+        const long per = (long)j.tiles_m * j.tiles_n;
+        r.sp = (int)(u / per);
+        const long t = u - r.sp * per;
+        // neighbours share the larger operand's rows: a gradient's dG or dU, the weights
+        if (EPI == OUT) r.tn = (int)(t % j.tiles_n), r.tm = (int)(t / j.tiles_n);
+        else r.tm = (int)(t % j.tiles_m), r.tn = (int)(t / j.tiles_m);
+        r.k0 = r.sp * j.blocks;
+        r.k1 = min(r.k0 + j.blocks, (j.k + BK - 1) / BK);
+        return r;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            long it = 0;
+            bool ok = true;
+            for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                const Unit r = unit(u);
+                const Job& j = a.job[r.job];
+                const bool amn = EPI == OUT && r.job > 0;
+                for (int from = r.k0; ok && from < r.k1; from += a.run) {
+                    for (int p = 0; ok && p < j.pairs; ++p) {
+                        const CUtensorMap* tb = &maps.b[j.mb[p]];
+                        for (int kb = from; kb < min(from + a.run, r.k1); ++kb, ++it) {
+                            const int s = (int)(it % S);
+                            if (!(ok = mbar_wait(empty + s, (uint32_t)((it / S) & 1) ^ 1u, fail))) break;
+                            unsigned char* at = tiles + s * TL::STAGE;
+                            mbar_expect(full + s, TL::STAGE);
+                            if (amn) {
+                                for (int q = 0; q < BM / 64; ++q)
+                                    tma_load(&maps.a[1], full + s, at + q * 8192, r.tm * BM + q * 64, kb * BK, j.ia[p]);
+                            } else {
+                                tma_load(&maps.a[0], full + s, at, kb * BK, r.tm * BM, j.ia[p]);
+                            }
+                            if (BMN) {
+                                for (int q = 0; q < BN / 64; ++q)
+                                    tma_load(tb, full + s, at + TL::A + q * 8192, r.tn * BN + q * 64, kb * BK, j.ib[p]);
+                            } else {
+                                tma_load(&maps.b[0], full + s, at + TL::A, kb * BK, r.tn * (BN / 2), j.ib[p]);
+                                tma_load(&maps.b[1], full + s, at + TL::A + TL::B / 2, kb * BK, r.tn * (BN / 2), j.ib[p]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (!ok)
+                for (long j = it > S ? it - S : 0; j < it; ++j) mbar_drain(full + j % S, (uint32_t)((j / S) & 1));
+        }
+    } else if (warp == 1) {
+        int s = 0;
+        uint32_t ph = 0;
+        long tile = 0;
+        bool ok = true;
+        for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            const Unit r = unit(u);
+            const bool amn = EPI == OUT && r.job > 0;
+            const int pairs = a.job[r.job].pairs;
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((amn ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
+                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            const uint32_t astep = amn ? 2048 >> 4 : 32 >> 4, bstep = BMN ? 2048 >> 4 : 32 >> 4;
+            for (int from = r.k0; ok && from < r.k1; from += a.run, ++tile) {
+                const int buf = (int)(tile & 1);
+                if (!(ok = warp_wait(acc_empty + buf, (uint32_t)((tile >> 1) & 1) ^ 1u, fail))) break;
+                fence_after();
+                const int steps = pairs * (min(from + a.run, r.k1) - from);
+                const uint64_t ad0 = desc(smem_u32(tiles), amn), bd0 = desc(smem_u32(tiles) + TL::A, BMN);
+                for (int i = 0; i < steps; ++i) {
+                    if (!(ok = warp_wait(full + s, ph, fail))) break;
+                    fence_after();
+                    if (elect_one()) {
+                        const uint64_t ad = ad0 + s * (TL::STAGE >> 4), bd = bd0 + s * (TL::STAGE >> 4);
+#pragma unroll
+                        for (int q = 0; q < BK / 16; ++q)
+                            mma_bf16(tmem + buf * BN, ad + q * astep, bd + q * bstep, idesc, i > 0 || q > 0);
+                        mma_commit(empty + s);
+                        if (i == steps - 1) mma_commit(acc_full + buf);
+                    }
+                    __syncwarp();
+                    if (++s == S) s = 0, ph ^= 1u;
+                }
+            }
+        }
+        if (!ok) {
+            if (elect_one()) mma_commit(drained);
+            __syncwarp();
+            mbar_drain(drained, 0);
+        }
+    } else {
+        // two warps share a quarter of the rows and take its blocks of 32 columns in turn
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        long tile = 0;
+        bool ok = true;
+        for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            const Unit r = unit(u);
+            const Job& job = a.job[r.job];
+            const int row = r.tm * BM + quarter * 32 + lane;
+            const bool in = row < job.m;
+            float s0[SUM ? 32 : 1], s1[SUM ? 32 : 1];  // float32: the runs' sums
+            for (int from = r.k0; from < r.k1; from += a.run, ++tile) {
+                const int buf = (int)(tile & 1);
+                if (!(ok = __all_sync(kFull, mbar_wait(acc_full + buf, (uint32_t)((tile >> 1) & 1), fail)))) break;
+                fence_after();
+                const uint32_t src = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
+                const bool last = !SUM || from + a.run >= r.k1;
+                constexpr int SPAN = EPI == FWD ? BN / 2 : BN;
+                auto close_fwd = [&](int c, float g[32], float up[32]) {
+                    const int col = r.tn * (BN / 2) + c, w = min(32, job.n - col);
+                    if (!in || w <= 0) return;
+                    const long at = (long)row * job.n + col;
+                    if (a.g) {
+                        store_row<T>(static_cast<T*>(a.g) + at, g, w, whole_rows<T>(a.g, job.n));
+                        store_row<T>(static_cast<T*>(a.u) + at, up, w, whole_rows<T>(a.u, job.n));
+                    }
+                    if (a.act == SILU) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) up[j] *= act_of<SUM>(g[j], SILU);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) up[j] *= act_of<SUM>(g[j], GELU);
+                    }
+                    store_row<T>(static_cast<T*>(job.out) + at, up, w, whole_rows<T>(job.out, job.n));
+                };
+                auto close_out = [&](int c, const float v[32]) {
+                    const int col = r.tn * BN + c, w = min(32, job.n - col);
+                    if (!in || w <= 0) return;
+                    if (job.acc) store_row<float>(job.acc + ((long)r.sp * job.m + row) * job.n + col, v, w, whole_rows<float>(job.acc, job.n));
+                    else store_row<T>(static_cast<T*>(job.out) + (long)row * job.n + col, v, w, whole_rows<T>(job.out, job.n));
+                };
+                if constexpr (EPI == FWD) {
+                    for (int c = half * 32; c < SPAN; c += 64) {
+                        uint32_t p[32], q[32];
+                        tmem_ld32x2(src + c, src + BN / 2 + c, p, q);
+                        float g[32], up[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) g[j] = __uint_as_float(p[j]), up[j] = __uint_as_float(q[j]);
+                        if constexpr (SUM) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                g[j] = s0[j] = from > r.k0 ? s0[j] + g[j] : g[j];
+                                up[j] = s1[j] = from > r.k0 ? s1[j] + up[j] : up[j];
+                            }
+                        }
+                        if (last) close_fwd(c, g, up);
+                    }
+                } else {
+#pragma unroll
+                    for (int c0 = 0; c0 < SPAN; c0 += 64) {
+                        const int c = c0 + half * 32;
+                        float v[32];
+                        tmem_ld32(src + c, v);
+                        if constexpr (SUM) {
+                            float* s = c0 ? s1 : s0;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = s[j] = from > r.k0 ? s[j] + v[j] : v[j];
+                        }
+                        if (last) close_out(c, v);
+                    }
+                }
+                fence_before();
+                mbar_arrive(acc_empty + buf);
+            }
+        }
+    }
+    __syncthreads();
+    fence_after();
+    if (threadIdx.x == 0 && *fail) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+}
+
+// ---- the passes around it ------------------------------------------------------------------------------------
+
+// Rows as bfloat16 planes of `ld` columns, zero beyond `dim`. Several matrices in one launch.
+template <typename T>
+struct Pack {
+    const T* in;
+    long stride, rows;
+    bf16* out;
+    long plane;
+};
+template <typename T>
+struct Packs {
+    Pack<T> p[3];
+};
+
+template <typename T>
+__device__ __forceinline__ void split8(const float v_in[8], bf16* out, long plane, int planes) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v_in[j];
+    for (int s = 0; s < planes; ++s) {
+        Vec<bf16, true>::store(out + s * plane, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] -= to_f(from_f<bf16>(v[j]));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int there, bool vec, float v[8]) {
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < 8; j += Vec<T, true>::N) Vec<T, true>::load(p + j, v + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < there ? to_f(p[j]) : 0.f;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs<T> a, int dim, int ld, int planes) {
+    const int per = ld / 8;
+    const long total = (a.p[0].rows + a.p[1].rows + a.p[2].rows) * per;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
+        long row = e / per;
+        const int col = (int)(e - row * per) * 8;
+        int k = 0;
+        while (row >= a.p[k].rows) row -= a.p[k++].rows;
+        const Pack<T>& m = a.p[k];
+        float v[8];
+        load8<T>(m.in + row * m.stride + col, dim - col, m.stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(m.in), v);
+        split8<T>(v, m.out + row * ld + col, m.plane, planes);
+    }
+}
+
+// dG and dU from dH, G and U, as operands: planes of (rows, ld), first dG's, then dU's.
+template <typename T>
+__global__ void __launch_bounds__(256) grad_kernel(const T* __restrict__ dout, long dout_stride, const T* __restrict__ g, const T* __restrict__ u,
+                                                   long rows, int inner, int ld, int act, int planes, bf16* __restrict__ out) {
+    const int per = ld / 8;
+    const bool vec = inner % 8 == 0 && aligned16_dev(g) && aligned16_dev(u) && aligned16_dev(dout) && dout_stride % (16 / (int)sizeof(T)) == 0;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < rows * per; e += (long)gridDim.x * 256) {
+        const long row = e / per;
+        const int col = (int)(e - row * per) * 8;
+        float d[8], gv[8], uv[8];
+        load8<T>(dout + row * dout_stride + col, inner - col, vec, d);
+        load8<T>(g + row * inner + col, inner - col, vec, gv);
+        load8<T>(u + row * inner + col, inner - col, vec, uv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float f, slope;
+            act_grad<sizeof(T) == 4>(gv[j], act, &f, &slope);
+            gv[j] = d[j] * uv[j] * slope;
+            uv[j] = d[j] * f;
+        }
+        bf16* at = out + row * ld + col;
+        split8<T>(gv, at, rows * ld, planes);
+        split8<T>(uv, at + planes * rows * ld, rows * ld, planes);
+    }
+}
+
+// A gradient from its float32 partials, summed in order and rounded once.
+struct Reduce {
+    const float* acc;
+    void* out;
+    int splits;
+    long count;  // of four elements
+};
+struct Reduces {
+    Reduce r[3];
+};
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Reduces a) {
+    constexpr int W = VEC ? 4 : 1;
+    const long total = a.r[0].count + a.r[1].count + a.r[2].count;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
+        long i = e;
+        int k = 0;
+        while (i >= a.r[k].count) i -= a.r[k++].count;
+        const Reduce& r = a.r[k];
+        float s[W];
+        Vec<float, VEC>::load(r.acc + i * W, s);
+        for (int p = 1; p < r.splits; ++p) {
+            float v[W];
+            Vec<float, VEC>::load(r.acc + (p * r.count + i) * W, v);
+#pragma unroll
+            for (int j = 0; j < W; ++j) s[j] += v[j];
+        }
+        T* o = static_cast<T*>(r.out) + i * W;
+        if constexpr (VEC && sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+        else Vec<T, VEC>::store(o, s);
+    }
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------
+
+template <typename T>
+struct Few {
+    const T *x, *wg, *wu;
+    long xs, gs, us;
+    int rows, dim, inner, act;
+    T *out, *g, *u;
+};
+
+// D (16 x 8) += A (16 x 16, rows) B (16 x 8, columns), bfloat16 into float32.
+__device__ __forceinline__ void mma_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int FEW_WARPS = 8;
+
+// 16 rows of each weight a CTA; a warp takes every eighth block of 32 of K. The order of K within a block is the operands' own
+// choice, so a lane takes eight consecutive elements of a row, one 16-byte load, as the four words that two products want of it
+// (the same of X's rows). 8 NT rows of X.
+template <int NT, bool VEC>
+__global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const __grid_constant__ Few<bf16> a) {
+    extern __shared__ float red[];  // (warps, 2, 16, 8 NT)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 2, quad = lane & 3;
+    const int f0 = blockIdx.x * 16;
+    float acc[2][NT][4];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[w][n][e] = 0.f;
+    auto load = [&](const bf16* base, long stride, int row, int rows, int k) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row >= rows || k >= a.dim) return v;
+        const bf16* p = base + row * stride + k;
+        if (VEC) return __ldg(reinterpret_cast<const uint4*>(p));
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float lo = k + 2 * j < a.dim ? to_f(p[2 * j]) : 0.f, hi = k + 2 * j + 1 < a.dim ? to_f(p[2 * j + 1]) : 0.f;
+            w[j] = pack_bf16(lo, hi);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    const int blocks = (a.dim + 31) / 32;
+    constexpr int U = NT <= 2 ? 4 : 2;  // blocks in flight
+    for (int b0 = warp; b0 < blocks; b0 += FEW_WARPS * U) {
+        uint4 wv[U][4], xv[U][NT];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int k = (b0 + i * FEW_WARPS) * 32 + quad * 8;  // beyond the last block: zeros
+            wv[i][0] = load(a.wg, a.gs, f0 + grp, a.inner, k), wv[i][1] = load(a.wg, a.gs, f0 + grp + 8, a.inner, k);
+            wv[i][2] = load(a.wu, a.us, f0 + grp, a.inner, k), wv[i][3] = load(a.wu, a.us, f0 + grp + 8, a.inner, k);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) xv[i][n] = load(a.x, a.xs, n * 8 + grp, a.rows, k);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint4 lo = wv[i][2 * w], hi = wv[i][2 * w + 1], x = xv[i][n];
+                    mma_16816(acc[w][n], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+                    mma_16816(acc[w][n], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+                }
+    }
+    constexpr int COLS = 8 * NT;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float* p = red + ((warp * 2 + w) * 16 + grp) * COLS + n * 8 + quad * 2;
+            p[0] = acc[w][n][0], p[1] = acc[w][n][1];
+            p[8 * COLS] = acc[w][n][2], p[8 * COLS + 1] = acc[w][n][3];
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * COLS; e += FEW_WARPS * 32) {
+        const int f = e & 15, n = e >> 4;
+        if (f0 + f >= a.inner || n >= a.rows) continue;
+        float g = 0.f, u = 0.f;
+#pragma unroll
+        for (int k = 0; k < FEW_WARPS; ++k) g += red[(k * 2 * 16 + f) * COLS + n], u += red[((k * 2 + 1) * 16 + f) * COLS + n];
+        const long at = (long)n * a.inner + f0 + f;
+        if (a.g) a.g[at] = from_f<bf16>(g), a.u[at] = from_f<bf16>(u);
+        a.out[at] = from_f<bf16>(u * act_of<false>(g, a.act));
+    }
+}
+
+// float32: a warp has two rows of each weight and runs along K, its lanes on consecutive fours of it (however they are
+// loaded: the sums' order does not depend on the alignment), for R rows of X.
+template <int R, bool VEC>
+__global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Few<float> a) {
+    constexpr int W = 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int f = (blockIdx.x * 4 + warp) * 2;
+    auto load = [&](const float* p, int k, float v[4]) {
+        if (VEC) return Vec<float, true>::load(p + k, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = k + e < a.dim ? p[k + e] : 0.f;
+    };
+    if (f >= a.inner) return;
+    const int f1 = f + 1 < a.inner ? f + 1 : f;
+    const float* w[4] = {a.wg + f * a.gs, a.wg + f1 * a.gs, a.wu + f * a.us, a.wu + f1 * a.us};
+    float acc[4][R];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[j][r] = 0.f;
+#pragma unroll 2
+    for (int k = lane * W; k < a.dim; k += 32 * W) {
+        float wv[4][W];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load(w[j], k, wv[j]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (r >= a.rows) continue;
+            float xv[W];
+            load(a.x + r * a.xs, k, xv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < W; ++e) acc[j][r] = fmaf(wv[j][e], xv[e], acc[j][r]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) acc[j][r] += __shfl_xor_sync(kFull, acc[j][r], o);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (r >= a.rows || lane >= 2 || f + lane >= a.inner) continue;
+        const float g = lane ? acc[1][r] : acc[0][r], u = lane ? acc[3][r] : acc[2][r];
+        const long at = (long)r * a.inner + f + lane;
+        if (a.g) a.g[at] = g, a.u[at] = u;
+        a.out[at] = u * act_of<true>(g, a.act);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------
+
+// (planes, rows, cols) bfloat16 with rows `ld` apart.
+struct Operand {
+    const bf16* p;
+    long rows, cols, ld, plane;
+    int planes;
+};
+
+bool make_map(CUtensorMap* map, const Operand& o, int box_rows) {
+    EncodeFn enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld * o.rows) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+long up(long n, long to) { return (n + to - 1) / to * to; }
+
+int check(const ews_gated_args* a) {
+    if (!a || a->rows < 0 || a->dim <= 0 || a->inner <= 0) return EWS_ERR_INVALID_ARGUMENT;
+    if (a->x_stride < a->dim || a->gate_stride < a->dim || a->up_stride < a->dim) return EWS_ERR_INVALID_ARGUMENT;
+    if (a->activation != SILU && a->activation != GELU) return EWS_ERR_UNSUPPORTED;
+    if (a->dtype != EWS_DTYPE_F32 && a->dtype != EWS_DTYPE_BF16) return EWS_ERR_UNSUPPORTED;
+    if (a->rows >= (1l << 30) || a->inner >= (1l << 29) || a->dim >= (1l << 29)) return EWS_ERR_UNSUPPORTED;
+    return EWS_OK;
+}
+
+bool few(const ews_gated_args* a) { return a->rows <= (a->dtype == EWS_DTYPE_BF16 ? kFewBf16 : kFewF32); }
+
+// A matrix of (rows, dim) as an operand: as it lies where TMA can read it, else packed at `at` of the workspace.
+struct Source {
+    bool packed;
+    size_t at;
+};
+
+struct Plan {
+    int planes;
+    long ldd, ldf;
+    Source x, wg, wu;
+    size_t dgu, acc[3], bytes;
+    int bn, splits[3];
+};
+
+bool readable(const ews_gated_args* a, const void* p, int64_t stride) {
+    return a->dtype == EWS_DTYPE_BF16 && stride % 8 == 0 && a->dim % 8 == 0 && aligned16(p);
+}
+
+// Column tiles: 256 wide (both operands of a product then come at 96 bytes a clock from shared memory, under its 128), or as
+// narrow as it takes to give every SM one. float32 sums stay in registers at 128.
+int forward_bn(const ews_gated_args* a) {
+    if (a->dtype == EWS_DTYPE_F32) return 128;
+    const long tm = (a->rows + BM - 1) / BM;
+    for (int bn = 256; bn > 64; bn /= 2)
+        if (tm * ((a->inner + bn / 2 - 1) / (bn / 2)) >= SMS) return bn;
+    return 64;
+}
+
+Job job_of(long m, long n, long k, int bn, int splits) {
+    Job j{};
+    j.m = (int)m, j.n = (int)n, j.k = (int)k, j.splits = splits;
+    j.tiles_m = (int)((m + BM - 1) / BM), j.tiles_n = (int)((n + bn - 1) / bn);
+    j.blocks = (int)(((k + BK - 1) / BK + splits - 1) / splits);
+    j.splits = (int)(((k + BK - 1) / BK + j.blocks - 1) / j.blocks);  // none empty
+    j.units = (long)j.tiles_m * j.tiles_n * j.splits;
+    return j;
+}
+
+// Splits of K so that the gradients' units, weighed by their K, fill the SMs: none below eight k blocks.
+void pick_splits(Plan* p, const ews_gated_args* a, const bool want[3]) {
+    const long m[3] = {a->rows, a->inner, a->inner}, k[3] = {2 * a->inner, a->rows, a->rows};
+    long tiles[3];
+    double work = 0;
+    for (int j = 0; j < 3; ++j) {
+        tiles[j] = want[j] ? ((m[j] + BM - 1) / BM) * ((a->dim + p->bn - 1) / p->bn) : 0;
+        work += (double)tiles[j] * k[j];
+    }
+    for (int j = 0; j < 3; ++j) {
+        p->splits[j] = 1;
+        if (!want[j]) continue;
+        const double share = work / SMS;  // of an SM
+        const long blocks = (k[j] / (j ? 1 : 2) + BK - 1) / BK;
+        long s = (long)(k[j] / share);    // a unit longer than an SM's share holds the launch up
+        if (s > blocks / 8) s = blocks / 8;
+        if (s > 1) p->splits[j] = job_of(m[j], a->dim, k[j] / (j ? 1 : 2), p->bn, (int)s).splits;
+    }
+}
+
+Plan plan(const ews_gated_args* a, bool bwd) {
+    Plan p{};
+    p.planes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
+    p.ldd = up(a->dim, 8), p.ldf = up(a->inner, 8);
+    if (!bwd && few(a)) return p;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    auto source = [&](const void* m, int64_t stride, long rows) {
+        Source s{!readable(a, m, stride), 0};
+        if (s.packed) s.at = take(sizeof(bf16) * (size_t)p.planes * rows * p.ldd);
+        return s;
+    };
+    p.x = source(a->x, a->x_stride, a->rows);
+    p.wg = source(a->w_gate, a->gate_stride, a->inner);
+    p.wu = source(a->w_up, a->up_stride, a->inner);
+    if (!bwd) {
+        p.bn = forward_bn(a);
+    } else {
+        const bool want[3] = {a->dx != nullptr, a->dw_gate != nullptr, a->dw_up != nullptr};
+        p.bn = p.planes > 1 || a->dim <= 128 ? 128 : 256;
+        pick_splits(&p, a, want);
+        p.dgu = take(sizeof(bf16) * 2 * (size_t)p.planes * a->rows * p.ldf);
+        for (int j = 0; j < 3; ++j)
+            if (p.splits[j] > 1) p.acc[j] = take(sizeof(float) * (size_t)p.splits[j] * (j ? a->inner : a->rows) * a->dim);
+    }
+    p.bytes = at;
+    return p;
+}
+
+unsigned grid_of(long threads) {
+    const long b = (threads + 255) / 256;
+    return (unsigned)(b < 1 ? 1 : b < SMS * 16 ? b : SMS * 16);
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH; }
+
+template <typename T, int EPI, int BN>
+int gemm(const Maps& maps, const Gemm& g, cudaStream_t s) {
+    auto* kern = gemm_kernel<T, EPI, BN>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
+    const long units = g.job[0].units + g.job[1].units + g.job[2].units;
+    kern<<<(unsigned)(units < SMS ? units : SMS), NTH, Tile<BN>::bytes, s>>>(maps, g);
+    return launched();
+}
+
+const signed char kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
+
+// The three matrices as operands, packed in one launch where they have to be.
+template <typename T>
+int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Operand* wu, bool need_x, bool need_w, cudaStream_t s) {
+    char* w = static_cast<char*>(a->work);
+    Packs<T> packs{};
+    long total = 0;
+    int n = 0;
+    auto make = [&](const Source& src, const void* m, int64_t stride, long rows, bool need, Operand* o) {
+        o->rows = rows, o->planes = p.planes;
+        if (!src.packed) {
+            o->p = static_cast<const bf16*>(m), o->cols = a->dim, o->ld = stride;
+            return;
+        }
+        bf16* at = reinterpret_cast<bf16*>(w + src.at);
+        o->p = at, o->cols = o->ld = p.ldd, o->plane = rows * p.ldd;
+        if (need) packs.p[n++] = Pack<T>{static_cast<const T*>(m), (long)stride, rows, at, o->plane}, total += rows;
+    };
+    make(p.x, a->x, a->x_stride, a->rows, need_x, x);
+    make(p.wg, a->w_gate, a->gate_stride, a->inner, need_w, wg);
+    make(p.wu, a->w_up, a->up_stride, a->inner, need_w, wu);
+    if (total == 0) return EWS_OK;
+    pack_kernel<T><<<grid_of(total * (p.ldd / 8)), 256, 0, s>>>(packs, (int)a->dim, (int)p.ldd, p.planes);
+    return launched();
+}
+
+template <int NT, bool VEC>
+int run_few(const Few<bf16>& f, cudaStream_t s) {
+    auto* kern = few_kernel<NT, VEC>;
+    constexpr int bytes = FEW_WARPS * 2 * 16 * 8 * NT * 4;
+    if (bytes > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
+    kern<<<(unsigned)((f.inner + 15) / 16), FEW_WARPS * 32, bytes, s>>>(f);
+    return launched();
+}
+
+template <typename T>
+int forward_few(const ews_gated_args* a, cudaStream_t s) {
+    Few<T> f{};
+    f.x = static_cast<const T*>(a->x), f.wg = static_cast<const T*>(a->w_gate), f.wu = static_cast<const T*>(a->w_up);
+    f.xs = a->x_stride, f.gs = a->gate_stride, f.us = a->up_stride;
+    f.rows = (int)a->rows, f.dim = (int)a->dim, f.inner = (int)a->inner, f.act = a->activation;
+    f.out = static_cast<T*>(a->out), f.g = static_cast<T*>(a->gate), f.u = static_cast<T*>(a->up);
+    constexpr int E = 16 / sizeof(T);
+    const bool vec = a->dim % E == 0 && f.gs % E == 0 && f.us % E == 0 && (a->rows == 1 || f.xs % E == 0) && aligned16(f.x) &&
+                     aligned16(f.wg) && aligned16(f.wu);
+    if constexpr (sizeof(T) == 2) {
+        const int nt = (f.rows + 7) / 8;
+        if (nt <= 1) return vec ? run_few<1, true>(f, s) : run_few<1, false>(f, s);
+        if (nt <= 2) return vec ? run_few<2, true>(f, s) : run_few<2, false>(f, s);
+        if (nt <= 4) return vec ? run_few<4, true>(f, s) : run_few<4, false>(f, s);
+        return vec ? run_few<8, true>(f, s) : run_few<8, false>(f, s);
+    } else {
+        const unsigned grid = (unsigned)((f.inner + 7) / 8);
+        auto go = [&](auto* kern) {
+            kern<<<grid, 128, 0, s>>>(f);
+            return launched();
+        };
+        if (f.rows <= 1) return vec ? go(few_f32_kernel<1, true>) : go(few_f32_kernel<1, false>);
+        if (f.rows <= 4) return vec ? go(few_f32_kernel<4, true>) : go(few_f32_kernel<4, false>);
+        return vec ? go(few_f32_kernel<16, true>) : go(few_f32_kernel<16, false>);
+    }
+}
+
+template <typename T>
+int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
+    if (few(a)) return forward_few<T>(a, s);
+    Operand x{}, wg{}, wu{};
+    int rc = operands<T>(a, p, &x, &wg, &wu, true, true, s);
+    if (rc != EWS_OK) return rc;
+    Maps m{};
+    if (!make_map(&m.a[0], x, BM) || !make_map(&m.b[0], wg, p.bn / 2) || !make_map(&m.b[1], wu, p.bn / 2)) return EWS_ERR_LAUNCH;
+    Gemm g{};
+    g.job[0] = job_of(a->rows, a->inner, a->dim, p.bn / 2, 1);
+    Job& j = g.job[0];
+    j.out = a->out, j.pairs = p.planes == 1 ? 1 : 6;
+    for (int i = 0; i < j.pairs; ++i) j.ia[i] = p.planes == 1 ? 0 : kPlaneA[i], j.ib[i] = p.planes == 1 ? 0 : kPlaneB[i];
+    g.run = p.planes > 1 ? kRun : 1 << 28;
+    g.act = a->activation, g.g = a->gate, g.u = a->up, g.status = a->status;
+    if constexpr (sizeof(T) == 4) {
+        return gemm<T, FWD, 128>(m, g, s);
+    } else {
+        if (p.bn == 256) return gemm<T, FWD, 256>(m, g, s);
+        return p.bn == 128 ? gemm<T, FWD, 128>(m, g, s) : gemm<T, FWD, 64>(m, g, s);
+    }
+}
+
+template <typename T>
+int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
+    char* w = static_cast<char*>(a->work);
+    Operand x{}, wg{}, wu{}, d{};
+    const bool dw = a->dw_gate || a->dw_up;
+    int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, s);
+    if (rc != EWS_OK) return rc;
+    bf16* dgu = reinterpret_cast<bf16*>(w + p.dgu);
+    grad_kernel<T><<<grid_of(a->rows * (p.ldf / 8)), 256, 0, s>>>(static_cast<const T*>(a->dout), a->dout_stride, static_cast<const T*>(a->gate),
+                                                               static_cast<const T*>(a->up), a->rows, (int)a->inner, (int)p.ldf, a->activation,
+                                                               p.planes, dgu);
+    if ((rc = launched()) != EWS_OK) return rc;
+    d.p = dgu, d.rows = a->rows, d.cols = d.ld = p.ldf, d.plane = a->rows * p.ldf, d.planes = 2 * p.planes;
+    Maps m{};
+    if (!make_map(&m.a[0], d, BM) || !make_map(&m.a[1], d, 64)) return EWS_ERR_LAUNCH;
+    if (a->dx && (!make_map(&m.b[0], wg, 64) || !make_map(&m.b[1], wu, 64))) return EWS_ERR_LAUNCH;
+    if (dw && !make_map(&m.b[2], x, 64)) return EWS_ERR_LAUNCH;
+    Gemm g{};
+    g.run = p.planes > 1 ? kRun : 1 << 28;
+    g.status = a->status;
+    void* out[3] = {a->dx, a->dw_gate, a->dw_up};
+    const int products = p.planes == 1 ? 1 : 6;
+    Reduces red{};
+    long total = 0;
+    bool vec = a->dim % 4 == 0;
+    for (int k = 0; k < 3; ++k) {
+        if (!out[k]) continue;
+        Job& j = g.job[k];
+        j = k ? job_of(a->inner, a->dim, a->rows, p.bn, p.splits[k]) : job_of(a->rows, a->dim, a->inner, p.bn, p.splits[k]);
+        j.out = out[k];
+        for (int side = 0; side < (k ? 1 : 2); ++side)
+            for (int i = 0; i < products; ++i) {
+                const int which = k ? k - 1 : side;  // dG or dU
+                j.ia[j.pairs] = (signed char)(which * p.planes + (products == 1 ? 0 : kPlaneA[i]));
+                j.ib[j.pairs] = products == 1 ? 0 : kPlaneB[i];
+                j.mb[j.pairs++] = (signed char)(k ? 2 : side);
+            }
+        if (j.splits > 1) {
+            j.acc = reinterpret_cast<float*>(w + p.acc[k]);
+            red.r[k] = Reduce{j.acc, out[k], j.splits, (long)j.m * j.n};
+            total += red.r[k].count;
+            vec = vec && aligned16(out[k]);
+        }
+    }
+    if constexpr (sizeof(T) == 4) rc = gemm<T, OUT, 128>(m, g, s);
+    else rc = p.bn == 256 ? gemm<T, OUT, 256>(m, g, s) : gemm<T, OUT, 128>(m, g, s);
+    if (rc != EWS_OK || total == 0) return rc;
+    if (vec) {
+        for (Reduce& r : red.r) r.count /= 4;
+        reduce_kernel<T, true><<<grid_of(total / 4), 256, 0, s>>>(red);
+    } else {
+        reduce_kernel<T, false><<<grid_of(total), 256, 0, s>>>(red);
+    }
+    return launched();
+}
+
+}  // namespace gated
+}  // namespace ews
+
+using namespace ews::gated;
+
+extern "C" size_t ews_gated_work_size(const ews_gated_args* a, int backward_pass) {
+    return check(a) == EWS_OK && a->rows > 0 ? plan(a, backward_pass != 0).bytes : 0;
+}
+
+extern "C" int ews_gated_fwd(const ews_gated_args* a, ews_stream_t stream) {
+    const int rc = check(a);
+    if (rc != EWS_OK) return rc;
+    if (a->rows == 0) return EWS_OK;
+    if (!a->x || !a->w_gate || !a->w_up || !a->out || !a->gate != !a->up) return EWS_ERR_INVALID_ARGUMENT;
+    const Plan p = plan(a, false);
+    if (p.bytes && (!a->work || !ews::token::aligned16(a->work) || a->work_bytes < p.bytes)) return EWS_ERR_WORKSPACE;
+    cudaStream_t s = (cudaStream_t)stream;
+    return a->dtype == EWS_DTYPE_BF16 ? forward<ews::token::bf16>(a, p, s) : forward<float>(a, p, s);
+}
+
+extern "C" int ews_gated_bwd(const ews_gated_args* a, ews_stream_t stream) {
+    const int rc = check(a);
+    if (rc != EWS_OK) return rc;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (a->rows == 0) {
+        const size_t bytes = (a->dtype == EWS_DTYPE_BF16 ? 2 : 4) * (size_t)a->inner * a->dim;
+        for (void* w : {a->dw_gate, a->dw_up})
+            if (w && cudaMemsetAsync(w, 0, bytes, s) != cudaSuccess) return EWS_ERR_LAUNCH;
+        return EWS_OK;
+    }
+    if (!a->dx && !a->dw_gate && !a->dw_up) return EWS_OK;
+    if (!a->x || !a->w_gate || !a->w_up || !a->dout || !a->gate || !a->up || a->dout_stride < a->inner) return EWS_ERR_INVALID_ARGUMENT;
+    const Plan p = plan(a, true);
+    if (p.bytes && (!a->work || !ews::token::aligned16(a->work) || a->work_bytes < p.bytes)) return EWS_ERR_WORKSPACE;
+    return a->dtype == EWS_DTYPE_BF16 ? backward<ews::token::bf16>(a, p, s) : backward<float>(a, p, s);
+}
