@@ -13,7 +13,7 @@ from .params import AParamBlockDiag, AParamConstant, AParamDiag, AParamEFM, APar
 from .recur_ops import gated_recurrence, gated_recurrence_step
 from .series import check_series_q, series_error_bound, suggest_series_q
 from .token_model import DecayBlock, TokenModel
-from .token_ops import decayed_attention, decayed_attention_step, token_embedding, vocab_loss
+from .token_ops import decayed_attention, decayed_attention_step, distill_loss, token_embedding, vocab_loss
 
 __all__ = [
     "COMBINE_KINDS",
@@ -37,6 +37,7 @@ __all__ = [
     "decayed_attention_step",
     "token_embedding",
     "vocab_loss",
+    "distill_loss",
     "gated_linear",
     "gated_recurrence",
     "gated_recurrence_step",

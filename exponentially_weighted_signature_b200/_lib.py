@@ -296,6 +296,14 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_char_p, _vp]
             fn.restype = _c_int
+        lib.ews_distill_entries_size.argtypes = [_i64, _c_int]
+        lib.ews_distill_entries_size.restype = _c_size
+        lib.ews_distill_work_size.argtypes = [ctypes.c_char_p, _c_int]
+        lib.ews_distill_work_size.restype = _c_size
+        for name in ("ews_distill_fwd", "ews_distill_bwd"):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.c_char_p, _vp]
+            fn.restype = _c_int
         lib.ews_read_device_status.argtypes = [_vp, _vp, ctypes.POINTER(_c_int)]
         lib.ews_read_device_status.restype = _c_int
         lib.ews_diag_fwd_noalloc_status.argtypes = [_vp, ctypes.POINTER(_c_int)]

@@ -21,8 +21,15 @@
 // GRAD (1.27 PFLOP/s) and 256 us for both gradients in one launch (1.21 PFLOP/s; as launches of their own, 116 and 119 us
 // for 7,424 entries, each left a fifth of its last wave of tiles idle). What bounds them is the tensor pipe under the
 // power cap. Pieces of 16, 32, 64 M entries of G took 3.95, 3.24, 3.16 ms for a step that took 3.02 ms with 128 M (2.80 now).
+// Targets may also be distributions over a few entries of the vocabulary, a teacher's top logits (TOP): p = softmax(t / tau)
+// over a row's entries, loss_n = sum_k p_k (log p_k - log q_{id_k}) with q = softmax(z / tau), G = (q - p) dloss_n / tau. A row's
+// entries are sorted by their ids once, so that an epilogue lane, which has one row, finds its tile's by a binary search while
+// the tile's products run, and then looks at one id a block of 32 columns.
 // Rows without a target cost nothing: a first kernel lists the rows that have one, and everything after works on those
 // rows alone, packed (their number stays on the device: the kernels read it).
+#include <float.h>
+#include <limits.h>
+
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -55,8 +62,8 @@ __device__ __forceinline__ float ex2(float x) {
 // changes its size by more than 2. Without it one random bfloat16 case in four had a gradient 1.5 times as far from
 // the exact one as a float32 G rounded once at the end, with it one in a hundred. Loss gradients that differ from row to row,
 // or a first row that differs from all others, leave the rounding as it is.
-__device__ __forceinline__ float common_factor(const float* dloss, const int* row, int live) {
-    const float x = live > 0 ? fabsf(dloss[row[0]]) : 0.f;
+__device__ __forceinline__ float common_factor(const float* dloss, const int* row, int live, float inv_tau) {
+    const float x = live > 0 ? fabsf(dloss[row[0]] * inv_tau) : 0.f;
     if (!(x > 1e-37f && x < 1e37f)) return 1.f;
     return __uint_as_float((__float_as_uint(x) & 0x007FFFFFu) | 0x3F800000u);
 }
@@ -89,6 +96,11 @@ struct Gemm {
     int part_tile0;
     float* picked;        // the target's logit
     const float *lse, *dloss;
+    float inv_tau;        // 1 without TOP
+    const int* ids;       // TOP, of the rows as they were given: (rows, top) ids in rising order, absent ones INT_MAX
+    const float* prob;    // their probabilities
+    float* logit;         // their logits
+    int top;
     bf16* g;              // (planes, rows, ldg)
     long ldg, g_plane;
     int planes;
@@ -107,7 +119,18 @@ struct Tile {
     static constexpr size_t bytes = (size_t)STAGES * STAGE + EPW * OUTW + 1024 + 256;
 };
 
-template <int EPI, int BN>
+// The first of a row's entries at or behind `from`.
+__device__ __forceinline__ int first_entry(const int* ids, int n, int from) {
+    int lo = 0;
+    while (n > 0) {
+        const int half = n >> 1;
+        if (__ldg(ids + lo + half) < from) lo += half + 1, n -= half + 1;
+        else n = half;
+    }
+    return lo;
+}
+
+template <int EPI, int BN, bool TOP>
 __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Gemm a) {
     using TL = Tile<EPI, BN>;
     constexpr int S = TL::STAGES, HALF = BN / 2;
@@ -141,7 +164,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     const int live = __shfl_sync(kFull, *a.live, 0);
     const int m0 = min(a.job[0].m, live), tiles0 = (m0 + BM - 1) / BM;
     const int kb1 = (min(a.job[1].k, live) + BK - 1) / BK, blocks1 = EPI == OUT ? (kb1 + max(a.job[1].splits, 1) - 1) / max(a.job[1].splits, 1) : 0;
-    const float factor = EPI == LSE ? 1.f : common_factor(a.dloss, a.row, live);
+    const float factor = EPI == LSE ? 1.f : common_factor(a.dloss, a.row, live, a.inv_tau);
     const long units0 = (long)tiles0 * a.job[0].tiles_n * a.job[0].splits;
     const long units = units0 + (EPI == OUT ? a.job[1].units : 0);
 
@@ -250,6 +273,21 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
         for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
             const Unit r = unit(u);
             const Job& job = a.job[r.job];
+            const int* ids = nullptr;
+            long entry0 = 0;
+            int entry = 0, next = INT_MAX;  // the row's next entry, as a column of the tile
+            if constexpr (TOP) {
+                const int row = r.tm * BM + quarter * 32 + lane, col0 = a.v0 + r.tn * BN;
+                if (row < m0) {
+                    entry0 = (long)a.row[row] * a.top, ids = a.ids + entry0;
+                    entry = first_entry(ids, a.top, col0 + half * HALF);
+                    if (entry < a.top) next = __ldg(ids + entry) - col0;
+                }
+            }
+            auto step_entry = [&] {
+                ++entry;
+                next = entry < a.top ? __ldg(ids + entry) - a.v0 - r.tn * BN : INT_MAX;
+            };
             for (int from = r.k0; from == r.k0 || from < r.k1; from += a.run, ++tile) {
                 const int buf = (int)(tile & 1);
                 if (!(ok = __all_sync(kFull, mbar_wait(acc_full + buf, (uint32_t)((tile >> 1) & 1), fail)))) break;
@@ -260,7 +298,8 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 const int cols = min(half * HALF + HALF, job.n - r.tn * BN);
                 const bool add = job.add || from > r.k0;
                 if (EPI == LSE) {
-                    const int pick = in ? a.target[row] - a.v0 - r.tn * BN : -1;
+                    const int pick = !TOP && in ? a.target[row] - a.v0 - r.tn * BN : -1;
+                    const float scale = TOP ? kLog2e * a.inv_tau : kLog2e;
                     float mx = -INFINITY, sum = 0.f;
                     for (int c = half * HALF; c < cols; c += 32) {
                         float v[32];
@@ -278,7 +317,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                         // the maximum leaves before the scaling: its own term is 1 and no other one exceeds it, where a rounded
                         // -mx * log2(e) put every exponent off by up to 2^-24 of the maximum
                         const float base = mx == -INFINITY ? 0.f : mx;
-                        const uint64_t scale2 = pair(kLog2e, kLog2e), base2 = pair(-base, -base);
+                        const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
                         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
@@ -286,8 +325,17 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                             unpair(mul2(add2(pair(v[j], v[j + 1]), base2), scale2), e0, e1);
                             part[j & 3] += ex2(e0), part[(j & 3) + 1] += ex2(e1);
                         }
-                        sum = sum * exp2f((was - base) * kLog2e) + ((part[0] + part[1]) + (part[2] + part[3]));
-                        if ((unsigned)(pick - c) < 32u) {
+                        sum = sum * exp2f((was - base) * scale) + ((part[0] + part[1]) + (part[2] + part[3]));
+                        if constexpr (TOP) {
+                            const int end = min(c + 32, cols);
+                            while (next < end) {
+                                float z = 0.f;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) z = next - c == j ? v[j] : z;
+                                a.logit[entry0 + entry] = z;
+                                step_entry();
+                            }
+                        } else if ((unsigned)(pick - c) < 32u) {
                             float z = 0.f;
 #pragma unroll
                             for (int j = 0; j < 32; ++j) z = pick - c == j ? v[j] : z;
@@ -297,16 +345,17 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                     if (in) a.part[(long)((a.part_tile0 + r.tn) * 2 + half) * job.m + row] = make_float2(mx, sum);
                 } else if (EPI == GRAD) {
                     const int t = in ? a.target[row] : -1;
-                    const int pick = t < 0 ? -1 : t - a.v0 - r.tn * BN;
-                    const float w = t < 0 ? 0.f : a.dloss[a.row[row]] / factor;
+                    const int pick = TOP || t < 0 ? -1 : t - a.v0 - r.tn * BN;
+                    const float w = t < 0 ? 0.f : a.dloss[a.row[row]] * a.inv_tau / factor;
+                    const float scale = TOP ? kLog2e * a.inv_tau : kLog2e;
                     const float lse = in ? a.lse[row] : 0.f, shift = -lse * kLog2e;
-                    const uint64_t scale2 = pair(kLog2e, kLog2e), shift2 = pair(shift, shift);
+                    const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
                     for (int c = half * HALF; c < cols; c += 32) {
                         float v[32];
                         tmem_ld32(src + c, v);
                         if (a.planes > 1) {  // float32: the scaled exponent's own rounding (2^-24 of some 15) would be the largest error
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = expf(v[j] - lse);
+                            for (int j = 0; j < 32; ++j) v[j] = expf(TOP ? fmaf(v[j], a.inv_tau, -lse) : v[j] - lse);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; j += 2) {
@@ -315,7 +364,15 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                                 v[j] = ex2(e0), v[j + 1] = ex2(e1);
                             }
                         }
-                        if ((unsigned)(pick - c) < 32u) {
+                        if constexpr (TOP) {
+                            const int end = min(c + 32, cols);
+                            while (next < end) {
+                                const float p = __ldg(a.prob + entry0 + entry);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] -= next - c == j ? p : 0.f;
+                                step_entry();
+                            }
+                        } else if ((unsigned)(pick - c) < 32u) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] -= pick - c == j ? 1.f : 0.f;
                         }
@@ -524,13 +581,90 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Pack<
     }
 }
 
-// The row's logsumexp from the tiles' maxima and sums: 32 rows by 8 groups of tiles a CTA.
+// A distribution's targets: by row of the call, see the epilogues.
+struct Entries {
+    int *ids, *flag;             // flag: 0 where the row has a distribution, else -1: the row plan's targets
+    float *prob, *self;          // self: sum p log p
+    int top;
+    float inv_tau;
+};
+
+inline Entries entries_of(void* p, long rows, int top, float inv_tau) {
+    int* at = static_cast<int*>(p);
+    float* f = reinterpret_cast<float*>(at + rows * (top + 1));
+    return Entries{at, at + rows * top, f, f + rows * top, top, inv_tau};
+}
+
+constexpr int kMaxTop = 128;
+
+// A warp a row: the probabilities of its entries, sorted by id (equal ids keep their order). Ids below zero and logits of -inf are
+// absent, a row of which is left nothing has no target; an id beyond the vocabulary is absent and reported.
+template <typename L>
+__global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ ids, int wide, const L* __restrict__ logits, long rows, long vocab,
+                                                      Entries e, int* status) {
+    constexpr int E = kMaxTop / 32;
+    __shared__ int keys[8][kMaxTop];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + warp;
+    if (row >= rows) return;
+    int id[E];
+    float t[E], top = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int i = k * 32 + lane;
+        id[k] = INT_MAX, t[k] = -INFINITY;
+        if (i < e.top) {
+            const long at = row * e.top + i;
+            const long v = wide ? (long)__ldg(static_cast<const long long*>(ids) + at) : (long)__ldg(static_cast<const int*>(ids) + at);
+            if (v >= vocab) report(status, EWS_ERR_INDEX);
+            const float x = to_f(logits[at]) * e.inv_tau;
+            if (v >= 0 && v < vocab && x != -INFINITY) id[k] = (int)v, t[k] = x, bad = bad || x != x, top = fmaxf(top, x);
+            keys[warp][i] = id[k];
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    if (__any_sync(kFull, bad)) top = NAN;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (id[k] != INT_MAX) sum += expf(t[k] - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    const float log_sum = logf(sum);
+    float self = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int i = k * 32 + lane;
+        if (i >= e.top) continue;
+        float p = 0.f;
+        if (id[k] != INT_MAX) {
+            p = expf(t[k] - top) / sum;
+            if (p != 0.f) self += p * (t[k] - top - log_sum);
+        }
+        int rank = 0;
+        for (int j = 0; j < e.top; ++j) {
+            const int other = keys[warp][j];
+            rank += other < id[k] || (other == id[k] && j < i);
+        }
+        e.ids[row * e.top + rank] = id[k];
+        e.prob[row * e.top + rank] = p;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) self += __shfl_xor_sync(kFull, self, o);
+    if (lane == 0) e.self[row] = self, e.flag[row] = top == -INFINITY ? -1 : 0;
+}
+
+// The row's logsumexp from the tiles' maxima and sums: 32 rows by 8 groups of tiles a CTA. TOP: `picked` are the entries' logits.
+template <bool TOP>
 __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ part, int tiles, long rows, RowPlan plan,
-                                                  const float* __restrict__ picked, float* __restrict__ loss, float* __restrict__ lse) {
+                                                  const float* __restrict__ picked, float* __restrict__ loss, float* __restrict__ lse, Entries e) {
     __shared__ float2 red[8][32];
     const int l = threadIdx.x & 31, g = threadIdx.x >> 5;
     const long row = (long)blockIdx.x * 32 + l;
     const int live = *plan.live;
+    const float scale = TOP ? kLog2e * e.inv_tau : kLog2e;
     float m = -INFINITY, s = 0.f;
     if (row < live)
         for (int t0 = g; t0 < tiles; t0 += 64) {
@@ -541,20 +675,40 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
 #pragma unroll
             for (int k = 0; k < 8; ++k) n = fmaxf(n, p[k].x);
             const float base = n == -INFINITY ? 0.f : n;
-            s *= exp2f((m - base) * kLog2e);
+            s *= exp2f((m - base) * scale);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s += p[k].y * exp2f((p[k].x - base) * kLog2e);
+            for (int k = 0; k < 8; ++k) s += p[k].y * exp2f((p[k].x - base) * scale);
             m = n;
         }
     red[g][l] = make_float2(m, s);
     __syncthreads();
-    if (g > 0 || row >= live) return;
+    if (!TOP && (g > 0 || row >= live)) return;
+    m = red[0][l].x, s = red[0][l].y;
     for (int j = 1; j < 8; ++j) {
         const float2 p = red[j][l];
         const float n = fmaxf(m, p.x);
         const float base = n == -INFINITY ? 0.f : n;
-        s = s * exp2f((m - base) * kLog2e) + p.y * exp2f((p.x - base) * kLog2e);
+        s = s * exp2f((m - base) * scale) + p.y * exp2f((p.x - base) * scale);
         m = n;
+    }
+    if constexpr (TOP) {
+        // sum p (m - z) / tau: what a student is sure of and right about cancels first; the groups take the entries in turn
+        const long at = row < live ? (long)plan.row[row] * e.top : 0;
+        float far = 0.f;
+        if (row < live)
+            for (int k = g; k < e.top; k += 8) {
+                const float p = e.prob[at + k];
+                if (p != 0.f) far += p * ((m - picked[at + k]) * e.inv_tau);
+            }
+        __shared__ float sums[8][32];
+        sums[g][l] = far;
+        __syncthreads();
+        if (g > 0 || row >= live) return;
+        for (int j = 1; j < 8; ++j) far += sums[j][l];
+        const float rest = logf(s), kl = far + rest + e.self[plan.row[row]];
+        lse[row] = fmaf(m, e.inv_tau, rest);
+        loss[plan.row[row]] = kl < 0.f ? 0.f : kl;  // no divergence is negative, its rounding may be
+        return;
     }
     // The maximum and the target's logit cancel first, exactly where the target is the maximum: a sum rounded at the
     // logits' size would lose a confident row's loss, or turn it negative. With s >= 1 no loss is.
@@ -568,14 +722,14 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ acc, int splits, long rows, int n, const int* __restrict__ slot,
                                                      const float* __restrict__ dloss, const int* __restrict__ live_rows,
-                                                     const int* __restrict__ row_of, T* __restrict__ out) {
+                                                     const int* __restrict__ row_of, float inv_tau, T* __restrict__ out) {
     constexpr int W = VEC ? 4 : 1;
     const int per = n / W;
     const long total = rows * n;
     // a row's vectors to consecutive threads
     const int lanes = per < 256 ? per : 256, group = 256 / lanes, l = threadIdx.x % lanes, g = threadIdx.x / lanes;
     if (g >= group) return;
-    const float factor = common_factor(dloss, row_of, *live_rows);
+    const float factor = common_factor(dloss, row_of, *live_rows, inv_tau);
     for (long row = (long)blockIdx.x * group + g; row < rows; row += (long)gridDim.x * group) {
         const long at = slot ? slot[row] : row;
         for (int c = l; c < per; c += lanes) {
@@ -641,9 +795,9 @@ Job job_of(long m, long n, long k, int splits) {
     return j;
 }
 
-template <int EPI, int BN>
+template <int EPI, int BN, bool TOP>
 int gemm_bn(const Maps& maps, const Gemm& g, cudaStream_t s) {
-    auto* kern = gemm_kernel<EPI, BN>;
+    auto* kern = gemm_kernel<EPI, BN, TOP>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<EPI, BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
     const long units = g.job[0].units + g.job[1].units;
     kern<<<(unsigned)(units < SMS ? units : SMS), NTH, Tile<EPI, BN>::bytes, s>>>(maps, g);
@@ -664,7 +818,9 @@ int gemm(Gemm g, const Operand& a0, const Operand& b0, const Operand& a1, const 
     const int bn = tile_n(g.job[0].units ? g.job[0].n : g.job[1].n);
     if (g.job[0].units && (!make_map(&m.a[0], a0, BM) || !make_map(&m.b[0], b0, EPI == OUT ? 64 : bn))) return EWS_ERR_LAUNCH;
     if (g.job[1].units && (!make_map(&m.a[1], a1, 64) || !make_map(&m.b[1], b1, 64))) return EWS_ERR_LAUNCH;
-    return bn == 128 ? gemm_bn<EPI, 128>(m, g, s) : gemm_bn<EPI, 256>(m, g, s);
+    if constexpr (EPI != OUT)
+        if (g.top) return bn == 128 ? gemm_bn<EPI, 128, true>(m, g, s) : gemm_bn<EPI, 256, true>(m, g, s);
+    return bn == 128 ? gemm_bn<EPI, 128, false>(m, g, s) : gemm_bn<EPI, 256, false>(m, g, s);
 }
 
 struct Plan {
@@ -712,7 +868,7 @@ void pick_pieces(Plan* p, long n, long v, long d, bool bwd) {
     }
 }
 
-Plan plan(const ews_vocab_args* a, bool bwd) {
+Plan plan(const ews_vocab_args* a, bool bwd, int top = 1) {
     Plan p{};
     p.planes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
     p.ldd = (int)up(a->dim, 8);
@@ -728,7 +884,7 @@ Plan plan(const ews_vocab_args* a, bool bwd) {
     p.h = take(sizeof(bf16) * (size_t)p.planes * n * p.ldd);
     if (p.pack_w) p.w = take(sizeof(bf16) * (size_t)p.planes * p.piece * p.ldd);
     if (!bwd) {
-        p.picked = take(sizeof(float) * n);
+        p.picked = take(sizeof(float) * n * top);
         const long tiles = p.pieces * ((p.piece + tile_n(p.piece) - 1) / tile_n(p.piece));
         p.part = take(sizeof(float2) * 2 * tiles * n);
     } else {
@@ -751,12 +907,12 @@ unsigned grid_of(long total) {
 }
 
 template <typename T>
-int reduce(const ews_vocab_args* a, const float* acc, int splits, long rows, const int* slot, T* out, cudaStream_t s) {
+int reduce(const ews_vocab_args* a, const float* acc, int splits, long rows, const int* slot, float inv_tau, T* out, cudaStream_t s) {
     const RowPlan plan = row_plan(a->plan, a->rows);
     const long n = a->dim;
     const unsigned grid = grid_of(rows * n / 4 + 1);
-    if (n % 4 == 0 && aligned16(out)) reduce_kernel<T, true><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, a->dloss, plan.live, plan.row, out);
-    else reduce_kernel<T, false><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, a->dloss, plan.live, plan.row, out);
+    if (n % 4 == 0 && aligned16(out)) reduce_kernel<T, true><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, a->dloss, plan.live, plan.row, inv_tau, out);
+    else reduce_kernel<T, false><<<grid, 256, 0, s>>>(acc, splits, rows, (int)n, slot, a->dloss, plan.live, plan.row, inv_tau, out);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -785,18 +941,26 @@ int operands(const ews_vocab_args* a, const Plan& p, char* w, long v0, long n, O
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
+// The rows' distributions in a product's arguments; without any, the targets' own.
+void targets(Gemm* g, const Entries* e) {
+    g->inv_tau = e ? e->inv_tau : 1.f;
+    if (e) g->ids = e->ids, g->prob = e->prob, g->top = e->top;
+}
+
 template <typename T>
-int forward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
+int forward(const ews_vocab_args* a, const Plan& p, const Entries* e, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     Operand h{}, wt{}, none{};
     int rc = EWS_OK;
     Gemm g{};
     const RowPlan plan = row_plan(a->plan, a->rows);
-    plan_kernel<<<1, 1024, 0, s>>>(a->targets, a->targets_wide, a->rows, a->vocab, a->ignore, plan, a->loss, a->status);
+    if (e) plan_kernel<<<1, 1024, 0, s>>>(e->flag, 0, a->rows, a->vocab, -1, plan, a->loss, a->status);
+    else plan_kernel<<<1, 1024, 0, s>>>(a->targets, a->targets_wide, a->rows, a->vocab, a->ignore, plan, a->loss, a->status);
     g.status = a->status;
+    targets(&g, e);
     g.live = plan.live, g.target = plan.target, g.row = plan.row;
     g.part = reinterpret_cast<float2*>(w + p.part);
-    g.picked = reinterpret_cast<float*>(w + p.picked);
+    g.picked = g.logit = reinterpret_cast<float*>(w + p.picked);
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
         const long n = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
         if ((rc = operands<T>(a, p, w, v0, n, &h, &wt, s)) != EWS_OK) break;
@@ -805,12 +969,14 @@ int forward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
         g.part_tile0 += g.job[0].tiles_n;
     }
     if (rc != EWS_OK) return rc;
-    lse_kernel<<<(unsigned)((a->rows + 31) / 32), 256, 0, s>>>(g.part, 2 * g.part_tile0, a->rows, plan, g.picked, a->loss, a->lse);
+    const unsigned grid = (unsigned)((a->rows + 31) / 32);
+    if (e) lse_kernel<true><<<grid, 256, 0, s>>>(g.part, 2 * g.part_tile0, a->rows, plan, g.picked, a->loss, a->lse, *e);
+    else lse_kernel<false><<<grid, 256, 0, s>>>(g.part, 2 * g.part_tile0, a->rows, plan, g.picked, a->loss, a->lse, Entries{});
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
 template <typename T>
-int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
+int backward(const ews_vocab_args* a, const Plan& p, const Entries* e, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     Operand h{}, wt{}, go{}, none{};
     int rc = EWS_OK;
@@ -819,6 +985,7 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
     float* acc_w = p.acc_w ? reinterpret_cast<float*>(w + p.aw) : nullptr;
     Gemm base{};
     base.status = a->status;
+    targets(&base, e);
     base.live = plan.live, base.target = plan.target, base.row = plan.row, base.lse = a->lse, base.dloss = a->dloss;
     base.g = reinterpret_cast<bf16*>(w + p.g), base.planes = p.planes;
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
@@ -841,9 +1008,9 @@ int backward(const ews_vocab_args* a, const Plan& p, cudaStream_t s) {
             if constexpr (sizeof(T) == 2) o.job[1].out = out;  // read where there are no partials
         }
         if ((rc = gemm<OUT>(o, go, wt, go, h, p.planes, s)) != EWS_OK) break;
-        if (a->dweight && acc_w) rc = reduce<T>(a, acc_w, p.split_w, n, nullptr, out, s);
+        if (a->dweight && acc_w) rc = reduce<T>(a, acc_w, p.split_w, n, nullptr, base.inv_tau, out, s);
     }
-    if (rc == EWS_OK && a->dhidden) rc = reduce<T>(a, acc_h, p.split_h, a->rows, plan.slot, static_cast<T*>(a->dhidden), s);
+    if (rc == EWS_OK && a->dhidden) rc = reduce<T>(a, acc_h, p.split_h, a->rows, plan.slot, base.inv_tau, static_cast<T*>(a->dhidden), s);
     return rc;
 }
 
@@ -856,28 +1023,84 @@ extern "C" size_t ews_vocab_work_size(const ews_vocab_args* a, int backward_pass
     return check(a) == EWS_OK && a->rows > 0 ? plan(a, backward_pass != 0).bytes : 0;
 }
 
-extern "C" int ews_vocab_fwd(const ews_vocab_args* a, ews_stream_t stream) {
-    const int rc = check(a);
-    if (rc != EWS_OK) return rc;
-    if (a->rows == 0) return EWS_OK;
-    if (!a->hidden || !a->weight || !a->targets || !a->loss || !a->lse || !a->plan) return EWS_ERR_INVALID_ARGUMENT;
-    const Plan p = plan(a, false);
+namespace ews {
+namespace vocab {
+
+int run_forward(const ews_vocab_args* a, const Entries* e, cudaStream_t s) {
+    const Plan p = plan(a, false, e ? e->top : 1);
     if (!a->work || !aligned16(a->work) || a->work_bytes < p.bytes) return EWS_ERR_WORKSPACE;
-    return a->dtype == EWS_DTYPE_BF16 ? forward<bf16>(a, p, (cudaStream_t)stream) : forward<float>(a, p, (cudaStream_t)stream);
+    return a->dtype == EWS_DTYPE_BF16 ? forward<bf16>(a, p, e, s) : forward<float>(a, p, e, s);
 }
 
-extern "C" int ews_vocab_bwd(const ews_vocab_args* a, ews_stream_t stream) {
-    const int rc = check(a);
-    if (rc != EWS_OK) return rc;
-    cudaStream_t s = (cudaStream_t)stream;
+int run_backward(const ews_vocab_args* a, const Entries* e, cudaStream_t s) {
     if (a->rows == 0) {
-        const size_t e = a->dtype == EWS_DTYPE_BF16 ? 2 : 4;
-        if (a->dweight && cudaMemsetAsync(a->dweight, 0, e * a->vocab * a->dim, s) != cudaSuccess) return EWS_ERR_LAUNCH;
+        const size_t size = a->dtype == EWS_DTYPE_BF16 ? 2 : 4;
+        if (a->dweight && cudaMemsetAsync(a->dweight, 0, size * a->vocab * a->dim, s) != cudaSuccess) return EWS_ERR_LAUNCH;
         return EWS_OK;
     }
     if (!a->hidden || !a->weight || !a->dloss || !a->lse || !a->plan) return EWS_ERR_INVALID_ARGUMENT;
     if (!a->dhidden && !a->dweight) return EWS_OK;
     const Plan p = plan(a, true);
     if (!a->work || !aligned16(a->work) || a->work_bytes < p.bytes) return EWS_ERR_WORKSPACE;
-    return a->dtype == EWS_DTYPE_BF16 ? backward<bf16>(a, p, s) : backward<float>(a, p, s);
+    return a->dtype == EWS_DTYPE_BF16 ? backward<bf16>(a, p, e, s) : backward<float>(a, p, e, s);
+}
+
+int check_top(const ews_distill_args* a) {
+    if (!a) return EWS_ERR_INVALID_ARGUMENT;
+    const int rc = check(&a->v);
+    if (rc != EWS_OK) return rc;
+    if (a->top <= 0 || !(a->inv_temperature >= FLT_MIN && a->inv_temperature <= FLT_MAX)) return EWS_ERR_INVALID_ARGUMENT;
+    if (a->top > kMaxTop || (a->logits_dtype != EWS_DTYPE_F32 && a->logits_dtype != EWS_DTYPE_BF16)) return EWS_ERR_UNSUPPORTED;
+    return EWS_OK;
+}
+
+}  // namespace vocab
+}  // namespace ews
+
+extern "C" int ews_vocab_fwd(const ews_vocab_args* a, ews_stream_t stream) {
+    const int rc = check(a);
+    if (rc != EWS_OK) return rc;
+    if (a->rows == 0) return EWS_OK;
+    if (!a->hidden || !a->weight || !a->targets || !a->loss || !a->lse || !a->plan) return EWS_ERR_INVALID_ARGUMENT;
+    return run_forward(a, nullptr, (cudaStream_t)stream);
+}
+
+extern "C" int ews_vocab_bwd(const ews_vocab_args* a, ews_stream_t stream) {
+    const int rc = check(a);
+    return rc != EWS_OK ? rc : run_backward(a, nullptr, (cudaStream_t)stream);
+}
+
+extern "C" size_t ews_distill_entries_size(int64_t rows, int top) {
+    return rows > 0 && top > 0 ? sizeof(int) * 2 * (size_t)rows * ((size_t)top + 1) : 0;
+}
+
+extern "C" size_t ews_distill_work_size(const ews_distill_args* a, int backward_pass) {
+    return check_top(a) == EWS_OK && a->v.rows > 0 ? plan(&a->v, backward_pass != 0, a->top).bytes : 0;
+}
+
+extern "C" int ews_distill_fwd(const ews_distill_args* a, ews_stream_t stream) {
+    const int rc = check_top(a);
+    if (rc != EWS_OK) return rc;
+    const ews_vocab_args* v = &a->v;
+    if (v->rows == 0) return EWS_OK;
+    if (!v->hidden || !v->weight || !v->loss || !v->lse || !v->plan || !a->ids || !a->logits || !a->entries) return EWS_ERR_INVALID_ARGUMENT;
+    const Plan p = plan(v, false, a->top);
+    if (!v->work || !ews::token::aligned16(v->work) || v->work_bytes < p.bytes) return EWS_ERR_WORKSPACE;
+    cudaStream_t s = (cudaStream_t)stream;
+    const Entries e = entries_of(a->entries, v->rows, a->top, a->inv_temperature);
+    const unsigned grid = (unsigned)((v->rows + 7) / 8);
+    if (a->logits_dtype == EWS_DTYPE_BF16)
+        entries_kernel<ews::token::bf16><<<grid, 256, 0, s>>>(a->ids, a->ids_wide, static_cast<const ews::token::bf16*>(a->logits), v->rows, v->vocab, e, v->status);
+    else
+        entries_kernel<float><<<grid, 256, 0, s>>>(a->ids, a->ids_wide, static_cast<const float*>(a->logits), v->rows, v->vocab, e, v->status);
+    if (cudaGetLastError() != cudaSuccess) return EWS_ERR_LAUNCH;
+    return run_forward(v, &e, s);
+}
+
+extern "C" int ews_distill_bwd(const ews_distill_args* a, ews_stream_t stream) {
+    const int rc = check_top(a);
+    if (rc != EWS_OK) return rc;
+    if (a->v.rows > 0 && !a->entries) return EWS_ERR_INVALID_ARGUMENT;
+    const Entries e = entries_of(a->entries, a->v.rows, a->top, a->inv_temperature);
+    return run_backward(&a->v, &e, (cudaStream_t)stream);
 }

@@ -2,7 +2,8 @@
 
 ``token_embedding`` (scaled lookup, gradient by sorted tokens), ``decayed_attention`` (linear attention with a decay
 per head, over prompts and in training) with ``decayed_attention_step`` (one token per row on a pool of states), and
-``vocab_loss`` (softmax cross entropy over a large vocabulary whose logits are never kept). All run on the caller's
+``vocab_loss`` (softmax cross entropy over a large vocabulary whose logits are never kept) with ``distill_loss`` (the same
+against a teacher's top logits). All run on the caller's
 current stream through the C ABI, on float32 or bfloat16 CUDA tensors; states, sums, softmax statistics and losses
 are float32. There is no CPU fallback. Derivatives are reverse-mode and first-order: a dual tensor is refused, and so
 is differentiating a gradient again. Indices out of range do not stop the GPU: the entry counts as absent and the next
@@ -24,10 +25,12 @@ from .engine import _require_cuda, _timed, first_order
 _DTYPES = {torch.float32: _lib.EWS_DTYPE_F32, torch.bfloat16: _lib.EWS_DTYPE_BF16}
 _WIDE = {torch.int64: 1, torch.int32: 0}
 MAX_HEAD = 128
+MAX_TOP = 128
 
 # ews_decay_args and ews_vocab_args, packed in one call (native alignment; the fields in the header's order).
 _DECAY = struct.Struct("@7if3P9q6P3q6PNP").pack
 _VOCAB = struct.Struct("@3q2i3P3q7PNP").pack
+_TOP = struct.Struct("@2P3ifP").pack  # what ews_distill_args has behind its ews_vocab_args
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without building a Stream
 
@@ -395,3 +398,106 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _VocabLoss.apply(flat, weight, t, int(ignore_index), targets.shape)
     return _vocab(_rows(flat), _rows(weight), t, int(ignore_index), targets.shape)[0]
+
+
+# ------------------------------------------------------------------------------------- a teacher's top logits
+
+
+@functools.lru_cache(maxsize=256)
+def _distill_size(rows: int, vocab: int, dim: int, code: int, hidden_stride: int, weight_stride: int, weight_at: int, top: int,
+                  backward: int) -> int:
+    args = _VOCAB(rows, vocab, dim, code, 0, 0, weight_at, 0, hidden_stride, weight_stride, 0, *([0] * 7), 0, 0)
+    return _lib.load().ews_distill_work_size(args + _TOP(0, 0, 0, top, _lib.EWS_DTYPE_F32, 1.0, 0), backward)
+
+
+def _distill_args(hidden, weight, ids, logits, top, inv_tau, entries, loss=None, lse=None, plan=None, dloss=None, dh=None, dw=None,
+                  work=None):
+    rows, dim = hidden.shape
+    return _VOCAB(rows, weight.shape[0], dim, _DTYPES[hidden.dtype], 0, hidden.data_ptr(), weight.data_ptr(), 0, _row_stride(hidden),
+                  _row_stride(weight), 0, _addr(loss), _addr(lse), _addr(plan), _addr(dloss), _addr(dh), _addr(dw), _addr(work),
+                  0 if work is None else work.numel(), engine.index_word(hidden.get_device())[0]) + _TOP(
+                      _addr(ids), _addr(logits), 0 if ids is None else _WIDE[ids.dtype], top,
+                      _lib.EWS_DTYPE_F32 if logits is None else _DTYPES[logits.dtype], inv_tau, entries.data_ptr())
+
+
+def _distill_work(hidden, weight, top, backward):
+    return _work(_distill_size(*hidden.shape[:1], *weight.shape, _DTYPES[hidden.dtype], _row_stride(hidden), _row_stride(weight),
+                               weight.data_ptr() % 16, top, backward), hidden)
+
+
+def _distill(hidden, weight, ids, logits, inv_tau, shape):
+    lib = _lib.load()
+    rows, top = hidden.shape[0], ids.shape[1]
+    loss = torch.empty(shape, dtype=torch.float32, device=hidden.device)  # of its own memory, as vocab_loss's
+    lse = torch.empty(rows, dtype=torch.float32, device=hidden.device)
+    plan = torch.empty(3 * rows + 4, dtype=torch.int32, device=hidden.device)
+    entries = torch.empty(2 * rows * (top + 1), dtype=torch.int32, device=hidden.device)
+    work = _distill_work(hidden, weight, top, 0)
+    args = _distill_args(hidden, weight, ids, logits, top, inv_tau, entries, loss, lse, plan, work=work)
+    _launch(hidden.get_device(), "ews_distill_fwd", rows, lib.ews_distill_fwd, args)
+    return loss, lse, plan, entries
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, logits, inv_tau, shape):
+        hidden, weight = _rows(hidden), _rows(weight)
+        loss, lse, plan, entries = _distill(hidden, weight, ids, logits, inv_tau, shape)
+        ctx.meta = inv_tau, ids.shape[1]
+        ctx.save_for_backward(hidden, weight, lse, plan, entries)
+        return loss
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dloss):
+        hidden, weight, lse, plan, entries = ctx.saved_tensors
+        inv_tau, top = ctx.meta
+        dloss = dloss.contiguous()
+        dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+                  for t, need in ((hidden, ctx.needs_input_grad[0]), (weight, ctx.needs_input_grad[1])))
+        work = _distill_work(hidden, weight, top, 1)
+        args = _distill_args(hidden, weight, None, None, top, inv_tau, entries, None, lse, plan, dloss, dh, dw, work)
+        _launch(hidden.get_device(), "ews_distill_bwd", hidden.shape[0], _lib.load().ews_distill_bwd, args)
+        return dh, dw, None, None, None, None
+
+
+def distill_loss(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                 temperature: float = 1.0) -> torch.Tensor:
+    """Divergence of the student ``softmax(hidden @ weight.T / temperature)`` from a teacher known by its top logits, per
+    position, in float32: ``sum_k p_k (log p_k - log q_k)`` with ``p = softmax(teacher_logits / temperature)`` over a
+    position's entries and q the student's probabilities of ``teacher_ids``.
+
+    hidden (..., D) and weight (V, D), both float32 or both bfloat16; teacher_ids (..., K) int64 or int32, teacher_logits
+    (..., K) float32 or bfloat16, K from 1 to 128, in any order. An entry with a negative id, or with a logit of -inf, is absent;
+    a position of which none is left has loss 0 and no gradient, and costs nothing. An id that occurs twice is two entries; one
+    beyond the vocabulary is absent and raises IndexError on the next call.
+
+    Returns the losses with the shape of ``hidden`` without its last axis, never negative; the logits (N, V) are formed in tiles
+    and pieces and never kept. Differentiable in hidden and weight, the teacher is a constant. (Many scale the mean by
+    temperature^2 beside another loss.)"""
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not fit together")
+    if hidden.dtype != weight.dtype:
+        raise TypeError(f"hidden and weight must share a type, got {hidden.dtype} and {weight.dtype}")
+    _dtype(hidden, "hidden and weight")
+    _wide(teacher_ids, "teacher_ids")
+    _dtype(teacher_logits, "teacher_logits")
+    if teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_logits.shape != teacher_ids.shape:
+        raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} must have the shape "
+                         f"{(*hidden.shape[:-1], 'K')}")
+    top = teacher_ids.shape[-1]
+    if top == 0:
+        raise ValueError("a teacher needs at least one entry a position")
+    if top > MAX_TOP:
+        raise NotImplementedError(f"a teacher has at most {MAX_TOP} entries a position, got {top}")
+    temperature = float(temperature)
+    if not 2.0**-100 <= temperature <= 2.0**100:  # its inverse is taken in float32 too
+        raise ValueError(f"temperature must be positive and within 2^-100 to 2^100, got {temperature}")
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("the teacher is a constant: no gradient is built for its logits")
+    _device(hidden, weight, teacher_ids, teacher_logits)
+    flat = hidden.reshape(-1, hidden.shape[-1])
+    ids, logits = teacher_ids.reshape(-1, top).contiguous(), teacher_logits.detach().reshape(-1, top).contiguous()
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _DistillLoss.apply(flat, weight, ids, logits, 1.0 / temperature, hidden.shape[:-1])
+    return _distill(_rows(flat), _rows(weight), ids, logits, 1.0 / temperature, hidden.shape[:-1])[0]

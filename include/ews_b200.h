@@ -480,6 +480,27 @@ size_t ews_vocab_work_size(const ews_vocab_args* args, int backward);
 int ews_vocab_fwd(const ews_vocab_args* args, ews_stream_t stream);
 int ews_vocab_bwd(const ews_vocab_args* args, ews_stream_t stream);
 
+/* ---- loss against a teacher's top logits -----------------------------------------------------------
+ * loss_n = sum_k p_nk (log p_nk - log q_n[ids_nk]) with p = softmax(logits / temperature) over a row's `top` entries and
+ * q = softmax(<hidden_n, weight_v> / temperature) over the vocabulary. `v` as for ews_vocab_*, without targets and ignore;
+ * ids (rows, top) int64 (ids_wide) or int32, logits (rows, top) of logits_dtype, contiguous, top <= 128. An entry of a
+ * negative id or of a logit of -inf is absent; a row of which none is left has loss 0 and no gradient, and is not computed. An
+ * id that occurs twice is two entries. entries: ews_distill_entries_size(rows, top) bytes, written by the forward for the
+ * backward (`v.dloss` in, `v.dhidden` and `v.dweight` out).
+ * An id beyond the vocabulary is absent and sets *status to EWS_ERR_INDEX. `v.work`: ews_distill_work_size(args, backward)
+ * bytes. */
+typedef struct {
+    ews_vocab_args v;
+    const void *ids, *logits;
+    int ids_wide, top, logits_dtype;
+    float inv_temperature;
+    void* entries;
+} ews_distill_args;
+size_t ews_distill_entries_size(int64_t rows, int top);
+size_t ews_distill_work_size(const ews_distill_args* args, int backward);
+int ews_distill_fwd(const ews_distill_args* args, ews_stream_t stream);
+int ews_distill_bwd(const ews_distill_args* args, ews_stream_t stream);
+
 /* ---- utilities --------------------------------------------------------------------------------- */
 /* Every forward and backward workspace begins with a status block whose error word the call clears and
  * a timed-out device wait sets. */
