@@ -12,7 +12,7 @@ from .logsig import log_level_sizes, log_signature_dim
 from .params import AParamBlockDiag, AParamConstant, AParamDiag, AParamEFM, AParamGeneral, AParamJordanRepeated, B
 from .recur_ops import gated_recurrence, gated_recurrence_step
 from .series import check_series_q, series_error_bound, suggest_series_q
-from .token_model import DecayBlock, TokenModel
+from .token_model import DecayBlock, GatedBlock, TokenModel
 from .token_ops import decayed_attention, decayed_attention_step, distill_loss, token_embedding, vocab_loss
 
 __all__ = [
@@ -32,6 +32,7 @@ __all__ = [
     "series_error_bound",
     "suggest_series_q",
     "DecayBlock",
+    "GatedBlock",
     "TokenModel",
     "decayed_attention",
     "decayed_attention_step",

@@ -1,10 +1,10 @@
-"""A token model on the package's operators: the embedding, residual blocks whose mixer is a decayed linear attention or
-an EWS block, and the vocabulary loss on the tied table. One module for training (``loss``), prompts (``prompt``) and
-single tokens (``step``), so that the operators run together as they are meant to.
+"""A token model on the package's operators: the embedding, residual blocks whose mixer is a decayed linear attention, a gated
+linear recurrence or an EWS block, and the vocabulary loss on the tied table. One module for training (``loss``, from a
+teacher ``distill``), prompts (``prompt``) and single tokens (``step``), so that the operators run together as they are meant to.
 
 The reference's stacked model takes tokens through an embedding (ews/block.py:473-600, ``tokens=True``); the decayed
-attention blocks keep a matrix state a head that a served request carries from token to token, which the EWS blocks'
-prefix scan does not, so ``prompt`` and ``step`` need a model of attention blocks alone.
+attention blocks keep a matrix state a head, the gated blocks one number a channel, that a served request carries from token to
+token, which the EWS blocks' prefix scan does not, so ``prompt`` and ``step`` need a model without EWS blocks.
 """
 
 from __future__ import annotations
@@ -17,7 +17,9 @@ import torch.nn.functional as F
 from torch import nn
 
 from .block import EWSBlock, RMSNorm
-from .token_ops import decayed_attention, decayed_attention_step, token_embedding, vocab_loss
+from .gated_ops import gated_linear
+from .recur_ops import gated_recurrence, gated_recurrence_step
+from .token_ops import decayed_attention, decayed_attention_step, distill_loss, token_embedding, vocab_loss
 
 
 class DecayBlock(nn.Module):
@@ -65,15 +67,57 @@ class DecayBlock(nn.Module):
         q, k, v = self._heads(x)
         return self._close(x, decayed_attention_step(q, k, v, self.rate, state, slots=slots))
 
+    def states(self, slots: int):
+        return torch.zeros(slots, self.heads, self.head_dim, self.head_dim, device=self.out.weight.device)
+
+
+class GatedBlock(nn.Module):
+    """Pre-norm residual block: RMSNorm -> input, decay gate, input gate -> gated recurrence -> projection -> residual -> RMSNorm ->
+    gated linear layer -> projection -> residual. The channels' rates are learned (their logarithms, float32 in the recurrence),
+    at first 1 to 2^-8: half-open gates forget over 2 to 512 tokens. ``width``: the recurrence's channels (hidden_dim);
+    ``ff_dim``: the channel stage's (8/3 hidden_dim, in steps of 8: as many weights as an MLP of four times the width)."""
+
+    def __init__(self, hidden_dim: int, width: Optional[int] = None, ff_dim: Optional[int] = None, *, activation: str = "silu",
+                 norm_eps: float = 1e-6):
+        super().__init__()
+        self.width, self.activation = int(width or hidden_dim), activation
+        ff = int(ff_dim or -(-hidden_dim // 3) * 8)
+        self.norm1, self.norm2 = RMSNorm(hidden_dim, eps=norm_eps), RMSNorm(hidden_dim, eps=norm_eps)
+        self.inputs = nn.Linear(hidden_dim, 3 * self.width, bias=False)
+        self.out = nn.Linear(self.width, hidden_dim, bias=False)
+        self.log_rate = nn.Parameter(-math.log(2.0) * torch.linspace(0.0, 8.0, self.width))
+        self.ff_gate, self.ff_up = nn.Linear(hidden_dim, ff, bias=False), nn.Linear(hidden_dim, ff, bias=False)
+        self.ff_down = nn.Linear(ff, hidden_dim, bias=False)
+
+    def _mixer(self, x):
+        """The recurrence's x, decay, gate and rate."""
+        return (*self.inputs(self.norm1(x)).split(self.width, -1), torch.exp(self.log_rate.float()))
+
+    def _close(self, x, h):
+        x = x + self.out(h)
+        return x + self.ff_down(gated_linear(self.norm2(x), self.ff_gate.weight, self.ff_up.weight, activation=self.activation))
+
+    def forward(self, x, lengths=None, state=None, return_state=False):
+        got = gated_recurrence(*self._mixer(x), initial_state=state, lengths=lengths, return_state=return_state)
+        return (self._close(x, got[0]), got[1]) if return_state else self._close(x, got)
+
+    def step(self, x, state, slots=None):
+        return self._close(x, gated_recurrence_step(*self._mixer(x), state, slots=slots))
+
+    def states(self, slots: int):
+        return torch.zeros(slots, self.width, device=self.out.weight.device)
+
 
 class TokenModel(nn.Module):
     """Embedding (scaled by sqrt(hidden)), blocks, RMSNorm, and logits on the embedding's table.
 
-    ``mixers``: one entry a block, "decay" (DecayBlock) or "ews" (EWSBlock with ``ews_kwargs``; float32). ``seed`` is for the
-    table and the EWS blocks' generators; linear layers draw from torch's global generator, as in ``StackedEWS``."""
+    ``mixers``: one entry a block, "decay" (DecayBlock), "gated" (GatedBlock with ``gated_kwargs``) or "ews" (EWSBlock with
+    ``ews_kwargs``; float32). ``seed`` is for the table and the EWS blocks' generators; linear layers draw from torch's global
+    generator, as in ``StackedEWS``."""
 
     def __init__(self, vocab: int, hidden_dim: int = 128, heads: int = 4, mixers=("decay", "decay"), *,
-                 kv_heads: Optional[int] = None, head_dim: Optional[int] = None, ews_kwargs: Optional[dict] = None, seed: int = 0):
+                 kv_heads: Optional[int] = None, head_dim: Optional[int] = None, ews_kwargs: Optional[dict] = None,
+                 gated_kwargs: Optional[dict] = None, seed: int = 0):
         super().__init__()
         g = torch.Generator().manual_seed(int(seed))
         self.vocab, self.hidden_dim = int(vocab), int(hidden_dim)
@@ -82,23 +126,25 @@ class TokenModel(nn.Module):
         for kind in mixers:
             if kind == "decay":
                 blocks.append(DecayBlock(hidden_dim, heads, kv_heads, head_dim))
+            elif kind == "gated":
+                blocks.append(GatedBlock(hidden_dim, **(gated_kwargs or {})))
             elif kind == "ews":
                 blocks.append(EWSBlock(hidden_dim, generator=g, **(ews_kwargs or {})))
             else:
-                raise ValueError(f"a mixer is 'decay' or 'ews', got {kind!r}")
+                raise ValueError(f"a mixer is 'decay', 'gated' or 'ews', got {kind!r}")
         self.blocks = nn.ModuleList(blocks)
         self.norm = RMSNorm(hidden_dim)
 
     def _served(self):
         for block in self.blocks:
-            if not isinstance(block, DecayBlock):
-                raise NotImplementedError("prompt and step need a model of decayed attention blocks alone")
+            if not isinstance(block, (DecayBlock, GatedBlock)):
+                raise NotImplementedError("prompt and step need a model of decayed attention and gated blocks alone")
 
     def hidden(self, ids, lengths=None):
         """(B, T) ids -> the normalised hidden rows (B, T, hidden)."""
         x = token_embedding(ids, self.table, scale=math.sqrt(self.hidden_dim))
         for block in self.blocks:
-            x = block(x, lengths) if isinstance(block, DecayBlock) else block(x)
+            x = block(x, lengths) if isinstance(block, (DecayBlock, GatedBlock)) else block(x)
         return self.norm(x)
 
     def loss(self, ids, targets, lengths=None, ignore_index: int = -100):
@@ -106,10 +152,17 @@ class TokenModel(nn.Module):
         losses = vocab_loss(self.hidden(ids, lengths), self.table, targets, ignore_index=ignore_index)
         return losses.sum() / (targets != ignore_index).sum().clamp(min=1)
 
+    def distill(self, ids, teacher_ids, teacher_logits, lengths=None, temperature: float = 1.0):
+        """temperature^2 times the mean divergence from a teacher's top logits (B, T, K) over the positions that have any; an entry
+        with a negative id is absent."""
+        losses = distill_loss(self.hidden(ids, lengths), self.table, teacher_ids, teacher_logits, temperature=temperature)
+        there = ((teacher_ids >= 0) & (teacher_logits != -math.inf)).any(-1).sum()
+        return temperature**2 * losses.sum() / there.clamp(min=1)
+
     def states(self, slots: int):
         """Zero states for ``slots`` requests, one pool a block."""
         self._served()
-        return [torch.zeros(slots, b.heads, b.head_dim, b.head_dim, device=self.table.device) for b in self.blocks]
+        return [b.states(slots) for b in self.blocks]
 
     @torch.no_grad()
     def prompt(self, ids, lengths=None):
