@@ -290,6 +290,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             fn.restype = _c_int
         lib.ews_recur_step.argtypes = [ctypes.c_char_p, _vp, _c_int, _vp, _vp]
         lib.ews_recur_step.restype = _c_int
+        lib.ews_gated_kept_size.argtypes = [ctypes.c_char_p]
+        lib.ews_gated_kept_size.restype = _c_size
         lib.ews_gated_work_size.argtypes = [ctypes.c_char_p, _c_int]
         lib.ews_gated_work_size.restype = _c_size
         for name in ("ews_gated_fwd", "ews_gated_bwd"):

@@ -7,12 +7,14 @@
 // 128-byte-swizzled tiles, K-major or MN-major as they lie in memory, tcgen05.mma of 128 x BN x 16, the accumulator in tensor
 // memory, two deep, so that a tile's epilogue runs under the next one's products.
 //   FWD  a tile's B operand is BN / 2 rows of Wg above the same rows of Wu, so that a gate and its partner end in one lane:
-//        the epilogue forms H, and for training also leaves G and U in the inputs' type (rounded once; H is formed from the
-//        float32 sums). Keeping them costs 2 N F values and spares the backward a third of its products.
+//        the epilogue forms H, and for training also leaves G and U: float32 as they are, for bfloat16 inputs their first 24 bits,
+//        so that the gradients see one rounding between the products, dG's and dU's own (with G and U in bfloat16 they were 1.8
+//        times as far from the exact ones as a single rounding leaves them, so 1.35 times). Keeping them spares the backward a
+//        third of its products.
 //   OUT  all gradients' tiles in one launch: dX (K runs over both pairs), dWg and dWu.
 // dG and dU are formed by one pass over dH, G and U in between.
 // Operands are bfloat16. float32 inputs are split into three bfloat16 planes (8 bits each) and a product runs over the six pairs
-// of planes that matter (2^-24), smallest first; every 256 of K the sum leaves the tensor core's accumulator, which truncates at
+// of planes that matter (2^-24), smallest first; every 128 of K the sum leaves the tensor core's accumulator, which truncates at
 // every addition, and is added in registers.
 //
 // Few rows (a served batch's tokens) are bound by the weights' bytes: few_kernel gives each CTA 16 rows of both weights, its warps
@@ -29,7 +31,7 @@ constexpr int BM = 128, BK = 64;
 constexpr int EPW = 8;              // epilogue warps
 constexpr int NTH = 64 + EPW * 32;  // and one each for TMA and MMA
 constexpr int SMS = 148;
-constexpr int kRun = 4;             // float32: k blocks of 64 in one accumulator
+constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulator
 constexpr int kFewBf16 = 64, kFewF32 = 16;  // rows up to which few_kernel / few_f32_kernel run
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
@@ -77,7 +79,8 @@ struct Gemm {
     Job job[3];   // FWD: one; OUT: dX (A K-major), dWg, dWu (A MN-major)
     int run;      // k blocks in one accumulator
     int act;
-    void *g, *u;  // FWD: the projections, or null
+    void* kept;   // FWD: the projections, or null
+    long plane;   // bytes from one plane of it to the next
     int* status;
 };
 
@@ -89,40 +92,97 @@ template <int BN>
 struct Tile {
     static constexpr int A = BM * BK * 2, B = BN * BK * 2, STAGE = A + B;
     static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr size_t bytes = (size_t)STAGES * STAGE + 1024 + 256;
+    static constexpr int SHARE = 32 * 17 * 4;  // a warp's exchange of 32 rows by 16 columns, see store_block
+    static constexpr size_t bytes = (size_t)STAGES * STAGE + EPW * SHARE + 1024 + 256;
 };
 
-// Up to 32 consecutive results of a row, `w` of them there: whole sectors where the rows allow them.
-template <typename T>
-__device__ __forceinline__ void store_row(T* p, const float v[32], int w, bool vec) {
-    if (w == 32 && vec) {
-        if constexpr (sizeof(T) == 2) {
-            uint32_t q[16];
+// A warp's block of 32 rows (one a lane, `rows` of them there) by 32 columns (w there) of BYTES an element, packed in words.
+// Whole sectors from each lane where the rows start on them; else by way of shared memory, so that a store has 16 neighbours
+// of a row instead of 32 rows' single elements (341 columns of float32: 47 -> 15 us for 5,760 rows).
+template <int BYTES>
+__device__ __forceinline__ void store_block(char* base, long row_bytes, int rows, int w, const uint32_t* q, bool whole, uint32_t* share, int lane) {
+    constexpr int WORDS = 8 * BYTES;
+    if (whole && w >= 32) {
+        if (lane < rows) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) q[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-            store32(p, q);
-            store32(p + 16, q + 8);
-        } else {
+            for (int j = 0; j < WORDS; j += 8) store32(base + lane * row_bytes + j * 4, q + j);
+        }
+        return;
+    }
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-                uint32_t q[8];
+    for (int h = 0; h < 32; h += 16) {
+        if (h >= w) break;
+        __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(v[j + e]);
-                store32(p + j, q);
+        for (int j = 0; j < 16; ++j) {
+            const int c = h + j;
+            share[lane * 17 + j] = BYTES == 4 ? q[c % WORDS] : (q[(c / 2) % WORDS] >> (16 * (c & 1)));
+        }
+        __syncwarp();
+        const int col = h + (lane & 15);
+        for (int r = lane >> 4; r < rows; r += 2) {
+            const uint32_t v = share[r * 17 + (lane & 15)];
+            char* p = base + r * row_bytes + col * BYTES;
+            if (col < w) {
+                if (BYTES == 4) *reinterpret_cast<uint32_t*>(p) = v;
+                else *reinterpret_cast<uint16_t*>(p) = (uint16_t)v;
             }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < w) p[j] = from_f<T>(v[j]);
     }
 }
 
+// The same of float results, rounded to T.
 template <typename T>
-__device__ __forceinline__ bool whole_rows(const void* p, int n) {
-    return n % (32 / (int)sizeof(T)) == 0 && ((uintptr_t)p & 31u) == 0;
+__device__ __forceinline__ void store_results(void* out, long row, int rows, int n, int col, int w, const float v[32], uint32_t* share, int lane) {
+    uint32_t q[8 * sizeof(T)];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) q[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) q[j] = __float_as_uint(v[j]);
+    }
+    const bool whole = n % (32 / (int)sizeof(T)) == 0 && ((uintptr_t)out & 31u) == 0;
+    store_block<sizeof(T)>(static_cast<char*>(out) + (row * n + col) * (long)sizeof(T), (long)n * (long)sizeof(T), rows, w, q, whole, share, lane);
 }
 
+// The projections as they are kept. bfloat16: a plane of G's upper halves, one of U's, and one of the bytes below them, G's
+// in the low byte.
+__device__ __forceinline__ uint32_t upper(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+__device__ __forceinline__ uint32_t below(float g, float u) { return __byte_perm(__float_as_uint(g), __float_as_uint(u), 0x0051) & 0xFFFFu; }
+template <typename T>
+__device__ __forceinline__ void keep_block(void* kept, long plane, long row, int rows, int n, int col, int w, const float g[32], const float u[32],
+                                           uint32_t* share, int lane) {
+    char* at = static_cast<char*>(kept);
+    if constexpr (sizeof(T) == 4) {
+        store_results<float>(at, row, rows, n, col, w, g, share, lane);
+        store_results<float>(at + plane, row, rows, n, col, w, u, share, lane);
+    } else {
+        const bool whole = n % 16 == 0 && ((uintptr_t)kept & 31u) == 0;
+        at += (row * n + col) * 2;
+        uint32_t q[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) q[j] = upper(g[2 * j], g[2 * j + 1]);
+        store_block<2>(at, n * 2l, rows, w, q, whole, share, lane);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) q[j] = upper(u[2 * j], u[2 * j + 1]);
+        store_block<2>(at + plane, n * 2l, rows, w, q, whole, share, lane);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) q[j] = below(g[2 * j], u[2 * j]) | below(g[2 * j + 1], u[2 * j + 1]) << 16;
+        store_block<2>(at + 2 * plane, n * 2l, rows, w, q, whole, share, lane);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void keep_one(void* kept, long plane, long at, float g, float u) {
+    char* p = static_cast<char*>(kept) + at * (long)sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float*>(p) = g, *reinterpret_cast<float*>(p + plane) = u;
+    } else {
+        *reinterpret_cast<uint16_t*>(p) = (uint16_t)(__float_as_uint(g) >> 16);
+        *reinterpret_cast<uint16_t*>(p + plane) = (uint16_t)(__float_as_uint(u) >> 16);
+        *reinterpret_cast<uint16_t*>(p + 2 * plane) = (uint16_t)below(g, u);
+    }
+}
 template <typename T, int EPI, int BN>
 __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Gemm a) {
     using TL = Tile<BN>;
@@ -131,7 +191,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     static_assert(!SUM || BN == 128, "the sums of a float32 tile stay in registers");
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S * TL::STAGE);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S * TL::STAGE + EPW * TL::SHARE);
     uint64_t* empty = full + S;
     uint64_t* acc_full = empty + S;   // 2
     uint64_t* acc_empty = acc_full + 2;
@@ -255,13 +315,13 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     } else {
         // two warps share a quarter of the rows and take its blocks of 32 columns in turn
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        uint32_t* share = reinterpret_cast<uint32_t*>(tiles + S * TL::STAGE + (warp - 2) * TL::SHARE);
         long tile = 0;
         bool ok = true;
         for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
             const Unit r = unit(u);
             const Job& job = a.job[r.job];
-            const int row = r.tm * BM + quarter * 32 + lane;
-            const bool in = row < job.m;
+            const int row0 = r.tm * BM + quarter * 32;
             float s0[SUM ? 32 : 1], s1[SUM ? 32 : 1];  // float32: the runs' sums
             for (int from = r.k0; from < r.k1; from += a.run, ++tile) {
                 const int buf = (int)(tile & 1);
@@ -270,14 +330,11 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 const uint32_t src = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
                 const bool last = !SUM || from + a.run >= r.k1;
                 constexpr int SPAN = EPI == FWD ? BN / 2 : BN;
+                const int left = min(job.m - row0, 32);
                 auto close_fwd = [&](int c, float g[32], float up[32]) {
                     const int col = r.tn * (BN / 2) + c, w = min(32, job.n - col);
-                    if (!in || w <= 0) return;
-                    const long at = (long)row * job.n + col;
-                    if (a.g) {
-                        store_row<T>(static_cast<T*>(a.g) + at, g, w, whole_rows<T>(a.g, job.n));
-                        store_row<T>(static_cast<T*>(a.u) + at, up, w, whole_rows<T>(a.u, job.n));
-                    }
+                    if (left <= 0 || w <= 0) return;
+                    if (a.kept) keep_block<T>(a.kept, a.plane, row0, left, job.n, col, w, g, up, share, lane);
                     if (a.act == SILU) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) up[j] *= act_of<SUM>(g[j], SILU);
@@ -285,13 +342,13 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
 #pragma unroll
                         for (int j = 0; j < 32; ++j) up[j] *= act_of<SUM>(g[j], GELU);
                     }
-                    store_row<T>(static_cast<T*>(job.out) + at, up, w, whole_rows<T>(job.out, job.n));
+                    store_results<T>(job.out, row0, left, job.n, col, w, up, share, lane);
                 };
                 auto close_out = [&](int c, const float v[32]) {
                     const int col = r.tn * BN + c, w = min(32, job.n - col);
-                    if (!in || w <= 0) return;
-                    if (job.acc) store_row<float>(job.acc + ((long)r.sp * job.m + row) * job.n + col, v, w, whole_rows<float>(job.acc, job.n));
-                    else store_row<T>(static_cast<T*>(job.out) + (long)row * job.n + col, v, w, whole_rows<T>(job.out, job.n));
+                    if (left <= 0 || w <= 0) return;
+                    if (job.acc) store_results<float>(job.acc, (long)r.sp * job.m + row0, left, job.n, col, w, v, share, lane);
+                    else store_results<T>(job.out, row0, left, job.n, col, w, v, share, lane);
                 };
                 if constexpr (EPI == FWD) {
                     for (int c = half * 32; c < SPAN; c += 64) {
@@ -372,45 +429,81 @@ __device__ __forceinline__ void load8(const T* p, int there, bool vec, float v[8
     }
 }
 
+// Eight projections as they are kept, from element `at` on (`there` of the row left; vec: 16-byte vectors).
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs<T> a, int dim, int ld, int planes) {
-    const int per = ld / 8;
-    const long total = (a.p[0].rows + a.p[1].rows + a.p[2].rows) * per;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        long row = e / per;
-        const int col = (int)(e - row * per) * 8;
-        int k = 0;
-        while (row >= a.p[k].rows) row -= a.p[k++].rows;
-        const Pack<T>& m = a.p[k];
-        float v[8];
-        load8<T>(m.in + row * m.stride + col, dim - col, m.stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(m.in), v);
-        split8<T>(v, m.out + row * ld + col, m.plane, planes);
+__device__ __forceinline__ void load_kept(const void* kept, long plane, long at, int there, bool vec, float g[8], float u[8]) {
+    const char* p = static_cast<const char*>(kept) + at * (long)sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+        load8<float>(reinterpret_cast<const float*>(p), there, vec, g);
+        load8<float>(reinterpret_cast<const float*>(p + plane), there, vec, u);
+    } else {
+        uint32_t q[3][4];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            if (vec) {
+                const uint4 v = *reinterpret_cast<const uint4*>(p + k * plane);
+                q[k][0] = v.x, q[k][1] = v.y, q[k][2] = v.z, q[k][3] = v.w;
+            } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(p + k * plane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[k][j] = (2 * j < there ? h[2 * j] : 0u) | (2 * j + 1 < there ? (uint32_t)h[2 * j + 1] << 16 : 0u);
+            }
+        }
+        // upper half of an element above its byte: bytes (0, below, upper, upper)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            g[2 * j] = __uint_as_float(__byte_perm(q[0][j], q[2][j], 0x1040) & 0xFFFFFF00u);
+            g[2 * j + 1] = __uint_as_float(__byte_perm(q[0][j], q[2][j], 0x3260) & 0xFFFFFF00u);
+            u[2 * j] = __uint_as_float(__byte_perm(q[1][j], q[2][j], 0x1050) & 0xFFFFFF00u);
+            u[2 * j + 1] = __uint_as_float(__byte_perm(q[1][j], q[2][j], 0x3270) & 0xFFFFFF00u);
+        }
     }
 }
 
-// dG and dU from dH, G and U, as operands: planes of (rows, ld), first dG's, then dU's.
+// dG and dU from dH and what is kept, as operands: planes of (rows, ld), first dG's, then dU's.
 template <typename T>
-__global__ void __launch_bounds__(256) grad_kernel(const T* __restrict__ dout, long dout_stride, const T* __restrict__ g, const T* __restrict__ u,
-                                                   long rows, int inner, int ld, int act, int planes, bf16* __restrict__ out) {
-    const int per = ld / 8;
-    const bool vec = inner % 8 == 0 && aligned16_dev(g) && aligned16_dev(u) && aligned16_dev(dout) && dout_stride % (16 / (int)sizeof(T)) == 0;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < rows * per; e += (long)gridDim.x * 256) {
-        const long row = e / per;
-        const int col = (int)(e - row * per) * 8;
-        float d[8], gv[8], uv[8];
-        load8<T>(dout + row * dout_stride + col, inner - col, vec, d);
-        load8<T>(g + row * inner + col, inner - col, vec, gv);
-        load8<T>(u + row * inner + col, inner - col, vec, uv);
+struct Grad {
+    const T* dout;
+    long dout_stride, rows;  // no rows: nothing of it
+    const void* kept;
+    long plane;
+    int inner, ld, act;
+    bf16* out;
+};
+
+// The operands of a launch of products: dG and dU, and whatever has to be packed.
+template <typename T>
+__global__ void __launch_bounds__(256) operand_kernel(const __grid_constant__ Grad<T> d, const __grid_constant__ Packs<T> a, int dim, int ld, int planes) {
+    const int per = ld / 8, dper = d.ld / 8;
+    const long grads = d.rows * dper, total = grads + (a.p[0].rows + a.p[1].rows + a.p[2].rows) * per;
+    const bool vec = d.inner % 8 == 0 && aligned16_dev(d.kept) && aligned16_dev(d.dout) && d.dout_stride % (16 / (int)sizeof(T)) == 0;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
+        if (e < grads) {
+            const long row = e / dper;
+            const int col = (int)(e - row * dper) * 8;
+            float g[8], u[8], o[8];
+            load8<T>(d.dout + row * d.dout_stride + col, d.inner - col, vec, o);
+            load_kept<T>(d.kept, d.plane, row * d.inner + col, d.inner - col, vec, g, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float f, slope;
-            act_grad<sizeof(T) == 4>(gv[j], act, &f, &slope);
-            gv[j] = d[j] * uv[j] * slope;
-            uv[j] = d[j] * f;
+            for (int j = 0; j < 8; ++j) {
+                float f, slope;
+                act_grad<sizeof(T) == 4>(g[j], d.act, &f, &slope);
+                g[j] = o[j] * u[j] * slope;
+                u[j] = o[j] * f;
+            }
+            bf16* at = d.out + row * d.ld + col;
+            split8<T>(g, at, d.rows * d.ld, planes);
+            split8<T>(u, at + planes * d.rows * d.ld, d.rows * d.ld, planes);
+        } else {
+            long row = (e - grads) / per;
+            const int col = (int)(e - grads - row * per) * 8;
+            int k = 0;
+            while (row >= a.p[k].rows) row -= a.p[k++].rows;
+            const Pack<T>& m = a.p[k];
+            float v[8];
+            load8<T>(m.in + row * m.stride + col, dim - col, m.stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(m.in), v);
+            split8<T>(v, m.out + row * ld + col, m.plane, planes);
         }
-        bf16* at = out + row * ld + col;
-        split8<T>(gv, at, rows * ld, planes);
-        split8<T>(uv, at + planes * rows * ld, rows * ld, planes);
     }
 }
 
@@ -454,7 +547,9 @@ struct Few {
     const T *x, *wg, *wu;
     long xs, gs, us;
     int rows, dim, inner, act;
-    T *out, *g, *u;
+    T* out;
+    void* kept;
+    long plane;
 };
 
 // D (16 x 8) += A (16 x 16, rows) B (16 x 8, columns), bfloat16 into float32.
@@ -534,7 +629,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const __grid_consta
 #pragma unroll
         for (int k = 0; k < FEW_WARPS; ++k) g += red[(k * 2 * 16 + f) * COLS + n], u += red[((k * 2 + 1) * 16 + f) * COLS + n];
         const long at = (long)n * a.inner + f0 + f;
-        if (a.g) a.g[at] = from_f<bf16>(g), a.u[at] = from_f<bf16>(u);
+        if (a.kept) keep_one<bf16>(a.kept, a.plane, at, g, u);
         a.out[at] = from_f<bf16>(u * act_of<false>(g, a.act));
     }
 }
@@ -586,7 +681,7 @@ __global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Fe
         if (r >= a.rows || lane >= 2 || f + lane >= a.inner) continue;
         const float g = lane ? acc[1][r] : acc[0][r], u = lane ? acc[3][r] : acc[2][r];
         const long at = (long)r * a.inner + f + lane;
-        if (a.g) a.g[at] = g, a.u[at] = u;
+        if (a.kept) keep_one<float>(a.kept, a.plane, at, g, u);
         a.out[at] = u * act_of<true>(g, a.act);
     }
 }
@@ -620,6 +715,9 @@ int check(const ews_gated_args* a) {
     if (a->rows >= (1l << 30) || a->inner >= (1l << 29) || a->dim >= (1l << 29)) return EWS_ERR_UNSUPPORTED;
     return EWS_OK;
 }
+
+// Bytes from one plane of the kept projections to the next.
+long kept_plane(const ews_gated_args* a) { return up(a->rows * a->inner * (a->dtype == EWS_DTYPE_BF16 ? 2 : 4), 256); }
 
 bool few(const ews_gated_args* a) { return a->rows <= (a->dtype == EWS_DTYPE_BF16 ? kFewBf16 : kFewF32); }
 
@@ -732,9 +830,10 @@ int gemm(const Maps& maps, const Gemm& g, cudaStream_t s) {
 
 const signed char kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
 
-// The three matrices as operands, packed in one launch where they have to be.
+// The three matrices as operands, packed where they have to be, in one launch with the gradients' own.
 template <typename T>
-int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Operand* wu, bool need_x, bool need_w, cudaStream_t s) {
+int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Operand* wu, bool need_x, bool need_w, const Grad<T>& grad,
+             cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     Packs<T> packs{};
     long total = 0;
@@ -752,8 +851,8 @@ int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Op
     make(p.x, a->x, a->x_stride, a->rows, need_x, x);
     make(p.wg, a->w_gate, a->gate_stride, a->inner, need_w, wg);
     make(p.wu, a->w_up, a->up_stride, a->inner, need_w, wu);
-    if (total == 0) return EWS_OK;
-    pack_kernel<T><<<grid_of(total * (p.ldd / 8)), 256, 0, s>>>(packs, (int)a->dim, (int)p.ldd, p.planes);
+    if (total + grad.rows == 0) return EWS_OK;
+    operand_kernel<T><<<grid_of(total * (p.ldd / 8) + grad.rows * (p.ldf / 8)), 256, 0, s>>>(grad, packs, (int)a->dim, (int)p.ldd, p.planes);
     return launched();
 }
 
@@ -772,7 +871,7 @@ int forward_few(const ews_gated_args* a, cudaStream_t s) {
     f.x = static_cast<const T*>(a->x), f.wg = static_cast<const T*>(a->w_gate), f.wu = static_cast<const T*>(a->w_up);
     f.xs = a->x_stride, f.gs = a->gate_stride, f.us = a->up_stride;
     f.rows = (int)a->rows, f.dim = (int)a->dim, f.inner = (int)a->inner, f.act = a->activation;
-    f.out = static_cast<T*>(a->out), f.g = static_cast<T*>(a->gate), f.u = static_cast<T*>(a->up);
+    f.out = static_cast<T*>(a->out), f.kept = a->kept, f.plane = kept_plane(a);
     constexpr int E = 16 / sizeof(T);
     const bool vec = a->dim % E == 0 && f.gs % E == 0 && f.us % E == 0 && (a->rows == 1 || f.xs % E == 0) && aligned16(f.x) &&
                      aligned16(f.wg) && aligned16(f.wu);
@@ -798,7 +897,9 @@ template <typename T>
 int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     if (few(a)) return forward_few<T>(a, s);
     Operand x{}, wg{}, wu{};
-    int rc = operands<T>(a, p, &x, &wg, &wu, true, true, s);
+    Grad<T> none{};
+    none.ld = 8;
+    int rc = operands<T>(a, p, &x, &wg, &wu, true, true, none, s);
     if (rc != EWS_OK) return rc;
     Maps m{};
     if (!make_map(&m.a[0], x, BM) || !make_map(&m.b[0], wg, p.bn / 2) || !make_map(&m.b[1], wu, p.bn / 2)) return EWS_ERR_LAUNCH;
@@ -808,7 +909,7 @@ int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     j.out = a->out, j.pairs = p.planes == 1 ? 1 : 6;
     for (int i = 0; i < j.pairs; ++i) j.ia[i] = p.planes == 1 ? 0 : kPlaneA[i], j.ib[i] = p.planes == 1 ? 0 : kPlaneB[i];
     g.run = p.planes > 1 ? kRun : 1 << 28;
-    g.act = a->activation, g.g = a->gate, g.u = a->up, g.status = a->status;
+    g.act = a->activation, g.kept = a->kept, g.plane = kept_plane(a), g.status = a->status;
     if constexpr (sizeof(T) == 4) {
         return gemm<T, FWD, 128>(m, g, s);
     } else {
@@ -822,13 +923,10 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     Operand x{}, wg{}, wu{}, d{};
     const bool dw = a->dw_gate || a->dw_up;
-    int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, s);
-    if (rc != EWS_OK) return rc;
     bf16* dgu = reinterpret_cast<bf16*>(w + p.dgu);
-    grad_kernel<T><<<grid_of(a->rows * (p.ldf / 8)), 256, 0, s>>>(static_cast<const T*>(a->dout), a->dout_stride, static_cast<const T*>(a->gate),
-                                                               static_cast<const T*>(a->up), a->rows, (int)a->inner, (int)p.ldf, a->activation,
-                                                               p.planes, dgu);
-    if ((rc = launched()) != EWS_OK) return rc;
+    const Grad<T> grad{static_cast<const T*>(a->dout), (long)a->dout_stride, a->rows, a->kept, kept_plane(a), (int)a->inner, (int)p.ldf, a->activation, dgu};
+    int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, grad, s);
+    if (rc != EWS_OK) return rc;
     d.p = dgu, d.rows = a->rows, d.cols = d.ld = p.ldf, d.plane = a->rows * p.ldf, d.planes = 2 * p.planes;
     Maps m{};
     if (!make_map(&m.a[0], d, BM) || !make_map(&m.a[1], d, 64)) return EWS_ERR_LAUNCH;
@@ -847,8 +945,8 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
         Job& j = g.job[k];
         j = k ? job_of(a->inner, a->dim, a->rows, p.bn, p.splits[k]) : job_of(a->rows, a->dim, a->inner, p.bn, p.splits[k]);
         j.out = out[k];
-        for (int side = 0; side < (k ? 1 : 2); ++side)
-            for (int i = 0; i < products; ++i) {
+        for (int i = 0; i < products; ++i)  // the smallest of both sides first
+            for (int side = 0; side < (k ? 1 : 2); ++side) {
                 const int which = k ? k - 1 : side;  // dG or dU
                 j.ia[j.pairs] = (signed char)(which * p.planes + (products == 1 ? 0 : kPlaneA[i]));
                 j.ib[j.pairs] = products == 1 ? 0 : kPlaneB[i];
@@ -882,11 +980,15 @@ extern "C" size_t ews_gated_work_size(const ews_gated_args* a, int backward_pass
     return check(a) == EWS_OK && a->rows > 0 ? plan(a, backward_pass != 0).bytes : 0;
 }
 
+extern "C" size_t ews_gated_kept_size(const ews_gated_args* a) {
+    return check(a) == EWS_OK ? (size_t)kept_plane(a) * (a->dtype == EWS_DTYPE_BF16 ? 3 : 2) : 0;
+}
+
 extern "C" int ews_gated_fwd(const ews_gated_args* a, ews_stream_t stream) {
     const int rc = check(a);
     if (rc != EWS_OK) return rc;
     if (a->rows == 0) return EWS_OK;
-    if (!a->x || !a->w_gate || !a->w_up || !a->out || !a->gate != !a->up) return EWS_ERR_INVALID_ARGUMENT;
+    if (!a->x || !a->w_gate || !a->w_up || !a->out) return EWS_ERR_INVALID_ARGUMENT;
     const Plan p = plan(a, false);
     if (p.bytes && (!a->work || !ews::token::aligned16(a->work) || a->work_bytes < p.bytes)) return EWS_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
@@ -904,7 +1006,7 @@ extern "C" int ews_gated_bwd(const ews_gated_args* a, ews_stream_t stream) {
         return EWS_OK;
     }
     if (!a->dx && !a->dw_gate && !a->dw_up) return EWS_OK;
-    if (!a->x || !a->w_gate || !a->w_up || !a->dout || !a->gate || !a->up || a->dout_stride < a->inner) return EWS_ERR_INVALID_ARGUMENT;
+    if (!a->x || !a->w_gate || !a->w_up || !a->dout || !a->kept || a->dout_stride < a->inner) return EWS_ERR_INVALID_ARGUMENT;
     const Plan p = plan(a, true);
     if (p.bytes && (!a->work || !ews::token::aligned16(a->work) || a->work_bytes < p.bytes)) return EWS_ERR_WORKSPACE;
     return a->dtype == EWS_DTYPE_BF16 ? backward<ews::token::bf16>(a, p, s) : backward<float>(a, p, s);

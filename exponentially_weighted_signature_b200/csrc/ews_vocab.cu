@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                             while (next < end) {
                                 float z = 0.f;
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) z = next - c == j ? v[j] : z;
+                                for (int j = 0; j < 32; ++j) z += next - c == j ? v[j] : 0.f;  // a sum: selects became a copy of v in local memory
                                 a.logit[entry0 + entry] = z;
                                 step_entry();
                             }

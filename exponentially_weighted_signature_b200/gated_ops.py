@@ -16,13 +16,13 @@ from .engine import first_order
 from .token_ops import _DTYPES, _addr, _device, _dtype, _launch, _row_stride, _rows, _work
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
-_GATED = struct.Struct("@3q2i3P3q4Pq4PNP").pack  # ews_gated_args
+_GATED = struct.Struct("@3q2i3P3q3Pq4PNP").pack  # ews_gated_args
 
 
-def _args(x, wg, wu, act, out=None, gate=None, up=None, dout=None, grads=(None, None, None), work=None):
+def _args(x, wg, wu, act, out=None, kept=None, dout=None, grads=(None, None, None), work=None):
     (rows, dim), inner = x.shape, wg.shape[0]
     return _GATED(rows, dim, inner, _DTYPES[x.dtype], act, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _row_stride(x),
-                  _row_stride(wg), _row_stride(wu), _addr(out), _addr(gate), _addr(up), _addr(dout),
+                  _row_stride(wg), _row_stride(wu), _addr(out), _addr(kept), _addr(dout),
                   0 if dout is None else _row_stride(dout), *map(_addr, grads), _addr(work), 0 if work is None else work.numel(),
                   engine.index_word(x.get_device())[0])
 
@@ -30,8 +30,13 @@ def _args(x, wg, wu, act, out=None, gate=None, up=None, dout=None, grads=(None, 
 @functools.lru_cache(maxsize=256)
 def _size(rows, dim, inner, code, strides, at, wanted, backward):
     """Workspace bytes: a function of the sizes, the strides, the addresses modulo 16 and the gradients asked for."""
-    args = _GATED(rows, dim, inner, code, 0, *at, *strides, 0, 0, 0, 0, inner, *wanted, 0, 0, 0)
+    args = _GATED(rows, dim, inner, code, 0, *at, *strides, 0, 0, 0, inner, *wanted, 0, 0, 0)
     return _lib.load().ews_gated_work_size(args, backward)
+
+
+@functools.lru_cache(maxsize=256)
+def _kept_size(rows, dim, inner, code):
+    return _lib.load().ews_gated_kept_size(_GATED(rows, dim, inner, code, 0, 0, 0, 0, dim, dim, dim, *([0] * 10)))
 
 
 def _workspace(x, wg, wu, wanted, backward):
@@ -44,31 +49,31 @@ def _forward(x, wg, wu, act, shape, keep):
     lib = _lib.load()
     rows, inner = x.shape[0], wg.shape[0]
     out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    gate, up = (torch.empty((rows, inner), dtype=x.dtype, device=x.device) if keep else None for _ in range(2))
+    kept = _work(_kept_size(rows, x.shape[1], inner, _DTYPES[x.dtype]), x) if keep else None
     work = _workspace(x, wg, wu, (0, 0, 0), 0)
-    _launch(x.get_device(), "ews_gated_fwd", rows, lib.ews_gated_fwd, _args(x, wg, wu, act, out, gate, up, work=work))
-    return out, gate, up
+    _launch(x.get_device(), "ews_gated_fwd", rows, lib.ews_gated_fwd, _args(x, wg, wu, act, out, kept, work=work))
+    return out, kept
 
 
 class _Gated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, act, shape):
         x, wg, wu = _rows(x), _rows(wg), _rows(wu)
-        out, gate, up = _forward(x, wg, wu, act, shape, True)
+        out, kept = _forward(x, wg, wu, act, shape, True)
         ctx.act = act
-        ctx.save_for_backward(x, wg, wu, gate, up)
+        ctx.save_for_backward(x, wg, wu, kept)
         return out
 
     @staticmethod
     @first_order
     def backward(ctx, dout):
-        x, wg, wu, gate, up = ctx.saved_tensors
+        x, wg, wu, kept = ctx.saved_tensors
         lib = _lib.load()
-        dout = _rows(dout.reshape(gate.shape))
+        dout = _rows(dout.reshape(x.shape[0], wg.shape[0]))
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
                  for t, need in zip((x, wg, wu), ctx.needs_input_grad)]
         work = _workspace(x, wg, wu, tuple(int(g is not None) for g in grads), 1)
-        args = _args(x, wg, wu, ctx.act, None, gate, up, dout, grads, work)
+        args = _args(x, wg, wu, ctx.act, None, kept, dout, grads, work)
         _launch(x.get_device(), "ews_gated_bwd", x.shape[0], lib.ews_gated_bwd, args)
         return (*grads, None, None)
 
@@ -78,7 +83,7 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
 
     x (..., D); gate_weight and up_weight (F, D), all float32 or all bfloat16 (rows of any stride). activation: "silu",
     ``g sigmoid(g)``, or "gelu", ``g Phi(g)``. Returns (..., F). Sums are float32; the product is formed from them and rounded
-    once. Differentiable in x and both weights (the two projections, rounded to the inputs' type, are kept for it)."""
+    once. Differentiable in x and both weights (the two projections are kept for it, 6 bytes a pair for bfloat16, 8 for float32)."""
     if gate_weight.dim() != 2 or up_weight.shape != gate_weight.shape or 0 in gate_weight.shape:
         raise ValueError(f"gate_weight and up_weight must be (F, D) with F, D > 0, got {tuple(gate_weight.shape)} and {tuple(up_weight.shape)}")
     if x.dim() < 1 or x.shape[-1] != gate_weight.shape[1]:

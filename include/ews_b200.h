@@ -429,8 +429,8 @@ int ews_recur_step(const ews_recur_args* args, const int* slots, int pool, float
 /* ---- gated linear layer ---------------------------------------------------------------------------
  * out = act(x w_gate^T) * (x w_up^T) for x (rows, dim), w_gate and w_up (inner, dim) of `dtype` (rows `x_stride`, `gate_stride`,
  * `up_stride` elements apart), out (rows, inner) contiguous; activation EWS_ACT_SILU, g sigmoid(g), or EWS_ACT_GELU, g Phi(g).
- * gate and up (rows, inner; both or neither): the two projections, for the backward.
- *   ews_gated_bwd: from dout (rows, inner; rows `dout_stride` apart), gate and up the gradients dx (rows, dim), dw_gate and dw_up
+ * kept: ews_gated_kept_size(args) bytes, the two projections for the backward, or NULL.
+ *   ews_gated_bwd: from dout (rows, inner; rows `dout_stride` apart) and kept the gradients dx (rows, dim), dw_gate and dw_up
  *   (inner, dim), contiguous; any may be NULL.
  * status as above. `work`: ews_gated_work_size(args, backward) bytes; the size also depends on which of dx, dw_gate and dw_up
  * are asked for, and on the matrices' strides and on their addresses modulo 16. */
@@ -441,7 +441,7 @@ typedef struct {
     int dtype, activation;
     const void *x, *w_gate, *w_up;
     int64_t x_stride, gate_stride, up_stride;
-    void *out, *gate, *up;
+    void *out, *kept;
     const void* dout;
     int64_t dout_stride;
     void *dx, *dw_gate, *dw_up;
@@ -449,6 +449,7 @@ typedef struct {
     size_t work_bytes;
     int* status;
 } ews_gated_args;
+size_t ews_gated_kept_size(const ews_gated_args* args);
 size_t ews_gated_work_size(const ews_gated_args* args, int backward);
 int ews_gated_fwd(const ews_gated_args* args, ews_stream_t stream);
 int ews_gated_bwd(const ews_gated_args* args, ews_stream_t stream);

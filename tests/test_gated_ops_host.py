@@ -15,8 +15,8 @@ def _recur(batch=2, steps=300, channels=64, dtype=1, x=16, rate=16, out=16, dx=1
     return recur_ops._RECUR(batch, steps, channels, dtype, x, 16, 16, *([0] * 6), rate, 0, 0, out, 0, carry, 16, 0, 0, 0, dx, 16, 16, 0, 0, 0, 0, 0)
 
 
-def _gated(rows=200, dim=64, inner=128, dtype=1, act=0, xs=64, gs=64, us=64, x=16, gate=16, up=16, dout_stride=128, dx=16):
-    return gated_ops._GATED(rows, dim, inner, dtype, act, x, 16, 16, xs, gs, us, 16, gate, up, 16, dout_stride, dx, 16, 16, 0, 0, 0)
+def _gated(rows=200, dim=64, inner=128, dtype=1, act=0, xs=64, gs=64, us=64, x=16, kept=16, dout_stride=128, dx=16):
+    return gated_ops._GATED(rows, dim, inner, dtype, act, x, 16, 16, xs, gs, us, 16, kept, 16, dout_stride, dx, 16, 16, 0, 0, 0)
 
 
 def _distill(rows=10, vocab=100, dim=16, dtype=1, hs=16, ws=16, top=4, logits_dtype=0, inv_tau=1.0, ids=16, entries=16):
@@ -58,8 +58,8 @@ def test_gated_arguments_are_checked_before_the_device():
         assert lib.ews_gated_work_size(_gated(**bad), 1) == 0
         assert lib.ews_gated_fwd(_gated(**bad), None) == code and lib.ews_gated_bwd(_gated(**bad), None) == code, bad
     assert lib.ews_gated_fwd(_gated(x=0), None) == 1
-    assert lib.ews_gated_fwd(_gated(gate=0), None) == 1  # both projections or neither
-    assert lib.ews_gated_bwd(_gated(gate=0, up=0), None) == 1 and lib.ews_gated_bwd(_gated(dout_stride=100), None) == 1
+    assert lib.ews_gated_kept_size(_gated()) == gated_ops._kept_size(200, 64, 128, 1) == 3 * 2 * 200 * 128
+    assert lib.ews_gated_bwd(_gated(kept=0), None) == 1 and lib.ews_gated_bwd(_gated(dout_stride=100), None) == 1
     assert lib.ews_gated_bwd(_gated(), None) == 3
     assert lib.ews_gated_fwd(_gated(dtype=0), None) == 3  # float32 is packed in planes
     assert lib.ews_gated_fwd(_gated(rows=0), None) == 0

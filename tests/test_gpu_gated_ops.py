@@ -2,7 +2,7 @@
 
 Tolerances are bounds, element by element, from the arithmetic, with u half a step of the type (bfloat16 2^-8, float32 2^-24)
 and s = 2e-5 (products exact to 2^-21, chains of some hundred truncated additions of 2^-23 each) of the sum over absolute values:
-a projection is off by s |X| |W|, and kept for the backward by u of itself more. Through the product and the activation, whose slope
+a projection is off by s |X| |W|, and as it is kept for the backward by 2^-15 of itself more (24 bits, cut off). Through the product and the activation, whose slope
 is at most 1.13 and whose second derivative at most 0.8, that gives the bound of H, dG and dU; dG and dU are rounded once more as
 operands (float32: three planes, 2^-24). The activation itself costs 2^-20."""
 
@@ -42,7 +42,7 @@ def reference(x, wg, wu, dh, kind):
     act, slope = act_of(g, kind)
     h = act * up
     eh = 1.13 * eg * (up.abs() + eu) + act.abs() * eu + 2.0**-20 * h.abs() + u * h.abs()
-    eg, eu = eg + u * g.abs(), eu + u * up.abs()
+    eg, eu = eg + 2.0**-15 * g.abs(), eu + 2.0**-15 * up.abs()
     dg, du = dh * up * slope, dh * act
     edg = dh.abs() * (eu * (slope.abs() + 0.8 * eg) + up.abs() * (0.8 * eg + 2.0**-20)) + u * dg.abs()
     edu = dh.abs() * (1.13 * eg + 2.0**-20 * act.abs()) + u * du.abs()
