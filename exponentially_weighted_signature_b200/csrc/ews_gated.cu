@@ -17,8 +17,8 @@
 // of planes that matter (2^-24), smallest first; every 128 of K the sum leaves the tensor core's accumulator, which truncates at
 // every addition, and is added in registers.
 //
-// Few rows (a served batch's tokens) are bound by the weights' bytes: few_kernel gives each CTA 16 rows of both weights, its warps
-// shares of K, and multiplies with mma.sync as the bytes arrive, the rows of X as the narrow side.
+// Few rows (a served batch's tokens) are bound by the weights' bytes: served_kernel takes the weights as the wide operand, 64 rows
+// of both a CTA, and keeps as many of their bytes in flight as fit; few_f32_kernel reads float32 weights as they are, once.
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -32,7 +32,9 @@ constexpr int EPW = 8;              // epilogue warps
 constexpr int NTH = 64 + EPW * 32;  // and one each for TMA and MMA
 constexpr int SMS = 148;
 constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulator
-constexpr int kFewBf16 = 64, kFewF32 = 16;  // rows up to which few_kernel / few_f32_kernel run
+// Rows up to which served_kernel runs (100 rows, 4,096 x 1,024: 22 us there, 14 as tiles; 64 rows, 5,632 x 2,048: 21 us), and up to
+// which few_f32_kernel does.
+constexpr int kServed = 64, kFewF32 = 16;
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
 
@@ -542,102 +544,19 @@ __global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Red
 
 // ---- few rows -------------------------------------------------------------------------------------------------
 
-template <typename T>
 struct Few {
-    const T *x, *wg, *wu;
+    const float *x, *wg, *wu;
     long xs, gs, us;
     int rows, dim, inner, act;
-    T* out;
+    float* out;
     void* kept;
     long plane;
 };
 
-// D (16 x 8) += A (16 x 16, rows) B (16 x 8, columns), bfloat16 into float32.
-__device__ __forceinline__ void mma_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-constexpr int FEW_WARPS = 8;
-
-// 16 rows of each weight a CTA; a warp takes every eighth block of 32 of K. The order of K within a block is the operands' own
-// choice, so a lane takes eight consecutive elements of a row, one 16-byte load, as the four words that two products want of it
-// (the same of X's rows). 8 NT rows of X.
-template <int NT, bool VEC>
-__global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const __grid_constant__ Few<bf16> a) {
-    extern __shared__ float red[];  // (warps, 2, 16, 8 NT)
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 2, quad = lane & 3;
-    const int f0 = blockIdx.x * 16;
-    float acc[2][NT][4];
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[w][n][e] = 0.f;
-    auto load = [&](const bf16* base, long stride, int row, int rows, int k) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row >= rows || k >= a.dim) return v;
-        const bf16* p = base + row * stride + k;
-        if (VEC) return __ldg(reinterpret_cast<const uint4*>(p));
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float lo = k + 2 * j < a.dim ? to_f(p[2 * j]) : 0.f, hi = k + 2 * j + 1 < a.dim ? to_f(p[2 * j + 1]) : 0.f;
-            w[j] = pack_bf16(lo, hi);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    };
-    const int blocks = (a.dim + 31) / 32;
-    constexpr int U = NT <= 2 ? 4 : 2;  // blocks in flight
-    for (int b0 = warp; b0 < blocks; b0 += FEW_WARPS * U) {
-        uint4 wv[U][4], xv[U][NT];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int k = (b0 + i * FEW_WARPS) * 32 + quad * 8;  // beyond the last block: zeros
-            wv[i][0] = load(a.wg, a.gs, f0 + grp, a.inner, k), wv[i][1] = load(a.wg, a.gs, f0 + grp + 8, a.inner, k);
-            wv[i][2] = load(a.wu, a.us, f0 + grp, a.inner, k), wv[i][3] = load(a.wu, a.us, f0 + grp + 8, a.inner, k);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) xv[i][n] = load(a.x, a.xs, n * 8 + grp, a.rows, k);
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint4 lo = wv[i][2 * w], hi = wv[i][2 * w + 1], x = xv[i][n];
-                    mma_16816(acc[w][n], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-                    mma_16816(acc[w][n], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
-                }
-    }
-    constexpr int COLS = 8 * NT;
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float* p = red + ((warp * 2 + w) * 16 + grp) * COLS + n * 8 + quad * 2;
-            p[0] = acc[w][n][0], p[1] = acc[w][n][1];
-            p[8 * COLS] = acc[w][n][2], p[8 * COLS + 1] = acc[w][n][3];
-        }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * COLS; e += FEW_WARPS * 32) {
-        const int f = e & 15, n = e >> 4;
-        if (f0 + f >= a.inner || n >= a.rows) continue;
-        float g = 0.f, u = 0.f;
-#pragma unroll
-        for (int k = 0; k < FEW_WARPS; ++k) g += red[(k * 2 * 16 + f) * COLS + n], u += red[((k * 2 + 1) * 16 + f) * COLS + n];
-        const long at = (long)n * a.inner + f0 + f;
-        if (a.kept) keep_one<bf16>(a.kept, a.plane, at, g, u);
-        a.out[at] = from_f<bf16>(u * act_of<false>(g, a.act));
-    }
-}
-
 // float32: a warp has two rows of each weight and runs along K, its lanes on consecutive fours of it (however they are
 // loaded: the sums' order does not depend on the alignment), for R rows of X.
 template <int R, bool VEC>
-__global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Few<float> a) {
+__global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Few a) {
     constexpr int W = 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int f = (blockIdx.x * 4 + warp) * 2;
@@ -686,6 +605,131 @@ __global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Fe
     }
 }
 
+// Up to 64 rows: the weights as the wide operand, 64 rows of Wg above the same of Wu a CTA (their partners in lanes 64
+// apart), the rows of X as the narrow one (BN of them). One tile a CTA, whatever K; what counts is how many bytes of the
+// weights are in flight: eight stages of 16 KB and X's rows where one CTA an SM is enough, four where there are more tiles.
+struct Served {
+    int rows, inner, act, blocks, stages;  // k blocks of 64
+    bf16* out;
+    void* kept;
+    long plane;
+    int* status;
+};
+constexpr int SERVED_T = 192;  // a warp for TMA, one for MMA, four for the epilogue
+
+template <int BN>
+__global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensorMap mu,
+                                                          const __grid_constant__ CUtensorMap mx, const __grid_constant__ Served a) {
+    constexpr int A = BM * BK * 2, STAGE = A + BN * BK * 2, COLS = BN < 32 ? 32 : BN;
+    extern __shared__ unsigned char raw[];
+    unsigned char* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + a.stages * STAGE);
+    uint64_t* empty = full + a.stages;
+    uint64_t* done = empty + a.stages;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < a.stages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+        mbar_init(done, 1);
+        *fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "r"(COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
+    const int f0 = blockIdx.x * 64;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, kb = 0;
+            uint32_t ph = 1;
+            for (; kb < a.blocks; ++kb) {
+                if (!(ok = mbar_wait(empty + s, ph, fail))) break;
+                unsigned char* at = tiles + s * STAGE;
+                mbar_expect(full + s, STAGE);
+                tma_load(&mg, full + s, at, kb * BK, f0, 0);
+                tma_load(&mu, full + s, at + A / 2, kb * BK, f0, 0);
+                tma_load(&mx, full + s, at + A, kb * BK, 0, 0);
+                if (++s == a.stages) s = 0, ph ^= 1u;
+            }
+            if (!ok)
+                for (int j = kb > a.stages ? kb - a.stages : 0; j < kb; ++j) mbar_drain(full + j % a.stages, (uint32_t)((j / a.stages) & 1));
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+        const uint64_t ad0 = desc(smem_u32(tiles), false), bd0 = desc(smem_u32(tiles) + A, false);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int kb = 0; kb < a.blocks; ++kb) {
+            if (!(ok = warp_wait(full + s, ph, fail))) break;
+            fence_after();
+            if (elect_one()) {
+                const uint64_t ad = ad0 + s * (STAGE >> 4), bd = bd0 + s * (STAGE >> 4);
+#pragma unroll
+                for (int q = 0; q < BK / 16; ++q) mma_bf16(tmem, ad + q * (32 >> 4), bd + q * (32 >> 4), idesc, kb > 0 || q > 0);
+                mma_commit(empty + s);
+                if (kb == a.blocks - 1) mma_commit(done);
+            }
+            __syncwarp();
+            if (++s == a.stages) s = 0, ph ^= 1u;
+        }
+        if (!ok) {  // what was issued has to end before the memory goes
+            if (elect_one()) mma_commit(done);
+            __syncwarp();
+            mbar_drain(done, 0);
+        }
+    }
+    float v[BN < 32 ? 1 : BN / 32][32];
+    const int quarter = warp & 3, half = quarter >> 1, ch = (quarter & 1) * 32 + lane;
+    float* swap = reinterpret_cast<float*>(tiles);  // (2, BN / 2, 64): U of the first rows, G of the others
+    constexpr int HALF = BN / 2;
+    if (warp >= 2) {
+        ok = __all_sync(kFull, mbar_wait(done, 0, fail)) && !*fail;
+        fence_after();
+        if (ok) {
+            const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+            for (int c = 0; c < COLS / 32; ++c) tmem_ld32(src + c * 32, v[c]);
+            // each side gives the other half of its rows away
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) {
+                const float give = half ? v[j / 32][j % 32] : v[(j + HALF) / 32][(j + HALF) % 32];
+                swap[(half ? 0 : HALF * 64) + j * 64 + ch] = give;
+            }
+        }
+    }
+    __syncthreads();
+    if (warp >= 2 && ok) {
+        const int f = f0 + ch;
+        if (f < a.inner) {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) {
+                const int row = half ? j + HALF : j;
+                if (row < a.rows) {
+                    const float got = swap[(half ? HALF * 64 : 0) + j * 64 + ch];
+                    const float own = half ? v[(j + HALF) / 32][(j + HALF) % 32] : v[j / 32][j % 32];
+                    const float g = half ? got : own, u = half ? own : got;
+                    const long at = (long)row * a.inner + f;
+                    if (a.kept) keep_one<bf16>(a.kept, a.plane, at, g, u);
+                    a.out[at] = from_f<bf16>(u * act_of<false>(g, a.act));
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (threadIdx.x == 0 && *fail) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------
 
 // (planes, rows, cols) bfloat16 with rows `ld` apart.
@@ -719,7 +763,12 @@ int check(const ews_gated_args* a) {
 // Bytes from one plane of the kept projections to the next.
 long kept_plane(const ews_gated_args* a) { return up(a->rows * a->inner * (a->dtype == EWS_DTYPE_BF16 ? 2 : 4), 256); }
 
-bool few(const ews_gated_args* a) { return a->rows <= (a->dtype == EWS_DTYPE_BF16 ? kFewBf16 : kFewF32); }
+// How the forward runs: as many rows as make the tensor core's tiles, or few of them.
+enum Path { TILES, SERVED, FEW };
+Path path_of(const ews_gated_args* a) {
+    if (a->dtype == EWS_DTYPE_F32) return a->rows <= kFewF32 ? FEW : TILES;
+    return a->rows <= kServed ? SERVED : TILES;
+}
 
 // A matrix of (rows, dim) as an operand: as it lies where TMA can read it, else packed at `at` of the workspace.
 struct Source {
@@ -783,7 +832,7 @@ Plan plan(const ews_gated_args* a, bool bwd) {
     Plan p{};
     p.planes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
     p.ldd = up(a->dim, 8), p.ldf = up(a->inner, 8);
-    if (!bwd && few(a)) return p;
+    if (!bwd && path_of(a) == FEW) return p;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -856,51 +905,53 @@ int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Op
     return launched();
 }
 
-template <int NT, bool VEC>
-int run_few(const Few<bf16>& f, cudaStream_t s) {
-    auto* kern = few_kernel<NT, VEC>;
-    constexpr int bytes = FEW_WARPS * 2 * 16 * 8 * NT * 4;
-    if (bytes > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
-    kern<<<(unsigned)((f.inner + 15) / 16), FEW_WARPS * 32, bytes, s>>>(f);
+int forward_few(const ews_gated_args* a, cudaStream_t s) {
+    Few f{};
+    f.x = static_cast<const float*>(a->x), f.wg = static_cast<const float*>(a->w_gate), f.wu = static_cast<const float*>(a->w_up);
+    f.xs = a->x_stride, f.gs = a->gate_stride, f.us = a->up_stride;
+    f.rows = (int)a->rows, f.dim = (int)a->dim, f.inner = (int)a->inner, f.act = a->activation;
+    f.out = static_cast<float*>(a->out), f.kept = a->kept, f.plane = kept_plane(a);
+    const bool vec = a->dim % 4 == 0 && f.gs % 4 == 0 && f.us % 4 == 0 && (a->rows == 1 || f.xs % 4 == 0) && aligned16(f.x) &&
+                     aligned16(f.wg) && aligned16(f.wu);
+    const unsigned grid = (unsigned)((f.inner + 7) / 8);
+    auto go = [&](auto* kern) {
+        kern<<<grid, 128, 0, s>>>(f);
+        return launched();
+    };
+    if (f.rows <= 1) return vec ? go(few_f32_kernel<1, true>) : go(few_f32_kernel<1, false>);
+    if (f.rows <= 4) return vec ? go(few_f32_kernel<4, true>) : go(few_f32_kernel<4, false>);
+    return vec ? go(few_f32_kernel<16, true>) : go(few_f32_kernel<16, false>);
+}
+
+template <int BN>
+int run_served(const ews_gated_args* a, const Operand& x, const Operand& wg, const Operand& wu, cudaStream_t s) {
+    CUtensorMap mx, mg, mu;
+    if (!make_map(&mx, x, BN) || !make_map(&mg, wg, 64) || !make_map(&mu, wu, 64)) return EWS_ERR_LAUNCH;
+    const unsigned grid = (unsigned)((a->inner + 63) / 64);
+    const Served v{(int)a->rows, (int)a->inner, a->activation, (int)((a->dim + BK - 1) / BK), grid <= SMS ? 8 : 4,
+                   static_cast<bf16*>(a->out), a->kept, kept_plane(a), a->status};
+    constexpr int stage = BM * BK * 2 + BN * BK * 2, rest = 1024 + 256;
+    auto* kern = served_kernel<BN>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * stage + rest) != cudaSuccess) return EWS_ERR_LAUNCH;
+    kern<<<grid, SERVED_T, v.stages * stage + rest, s>>>(mg, mu, mx, v);
     return launched();
 }
 
 template <typename T>
-int forward_few(const ews_gated_args* a, cudaStream_t s) {
-    Few<T> f{};
-    f.x = static_cast<const T*>(a->x), f.wg = static_cast<const T*>(a->w_gate), f.wu = static_cast<const T*>(a->w_up);
-    f.xs = a->x_stride, f.gs = a->gate_stride, f.us = a->up_stride;
-    f.rows = (int)a->rows, f.dim = (int)a->dim, f.inner = (int)a->inner, f.act = a->activation;
-    f.out = static_cast<T*>(a->out), f.kept = a->kept, f.plane = kept_plane(a);
-    constexpr int E = 16 / sizeof(T);
-    const bool vec = a->dim % E == 0 && f.gs % E == 0 && f.us % E == 0 && (a->rows == 1 || f.xs % E == 0) && aligned16(f.x) &&
-                     aligned16(f.wg) && aligned16(f.wu);
-    if constexpr (sizeof(T) == 2) {
-        const int nt = (f.rows + 7) / 8;
-        if (nt <= 1) return vec ? run_few<1, true>(f, s) : run_few<1, false>(f, s);
-        if (nt <= 2) return vec ? run_few<2, true>(f, s) : run_few<2, false>(f, s);
-        if (nt <= 4) return vec ? run_few<4, true>(f, s) : run_few<4, false>(f, s);
-        return vec ? run_few<8, true>(f, s) : run_few<8, false>(f, s);
-    } else {
-        const unsigned grid = (unsigned)((f.inner + 7) / 8);
-        auto go = [&](auto* kern) {
-            kern<<<grid, 128, 0, s>>>(f);
-            return launched();
-        };
-        if (f.rows <= 1) return vec ? go(few_f32_kernel<1, true>) : go(few_f32_kernel<1, false>);
-        if (f.rows <= 4) return vec ? go(few_f32_kernel<4, true>) : go(few_f32_kernel<4, false>);
-        return vec ? go(few_f32_kernel<16, true>) : go(few_f32_kernel<16, false>);
-    }
-}
-
-template <typename T>
 int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
-    if (few(a)) return forward_few<T>(a, s);
+    const Path path = path_of(a);
+    if (path == FEW) return forward_few(a, s);
     Operand x{}, wg{}, wu{};
     Grad<T> none{};
     none.ld = 8;
     int rc = operands<T>(a, p, &x, &wg, &wu, true, true, none, s);
     if (rc != EWS_OK) return rc;
+    if constexpr (sizeof(T) == 2) {
+        if (path == SERVED) {
+            if (a->rows <= 16) return run_served<16>(a, x, wg, wu, s);
+            return a->rows <= 32 ? run_served<32>(a, x, wg, wu, s) : run_served<64>(a, x, wg, wu, s);
+        }
+    }
     Maps m{};
     if (!make_map(&m.a[0], x, BM) || !make_map(&m.b[0], wg, p.bn / 2) || !make_map(&m.b[1], wu, p.bn / 2)) return EWS_ERR_LAUNCH;
     Gemm g{};
