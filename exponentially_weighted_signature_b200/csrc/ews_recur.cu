@@ -30,10 +30,13 @@ using tc5::mul2;
 using tc5::pair;
 using tc5::unpair;
 
-constexpr int kMaxWarps = 16;
-constexpr int FL = 16, FW = 8, FCTAS = 2;  // forward: tokens a warp, warps a tile, CTAs an SM
-constexpr int BL = 8, BW = 8, BCTAS = 2;   // backward
-constexpr int FT = FL * FW, BT = BL * BW;
+constexpr int kMaxWarps = 16, SMS = 148;
+constexpr int TILE = 64;                  // tokens a tile
+constexpr int FL = 8, FW = TILE / FL, FCTAS = 3;  // forward: tokens a warp, warps a tile, CTAs an SM
+constexpr int BL = 8, BW = TILE / BL, BCTAS = 2;  // backward
+constexpr int PL = 8, PW = TILE / PL, PCTAS = 3;  // the same where TMA brings the tiles
+constexpr int QL = 8, QW = TILE / QL, QCTAS = 2;
+constexpr int kPipedFrom = 33;            // steps from which it does: below, most of a tile would be empty
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
@@ -46,19 +49,19 @@ template <typename T>
 struct Params {
     int batch, steps, channels;
     int tiles, blocks;  // along the steps and the channels
+    long total;         // tiles in all
     Stream<T> x, decay, gate, dout;
     const float* rate;
     const int* lengths;
     const float *initial, *dfinal;
     T* out;
     float* final_state;
-    float* carry;  // (batch, tiles of the backward, channels): the state in front of each of its tiles
+    float* carry;  // (batch, tiles, channels): the state in front of each tile, for the backward
     T *dx, *ddecay, *dgate;
     float *drate_part, *dinitial;
     // look-back
     DeviceStatus* st;
-    int* flags;    // (batch, blocks, tiles)
-    float *map_a, *map_h, *ends;  // (batch, tiles, channels)
+    uint2* slots;  // (batch, tiles, 2, channels): a value and what it is, see publish
     int* status;
 };
 
@@ -121,6 +124,7 @@ struct Word<float, 1> {
     __device__ __forceinline__ void load(const float* p) { w = __ldg(p); }
     __device__ __forceinline__ void fill(float x) { w = x; }
     __device__ __forceinline__ F<1> get() const { return F<1>(w); }
+    __device__ __forceinline__ void put(F<1> v) { w = v.r; }
     __device__ static __forceinline__ void store(float* p, F<1> v) { *p = v.r; }
 };
 template <>
@@ -137,6 +141,7 @@ struct Word<bf16, 2> {
     __device__ __forceinline__ void load(const bf16* p) { w = __ldg(reinterpret_cast<const uint32_t*>(p)); }
     __device__ __forceinline__ void fill(float x) { w = pack_bf16(x, x); }
     __device__ __forceinline__ F<2> get() const { return F<2>(bf16_lo(w), bf16_hi(w)); }
+    __device__ __forceinline__ void put(F<2> v) { w = pack_bf16(v.get(0), v.get(1)); }
     __device__ static __forceinline__ void store(bf16* p, F<2> v) { *reinterpret_cast<uint32_t*>(p) = pack_bf16(v.get(0), v.get(1)); }
 };
 
@@ -210,28 +215,25 @@ __device__ __forceinline__ float rate_at(const float* p) {
 
 struct Tile {
     int b, tt, c0;  // sample, tile along the steps, first channel
-    int slot;       // of the flags
 };
 
 // Tiles are given out by the steps first, so that a tile only waits on lower tickets.
 template <typename T>
-__device__ __forceinline__ Tile tile_of(const Params<T>& a, long ticket, bool down, int width) {
-    const long per = (long)a.batch * a.blocks;
+__device__ __forceinline__ Tile tile_of(const Params<T>& a, int ticket, bool down, int width) {
+    const unsigned per = (unsigned)(a.batch * a.blocks);
     Tile t;
-    t.tt = (int)(ticket / per);
-    const int rest = (int)(ticket - t.tt * per);
+    t.tt = (int)((unsigned)ticket / per);
+    const unsigned rest = (unsigned)ticket - t.tt * per;
     if (down) t.tt = a.tiles - 1 - t.tt;
-    t.b = rest / a.blocks;
-    const int cb = rest - t.b * a.blocks;
-    t.c0 = cb * width;
-    t.slot = rest * a.tiles;
+    t.b = (int)(rest / (unsigned)a.blocks);
+    t.c0 = (int)(rest - t.b * (unsigned)a.blocks) * width;
     return t;
 }
 
 template <int V>
 struct Shared {
-    F<V> A[kMaxWarps][32], H[kMaxWarps][32];
-    int flag[kMaxWarps];
+    F<V> A[kMaxWarps][32], H[kMaxWarps][32], D[kMaxWarps][32];
+    int flag[kMaxWarps][32];
     int ticket;
 };
 
@@ -247,57 +249,96 @@ __device__ __forceinline__ void store_channels(float* p, int c, int channels, F<
         if (c + j < channels) __stcg(p + c + j, v.get(j));
 }
 
+// What a tile publishes is a value and its kind in one word of 64 bits, so that a reader needs no flag beside it and a writer no
+// fence: a reader polls the values themselves (a flag with release and acquire took a hop from tile to tile from under one
+// to some three microseconds). Two words a channel: A, and H until the state at the tile's end takes its place.
+constexpr unsigned kMap = 1, kState = 2;
+
+template <int V>
+__device__ __forceinline__ void publish(uint2* p, F<V> v, unsigned kind) {
+    if constexpr (V == 2)
+        asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(((uint64_t)kind << 32) | __float_as_uint(v.get(0))),
+                     "l"(((uint64_t)kind << 32) | __float_as_uint(v.get(1)))
+                     : "memory");
+    else
+        asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(((uint64_t)kind << 32) | __float_as_uint(v.get(0))) : "memory");
+}
+
+// The words of the lane's channels once all are of at least the kind `want`; zero where the wait ran out.
+template <int V>
+__device__ __forceinline__ unsigned await(const uint2* p, unsigned want, DeviceStatus* st, F<V>* v) {
+#pragma unroll 1
+    for (int it = 0; it < kDefaultSpinLimit; ++it) {
+        uint64_t x, y;
+        if constexpr (V == 2) asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "l"(p) : "memory");
+        else asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(x) : "l"(p) : "memory");
+        if constexpr (V == 1) y = x;
+        const unsigned kind = (unsigned)(x >> 32);
+        if (kind >= want && kind == (unsigned)(y >> 32)) {
+            if constexpr (V == 2) *v = F<2>(__uint_as_float((unsigned)x), __uint_as_float((unsigned)y));
+            else *v = F<1>(__uint_as_float((unsigned)x));
+            return kind;
+        }
+        if (it > 16) __nanosleep(32);
+        if ((it & 63) == 63 && *((volatile int*)&st->error) != 0) return 0;
+    }
+    atomicCAS(&st->error, 0, EWS_ERR_LOOKBACK_TIMEOUT);
+    return 0;
+}
+
+template <typename T>
+__device__ __forceinline__ uint2* slot_of(const Params<T>& a, const Tile& t, int tt, int c) {
+    return a.slots + (((long)t.b * a.tiles + tt) * 2) * a.channels + c;
+}
+
 // The state that comes into the tile from the tiles before it (down: behind it). Every thread of the CTA calls it, after the
 // tile's own map was published; false when a wait ran out.
 template <typename T, int V>
 __device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, bool down, Shared<V>& sh, int warp, int lane, int warps, F<V>* state) {
-    const int step = down ? 1 : -1;
     const int before = down ? a.tiles - 1 - t.tt : t.tt;  // how many there are
     const int window = before < warps ? before : warps;
-    if (warp < window) {
-        const int at = t.tt + step * (1 + warp);
-        // the last of the window has to have its state: nothing further back is folded
-        const int flag = wait_slot(a.flags + t.slot + at, a.st, kDefaultSpinLimit, t.slot + at, warp == window - 1 ? kFlagIncl : kFlagAgg);
-        const long base = ((long)t.b * a.tiles + at) * a.channels;
-        const int c = t.c0 + lane * V;
-        if (flag == kFlagIncl) {
-            sh.H[warp][lane] = load_channels<V>(a.ends + base, c, a.channels);
-        } else if (flag == kFlagAgg) {
-            sh.A[warp][lane] = load_channels<V>(a.map_a + base, c, a.channels);
-            sh.H[warp][lane] = load_channels<V>(a.map_h + base, c, a.channels);
-        }
-        if (lane == 0) sh.flag[warp] = flag;
-    }
-    __syncthreads();
-    int n = -1;
     bool ok = true;
-    for (int w = window - 1; w >= 0; --w) {
-        if (sh.flag[w] == kFlagIncl) n = w;
-        if (sh.flag[w] < 0) ok = false;
+    if (warp < window) {
+        const int c = t.c0 + lane * V;
+        const uint2* p = slot_of(a, t, down ? t.tt + 1 + warp : t.tt - 1 - warp, c);
+        unsigned kind = kState;
+        F<V> A(0.f), H(0.f);
+        if (c < a.channels) {
+            // the last of the window has to have its state: nothing further back is folded
+            kind = await<V>(p + a.channels, warp == window - 1 ? kState : kMap, a.st, &H);
+            ok = kind != 0 && (kind == kState || await<V>(p, kMap, a.st, &A) != 0);
+        }
+        sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.flag[warp][lane] = (int)kind;
     }
-    if (!ok) return false;
-    F<V> h = sh.H[n][lane];
-    for (int w = n - 1; w >= 0; --w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
+    if (!__syncthreads_and(ok)) return false;
+    // from the furthest state on; where a nearer tile has its own already, that is the same number
+    F<V> h(0.f);
+    for (int w = window - 1; w >= 0; --w) {
+        const F<V> H = sh.H[w][lane];
+        if (sh.flag[w][lane] == (int)kState) h = H;
+        else h = fma(sh.A[w][lane], h, H);
+    }
     *state = h;
     return true;
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void publish_map(const Params<T>& a, const Tile& t, int lane, F<V> A, F<V> H) {
-    const long base = ((long)t.b * a.tiles + t.tt) * a.channels;
-    store_channels<V>(a.map_a + base, t.c0 + lane * V, a.channels, A);
-    store_channels<V>(a.map_h + base, t.c0 + lane * V, a.channels, H);
-    publish(a.flags + t.slot + t.tt, kFlagAgg);
+    const int c = t.c0 + lane * V;
+    if (c >= a.channels) return;
+    uint2* p = slot_of(a, t, t.tt, c);
+    publish<V>(p, A, kMap);
+    publish<V>(p + a.channels, H, kMap);
 }
 template <typename T, int V>
 __device__ __forceinline__ void publish_end(const Params<T>& a, const Tile& t, int lane, F<V> h) {
-    store_channels<V>(a.ends + ((long)t.b * a.tiles + t.tt) * a.channels, t.c0 + lane * V, a.channels, h);
-    publish(a.flags + t.slot + t.tt, kFlagIncl);
+    const int c = t.c0 + lane * V;
+    if (c < a.channels) publish<V>(slot_of(a, t, t.tt, c) + a.channels, h, kState);
 }
 
 template <typename T, int V>
 __device__ __forceinline__ Tile take_tile(const Params<T>& a, bool down, Shared<V>& sh) {
-    long ticket = blockIdx.x;
+    int ticket = blockIdx.x;
     if (a.tiles > 1) {
         if (threadIdx.x == 0) sh.ticket = atomicAdd(&a.st->ticket, 1);
         __syncthreads();
@@ -314,7 +355,7 @@ __global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_co
     const int c = t.c0 + lane * V;
     const bool in = c < a.channels;
     const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
-    const int from = t.tt * warps * FL + warp * FL;
+    const int from = t.tt * TILE + warp * FL;
     const int live = in ? min(max(len - from, 0), FL) : 0, rows = in ? min(max(a.steps - from, 0), FL) : 0;
 
     Word<T, V> wx[FL], wr[FL], wi[FL];
@@ -366,8 +407,7 @@ __global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_co
         else if (a.final_state) store_channels<V>(a.final_state + (long)t.b * a.channels, c, a.channels, end);
     }
     h = fma(pa, h, ph);
-    if (a.carry && from % BT == 0 && from < a.steps)
-        store_channels<V>(a.carry + ((long)t.b * ((a.steps + BT - 1) / BT) + from / BT) * a.channels, c, a.channels, h);
+    if (a.carry && warp == 0) store_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, h);
     T* po = a.out + ((long)t.b * a.steps + from) * a.channels + c;
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
@@ -375,6 +415,26 @@ __global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_co
         if (l < rows) Word<T, V>::store(po, l < live ? h : F<V>(0.f));
         po += a.channels;
     }
+}
+
+// One token's gradients: `g` comes in as what flows into its state from behind and leaves as what flows on, `sum` collects the
+// rate's.
+template <int V>
+struct Slopes {
+    F<V> x, decay, gate;
+};
+template <int V>
+__device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, F<V> a, F<V> r, F<V> i, F<V> before, F<V> x, F<V> dout, F<V>* g, F<V>* sum) {
+    const F<V> minus(-1.f), one(1.f);
+    const F<V> w = rest_of(rate * r, a);  // formed again: kept, it would take too many registers
+    // no step of the clock: the state passes, whatever the input
+    const F<V> inv = w.each([](float t) { return fabsf(t) < FLT_MIN ? 0.f : inverse_root(t); });
+    *g = *g + dout;
+    const F<V> ix = i * x, gm = *g * (w * inv);
+    const F<V> rd = r * *g * fma(a * a * inv * ix, minus, a * before);
+    *sum = fma(rd, minus, *sum);
+    *g = a * *g;
+    return Slopes<V>{gm * i, rate * rd * fma(r, one, minus), gm * ix * fma(i, minus, one)};
 }
 
 template <typename T, int V>
@@ -385,7 +445,7 @@ __global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_c
     const int c = t.c0 + lane * V;
     const bool in = c < a.channels;
     const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
-    const int from = t.tt * BT + warp * BL;
+    const int from = t.tt * TILE + warp * BL;
     const int live = in ? min(max(len - from, 0), BL) : 0, rows = in ? min(max(a.steps - from, 0), BL) : 0;
 
     Word<T, V> wx[BL], wg[BL];
@@ -419,19 +479,15 @@ __global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_c
     }
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) D = av[l] * (wg[l].get() + D);
-    // the states: maps of the warps in front
-    sh.A[warp][lane] = A, sh.H[warp][lane] = H;
+    // the states by the maps of the warps in front, the gradients by those of the warps behind
+    F<V> pa(1.f), pd(0.f), g(0.f);
+    sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
     __syncthreads();
     for (int w = 0; w < warp; ++w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
-    __syncthreads();
-    // the gradients: maps of the warps behind
-    F<V> pa(1.f), pd(0.f), g(0.f);
-    sh.H[warp][lane] = D;
-    __syncthreads();
     for (int w = warps - 1; w > warp; --w) {
         const F<V> m = sh.A[w][lane];
         pa = pa * m;
-        pd = fma(m, pd, sh.H[w][lane]);
+        pd = fma(m, pd, sh.D[w][lane]);
     }
     const F<V> ta = A * pa, td = fma(A, pd, D);
     if (t.tt == a.tiles - 1) {
@@ -456,27 +512,18 @@ __global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_c
         h = av[l] * h;
     }
     F<V> sum(0.f);
-    const F<V> minus(-1.f), one(1.f);
     const long at = ((long)t.b * a.steps + from + BL - 1) * a.channels + c;
     T *ox = a.dx + at, *od = a.ddecay + at, *oi = a.dgate + at;
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
-        const F<V> e = av[l], r = rv[l], i = iv[l];
-        const F<V> w = rest_of(rate * r, e);  // formed again: kept, it would take too many registers
-        // no step of the clock: the state passes, whatever the input
-        const F<V> inv = w.each([](float x) { return fabsf(x) < FLT_MIN ? 0.f : inverse_root(x); });
-        g = g + wg[l].get();
-        const F<V> ix = i * wx[l].get(), gm = g * (w * inv);
-        const F<V> rd = r * g * fma(e * e * inv * ix, minus, e * hb[l]);
+        const Slopes<V> o = slopes_of(rate, av[l], rv[l], iv[l], hb[l], wx[l].get(), wg[l].get(), &g, &sum);
         if (l < rows) {
             const bool there = l < live;
-            Word<T, V>::store(ox, there ? gm * i : F<V>(0.f));
-            Word<T, V>::store(oi, there ? gm * ix * fma(i, minus, one) : F<V>(0.f));
-            Word<T, V>::store(od, there ? rate * rd * fma(r, one, minus) : F<V>(0.f));
+            Word<T, V>::store(ox, there ? o.x : F<V>(0.f));
+            Word<T, V>::store(oi, there ? o.gate : F<V>(0.f));
+            Word<T, V>::store(od, there ? o.decay : F<V>(0.f));
         }
         ox -= a.channels, od -= a.channels, oi -= a.channels;
-        sum = fma(rd, minus, sum);
-        g = e * g;
     }
     if (a.drate_part) {  // of the tile, the warps in order
         __syncthreads();
@@ -488,6 +535,265 @@ __global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_c
             store_channels<V>(a.drate_part + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, s);
         }
     }
+}
+
+// ---- the same on tiles that TMA brings --------------------------------------------------------------------------
+//
+// Persistent kernels: thread 0 takes the tickets, has two tiles loaded ahead of the one in work and the one behind it stored. Rows
+// of 128 bytes, so that a warp's access to shared memory has no conflict and no address of its own; results go where what they
+// replace was read from.
+
+struct Maps {
+    CUtensorMap in[4];   // x, decay, gate; backward: dout
+    CUtensorMap out[3];  // h; backward: dx, ddecay, dgate
+};
+
+constexpr int STAGES = 3;
+
+template <int IN, int OUTS>
+struct Pipe {
+    static constexpr int STREAM = TILE * 128, STAGE = IN * STREAM;
+    static constexpr size_t bytes = (size_t)STAGES * STAGE + 128;
+    uint64_t full[STAGES];
+    Tile tile[STAGES];  // b < 0: there is none left
+    int failed;
+
+    __device__ __forceinline__ void init() {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < STAGES; ++i) tc5::mbar_init(full + i, 1);
+            failed = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
+    }
+    // Thread 0: the tile of the ticket on its way into stage s.
+    template <typename T>
+    __device__ __forceinline__ void load(const Params<T>& a, const Maps& maps, unsigned char* stage, int s, long ticket, bool down) {
+        if (ticket >= a.total) {
+            tile[s].b = -1;
+            tc5::mbar_arrive(full + s);
+            return;
+        }
+        const Tile t = tile_of(a, (int)ticket, down, 128 / (int)sizeof(T));
+        tile[s] = t;
+        tc5::mbar_expect(full + s, STAGE);
+#pragma unroll
+        for (int k = 0; k < IN; ++k) tc5::tma_load(&maps.in[k], full + s, stage + s * STAGE + k * STREAM, t.c0, t.tt * TILE, t.b);
+    }
+    __device__ __forceinline__ void store(const Maps& maps, unsigned char* stage, int s) {
+        const Tile t = tile[s];
+#pragma unroll
+        for (int k = 0; k < OUTS; ++k) tc5::tma_store(&maps.out[k], stage + s * STAGE + k * STREAM, t.c0, t.tt * TILE, t.b);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    // All threads, at the top of a tile: its stage is there and everyone is done with the tile before. False when a wait ran out.
+    __device__ __forceinline__ bool arrive(int s, uint32_t phase) {
+        return __syncthreads_and(tc5::warp_wait(full + s, phase, &failed)) != 0;
+    }
+    // All threads, after the last tile (or a wait that ran out in stage s): what is in flight lands.
+    __device__ __forceinline__ void finish(const Maps& maps, unsigned char* stage, int s, uint32_t phase, bool any, bool ok, int* status) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            if (ok && any) store(maps, stage, (s + STAGES - 1) % STAGES);
+            if (!ok) {
+                tc5::mbar_drain(full + s, phase);
+                tc5::mbar_drain(full + (s + 1) % STAGES, s + 1 == STAGES ? phase ^ 1u : phase);
+                report(status, EWS_ERR_LOOKBACK_TIMEOUT);
+            }
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ long take_ticket(const Params<T>& a, int it) {
+    return a.tiles > 1 ? (long)atomicAdd(&a.st->ticket, 1) : blockIdx.x + (long)it * gridDim.x;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
+    constexpr int V = 4 / sizeof(T);
+    using P = Pipe<3, 1>;
+    using W = Word<T, V>;
+    constexpr int STREAM = P::STREAM / 4;
+    extern __shared__ __align__(128) unsigned char raw[];
+    unsigned char* stage = raw + ((128 - (smem_addr(raw) & 127)) & 127);
+    __shared__ Shared<V> sh;
+    __shared__ P pipe;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    pipe.init();
+    if (threadIdx.x == 0)
+        for (int k = 0; k < 2; ++k) pipe.load(a, maps, stage, k, take_ticket(a, k), false);
+    int s = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (;; ++it) {
+        if (!(ok = pipe.arrive(s, phase))) break;
+        const Tile t = pipe.tile[s];
+        if (t.b < 0) break;
+        long next = 0;
+        if (threadIdx.x == 0) {
+            if (it > 0) pipe.store(maps, stage, s == 0 ? STAGES - 1 : s - 1);
+            next = take_ticket(a, it + 2);
+        }
+        const int c = t.c0 + lane * V, from = t.tt * TILE + warp * PL;
+        const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
+        const int live = min(max(len - from, 0), PL);
+        W* row = reinterpret_cast<W*>(stage + s * P::STAGE + warp * PL * 128) + lane;
+        // where there is no token: a = 1, b = 0
+        for (int l = live; l < PL; ++l) row[l * 32].fill(0.f), row[STREAM + l * 32].fill(-INFINITY), row[2 * STREAM + l * 32].fill(0.f);
+        const F<V> rate = F<V>::make([&](int j) { return c + j < a.channels ? rate_at(a.rate + c + j) : 0.f; });
+        F<V> av[PL], bv[PL], A(1.f), H(0.f);
+#pragma unroll
+        for (int l = 0; l < PL; ++l) {
+            const Decay<V> d = decay_of(rate * sigmoid(row[STREAM + l * 32].get()));
+            av[l] = d.a;
+            bv[l] = root(d.w) * sigmoid(row[2 * STREAM + l * 32].get()) * row[l * 32].get();
+            A = A * av[l];
+            H = fma(av[l], H, bv[l]);
+        }
+        F<V> pa(1.f), ph(0.f), h(0.f);
+        sh.A[warp][lane] = A, sh.H[warp][lane] = H;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) {
+            const F<V> m = sh.A[w][lane];
+            pa = pa * m;
+            ph = fma(m, ph, sh.H[w][lane]);
+        }
+        const bool last = warp == PW - 1;
+        const F<V> ta = A * pa, th = fma(A, ph, H);
+        if (t.tt == 0) {
+            if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
+        } else {
+            if (last) publish_map<T, V>(a, t, lane, ta, th);
+            __syncthreads();  // every warp has read the maps
+            if (!(ok = look_back<T, V>(a, t, false, sh, warp, lane, PW, &h))) break;
+        }
+        if (last) {
+            const F<V> end = fma(ta, h, th);
+            if (t.tt < a.tiles - 1) publish_end<T, V>(a, t, lane, end);
+            else if (a.final_state) store_channels<V>(a.final_state + (long)t.b * a.channels, c, a.channels, end);
+        }
+        if (threadIdx.x == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            pipe.load(a, maps, stage, s == 0 ? STAGES - 1 : s - 1, next, false);  // two tiles on
+        }
+        h = fma(pa, h, ph);
+        if (a.carry && warp == 0) store_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, h);
+#pragma unroll
+        for (int l = 0; l < PL; ++l) {
+            h = fma(av[l], h, bv[l]);
+            row[l * 32].put(h);
+        }
+        for (int l = live; l < PL; ++l) row[l * 32].fill(0.f);
+        tc5::fence_async_smem();
+        if (++s == STAGES) s = 0, phase ^= 1u;
+    }
+    pipe.finish(maps, stage, s, phase, it > 0, ok, a.status);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
+    constexpr int V = 4 / sizeof(T);
+    using P = Pipe<4, 3>;
+    using W = Word<T, V>;
+    constexpr int STREAM = P::STREAM / 4;
+    extern __shared__ __align__(128) unsigned char raw[];
+    unsigned char* stage = raw + ((128 - (smem_addr(raw) & 127)) & 127);
+    __shared__ Shared<V> sh;
+    __shared__ P pipe;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    pipe.init();
+    if (threadIdx.x == 0)
+        for (int k = 0; k < 2; ++k) pipe.load(a, maps, stage, k, take_ticket(a, k), true);
+    int s = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (;; ++it) {
+        if (!(ok = pipe.arrive(s, phase))) break;
+        const Tile t = pipe.tile[s];
+        if (t.b < 0) break;
+        long next = 0;
+        if (threadIdx.x == 0) {
+            if (it > 0) pipe.store(maps, stage, s == 0 ? STAGES - 1 : s - 1);
+            next = take_ticket(a, it + 2);
+        }
+        const int c = t.c0 + lane * V, from = t.tt * TILE + warp * QL;
+        const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
+        const int live = min(max(len - from, 0), QL);
+        W* row = reinterpret_cast<W*>(stage + s * P::STAGE + warp * QL * 128) + lane;
+        for (int l = live; l < QL; ++l) {
+            row[l * 32].fill(0.f), row[STREAM + l * 32].fill(-INFINITY);
+            row[2 * STREAM + l * 32].fill(0.f), row[3 * STREAM + l * 32].fill(0.f);
+        }
+        const F<V> rate = F<V>::make([&](int j) { return c + j < a.channels ? rate_at(a.rate + c + j) : 0.f; });
+        F<V> av[QL], rv[QL], iv[QL], hb[QL];  // as in backward_kernel
+        F<V> A(1.f), H(0.f), D(0.f), h(0.f);
+        if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels);
+        else if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
+#pragma unroll
+        for (int l = 0; l < QL; ++l) {
+            rv[l] = sigmoid(row[STREAM + l * 32].get()), iv[l] = sigmoid(row[2 * STREAM + l * 32].get());
+            const Decay<V> d = decay_of(rate * rv[l]);
+            av[l] = d.a;
+            hb[l] = H;
+            H = fma(av[l], H, root(d.w) * iv[l] * row[l * 32].get());
+            A = A * av[l];
+        }
+#pragma unroll
+        for (int l = QL - 1; l >= 0; --l) D = av[l] * (row[3 * STREAM + l * 32].get() + D);
+        F<V> pa(1.f), pd(0.f), g(0.f);
+        sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
+        for (int w = QW - 1; w > warp; --w) {
+            const F<V> m = sh.A[w][lane];
+            pa = pa * m;
+            pd = fma(m, pd, sh.D[w][lane]);
+        }
+        const F<V> ta = A * pa, td = fma(A, pd, D);
+        if (t.tt == a.tiles - 1) {
+            if (a.dfinal) g = load_channels<V>(a.dfinal + (long)t.b * a.channels, c, a.channels);
+        } else {
+            if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
+            __syncthreads();
+            if (!(ok = look_back<T, V>(a, t, true, sh, warp, lane, QW, &g))) break;
+        }
+        if (warp == 0) {
+            const F<V> end = fma(ta, g, td);
+            if (t.tt > 0) publish_end<T, V>(a, t, lane, end);
+            else if (a.dinitial) store_channels<V>(a.dinitial + (long)t.b * a.channels, c, a.channels, end);
+        }
+        if (threadIdx.x == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            pipe.load(a, maps, stage, s == 0 ? STAGES - 1 : s - 1, next, true);  // two tiles on
+        }
+        g = fma(pa, g, pd);
+#pragma unroll
+        for (int l = 0; l < QL; ++l) {
+            hb[l] = hb[l] + h;
+            h = av[l] * h;
+        }
+        F<V> sum(0.f);
+#pragma unroll
+        for (int l = QL - 1; l >= 0; --l) {
+            const Slopes<V> o = slopes_of(rate, av[l], rv[l], iv[l], hb[l], row[l * 32].get(), row[3 * STREAM + l * 32].get(), &g, &sum);
+            row[l * 32].put(o.x), row[STREAM + l * 32].put(o.decay), row[2 * STREAM + l * 32].put(o.gate);
+        }
+        for (int l = live; l < QL; ++l) row[l * 32].fill(0.f), row[STREAM + l * 32].fill(0.f), row[2 * STREAM + l * 32].fill(0.f);
+        tc5::fence_async_smem();
+        if (a.drate_part) {  // of the tile, the warps in order
+            sh.D[warp][lane] = sum;  // read last before the look-back
+            __syncthreads();
+            if (warp == 0) {
+                F<V> total_sum(0.f);
+                for (int w = 0; w < QW; ++w) total_sum = total_sum + sh.D[w][lane];
+                store_channels<V>(a.drate_part + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, total_sum);
+            }
+        }
+        if (++s == STAGES) s = 0, phase ^= 1u;
+    }
+    pipe.finish(maps, stage, s, phase, it > 0, ok, a.status);
 }
 
 // drate from the tiles' sums, in a fixed order: 32 channels by 32 groups of rows a CTA.
@@ -583,22 +889,18 @@ int check(const ews_recur_args* a) {
 }
 
 size_t up(size_t b) { return (b + 255) / 256 * 256; }
-int tiles_of(int steps, bool bwd) { return (steps + (bwd ? BT : FT) - 1) / (bwd ? BT : FT); }
+int tiles_of(int steps) { return (steps + TILE - 1) / TILE; }
 
 struct Sizes {
-    size_t flags, maps, ends, part, bytes;
+    size_t slots, part, bytes;  // slots: behind the status block, both cleared by a call
 };
 
-// The flags lie behind the status block, counted for one channel a lane (the narrowest tile).
 Sizes sizes(const ews_recur_args* a, bool bwd) {
     Sizes z{};
-    const size_t tiles = tiles_of(a->steps, bwd), states = (size_t)a->batch * tiles * a->channels;
-    if (tiles > 1) {
-        z.flags = up(sizeof(DeviceStatus) + sizeof(int) * (size_t)a->batch * tiles * ((a->channels + 31) / 32));
-        z.maps = up(2 * sizeof(float) * states), z.ends = up(sizeof(float) * states);
-    }
+    const size_t tiles = tiles_of(a->steps), states = (size_t)a->batch * tiles * a->channels;
+    if (tiles > 1) z.slots = up(sizeof(DeviceStatus) + 2 * sizeof(uint2) * states);
     if (bwd) z.part = up(sizeof(float) * states);
-    z.bytes = z.flags + z.maps + z.ends + z.part;
+    z.bytes = z.slots + z.part;
     return z;
 }
 
@@ -612,10 +914,28 @@ bool even(const ews_recur_args* a, const Stream<T>& s) {
     return ((uintptr_t)s.p & 3u) == 0 && (a->batch == 1 || s.sb % 2 == 0) && (a->steps == 1 || s.st % 2 == 0);
 }
 
+// A stream (batch, steps, channels) for TMA: boxes of 128 bytes of channels by a tile's steps. False where it cannot be read so.
+template <typename T>
+bool make_map(CUtensorMap* map, const ews_recur_args* a, const void* p, long sb, long st) {
+    constexpr long E = 16 / sizeof(T);
+    const long one = (a->channels + E - 1) / E * E;  // an axis of one has no stride to speak of
+    if (a->steps == 1) st = one;
+    if (a->batch == 1) sb = st * a->steps;
+    if (!aligned16(p) || st <= 0 || sb <= 0 || st % E || sb % E || a->channels % E) return false;
+    tc5::EncodeFn enc = tc5::encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)a->channels, (cuuint64_t)a->steps, (cuuint64_t)a->batch};
+    const cuuint64_t strides[2] = {(cuuint64_t)st * sizeof(T), (cuuint64_t)sb * sizeof(T)};
+    const cuuint32_t box[3] = {128 / sizeof(T), (cuuint32_t)TILE, 1}, es[3] = {1, 1, 1};
+    return enc(map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims, strides,
+               box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T>
 int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     Params<T> p{};
-    p.batch = a->batch, p.steps = a->steps, p.channels = a->channels, p.tiles = tiles_of(a->steps, bwd);
+    p.batch = a->batch, p.steps = a->steps, p.channels = a->channels, p.tiles = tiles_of(a->steps);
     p.x = stream_of<T>(a->x, a->x_stride), p.decay = stream_of<T>(a->decay, a->decay_stride), p.gate = stream_of<T>(a->gate, a->gate_stride);
     p.rate = a->rate, p.lengths = a->lengths, p.initial = a->initial, p.carry = a->carry, p.status = a->status;
     bool pairs = sizeof(T) == 2 && a->channels % 2 == 0 && even(a, p.x) && even(a, p.decay) && even(a, p.gate);
@@ -633,23 +953,39 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     if (p.tiles > 1) {
         p.st = reinterpret_cast<DeviceStatus*>(w);
-        p.flags = reinterpret_cast<int*>(w + sizeof(DeviceStatus));
-        p.map_a = reinterpret_cast<float*>(w + z.flags);
-        p.map_h = p.map_a + (size_t)a->batch * p.tiles * a->channels;
-        p.ends = reinterpret_cast<float*>(w + z.flags + z.maps);
-        if (cudaMemsetAsync(w, 0, z.flags, s) != cudaSuccess) return EWS_ERR_LAUNCH;
+        p.slots = reinterpret_cast<uint2*>(w + sizeof(DeviceStatus));
+        if (cudaMemsetAsync(w, 0, z.slots, s) != cudaSuccess) return EWS_ERR_LAUNCH;
     }
-    if (bwd && a->drate) p.drate_part = reinterpret_cast<float*>(w + z.flags + z.maps + z.ends);
+    if (bwd && a->drate) p.drate_part = reinterpret_cast<float*>(w + z.slots);
     const long ctas = (long)p.batch * p.blocks * p.tiles;
-    if (ctas > 0x7FFFFFFFl) return EWS_ERR_UNSUPPORTED;
+    if (ctas > 0x7FFFFFFFl - 65536) return EWS_ERR_UNSUPPORTED;  // the tickets count a little further
+    p.total = ctas;
+    Maps m{};
+    const long C = a->channels, whole = (long)a->steps * C;
+    bool piped = a->steps >= kPipedFrom && make_map<T>(&m.in[0], a, a->x, p.x.sb, p.x.st) &&
+                 make_map<T>(&m.in[1], a, a->decay, p.decay.sb, p.decay.st) && make_map<T>(&m.in[2], a, a->gate, p.gate.sb, p.gate.st);
+    if (bwd)
+        piped = piped && a->dout && make_map<T>(&m.in[3], a, a->dout, p.dout.sb, p.dout.st) && make_map<T>(&m.out[0], a, a->dx, whole, C) &&
+                make_map<T>(&m.out[1], a, a->ddecay, whole, C) && make_map<T>(&m.out[2], a, a->dgate, whole, C);
+    else
+        piped = piped && make_map<T>(&m.out[0], a, a->out, whole, C);
     const int per = bwd ? BL : FL;
     const int warps = p.tiles > 1 ? (bwd ? BW : FW) : (a->steps + per - 1) / per;  // a short axis: as many as it has work for
     auto go = [&](auto* kernel) {
         kernel<<<(unsigned)ctas, warps * 32, 0, s>>>(p);
         return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
     };
+    auto go_piped = [&](auto* kernel, size_t bytes, int threads, int resident) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return (int)EWS_ERR_LAUNCH;
+        const long most = (long)SMS * resident;
+        kernel<<<(unsigned)(ctas < most ? ctas : most), threads, bytes, s>>>(p, m);
+        return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
+    };
     int rc;
-    if constexpr (sizeof(T) == 2) {
+    if (piped) {
+        rc = bwd ? go_piped(backward_tma_kernel<T>, Pipe<4, 3>::bytes, QW * 32, QCTAS)
+                 : go_piped(forward_tma_kernel<T>, Pipe<3, 1>::bytes, PW * 32, PCTAS);
+    } else if constexpr (sizeof(T) == 2) {
         if (pairs) rc = bwd ? go(backward_kernel<T, 2>) : go(forward_kernel<T, 2>);
         else rc = bwd ? go(backward_kernel<T, 1>) : go(forward_kernel<T, 1>);
     } else {
@@ -692,7 +1028,7 @@ int step(const ews_recur_args* a, const int* slots, int pool, float* state, cuda
 using namespace ews::recur;
 
 extern "C" size_t ews_recur_carry_size(const ews_recur_args* a) {
-    return check(a) == EWS_OK ? sizeof(float) * (size_t)a->batch * tiles_of(a->steps, true) * a->channels : 0;
+    return check(a) == EWS_OK ? sizeof(float) * (size_t)a->batch * tiles_of(a->steps) * a->channels : 0;
 }
 
 extern "C" size_t ews_recur_work_size(const ews_recur_args* a, int backward) {
@@ -719,7 +1055,7 @@ extern "C" int ews_recur_bwd(const ews_recur_args* a, ews_stream_t stream) {
         return pass(a, a->dfinal, a->dinitial, s);
     }
     if (!a->x || !a->decay || !a->gate || !a->rate || !a->dx || !a->ddecay || !a->dgate) return EWS_ERR_INVALID_ARGUMENT;
-    if (tiles_of(a->steps, true) > 1 && !a->carry) return EWS_ERR_INVALID_ARGUMENT;
+    if (tiles_of(a->steps) > 1 && !a->carry) return EWS_ERR_INVALID_ARGUMENT;
     const Sizes z = sizes(a, true);
     if (z.bytes && (!a->work || !ews::token::aligned16(a->work) || a->work_bytes < z.bytes)) return EWS_ERR_WORKSPACE;
     return a->dtype == EWS_DTYPE_BF16 ? run<ews::token::bf16>(a, true, s) : run<float>(a, true, s);

@@ -45,7 +45,7 @@ def test_recurrence_arguments_are_checked_before_the_device():
     assert lib.ews_recur_bwd(_recur(carry=0), None) == 1  # several tiles need the forward's states
     assert lib.ews_recur_fwd(_recur(), None) == 3 and lib.ews_recur_bwd(_recur(), None) == 3
     assert lib.ews_recur_work_size(_recur(batch=0), 0) == 0 and lib.ews_recur_fwd(_recur(batch=0), None) == 0
-    assert lib.ews_recur_work_size(_recur(steps=100), 0) == 0  # one tile waits for nobody
+    assert lib.ews_recur_work_size(_recur(steps=64), 0) == 0  # one tile waits for nobody
     assert lib.ews_recur_step(_recur(), None, 1, 16, None) == 1  # fewer states than rows and no slots
     assert lib.ews_recur_step(_recur(), 16, -1, 16, None) == 1 and lib.ews_recur_step(_recur(), 16, 8, None, None) == 1
     assert recur_ops._sizes(2, 300, 64, 1) == (lib.ews_recur_carry_size(_recur()), lib.ews_recur_work_size(_recur(), 0), lib.ews_recur_work_size(_recur(), 1))
