@@ -30,12 +30,13 @@ using tc5::mul2;
 using tc5::pair;
 using tc5::unpair;
 
-constexpr int kMaxWarps = 16, SMS = 148;
-constexpr int TILE = 64;                  // tokens a tile
-constexpr int FL = 8, FW = TILE / FL, FCTAS = 3;  // forward: tokens a warp, warps a tile, CTAs an SM
-constexpr int BL = 8, BW = TILE / BL, BCTAS = 2;  // backward
-constexpr int PL = 8, PW = TILE / PL, PCTAS = 3;  // the same where TMA brings the tiles
+constexpr int SMS = 148;
+constexpr int TILE = 64;                           // tokens a tile
+constexpr int FL = 8, FW = TILE / FL, FCTAS = 3;   // forward: tokens a warp, warps a tile, CTAs an SM
+constexpr int BL = 8, BW = TILE / BL, BCTAS = 2;   // backward
+constexpr int PL = 16, PW = TILE / PL, PCTAS = 4;  // the same where TMA brings the tiles
 constexpr int QL = 8, QW = TILE / QL, QCTAS = 2;
+constexpr int PSTAGES = 2, QSTAGES = 2;
 constexpr int kPipedFrom = 33;            // steps from which it does: below, most of a tile would be empty
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -230,10 +231,10 @@ __device__ __forceinline__ Tile tile_of(const Params<T>& a, int ticket, bool dow
     return t;
 }
 
-template <int V>
+template <int V, int WARPS, bool BACK>
 struct Shared {
-    F<V> A[kMaxWarps][32], H[kMaxWarps][32], D[kMaxWarps][32];
-    int flag[kMaxWarps][32];
+    F<V> A[WARPS][32], H[WARPS][32], D[BACK ? WARPS : 1][32];
+    unsigned kind[WARPS][32];
     int ticket;
 };
 
@@ -293,8 +294,8 @@ __device__ __forceinline__ uint2* slot_of(const Params<T>& a, const Tile& t, int
 
 // The state that comes into the tile from the tiles before it (down: behind it). Every thread of the CTA calls it, after the
 // tile's own map was published; false when a wait ran out.
-template <typename T, int V>
-__device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, bool down, Shared<V>& sh, int warp, int lane, int warps, F<V>* state) {
+template <typename T, int V, int WARPS, bool BACK>
+__device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, bool down, Shared<V, WARPS, BACK>& sh, int warp, int lane, int warps, F<V>* state) {
     const int before = down ? a.tiles - 1 - t.tt : t.tt;  // how many there are
     const int window = before < warps ? before : warps;
     bool ok = true;
@@ -308,14 +309,14 @@ __device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, boo
             kind = await<V>(p + a.channels, warp == window - 1 ? kState : kMap, a.st, &H);
             ok = kind != 0 && (kind == kState || await<V>(p, kMap, a.st, &A) != 0);
         }
-        sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.flag[warp][lane] = (int)kind;
+        sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.kind[warp][lane] = kind;
     }
     if (!__syncthreads_and(ok)) return false;
     // from the furthest state on; where a nearer tile has its own already, that is the same number
     F<V> h(0.f);
     for (int w = window - 1; w >= 0; --w) {
         const F<V> H = sh.H[w][lane];
-        if (sh.flag[w][lane] == (int)kState) h = H;
+        if (sh.kind[w][lane] == kState) h = H;
         else h = fma(sh.A[w][lane], h, H);
     }
     *state = h;
@@ -336,8 +337,8 @@ __device__ __forceinline__ void publish_end(const Params<T>& a, const Tile& t, i
     if (c < a.channels) publish<V>(slot_of(a, t, t.tt, c) + a.channels, h, kState);
 }
 
-template <typename T, int V>
-__device__ __forceinline__ Tile take_tile(const Params<T>& a, bool down, Shared<V>& sh) {
+template <typename T, int V, int WARPS, bool BACK>
+__device__ __forceinline__ Tile take_tile(const Params<T>& a, bool down, Shared<V, WARPS, BACK>& sh) {
     int ticket = blockIdx.x;
     if (a.tiles > 1) {
         if (threadIdx.x == 0) sh.ticket = atomicAdd(&a.st->ticket, 1);
@@ -349,7 +350,7 @@ __device__ __forceinline__ Tile take_tile(const Params<T>& a, bool down, Shared<
 
 template <typename T, int V>
 __global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_constant__ Params<T> a) {
-    __shared__ Shared<V> sh;
+    __shared__ Shared<V, FW, false> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Tile t = take_tile(a, false, sh);
     const int c = t.c0 + lane * V;
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_co
     } else {
         if (last) publish_map<T, V>(a, t, lane, ta, th);
         __syncthreads();  // every warp has read the maps
-        if (!look_back<T, V>(a, t, false, sh, warp, lane, warps, &h)) {
+        if (!look_back(a, t, false, sh, warp, lane, warps, &h)) {
             if (threadIdx.x == 0) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
             return;
         }
@@ -439,7 +440,7 @@ __device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, F<V> a, F<V> r, F<V> i
 
 template <typename T, int V>
 __global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_constant__ Params<T> a) {
-    __shared__ Shared<V> sh;
+    __shared__ Shared<V, BW, true> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Tile t = take_tile(a, true, sh);
     const int c = t.c0 + lane * V;
@@ -495,7 +496,7 @@ __global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_c
     } else {
         if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
         __syncthreads();
-        if (!look_back<T, V>(a, t, true, sh, warp, lane, warps, &g)) {
+        if (!look_back(a, t, true, sh, warp, lane, warps, &g)) {
             if (threadIdx.x == 0) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
             return;
         }
@@ -548,9 +549,7 @@ struct Maps {
     CUtensorMap out[3];  // h; backward: dx, ddecay, dgate
 };
 
-constexpr int STAGES = 3;
-
-template <int IN, int OUTS>
+template <int IN, int OUTS, int STAGES>
 struct Pipe {
     static constexpr int STREAM = TILE * 128, STAGE = IN * STREAM;
     static constexpr size_t bytes = (size_t)STAGES * STAGE + 128;
@@ -596,8 +595,10 @@ struct Pipe {
         if (threadIdx.x == 0) {
             if (ok && any) store(maps, stage, (s + STAGES - 1) % STAGES);
             if (!ok) {
-                tc5::mbar_drain(full + s, phase);
-                tc5::mbar_drain(full + (s + 1) % STAGES, s + 1 == STAGES ? phase ^ 1u : phase);
+                for (int k = 0; k < STAGES; ++k) {  // the stages from this one on, as far as they were filled
+                    tc5::mbar_drain(full + s, phase);
+                    if (++s == STAGES) s = 0, phase ^= 1u;
+                }
                 report(status, EWS_ERR_LOOKBACK_TIMEOUT);
             }
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -613,17 +614,17 @@ __device__ __forceinline__ long take_ticket(const Params<T>& a, int it) {
 template <typename T>
 __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
     constexpr int V = 4 / sizeof(T);
-    using P = Pipe<3, 1>;
+    using P = Pipe<3, 1, PSTAGES>;
     using W = Word<T, V>;
     constexpr int STREAM = P::STREAM / 4;
     extern __shared__ __align__(128) unsigned char raw[];
     unsigned char* stage = raw + ((128 - (smem_addr(raw) & 127)) & 127);
-    __shared__ Shared<V> sh;
+    __shared__ Shared<V, PW, false> sh;
     __shared__ P pipe;
     const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     pipe.init();
     if (threadIdx.x == 0)
-        for (int k = 0; k < 2; ++k) pipe.load(a, maps, stage, k, take_ticket(a, k), false);
+        for (int k = 0; k < PSTAGES - 1; ++k) pipe.load(a, maps, stage, k, take_ticket(a, k), false);
     int s = 0, it = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -633,8 +634,8 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
         if (t.b < 0) break;
         long next = 0;
         if (threadIdx.x == 0) {
-            if (it > 0) pipe.store(maps, stage, s == 0 ? STAGES - 1 : s - 1);
-            next = take_ticket(a, it + 2);
+            if (it > 0) pipe.store(maps, stage, s == 0 ? PSTAGES - 1 : s - 1);
+            next = take_ticket(a, it + PSTAGES - 1);
         }
         const int c = t.c0 + lane * V, from = t.tt * TILE + warp * PL;
         const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
@@ -654,6 +655,10 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
         }
         F<V> pa(1.f), ph(0.f), h(0.f);
         sh.A[warp][lane] = A, sh.H[warp][lane] = H;
+        if (threadIdx.x == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            pipe.load(a, maps, stage, s == 0 ? PSTAGES - 1 : s - 1, next, false);
+        }
         __syncthreads();
         for (int w = 0; w < warp; ++w) {
             const F<V> m = sh.A[w][lane];
@@ -667,16 +672,12 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
         } else {
             if (last) publish_map<T, V>(a, t, lane, ta, th);
             __syncthreads();  // every warp has read the maps
-            if (!(ok = look_back<T, V>(a, t, false, sh, warp, lane, PW, &h))) break;
+            if (!(ok = look_back(a, t, false, sh, warp, lane, PW, &h))) break;
         }
         if (last) {
             const F<V> end = fma(ta, h, th);
             if (t.tt < a.tiles - 1) publish_end<T, V>(a, t, lane, end);
             else if (a.final_state) store_channels<V>(a.final_state + (long)t.b * a.channels, c, a.channels, end);
-        }
-        if (threadIdx.x == 0) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            pipe.load(a, maps, stage, s == 0 ? STAGES - 1 : s - 1, next, false);  // two tiles on
         }
         h = fma(pa, h, ph);
         if (a.carry && warp == 0) store_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, h);
@@ -687,7 +688,7 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
         }
         for (int l = live; l < PL; ++l) row[l * 32].fill(0.f);
         tc5::fence_async_smem();
-        if (++s == STAGES) s = 0, phase ^= 1u;
+        if (++s == PSTAGES) s = 0, phase ^= 1u;
     }
     pipe.finish(maps, stage, s, phase, it > 0, ok, a.status);
 }
@@ -695,17 +696,17 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
 template <typename T>
 __global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
     constexpr int V = 4 / sizeof(T);
-    using P = Pipe<4, 3>;
+    using P = Pipe<4, 3, QSTAGES>;
     using W = Word<T, V>;
     constexpr int STREAM = P::STREAM / 4;
     extern __shared__ __align__(128) unsigned char raw[];
     unsigned char* stage = raw + ((128 - (smem_addr(raw) & 127)) & 127);
-    __shared__ Shared<V> sh;
+    __shared__ Shared<V, QW, true> sh;
     __shared__ P pipe;
     const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     pipe.init();
     if (threadIdx.x == 0)
-        for (int k = 0; k < 2; ++k) pipe.load(a, maps, stage, k, take_ticket(a, k), true);
+        for (int k = 0; k < QSTAGES - 1; ++k) pipe.load(a, maps, stage, k, take_ticket(a, k), true);
     int s = 0, it = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -715,8 +716,8 @@ __global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __gr
         if (t.b < 0) break;
         long next = 0;
         if (threadIdx.x == 0) {
-            if (it > 0) pipe.store(maps, stage, s == 0 ? STAGES - 1 : s - 1);
-            next = take_ticket(a, it + 2);
+            if (it > 0) pipe.store(maps, stage, s == 0 ? QSTAGES - 1 : s - 1);
+            next = take_ticket(a, it + QSTAGES - 1);
         }
         const int c = t.c0 + lane * V, from = t.tt * TILE + warp * QL;
         const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
@@ -744,6 +745,10 @@ __global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __gr
         for (int l = QL - 1; l >= 0; --l) D = av[l] * (row[3 * STREAM + l * 32].get() + D);
         F<V> pa(1.f), pd(0.f), g(0.f);
         sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
+        if (threadIdx.x == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            pipe.load(a, maps, stage, s == 0 ? QSTAGES - 1 : s - 1, next, true);
+        }
         __syncthreads();
         for (int w = 0; w < warp; ++w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
         for (int w = QW - 1; w > warp; --w) {
@@ -757,16 +762,12 @@ __global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __gr
         } else {
             if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
             __syncthreads();
-            if (!(ok = look_back<T, V>(a, t, true, sh, warp, lane, QW, &g))) break;
+            if (!(ok = look_back(a, t, true, sh, warp, lane, QW, &g))) break;
         }
         if (warp == 0) {
             const F<V> end = fma(ta, g, td);
             if (t.tt > 0) publish_end<T, V>(a, t, lane, end);
             else if (a.dinitial) store_channels<V>(a.dinitial + (long)t.b * a.channels, c, a.channels, end);
-        }
-        if (threadIdx.x == 0) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            pipe.load(a, maps, stage, s == 0 ? STAGES - 1 : s - 1, next, true);  // two tiles on
         }
         g = fma(pa, g, pd);
 #pragma unroll
@@ -791,7 +792,7 @@ __global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __gr
                 store_channels<V>(a.drate_part + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, total_sum);
             }
         }
-        if (++s == STAGES) s = 0, phase ^= 1u;
+        if (++s == QSTAGES) s = 0, phase ^= 1u;
     }
     pipe.finish(maps, stage, s, phase, it > 0, ok, a.status);
 }
@@ -983,8 +984,8 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     };
     int rc;
     if (piped) {
-        rc = bwd ? go_piped(backward_tma_kernel<T>, Pipe<4, 3>::bytes, QW * 32, QCTAS)
-                 : go_piped(forward_tma_kernel<T>, Pipe<3, 1>::bytes, PW * 32, PCTAS);
+        rc = bwd ? go_piped(backward_tma_kernel<T>, Pipe<4, 3, QSTAGES>::bytes, QW * 32, QCTAS)
+                 : go_piped(forward_tma_kernel<T>, Pipe<3, 1, PSTAGES>::bytes, PW * 32, PCTAS);
     } else if constexpr (sizeof(T) == 2) {
         if (pairs) rc = bwd ? go(backward_kernel<T, 2>) : go(forward_kernel<T, 2>);
         else rc = bwd ? go(backward_kernel<T, 1>) : go(forward_kernel<T, 1>);
