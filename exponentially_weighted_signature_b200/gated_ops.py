@@ -13,18 +13,11 @@ import torch
 
 from . import _lib, engine
 from .engine import first_order
-from .token_ops import _DTYPES, _addr, _device, _dtype, _launch, _row_stride, _rows, _work
+from .token_ops import _DTYPES, _addr, _device, _dtype, _launch, _work
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 _GATED = struct.Struct("@3q2i3P3q3Pq4PNP").pack  # ews_gated_args
-
-
-def _args(x, wg, wu, act, out=None, kept=None, dout=None, grads=(None, None, None), work=None):
-    (rows, dim), inner = x.shape, wg.shape[0]
-    return _GATED(rows, dim, inner, _DTYPES[x.dtype], act, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _row_stride(x),
-                  _row_stride(wg), _row_stride(wu), _addr(out), _addr(kept), _addr(dout),
-                  0 if dout is None else _row_stride(dout), *map(_addr, grads), _addr(work), 0 if work is None else work.numel(),
-                  engine.index_word(x.get_device())[0])
+_BF16 = _lib.EWS_DTYPE_BF16
 
 
 @functools.lru_cache(maxsize=256)
@@ -39,43 +32,65 @@ def _kept_size(rows, dim, inner, code):
     return _lib.load().ews_gated_kept_size(_GATED(rows, dim, inner, code, 0, 0, 0, 0, dim, dim, dim, *([0] * 10)))
 
 
-def _workspace(x, wg, wu, wanted, backward):
-    at = (x.data_ptr() % 16, wg.data_ptr() % 16, wu.data_ptr() % 16)
-    strides = (_row_stride(x), _row_stride(wg), _row_stride(wu))
-    return _work(_size(*x.shape, wg.shape[0], _DTYPES[x.dtype], strides, at, wanted, backward), x)
+def _operand(t):
+    """A matrix with contiguous rows, and how far apart they are."""
+    rows, dim = t.shape
+    stride, one = t.stride()
+    if rows <= 1:
+        stride = dim
+    if one != 1 and dim > 1 or stride < dim:
+        return t.contiguous(), dim
+    return t, stride
 
 
 def _forward(x, wg, wu, act, shape, keep):
-    lib = _lib.load()
-    rows, inner = x.shape[0], wg.shape[0]
-    out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    kept = _work(_kept_size(rows, x.shape[1], inner, _DTYPES[x.dtype]), x) if keep else None
-    work = _workspace(x, wg, wu, (0, 0, 0), 0)
-    _launch(x.get_device(), "ews_gated_fwd", rows, lib.ews_gated_fwd, _args(x, wg, wu, act, out, kept, work=work))
+    """The layer on operands: (tensor, stride) each. A single token's call is the host's time: what it can do without it does not
+    ask for."""
+    (x, xs), (wg, gs), (wu, us) = x, wg, wu
+    rows, dim = x.shape
+    inner, code, device = wg.shape[0], _DTYPES[x.dtype], x.device
+    xp, gp, up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
+    out = torch.empty(shape, dtype=x.dtype, device=device)
+    kept = torch.empty(_kept_size(rows, dim, inner, code), dtype=torch.uint8, device=device) if keep else None
+    work, size = 0, 0
+    if code != _BF16 or (xs | gs | us | dim) & 7 or (xp | gp | up) & 15:  # else nothing is packed
+        size = _size(rows, dim, inner, code, (xs, gs, us), (xp % 16, gp % 16, up % 16), (0, 0, 0), 0)
+        space = _work(size, x)
+        work = _addr(space)
+    idx = x.get_device()
+    args = _GATED(rows, dim, inner, code, act, xp, gp, up, xs, gs, us, out.data_ptr(), _addr(kept), 0, 0, 0, 0, 0, work, size,
+                  engine.index_word(idx)[0])
+    _launch(idx, "ews_gated_fwd", rows, _lib.load().ews_gated_fwd, args)
     return out, kept
 
 
 class _Gated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, act, shape):
-        x, wg, wu = _rows(x), _rows(wg), _rows(wu)
+        x, wg, wu = _operand(x), _operand(wg), _operand(wu)
         out, kept = _forward(x, wg, wu, act, shape, True)
-        ctx.act = act
-        ctx.save_for_backward(x, wg, wu, kept)
+        ctx.meta = act, x[1], wg[1], wu[1]
+        ctx.save_for_backward(x[0], wg[0], wu[0], kept)
         return out
 
     @staticmethod
     @first_order
     def backward(ctx, dout):
         x, wg, wu, kept = ctx.saved_tensors
-        lib = _lib.load()
-        dout = _rows(dout.reshape(x.shape[0], wg.shape[0]))
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
-                 for t, need in zip((x, wg, wu), ctx.needs_input_grad)]
-        work = _workspace(x, wg, wu, tuple(int(g is not None) for g in grads), 1)
-        args = _args(x, wg, wu, ctx.act, None, kept, dout, grads, work)
-        _launch(x.get_device(), "ews_gated_bwd", x.shape[0], lib.ews_gated_bwd, args)
-        return (*grads, None, None)
+        act, xs, gs, us = ctx.meta
+        (rows, dim), inner, code = x.shape, wg.shape[0], _DTYPES[x.dtype]
+        dout, ds = _operand(dout if dout.dim() == 2 else dout.reshape(rows, inner))
+        dx, dwg, dwu = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+                        for t, need in zip((x, wg, wu), ctx.needs_input_grad))
+        xp, gp, up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
+        size = _size(rows, dim, inner, code, (xs, gs, us), (xp % 16, gp % 16, up % 16),
+                     (int(dx is not None), int(dwg is not None), int(dwu is not None)), 1)
+        work = _work(size, x)
+        idx = x.get_device()
+        args = _GATED(rows, dim, inner, code, act, xp, gp, up, xs, gs, us, 0, kept.data_ptr(), dout.data_ptr(), ds, _addr(dx), _addr(dwg),
+                      _addr(dwu), _addr(work), size, engine.index_word(idx)[0])
+        _launch(idx, "ews_gated_bwd", rows, _lib.load().ews_gated_bwd, args)
+        return dx, dwg, dwu, None, None
 
 
 def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, *, activation: str = "silu") -> torch.Tensor:
@@ -84,10 +99,12 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
     x (..., D); gate_weight and up_weight (F, D), all float32 or all bfloat16 (rows of any stride). activation: "silu",
     ``g sigmoid(g)``, or "gelu", ``g Phi(g)``. Returns (..., F). Sums are float32; the product is formed from them and rounded
     once. Differentiable in x and both weights (the two projections are kept for it, 6 bytes a pair for bfloat16, 8 for float32)."""
-    if gate_weight.dim() != 2 or up_weight.shape != gate_weight.shape or 0 in gate_weight.shape:
-        raise ValueError(f"gate_weight and up_weight must be (F, D) with F, D > 0, got {tuple(gate_weight.shape)} and {tuple(up_weight.shape)}")
-    if x.dim() < 1 or x.shape[-1] != gate_weight.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)} and weights {tuple(gate_weight.shape)} do not fit together")
+    inner = gate_weight.shape
+    if len(inner) != 2 or up_weight.shape != inner or 0 in inner:
+        raise ValueError(f"gate_weight and up_weight must be (F, D) with F, D > 0, got {tuple(inner)} and {tuple(up_weight.shape)}")
+    shape = x.shape
+    if not shape or shape[-1] != inner[1]:
+        raise ValueError(f"x {tuple(shape)} and weights {tuple(inner)} do not fit together")
     if not (x.dtype == gate_weight.dtype == up_weight.dtype):
         raise TypeError(f"x and the weights must share a type, got {x.dtype}, {gate_weight.dtype}, {up_weight.dtype}")
     _dtype(x, "x and the weights")
@@ -95,7 +112,8 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
     if act is None:
         raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
     _device(x, gate_weight, up_weight)
-    flat, shape = x.reshape(-1, x.shape[-1]), (*x.shape[:-1], gate_weight.shape[0])
+    flat = x if len(shape) == 2 else x.reshape(-1, inner[1])
+    shape = (*shape[:-1], inner[0])
     if torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad):
         return _Gated.apply(flat, gate_weight, up_weight, act, shape)
-    return _forward(_rows(flat), _rows(gate_weight), _rows(up_weight), act, shape, False)[0]
+    return _forward(_operand(flat), _operand(gate_weight), _operand(up_weight), act, shape, False)[0]

@@ -75,10 +75,11 @@ def _check(x, decay, gate, rate, axes):
     if not (x.dtype == decay.dtype == gate.dtype):
         raise TypeError(f"x, decay and gate must share a type, got {x.dtype}, {decay.dtype}, {gate.dtype}")
     _dtype(x, "x, decay and gate")
-    if x.dim() != axes or x.shape[-1] == 0 or decay.shape != x.shape or gate.shape != x.shape:
-        raise ValueError(f"x, decay and gate must share a shape of {axes} axes with channels, got {tuple(x.shape)}, "
+    shape = x.shape
+    if len(shape) != axes or shape[-1] == 0 or decay.shape != shape or gate.shape != shape:
+        raise ValueError(f"x, decay and gate must share a shape of {axes} axes with channels, got {tuple(shape)}, "
                          f"{tuple(decay.shape)}, {tuple(gate.shape)}")
-    C = x.shape[-1]
+    C = shape[-1]
     if rate.shape != (C,) or rate.dtype != torch.float32 or not rate.is_contiguous():
         raise ValueError(f"rate must be a contiguous float32 tensor of {C} values, got {rate.dtype} {tuple(rate.shape)}")
     return C
@@ -129,23 +130,27 @@ def gated_recurrence_step(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tens
     a slot; one out of range gives a zero row and IndexError on the next call. Returns h (B, C). For serving: no
     gradient; a backward that needs the states as they were raises, as after any operation in place."""
     C = _check(x, decay, gate, rate, 2)
-    B = x.shape[0]
-    if state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
-        raise ValueError(f"state must be contiguous float32 (P, {C}), got {state.dtype} {tuple(state.shape)}")
+    B, pool = x.shape[0], state.shape
+    if len(pool) != 2 or pool[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous float32 (P, {C}), got {state.dtype} {tuple(pool)}")
     if slots is None:
-        if state.shape[0] < B:
-            raise ValueError(f"{B} rows need as many states or slots, got {state.shape[0]} states")
+        if pool[0] < B:
+            raise ValueError(f"{B} rows need as many states or slots, got {pool[0]} states")
     elif slots.shape != (B,) or slots.dtype != torch.int32 or not slots.is_contiguous():
         raise ValueError(f"slots must be contiguous int32 ({B},), got {slots.dtype} {tuple(slots.shape)}")
     if torch.is_grad_enabled() and (x.requires_grad or decay.requires_grad or gate.requires_grad or rate.requires_grad
                                     or state.requires_grad):
         raise RuntimeError("gated_recurrence_step has no gradient: call it under torch.no_grad()")
     idx = _device(x, decay, gate, rate, state, slots)
-    x, decay, gate = _last_contiguous(x), _last_contiguous(decay), _last_contiguous(gate)
+    (xs, x1), (ds, d1), (gs, g1) = x.stride(), decay.stride(), gate.stride()
+    if (x1 != 1 or d1 != 1 or g1 != 1) and C > 1:
+        x, decay, gate = x.contiguous(), decay.contiguous(), gate.contiguous()
+        xs = ds = gs = C
     out = torch.empty((B, C), dtype=x.dtype, device=x.device)
-    args = _RECUR(B, 1, C, _DTYPES[x.dtype], x.data_ptr(), decay.data_ptr(), gate.data_ptr(), x.stride(0), 0, decay.stride(0), 0,
-                  gate.stride(0), 0, rate.data_ptr(), 0, 0, out.data_ptr(), *([0] * 13), engine.index_word(idx)[0])
-    _launch(idx, "ews_recur_step", B, _lib.load().ews_recur_step, args, _addr(slots), state.shape[0], state.data_ptr())
+    args = _RECUR(B, 1, C, _DTYPES[x.dtype], x.data_ptr(), decay.data_ptr(), gate.data_ptr(), xs, 0, ds, 0, gs, 0, rate.data_ptr(),
+                  0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, engine.index_word(idx)[0])
+    _launch(idx, "ews_recur_step", B, _lib.load().ews_recur_step, args, 0 if slots is None else slots.data_ptr(), pool[0],
+            state.data_ptr())
     if not state.is_inference():  # autograd cannot see the write: a backward that saved these states must
         torch.autograd.graph.increment_version(state)
     return out
