@@ -32,10 +32,15 @@ using tc5::unpair;
 
 constexpr int SMS = 148;
 constexpr int TILE = 64;                           // tokens a tile
-constexpr int FL = 8, FW = TILE / FL, FCTAS = 3;   // forward: tokens a warp, warps a tile, CTAs an SM
-constexpr int BL = 8, BW = TILE / BL, BCTAS = 2;   // backward
-constexpr int PL = 16, PW = TILE / PL, PCTAS = 4;  // the same where TMA brings the tiles
-constexpr int QL = 8, QW = TILE / QL, QCTAS = 2;
+// Tokens a warp, warps a tile and CTAs an SM, of V channels a lane: what the registers of a token's values allow. (333 channels
+// of float32, 16 x 1,440 tokens: 8 tokens a warp took 44 and 93 us forwards and back, 16 take 40 and 69.)
+template <int V>
+struct Shape {
+    static constexpr int FL = V == 1 ? 16 : 8, FW = TILE / FL, FCTAS = V == 1 ? 8 : 3;  // forward
+    static constexpr int BL = V == 1 ? 16 : 8, BW = TILE / BL, BCTAS = V == 1 ? 4 : 2;  // backward
+    static constexpr int QL = V == 1 ? 16 : 8, QW = TILE / QL, QCTAS = V == 1 ? 3 : 2;  // the same where TMA brings the tiles
+};
+constexpr int PL = 16, PW = TILE / PL, PCTAS = 4;
 constexpr int PSTAGES = 2, QSTAGES = 2;
 constexpr int kPipedFrom = 33;            // steps from which it does: below, most of a tile would be empty
 constexpr float kLog2e = 1.4426950408889634f;
@@ -349,7 +354,8 @@ __device__ __forceinline__ Tile take_tile(const Params<T>& a, bool down, Shared<
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(FW * 32, FCTAS) forward_kernel(const __grid_constant__ Params<T> a) {
+__global__ void __launch_bounds__(Shape<V>::FW * 32, Shape<V>::FCTAS) forward_kernel(const __grid_constant__ Params<T> a) {
+    constexpr int FL = Shape<V>::FL, FW = Shape<V>::FW;
     __shared__ Shared<V, FW, false> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Tile t = take_tile(a, false, sh);
@@ -439,7 +445,8 @@ __device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, F<V> a, F<V> r, F<V> i
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(BW * 32, BCTAS) backward_kernel(const __grid_constant__ Params<T> a) {
+__global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_kernel(const __grid_constant__ Params<T> a) {
+    constexpr int BL = Shape<V>::BL, BW = Shape<V>::BW;
     __shared__ Shared<V, BW, true> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Tile t = take_tile(a, true, sh);
@@ -694,8 +701,9 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
 }
 
 template <typename T>
-__global__ void __launch_bounds__(QW * 32, QCTAS) backward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
-    constexpr int V = 4 / sizeof(T);
+__global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeof(T)>::QCTAS)
+    backward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
+    constexpr int V = 4 / sizeof(T), QL = Shape<V>::QL, QW = Shape<V>::QW;
     using P = Pipe<4, 3, QSTAGES>;
     using W = Word<T, V>;
     constexpr int STREAM = P::STREAM / 4;
@@ -970,8 +978,11 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
                 make_map<T>(&m.out[1], a, a->ddecay, whole, C) && make_map<T>(&m.out[2], a, a->dgate, whole, C);
     else
         piped = piped && make_map<T>(&m.out[0], a, a->out, whole, C);
-    const int per = bwd ? BL : FL;
-    const int warps = p.tiles > 1 ? (bwd ? BW : FW) : (a->steps + per - 1) / per;  // a short axis: as many as it has work for
+    using One = Shape<1>;
+    using Two = Shape<2>;
+    using Word = Shape<4 / sizeof(T)>;
+    const int per = pairs ? (bwd ? Two::BL : Two::FL) : (bwd ? One::BL : One::FL);
+    const int warps = (int)((p.tiles > 1 ? TILE : a->steps) + per - 1) / per;  // a short axis: as many as it has work for
     auto go = [&](auto* kernel) {
         kernel<<<(unsigned)ctas, warps * 32, 0, s>>>(p);
         return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
@@ -984,7 +995,7 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     };
     int rc;
     if (piped) {
-        rc = bwd ? go_piped(backward_tma_kernel<T>, Pipe<4, 3, QSTAGES>::bytes, QW * 32, QCTAS)
+        rc = bwd ? go_piped(backward_tma_kernel<T>, Pipe<4, 3, QSTAGES>::bytes, Word::QW * 32, Word::QCTAS)
                  : go_piped(forward_tma_kernel<T>, Pipe<3, 1, PSTAGES>::bytes, PW * 32, PCTAS);
     } else if constexpr (sizeof(T) == 2) {
         if (pairs) rc = bwd ? go(backward_kernel<T, 2>) : go(forward_kernel<T, 2>);
