@@ -11,7 +11,10 @@
 //        so that the gradients see one rounding between the products, dG's and dU's own (with G and U in bfloat16 they were 1.8
 //        times as far from the exact ones as a single rounding leaves them, so 1.35 times). Keeping them spares the backward a
 //        third of its products.
-//   OUT  all gradients' tiles in one launch: dX (K runs over both pairs), dWg and dWu.
+//   OUT  all gradients' tiles in one launch: dX (K runs over both pairs), dWg and dWu, neighbours at the same time. Where the tiles
+//        are few for the SMs (8,192 rows, 1,024 x 4,096: 512 tiles, 3.46 for each) the last of them are one line of k blocks,
+//        cut into equal pieces: a tile across a cut is added up from float32 pieces afterwards, in order (233 -> 208 us, and
+//        11 for the sums). Where they are many but of two lengths of K, the longer ones go first and the others fill in.
 // dG and dU are formed by one pass over dH, G and U in between.
 // Operands are bfloat16. float32 inputs are split into three bfloat16 planes (8 bits each) and a product runs over the six pairs
 // of planes that matter (2^-24), smallest first; every 128 of K the sum leaves the tensor core's accumulator, which truncates at
@@ -66,24 +69,93 @@ __device__ __forceinline__ void act_grad(float g, int kind, float* act, float* s
 
 // ---- the GEMM -------------------------------------------------------------------------------------------------
 
-// C (m, n) = the sum over pairs of A (m, k) B (n, k)^T, in tiles and K splits.
+// C (m, n) = the sum over pairs of A (m, k) B (n, k)^T, in tiles.
 struct Job {
-    int m, n, k;
-    int tiles_m, tiles_n, splits, blocks;  // k blocks of 64 a split, of every pair
-    long units;
+    int m, n;
+    int tiles_m, tiles_n, blocks;          // k blocks of 64
+    int left, weight;                      // OUT: the last `left` tiles are on the line, `weight` a k block
     int pairs;
     signed char ia[12], ib[12], mb[12];    // A's plane, B's plane, B's map
     void* out;
-    float* acc;                            // splits > 1: (splits, m, n) float32 partials
 };
 
 struct Gemm {
     Job job[3];   // FWD: one; OUT: dX (A K-major), dWg, dWu (A MN-major)
+    int ctas;
+    int job0[2];         // two lists of tiles, each from this job on: first one, then the other,
+    long whole[2];       // so many whole tiles of each;
+    int start, extra;    // in between, the CTAs from `start` on take `extra` tiles each of the second
+    long line;    // the tiles on it, by weight
+    float* slots; // two pieces a CTA of 128 x BN: the one that its share of the line starts with, and the one it ends with
     int run;      // k blocks in one accumulator
     int act;
     void* kept;   // FWD: the projections, or null
     long plane;   // bytes from one plane of it to the next
     int* status;
+};
+
+// A job's tiles that are not on the line.
+__host__ __device__ inline long whole_of(const Job& j) { return (long)j.tiles_m * j.tiles_n - j.left; }
+// Where CTA b's share of the line starts.
+__host__ __device__ inline long cut(const Gemm& a, int b) { return a.line * b / a.ctas; }
+
+// A tile, or the k blocks [k0, k1) of one: slot < 0 where it is whole.
+struct Unit {
+    int job, tm, tn, k0, k1, slot;
+};
+
+// What a CTA computes, in the order that all of its roles follow.
+template <int EPI>
+struct Walk {
+    int phase = 0, round = 0;
+    long at = -1;
+
+    __device__ __forceinline__ Unit tile(const Gemm& a, int job, long t, int k0, int k1, int slot) const {
+        const Job& j = a.job[job];
+        Unit r;
+        r.job = job, r.k0 = k0, r.k1 = k1, r.slot = slot;
+        // neighbours share the larger operand's rows: a gradient's dG or dU, the weights
+        if (EPI == OUT) r.tn = (int)(t % j.tiles_n), r.tm = (int)(t / j.tiles_n);
+        else r.tm = (int)(t % j.tiles_m), r.tn = (int)(t / j.tiles_m);
+        return r;
+    }
+    __device__ __forceinline__ bool next(const Gemm& a, Unit* r) {
+        const int b = blockIdx.x;
+        for (; phase < (EPI == OUT ? 3 : 1); ++phase, round = 0) {
+            long t = (long)round * a.ctas + b;
+            if (phase == 1) {
+                if (round >= a.extra || b < a.start) continue;
+                t = (long)round * (a.ctas - a.start) + b - a.start;
+            } else if (phase == 2) {
+                t += (long)a.extra * (a.ctas - a.start);
+            }
+            const int list = phase > 0;
+            if (t >= a.whole[list]) continue;
+            ++round;
+            int job = a.job0[list];
+            if (EPI == OUT)
+                while (t >= whole_of(a.job[job])) t -= whole_of(a.job[job]), ++job;
+            *r = tile(a, job, t, 0, a.job[job].blocks, -1);
+            return true;
+        }
+        if (EPI != OUT) return false;
+        if (at < 0) at = cut(a, b);
+        const long end = cut(a, b + 1);
+        while (at < end) {
+            long pos = at;
+            int k = 0;
+            while (pos >= (long)a.job[k].left * a.job[k].blocks * a.job[k].weight) pos -= (long)a.job[k].left * a.job[k].blocks * a.job[k].weight, ++k;
+            const Job& j = a.job[k];
+            const long cost = (long)j.blocks * j.weight, i = pos / cost, within = pos - i * cost;
+            const long stop = at - within + cost < end ? at - within + cost : end;
+            const int k0 = (int)(within / j.weight), k1 = stop == at - within + cost ? j.blocks : (int)((stop - at + within) / j.weight);
+            at = stop;
+            if (k0 >= k1) continue;
+            *r = tile(a, k, whole_of(j) + i, k0, k1, k0 == 0 && k1 == j.blocks ? -1 : 2 * b + (k0 == 0));
+            return true;
+        }
+        return false;
+    }
 };
 
 struct Maps {
@@ -217,34 +289,14 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     __syncthreads();
     fence_after();
     const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
-    const long units = a.job[0].units + (EPI == OUT ? a.job[1].units + a.job[2].units : 0);
-
-    struct Unit {
-        int job, tm, tn, sp, k0, k1;
-    };
-    auto unit = [&](long u) {
-        Unit r;
-        r.job = 0;
-        if (EPI == OUT)
-            while (u >= a.job[r.job].units) u -= a.job[r.job++].units;
-        const Job& j = a.job[r.job];
-        const long per = (long)j.tiles_m * j.tiles_n;
-        r.sp = (int)(u / per);
-        const long t = u - r.sp * per;
-        // neighbours share the larger operand's rows: a gradient's dG or dU, the weights
-        if (EPI == OUT) r.tn = (int)(t % j.tiles_n), r.tm = (int)(t / j.tiles_n);
-        else r.tm = (int)(t % j.tiles_m), r.tn = (int)(t / j.tiles_m);
-        r.k0 = r.sp * j.blocks;
-        r.k1 = min(r.k0 + j.blocks, (j.k + BK - 1) / BK);
-        return r;
-    };
+    Walk<EPI> walk;
+    Unit r;
 
     if (warp == 0) {
         if (lane == 0) {
             long it = 0;
             bool ok = true;
-            for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const Unit r = unit(u);
+            while (ok && walk.next(a, &r)) {
                 const Job& j = a.job[r.job];
                 const bool amn = EPI == OUT && r.job > 0;
                 for (int from = r.k0; ok && from < r.k1; from += a.run) {
@@ -280,8 +332,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
         uint32_t ph = 0;
         long tile = 0;
         bool ok = true;
-        for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            const Unit r = unit(u);
+        while (ok && walk.next(a, &r)) {
             const bool amn = EPI == OUT && r.job > 0;
             const int pairs = a.job[r.job].pairs;
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((amn ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) |
@@ -320,8 +371,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
         uint32_t* share = reinterpret_cast<uint32_t*>(tiles + S * TL::STAGE + (warp - 2) * TL::SHARE);
         long tile = 0;
         bool ok = true;
-        for (long u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            const Unit r = unit(u);
+        while (ok && walk.next(a, &r)) {
             const Job& job = a.job[r.job];
             const int row0 = r.tm * BM + quarter * 32;
             float s0[SUM ? 32 : 1], s1[SUM ? 32 : 1];  // float32: the runs' sums
@@ -349,7 +399,7 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                 auto close_out = [&](int c, const float v[32]) {
                     const int col = r.tn * BN + c, w = min(32, job.n - col);
                     if (left <= 0 || w <= 0) return;
-                    if (job.acc) store_results<float>(job.acc, (long)r.sp * job.m + row0, left, job.n, col, w, v, share, lane);
+                    if (r.slot >= 0) store_results<float>(a.slots + (long)r.slot * BM * BN, quarter * 32, 32, BN, c, 32, v, share, lane);
                     else store_results<T>(job.out, row0, left, job.n, col, w, v, share, lane);
                 };
                 if constexpr (EPI == FWD) {
@@ -509,36 +559,56 @@ __global__ void __launch_bounds__(256) operand_kernel(const __grid_constant__ Gr
     }
 }
 
-// A gradient from its float32 partials, summed in order and rounded once.
-struct Reduce {
-    const float* acc;
-    void* out;
-    int splits;
-    long count;  // of four elements
-};
-struct Reduces {
-    Reduce r[3];
-};
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Reduces a) {
-    constexpr int W = VEC ? 4 : 1;
-    const long total = a.r[0].count + a.r[1].count + a.r[2].count;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        long i = e;
-        int k = 0;
-        while (i >= a.r[k].count) i -= a.r[k++].count;
-        const Reduce& r = a.r[k];
-        float s[W];
-        Vec<float, VEC>::load(r.acc + i * W, s);
-        for (int p = 1; p < r.splits; ++p) {
-            float v[W];
-            Vec<float, VEC>::load(r.acc + (p * r.count + i) * W, v);
-#pragma unroll
-            for (int j = 0; j < W; ++j) s[j] += v[j];
+// The tiles of the line that are in pieces: their sum in the order of K, rounded once. Eight CTAs a tile, 16 rows each.
+template <typename T, int BN>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Gemm a) {
+    __shared__ int piece[SMS], pieces;
+    int i = blockIdx.x / 8, k = 0;
+    if (threadIdx.x == 0) {
+        long start = 0;
+        int left = i;
+        for (; left >= a.job[k].left; ++k) left -= a.job[k].left, start += (long)a.job[k].left * a.job[k].blocks * a.job[k].weight;
+        const Job& j = a.job[k];
+        const long cost = (long)j.blocks * j.weight;
+        start += left * cost;
+        int b = (int)(start * a.ctas / a.line), n = 0;
+        while (cut(a, b + 1) <= start) ++b;
+        while (cut(a, b) > start) --b;
+        for (long from = cut(a, b); from < start + cost; ++b) {
+            const long to = cut(a, b + 1);
+            const int k0 = from > start ? (int)((from - start) / j.weight) : 0, k1 = to >= start + cost ? j.blocks : (int)((to - start) / j.weight);
+            from = to;
+            if (k0 >= k1) continue;
+            if (k0 > 0 || k1 < j.blocks) piece[n++] = 2 * b + (k0 == 0);
         }
-        T* o = static_cast<T*>(r.out) + i * W;
-        if constexpr (VEC && sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
-        else Vec<T, VEC>::store(o, s);
+        pieces = n;  // none: the tile is whole
+    }
+    __syncthreads();
+    if (pieces == 0) return;
+    for (k = 0; i >= a.job[k].left; ++k) i -= a.job[k].left;
+    const Job& j = a.job[k];
+    const int t = j.tiles_m * j.tiles_n - j.left + i, row0 = (blockIdx.x & 7) * 16, tn = t % j.tiles_n, tm = t / j.tiles_n;
+    const bool vec = j.n % 4 == 0 && ((uintptr_t)j.out & 15u) == 0;
+    for (int e = threadIdx.x; e < 16 * BN / 4; e += 256) {
+        const int r = row0 + e / (BN / 4), c = e % (BN / 4) * 4, row = tm * BM + r, col = tn * BN + c;
+        if (row >= j.m || col >= j.n) continue;
+        float s[4];
+        Vec<float, true>::load(a.slots + ((long)piece[0] * BM + r) * BN + c, s);
+        for (int p = 1; p < pieces; ++p) {
+            float v[4];
+            Vec<float, true>::load(a.slots + ((long)piece[p] * BM + r) * BN + c, v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] += v[q];
+        }
+        T* o = static_cast<T*>(j.out) + (long)row * j.n + col;
+        if (vec) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+            else Vec<float, true>::store(o, s);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (col + q < j.n) o[q] = from_f<T>(s[q]);
+        }
     }
 }
 
@@ -739,8 +809,7 @@ struct Operand {
     int planes;
 };
 
-bool make_map(CUtensorMap* map, const Operand& o, int box_rows) {
-    EncodeFn enc = encoder();
+bool make_map(EncodeFn enc, CUtensorMap* map, const Operand& o, int box_rows) {
     if (!enc) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
     const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld * o.rows) * 2};
@@ -780,8 +849,9 @@ struct Plan {
     int planes;
     long ldd, ldf;
     Source x, wg, wu;
-    size_t dgu, acc[3], bytes;
-    int bn, splits[3];
+    size_t dgu, slots, bytes;
+    int bn;
+    Gemm gemm;  // its shares; the backward's tiles
 };
 
 bool readable(const ews_gated_args* a, const void* p, int64_t stride) {
@@ -798,33 +868,62 @@ int forward_bn(const ews_gated_args* a) {
     return 64;
 }
 
-Job job_of(long m, long n, long k, int bn, int splits) {
+Job job_of(long m, long n, long k, int bn, int pairs) {
     Job j{};
-    j.m = (int)m, j.n = (int)n, j.k = (int)k, j.splits = splits;
-    j.tiles_m = (int)((m + BM - 1) / BM), j.tiles_n = (int)((n + bn - 1) / bn);
-    j.blocks = (int)(((k + BK - 1) / BK + splits - 1) / splits);
-    j.splits = (int)(((k + BK - 1) / BK + j.blocks - 1) / j.blocks);  // none empty
-    j.units = (long)j.tiles_m * j.tiles_n * j.splits;
+    j.m = (int)m, j.n = (int)n;
+    j.tiles_m = (int)((m + BM - 1) / BM), j.tiles_n = (int)((n + bn - 1) / bn), j.blocks = (int)((k + BK - 1) / BK);
+    j.pairs = pairs, j.weight = 1;
     return j;
 }
 
-// Splits of K so that the gradients' units, weighed by their K, fill the SMs: none below eight k blocks.
-void pick_splits(Plan* p, const ews_gated_args* a, const bool want[3]) {
-    const long m[3] = {a->rows, a->inner, a->inner}, k[3] = {2 * a->inner, a->rows, a->rows};
-    long tiles[3];
-    double work = 0;
-    for (int j = 0; j < 3; ++j) {
-        tiles[j] = want[j] ? ((m[j] + BM - 1) / BM) * ((a->dim + p->bn - 1) / p->bn) : 0;
-        work += (double)tiles[j] * k[j];
+// The gradients' tiles among the CTAs: as many of these as keep eight steps of 64 of K each busy.
+void share_out(Gemm* g) {
+    long steps = 0, tiles[3], cost[3];
+    for (int k = 0; k < 3; ++k) {
+        const Job& j = g->job[k];
+        tiles[k] = (long)j.tiles_m * j.tiles_n, cost[k] = (long)j.blocks * j.pairs;
+        steps += tiles[k] * cost[k];
     }
-    for (int j = 0; j < 3; ++j) {
-        p->splits[j] = 1;
-        if (!want[j]) continue;
-        const double share = work / SMS;  // of an SM
-        const long blocks = (k[j] / (j ? 1 : 2) + BK - 1) / BK;
-        long s = (long)(k[j] / share);    // a unit longer than an SM's share holds the launch up
-        if (s > blocks / 8) s = blocks / 8;
-        if (s > 1) p->splits[j] = job_of(m[j], a->dim, k[j] / (j ? 1 : 2), p->bn, (int)s).splits;
+    g->ctas = (int)(steps / 8 < 1 ? 1 : steps / 8 < SMS ? steps / 8 : SMS);
+    const long costw = cost[1] ? cost[1] : cost[2];  // of a weight gradient's tile
+    const bool two = cost[0] && costw && (cost[0] > 1.05 * costw || costw > 1.05 * cost[0]);
+    const long least = !costw || (cost[0] && cost[0] < costw) ? cost[0] : costw, share = steps / g->ctas;
+    // The list of the longer tiles first. One length: one list.
+    const bool swap = two && costw > cost[0];
+    g->job0[0] = swap ? 1 : 0, g->job0[1] = swap ? 0 : two ? 1 : 3;
+    const long n[2] = {two ? (swap ? tiles[1] + tiles[2] : tiles[0]) : tiles[0] + tiles[1] + tiles[2], two ? (swap ? tiles[0] : tiles[1] + tiles[2]) : 0};
+    g->whole[0] = n[0], g->whole[1] = n[1];
+    // Whole tiles alone, if that keeps the SMs within a twenty-fifth of even. (4,001 rows, 2,048 x 8,192, even to 1.3%: 477 us for
+    // both passes so, 503 with a line; 8,192 rows, 2,048 x 5,632, 10% off: 704 and 673.)
+    const long longer = swap ? costw : cost[0] ? cost[0] : costw;
+    if (two) {
+        g->start = (int)(n[0] % g->ctas);
+        if (g->start) g->extra = (int)(longer / least);
+    }
+    long most = 0;
+    for (int b = 0; b < g->ctas; ++b) {
+        auto count = [&](long total) { return total > b ? (total - b + g->ctas - 1) / g->ctas : 0; };
+        long load = count(n[0]) * longer;
+        if (two) {
+            const long early = (long)g->extra * (g->ctas - g->start), here = b - g->start;
+            if (here >= 0 && g->extra) load += least * (n[1] >= early ? g->extra : n[1] > here ? (n[1] - here + g->ctas - g->start - 1) / (g->ctas - g->start) : 0);
+            load += least * count(n[1] - early);
+        }
+        if (load > most) most = load;
+    }
+    if (most <= 1.04 * share) return;
+    g->start = g->extra = 0;
+    const int base = g->job[1].pairs ? g->job[1].pairs : g->job[2].pairs ? g->job[2].pairs : g->job[0].pairs;
+    for (int l = 0; l < 2; ++l) {
+        long whole = g->whole[l] = n[l] / g->ctas * g->ctas;
+        const int from = g->job0[l], to = l == 1 || !two ? (from == 0 && two ? 1 : 3) : (from == 0 ? 1 : 3);
+        for (int k = from; k < to; ++k) {
+            Job& j = g->job[k];
+            const long kept = tiles[k] < whole ? tiles[k] : whole;
+            whole -= kept;
+            j.left = (int)(tiles[k] - kept), j.weight = j.pairs > base ? j.pairs / base : 1;
+            g->line += (long)j.left * j.blocks * j.weight;
+        }
     }
 }
 
@@ -850,12 +949,14 @@ Plan plan(const ews_gated_args* a, bool bwd) {
     if (!bwd) {
         p.bn = forward_bn(a);
     } else {
-        const bool want[3] = {a->dx != nullptr, a->dw_gate != nullptr, a->dw_up != nullptr};
         p.bn = p.planes > 1 || a->dim <= 128 ? 128 : 256;
-        pick_splits(&p, a, want);
+        const int products = p.planes == 1 ? 1 : 6;
+        if (a->dx) p.gemm.job[0] = job_of(a->rows, a->dim, a->inner, p.bn, 2 * products);
+        if (a->dw_gate) p.gemm.job[1] = job_of(a->inner, a->dim, a->rows, p.bn, products);
+        if (a->dw_up) p.gemm.job[2] = job_of(a->inner, a->dim, a->rows, p.bn, products);
+        share_out(&p.gemm);
         p.dgu = take(sizeof(bf16) * 2 * (size_t)p.planes * a->rows * p.ldf);
-        for (int j = 0; j < 3; ++j)
-            if (p.splits[j] > 1) p.acc[j] = take(sizeof(float) * (size_t)p.splits[j] * (j ? a->inner : a->rows) * a->dim);
+        if (p.gemm.line) p.slots = take(sizeof(float) * 2 * (size_t)p.gemm.ctas * BM * p.bn);
     }
     p.bytes = at;
     return p;
@@ -872,8 +973,10 @@ template <typename T, int EPI, int BN>
 int gemm(const Maps& maps, const Gemm& g, cudaStream_t s) {
     auto* kern = gemm_kernel<T, EPI, BN>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
-    const long units = g.job[0].units + g.job[1].units + g.job[2].units;
-    kern<<<(unsigned)(units < SMS ? units : SMS), NTH, Tile<BN>::bytes, s>>>(maps, g);
+    kern<<<(unsigned)g.ctas, NTH, Tile<BN>::bytes, s>>>(maps, g);
+    const int left = g.job[0].left + g.job[1].left + g.job[2].left;
+    if constexpr (EPI == OUT)
+        if (left) join_kernel<T, BN><<<(unsigned)left * 8, 256, 0, s>>>(g);
     return launched();
 }
 
@@ -925,8 +1028,9 @@ int forward_few(const ews_gated_args* a, cudaStream_t s) {
 
 template <int BN>
 int run_served(const ews_gated_args* a, const Operand& x, const Operand& wg, const Operand& wu, cudaStream_t s) {
+    const EncodeFn enc = encoder();
     CUtensorMap mx, mg, mu;
-    if (!make_map(&mx, x, BN) || !make_map(&mg, wg, 64) || !make_map(&mu, wu, 64)) return EWS_ERR_LAUNCH;
+    if (!make_map(enc, &mx, x, BN) || !make_map(enc, &mg, wg, 64) || !make_map(enc, &mu, wu, 64)) return EWS_ERR_LAUNCH;
     const unsigned grid = (unsigned)((a->inner + 63) / 64);
     const Served v{(int)a->rows, (int)a->inner, a->activation, (int)((a->dim + BK - 1) / BK), grid <= SMS ? 8 : 4,
                    static_cast<bf16*>(a->out), a->kept, kept_plane(a), a->status};
@@ -952,12 +1056,15 @@ int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
             return a->rows <= 32 ? run_served<32>(a, x, wg, wu, s) : run_served<64>(a, x, wg, wu, s);
         }
     }
+    const EncodeFn enc = encoder();
     Maps m{};
-    if (!make_map(&m.a[0], x, BM) || !make_map(&m.b[0], wg, p.bn / 2) || !make_map(&m.b[1], wu, p.bn / 2)) return EWS_ERR_LAUNCH;
+    if (!make_map(enc, &m.a[0], x, BM) || !make_map(enc, &m.b[0], wg, p.bn / 2) || !make_map(enc, &m.b[1], wu, p.bn / 2)) return EWS_ERR_LAUNCH;
     Gemm g{};
-    g.job[0] = job_of(a->rows, a->inner, a->dim, p.bn / 2, 1);
+    g.job[0] = job_of(a->rows, a->inner, a->dim, p.bn / 2, p.planes == 1 ? 1 : 6);
     Job& j = g.job[0];
-    j.out = a->out, j.pairs = p.planes == 1 ? 1 : 6;
+    const long tiles = (long)j.tiles_m * j.tiles_n;
+    g.ctas = (int)(tiles < SMS ? tiles : SMS);
+    j.out = a->out, g.whole[0] = tiles;
     for (int i = 0; i < j.pairs; ++i) j.ia[i] = p.planes == 1 ? 0 : kPlaneA[i], j.ib[i] = p.planes == 1 ? 0 : kPlaneB[i];
     g.run = p.planes > 1 ? kRun : 1 << 28;
     g.act = a->activation, g.kept = a->kept, g.plane = kept_plane(a), g.status = a->status;
@@ -979,47 +1086,31 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, grad, s);
     if (rc != EWS_OK) return rc;
     d.p = dgu, d.rows = a->rows, d.cols = d.ld = p.ldf, d.plane = a->rows * p.ldf, d.planes = 2 * p.planes;
+    const EncodeFn enc = encoder();
     Maps m{};
-    if (!make_map(&m.a[0], d, BM) || !make_map(&m.a[1], d, 64)) return EWS_ERR_LAUNCH;
-    if (a->dx && (!make_map(&m.b[0], wg, 64) || !make_map(&m.b[1], wu, 64))) return EWS_ERR_LAUNCH;
-    if (dw && !make_map(&m.b[2], x, 64)) return EWS_ERR_LAUNCH;
-    Gemm g{};
+    if (!make_map(enc, &m.a[0], d, BM) || !make_map(enc, &m.a[1], d, 64)) return EWS_ERR_LAUNCH;
+    if (a->dx && (!make_map(enc, &m.b[0], wg, 64) || !make_map(enc, &m.b[1], wu, 64))) return EWS_ERR_LAUNCH;
+    if (dw && !make_map(enc, &m.b[2], x, 64)) return EWS_ERR_LAUNCH;
+    Gemm g = p.gemm;
     g.run = p.planes > 1 ? kRun : 1 << 28;
     g.status = a->status;
+    g.slots = reinterpret_cast<float*>(w + p.slots);
     void* out[3] = {a->dx, a->dw_gate, a->dw_up};
     const int products = p.planes == 1 ? 1 : 6;
-    Reduces red{};
-    long total = 0;
-    bool vec = a->dim % 4 == 0;
     for (int k = 0; k < 3; ++k) {
-        if (!out[k]) continue;
         Job& j = g.job[k];
-        j = k ? job_of(a->inner, a->dim, a->rows, p.bn, p.splits[k]) : job_of(a->rows, a->dim, a->inner, p.bn, p.splits[k]);
         j.out = out[k];
-        for (int i = 0; i < products; ++i)  // the smallest of both sides first
-            for (int side = 0; side < (k ? 1 : 2); ++side) {
+        int at = 0;
+        for (int i = 0; j.pairs && i < products; ++i)  // the smallest of both sides first
+            for (int side = 0; side < (k ? 1 : 2); ++side, ++at) {
                 const int which = k ? k - 1 : side;  // dG or dU
-                j.ia[j.pairs] = (signed char)(which * p.planes + (products == 1 ? 0 : kPlaneA[i]));
-                j.ib[j.pairs] = products == 1 ? 0 : kPlaneB[i];
-                j.mb[j.pairs++] = (signed char)(k ? 2 : side);
+                j.ia[at] = (signed char)(which * p.planes + (products == 1 ? 0 : kPlaneA[i]));
+                j.ib[at] = products == 1 ? 0 : kPlaneB[i];
+                j.mb[at] = (signed char)(k ? 2 : side);
             }
-        if (j.splits > 1) {
-            j.acc = reinterpret_cast<float*>(w + p.acc[k]);
-            red.r[k] = Reduce{j.acc, out[k], j.splits, (long)j.m * j.n};
-            total += red.r[k].count;
-            vec = vec && aligned16(out[k]);
-        }
     }
-    if constexpr (sizeof(T) == 4) rc = gemm<T, OUT, 128>(m, g, s);
-    else rc = p.bn == 256 ? gemm<T, OUT, 256>(m, g, s) : gemm<T, OUT, 128>(m, g, s);
-    if (rc != EWS_OK || total == 0) return rc;
-    if (vec) {
-        for (Reduce& r : red.r) r.count /= 4;
-        reduce_kernel<T, true><<<grid_of(total / 4), 256, 0, s>>>(red);
-    } else {
-        reduce_kernel<T, false><<<grid_of(total), 256, 0, s>>>(red);
-    }
-    return launched();
+    if constexpr (sizeof(T) == 4) return gemm<T, OUT, 128>(m, g, s);
+    else return p.bn == 256 ? gemm<T, OUT, 256>(m, g, s) : gemm<T, OUT, 128>(m, g, s);
 }
 
 }  // namespace gated
