@@ -13,7 +13,7 @@ import torch
 
 from . import _lib, engine
 from .engine import first_order
-from .token_ops import _DTYPES, _addr, _device, _dtype, _launch, _work
+from .token_ops import _DTYPES, _addr, _device, _dtype, _launch, _operand, _work
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 _GATED = struct.Struct("@3q2i3P3q3Pq4PNP").pack  # ews_gated_args
@@ -30,17 +30,6 @@ def _size(rows, dim, inner, code, strides, at, wanted, backward):
 @functools.lru_cache(maxsize=256)
 def _kept_size(rows, dim, inner, code):
     return _lib.load().ews_gated_kept_size(_GATED(rows, dim, inner, code, 0, 0, 0, 0, dim, dim, dim, *([0] * 10)))
-
-
-def _operand(t):
-    """A matrix with contiguous rows, and how far apart they are."""
-    rows, dim = t.shape
-    stride, one = t.stride()
-    if rows <= 1:
-        stride = dim
-    if one != 1 and dim > 1 or stride < dim:
-        return t.contiguous(), dim
-    return t, stride
 
 
 def _forward(x, wg, wu, act, shape, keep):

@@ -410,54 +410,59 @@ def _distill_size(rows: int, vocab: int, dim: int, code: int, hidden_stride: int
     return _lib.load().ews_distill_work_size(args + _TOP(0, 0, 0, top, _lib.EWS_DTYPE_F32, 1.0, 0), backward)
 
 
-def _distill_args(hidden, weight, ids, logits, top, inv_tau, entries, loss=None, lse=None, plan=None, dloss=None, dh=None, dw=None,
-                  work=None):
-    rows, dim = hidden.shape
-    return _VOCAB(rows, weight.shape[0], dim, _DTYPES[hidden.dtype], 0, hidden.data_ptr(), weight.data_ptr(), 0, _row_stride(hidden),
-                  _row_stride(weight), 0, _addr(loss), _addr(lse), _addr(plan), _addr(dloss), _addr(dh), _addr(dw), _addr(work),
-                  0 if work is None else work.numel(), engine.index_word(hidden.get_device())[0]) + _TOP(
-                      _addr(ids), _addr(logits), 0 if ids is None else _WIDE[ids.dtype], top,
-                      _lib.EWS_DTYPE_F32 if logits is None else _DTYPES[logits.dtype], inv_tau, entries.data_ptr())
-
-
-def _distill_work(hidden, weight, top, backward):
-    return _work(_distill_size(*hidden.shape[:1], *weight.shape, _DTYPES[hidden.dtype], _row_stride(hidden), _row_stride(weight),
-                               weight.data_ptr() % 16, top, backward), hidden)
+def _operand(t):
+    """A matrix with contiguous rows, and how far apart they are."""
+    rows, dim = t.shape
+    stride, one = t.stride()
+    if rows <= 1:
+        stride = dim
+    if one != 1 and dim > 1 or stride < dim:
+        return t.contiguous(), dim
+    return t, stride
 
 
 def _distill(hidden, weight, ids, logits, inv_tau, shape):
-    lib = _lib.load()
-    rows, top = hidden.shape[0], ids.shape[1]
-    loss = torch.empty(shape, dtype=torch.float32, device=hidden.device)  # of its own memory, as vocab_loss's
-    lse = torch.empty(rows, dtype=torch.float32, device=hidden.device)
-    plan = torch.empty(3 * rows + 4, dtype=torch.int32, device=hidden.device)
-    entries = torch.empty(2 * rows * (top + 1), dtype=torch.int32, device=hidden.device)
-    work = _distill_work(hidden, weight, top, 0)
-    args = _distill_args(hidden, weight, ids, logits, top, inv_tau, entries, loss, lse, plan, work=work)
-    _launch(hidden.get_device(), "ews_distill_fwd", rows, lib.ews_distill_fwd, args)
-    return loss, lse, plan, entries
+    """The loss on operands, and what its backward needs: logsumexps, row plan and entries, in one block."""
+    (h, hs), (w, ws) = hidden, weight
+    (rows, dim), vocab, top, device = h.shape, w.shape[0], ids.shape[1], h.device
+    loss = torch.empty(shape, dtype=torch.float32, device=device)  # of its own memory, as vocab_loss's
+    kept = torch.empty(rows * (2 * top + 6) + 4, dtype=torch.int32, device=device)
+    code, wp, lse = _DTYPES[h.dtype], w.data_ptr(), kept.data_ptr()
+    size = _distill_size(rows, vocab, dim, code, hs, ws, wp % 16, top, 0)
+    work = _work(size, h)
+    idx = h.get_device()
+    args = _VOCAB(rows, vocab, dim, code, 0, h.data_ptr(), wp, 0, hs, ws, 0, loss.data_ptr(), lse, lse + 4 * rows, 0, 0, 0, _addr(work), size,
+                  engine.index_word(idx)[0]) + _TOP(ids.data_ptr(), logits.data_ptr(), _WIDE[ids.dtype], top, _DTYPES[logits.dtype],
+                                                    inv_tau, lse + 16 * rows + 16)
+    _launch(idx, "ews_distill_fwd", rows, _lib.load().ews_distill_fwd, args)
+    return loss, kept
 
 
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, ids, logits, inv_tau, shape):
-        hidden, weight = _rows(hidden), _rows(weight)
-        loss, lse, plan, entries = _distill(hidden, weight, ids, logits, inv_tau, shape)
-        ctx.meta = inv_tau, ids.shape[1]
-        ctx.save_for_backward(hidden, weight, lse, plan, entries)
+        hidden, weight = _operand(hidden), _operand(weight)
+        loss, kept = _distill(hidden, weight, ids, logits, inv_tau, shape)
+        ctx.meta = inv_tau, ids.shape[1], hidden[1], weight[1]
+        ctx.save_for_backward(hidden[0], weight[0], kept)
         return loss
 
     @staticmethod
     @first_order
     def backward(ctx, dloss):
-        hidden, weight, lse, plan, entries = ctx.saved_tensors
-        inv_tau, top = ctx.meta
+        h, w, kept = ctx.saved_tensors
+        inv_tau, top, hs, ws = ctx.meta
+        (rows, dim), vocab, code = h.shape, w.shape[0], _DTYPES[h.dtype]
         dloss = dloss.contiguous()
         dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
-                  for t, need in ((hidden, ctx.needs_input_grad[0]), (weight, ctx.needs_input_grad[1])))
-        work = _distill_work(hidden, weight, top, 1)
-        args = _distill_args(hidden, weight, None, None, top, inv_tau, entries, None, lse, plan, dloss, dh, dw, work)
-        _launch(hidden.get_device(), "ews_distill_bwd", hidden.shape[0], _lib.load().ews_distill_bwd, args)
+                  for t, need in ((h, ctx.needs_input_grad[0]), (w, ctx.needs_input_grad[1])))
+        wp, lse = w.data_ptr(), kept.data_ptr()
+        size = _distill_size(rows, vocab, dim, code, hs, ws, wp % 16, top, 1)
+        work = _work(size, h)
+        idx = h.get_device()
+        args = _VOCAB(rows, vocab, dim, code, 0, h.data_ptr(), wp, 0, hs, ws, 0, 0, lse, lse + 4 * rows, dloss.data_ptr(), _addr(dh),
+                      _addr(dw), _addr(work), size, engine.index_word(idx)[0]) + _TOP(0, 0, 0, top, _lib.EWS_DTYPE_F32, inv_tau, lse + 16 * rows + 16)
+        _launch(idx, "ews_distill_bwd", rows, _lib.load().ews_distill_bwd, args)
         return dh, dw, None, None, None, None
 
 
@@ -500,4 +505,4 @@ def distill_loss(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.
     ids, logits = teacher_ids.reshape(-1, top).contiguous(), teacher_logits.detach().reshape(-1, top).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _DistillLoss.apply(flat, weight, ids, logits, 1.0 / temperature, hidden.shape[:-1])
-    return _distill(_rows(flat), _rows(weight), ids, logits, 1.0 / temperature, hidden.shape[:-1])[0]
+    return _distill(_operand(flat), _operand(weight), ids, logits, 1.0 / temperature, hidden.shape[:-1])[0]
