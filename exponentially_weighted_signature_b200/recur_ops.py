@@ -19,15 +19,6 @@ from .token_ops import _DTYPES, _addr, _device, _dtype, _last_contiguous, _launc
 _RECUR = struct.Struct("@4i3P6q3P3PP2qP3P2PPNP").pack  # ews_recur_args
 
 
-def _args(x, decay, gate, rate, lengths=None, initial=None, out=None, end=None, carry=None, dout=None, dend=None,
-          grads=(None, None, None), drate=None, d0=None, work=None):
-    B, T, C = x.shape
-    return _RECUR(B, T, C, _DTYPES[x.dtype], x.data_ptr(), decay.data_ptr(), gate.data_ptr(), *x.stride()[:2], *decay.stride()[:2],
-                  *gate.stride()[:2], rate.data_ptr(), _addr(lengths), _addr(initial), _addr(out), _addr(end), _addr(carry),
-                  _addr(dout), *((0, 0) if dout is None else dout.stride()[:2]), _addr(dend), *map(_addr, grads), _addr(drate),
-                  _addr(d0), _addr(work), 0 if work is None else work.numel(), engine.index_word(x.get_device())[0])
-
-
 @functools.lru_cache(maxsize=256)
 def _sizes(B: int, T: int, C: int, code: int):
     """(carry, forward's and backward's workspace) in bytes: a function of the sizes alone."""
@@ -36,13 +27,17 @@ def _sizes(B: int, T: int, C: int, code: int):
 
 
 def _forward(x, decay, gate, rate, initial, lengths, want_state, want_carry):
-    B, T, C = x.shape
-    carry_bytes, work_bytes, _ = _sizes(B, T, C, _DTYPES[x.dtype])
-    out = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
-    end = torch.empty((B, C), dtype=torch.float32, device=x.device) if want_state else None
-    carry = torch.empty(carry_bytes // 4, dtype=torch.float32, device=x.device) if want_carry else None
-    args = _args(x, decay, gate, rate, lengths, initial, out, end, carry, work=(work := _work(work_bytes, x)))
-    _launch(x.get_device(), "ews_recur_fwd", B * T, _lib.load().ews_recur_fwd, args)
+    (B, T, C), device, code = x.shape, x.device, _DTYPES[x.dtype]
+    carry_bytes, size, _ = _sizes(B, T, C, code)
+    out = torch.empty((B, T, C), dtype=x.dtype, device=device)
+    end = torch.empty((B, C), dtype=torch.float32, device=device) if want_state else None
+    carry = torch.empty(carry_bytes // 4, dtype=torch.float32, device=device) if want_carry else None
+    work = _work(size, x)
+    idx, xs, ds, gs = x.get_device(), x.stride(), decay.stride(), gate.stride()
+    args = _RECUR(B, T, C, code, x.data_ptr(), decay.data_ptr(), gate.data_ptr(), xs[0], xs[1], ds[0], ds[1], gs[0], gs[1], rate.data_ptr(),
+                  _addr(lengths), _addr(initial), out.data_ptr(), _addr(end), _addr(carry), 0, 0, 0, 0, 0, 0, 0, 0, 0, _addr(work), size,
+                  engine.index_word(idx)[0])
+    _launch(idx, "ews_recur_fwd", B * T, _lib.load().ews_recur_fwd, args)
     return out, end, carry
 
 
@@ -59,16 +54,21 @@ class _Recurrence(torch.autograd.Function):
     @first_order
     def backward(ctx, dout, dend):
         x, decay, gate, rate, initial, lengths, carry = ctx.saved_tensors
-        B, T, C = x.shape
+        (B, T, C), device, dtype, code = x.shape, x.device, x.dtype, _DTYPES[x.dtype]
         dout = None if dout is None else _last_contiguous(dout)
         dend = None if dend is None else dend.contiguous()
-        grads = [torch.empty((B, T, C), dtype=x.dtype, device=x.device) for _ in range(3)]
-        drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
-        d0 = torch.empty((B, C), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[4] else None
-        work = _work(_sizes(B, T, C, _DTYPES[x.dtype])[2], x)
-        args = _args(x, decay, gate, rate, lengths, initial, None, None, carry, dout, dend, grads, drate, d0, work)
-        _launch(x.get_device(), "ews_recur_bwd", B * T, _lib.load().ews_recur_bwd, args)
-        return (*grads, drate, d0, None, None)
+        dx, ddecay, dgate = (torch.empty((B, T, C), dtype=dtype, device=device) for _ in range(3))
+        drate = torch.empty(C, dtype=torch.float32, device=device) if ctx.needs_input_grad[3] else None
+        d0 = torch.empty((B, C), dtype=torch.float32, device=device) if ctx.needs_input_grad[4] else None
+        size = _sizes(B, T, C, code)[2]
+        work = _work(size, x)
+        idx, xs, ds, gs = x.get_device(), x.stride(), decay.stride(), gate.stride()
+        os = (0, 0) if dout is None else dout.stride()
+        args = _RECUR(B, T, C, code, x.data_ptr(), decay.data_ptr(), gate.data_ptr(), xs[0], xs[1], ds[0], ds[1], gs[0], gs[1],
+                      rate.data_ptr(), _addr(lengths), _addr(initial), 0, 0, carry.data_ptr(), _addr(dout), os[0], os[1], _addr(dend),
+                      dx.data_ptr(), ddecay.data_ptr(), dgate.data_ptr(), _addr(drate), _addr(d0), _addr(work), size, engine.index_word(idx)[0])
+        _launch(idx, "ews_recur_bwd", B * T, _lib.load().ews_recur_bwd, args)
+        return dx, ddecay, dgate, drate, d0, None, None
 
 
 def _check(x, decay, gate, rate, axes):
