@@ -69,6 +69,19 @@ EXPORTED = (
     "ews_vocab_work_size",
     "ews_vocab_fwd",
     "ews_vocab_bwd",
+    "ews_distill_entries_size",
+    "ews_distill_work_size",
+    "ews_distill_fwd",
+    "ews_distill_bwd",
+    "ews_recur_carry_size",
+    "ews_recur_work_size",
+    "ews_recur_fwd",
+    "ews_recur_bwd",
+    "ews_recur_step",
+    "ews_gated_kept_size",
+    "ews_gated_work_size",
+    "ews_gated_fwd",
+    "ews_gated_bwd",
     "ews_read_device_status",
     "ews_status_fold",
     "ews_error_string",

@@ -893,6 +893,7 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Step<
 
 int check(const ews_recur_args* a) {
     if (!a || a->batch < 0 || a->steps < 0 || a->channels <= 0) return EWS_ERR_INVALID_ARGUMENT;
+    if (a->steps > 1 << 30 || a->channels > 1 << 30) return EWS_ERR_UNSUPPORTED;
     if (a->dtype != EWS_DTYPE_F32 && a->dtype != EWS_DTYPE_BF16) return EWS_ERR_UNSUPPORTED;
     return EWS_OK;
 }
