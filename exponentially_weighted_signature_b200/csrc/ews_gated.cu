@@ -21,7 +21,13 @@
 // every addition, and is added in registers.
 //
 // Few rows (a served batch's tokens) are bound by the weights' bytes: served_kernel takes the weights as the wide operand, 64 rows
-// of both a CTA, and keeps as many of their bytes in flight as fit; few_f32_kernel reads float32 weights as they are, once.
+// of both a CTA, and keeps as many of their bytes in flight as fit; few_f32_kernel multiplies float32 weights as they are.
+//
+// Measured, bfloat16: 4,001 rows, 2,048 x 8,192: 182 us, 1.47 PFLOP/s, against 169 us for the library's product of the same
+// operands without activation and product; 8,192 rows, 1,024 x 4,096: 102 us (97), 124 us where G and U are kept, the backward 298
+// us: 63 to 79 for its operands, 208 for 8 N D F at 1.32 PFLOP/s, 11 to join pieces. What bounds them is the tensor pipe, under the
+// power cap in a long run. 48 rows, 2,048 x 5,632: 18 us (2.6 TB/s), 11,008 x 4,096: 42 us (4.3 TB/s): a CTA's start, first bytes and
+// epilogue beside its share of the weights; one row, 1,024 x 4,096: 8.5 us, the same. float32, 16 rows, 1,024 x 4,096: 20 us.
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -35,9 +41,9 @@ constexpr int EPW = 8;              // epilogue warps
 constexpr int NTH = 64 + EPW * 32;  // and one each for TMA and MMA
 constexpr int SMS = 148;
 constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulator
-// Rows up to which served_kernel runs (100 rows, 4,096 x 1,024: 22 us there, 14 as tiles; 64 rows, 5,632 x 2,048: 21 us), and up to
-// which few_f32_kernel does.
-constexpr int kServed = 64, kFewF32 = 16;
+// Rows up to which served_kernel runs (bfloat16; 64 rows, 4,096 x 1,024: 17 us, 100: 22 us there, 14 as tiles), and up to which
+// few_f32_kernel does (32 rows, 5,632 x 2,048: 88 us there, 109 as tiles of three planes; 64 rows: 139, 111).
+constexpr int kServed = 64, kFewF32 = 32;
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
 
@@ -623,55 +629,106 @@ struct Few {
     long plane;
 };
 
-// float32: a warp has two rows of each weight and runs along K, its lanes on consecutive fours of it (however they are
-// loaded: the sums' order does not depend on the alignment), for R rows of X.
+// float32: a warp has FS rows of each weight and runs along K, its lanes on consecutive fours of it (however they are loaded:
+// the sums' order does not depend on the alignment), for R rows of X (blockIdx.y: which). From eight rows on X comes by way of
+// shared memory, CHUNK of K at a time, and four rows of each weight share what is read of it: with two, and X from the caches,
+// 8 rows took 68 us for 5,632 x 2,048 and 16 took 106, so 31 and 65.
+template <int R>
+struct FewShape {
+    static constexpr int FS = R >= 8 ? 4 : 2, VALUES = 2 * FS * R, CHUNK = 512;
+    static constexpr bool SHARED = R >= 8;
+};
+
 template <int R, bool VEC>
 __global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Few a) {
-    constexpr int W = 4;
+    using S = FewShape<R>;
+    constexpr int FS = S::FS, VALUES = S::VALUES;
+    __shared__ float4 xs[S::SHARED ? R : 1][S::SHARED ? S::CHUNK / 4 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int f = (blockIdx.x * 4 + warp) * 2;
+    const int f0 = (blockIdx.x * 4 + warp) * FS, row0 = blockIdx.y * R, rows = min(a.rows - row0, R);
     auto load = [&](const float* p, int k, float v[4]) {
         if (VEC) return Vec<float, true>::load(p + k, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = k + e < a.dim ? p[k + e] : 0.f;
     };
-    if (f >= a.inner) return;
-    const int f1 = f + 1 < a.inner ? f + 1 : f;
-    const float* w[4] = {a.wg + f * a.gs, a.wg + f1 * a.gs, a.wu + f * a.us, a.wu + f1 * a.us};
-    float acc[4][R];
+    const float* w[2 * FS];  // rows beyond the last: the last
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < FS; ++j) {
+        const long f = min(f0 + j, a.inner - 1);
+        w[2 * j] = a.wg + f * a.gs, w[2 * j + 1] = a.wu + f * a.us;
+    }
+    float acc[VALUES];  // ((f, row), side)
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[j][r] = 0.f;
-#pragma unroll 2
-    for (int k = lane * W; k < a.dim; k += 32 * W) {
-        float wv[4][W];
+    for (int j = 0; j < VALUES; ++j) acc[j] = 0.f;
+    auto step = [&](int k, int at) {
+        float wv[2 * FS][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load(w[j], k, wv[j]);
+        for (int j = 0; j < 2 * FS; ++j) load(w[j], k, wv[j]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r >= a.rows) continue;
-            float xv[W];
-            load(a.x + r * a.xs, k, xv);
+            if (!S::SHARED && r >= rows) continue;
+            float xv[4];
+            if constexpr (S::SHARED) {
+                const float4 q = xs[r][at];
+                xv[0] = q.x, xv[1] = q.y, xv[2] = q.z, xv[3] = q.w;
+            } else {
+                load(a.x + (row0 + r) * a.xs, k, xv);
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2 * FS; ++j)
 #pragma unroll
-                for (int e = 0; e < W; ++e) acc[j][r] = fmaf(wv[j][e], xv[e], acc[j][r]);
+                for (int e = 0; e < 4; ++e) {
+                    float& s = acc[((j >> 1) * R + r) * 2 + (j & 1)];
+                    s = fmaf(wv[j][e], xv[e], s);
+                }
         }
+    };
+    if constexpr (S::SHARED) {
+        for (int k0 = 0; k0 < a.dim; k0 += S::CHUNK) {
+            __syncthreads();
+            for (int e = threadIdx.x; e < R * (S::CHUNK / 4); e += 128) {
+                const int r = e / (S::CHUNK / 4), at = e % (S::CHUNK / 4), k = k0 + at * 4;
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+                if (r < rows && k < a.dim) load(a.x + (row0 + r) * a.xs, k, v);
+                xs[r][at] = make_float4(v[0], v[1], v[2], v[3]);
+            }
+            __syncthreads();
+#pragma unroll 2
+            for (int at = lane; at < S::CHUNK / 4; at += 32)
+                if (k0 + at * 4 < a.dim) step(k0 + at * 4, at);
+        }
+    } else {
+#pragma unroll 2
+        for (int k = lane * 4; k < a.dim; k += 128) step(k, 0);
     }
+    // The lanes' sums: each halving sends one half of the values and keeps the other, until a lane has VALUES / 32 of them (of
+    // few values all lanes have all).
+    if constexpr (VALUES >= 64) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+        for (int o = 16, n = VALUES; o > 0; o >>= 1) {
+            n >>= 1;
+            const bool upper = lane & o;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+            for (int j = 0; j < n; ++j) {
+                const float mine = upper ? acc[j + n] : acc[j], other = upper ? acc[j] : acc[j + n];
+                acc[j] = mine + __shfl_xor_sync(kFull, other, o);
+            }
+        }
+    } else {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) acc[j][r] += __shfl_xor_sync(kFull, acc[j][r], o);
+        for (int j = 0; j < VALUES; ++j)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (r >= a.rows || lane >= 2 || f + lane >= a.inner) continue;
-        const float g = lane ? acc[1][r] : acc[0][r], u = lane ? acc[3][r] : acc[2][r];
-        const long at = (long)r * a.inner + f + lane;
-        if (a.kept) keep_one<float>(a.kept, a.plane, at, g, u);
-        a.out[at] = u * act_of<true>(g, a.act);
+            for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(kFull, acc[j], o);
+    }
+    constexpr int PAIRS = VALUES >= 64 ? VALUES / 64 : VALUES / 2;
+#pragma unroll
+    for (int q = 0; q < PAIRS; ++q) {
+        const int at = VALUES >= 64 ? lane * PAIRS + q : q, f = f0 + at / R, r = at % R;
+        if ((VALUES < 64 && lane != q) || r >= rows || f >= a.inner) continue;
+        const float g = acc[2 * q], u = acc[2 * q + 1];
+        const long o = (long)(row0 + r) * a.inner + f;
+        if (a.kept) keep_one<float>(a.kept, a.plane, o, g, u);
+        a.out[o] = u * act_of<true>(g, a.act);
     }
 }
 
@@ -1016,14 +1073,14 @@ int forward_few(const ews_gated_args* a, cudaStream_t s) {
     f.out = static_cast<float*>(a->out), f.kept = a->kept, f.plane = kept_plane(a);
     const bool vec = a->dim % 4 == 0 && f.gs % 4 == 0 && f.us % 4 == 0 && (a->rows == 1 || f.xs % 4 == 0) && aligned16(f.x) &&
                      aligned16(f.wg) && aligned16(f.wu);
-    const unsigned grid = (unsigned)((f.inner + 7) / 8);
-    auto go = [&](auto* kern) {
-        kern<<<grid, 128, 0, s>>>(f);
+    auto go = [&](auto* kern, int fs, int r) {
+        kern<<<dim3((unsigned)((f.inner + 4 * fs - 1) / (4 * fs)), (unsigned)((f.rows + r - 1) / r)), 128, 0, s>>>(f);
         return launched();
     };
-    if (f.rows <= 1) return vec ? go(few_f32_kernel<1, true>) : go(few_f32_kernel<1, false>);
-    if (f.rows <= 4) return vec ? go(few_f32_kernel<4, true>) : go(few_f32_kernel<4, false>);
-    return vec ? go(few_f32_kernel<16, true>) : go(few_f32_kernel<16, false>);
+    if (f.rows <= 1) return vec ? go(few_f32_kernel<1, true>, 2, 1) : go(few_f32_kernel<1, false>, 2, 1);
+    if (f.rows <= 4) return vec ? go(few_f32_kernel<4, true>, 2, 4) : go(few_f32_kernel<4, false>, 2, 4);
+    if (f.rows <= 8) return vec ? go(few_f32_kernel<8, true>, 4, 8) : go(few_f32_kernel<8, false>, 4, 8);
+    return vec ? go(few_f32_kernel<16, true>, 4, 16) : go(few_f32_kernel<16, false>, 4, 16);
 }
 
 template <int BN>

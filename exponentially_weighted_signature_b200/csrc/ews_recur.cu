@@ -9,13 +9,19 @@
 // (the flow exp(-dtheta lambda) of a diagonal generator at depth one with a clock step of each token and channel, and
 // the input scaled so that unit inputs give a unit state.)
 //
-// Both directions are a scan of maps h -> A h + H. A CTA takes a tile of 32 V channels by warps x L tokens, each warp L
-// consecutive tokens with everything of them in registers: the streams are read once. The warps' maps are joined in shared
-// memory, the tiles' by a decoupled look-back in ticket order (a tile publishes its map, then its state): a tile folds the
-// maps of up to `warps` tiles onto the nearest published state, always from the state upwards, so that the sum has one order
-// and the results do not depend on timing. The backward reads no states: the forward leaves one a tile of the backward
-// (float32, 1 / 64 of the stream), from which the tile runs the recurrence again. So the gradient of the rates, a float32 sum
-// over all tokens, does not see the rounding of the stored states, and a stream less is read.
+// Both directions are a scan of maps h -> A h + H. A tile is 64 tokens by 32 V channels (128 bytes a token); its warps take 8 or
+// 16 consecutive tokens each, with a and b of them in registers, so that the streams are read once. The warps' maps are joined in
+// shared memory, the tiles' by a decoupled look-back in ticket order (a tile publishes its map, then its state): a tile folds the
+// maps of up to as many tiles as it has warps onto a published state, always from the state upwards, so that the sum has one order
+// and the results do not depend on timing. The backward reads no states: the forward leaves one a tile (float32, 1 / 64 of the
+// stream), from which the tile runs the recurrence again. So the gradient of the rates, a float32 sum over all tokens, does not
+// see the rounding of the stored states, and a stream less is read.
+//
+// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 81 us forwards (four streams, 3.3 TB/s) and 153 back (seven, 3.1),
+// float32 106 and 177 us (5.1 and 5.3 TB/s). bfloat16 is bound by the gates: some 45 instructions an element forwards, 70 back,
+// issued at half the rate that the SM could; without their arithmetic 60 and 134 us, without the look-back too 56 and 116. One
+// sample of 17,984 tokens: 120 us, 79 without the look-back: 32 chains of tiles, 18 of each in work at a time, wait for one
+// another's maps and states (a window of 12 or 16 tiles instead of 4 changed nothing).
 #include <float.h>
 
 #include "ews_tc.cuh"
