@@ -24,6 +24,8 @@
 // another's maps and states (a window of 12 or 16 tiles instead of 4 changed nothing).
 #include <float.h>
 
+#include <type_traits>
+
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -107,7 +109,7 @@ struct F<2> {
     template <typename Fn>
     __device__ __forceinline__ static F make(Fn f) { return F(f(0), f(1)); }
 };
-// rounded as the packed ones are: whether a call's tensors allow pairs does not change its results
+// rounded as the packed ones are
 __device__ __forceinline__ F<1> operator*(F<1> a, F<1> b) { return F<1>(__fmul_rn(a.r, b.r)); }
 __device__ __forceinline__ F<1> operator+(F<1> a, F<1> b) { return F<1>(__fadd_rn(a.r, b.r)); }
 __device__ __forceinline__ F<1> fma(F<1> a, F<1> b, F<1> c) { return F<1>(fmaf(a.r, b.r, c.r)); }
@@ -185,9 +187,9 @@ __device__ __forceinline__ F<V> sigmoid(F<V> x) {
     return (e + F<V>(1.f)).each([](float t) { return rcp(t); });
 }
 
-// a = exp(-p) and w = 1 - a^2. Up to p = 0.175 from q = 1 - exp(-p) by its series (the first dropped term is 2^-27 of q there):
-// a = 1 - q then has no error but its rounding, where the exponent unit's 2^-22 would add up over the hundreds of tokens such
-// an a remembers, and w = q (2 - q) loses nothing to cancellation. Beyond, a state forgets within some six tokens.
+// a = exp(-p) and w = 1 - a^2, by way of q = 1 - a, whose series has no cancellation: a = 1 - q then has no error but its rounding,
+// where the exponent unit's 2^-22 would add up over the hundreds of tokens that an a near one remembers, and w = q (2 - q).
+// The series to the sixth power up to 0.175 (the first dropped term is 2^-27 of q there).
 constexpr float kSeries = 0.175f;
 template <int V>
 __device__ __forceinline__ F<V> decay_loss(F<V> p) {
@@ -197,24 +199,43 @@ __device__ __forceinline__ F<V> decay_loss(F<V> p) {
     q = fma(p, q, F<V>(-0.5f));
     return fma(p * p, q, p);
 }
-template <int V>
+// What a token keeps of its decay, and a and w of it. NEAR, where no rate of the warp exceeds 1.4, and with it no p: q, from the
+// series at p / 8 and 1 - exp(-2 t) = q (2 - q) three times over, without the exponent unit, whose 16 results a clock bound the
+// bfloat16 kernels. Else a: 1 - q up to 0.175, exp(-p) beyond, where a state forgets within some six tokens.
+constexpr float kNear = 8.f * kSeries;
+template <bool NEAR, int V>
 struct Decay {
-    F<V> a, w;
+    F<V> k;
+    __device__ __forceinline__ Decay() {}
+    __device__ __forceinline__ explicit Decay(F<V> p) {
+        if constexpr (NEAR) {
+            k = decay_loss(p * F<V>(0.125f));
+#pragma unroll
+            for (int i = 0; i < 3; ++i) k = fma(k * F<V>(-1.f), k, k + k);
+        } else {
+            const F<V> near = fma(decay_loss(p), F<V>(-1.f), F<V>(1.f));
+            const F<V> e = (p * F<V>(-kLog2e)).each([](float t) { return ex2(t); });
+            k = F<V>::make([&](int j) { return p.get(j) < kSeries ? near.get(j) : e.get(j); });
+        }
+    }
+    __device__ __forceinline__ static Decay of(F<V> kept) {
+        Decay d;
+        d.k = kept;
+        return d;
+    }
+    __device__ __forceinline__ F<V> a() const { return NEAR ? fma(k, F<V>(-1.f), F<V>(1.f)) : k; }
+    __device__ __forceinline__ F<V> w(F<V> p) const {
+        if constexpr (NEAR) return fma(k, a(), k);
+        const F<V> q = decay_loss(p), near = fma(q, fma(q, F<V>(-1.f), F<V>(1.f)), q);
+        return F<V>::make([&](int j) { return p.get(j) < kSeries ? near.get(j) : fmaf(-k.get(j), k.get(j), 1.f); });
+    }
 };
 template <int V>
-__device__ __forceinline__ Decay<V> decay_of(F<V> p) {
-    const F<V> q = decay_loss(p), near = fma(q, F<V>(-1.f), F<V>(1.f)), w = fma(q, near, q);
-    const F<V> e = (p * F<V>(-kLog2e)).each([](float t) { return ex2(t); });
-    Decay<V> d;
-    d.a = F<V>::make([&](int j) { return p.get(j) < kSeries ? near.get(j) : e.get(j); });
-    d.w = F<V>::make([&](int j) { return p.get(j) < kSeries ? w.get(j) : fmaf(-e.get(j), e.get(j), 1.f); });
-    return d;
-}
-// w once more where a is at hand.
-template <int V>
-__device__ __forceinline__ F<V> rest_of(F<V> p, F<V> a) {
-    const F<V> q = decay_loss(p), w = fma(q, fma(q, F<V>(-1.f), F<V>(1.f)), q);
-    return F<V>::make([&](int j) { return p.get(j) < kSeries ? w.get(j) : fmaf(-a.get(j), a.get(j), 1.f); });
+__device__ __forceinline__ bool is_near(F<V> rate) {
+    bool near = true;
+#pragma unroll
+    for (int j = 0; j < V; ++j) near = near && rate.get(j) <= kNear;
+    return __all_sync(kFull, near);
 }
 template <int V>
 __device__ __forceinline__ F<V> root(F<V> w) { return w.each([](float t) { return root(t); }); }
@@ -385,14 +406,19 @@ __global__ void __launch_bounds__(Shape<V>::FW * 32, Shape<V>::FCTAS) forward_ke
     }
     const F<V> rate = F<V>::make([&](int j) { return in ? rate_at(a.rate + c + j) : 0.f; });
     F<V> av[FL], bv[FL], A(1.f), H(0.f);
+    auto gates = [&](auto near) {
 #pragma unroll
-    for (int l = 0; l < FL; ++l) {
-        const Decay<V> d = decay_of(rate * sigmoid(wr[l].get()));
-        av[l] = d.a;
-        bv[l] = root(d.w) * sigmoid(wi[l].get()) * wx[l].get();
-        A = A * av[l];
-        H = fma(av[l], H, bv[l]);
-    }
+        for (int l = 0; l < FL; ++l) {
+            const F<V> p = rate * sigmoid(wr[l].get());
+            const Decay<decltype(near)::value, V> d(p);
+            av[l] = d.a();
+            bv[l] = root(d.w(p)) * sigmoid(wi[l].get()) * wx[l].get();
+            A = A * av[l];
+            H = fma(av[l], H, bv[l]);
+        }
+    };
+    if (is_near(rate)) gates(std::true_type());
+    else gates(std::false_type());
     // the warps' maps in front of this one
     F<V> pa(1.f), ph(0.f), h(0.f);
     sh.A[warp][lane] = A, sh.H[warp][lane] = H;
@@ -436,10 +462,10 @@ template <int V>
 struct Slopes {
     F<V> x, decay, gate;
 };
-template <int V>
-__device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, F<V> a, F<V> r, F<V> i, F<V> before, F<V> x, F<V> dout, F<V>* g, F<V>* sum) {
+template <bool NEAR, int V>
+__device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, Decay<NEAR, V> d, F<V> r, F<V> i, F<V> before, F<V> x, F<V> dout, F<V>* g, F<V>* sum) {
     const F<V> minus(-1.f), one(1.f);
-    const F<V> w = rest_of(rate * r, a);  // formed again: kept, it would take too many registers
+    const F<V> a = d.a(), w = d.w(rate * r);  // formed again: kept, they would take too many registers
     // no step of the clock: the state passes, whatever the input
     const F<V> inv = w.each([](float t) { return fabsf(t) < FLT_MIN ? 0.f : inverse_root(t); });
     *g = *g + dout;
@@ -463,9 +489,10 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
     const int live = in ? min(max(len - from, 0), BL) : 0, rows = in ? min(max(a.steps - from, 0), BL) : 0;
 
     Word<T, V> wx[BL], wg[BL];
-    F<V> av[BL], rv[BL], iv[BL], hb[BL];  // hb: the state in front of each token, at first from zero at the warp's start
+    F<V> kv[BL], rv[BL], iv[BL], hb[BL];  // hb: the state in front of each token, at first from zero at the warp's start
     F<V> A(1.f), H(0.f), D(0.f), h(0.f);
     const F<V> rate = F<V>::make([&](int j) { return in ? rate_at(a.rate + c + j) : 0.f; });
+    const bool near = is_near(rate);
     {
         Word<T, V> wr[BL], wi[BL];
         const T* px = a.x.p + t.b * a.x.sb + (long)from * a.x.st + c;
@@ -481,18 +508,23 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
         }
         if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels);
         else if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
+        auto gates = [&](auto near) {
+            using K = Decay<decltype(near)::value, V>;
 #pragma unroll
-        for (int l = 0; l < BL; ++l) {
-            rv[l] = sigmoid(wr[l].get()), iv[l] = sigmoid(wi[l].get());
-            const Decay<V> d = decay_of(rate * rv[l]);
-            av[l] = d.a;
-            hb[l] = H;
-            H = fma(av[l], H, root(d.w) * iv[l] * wx[l].get());
-            A = A * av[l];
-        }
+            for (int l = 0; l < BL; ++l) {
+                rv[l] = sigmoid(wr[l].get()), iv[l] = sigmoid(wi[l].get());
+                const K d(rate * rv[l]);
+                kv[l] = d.k;
+                hb[l] = H;
+                H = fma(d.a(), H, root(d.w(rate * rv[l])) * iv[l] * wx[l].get());
+                A = A * d.a();
+            }
+#pragma unroll
+            for (int l = BL - 1; l >= 0; --l) D = K::of(kv[l]).a() * (wg[l].get() + D);
+        };
+        if (near) gates(std::true_type());
+        else gates(std::false_type());
     }
-#pragma unroll
-    for (int l = BL - 1; l >= 0; --l) D = av[l] * (wg[l].get() + D);
     // the states by the maps of the warps in front, the gradients by those of the warps behind
     F<V> pa(1.f), pd(0.f), g(0.f);
     sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
@@ -520,25 +552,30 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
         else if (a.dinitial) store_channels<V>(a.dinitial + (long)t.b * a.channels, c, a.channels, end);
     }
     g = fma(pa, g, pd);
-#pragma unroll
-    for (int l = 0; l < BL; ++l) {
-        hb[l] = hb[l] + h;
-        h = av[l] * h;
-    }
     F<V> sum(0.f);
     const long at = ((long)t.b * a.steps + from + BL - 1) * a.channels + c;
     T *ox = a.dx + at, *od = a.ddecay + at, *oi = a.dgate + at;
+    auto slopes = [&](auto near) {
+        using K = Decay<decltype(near)::value, V>;
 #pragma unroll
-    for (int l = BL - 1; l >= 0; --l) {
-        const Slopes<V> o = slopes_of(rate, av[l], rv[l], iv[l], hb[l], wx[l].get(), wg[l].get(), &g, &sum);
-        if (l < rows) {
-            const bool there = l < live;
-            Word<T, V>::store(ox, there ? o.x : F<V>(0.f));
-            Word<T, V>::store(oi, there ? o.gate : F<V>(0.f));
-            Word<T, V>::store(od, there ? o.decay : F<V>(0.f));
+        for (int l = 0; l < BL; ++l) {
+            hb[l] = hb[l] + h;
+            h = K::of(kv[l]).a() * h;
         }
-        ox -= a.channels, od -= a.channels, oi -= a.channels;
-    }
+#pragma unroll
+        for (int l = BL - 1; l >= 0; --l) {
+            const Slopes<V> o = slopes_of(rate, K::of(kv[l]), rv[l], iv[l], hb[l], wx[l].get(), wg[l].get(), &g, &sum);
+            if (l < rows) {
+                const bool there = l < live;
+                Word<T, V>::store(ox, there ? o.x : F<V>(0.f));
+                Word<T, V>::store(oi, there ? o.gate : F<V>(0.f));
+                Word<T, V>::store(od, there ? o.decay : F<V>(0.f));
+            }
+            ox -= a.channels, od -= a.channels, oi -= a.channels;
+        }
+    };
+    if (near) slopes(std::true_type());
+    else slopes(std::false_type());
     if (a.drate_part) {  // of the tile, the warps in order
         __syncthreads();
         sh.H[warp][lane] = sum;
@@ -658,14 +695,19 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
         for (int l = live; l < PL; ++l) row[l * 32].fill(0.f), row[STREAM + l * 32].fill(-INFINITY), row[2 * STREAM + l * 32].fill(0.f);
         const F<V> rate = F<V>::make([&](int j) { return c + j < a.channels ? rate_at(a.rate + c + j) : 0.f; });
         F<V> av[PL], bv[PL], A(1.f), H(0.f);
+        auto gates = [&](auto near) {
 #pragma unroll
-        for (int l = 0; l < PL; ++l) {
-            const Decay<V> d = decay_of(rate * sigmoid(row[STREAM + l * 32].get()));
-            av[l] = d.a;
-            bv[l] = root(d.w) * sigmoid(row[2 * STREAM + l * 32].get()) * row[l * 32].get();
-            A = A * av[l];
-            H = fma(av[l], H, bv[l]);
-        }
+            for (int l = 0; l < PL; ++l) {
+                const F<V> p = rate * sigmoid(row[STREAM + l * 32].get());
+                const Decay<decltype(near)::value, V> d(p);
+                av[l] = d.a();
+                bv[l] = root(d.w(p)) * sigmoid(row[2 * STREAM + l * 32].get()) * row[l * 32].get();
+                A = A * av[l];
+                H = fma(av[l], H, bv[l]);
+            }
+        };
+        if (is_near(rate)) gates(std::true_type());
+        else gates(std::false_type());
         F<V> pa(1.f), ph(0.f), h(0.f);
         sh.A[warp][lane] = A, sh.H[warp][lane] = H;
         if (threadIdx.x == 0) {
@@ -742,21 +784,27 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
             row[2 * STREAM + l * 32].fill(0.f), row[3 * STREAM + l * 32].fill(0.f);
         }
         const F<V> rate = F<V>::make([&](int j) { return c + j < a.channels ? rate_at(a.rate + c + j) : 0.f; });
-        F<V> av[QL], rv[QL], iv[QL], hb[QL];  // as in backward_kernel
+        F<V> kv[QL], rv[QL], iv[QL], hb[QL];  // as in backward_kernel
+        const bool near = is_near(rate);
         F<V> A(1.f), H(0.f), D(0.f), h(0.f);
         if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels);
         else if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
+        auto gates = [&](auto near) {
+            using K = Decay<decltype(near)::value, V>;
 #pragma unroll
-        for (int l = 0; l < QL; ++l) {
-            rv[l] = sigmoid(row[STREAM + l * 32].get()), iv[l] = sigmoid(row[2 * STREAM + l * 32].get());
-            const Decay<V> d = decay_of(rate * rv[l]);
-            av[l] = d.a;
-            hb[l] = H;
-            H = fma(av[l], H, root(d.w) * iv[l] * row[l * 32].get());
-            A = A * av[l];
-        }
+            for (int l = 0; l < QL; ++l) {
+                rv[l] = sigmoid(row[STREAM + l * 32].get()), iv[l] = sigmoid(row[2 * STREAM + l * 32].get());
+                const K d(rate * rv[l]);
+                kv[l] = d.k;
+                hb[l] = H;
+                H = fma(d.a(), H, root(d.w(rate * rv[l])) * iv[l] * row[l * 32].get());
+                A = A * d.a();
+            }
 #pragma unroll
-        for (int l = QL - 1; l >= 0; --l) D = av[l] * (row[3 * STREAM + l * 32].get() + D);
+            for (int l = QL - 1; l >= 0; --l) D = K::of(kv[l]).a() * (row[3 * STREAM + l * 32].get() + D);
+        };
+        if (near) gates(std::true_type());
+        else gates(std::false_type());
         F<V> pa(1.f), pd(0.f), g(0.f);
         sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
         if (threadIdx.x == 0) {
@@ -784,17 +832,22 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
             else if (a.dinitial) store_channels<V>(a.dinitial + (long)t.b * a.channels, c, a.channels, end);
         }
         g = fma(pa, g, pd);
-#pragma unroll
-        for (int l = 0; l < QL; ++l) {
-            hb[l] = hb[l] + h;
-            h = av[l] * h;
-        }
         F<V> sum(0.f);
+        auto slopes = [&](auto near) {
+            using K = Decay<decltype(near)::value, V>;
 #pragma unroll
-        for (int l = QL - 1; l >= 0; --l) {
-            const Slopes<V> o = slopes_of(rate, av[l], rv[l], iv[l], hb[l], row[l * 32].get(), row[3 * STREAM + l * 32].get(), &g, &sum);
-            row[l * 32].put(o.x), row[STREAM + l * 32].put(o.decay), row[2 * STREAM + l * 32].put(o.gate);
-        }
+            for (int l = 0; l < QL; ++l) {
+                hb[l] = hb[l] + h;
+                h = K::of(kv[l]).a() * h;
+            }
+#pragma unroll
+            for (int l = QL - 1; l >= 0; --l) {
+                const Slopes<V> o = slopes_of(rate, K::of(kv[l]), rv[l], iv[l], hb[l], row[l * 32].get(), row[3 * STREAM + l * 32].get(), &g, &sum);
+                row[l * 32].put(o.x), row[STREAM + l * 32].put(o.decay), row[2 * STREAM + l * 32].put(o.gate);
+            }
+        };
+        if (near) slopes(std::true_type());
+        else slopes(std::false_type());
         for (int l = live; l < QL; ++l) row[l * 32].fill(0.f), row[STREAM + l * 32].fill(0.f), row[2 * STREAM + l * 32].fill(0.f);
         tc5::fence_async_smem();
         if (a.drate_part) {  // of the tile, the warps in order
@@ -881,8 +934,9 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Step<
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const Decay<1> d = decay_of(F<1>(k[j]) * sigmoid(F<1>(r[j])));
-            o[j] = fma(d.a, F<1>(h[j]), root(d.w) * sigmoid(F<1>(i[j])) * F<1>(x[j])).r;
+            const F<1> p = F<1>(k[j]) * sigmoid(F<1>(r[j]));
+            const Decay<false, 1> d(p);
+            o[j] = fma(d.a(), F<1>(h[j]), root(d.w(p)) * sigmoid(F<1>(i[j])) * F<1>(x[j])).r;
         }
         if constexpr (V == 4) Vec<float, true>::store(state, o);
         else *state = o[0];
