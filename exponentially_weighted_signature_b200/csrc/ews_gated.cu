@@ -26,8 +26,8 @@
 // Measured, bfloat16: 4,001 rows, 2,048 x 8,192: 182 us, 1.47 PFLOP/s, against 169 us for the library's product of the same
 // operands without activation and product; 8,192 rows, 1,024 x 4,096: 102 us (97), 124 us where G and U are kept, the backward 298
 // us: 63 to 79 for its operands, 208 for 8 N D F at 1.32 PFLOP/s, 11 to join pieces. What bounds them is the tensor pipe, under the
-// power cap in a long run. 48 rows, 2,048 x 5,632: 18 us (2.6 TB/s), 11,008 x 4,096: 42 us (4.3 TB/s): a CTA's start, first bytes and
-// epilogue beside its share of the weights; one row, 1,024 x 4,096: 8.5 us, the same. float32, 16 rows, 1,024 x 4,096: 20 us.
+// power cap in a long run. Up to 64 rows, 5,632 x 2,048: 15 us (3.2 TB/s; 46 MB take 7), 11,008 x 4,096: 38 us (4.8 TB/s; 28): a CTA's
+// start, first bytes and epilogue beside its share of the weights; 4,096 x 1,024: 9 us, the same. float32, 16 rows, 1,024 x 4,096: 20.
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -41,9 +41,9 @@ constexpr int EPW = 8;              // epilogue warps
 constexpr int NTH = 64 + EPW * 32;  // and one each for TMA and MMA
 constexpr int SMS = 148;
 constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulator
-// Rows up to which served_kernel runs (bfloat16; 64 rows, 4,096 x 1,024: 17 us, 100: 22 us there, 14 as tiles), and up to which
-// few_f32_kernel does (32 rows, 5,632 x 2,048: 88 us there, 109 as tiles of three planes; 64 rows: 139, 111).
-constexpr int kServed = 64, kFewF32 = 32;
+// Rows up to which served_kernel runs (bfloat16; 100 rows, 5,632 x 2,048: 20 us there, 26 as tiles; 4,096 x 1,024: 14, 13), and up
+// to which few_f32_kernel does (32 rows, 5,632 x 2,048: 88 us there, 109 as tiles of three planes; 64 rows: 139, 111).
+constexpr int kServed = 128, kFewF32 = 32;
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
 
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Fe
     }
 }
 
-// Up to 64 rows: the weights as the wide operand, 64 rows of Wg above the same of Wu a CTA (their partners in lanes 64
+// Up to 128 rows: the weights as the wide operand, 64 rows of Wg above the same of Wu a CTA (their partners in lanes 64
 // apart), the rows of X as the narrow one (BN of them). One tile a CTA, whatever K; what counts is how many bytes of the
 // weights are in flight: eight stages of 16 KB and X's rows where one CTA an SM is enough, four where there are more tiles.
 struct Served {
@@ -747,7 +747,7 @@ constexpr int SERVED_T = 192;  // a warp for TMA, one for MMA, four for the epil
 template <int BN>
 __global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensorMap mu,
                                                           const __grid_constant__ CUtensorMap mx, const __grid_constant__ Served a) {
-    constexpr int A = BM * BK * 2, STAGE = A + BN * BK * 2, COLS = BN < 32 ? 32 : BN;
+    constexpr int A = BM * BK * 2, STAGE = A + BN * BK * 2, COLS = BN <= 32 ? 32 : BN <= 64 ? 64 : 128;  // of tensor memory
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(tiles + a.stages * STAGE);
@@ -755,12 +755,22 @@ __global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant_
     uint64_t* done = empty + a.stages;
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_at + 1);
-    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, f0 = blockIdx.x * 64;
+    auto fill = [&](int s, int kb) {
+        unsigned char* at = tiles + s * STAGE;
+        mbar_expect(full + s, STAGE);
+        tma_load(&mg, full + s, at, kb * BK, f0, 0);
+        tma_load(&mu, full + s, at + A / 2, kb * BK, f0, 0);
+        tma_load(&mx, full + s, at + A, kb * BK, 0, 0);
+    };
+    const int first = min(a.stages, a.blocks);
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
         mbar_init(done, 1);
         *fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        for (int i = 0; i < first; ++i) fill(i, i);  // the first bytes are on their way while the rest of the CTA gets ready
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "r"(COLS));
@@ -770,19 +780,14 @@ __global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant_
     __syncthreads();
     fence_after();
     const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
-    const int f0 = blockIdx.x * 64;
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
-            int s = 0, kb = 0;
-            uint32_t ph = 1;
+            int s = 0, kb = first;
+            uint32_t ph = 0;
             for (; kb < a.blocks; ++kb) {
                 if (!(ok = mbar_wait(empty + s, ph, fail))) break;
-                unsigned char* at = tiles + s * STAGE;
-                mbar_expect(full + s, STAGE);
-                tma_load(&mg, full + s, at, kb * BK, f0, 0);
-                tma_load(&mu, full + s, at + A / 2, kb * BK, f0, 0);
-                tma_load(&mx, full + s, at + A, kb * BK, 0, 0);
+                fill(s, kb);
                 if (++s == a.stages) s = 0, ph ^= 1u;
             }
             if (!ok)
@@ -813,7 +818,8 @@ __global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant_
             mbar_drain(done, 0);
         }
     }
-    float v[BN < 32 ? 1 : BN / 32][32];
+    constexpr int CHUNKS = (BN + 31) / 32;
+    float v[CHUNKS][32];
     const int quarter = warp & 3, half = quarter >> 1, ch = (quarter & 1) * 32 + lane;
     float* swap = reinterpret_cast<float*>(tiles);  // (2, BN / 2, 64): U of the first rows, G of the others
     constexpr int HALF = BN / 2;
@@ -823,7 +829,7 @@ __global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant_
         if (ok) {
             const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-            for (int c = 0; c < COLS / 32; ++c) tmem_ld32(src + c * 32, v[c]);
+            for (int c = 0; c < CHUNKS; ++c) tmem_ld32(src + c * 32, v[c]);
             // each side gives the other half of its rows away
 #pragma unroll
             for (int j = 0; j < HALF; ++j) {
@@ -834,20 +840,32 @@ __global__ void __launch_bounds__(SERVED_T) served_kernel(const __grid_constant_
     }
     __syncthreads();
     if (warp >= 2 && ok) {
-        const int f = f0 + ch;
-        if (f < a.inner) {
+        const int f = f0 + ch, row0 = half ? HALF : 0;
+        float g[HALF], u[HALF];
 #pragma unroll
-            for (int j = 0; j < HALF; ++j) {
-                const int row = half ? j + HALF : j;
-                if (row < a.rows) {
-                    const float got = swap[(half ? HALF * 64 : 0) + j * 64 + ch];
-                    const float own = half ? v[(j + HALF) / 32][(j + HALF) % 32] : v[j / 32][j % 32];
-                    const float g = half ? got : own, u = half ? own : got;
-                    const long at = (long)row * a.inner + f;
-                    if (a.kept) keep_one<bf16>(a.kept, a.plane, at, g, u);
-                    a.out[at] = from_f<bf16>(u * act_of<false>(g, a.act));
-                }
-            }
+        for (int j = 0; j < HALF; ++j) {
+            const float got = swap[(half ? HALF * 64 : 0) + j * 64 + ch];
+            const float own = half ? v[(j + HALF) / 32][(j + HALF) % 32] : v[j / 32][j % 32];
+            g[j] = half ? got : own, u[j] = half ? own : got;
+        }
+        if (a.kept) {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j)
+                if (row0 + j < a.rows && f < a.inner) keep_one<bf16>(a.kept, a.plane, (long)(row0 + j) * a.inner + f, g[j], u[j]);
+        }
+        // a branch a row would leave each row's latency by itself: 5 us for 64 rows, so 2
+        if (a.act == SILU) {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) u[j] *= act_of<false>(g[j], SILU);
+        } else {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) u[j] *= act_of<false>(g[j], GELU);
+        }
+        bf16* out = a.out + (long)row0 * a.inner + f;
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) {
+            if (row0 + j < a.rows && f < a.inner) *out = from_f<bf16>(u[j]);
+            out += a.inner;
         }
     }
     fence_before();
@@ -1089,11 +1107,11 @@ int run_served(const ews_gated_args* a, const Operand& x, const Operand& wg, con
     CUtensorMap mx, mg, mu;
     if (!make_map(enc, &mx, x, BN) || !make_map(enc, &mg, wg, 64) || !make_map(enc, &mu, wu, 64)) return EWS_ERR_LAUNCH;
     const unsigned grid = (unsigned)((a->inner + 63) / 64);
-    const Served v{(int)a->rows, (int)a->inner, a->activation, (int)((a->dim + BK - 1) / BK), grid <= SMS ? 8 : 4,
+    const Served v{(int)a->rows, (int)a->inner, a->activation, (int)((a->dim + BK - 1) / BK), BN > 64 ? (grid <= SMS ? 6 : 3) : grid <= SMS ? 8 : 4,
                    static_cast<bf16*>(a->out), a->kept, kept_plane(a), a->status};
     constexpr int stage = BM * BK * 2 + BN * BK * 2, rest = 1024 + 256;
     auto* kern = served_kernel<BN>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * stage + rest) != cudaSuccess) return EWS_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (BN > 64 ? 6 : 8) * stage + rest) != cudaSuccess) return EWS_ERR_LAUNCH;
     kern<<<grid, SERVED_T, v.stages * stage + rest, s>>>(mg, mu, mx, v);
     return launched();
 }
@@ -1110,7 +1128,10 @@ int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     if constexpr (sizeof(T) == 2) {
         if (path == SERVED) {
             if (a->rows <= 16) return run_served<16>(a, x, wg, wu, s);
-            return a->rows <= 32 ? run_served<32>(a, x, wg, wu, s) : run_served<64>(a, x, wg, wu, s);
+            if (a->rows <= 32) return run_served<32>(a, x, wg, wu, s);
+            if (a->rows <= 48) return run_served<48>(a, x, wg, wu, s);
+            if (a->rows <= 64) return run_served<64>(a, x, wg, wu, s);
+            return a->rows <= 96 ? run_served<96>(a, x, wg, wu, s) : run_served<128>(a, x, wg, wu, s);
         }
     }
     const EncodeFn enc = encoder();

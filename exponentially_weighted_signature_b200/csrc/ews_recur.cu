@@ -17,11 +17,11 @@
 // stream), from which the tile runs the recurrence again. So the gradient of the rates, a float32 sum over all tokens, does not
 // see the rounding of the stored states, and a stream less is read.
 //
-// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 81 us forwards (four streams, 3.3 TB/s) and 153 back (seven, 3.1),
-// float32 106 and 177 us (5.1 and 5.3 TB/s). bfloat16 is bound by the gates: some 45 instructions an element forwards, 70 back,
-// issued at half the rate that the SM could; without their arithmetic 60 and 134 us, without the look-back too 56 and 116. One
-// sample of 17,984 tokens: 120 us, 79 without the look-back: 32 chains of tiles, 18 of each in work at a time, wait for one
-// another's maps and states (a window of 12 or 16 tiles instead of 4 changed nothing).
+// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 77 us forwards (four streams, 3.5 TB/s) and 142 back (seven, 3.3),
+// float32 109 and 179 us (4.9 and 5.2 TB/s). bfloat16 is bound by the gates, of which the SM issues at half its rate at best:
+// with the exponent unit for every decay 81 and 153 us, without the gates' arithmetic 60 and 134, without the look-back too 56 and
+// 116. One sample of 17,984 tokens: 118 and 185 us, 79 and 146 without the look-back: 32 chains of tiles, 18 of each in work at a
+// time, wait for one another's maps and states (folding 12 or 16 tiles at once instead of 4 changed nothing).
 #include <float.h>
 
 #include <type_traits>

@@ -65,7 +65,7 @@ def test_gated_arguments_are_checked_before_the_device():
     assert lib.ews_gated_fwd(_gated(rows=0), None) == 0
     # operands that TMA cannot read as they lie are packed; few float32 rows are read as they lie
     assert lib.ews_gated_work_size(_gated(), 0) == 0 < lib.ews_gated_work_size(_gated(xs=65), 0)
-    assert lib.ews_gated_work_size(_gated(rows=64), 0) == 0 < lib.ews_gated_work_size(_gated(rows=64, xs=65), 0)
+    assert lib.ews_gated_work_size(_gated(rows=128), 0) == 0 < lib.ews_gated_work_size(_gated(rows=128, xs=65), 0)
     assert lib.ews_gated_work_size(_gated(rows=32, dtype=0), 0) == 0 < lib.ews_gated_work_size(_gated(rows=33, dtype=0), 0)
     size = gated_ops._size(200, 64, 128, 1, (64, 64, 64), (0, 0, 0), (1, 1, 1), 1)
     assert size == lib.ews_gated_work_size(_gated(), 1) > 0

@@ -64,7 +64,7 @@ def inputs(dtype, N, D, F, seed=0):
     return r(N, D).to(dtype), (r(F, D) * D**-0.5).to(dtype), (r(F, D) * D**-0.5).to(dtype), r(N, F).to(dtype)
 
 
-SIZES = [(1, 1, 1), (7, 2052, 20), (12, 1301, 36), (32, 520, 40), (31, 516, 9),
+SIZES = [(1, 1, 1), (48, 136, 72), (41, 40, 130), (96, 72, 200), (81, 1000, 64), (7, 2052, 20), (12, 1301, 36), (32, 520, 40), (31, 516, 9),
          (1, 8, 16), (1, 1024, 520), (2, 33, 17), (4, 40, 31), (8, 64, 64), (9, 256, 48), (16, 128, 100), (17, 72, 33),
          (33, 96, 200), (64, 300, 24), (64, 1000, 72), (65, 64, 64), (127, 40, 129), (128, 64, 8), (129, 200, 130), (300, 512, 341),
          (1000, 136, 1000), (2050, 24, 260), (700, 1032, 2056)]
