@@ -44,6 +44,9 @@ constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulato
 // Rows up to which served_kernel runs (bfloat16; 100 rows, 5,632 x 2,048: 20 us there, 26 as tiles; 4,096 x 1,024: 14, 13), and up
 // to which few_f32_kernel does (32 rows, 5,632 x 2,048: 88 us there, 109 as tiles of three planes; 64 rows: 139, 111).
 constexpr int kServed = 128, kFewF32 = 32;
+// Where dG and dU are small or few, their rounding to bfloat16 does not average out of the gradients (five rows of 472: 2.5e-3 of the
+// exact ones where one rounding leaves 1.7e-3): up to this many multiplications a product they are kept in two planes, 16 bits.
+constexpr long kTwoPlanes = 1l << 30;
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
 
@@ -526,6 +529,7 @@ struct Grad {
     const void* kept;
     long plane;
     int inner, ld, act;
+    int planes;
     bf16* out;
 };
 
@@ -550,8 +554,8 @@ __global__ void __launch_bounds__(256) operand_kernel(const __grid_constant__ Gr
                 u[j] = o[j] * f;
             }
             bf16* at = d.out + row * d.ld + col;
-            split8<T>(g, at, d.rows * d.ld, planes);
-            split8<T>(u, at + planes * d.rows * d.ld, d.rows * d.ld, planes);
+            split8<T>(g, at, d.rows * d.ld, d.planes);
+            split8<T>(u, at + d.planes * d.rows * d.ld, d.rows * d.ld, d.planes);
         } else {
             long row = (e - grads) / per;
             const int col = (int)(e - grads - row * per) * 8;
@@ -921,7 +925,7 @@ struct Source {
 };
 
 struct Plan {
-    int planes;
+    int planes, gplanes;  // of an operand, of dG and dU
     long ldd, ldf;
     Source x, wg, wu;
     size_t dgu, slots, bytes;
@@ -1004,7 +1008,8 @@ void share_out(Gemm* g) {
 
 Plan plan(const ews_gated_args* a, bool bwd) {
     Plan p{};
-    p.planes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
+    p.planes = p.gplanes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
+    if (p.planes == 1 && a->rows * a->inner <= kTwoPlanes / a->dim) p.gplanes = 2;
     p.ldd = up(a->dim, 8), p.ldf = up(a->inner, 8);
     if (!bwd && path_of(a) == FEW) return p;
     size_t at = 0;
@@ -1025,12 +1030,12 @@ Plan plan(const ews_gated_args* a, bool bwd) {
         p.bn = forward_bn(a);
     } else {
         p.bn = p.planes > 1 || a->dim <= 128 ? 128 : 256;
-        const int products = p.planes == 1 ? 1 : 6;
+        const int products = p.planes == 1 ? p.gplanes : 6;
         if (a->dx) p.gemm.job[0] = job_of(a->rows, a->dim, a->inner, p.bn, 2 * products);
         if (a->dw_gate) p.gemm.job[1] = job_of(a->inner, a->dim, a->rows, p.bn, products);
         if (a->dw_up) p.gemm.job[2] = job_of(a->inner, a->dim, a->rows, p.bn, products);
         share_out(&p.gemm);
-        p.dgu = take(sizeof(bf16) * 2 * (size_t)p.planes * a->rows * p.ldf);
+        p.dgu = take(sizeof(bf16) * 2 * (size_t)p.gplanes * a->rows * p.ldf);
         if (p.gemm.line) p.slots = take(sizeof(float) * 2 * (size_t)p.gemm.ctas * BM * p.bn);
     }
     p.bytes = at;
@@ -1160,10 +1165,10 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     Operand x{}, wg{}, wu{}, d{};
     const bool dw = a->dw_gate || a->dw_up;
     bf16* dgu = reinterpret_cast<bf16*>(w + p.dgu);
-    const Grad<T> grad{static_cast<const T*>(a->dout), (long)a->dout_stride, a->rows, a->kept, kept_plane(a), (int)a->inner, (int)p.ldf, a->activation, dgu};
+    const Grad<T> grad{static_cast<const T*>(a->dout), (long)a->dout_stride, a->rows, a->kept, kept_plane(a), (int)a->inner, (int)p.ldf, a->activation, p.gplanes, dgu};
     int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, grad, s);
     if (rc != EWS_OK) return rc;
-    d.p = dgu, d.rows = a->rows, d.cols = d.ld = p.ldf, d.plane = a->rows * p.ldf, d.planes = 2 * p.planes;
+    d.p = dgu, d.rows = a->rows, d.cols = d.ld = p.ldf, d.plane = a->rows * p.ldf, d.planes = 2 * p.gplanes;
     const EncodeFn enc = encoder();
     Maps m{};
     if (!make_map(enc, &m.a[0], d, BM) || !make_map(enc, &m.a[1], d, 64)) return EWS_ERR_LAUNCH;
@@ -1174,7 +1179,7 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     g.status = a->status;
     g.slots = reinterpret_cast<float*>(w + p.slots);
     void* out[3] = {a->dx, a->dw_gate, a->dw_up};
-    const int products = p.planes == 1 ? 1 : 6;
+    const int products = p.planes == 1 ? p.gplanes : 6;
     for (int k = 0; k < 3; ++k) {
         Job& j = g.job[k];
         j.out = out[k];
@@ -1182,8 +1187,8 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
         for (int i = 0; j.pairs && i < products; ++i)  // the smallest of both sides first
             for (int side = 0; side < (k ? 1 : 2); ++side, ++at) {
                 const int which = k ? k - 1 : side;  // dG or dU
-                j.ia[at] = (signed char)(which * p.planes + (products == 1 ? 0 : kPlaneA[i]));
-                j.ib[at] = products == 1 ? 0 : kPlaneB[i];
+                j.ia[at] = (signed char)(which * p.gplanes + (p.planes == 1 ? p.gplanes - 1 - i : kPlaneA[i]));
+                j.ib[at] = p.planes == 1 ? 0 : kPlaneB[i];
                 j.mb[at] = (signed char)(k ? 2 : side);
             }
     }

@@ -47,6 +47,10 @@ constexpr long kPieceElems = 1l << 27; // entries of G (times planes) at a time:
 // is long: for float32 a tile's sum leaves the accumulator every 256 of K and is added, rounded, to the float32 partial.
 constexpr int kRun = 4;
 constexpr float kLog2e = 1.4426950408889634f;
+// A teacher's few entries dominate G, and with few rows their rounding to bfloat16 does not average out of the gradients (ten rows:
+// 2.6e-3 of the exact ones where one rounding leaves 1.7e-3). Up to this many multiplications a product G is kept in two planes,
+// 16 bits, which takes some 10 us more at most.
+constexpr long kTwoPlanes = 1l << 31;
 
 // 2^x: the exponent unit's own instruction, results below the normal range to zero.
 __device__ __forceinline__ float ex2(float x) {
@@ -829,11 +833,14 @@ int gemm_bn(const Maps& maps, const Gemm& g, cudaStream_t s) {
 // Operands of job[0], and of job[1] where it has units (OUT). Both jobs' n is the model's width, so they share BN.
 template <int EPI>
 int gemm(Gemm g, const Operand& a0, const Operand& b0, const Operand& a1, const Operand& b1, int planes, cudaStream_t s) {
+    const int gplanes = EPI == LSE ? planes : g.planes;
     static const signed char pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
     g.pairs = planes == 1 ? 1 : 6;
     for (int i = 0; i < g.pairs; ++i) g.ia[i] = planes == 1 ? 0 : pa[i], g.ib[i] = planes == 1 ? 0 : pb[i];
+    if (EPI == OUT && planes == 1)  // G's second plane first
+        for (g.pairs = 0; g.pairs < gplanes; ++g.pairs) g.ia[g.pairs] = (signed char)(gplanes - 1 - g.pairs);
     Maps m{};
-    if (EPI == GRAD && planes == 1 &&
+    if (EPI == GRAD && gplanes == 1 &&
         !make_map(&m.g, Operand{g.g, g.job[0].m, g.job[0].n, g.ldg, 0, 1}, 32))
         return EWS_ERR_LAUNCH;
     g.run = EPI == OUT && planes > 1 ? kRun : 1 << 28;
@@ -846,7 +853,8 @@ int gemm(Gemm g, const Operand& a0, const Operand& b0, const Operand& a1, const 
 }
 
 struct Plan {
-    int planes, ldd;       // planes of an operand, padded dim
+    int planes, gplanes;   // planes of an operand, of G
+    int ldd;               // padded dim
     bool pack_w;           // the weight is packed piece by piece
     long piece, pieces;    // vocabulary entries a piece
     int split_h, split_w;  // K splits of dhidden, dweight
@@ -868,7 +876,7 @@ long up(long n, long to) { return (n + to - 1) / to * to; }
 // where that fills the SMs' waves of tiles better (a launch whose last wave has a few tiles idles the rest).
 void pick_pieces(Plan* p, long n, long v, long d, bool bwd) {
     long most = v;
-    if (bwd) most = kPieceElems / (n * p->planes);
+    if (bwd) most = kPieceElems / (n * p->gplanes);
     if (p->pack_w && kPieceElems / ((long)p->ldd * p->planes) < most) most = kPieceElems / ((long)p->ldd * p->planes);
     if (most < 1024) most = 1024;
     const long least = (v + most - 1) / most;
@@ -905,7 +913,8 @@ int even_splits(long n, long d, long piece, int split) {
 // top: entries a row of a teacher's logits; 0 for the loss against single targets.
 Plan plan(const ews_vocab_args* a, bool bwd, int top = 0) {
     Plan p{};
-    p.planes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
+    p.planes = p.gplanes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
+    if (top && p.planes == 1 && a->rows * a->vocab <= kTwoPlanes / a->dim) p.gplanes = 2;
     p.ldd = (int)up(a->dim, 8);
     p.pack_w = p.planes > 1 || a->weight_stride % 8 || a->dim % 8 || !aligned16(a->weight);
     const long n = a->rows, v = a->vocab;
@@ -923,7 +932,7 @@ Plan plan(const ews_vocab_args* a, bool bwd, int top = 0) {
         const long tiles = p.pieces * ((p.piece + tile_n(p.piece) - 1) / tile_n(p.piece));
         p.part = take(sizeof(float2) * 2 * tiles * n);
     } else {
-        p.g = take(sizeof(bf16) * (size_t)p.planes * n * up(p.piece, 8));
+        p.g = take(sizeof(bf16) * (size_t)p.gplanes * n * up(p.piece, 8));
         const long th = ((n + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
         const long tw = ((p.piece + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
         p.split_h = splits_of(n, a->dim, p.piece, tw);
@@ -1023,7 +1032,7 @@ int backward(const ews_vocab_args* a, const Plan& p, const Entries* e, cudaStrea
     base.status = a->status;
     targets(&base, e);
     base.live = plan.live, base.target = plan.target, base.row = plan.row, base.lse = a->lse, base.dloss = a->dloss;
-    base.g = reinterpret_cast<bf16*>(w + p.g), base.planes = p.planes;
+    base.g = reinterpret_cast<bf16*>(w + p.g), base.planes = p.gplanes;
     for (long v0 = 0; rc == EWS_OK && v0 < a->vocab; v0 += p.piece) {
         const long n = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
         if ((rc = operands<T>(a, p, w, v0, n, &h, &wt, s)) != EWS_OK) break;
@@ -1031,7 +1040,7 @@ int backward(const ews_vocab_args* a, const Plan& p, const Entries* e, cudaStrea
         g.job[0] = job_of(a->rows, n, a->dim, 1), g.v0 = (int)v0;
         g.ldg = up(n, 8), g.g_plane = a->rows * g.ldg;
         if ((rc = gemm<GRAD>(g, h, wt, none, none, p.planes, s)) != EWS_OK) break;
-        go.p = g.g, go.rows = a->rows, go.cols = n, go.ld = g.ldg, go.plane = g.g_plane, go.planes = p.planes;
+        go.p = g.g, go.rows = a->rows, go.cols = n, go.ld = g.ldg, go.plane = g.g_plane, go.planes = p.gplanes;
         Gemm o = base;
         T* out = static_cast<T*>(a->dweight) + (a->dweight ? v0 * a->dim : 0);
         if (a->dhidden) {  // dH += G W: K is the piece of the vocabulary
