@@ -821,6 +821,7 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
         const F<V> ta = A * pa, td = fma(A, pd, D);
         if (t.tt == a.tiles - 1) {
             if (a.dfinal) g = load_channels<V>(a.dfinal + (long)t.b * a.channels, c, a.channels);
+            __syncthreads();  // every warp has read the maps, one of which the rate's sum replaces
         } else {
             if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
             __syncthreads();
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
         for (int l = live; l < QL; ++l) row[l * 32].fill(0.f), row[STREAM + l * 32].fill(0.f), row[2 * STREAM + l * 32].fill(0.f);
         tc5::fence_async_smem();
         if (a.drate_part) {  // of the tile, the warps in order
-            sh.D[warp][lane] = sum;  // read last before the look-back
+            sh.D[warp][lane] = sum;
             __syncthreads();
             if (warp == 0) {
                 F<V> total_sum(0.f);

@@ -648,6 +648,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ i
             keys[warp][i] = id[k];
         }
     }
+    __syncwarp();  // the keys
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
     if (__any_sync(kFull, bad)) top = NAN;

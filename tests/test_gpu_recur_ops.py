@@ -365,3 +365,25 @@ def test_refusals_on_the_device(ews):
     (g,) = torch.autograd.grad(rec(leaf, decay, gate, rate).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_broadcast_inputs(ews, dtype):
+    """Inputs without memory of their own along the samples or the tokens; their gradients are the sums over what they stand for."""
+    B, T, C = 3, 100, 32
+    x, decay, gate, rate, s0, do, ds = inputs(dtype, B, T, C)
+    one, two, three = x[:1].clone().requires_grad_(), decay[:, :1].clone().requires_grad_(), gate[:1, :1].clone().requires_grad_()
+    given = [t.expand(B, T, C) for t in (one, two, three)]
+    out = ews.gated_recurrence(*given, rate)
+    whole = [t.detach().contiguous().requires_grad_() for t in given]
+    want = ews.gated_recurrence(*whole, rate)
+    args = (*(t.detach() for t in whole), rate, None, None, do, None)
+    value, ab = reference(*args), reference(*args, absolute=True)
+    check(out.detach(), value[0], ab[0], T, "h")
+    check(want.detach(), value[0], ab[0], T, "h")
+    grads = torch.autograd.grad(out, (one, two, three), do)
+    for g, v, a, axes in zip(grads, value[2:5], ab[2:5], ((0,), (1,), (0, 1))):
+        # the sum that autograd forms of the operator's gradients, each rounded (bfloat16: half a step), in the inputs' type
+        n = B * T
+        bound = ((2 * T * 2.0**-23 + 2.0**-19) * a).sum(axes, keepdim=True) + n * torch.finfo(dtype).eps * a.sum(axes, keepdim=True)
+        assert ((g.double() - v.sum(axes, keepdim=True)).abs() <= bound + 1e-30).all()
