@@ -209,6 +209,8 @@ class EWSLookbackTimeout(EWSLibraryError):
 def load(path: str = LIB_PATH) -> ctypes.CDLL:
     """Loads the library (once). Raises if it has not been built."""
     global _lib
+    if _lib is not None:  # every call asks
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -1051,9 +1051,8 @@ int launched() { return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAU
 
 template <typename T, int EPI, int BN>
 int gemm(const Maps& maps, const Gemm& g, cudaStream_t s) {
-    auto* kern = gemm_kernel<T, EPI, BN>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
-    kern<<<(unsigned)g.ctas, NTH, Tile<BN>::bytes, s>>>(maps, g);
+    if (!allow_shared<gemm_kernel<T, EPI, BN>>((int)Tile<BN>::bytes)) return EWS_ERR_LAUNCH;
+    gemm_kernel<T, EPI, BN><<<(unsigned)g.ctas, NTH, Tile<BN>::bytes, s>>>(maps, g);
     const int left = g.job[0].left + g.job[1].left + g.job[2].left;
     if constexpr (EPI == OUT)
         if (left) join_kernel<T, BN><<<(unsigned)left * 8, 256, 0, s>>>(g);
@@ -1115,9 +1114,8 @@ int run_served(const ews_gated_args* a, const Operand& x, const Operand& wg, con
     const Served v{(int)a->rows, (int)a->inner, a->activation, (int)((a->dim + BK - 1) / BK), BN > 64 ? (grid <= SMS ? 6 : 3) : grid <= SMS ? 8 : 4,
                    static_cast<bf16*>(a->out), a->kept, kept_plane(a), a->status};
     constexpr int stage = BM * BK * 2 + BN * BK * 2, rest = 1024 + 256;
-    auto* kern = served_kernel<BN>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (BN > 64 ? 6 : 8) * stage + rest) != cudaSuccess) return EWS_ERR_LAUNCH;
-    kern<<<grid, SERVED_T, v.stages * stage + rest, s>>>(mg, mu, mx, v);
+    if (!allow_shared<served_kernel<BN>>((BN > 64 ? 6 : 8) * stage + rest)) return EWS_ERR_LAUNCH;
+    served_kernel<BN><<<grid, SERVED_T, v.stages * stage + rest, s>>>(mg, mu, mx, v);
     return launched();
 }
 

@@ -987,13 +987,12 @@ bool even(const ews_recur_args* a, const Stream<T>& s) {
 
 // A stream (batch, steps, channels) for TMA: boxes of 128 bytes of channels by a tile's steps. False where it cannot be read so.
 template <typename T>
-bool make_map(CUtensorMap* map, const ews_recur_args* a, const void* p, long sb, long st) {
+bool make_map(tc5::EncodeFn enc, CUtensorMap* map, const ews_recur_args* a, const void* p, long sb, long st) {
     constexpr long E = 16 / sizeof(T);
     const long one = (a->channels + E - 1) / E * E;  // an axis of one has no stride to speak of
     if (a->steps == 1) st = one;
     if (a->batch == 1) sb = st * a->steps;
     if (!aligned16(p) || st <= 0 || sb <= 0 || st % E || sb % E || a->channels % E) return false;
-    tc5::EncodeFn enc = tc5::encoder();
     if (!enc) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)a->channels, (cuuint64_t)a->steps, (cuuint64_t)a->batch};
     const cuuint64_t strides[2] = {(cuuint64_t)st * sizeof(T), (cuuint64_t)sb * sizeof(T)};
@@ -1001,6 +1000,14 @@ bool make_map(CUtensorMap* map, const ews_recur_args* a, const void* p, long sb,
     return enc(map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims, strides,
                box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <auto K, typename T>
+int piped_launch(const Params<T>& p, const Maps& m, size_t bytes, int threads, int resident, cudaStream_t s) {
+    if (!tc5::allow_shared<K>((int)bytes)) return EWS_ERR_LAUNCH;
+    const long most = (long)SMS * resident;
+    K<<<(unsigned)(p.total < most ? p.total : most), threads, bytes, s>>>(p, m);
+    return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
 template <typename T>
@@ -1033,13 +1040,14 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     p.total = ctas;
     Maps m{};
     const long C = a->channels, whole = (long)a->steps * C;
-    bool piped = a->steps >= kPipedFrom && make_map<T>(&m.in[0], a, a->x, p.x.sb, p.x.st) &&
-                 make_map<T>(&m.in[1], a, a->decay, p.decay.sb, p.decay.st) && make_map<T>(&m.in[2], a, a->gate, p.gate.sb, p.gate.st);
+    const tc5::EncodeFn enc = a->steps >= kPipedFrom ? tc5::encoder() : nullptr;
+    bool piped = enc && make_map<T>(enc, &m.in[0], a, a->x, p.x.sb, p.x.st) &&
+                 make_map<T>(enc, &m.in[1], a, a->decay, p.decay.sb, p.decay.st) && make_map<T>(enc, &m.in[2], a, a->gate, p.gate.sb, p.gate.st);
     if (bwd)
-        piped = piped && a->dout && make_map<T>(&m.in[3], a, a->dout, p.dout.sb, p.dout.st) && make_map<T>(&m.out[0], a, a->dx, whole, C) &&
-                make_map<T>(&m.out[1], a, a->ddecay, whole, C) && make_map<T>(&m.out[2], a, a->dgate, whole, C);
+        piped = piped && a->dout && make_map<T>(enc, &m.in[3], a, a->dout, p.dout.sb, p.dout.st) && make_map<T>(enc, &m.out[0], a, a->dx, whole, C) &&
+                make_map<T>(enc, &m.out[1], a, a->ddecay, whole, C) && make_map<T>(enc, &m.out[2], a, a->dgate, whole, C);
     else
-        piped = piped && make_map<T>(&m.out[0], a, a->out, whole, C);
+        piped = piped && make_map<T>(enc, &m.out[0], a, a->out, whole, C);
     using One = Shape<1>;
     using Two = Shape<2>;
     using Word = Shape<4 / sizeof(T)>;
@@ -1049,16 +1057,10 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
         kernel<<<(unsigned)ctas, warps * 32, 0, s>>>(p);
         return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
     };
-    auto go_piped = [&](auto* kernel, size_t bytes, int threads, int resident) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return (int)EWS_ERR_LAUNCH;
-        const long most = (long)SMS * resident;
-        kernel<<<(unsigned)(ctas < most ? ctas : most), threads, bytes, s>>>(p, m);
-        return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
-    };
     int rc;
     if (piped) {
-        rc = bwd ? go_piped(backward_tma_kernel<T>, Pipe<4, 3, QSTAGES>::bytes, Word::QW * 32, Word::QCTAS)
-                 : go_piped(forward_tma_kernel<T>, Pipe<3, 1, PSTAGES>::bytes, PW * 32, PCTAS);
+        rc = bwd ? piped_launch<backward_tma_kernel<T>>(p, m, Pipe<4, 3, QSTAGES>::bytes, Word::QW * 32, Word::QCTAS, s)
+                 : piped_launch<forward_tma_kernel<T>>(p, m, Pipe<3, 1, PSTAGES>::bytes, PW * 32, PCTAS, s);
     } else if constexpr (sizeof(T) == 2) {
         if (pairs) rc = bwd ? go(backward_kernel<T, 2>) : go(forward_kernel<T, 2>);
         else rc = bwd ? go(backward_kernel<T, 1>) : go(forward_kernel<T, 1>);

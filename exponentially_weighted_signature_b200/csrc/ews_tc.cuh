@@ -4,6 +4,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "ews_token.cuh"
 
 namespace ews {
@@ -255,6 +257,19 @@ inline EncodeFn encoder() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
     return fn;
+}
+
+// A kernel's dynamic shared memory, asked for once a device.
+template <auto K>
+bool allow_shared(int bytes) {
+    static std::atomic<unsigned long long> seen{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (seen.load(std::memory_order_relaxed) & bit) return true;
+    if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    seen.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
 }  // namespace tc5

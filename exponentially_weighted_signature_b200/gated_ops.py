@@ -37,10 +37,10 @@ def _forward(x, wg, wu, act, shape, keep):
     ask for."""
     (x, xs), (wg, gs), (wu, us) = x, wg, wu
     rows, dim = x.shape
-    inner, code, device = wg.shape[0], _DTYPES[x.dtype], x.device
+    inner, code = wg.shape[0], _DTYPES[x.dtype]
     xp, gp, up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
-    out = torch.empty(shape, dtype=x.dtype, device=device)
-    kept = torch.empty(_kept_size(rows, dim, inner, code), dtype=torch.uint8, device=device) if keep else None
+    out = x.new_empty(shape)
+    kept = _work(_kept_size(rows, dim, inner, code), x) if keep else None
     work, size = 0, 0
     if code != _BF16 or (xs | gs | us | dim) & 7 or (xp | gp | up) & 15:  # else nothing is packed
         size = _size(rows, dim, inner, code, (xs, gs, us), (xp % 16, gp % 16, up % 16), (0, 0, 0), 0)
@@ -69,14 +69,14 @@ class _Gated(torch.autograd.Function):
         act, xs, gs, us = ctx.meta
         (rows, dim), inner, code = x.shape, wg.shape[0], _DTYPES[x.dtype]
         dout, ds = _operand(dout if dout.dim() == 2 else dout.reshape(rows, inner))
-        dx, dwg, dwu = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+        dx, dwg, dwu = (t.new_empty(t.shape) if need else None
                         for t, need in zip((x, wg, wu), ctx.needs_input_grad))
         xp, gp, up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
         size = _size(rows, dim, inner, code, (xs, gs, us), (xp % 16, gp % 16, up % 16),
                      (int(dx is not None), int(dwg is not None), int(dwu is not None)), 1)
         work = _work(size, x)
         idx = x.get_device()
-        args = _GATED(rows, dim, inner, code, act, xp, gp, up, xs, gs, us, 0, kept.data_ptr(), dout.data_ptr(), ds, _addr(dx), _addr(dwg),
+        args = _GATED(rows, dim, inner, code, act, xp, gp, up, xs, gs, us, 0, _addr(kept), dout.data_ptr(), ds, _addr(dx), _addr(dwg),
                       _addr(dwu), _addr(work), size, engine.index_word(idx)[0])
         _launch(idx, "ews_gated_bwd", rows, _lib.load().ews_gated_bwd, args)
         return dx, dwg, dwu, None, None

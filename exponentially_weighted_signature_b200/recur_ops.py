@@ -27,11 +27,11 @@ def _sizes(B: int, T: int, C: int, code: int):
 
 
 def _forward(x, decay, gate, rate, initial, lengths, want_state, want_carry):
-    (B, T, C), device, code = x.shape, x.device, _DTYPES[x.dtype]
+    (B, T, C), code = x.shape, _DTYPES[x.dtype]
     carry_bytes, size, _ = _sizes(B, T, C, code)
-    out = torch.empty((B, T, C), dtype=x.dtype, device=device)
-    end = torch.empty((B, C), dtype=torch.float32, device=device) if want_state else None
-    carry = torch.empty(carry_bytes // 4, dtype=torch.float32, device=device) if want_carry else None
+    out = x.new_empty((B, T, C))
+    end = rate.new_empty((B, C)) if want_state else None
+    carry = rate.new_empty(carry_bytes // 4) if want_carry else None
     work = _work(size, x)
     idx, xs, ds, gs = x.get_device(), x.stride(), decay.stride(), gate.stride()
     args = _RECUR(B, T, C, code, x.data_ptr(), decay.data_ptr(), gate.data_ptr(), xs[0], xs[1], ds[0], ds[1], gs[0], gs[1], rate.data_ptr(),
@@ -54,12 +54,12 @@ class _Recurrence(torch.autograd.Function):
     @first_order
     def backward(ctx, dout, dend):
         x, decay, gate, rate, initial, lengths, carry = ctx.saved_tensors
-        (B, T, C), device, dtype, code = x.shape, x.device, x.dtype, _DTYPES[x.dtype]
+        (B, T, C), code = x.shape, _DTYPES[x.dtype]
         dout = None if dout is None else _last_contiguous(dout)
         dend = None if dend is None else dend.contiguous()
-        dx, ddecay, dgate = (torch.empty((B, T, C), dtype=dtype, device=device) for _ in range(3))
-        drate = torch.empty(C, dtype=torch.float32, device=device) if ctx.needs_input_grad[3] else None
-        d0 = torch.empty((B, C), dtype=torch.float32, device=device) if ctx.needs_input_grad[4] else None
+        dx, ddecay, dgate = x.new_empty((B, T, C)), x.new_empty((B, T, C)), x.new_empty((B, T, C))
+        drate = rate.new_empty(C) if ctx.needs_input_grad[3] else None
+        d0 = rate.new_empty((B, C)) if ctx.needs_input_grad[4] else None
         size = _sizes(B, T, C, code)[2]
         work = _work(size, x)
         idx, xs, ds, gs = x.get_device(), x.stride(), decay.stride(), gate.stride()
@@ -146,7 +146,7 @@ def gated_recurrence_step(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tens
     if (x1 != 1 or d1 != 1 or g1 != 1) and C > 1:
         x, decay, gate = x.contiguous(), decay.contiguous(), gate.contiguous()
         xs = ds = gs = C
-    out = torch.empty((B, C), dtype=x.dtype, device=x.device)
+    out = x.new_empty((B, C))
     args = _RECUR(B, 1, C, _DTYPES[x.dtype], x.data_ptr(), decay.data_ptr(), gate.data_ptr(), xs, 0, ds, 0, gs, 0, rate.data_ptr(),
                   0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, engine.index_word(idx)[0])
     _launch(idx, "ews_recur_step", B, _lib.load().ews_recur_step, args, 0 if slots is None else slots.data_ptr(), pool[0],

@@ -33,6 +33,7 @@ _VOCAB = struct.Struct("@3q2i3P3q7PNP").pack
 _TOP = struct.Struct("@2P3ifP").pack  # what ews_distill_args has behind its ews_vocab_args
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without building a Stream
+_current_device = torch._C._cuda_getDevice  # a tensor on the device exists, so CUDA has been set up
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -68,7 +69,7 @@ def _device(*tensors) -> int:
 
 def _launch(idx: int, name: str, units: int, fn, *args) -> None:
     """One library call on the device's current stream."""
-    if engine.PROFILE is None and idx == torch.cuda.current_device():
+    if engine.PROFILE is None and idx == _current_device():
         rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx), _timed(name, torch.device("cuda", idx), units):
@@ -454,7 +455,7 @@ class _DistillLoss(torch.autograd.Function):
         inv_tau, top, hs, ws = ctx.meta
         (rows, dim), vocab, code = h.shape, w.shape[0], _DTYPES[h.dtype]
         dloss = dloss.contiguous()
-        dh, dw = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+        dh, dw = (t.new_empty(t.shape) if need else None
                   for t, need in ((h, ctx.needs_input_grad[0]), (w, ctx.needs_input_grad[1])))
         wp, lse = w.data_ptr(), kept.data_ptr()
         size = _distill_size(rows, vocab, dim, code, hs, ws, wp % 16, top, 1)
