@@ -17,10 +17,10 @@
 // stream), from which the tile runs the recurrence again. So the gradient of the rates, a float32 sum over all tokens, does not
 // see the rounding of the stored states, and a stream less is read.
 //
-// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 77 us forwards (four streams, 3.5 TB/s) and 142 back (seven, 3.3),
-// float32 109 and 179 us (4.9 and 5.2 TB/s). bfloat16 is bound by the gates, of which the SM issues at half its rate at best:
+// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 76 us forwards (four streams, 3.5 TB/s) and 143 back (seven, 3.3),
+// float32 107 and 173 us (5.0 and 5.4 TB/s). bfloat16 is bound by the gates, of which the SM issues at half its rate at best:
 // with the exponent unit for every decay 81 and 153 us, without the gates' arithmetic 60 and 134, without the look-back too 56 and
-// 116. One sample of 17,984 tokens: 118 and 185 us, 79 and 146 without the look-back: 32 chains of tiles, 18 of each in work at a
+// 116. One sample of 17,984 tokens: 111 and 181 us, 79 and 146 without the look-back: 32 chains of tiles, 18 of each in work at a
 // time, wait for one another's maps and states (folding 12 or 16 tiles at once instead of 4 changed nothing).
 #include <float.h>
 
@@ -265,10 +265,41 @@ __device__ __forceinline__ Tile tile_of(const Params<T>& a, int ticket, bool dow
 
 template <int V, int WARPS, bool BACK>
 struct Shared {
-    F<V> A[WARPS][32], H[WARPS][32], D[BACK ? WARPS : 1][32];
+    F<V> A[WARPS][32], H[WARPS][32], D[BACK ? WARPS : 1][32];  // the warps' maps of the tile
+    F<V> before_a[WARPS][32], before_h[WARPS][32];             // the tiles' that a look-back folds
     unsigned kind[WARPS][32];
+    F<V> sum[BACK ? 2 : 1][BACK ? WARPS : 1][32];  // the rate's gradient, of this tile and of the last
     int ticket;
 };
+
+// The maps of the warps in front of this one (h -> pa h + ph), and of those behind it. All are read at once, those that
+// do not count as the identity: one after the other, each would wait for shared memory (a prompt of 17,984 tokens: 118 -> 111 us).
+template <int V, int WARPS, bool BACK>
+__device__ __forceinline__ void fold_front(const Shared<V, WARPS, BACK>& sh, int warp, int lane, F<V>* pa, F<V>* ph) {
+    F<V> A[WARPS], H[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS - 1; ++w) {
+        A[w] = F<V>(1.f), H[w] = F<V>(0.f);
+        if (w < warp) A[w] = sh.A[w][lane], H[w] = sh.H[w][lane];
+    }
+    F<V> a(1.f), h(0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS - 1; ++w) a = a * A[w], h = fma(A[w], h, H[w]);
+    *pa = a, *ph = h;
+}
+template <int V, int WARPS, bool BACK>
+__device__ __forceinline__ void fold_behind(const Shared<V, WARPS, BACK>& sh, int warp, int lane, F<V>* pa, F<V>* pd) {
+    F<V> A[WARPS], D[WARPS];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) {
+        A[w] = F<V>(1.f), D[w] = F<V>(0.f);
+        if (w > warp) A[w] = sh.A[w][lane], D[w] = sh.D[w][lane];
+    }
+    F<V> a(1.f), d(0.f);
+#pragma unroll
+    for (int w = WARPS - 1; w > 0; --w) a = a * A[w], d = fma(A[w], d, D[w]);
+    *pa = a, *pd = d;
+}
 
 // V consecutive floats of the lane's channels; what lies beyond the last is not touched.
 template <int V>
@@ -325,8 +356,8 @@ __device__ __forceinline__ uint2* slot_of(const Params<T>& a, const Tile& t, int
 }
 
 // The state that comes into the tile from the tiles before it (down: behind it). Every thread of the CTA calls it, after the
-// tile's own map was published; false when a wait ran out.
-template <typename T, int V, int WARPS, bool BACK>
+// tile's own map was published; false when a wait ran out. AT_ONCE: as fold_front, where there are registers for it.
+template <bool AT_ONCE, typename T, int V, int WARPS, bool BACK>
 __device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, bool down, Shared<V, WARPS, BACK>& sh, int warp, int lane, int warps, F<V>* state) {
     const int before = down ? a.tiles - 1 - t.tt : t.tt;  // how many there are
     const int window = before < warps ? before : warps;
@@ -341,15 +372,29 @@ __device__ __forceinline__ bool look_back(const Params<T>& a, const Tile& t, boo
             kind = await<V>(p + a.channels, warp == window - 1 ? kState : kMap, a.st, &H);
             ok = kind != 0 && (kind == kState || await<V>(p, kMap, a.st, &A) != 0);
         }
-        sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.kind[warp][lane] = kind;
+        sh.before_a[warp][lane] = A, sh.before_h[warp][lane] = H, sh.kind[warp][lane] = kind;
     }
     if (!__syncthreads_and(ok)) return false;
     // from the furthest state on; where a nearer tile has its own already, that is the same number
     F<V> h(0.f);
-    for (int w = window - 1; w >= 0; --w) {
-        const F<V> H = sh.H[w][lane];
-        if (sh.kind[w][lane] == kState) h = H;
-        else h = fma(sh.A[w][lane], h, H);
+    if constexpr (AT_ONCE) {
+        F<V> A[WARPS], H[WARPS];
+        unsigned kind[WARPS];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            kind[w] = kMap, A[w] = F<V>(1.f), H[w] = F<V>(0.f);
+            if (w < window) kind[w] = sh.kind[w][lane], A[w] = sh.before_a[w][lane], H[w] = sh.before_h[w][lane];
+        }
+#pragma unroll
+        for (int w = WARPS - 1; w >= 0; --w) {
+            const F<V> n = fma(A[w], h, H[w]);
+            h = kind[w] == kState ? H[w] : n;
+        }
+    } else {
+        for (int w = window - 1; w >= 0; --w) {
+            const F<V> A = sh.before_a[w][lane], H = sh.before_h[w][lane];
+            h = sh.kind[w][lane] == kState ? H : fma(A, h, H);
+        }
     }
     *state = h;
     return true;
@@ -423,19 +468,14 @@ __global__ void __launch_bounds__(Shape<V>::FW * 32, Shape<V>::FCTAS) forward_ke
     F<V> pa(1.f), ph(0.f), h(0.f);
     sh.A[warp][lane] = A, sh.H[warp][lane] = H;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) {
-        const F<V> m = sh.A[w][lane];
-        pa = pa * m;
-        ph = fma(m, ph, sh.H[w][lane]);
-    }
+    for (int w = 0; w < warp; ++w) pa = pa * sh.A[w][lane], ph = fma(sh.A[w][lane], ph, sh.H[w][lane]);
     const bool last = warp == warps - 1;
     const F<V> ta = A * pa, th = fma(A, ph, H);
     if (t.tt == 0) {
         if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
     } else {
         if (last) publish_map<T, V>(a, t, lane, ta, th);
-        __syncthreads();  // every warp has read the maps
-        if (!look_back(a, t, false, sh, warp, lane, warps, &h)) {
+        if (!look_back<false>(a, t, false, sh, warp, lane, warps, &h)) {
             if (threadIdx.x == 0) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
             return;
         }
@@ -530,18 +570,13 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
     sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
     __syncthreads();
     for (int w = 0; w < warp; ++w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
-    for (int w = warps - 1; w > warp; --w) {
-        const F<V> m = sh.A[w][lane];
-        pa = pa * m;
-        pd = fma(m, pd, sh.D[w][lane]);
-    }
+    for (int w = warps - 1; w > warp; --w) pa = pa * sh.A[w][lane], pd = fma(sh.A[w][lane], pd, sh.D[w][lane]);
     const F<V> ta = A * pa, td = fma(A, pd, D);
     if (t.tt == a.tiles - 1) {
         if (a.dfinal) g = load_channels<V>(a.dfinal + (long)t.b * a.channels, c, a.channels);
     } else {
         if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
-        __syncthreads();
-        if (!look_back(a, t, true, sh, warp, lane, warps, &g)) {
+        if (!look_back<false>(a, t, true, sh, warp, lane, warps, &g)) {
             if (threadIdx.x == 0) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
             return;
         }
@@ -577,12 +612,11 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
     if (near) slopes(std::true_type());
     else slopes(std::false_type());
     if (a.drate_part) {  // of the tile, the warps in order
-        __syncthreads();
-        sh.H[warp][lane] = sum;
+        sh.sum[0][warp][lane] = sum;
         __syncthreads();
         if (warp == 0) {
             F<V> s(0.f);
-            for (int w = 0; w < warps; ++w) s = s + sh.H[w][lane];
+            for (int w = 0; w < warps; ++w) s = s + sh.sum[0][w][lane];
             store_channels<V>(a.drate_part + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, s);
         }
     }
@@ -708,26 +742,21 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
         };
         if (is_near(rate)) gates(std::true_type());
         else gates(std::false_type());
-        F<V> pa(1.f), ph(0.f), h(0.f);
+        F<V> pa, ph, h(0.f);
         sh.A[warp][lane] = A, sh.H[warp][lane] = H;
         if (threadIdx.x == 0) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             pipe.load(a, maps, stage, s == 0 ? PSTAGES - 1 : s - 1, next, false);
         }
         __syncthreads();
-        for (int w = 0; w < warp; ++w) {
-            const F<V> m = sh.A[w][lane];
-            pa = pa * m;
-            ph = fma(m, ph, sh.H[w][lane]);
-        }
+        fold_front(sh, warp, lane, &pa, &ph);
         const bool last = warp == PW - 1;
         const F<V> ta = A * pa, th = fma(A, ph, H);
         if (t.tt == 0) {
             if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
         } else {
             if (last) publish_map<T, V>(a, t, lane, ta, th);
-            __syncthreads();  // every warp has read the maps
-            if (!(ok = look_back(a, t, false, sh, warp, lane, PW, &h))) break;
+            if (!(ok = look_back<true>(a, t, false, sh, warp, lane, PW, &h))) break;
         }
         if (last) {
             const F<V> end = fma(ta, h, th);
@@ -766,8 +795,15 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
     int s = 0, it = 0;
     uint32_t phase = 0;
     bool ok = true;
+    Tile last{};
     for (;; ++it) {
         if (!(ok = pipe.arrive(s, phase))) break;
+        if (it > 0 && warp == QW - 1 && a.drate_part) {  // the last tile's, the warps in order
+            F<V> total(0.f);
+#pragma unroll
+            for (int w = 0; w < QW; ++w) total = total + sh.sum[(it - 1) & 1][w][lane];
+            store_channels<V>(a.drate_part + ((long)last.b * a.tiles + last.tt) * a.channels, last.c0 + lane * V, a.channels, total);
+        }
         const Tile t = pipe.tile[s];
         if (t.b < 0) break;
         long next = 0;
@@ -805,27 +841,22 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
         };
         if (near) gates(std::true_type());
         else gates(std::false_type());
-        F<V> pa(1.f), pd(0.f), g(0.f);
+        F<V> pa, pd, g(0.f);
         sh.A[warp][lane] = A, sh.H[warp][lane] = H, sh.D[warp][lane] = D;
         if (threadIdx.x == 0) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             pipe.load(a, maps, stage, s == 0 ? QSTAGES - 1 : s - 1, next, true);
         }
         __syncthreads();
-        for (int w = 0; w < warp; ++w) h = fma(sh.A[w][lane], h, sh.H[w][lane]);
-        for (int w = QW - 1; w > warp; --w) {
-            const F<V> m = sh.A[w][lane];
-            pa = pa * m;
-            pd = fma(m, pd, sh.D[w][lane]);
-        }
+        fold_front(sh, warp, lane, &pa, &pd);
+        h = fma(pa, h, pd);
+        fold_behind(sh, warp, lane, &pa, &pd);
         const F<V> ta = A * pa, td = fma(A, pd, D);
         if (t.tt == a.tiles - 1) {
             if (a.dfinal) g = load_channels<V>(a.dfinal + (long)t.b * a.channels, c, a.channels);
-            __syncthreads();  // every warp has read the maps, one of which the rate's sum replaces
         } else {
             if (warp == 0) publish_map<T, V>(a, t, lane, ta, td);
-            __syncthreads();
-            if (!(ok = look_back(a, t, true, sh, warp, lane, QW, &g))) break;
+            if (!(ok = look_back<true>(a, t, true, sh, warp, lane, QW, &g))) break;
         }
         if (warp == 0) {
             const F<V> end = fma(ta, g, td);
@@ -851,15 +882,8 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
         else slopes(std::false_type());
         for (int l = live; l < QL; ++l) row[l * 32].fill(0.f), row[STREAM + l * 32].fill(0.f), row[2 * STREAM + l * 32].fill(0.f);
         tc5::fence_async_smem();
-        if (a.drate_part) {  // of the tile, the warps in order
-            sh.D[warp][lane] = sum;
-            __syncthreads();
-            if (warp == 0) {
-                F<V> total_sum(0.f);
-                for (int w = 0; w < QW; ++w) total_sum = total_sum + sh.D[w][lane];
-                store_channels<V>(a.drate_part + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, total_sum);
-            }
-        }
+        sh.sum[it & 1][warp][lane] = sum;
+        last = t;
         if (++s == QSTAGES) s = 0, phase ^= 1u;
     }
     pipe.finish(maps, stage, s, phase, it > 0, ok, a.status);
