@@ -765,12 +765,16 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ a
             if (at >= 0) {
                 const float* p = acc + at * n + c * W;
                 Vec<float, VEC>::load(p, s);
-#pragma unroll 8
-                for (int k = 1; k < splits; ++k) {
-                    float v[W];
-                    Vec<float, VEC>::load(p + k * total, v);
+                constexpr int AT_ONCE = VEC ? 2 : 8;  // in flight, added in order
+                for (int k0 = 1; k0 < splits; k0 += AT_ONCE) {
+                    float v[AT_ONCE][W];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) s[j] += v[j];
+                    for (int k = 0; k < AT_ONCE; ++k)
+                        if (k0 + k < splits) Vec<float, VEC>::load(p + (k0 + k) * total, v[k]);
+#pragma unroll
+                    for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                        for (int j = 0; j < W; ++j) s[j] = k0 + k < splits ? s[j] + v[k][j] : s[j];
                 }
             }
 #pragma unroll
@@ -899,16 +903,18 @@ void pick_pieces(Plan* p, long n, long v, long d, bool bwd) {
     }
 }
 
-// K splits of dhidden where the rows are few and their sums long: as many as bring a unit down to an SM's share of both products
-// (96 rows, V = 8,548, D = 800, float32: 524 -> 60 us for both gradients), at least eight k blocks and at most 48 to a sum.
-int even_splits(long n, long d, long piece, int split) {
-    const long td = (d + tile_n(d) - 1) / tile_n(d), th = (n + BM - 1) / BM * td, tw = (piece + BM - 1) / BM * td;
-    const long kh = (piece + BK - 1) / BK, kw = (n + BK - 1) / BK;
-    long want = kh * SMS / (th * kh + tw * kw);
-    const long most = (piece + BK * 8 - 1) / (BK * 8);
-    if (want > most) want = most;
-    if (want > 48) want = 48;
-    return want > split ? (int)want : split;
+// K splits of the gradients where one has few tiles and long sums: as many as bring a unit down to an SM's share of both products
+// (96 rows, V = 8,548, D = 800, float32: 524 -> 78 us for both gradients), at least eight k blocks and at most 48 to a sum.
+void even_splits(Plan* p, long n, long d) {
+    const long td = (d + tile_n(d) - 1) / tile_n(d), th = (n + BM - 1) / BM * td, tw = (p->piece + BM - 1) / BM * td;
+    const long kh = (p->piece + BK - 1) / BK, kw = (n + BK - 1) / BK, all = th * kh + tw * kw;
+    auto even = [&](long k, int split) {
+        long want = k * SMS / all;
+        if (want > k / 8) want = k / 8;
+        if (want > 48) want = 48;
+        return want > split ? (int)want : split;
+    };
+    p->split_h = even(kh, p->split_h), p->split_w = even(kw, p->split_w);
 }
 
 // top: entries a row of a teacher's logits; 0 for the loss against single targets.
@@ -937,8 +943,8 @@ Plan plan(const ews_vocab_args* a, bool bwd, int top = 0) {
         const long th = ((n + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
         const long tw = ((p.piece + BM - 1) / BM) * ((a->dim + tile_n(a->dim) - 1) / tile_n(a->dim));
         p.split_h = splits_of(n, a->dim, p.piece, tw);
-        if (top) p.split_h = even_splits(n, a->dim, p.piece, p.split_h);
         p.split_w = splits_of(p.piece, a->dim, n, th * p.split_h);
+        if (top) even_splits(&p, n, a->dim);
         p.acc_w = p.split_w > 1 || p.planes > 1;
         p.ah = take(sizeof(float) * (size_t)p.split_h * n * a->dim);
         if (p.acc_w) p.aw = take(sizeof(float) * (size_t)p.split_w * p.piece * a->dim);
