@@ -9,19 +9,20 @@
 // (the flow exp(-dtheta lambda) of a diagonal generator at depth one with a clock step of each token and channel, and
 // the input scaled so that unit inputs give a unit state.)
 //
-// Both directions are a scan of maps h -> A h + H. A tile is 64 tokens by 32 V channels (128 bytes a token); its warps take 8 or
-// 16 consecutive tokens each, with a and b of them in registers, so that the streams are read once. The warps' maps are joined in
-// shared memory, the tiles' by a decoupled look-back in ticket order (a tile publishes its map, then its state): a tile folds the
-// maps of up to as many tiles as it has warps onto a published state, always from the state upwards, so that the sum has one order
-// and the results do not depend on timing. The backward reads no states: the forward leaves one a tile (float32, 1 / 64 of the
-// stream), from which the tile runs the recurrence again. So the gradient of the rates, a float32 sum over all tokens, does not
-// see the rounding of the stored states, and a stream less is read.
+// Both directions are a scan of maps h -> A h + H. A tile is 64 tokens (or 32: see Back) by 32 V channels (128 bytes a token);
+// its warps take 8 or 16 consecutive tokens each, with a and b of them in registers, so that the streams are read once. The
+// warps' maps are joined in shared memory, the tiles' by a decoupled look-back in ticket order (a tile publishes its map, then
+// its state): a tile folds the maps of up to as many tiles as it has warps onto a published state, always from the state
+// upwards, so that the sum has one order and the results do not depend on timing. The backward reads no states: the forward
+// leaves one for each of its tiles (float32), from which the tile runs the recurrence again. So the gradient of the rates, a
+// float32 sum over all tokens, does not see the rounding of the stored states, and a stream less is read.
 //
-// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 76 us forwards (four streams, 3.5 TB/s) and 143 back (seven, 3.3),
+// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 76 us forwards (four streams, 3.5 TB/s) and 131 back (seven, 3.6),
 // float32 107 and 173 us (5.0 and 5.4 TB/s). bfloat16 is bound by the gates, of which the SM issues at half its rate at best:
-// with the exponent unit for every decay 81 and 153 us, without the gates' arithmetic 60 and 134, without the look-back too 56 and
-// 116. One sample of 17,984 tokens: 111 and 181 us, 79 and 146 without the look-back: 32 chains of tiles, 18 of each in work at a
-// time, wait for one another's maps and states (folding 12 or 16 tiles at once instead of 4 changed nothing).
+// with the exponent unit for every decay 81 and 153 us (backward tiles of 64 tokens), without the gates' arithmetic 60 and 134,
+// without the look-back too 56 and 116. One sample of 17,984 tokens: 111 and 181 us, 79 and 146 without the look-back: 32
+// chains of tiles, 18 of each in work at a time, wait for one another's maps and states (folding 12 or 16 tiles at once instead
+// of 4 changed nothing).
 #include <float.h>
 
 #include <type_traits>
@@ -46,9 +47,18 @@ template <int V>
 struct Shape {
     static constexpr int FL = V == 1 ? 16 : 8, FW = TILE / FL, FCTAS = V == 1 ? 8 : 3;  // forward
     static constexpr int BL = V == 1 ? 16 : 8, BW = TILE / BL, BCTAS = V == 1 ? 4 : 2;  // backward
-    static constexpr int QL = V == 1 ? 16 : 8, QW = TILE / QL, QCTAS = V == 1 ? 3 : 2;  // the same where TMA brings the tiles
 };
-constexpr int PL = 16, PW = TILE / PL, PCTAS = 4;
+constexpr int PL = 16, PW = TILE / PL, PCTAS = 4;  // the same where TMA brings the tiles
+// And backwards, in tiles of ROWS tokens: TILE or, of bfloat16 where the chains (of 64 channels a sample) fill the GPU, HALF. Then
+// more tiles are in work and fewer threads wait at a barrier; a chain of few passes through twice as many states. Tiles of 64
+// tokens and of 32, 2,048 channels, us: 256 chains x 2,048 tokens 140 and 132, 160 x 2,048 99 and 93, 128 x 4,096 144 and 147,
+// 64 x 8,192 151 and 163, 32 x 16,384 167 and 192. One tile is better than two: 8,192 chains x 40 tokens 121 and 126.
+// (float32 has a token's 32 channels a tile, and enough tiles: 8 x 2,048 x 1,024 95 and 105.)
+template <int V, int ROWS>
+struct Back {
+    static constexpr int QL = V == 1 ? 16 : 8, QW = ROWS / QL, QCTAS = V == 1 ? 3 : ROWS == TILE ? 2 : 4;
+};
+constexpr int HALF = TILE / 2;
 constexpr int PSTAGES = 2, QSTAGES = 2;
 constexpr int kPipedFrom = 33;            // steps from which it does: below, most of a tile would be empty
 constexpr float kLog2e = 1.4426950408889634f;
@@ -70,7 +80,8 @@ struct Params {
     const float *initial, *dfinal;
     T* out;
     float* final_state;
-    float* carry;  // (batch, tiles, channels): the state in front of each tile, for the backward
+    float* carry;  // (batch, carries, channels): the state in front of every `apart` tokens, for the backward
+    int carries, apart;
     T *dx, *ddecay, *dgate;
     float *drate_part, *dinitial;
     // look-back
@@ -486,7 +497,8 @@ __global__ void __launch_bounds__(Shape<V>::FW * 32, Shape<V>::FCTAS) forward_ke
         else if (a.final_state) store_channels<V>(a.final_state + (long)t.b * a.channels, c, a.channels, end);
     }
     h = fma(pa, h, ph);
-    if (a.carry && warp == 0) store_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, h);
+    if (a.carry && (from & (a.apart - 1)) == 0 && from < a.steps)
+        store_channels<V>(a.carry + ((long)t.b * a.carries + (from >> (a.apart == TILE ? 6 : 5))) * a.channels, c, a.channels, h);
     T* po = a.out + ((long)t.b * a.steps + from) * a.channels + c;
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
@@ -546,7 +558,7 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
             if (l < live && a.dout.p) wg[l].load(pg);
             px += a.x.st, pr += a.decay.st, pi += a.gate.st, pg += a.dout.st;
         }
-        if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels);
+        if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.carries + t.tt * (TILE / a.apart)) * a.channels, c, a.channels);
         else if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
         auto gates = [&](auto near) {
             using K = Decay<decltype(near)::value, V>;
@@ -633,9 +645,9 @@ struct Maps {
     CUtensorMap out[3];  // h; backward: dx, ddecay, dgate
 };
 
-template <int IN, int OUTS, int STAGES>
+template <int IN, int OUTS, int STAGES, int ROWS>
 struct Pipe {
-    static constexpr int STREAM = TILE * 128, STAGE = IN * STREAM;
+    static constexpr int STREAM = ROWS * 128, STAGE = IN * STREAM;
     static constexpr size_t bytes = (size_t)STAGES * STAGE + 128;
     uint64_t full[STAGES];
     Tile tile[STAGES];  // b < 0: there is none left
@@ -661,12 +673,12 @@ struct Pipe {
         tile[s] = t;
         tc5::mbar_expect(full + s, STAGE);
 #pragma unroll
-        for (int k = 0; k < IN; ++k) tc5::tma_load(&maps.in[k], full + s, stage + s * STAGE + k * STREAM, t.c0, t.tt * TILE, t.b);
+        for (int k = 0; k < IN; ++k) tc5::tma_load(&maps.in[k], full + s, stage + s * STAGE + k * STREAM, t.c0, t.tt * ROWS, t.b);
     }
     __device__ __forceinline__ void store(const Maps& maps, unsigned char* stage, int s) {
         const Tile t = tile[s];
 #pragma unroll
-        for (int k = 0; k < OUTS; ++k) tc5::tma_store(&maps.out[k], stage + s * STAGE + k * STREAM, t.c0, t.tt * TILE, t.b);
+        for (int k = 0; k < OUTS; ++k) tc5::tma_store(&maps.out[k], stage + s * STAGE + k * STREAM, t.c0, t.tt * ROWS, t.b);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
     // All threads, at the top of a tile: its stage is there and everyone is done with the tile before. False when a wait ran out.
@@ -698,7 +710,7 @@ __device__ __forceinline__ long take_ticket(const Params<T>& a, int it) {
 template <typename T>
 __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
     constexpr int V = 4 / sizeof(T);
-    using P = Pipe<3, 1, PSTAGES>;
+    using P = Pipe<3, 1, PSTAGES, TILE>;
     using W = Word<T, V>;
     constexpr int STREAM = P::STREAM / 4;
     extern __shared__ __align__(128) unsigned char raw[];
@@ -764,7 +776,8 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
             else if (a.final_state) store_channels<V>(a.final_state + (long)t.b * a.channels, c, a.channels, end);
         }
         h = fma(pa, h, ph);
-        if (a.carry && warp == 0) store_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels, h);
+        if (a.carry && (from & (a.apart - 1)) == 0 && from < a.steps)
+            store_channels<V>(a.carry + ((long)t.b * a.carries + (from >> (a.apart == TILE ? 6 : 5))) * a.channels, c, a.channels, h);
 #pragma unroll
         for (int l = 0; l < PL; ++l) {
             h = fma(av[l], h, bv[l]);
@@ -777,11 +790,11 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
     pipe.finish(maps, stage, s, phase, it > 0, ok, a.status);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeof(T)>::QCTAS)
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(Back<4 / sizeof(T), ROWS>::QW * 32, Back<4 / sizeof(T), ROWS>::QCTAS)
     backward_tma_kernel(const __grid_constant__ Params<T> a, const __grid_constant__ Maps maps) {
-    constexpr int V = 4 / sizeof(T), QL = Shape<V>::QL, QW = Shape<V>::QW;
-    using P = Pipe<4, 3, QSTAGES>;
+    constexpr int V = 4 / sizeof(T), QL = Back<V, ROWS>::QL, QW = Back<V, ROWS>::QW;
+    using P = Pipe<4, 3, QSTAGES, ROWS>;
     using W = Word<T, V>;
     constexpr int STREAM = P::STREAM / 4;
     extern __shared__ __align__(128) unsigned char raw[];
@@ -811,7 +824,7 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
             if (it > 0) pipe.store(maps, stage, s == 0 ? QSTAGES - 1 : s - 1);
             next = take_ticket(a, it + QSTAGES - 1);
         }
-        const int c = t.c0 + lane * V, from = t.tt * TILE + warp * QL;
+        const int c = t.c0 + lane * V, from = t.tt * ROWS + warp * QL;
         const int len = a.lengths ? min(max(__ldg(a.lengths + t.b), 0), a.steps) : a.steps;
         const int live = min(max(len - from, 0), QL);
         W* row = reinterpret_cast<W*>(stage + s * P::STAGE + warp * QL * 128) + lane;
@@ -823,7 +836,7 @@ __global__ void __launch_bounds__(Shape<4 / sizeof(T)>::QW * 32, Shape<4 / sizeo
         F<V> kv[QL], rv[QL], iv[QL], hb[QL];  // as in backward_kernel
         const bool near = is_near(rate);
         F<V> A(1.f), H(0.f), D(0.f), h(0.f);
-        if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.tiles + t.tt) * a.channels, c, a.channels);
+        if (t.tt > 0) h = load_channels<V>(a.carry + ((long)t.b * a.carries + t.tt) * a.channels, c, a.channels);
         else if (a.initial) h = load_channels<V>(a.initial + (long)t.b * a.channels, c, a.channels);
         auto gates = [&](auto near) {
             using K = Decay<decltype(near)::value, V>;
@@ -984,15 +997,21 @@ int check(const ews_recur_args* a) {
 }
 
 size_t up(size_t b) { return (b + 255) / 256 * 256; }
-int tiles_of(int steps) { return (steps + TILE - 1) / TILE; }
+int tiles_of(int steps, int tile = TILE) { return (steps + tile - 1) / tile; }
 
 struct Sizes {
     size_t slots, part, bytes;  // slots: behind the status block, both cleared by a call
 };
 
+// Tokens a tile of the backward that TMA feeds, and from one state that the forward leaves to the next: see Back.
+int back_rows(const ews_recur_args* a) {
+    const bool many = (long)a->batch * ((a->channels + 63) / 64) >= SMS;
+    return a->dtype == EWS_DTYPE_BF16 && a->steps > TILE && many ? HALF : TILE;
+}
+
 Sizes sizes(const ews_recur_args* a, bool bwd) {
     Sizes z{};
-    const size_t tiles = tiles_of(a->steps), states = (size_t)a->batch * tiles * a->channels;
+    const size_t tiles = tiles_of(a->steps, bwd ? back_rows(a) : TILE), states = (size_t)a->batch * tiles * a->channels;
     if (tiles > 1) z.slots = up(sizeof(DeviceStatus) + 2 * sizeof(uint2) * states);
     if (bwd) z.part = up(sizeof(float) * states);
     z.bytes = z.slots + z.part;
@@ -1011,7 +1030,7 @@ bool even(const ews_recur_args* a, const Stream<T>& s) {
 
 // A stream (batch, steps, channels) for TMA: boxes of 128 bytes of channels by a tile's steps. False where it cannot be read so.
 template <typename T>
-bool make_map(tc5::EncodeFn enc, CUtensorMap* map, const ews_recur_args* a, const void* p, long sb, long st) {
+bool make_map(tc5::EncodeFn enc, CUtensorMap* map, const ews_recur_args* a, const void* p, long sb, long st, int rows) {
     constexpr long E = 16 / sizeof(T);
     const long one = (a->channels + E - 1) / E * E;  // an axis of one has no stride to speak of
     if (a->steps == 1) st = one;
@@ -1020,7 +1039,7 @@ bool make_map(tc5::EncodeFn enc, CUtensorMap* map, const ews_recur_args* a, cons
     if (!enc) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)a->channels, (cuuint64_t)a->steps, (cuuint64_t)a->batch};
     const cuuint64_t strides[2] = {(cuuint64_t)st * sizeof(T), (cuuint64_t)sb * sizeof(T)};
-    const cuuint32_t box[3] = {128 / sizeof(T), (cuuint32_t)TILE, 1}, es[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {128 / sizeof(T), (cuuint32_t)rows, 1}, es[3] = {1, 1, 1};
     return enc(map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims, strides,
                box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1037,7 +1056,7 @@ int piped_launch(const Params<T>& p, const Maps& m, size_t bytes, int threads, i
 template <typename T>
 int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     Params<T> p{};
-    p.batch = a->batch, p.steps = a->steps, p.channels = a->channels, p.tiles = tiles_of(a->steps);
+    p.batch = a->batch, p.steps = a->steps, p.channels = a->channels, p.apart = back_rows(a), p.carries = tiles_of(a->steps, p.apart);
     p.x = stream_of<T>(a->x, a->x_stride), p.decay = stream_of<T>(a->decay, a->decay_stride), p.gate = stream_of<T>(a->gate, a->gate_stride);
     p.rate = a->rate, p.lengths = a->lengths, p.initial = a->initial, p.carry = a->carry, p.status = a->status;
     bool pairs = sizeof(T) == 2 && a->channels % 2 == 0 && even(a, p.x) && even(a, p.decay) && even(a, p.gate);
@@ -1049,6 +1068,18 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
         p.out = static_cast<T*>(a->out), p.final_state = a->final_state;
         pairs = pairs && ((uintptr_t)a->out & 3u) == 0;
     }
+    Maps m{};
+    const int rows = bwd ? p.apart : TILE;
+    const long C = a->channels, whole = (long)a->steps * C;
+    const tc5::EncodeFn enc = a->steps >= kPipedFrom ? tc5::encoder() : nullptr;
+    bool piped = enc && make_map<T>(enc, &m.in[0], a, a->x, p.x.sb, p.x.st, rows) &&
+                 make_map<T>(enc, &m.in[1], a, a->decay, p.decay.sb, p.decay.st, rows) && make_map<T>(enc, &m.in[2], a, a->gate, p.gate.sb, p.gate.st, rows);
+    if (bwd)
+        piped = piped && a->dout && make_map<T>(enc, &m.in[3], a, a->dout, p.dout.sb, p.dout.st, rows) && make_map<T>(enc, &m.out[0], a, a->dx, whole, C, rows) &&
+                make_map<T>(enc, &m.out[1], a, a->ddecay, whole, C, rows) && make_map<T>(enc, &m.out[2], a, a->dgate, whole, C, rows);
+    else
+        piped = piped && make_map<T>(enc, &m.out[0], a, a->out, whole, C, rows);
+    p.tiles = tiles_of(a->steps, piped ? rows : TILE);
     const int width = pairs ? 64 : 32;
     p.blocks = (a->channels + width - 1) / width;
     const Sizes z = sizes(a, bwd);
@@ -1062,19 +1093,9 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
     const long ctas = (long)p.batch * p.blocks * p.tiles;
     if (ctas > 0x7FFFFFFFl - 65536) return EWS_ERR_UNSUPPORTED;  // the tickets count a little further
     p.total = ctas;
-    Maps m{};
-    const long C = a->channels, whole = (long)a->steps * C;
-    const tc5::EncodeFn enc = a->steps >= kPipedFrom ? tc5::encoder() : nullptr;
-    bool piped = enc && make_map<T>(enc, &m.in[0], a, a->x, p.x.sb, p.x.st) &&
-                 make_map<T>(enc, &m.in[1], a, a->decay, p.decay.sb, p.decay.st) && make_map<T>(enc, &m.in[2], a, a->gate, p.gate.sb, p.gate.st);
-    if (bwd)
-        piped = piped && a->dout && make_map<T>(enc, &m.in[3], a, a->dout, p.dout.sb, p.dout.st) && make_map<T>(enc, &m.out[0], a, a->dx, whole, C) &&
-                make_map<T>(enc, &m.out[1], a, a->ddecay, whole, C) && make_map<T>(enc, &m.out[2], a, a->dgate, whole, C);
-    else
-        piped = piped && make_map<T>(enc, &m.out[0], a, a->out, whole, C);
     using One = Shape<1>;
     using Two = Shape<2>;
-    using Word = Shape<4 / sizeof(T)>;
+    constexpr int V = 4 / sizeof(T);
     const int per = pairs ? (bwd ? Two::BL : Two::FL) : (bwd ? One::BL : One::FL);
     const int warps = (int)((p.tiles > 1 ? TILE : a->steps) + per - 1) / per;  // a short axis: as many as it has work for
     auto go = [&](auto* kernel) {
@@ -1082,9 +1103,16 @@ int run(const ews_recur_args* a, bool bwd, cudaStream_t s) {
         return cudaGetLastError() == cudaSuccess ? (int)EWS_OK : (int)EWS_ERR_LAUNCH;
     };
     int rc;
-    if (piped) {
-        rc = bwd ? piped_launch<backward_tma_kernel<T>>(p, m, Pipe<4, 3, QSTAGES>::bytes, Word::QW * 32, Word::QCTAS, s)
-                 : piped_launch<forward_tma_kernel<T>>(p, m, Pipe<3, 1, PSTAGES>::bytes, PW * 32, PCTAS, s);
+    auto back = [&](auto of) {
+        using B = decltype(of);
+        constexpr int ROWS = B::QL * B::QW;
+        return piped_launch<backward_tma_kernel<T, ROWS>>(p, m, Pipe<4, 3, QSTAGES, ROWS>::bytes, B::QW * 32, B::QCTAS, s);
+    };
+    if (piped && bwd) {
+        if constexpr (V == 2) rc = rows == HALF ? back(Back<V, HALF>{}) : back(Back<V, TILE>{});
+        else rc = back(Back<V, TILE>{});
+    } else if (piped) {
+        rc = piped_launch<forward_tma_kernel<T>>(p, m, Pipe<3, 1, PSTAGES, TILE>::bytes, PW * 32, PCTAS, s);
     } else if constexpr (sizeof(T) == 2) {
         if (pairs) rc = bwd ? go(backward_kernel<T, 2>) : go(forward_kernel<T, 2>);
         else rc = bwd ? go(backward_kernel<T, 1>) : go(forward_kernel<T, 1>);
@@ -1128,7 +1156,7 @@ int step(const ews_recur_args* a, const int* slots, int pool, float* state, cuda
 using namespace ews::recur;
 
 extern "C" size_t ews_recur_carry_size(const ews_recur_args* a) {
-    return check(a) == EWS_OK ? sizeof(float) * (size_t)a->batch * tiles_of(a->steps) * a->channels : 0;
+    return check(a) == EWS_OK ? sizeof(float) * (size_t)a->batch * tiles_of(a->steps, back_rows(a)) * a->channels : 0;
 }
 
 extern "C" size_t ews_recur_work_size(const ews_recur_args* a, int backward) {
@@ -1155,7 +1183,7 @@ extern "C" int ews_recur_bwd(const ews_recur_args* a, ews_stream_t stream) {
         return pass(a, a->dfinal, a->dinitial, s);
     }
     if (!a->x || !a->decay || !a->gate || !a->rate || !a->dx || !a->ddecay || !a->dgate) return EWS_ERR_INVALID_ARGUMENT;
-    if (tiles_of(a->steps) > 1 && !a->carry) return EWS_ERR_INVALID_ARGUMENT;
+    if (a->steps > TILE && !a->carry) return EWS_ERR_INVALID_ARGUMENT;
     const Sizes z = sizes(a, true);
     if (z.bytes && (!a->work || !ews::token::aligned16(a->work) || a->work_bytes < z.bytes)) return EWS_ERR_WORKSPACE;
     return a->dtype == EWS_DTYPE_BF16 ? run<ews::token::bf16>(a, true, s) : run<float>(a, true, s);

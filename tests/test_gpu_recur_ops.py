@@ -119,6 +119,31 @@ def test_outputs_and_gradients(ews, dtype, B, T, C, lengths, state):
     assert torch.equal(plain[0] if state else plain, outs[0].detach())
 
 
+@pytest.mark.parametrize("T", [64, 65, 96, 97, 140, 333])
+@pytest.mark.parametrize("C,odd", [(192, None), (192, "dout"), (192, "x"), (130, None), (129, None)])
+def test_many_chains(ews, T, C, odd):
+    """More chains of 64 channels than the GPU has multiprocessors, so that states are kept every 32 tokens: backward in tiles of
+    32 tokens, and (where a layout does not let the forward or the backward copy tiles whole) of 64 on the same states."""
+    B = 75
+    x, decay, gate, rate, s0, do, ds = inputs(BF16, B, T, C, seed=T)
+    ln = (torch.arange(B, device="cuda", dtype=torch.int32) * 37) % (T + 1)
+
+    def shifted(t):
+        wide = torch.full((*t.shape[:2], C + 9), float("nan"), dtype=BF16, device="cuda")
+        wide[..., 1 : C + 1] = t
+        return wide[..., 1 : C + 1]
+
+    leaves = [t.clone().requires_grad_() for t in (x, decay, gate, rate, s0)]
+    if odd == "x":
+        leaves[0] = shifted(x).requires_grad_()
+    out = ews.gated_recurrence(*leaves[:4], initial_state=leaves[4], lengths=ln, return_state=True)
+    grads = torch.autograd.grad(out, leaves, (shifted(do) if odd == "dout" else do, ds))
+    args = (x, decay, gate, rate, s0, ln, do, ds)
+    want, ab = reference(*args), reference(*args, absolute=True)
+    for k, (name, got) in enumerate(zip(("h", "state", "dx", "ddecay", "dgate", "drate", "dstate"), (out[0].detach(), out[1].detach(), *grads))):
+        check(got, want[k], ab[k], T if k < 2 else 2 * T, name)
+
+
 def test_the_gradient_is_the_slope(ews):
     """Against central differences of the operator's own float32 results, in 64 bits' worth of directions: the difference's
     error is its curvature (h^2) and the results' 2^-19 over h."""
