@@ -651,9 +651,12 @@ __global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Fe
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int f0 = (blockIdx.x * 4 + warp) * FS, row0 = blockIdx.y * R, rows = min(a.rows - row0, R);
     auto load = [&](const float* p, int k, float v[4]) {
-        if (VEC) return Vec<float, true>::load(p + k, v);
+        if constexpr (VEC) {
+            Vec<float, true>::load(p + k, v);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k + e < a.dim ? p[k + e] : 0.f;
+            for (int e = 0; e < 4; ++e) v[e] = k + e < a.dim ? p[k + e] : 0.f;
+        }
     };
     const float* w[2 * FS];  // rows beyond the last: the last
 #pragma unroll
