@@ -721,19 +721,24 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
         // sum p (m - z) / tau: what a student is sure of and right about cancels first; the groups take the entries in turn
         const long at = row < live ? (long)plan.row[row] * e.top : 0;
         float far = 0.f;
+        bool twice = false;  // an id occurs twice: neighbours, the entries are sorted
         if (row < live)
             for (int k = g; k < e.top; k += 8) {
                 const float p = e.prob[at + k];
                 if (p != 0.f) far += p * ((m - picked[at + k]) * e.inv_tau);
+                twice = twice || (k > 0 && e.ids[at + k] != INT_MAX && e.ids[at + k] == e.ids[at + k - 1]);
             }
         __shared__ float sums[8][32];
-        sums[g][l] = far;
+        __shared__ bool again[8][32];
+        sums[g][l] = far, again[g][l] = twice;
         __syncthreads();
         if (g > 0 || row >= live) return;
-        for (int j = 1; j < 8; ++j) far += sums[j][l];
+        for (int j = 1; j < 8; ++j) far += sums[j][l], twice = twice || again[j][l];
         const float rest = logf(s), kl = far + rest + e.self[plan.row[row]];
         lse[row] = fmaf(m, e.inv_tau, rest);
-        loss[plan.row[row]] = kl < 0.f ? 0.f : kl;  // no divergence is negative, its rounding may be
+        // Of distinct ids the sum is never negative, its rounding may be. An id that is two entries can have more of the student's
+        // probability than either of the teacher's.
+        loss[plan.row[row]] = kl < 0.f && !twice ? 0.f : kl;
         return;
     }
     // The maximum and the target's logit cancel first, exactly where the target is the maximum: a sum rounded at the

@@ -478,8 +478,8 @@ def distill_loss(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.
     a position of which none is left has loss 0 and no gradient, and costs nothing. An id that occurs twice is two entries; one
     beyond the vocabulary is absent and raises IndexError on the next call.
 
-    Returns the losses with the shape of ``hidden`` without its last axis, never negative; the logits (N, V) are formed in tiles
-    and pieces and never kept. Differentiable in hidden and weight, the teacher is a constant. (Many scale the mean by
+    Returns the losses with the shape of ``hidden`` without its last axis, never negative where a position's ids are distinct (an id
+    that is two entries can make the sum so); the logits (N, V) are formed in tiles and pieces and never kept. Differentiable in hidden and weight, the teacher is a constant. (Many scale the mean by
     temperature^2 beside another loss.)"""
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not fit together")

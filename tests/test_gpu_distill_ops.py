@@ -257,3 +257,21 @@ def test_refusals_on_the_device(ews):
     (g,) = torch.autograd.grad(f(leaf, w, ids, t).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_a_repeated_id_may_take_the_sum_below_zero(ews, dtype):
+    """An id that occurs twice is two entries, of which a student can be surer than either: 2 (p / 2) (log(p / 2) - log q) with q near
+    p is negative. Rows whose ids are distinct lie beside them; a repeated id that is absent makes no row negative."""
+    h, w, ids, t, dloss = inputs(dtype, 96, 60, 24, 6, empty=0.0)
+    h = h * 3
+    best = (h.double() @ w.double().mT).argmax(1)
+    twice = torch.arange(96, device="cuda") % 2 == 0
+    ids[twice, 1], ids[twice, 4] = best[twice], best[twice]
+    t[twice, 1], t[twice, 4] = 12.0, 12.0
+    ids[1::4, 2:4] = -1
+    got = run(ews, h, w, ids, t, 1.0, dloss)
+    want, bound = reference(h, w, ids, t, 1.0, dloss)
+    for name, a, b, c in zip(("loss", "dh", "dw"), got, want, bound):
+        check(a, b, c, name)
+    assert float(want[0].min()) < -0.3 and float(got[0].min()) < -0.3
