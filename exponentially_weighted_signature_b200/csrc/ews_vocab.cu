@@ -623,7 +623,9 @@ inline Entries entries_of(void* p, long rows, int top, float inv_tau) {
 constexpr int kMaxTop = 128;
 
 // A warp a row: the probabilities of its entries, sorted by id (equal ids keep their order). Ids below zero and logits of -inf are
-// absent, a row of which is left nothing has no target; an id beyond the vocabulary is absent and reported.
+// absent, a row of which is left nothing has no target; an id beyond the vocabulary is absent and reported. The temperature comes
+// after the row's maximum has been subtracted: before, a finite logit near its type's ends would overflow, and every logit would be
+// rounded at its own size.
 template <typename L>
 __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ ids, int wide, const L* __restrict__ logits, long rows, long vocab,
                                                       Entries e, int* status) {
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ i
     if (row >= rows) return;
     int id[E];
     float t[E], top = -INFINITY;
-    bool bad = false;
+    bool bad = false, any = false;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
         const int i = k * 32 + lane;
@@ -643,8 +645,8 @@ __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ i
             const long at = row * e.top + i;
             const long v = wide ? (long)__ldg(static_cast<const long long*>(ids) + at) : (long)__ldg(static_cast<const int*>(ids) + at);
             if (v >= vocab) report(status, EWS_ERR_INDEX);
-            const float x = to_f(logits[at]) * e.inv_tau;
-            if (v >= 0 && v < vocab && x != -INFINITY) id[k] = (int)v, t[k] = x, bad = bad || x != x, top = fmaxf(top, x);
+            const float x = to_f(logits[at]);
+            if (v >= 0 && v < vocab && x != -INFINITY) id[k] = (int)v, t[k] = x, any = true, bad = bad || x != x, top = fmaxf(top, x);
             keys[warp][i] = id[k];
         }
     }
@@ -652,10 +654,13 @@ __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ i
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
     if (__any_sync(kFull, bad)) top = NAN;
+    any = __any_sync(kFull, any);
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < E; ++k)
-        if (id[k] != INT_MAX) sum += expf(t[k] - top);
+    for (int k = 0; k < E; ++k) {
+        t[k] = (t[k] - top) * e.inv_tau;
+        if (id[k] != INT_MAX) sum += expf(t[k]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
     const float log_sum = logf(sum);
@@ -666,8 +671,8 @@ __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ i
         if (i >= e.top) continue;
         float p = 0.f;
         if (id[k] != INT_MAX) {
-            p = expf(t[k] - top) / sum;
-            if (p != 0.f) self += p * (t[k] - top - log_sum);
+            p = expf(t[k]) / sum;
+            if (p != 0.f) self += p * (t[k] - log_sum);
         }
         int rank = 0;
         for (int j = 0; j < e.top; ++j) {
@@ -679,7 +684,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ i
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) self += __shfl_xor_sync(kFull, self, o);
-    if (lane == 0) e.self[row] = self, e.flag[row] = top == -INFINITY ? -1 : 0;
+    if (lane == 0) e.self[row] = self, e.flag[row] = any ? 0 : -1;
 }
 
 // The row's logsumexp from the tiles' maxima and sums: 32 rows by 8 groups of tiles a CTA. TOP: `picked` are the entries' logits.

@@ -275,3 +275,31 @@ def test_a_repeated_id_may_take_the_sum_below_zero(ews, dtype):
     for name, a, b, c in zip(("loss", "dh", "dw"), got, want, bound):
         check(a, b, c, name)
     assert float(want[0].min()) < -0.3 and float(got[0].min()) < -0.3
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("tau", [0.5, 0.7, 2.0**-20, 3.0])
+def test_logits_at_the_types_ends(ews, dtype, tau):
+    """Only a logit of -inf is absent: the type's lowest value is a logit like others, alone in a row or beside others, at any
+    temperature, and so is its largest. A constant added to a row changes nothing but the rounding of what is given."""
+    h, w, ids, t, dloss = inputs(dtype, 9, 50, 16, 6, empty=0.0)
+    ids = ids.clamp(min=0)
+    for row in range(9):
+        ids[row] = torch.randperm(50, device="cuda", generator=torch.Generator(device="cuda").manual_seed(row))[:6]
+    t = t * min(tau, 1.0)
+    low, high = torch.finfo(FP32).min, torch.finfo(FP32).max
+    t[0] = low
+    t[1, 1:] = low
+    t[2] = high
+    t[3, 2] = high
+    t[4, :3], t[4, 3:] = low, high
+    t[5] += 1000 * min(tau, 1.0)
+    t[6, 2:] = -float("inf")
+    t[7] = -float("inf")
+    got = run(ews, h, w, ids, t, tau, dloss)
+    want, bound = reference(h, w, ids, t, tau, dloss)
+    for name, a, b, c in zip(("loss", "dh", "dw"), got, want, bound):
+        check(a, b, c, name)
+    assert (got[1][7] == 0).all() and (got[1][[0, 2]] != 0).any(1).all()
+    half = torch.where(t == low, torch.finfo(BF16).min, torch.where(t == high, torch.finfo(BF16).max, t)).to(BF16)
+    assert torch.equal(ews.distill_loss(h, w, ids, half, temperature=tau), ews.distill_loss(h, w, ids, half.float(), temperature=tau))
