@@ -103,6 +103,7 @@ struct Gemm {
     float inv_tau;        // 1 without TOP
     const int* ids;       // TOP, of the rows as they were given: (rows, top) ids in rising order, absent ones INT_MAX
     const float* prob;    // their probabilities
+    const float* base;    // what a row's logits lose before they are scaled, see lse_kernel
     float* logit;         // their logits
     int top;
     bf16* g;              // (planes, rows, ldg)
@@ -364,11 +365,15 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                     const int pick = TOP || t < 0 ? -1 : t - a.v0 - r.tn * BN;
                     const float w = t < 0 ? 0.f : a.dloss[a.row[row]] * a.inv_tau / factor;
                     const float scale = TOP ? kLog2e * a.inv_tau : kLog2e;
-                    const float lse = in ? a.lse[row] : 0.f, shift = -lse * kLog2e;
+                    const float lse = in ? a.lse[row] : 0.f, shift = -lse * kLog2e, base = TOP && in ? a.base[a.row[row]] : 0.f;
                     const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
                     for (int c = half * HALF; c < cols; c += 32) {
                         float v[32];
                         tmem_ld32(src + c, v);
+                        if constexpr (TOP) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) unpair(add2(pair(v[j], v[j + 1]), pair(-base, -base)), v[j], v[j + 1]);
+                        }
                         if (a.planes > 1) {  // float32: the scaled exponent's own rounding (2^-24 of some 15) would be the largest error
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = expf(TOP ? fmaf(v[j], a.inv_tau, -lse) : v[j] - lse);
@@ -609,7 +614,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Pack<
 // A distribution's targets: by row of the call, see the epilogues.
 struct Entries {
     int *ids, *flag;             // flag: 0 where the row has a distribution, else -1: the row plan's targets
-    float *prob, *self;          // self: sum p log p
+    float *prob, *self;          // self: sum p log p, in whose place the base is left for the backward
+    float* base;
     int top;
     float inv_tau;
 };
@@ -617,7 +623,7 @@ struct Entries {
 inline Entries entries_of(void* p, long rows, int top, float inv_tau) {
     int* at = static_cast<int*>(p);
     float* f = reinterpret_cast<float*>(at + rows * (top + 1));
-    return Entries{at, at + rows * top, f, f + rows * top, top, inv_tau};
+    return Entries{at, at + rows * top, f, f + rows * top, f + rows * top, top, inv_tau};
 }
 
 constexpr int kMaxTop = 128;
@@ -740,7 +746,11 @@ __global__ void __launch_bounds__(256) lse_kernel(const float2* __restrict__ par
         if (g > 0 || row >= live) return;
         for (int j = 1; j < 8; ++j) far += sums[j][l], twice = twice || again[j][l];
         const float rest = logf(s), kl = far + rest + e.self[plan.row[row]];
-        lse[row] = fmaf(m, e.inv_tau, rest);
+        // For the gradient: q = exp((z - base) / tau - lse). A logsumexp is rounded at its own size, and q by as much relatively: beyond
+        // 64 (2^-18 of q) the row's maximum stays apart, and what is rounded are differences from it.
+        const float base = fabsf(m * e.inv_tau) > 64.f && fabsf(m) <= FLT_MAX ? m : 0.f;
+        lse[row] = fmaf(m - base, e.inv_tau, rest);
+        e.base[plan.row[row]] = base;
         // Of distinct ids the sum is never negative, its rounding may be. An id that is two entries can have more of the student's
         // probability than either of the teacher's.
         loss[plan.row[row]] = kl < 0.f && !twice ? 0.f : kl;
@@ -1006,7 +1016,7 @@ int operands(const ews_vocab_args* a, const Plan& p, char* w, long v0, long n, O
 // The rows' distributions in a product's arguments; without any, the targets' own.
 void targets(Gemm* g, const Entries* e) {
     g->inv_tau = e ? e->inv_tau : 1.f;
-    if (e) g->ids = e->ids, g->prob = e->prob, g->top = e->top;
+    if (e) g->ids = e->ids, g->prob = e->prob, g->base = e->base, g->top = e->top;
 }
 
 template <typename T>

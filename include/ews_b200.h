@@ -487,7 +487,8 @@ int ews_vocab_bwd(const ews_vocab_args* args, ews_stream_t stream);
  * ids (rows, top) int64 (ids_wide) or int32, logits (rows, top) of logits_dtype, contiguous, top <= 128. An entry of a
  * negative id or of a logit of -inf is absent; a row of which none is left has loss 0 and no gradient, and is not computed. An
  * id that occurs twice is two entries, and can make a loss negative; of distinct ids none is. entries:
- * ews_distill_entries_size(rows, top) bytes, written by the forward for the backward (`v.dloss` in, `v.dhidden` and `v.dweight` out).
+ * ews_distill_entries_size(rows, top) bytes, written by the forward for the backward (`v.dloss` in, `v.dhidden` and `v.dweight` out), as
+ * v.lse is: the logsumexp of a row's scaled logits, or, where that is large, of their differences from the largest.
  * An id beyond the vocabulary is absent and sets *status to EWS_ERR_INDEX. `v.work`: ews_distill_work_size(args, backward)
  * bytes. */
 typedef struct {

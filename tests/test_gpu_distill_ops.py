@@ -303,3 +303,35 @@ def test_logits_at_the_types_ends(ews, dtype, tau):
     assert (got[1][7] == 0).all() and (got[1][[0, 2]] != 0).any(1).all()
     half = torch.where(t == low, torch.finfo(BF16).min, torch.where(t == high, torch.finfo(BF16).max, t)).to(BF16)
     assert torch.equal(ews.distill_loss(h, w, ids, half, temperature=tau), ews.distill_loss(h, w, ids, half.float(), temperature=tau))
+
+
+def exact_products(dtype, N, V, D, seed=0):
+    """hidden and weight rows of small whole numbers: every product and every sum of them is exact."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h, w = (torch.randint(-2, 3, (n, D), device="cuda", generator=g).to(dtype) for n in (N, V))
+    return h, w
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("tau", [0.3, 0.013, 1e-4, 1e-18, 2.0**-90, 1e18])
+def test_gradients_at_any_temperature(ews, dtype, tau):
+    """Logits that are exact: what the probabilities lose is the rounding of (z - max) / temperature alone, 2^-22 of it (the difference is
+    exact), and beyond 20 they are 2^-28 and less. So q is within 2^-17 of itself, G = (q - p) w within that and two roundings to the
+    type, the gradients' sums within S and a rounding more."""
+    h, w = exact_products(dtype, 40, 70, 12)
+    _, _, ids, t, dloss = inputs(dtype, 40, 70, 12, 7, empty=0.1)
+    t = t * tau
+    got = run(ews, h, w, ids, t, tau, dloss)
+    u = torch.finfo(dtype).eps / 2
+    hd, wd, td = h.double(), w.double(), t.double() / tau
+    there = ids >= 0
+    live = there.any(1)
+    p = torch.softmax(td.masked_fill(~there, -float("inf")).masked_fill(~live[:, None], 0.0), 1) * there
+    z = hd @ wd.mT
+    q = torch.softmax((z - z.amax(1, keepdim=True)) / tau, 1)
+    target = torch.zeros_like(q).scatter_add_(1, ids.clamp(min=0), p)
+    weight = (dloss.double() * live / tau)[:, None]
+    g = (q - target) * weight
+    eg = 2.0**-17 * (q + target) * weight + 2 * u * g.abs()
+    for name, a, want, bound in (("dh", got[1], g @ wd, (eg + S * g.abs()) @ wd.abs()), ("dw", got[2], g.mT @ hd, (eg + S * g.abs()).mT @ hd.abs())):
+        check(a, want, bound + u * want.abs(), name)
