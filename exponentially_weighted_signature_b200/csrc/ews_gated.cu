@@ -50,16 +50,39 @@ constexpr long kTwoPlanes = 1l << 30;
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
 
-// act(g) and act'(g). bfloat16 results take the exponent unit's forms (2^-22).
+// act(g) and act'(g). bfloat16 results take the exponent unit's forms: 2^-19 of the result, and 2^-23 of |g| (GELU: g^2 / 2) more where the
+// exponent is large.
 template <bool EXACT>
 __device__ __forceinline__ float logistic(float g) {
     if (EXACT) return 1.f / (1.f + expf(-g));
     return __fdividef(1.f, 1.f + __expf(-g));
 }
+// Phi(g), and exp(-g^2 / 2). From its tail, which is small on the left: 1 + erf cancels there (at g = -5 it was off by a tenth, beyond -5.6
+// nothing was left). bfloat16: the tail over the exponential is smooth, and a polynomial in 1 / (1 + 0.36 |g|), fitted to its relative
+// error (2^-19.7, up to where the exponential is zero), takes half of erfc's instructions (8,192 rows, 1,024 x 4,096: backward 330 us with it,
+// 304 so).
+template <bool EXACT>
+__device__ __forceinline__ float normal(float g, float* e) {
+    if (EXACT) {
+        *e = expf(-0.5f * g * g);
+        return 0.5f * erfcf(-0.70710678118654752f * g);
+    }
+    *e = __expf(-0.5f * g * g);
+    const float t = __fdividef(1.f, fmaf(0.36f, fabsf(g), 1.f));
+    float r = fmaf(t, 0.0470563322f, -0.179764852f);
+    r = fmaf(t, r, 0.180954263f);
+    r = fmaf(t, r, 0.0265491139f);
+    r = fmaf(t, r, 0.139719367f);
+    r = fmaf(t, r, 0.141772434f);
+    r = fmaf(t, r, 0.143713042f);
+    r *= t * *e;
+    return g < 0.f ? r : 1.f - r;
+}
 // -inf: sigmoid and Phi are zero there, and 0 * inf is not the limit, which is zero.
 template <bool EXACT>
 __device__ __forceinline__ float act_of(float g, int kind) {
-    const float c = kind == SILU ? logistic<EXACT>(g) : EXACT ? 0.5f * erfcf(-0.70710678118654752f * g) : 0.5f + 0.5f * erff(0.70710678118654752f * g);
+    float e;
+    const float c = kind == SILU ? logistic<EXACT>(g) : normal<EXACT>(g, &e);
     return c == 0.f ? 0.f : g * c;
 }
 template <bool EXACT>
@@ -69,8 +92,8 @@ __device__ __forceinline__ void act_grad(float g, int kind, float* act, float* s
         *act = c == 0.f ? 0.f : g * c;
         *slope = c == 0.f || c == 1.f ? c : fmaf(*act, 1.f - c, c);
     } else {
-        const float c = EXACT ? 0.5f * erfcf(-0.70710678118654752f * g) : 0.5f + 0.5f * erff(0.70710678118654752f * g);
-        const float phi = 0.39894228040143268f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
+        float e;
+        const float c = normal<EXACT>(g, &e), phi = 0.39894228040143268f * e;
         *act = c == 0.f ? 0.f : g * c;
         *slope = phi == 0.f ? c : fmaf(g, phi, c);
     }

@@ -236,3 +236,37 @@ def test_refusals_on_the_device(ews):
     (g,) = torch.autograd.grad(f(leaf, wg, wu).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("N", [5, 40, 150])
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_activations_to_their_ends(ews, dtype, N, kind):
+    """Projections that are exact (one product each, U = 1), so that the activation shows: within 2^-15 of itself and a rounding
+    (a truncated addition leaves 2^-23 of G, which an exponential of -80, or of -81 / 2, makes 2^-16.6 of the result; its argument's
+    own rounding adds half of that, its last places less), both for H and, through
+    dU = dH act(G) and dG = dH act'(G), for the weights' gradients, which are rounded once as operands and once as results. GELU to
+    -9, where Phi is 1e-19, SiLU to -80."""
+    top = 9.0 if kind == "gelu" else 80.0
+    g = torch.linspace(-top, top, 145, device="cuda", dtype=torch.float64).to(dtype)
+    F = len(g)
+    x = torch.zeros(N, 16, device="cuda", dtype=dtype)
+    x[:, 0], x[:, 1] = 1, 1
+    wg, wu = (torch.zeros(F, 16, device="cuda", dtype=dtype) for _ in range(2))
+    wg[:, 0], wu[:, 1] = g, 1
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    dh = torch.zeros(N, F, device="cuda", dtype=dtype)
+    dh[N - 1] = 1
+    h = ews.gated_linear(*leaves, activation=kind)
+    _, dwg, dwu = torch.autograd.grad(h, leaves, dh)
+    act, slope = act_of(g.double(), kind)
+    u = torch.finfo(dtype).eps / 2
+    # where act' passes zero its two terms, sigmoid and g sigmoid (1 - sigmoid) or Phi and g phi, cancel
+    if kind == "silu":
+        terms = torch.sigmoid(g.double()) * (1 + (g.double() * torch.sigmoid(-g.double())).abs())
+    else:
+        terms = 0.5 * torch.special.erfc(-g.double() / math.sqrt(2)) + g.double().abs() * torch.exp(-(g.double() ** 2) / 2) / math.sqrt(2 * math.pi)
+    check(h.detach(), act.expand(N, F), (2.0**-15 + u) * act.abs().expand(N, F), "h")
+    # (kept in 24 bits, 2^-15 of g: exact for these numbers of bfloat16; float32 keeps all)
+    check(dwu[:, 1], act, (2.0**-15 + 2 * u) * act.abs(), "dwu")
+    check(dwg[:, 0], slope, 2.0**-15 * terms + 2 * u * slope.abs(), "dwg")
