@@ -18,7 +18,9 @@
 // dG and dU are formed by one pass over dH, G and U in between.
 // Operands are bfloat16. float32 inputs are split into three bfloat16 planes (8 bits each) and a product runs over the six pairs
 // of planes that matter (2^-24), smallest first; every 128 of K the sum leaves the tensor core's accumulator, which truncates at
-// every addition, and is added in registers.
+// every addition, and is added in registers. What bfloat16 holds as an infinity has no planes (inf - inf): the forward's results of such
+// values, which the sums leave as NaN, are formed again from the operands themselves (see repair), so that a row does not depend on
+// how many rows come with it. The gradients' are not: an infinity among their operands leaves NaN where the formula may have an infinity.
 //
 // Few rows (a served batch's tokens) are bound by the weights' bytes: served_kernel takes the weights as the wide operand, 64 rows
 // of both a CTA, and keeps as many of their bytes in flight as fit; few_f32_kernel multiplies float32 weights as they are.
@@ -123,6 +125,11 @@ struct Gemm {
     int act;
     void* kept;   // FWD: the projections, or null
     long plane;   // bytes from one plane of it to the next
+    // FWD, float32: the operands as they are, and what the CTAs that split them found (see operand_kernel)
+    const float *x, *wg, *wu;
+    long xs, gs, us;
+    int dim, finds;
+    const int* found;
     int* status;
 };
 
@@ -289,6 +296,42 @@ __device__ __forceinline__ void keep_one(void* kept, long plane, long at, float 
         *reinterpret_cast<uint16_t*>(p + 2 * plane) = (uint16_t)below(g, u);
     }
 }
+
+// The CTA's float32 results that are NaN, from the operands as they are: a warp an element. Only where an operand has an infinity, or a
+// value that bfloat16 rounds to one.
+template <int BN>
+__device__ __noinline__ void repair(const Gemm& a) {
+    constexpr int COLS = BN / 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Job& job = a.job[0];
+    float* out = static_cast<float*>(job.out);
+    Walk<FWD> walk;
+    Unit r;
+    while (walk.next(a, &r)) {
+        for (int e = warp * 32; e < BM * COLS; e += NTH) {
+            const int row = r.tm * BM + e / COLS, col0 = r.tn * COLS + e % COLS, mine = col0 + lane;
+            if (row >= job.m) break;
+            float h = 0.f;
+            if (mine < job.n) h = out[(long)row * job.n + mine];
+            for (unsigned left = __ballot_sync(kFull, h != h); left; left &= left - 1) {
+                const long col = col0 + __ffs(left) - 1;
+                float g = 0.f, u = 0.f;
+                for (int k = lane; k < a.dim; k += 32) {
+                    const float x = a.x[row * a.xs + k];
+                    g = fmaf(x, a.wg[col * a.gs + k], g), u = fmaf(x, a.wu[col * a.us + k], u);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) g += __shfl_xor_sync(kFull, g, o), u += __shfl_xor_sync(kFull, u, o);
+                if (lane == 0) {
+                    const long at = (long)row * job.n + col;
+                    out[at] = u * act_of<true>(g, a.act);
+                    if (a.kept) keep_one<float>(a.kept, a.plane, at, g, u);
+                }
+            }
+        }
+    }
+}
+
 template <typename T, int EPI, int BN>
 __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Gemm a) {
     using TL = Tile<BN>;
@@ -321,6 +364,9 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
     __syncthreads();
     fence_after();
     const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
+    int found = 0;
+    if constexpr (SUM && EPI == FWD)
+        for (int i = threadIdx.x; i < a.finds; i += NTH) found |= a.found[i];
     Walk<EPI> walk;
     Unit r;
 
@@ -469,10 +515,12 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
             }
         }
     }
-    __syncthreads();
+    found = __syncthreads_or(found);
     fence_after();
     if (threadIdx.x == 0 && *fail) report(a.status, EWS_ERR_LOOKBACK_TIMEOUT);
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+    if constexpr (SUM && EPI == FWD)
+        if (found) repair<BN>(a);
 }
 
 // ---- the passes around it ------------------------------------------------------------------------------------
@@ -556,9 +604,12 @@ struct Grad {
     bf16* out;
 };
 
-// The operands of a launch of products: dG and dU, and whatever has to be packed.
+// The operands of a launch of products: dG and dU, and whatever has to be packed. found: whether the CTA packed a value that bfloat16
+// rounds to an infinity.
 template <typename T>
-__global__ void __launch_bounds__(256) operand_kernel(const __grid_constant__ Grad<T> d, const __grid_constant__ Packs<T> a, int dim, int ld, int planes) {
+__global__ void __launch_bounds__(256) operand_kernel(const __grid_constant__ Grad<T> d, const __grid_constant__ Packs<T> a, int dim, int ld, int planes,
+                                                      int* found) {
+    bool huge = false;
     const int per = ld / 8, dper = d.ld / 8;
     const long grads = d.rows * dper, total = grads + (a.p[0].rows + a.p[1].rows + a.p[2].rows) * per;
     const bool vec = d.inner % 8 == 0 && aligned16_dev(d.kept) && aligned16_dev(d.dout) && d.dout_stride % (16 / (int)sizeof(T)) == 0;
@@ -587,8 +638,16 @@ __global__ void __launch_bounds__(256) operand_kernel(const __grid_constant__ Gr
             const Pack<T>& m = a.p[k];
             float v[8];
             load8<T>(m.in + row * m.stride + col, dim - col, m.stride % (16 / (int)sizeof(T)) == 0 && dim % 8 == 0 && aligned16_dev(m.in), v);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) huge = huge || ((__float_as_uint(v[j]) & 0x7FFFFFFFu) - 0x7F7F8000u) <= 0x8000u;
+            }
             split8<T>(v, m.out + row * ld + col, m.plane, planes);
         }
+    }
+    if (sizeof(T) == 4 && found) {
+        const int any = __syncthreads_or(huge);
+        if (threadIdx.x == 0) found[blockIdx.x] = any;
     }
 }
 
@@ -954,7 +1013,7 @@ struct Plan {
     int planes, gplanes;  // of an operand, of dG and dU
     long ldd, ldf;
     Source x, wg, wu;
-    size_t dgu, slots, bytes;
+    size_t found, dgu, slots, bytes;
     int bn;
     Gemm gemm;  // its shares; the backward's tiles
 };
@@ -1032,6 +1091,8 @@ void share_out(Gemm* g) {
     }
 }
 
+constexpr int kMostCtas = SMS * 16;  // of operand_kernel
+
 Plan plan(const ews_gated_args* a, bool bwd) {
     Plan p{};
     p.planes = p.gplanes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
@@ -1054,6 +1115,7 @@ Plan plan(const ews_gated_args* a, bool bwd) {
     p.wu = source(a->w_up, a->up_stride, a->inner);
     if (!bwd) {
         p.bn = forward_bn(a);
+        if (p.planes > 1) p.found = take(sizeof(int) * kMostCtas);
     } else {
         p.bn = p.planes > 1 || a->dim <= 128 ? 128 : 256;
         const int products = p.planes == 1 ? p.gplanes : 6;
@@ -1070,7 +1132,7 @@ Plan plan(const ews_gated_args* a, bool bwd) {
 
 unsigned grid_of(long threads) {
     const long b = (threads + 255) / 256;
-    return (unsigned)(b < 1 ? 1 : b < SMS * 16 ? b : SMS * 16);
+    return (unsigned)(b < 1 ? 1 : b < kMostCtas ? b : kMostCtas);
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH; }
@@ -1087,10 +1149,11 @@ int gemm(const Maps& maps, const Gemm& g, cudaStream_t s) {
 
 const signed char kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
 
-// The three matrices as operands, packed where they have to be, in one launch with the gradients' own.
+// The three matrices as operands, packed where they have to be, in one launch with the gradients' own. finds: the product that wants
+// to know of infinities, or null.
 template <typename T>
 int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Operand* wu, bool need_x, bool need_w, const Grad<T>& grad,
-             cudaStream_t s) {
+             Gemm* finds, cudaStream_t s) {
     char* w = static_cast<char*>(a->work);
     Packs<T> packs{};
     long total = 0;
@@ -1109,7 +1172,10 @@ int operands(const ews_gated_args* a, const Plan& p, Operand* x, Operand* wg, Op
     make(p.wg, a->w_gate, a->gate_stride, a->inner, need_w, wg);
     make(p.wu, a->w_up, a->up_stride, a->inner, need_w, wu);
     if (total + grad.rows == 0) return EWS_OK;
-    operand_kernel<T><<<grid_of(total * (p.ldd / 8) + grad.rows * (p.ldf / 8)), 256, 0, s>>>(grad, packs, (int)a->dim, (int)p.ldd, p.planes);
+    const unsigned grid = grid_of(total * (p.ldd / 8) + grad.rows * (p.ldf / 8));
+    int* found = finds ? reinterpret_cast<int*>(w + p.found) : nullptr;
+    if (finds) finds->found = found, finds->finds = (int)grid;
+    operand_kernel<T><<<grid, 256, 0, s>>>(grad, packs, (int)a->dim, (int)p.ldd, p.planes, found);
     return launched();
 }
 
@@ -1152,7 +1218,8 @@ int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     Operand x{}, wg{}, wu{};
     Grad<T> none{};
     none.ld = 8;
-    int rc = operands<T>(a, p, &x, &wg, &wu, true, true, none, s);
+    Gemm g{};
+    int rc = operands<T>(a, p, &x, &wg, &wu, true, true, none, p.planes > 1 ? &g : nullptr, s);
     if (rc != EWS_OK) return rc;
     if constexpr (sizeof(T) == 2) {
         if (path == SERVED) {
@@ -1166,7 +1233,6 @@ int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     const EncodeFn enc = encoder();
     Maps m{};
     if (!make_map(enc, &m.a[0], x, BM) || !make_map(enc, &m.b[0], wg, p.bn / 2) || !make_map(enc, &m.b[1], wu, p.bn / 2)) return EWS_ERR_LAUNCH;
-    Gemm g{};
     g.job[0] = job_of(a->rows, a->inner, a->dim, p.bn / 2, p.planes == 1 ? 1 : 6);
     Job& j = g.job[0];
     const long tiles = (long)j.tiles_m * j.tiles_n;
@@ -1176,6 +1242,8 @@ int forward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     g.run = p.planes > 1 ? kRun : 1 << 28;
     g.act = a->activation, g.kept = a->kept, g.plane = kept_plane(a), g.status = a->status;
     if constexpr (sizeof(T) == 4) {
+        g.x = static_cast<const T*>(a->x), g.wg = static_cast<const T*>(a->w_gate), g.wu = static_cast<const T*>(a->w_up);
+        g.xs = a->x_stride, g.gs = a->gate_stride, g.us = a->up_stride, g.dim = (int)a->dim;
         return gemm<T, FWD, 128>(m, g, s);
     } else {
         if (p.bn == 256) return gemm<T, FWD, 256>(m, g, s);
@@ -1190,7 +1258,7 @@ int backward(const ews_gated_args* a, const Plan& p, cudaStream_t s) {
     const bool dw = a->dw_gate || a->dw_up;
     bf16* dgu = reinterpret_cast<bf16*>(w + p.dgu);
     const Grad<T> grad{static_cast<const T*>(a->dout), (long)a->dout_stride, a->rows, a->kept, kept_plane(a), (int)a->inner, (int)p.ldf, a->activation, p.gplanes, dgu};
-    int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, grad, s);
+    int rc = operands<T>(a, p, &x, &wg, &wu, dw, a->dx != nullptr, grad, nullptr, s);
     if (rc != EWS_OK) return rc;
     d.p = dgu, d.rows = a->rows, d.cols = d.ld = p.ldf, d.plane = a->rows * p.ldf, d.planes = 2 * p.gplanes;
     const EncodeFn enc = encoder();

@@ -270,3 +270,29 @@ def test_activations_to_their_ends(ews, dtype, N, kind):
     # (kept in 24 bits, 2^-15 of g: exact for these numbers of bfloat16; float32 keeps all)
     check(dwu[:, 1], act, (2.0**-15 + 2 * u) * act.abs(), "dwu")
     check(dwg[:, 0], slope, 2.0**-15 * terms + 2 * u * slope.abs(), "dwg")
+
+
+@pytest.mark.parametrize("N", [3, 33, 64, 200])
+@pytest.mark.parametrize("kept", [False, True])
+def test_float32_values_that_planes_cannot_hold(ews, N, kept):
+    """Infinities and values beyond bfloat16's largest, in X and in either weight: what a row gives does not depend on how many rows
+    come with it, and is the definition's."""
+    x, wg, wu, _ = inputs(FP32, N, 72, 200)
+    x[2, 5], x[0, 7] = float("inf"), 3.4e38
+    x[1, 9] = -3.3999e38
+    wg[7, 5] = 0.0  # 0 x inf: NaN
+    wg[9, 4], wu[11, 6], wg[13, 3] = -float("inf"), float("inf"), float("nan")
+    wg[:, 7], wu[:, 7], wu[:, 9] = wg[:, 7] * 1e-36, wu[:, 7] * 1e-36, wu[:, 9] * 1e-30  # row 0 stays small, row 1's gates are shut or huge
+    g, u = x.double() @ wg.double().mT, x.double() @ wu.double().mT
+    c = torch.sigmoid(g)
+    want = torch.where(c == 0, torch.zeros_like(g), g * c) * u
+    clean = [torch.where(torch.isfinite(t), t, 0.0) for t in (x, wg, wu)]
+    bound = reference(*clean, torch.zeros(N, 200, device="cuda"), "silu")[1][0]
+    weight = wg.clone().requires_grad_(kept)
+    got = ews.gated_linear(x, weight, wu).detach().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    limit = torch.finfo(FP32).max
+    huge = want.abs() > limit * (1 - 2.0**-10)
+    assert torch.equal(got[huge & ~want.isnan()], torch.copysign(torch.full_like(want, float("inf")), want)[huge & ~want.isnan()])
+    rest = ~huge & ~want.isnan()
+    assert ((got - want).abs()[rest] <= bound[rest] * 1.001 + 1e-30).all()
