@@ -248,8 +248,19 @@ __device__ __forceinline__ bool is_near(F<V> rate) {
     for (int j = 0; j < V; ++j) near = near && rate.get(j) <= kNear;
     return __all_sync(kFull, near);
 }
+// v where the clock moves (w = 1 - a^2 in the normal range, or NaN), zero where it does not: such a token takes no input, and may hold
+// anything, which a product with the zero root would let through. (Forwards the choices cost nothing, backwards 134 -> 137 us for
+// 8 x 2,048 tokens of 2,048 channels. Looking for NaN in a warp's sums, and forming them once more where there is one, took registers from
+// both ways: 77 -> 95 us forwards.)
 template <int V>
-__device__ __forceinline__ F<V> root(F<V> w) { return w.each([](float t) { return root(t); }); }
+__device__ __forceinline__ F<V> open(F<V> w, F<V> v) {
+    return F<V>::make([&](int j) { return fabsf(w.get(j)) < FLT_MIN ? 0.f : v.get(j); });
+}
+// What a token brings into the state.
+template <int V>
+__device__ __forceinline__ F<V> input(F<V> w, F<V> i, F<V> x) {
+    return open(w, w.each([](float t) { return root(t); }) * i * x);
+}
 
 // A channel's rate; an infinite one as float32's largest, so that a shut gate's product with it is zero.
 __device__ __forceinline__ float rate_at(const float* p) {
@@ -468,7 +479,7 @@ __global__ void __launch_bounds__(Shape<V>::FW * 32, Shape<V>::FCTAS) forward_ke
             const F<V> p = rate * sigmoid(wr[l].get());
             const Decay<decltype(near)::value, V> d(p);
             av[l] = d.a();
-            bv[l] = root(d.w(p)) * sigmoid(wi[l].get()) * wx[l].get();
+            bv[l] = input(d.w(p), sigmoid(wi[l].get()), wx[l].get());
             A = A * av[l];
             H = fma(av[l], H, bv[l]);
         }
@@ -515,13 +526,14 @@ struct Slopes {
     F<V> x, decay, gate;
 };
 template <bool NEAR, int V>
-__device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, Decay<NEAR, V> d, F<V> r, F<V> i, F<V> before, F<V> x, F<V> dout, F<V>* g, F<V>* sum) {
+__device__ __forceinline__ Slopes<V> slopes_of(F<V> rate, Decay<NEAR, V> d, F<V> r, F<V> gate, F<V> before, F<V> x, F<V> dout, F<V>* g, F<V>* sum) {
     const F<V> minus(-1.f), one(1.f);
     const F<V> a = d.a(), w = d.w(rate * r);  // formed again: kept, they would take too many registers
+    const F<V> i = open(w, gate);
     // no step of the clock: the state passes, whatever the input
     const F<V> inv = w.each([](float t) { return fabsf(t) < FLT_MIN ? 0.f : inverse_root(t); });
     *g = *g + dout;
-    const F<V> ix = i * x, gm = *g * (w * inv);
+    const F<V> ix = open(w, gate * x), gm = *g * (w * inv);
     const F<V> rd = r * *g * fma(a * a * inv * ix, minus, a * before);
     *sum = fma(rd, minus, *sum);
     *g = a * *g;
@@ -568,7 +580,7 @@ __global__ void __launch_bounds__(Shape<V>::BW * 32, Shape<V>::BCTAS) backward_k
                 const K d(rate * rv[l]);
                 kv[l] = d.k;
                 hb[l] = H;
-                H = fma(d.a(), H, root(d.w(rate * rv[l])) * iv[l] * wx[l].get());
+                H = fma(d.a(), H, input(d.w(rate * rv[l]), iv[l], wx[l].get()));
                 A = A * d.a();
             }
 #pragma unroll
@@ -747,7 +759,7 @@ __global__ void __launch_bounds__(PW * 32, PCTAS) forward_tma_kernel(const __gri
                 const F<V> p = rate * sigmoid(row[STREAM + l * 32].get());
                 const Decay<decltype(near)::value, V> d(p);
                 av[l] = d.a();
-                bv[l] = root(d.w(p)) * sigmoid(row[2 * STREAM + l * 32].get()) * row[l * 32].get();
+                bv[l] = input(d.w(p), sigmoid(row[2 * STREAM + l * 32].get()), row[l * 32].get());
                 A = A * av[l];
                 H = fma(av[l], H, bv[l]);
             }
@@ -846,7 +858,7 @@ __global__ void __launch_bounds__(Back<4 / sizeof(T), ROWS>::QW * 32, Back<4 / s
                 const K d(rate * rv[l]);
                 kv[l] = d.k;
                 hb[l] = H;
-                H = fma(d.a(), H, root(d.w(rate * rv[l])) * iv[l] * row[l * 32].get());
+                H = fma(d.a(), H, input(d.w(rate * rv[l]), iv[l], row[l * 32].get()));
                 A = A * d.a();
             }
 #pragma unroll
@@ -974,7 +986,7 @@ __global__ void __launch_bounds__(128) step_kernel(const __grid_constant__ Step<
         for (int j = 0; j < V; ++j) {
             const F<1> p = F<1>(k[j]) * sigmoid(F<1>(r[j]));
             const Decay<false, 1> d(p);
-            o[j] = fma(d.a(), F<1>(h[j]), root(d.w(p)) * sigmoid(F<1>(i[j])) * F<1>(x[j])).r;
+            o[j] = fma(d.a(), F<1>(h[j]), input(d.w(p), sigmoid(F<1>(i[j])), F<1>(x[j]))).r;
         }
         if constexpr (V == 4) Vec<float, true>::store(state, o);
         else *state = o[0];

@@ -93,7 +93,8 @@ def gated_recurrence(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor, r
 
     x, decay, gate (B, T, C), float32 or bfloat16, any strides (views of one projection, for instance); rate (C,) float32,
     zero or larger (a negative one gives NaN): a diagonal generator's rates, with ``sigmoid(decay)`` as the clock's step.
-    A decay of -inf, or of its type's lowest value, passes the state on unchanged and takes no input. initial_state (B, C)
+    A decay of -inf, or of its type's lowest value, passes the state on unchanged and takes no input, whatever the token
+    holds (NaN and infinities too). initial_state (B, C)
     float32 or None (zero). lengths (B,) int32: positions at or beyond a sample's length are not read, give zeros and
     leave the state.
 

@@ -389,7 +389,8 @@ int ews_decay_bwd(const ews_decay_args* args, ews_stream_t stream);
 int ews_decay_step(const ews_decay_args* args, const int* slots, int pool, float* state, ews_stream_t stream);
 
 /* ---- gated linear recurrence ----------------------------------------------------------------------
- * For every sample and channel: a = exp(-rate sigmoid(decay_t)), h_t = a h_{t-1} + sqrt(1 - a^2) sigmoid(gate_t) x_t.
+ * For every sample and channel: a = exp(-rate sigmoid(decay_t)), h_t = a h_{t-1} + sqrt(1 - a^2) sigmoid(gate_t) x_t. Where a is one
+ * (a decay of -inf or of its type's lowest value, a rate of zero) the token brings nothing in, whatever it holds.
  * x, decay, gate (batch, steps, channels) of `dtype` with contiguous last axes and element strides {batch, step}; rate
  * (channels) float32, not negative (a negative one gives NaN); lengths (batch) int32 or NULL: positions at or beyond a
  * sample's length are not read, give zeros and leave the state; initial (batch, channels) float32 or NULL (zero). out (batch,

@@ -412,3 +412,30 @@ def test_broadcast_inputs(ews, dtype):
         n = B * T
         bound = ((2 * T * 2.0**-23 + 2.0**-19) * a).sum(axes, keepdim=True) + n * torch.finfo(dtype).eps * a.sum(axes, keepdim=True)
         assert ((g.double() - v.sum(axes, keepdim=True)).abs() <= bound + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("B,T,C", [(2, 30, 33), (3, 150, 64), (75, 140, 64), (2, 150, 34)])
+@pytest.mark.parametrize("top", [1.39, None])
+def test_what_a_shut_decay_gate_hides(ews, dtype, B, T, C, top):
+    """A token whose decay gate is shut may hold anything: nothing of it reaches the state or a gradient, and its own gradients are
+    zero. With a finite token in its place, the same numbers."""
+    x, decay, gate, rate, s0, do, ds = inputs(dtype, B, T, C)
+    rate = rate.clamp(max=1.39) if top else rate
+    shut = torch.rand(B, T, C, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) < 0.2
+    shut[:, 3] = True
+    kind = torch.randint(0, 4, (B, T, C), device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))
+    junk = torch.tensor([float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).max], device="cuda").to(dtype)[kind]
+    decay = torch.where(shut, torch.where(kind % 2 == 0, -float("inf"), torch.finfo(dtype).min).to(dtype), decay)
+    results = []
+    for a, b in ((x, gate), (torch.where(shut, junk, x), torch.where(shut, junk.flip(0), gate))):
+        leaves = [t.clone().requires_grad_() for t in (a, decay, b, rate, s0)]
+        out = ews.gated_recurrence(*leaves[:4], initial_state=leaves[4], return_state=True)
+        results.append([t.detach() for t in out] + list(torch.autograd.grad(out, leaves, (do, ds))))
+        pool = s0.clone()
+        with torch.no_grad():
+            results[-1] += [ews.gated_recurrence_step(a[:, 3], decay[:, 3], b[:, 3], rate, pool), pool]
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert all((g[shut] == 0).all() for g in results[1][2:5])
+    assert torch.equal(results[1][8], s0)
