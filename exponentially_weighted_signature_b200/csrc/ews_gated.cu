@@ -46,8 +46,10 @@ constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulato
 // Rows up to which served_kernel runs (bfloat16; 100 rows, 5,632 x 2,048: 20 us there, 26 as tiles; 4,096 x 1,024: 14, 13), and up
 // to which few_f32_kernel does (32 rows, 5,632 x 2,048: 88 us there, 109 as tiles of three planes; 64 rows: 139, 111).
 constexpr int kServed = 128, kFewF32 = 32;
-// Where dG and dU are small or few, their rounding to bfloat16 does not average out of the gradients (five rows of 472: 2.5e-3 of the
-// exact ones where one rounding leaves 1.7e-3): up to this many multiplications a product they are kept in two planes, 16 bits.
+// Rounded to bfloat16 once, dG and dU take the gradients from 1.7e-3 of the exact ones, which is their own rounding, to 2.3e-3. Up to this many
+// multiplications a product (of tiles, which are BM wide or more) they are kept in two planes, 16 bits: 6 us more at a width of 1,024
+// (512 rows of 2,048: 43 -> 49), 26 at 130 (8,192 rows of 1,000: 76 -> 102). Beyond, a second plane would cost a second product. (Counted
+// by the width itself, narrow rows had two planes of any length: 4,096 rows of 4,096, width 64, 111 us, so 82.)
 constexpr long kTwoPlanes = 1l << 30;
 enum Activation { SILU = 0, GELU = 1 };
 enum Epilogue { FWD, OUT };
@@ -1096,7 +1098,7 @@ constexpr int kMostCtas = SMS * 16;  // of operand_kernel
 Plan plan(const ews_gated_args* a, bool bwd) {
     Plan p{};
     p.planes = p.gplanes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
-    if (p.planes == 1 && a->rows * a->inner <= kTwoPlanes / a->dim) p.gplanes = 2;
+    if (p.planes == 1 && a->rows * a->inner <= kTwoPlanes / (a->dim < BM ? BM : a->dim)) p.gplanes = 2;
     p.ldd = up(a->dim, 8), p.ldf = up(a->inner, 8);
     if (!bwd && path_of(a) == FEW) return p;
     size_t at = 0;

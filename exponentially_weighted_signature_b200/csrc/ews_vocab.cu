@@ -47,9 +47,10 @@ constexpr long kPieceElems = 1l << 27; // entries of G (times planes) at a time:
 // is long: for float32 a tile's sum leaves the accumulator every 256 of K and is added, rounded, to the float32 partial.
 constexpr int kRun = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-// A teacher's few entries dominate G, and with few rows their rounding to bfloat16 does not average out of the gradients (ten rows:
-// 2.6e-3 of the exact ones where one rounding leaves 1.7e-3). Up to this many multiplications a product G is kept in two planes,
-// 16 bits, which takes some 10 us more at most.
+// Rounded to bfloat16 once, a teacher's G takes the gradients from 1.7e-3 of the exact ones, which is their own rounding, to 2.3e-3.
+// Up to this many multiplications a product (of tiles, which are BM wide or more) G is kept in two planes, 16 bits: 2 us more for ten rows, 10 to 13 at a width of 1,024 (2,048 rows of
+// 1,024: 57 -> 68 us), 34 at 127 (4,096 rows of 4,096: 82 -> 116). Beyond, a second plane would cost a second product. (Counted by the width
+// itself, narrow rows had two planes of any length: 8,192 rows of 12,000, width 16, 421 us, so 248.)
 constexpr long kTwoPlanes = 1l << 31;
 
 // 2^x: the exponent unit's own instruction, results below the normal range to zero.
@@ -941,7 +942,7 @@ void even_splits(Plan* p, long n, long d) {
 Plan plan(const ews_vocab_args* a, bool bwd, int top = 0) {
     Plan p{};
     p.planes = p.gplanes = a->dtype == EWS_DTYPE_F32 ? 3 : 1;
-    if (top && p.planes == 1 && a->rows * a->vocab <= kTwoPlanes / a->dim) p.gplanes = 2;
+    if (top && p.planes == 1 && a->rows * a->vocab <= kTwoPlanes / (a->dim < BM ? BM : a->dim)) p.gplanes = 2;
     p.ldd = (int)up(a->dim, 8);
     p.pack_w = p.planes > 1 || a->weight_stride % 8 || a->dim % 8 || !aligned16(a->weight);
     const long n = a->rows, v = a->vocab;

@@ -126,3 +126,18 @@ def test_a_gated_block_is_built_as_it_says():
     assert [s.shape for s in TokenModel(20, 32, 2, ("gated", "decay"), gated_kwargs=dict(width=24)).states(3)] == [(3, 24), (3, 2, 16, 16)]
     with pytest.raises(ValueError):
         TokenModel(20, mixers=("gate",))
+
+
+def test_narrow_rows_keep_one_plane():
+    """A second plane of what the gradients' products read costs as much as its elements and its tiles do, however narrow the rows are."""
+    from exponentially_weighted_signature_b200 import gated_ops, token_ops
+
+    rows, many = 8192, 16384
+    for dim in (1, 8, 16):
+        stride = -(-dim // 8) * 8
+        one = 2 * rows * many  # bytes of one plane of G, all of it in one piece
+        size = token_ops._distill_size(rows, many, dim, 1, stride, stride, 0, 16, 1)
+        assert one < size < 1.5 * one, dim
+        for rows_, inner in ((rows, many), (many, rows)):
+            size = gated_ops._size(rows_, dim, inner, 1, (stride, stride, stride), (0, 0, 0), (1, 1, 1), 1)
+            assert 2 * one < size < 3 * one, dim
