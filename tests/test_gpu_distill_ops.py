@@ -335,3 +335,36 @@ def test_gradients_at_any_temperature(ews, dtype, tau):
     eg = 2.0**-17 * (q + target) * weight + 2 * u * g.abs()
     for name, a, want, bound in (("dh", got[1], g @ wd, (eg + S * g.abs()) @ wd.abs()), ("dw", got[2], g.mT @ hd, (eg + S * g.abs()).mT @ hd.abs())):
         check(a, want, bound + u * want.abs(), name)
+
+
+@pytest.mark.parametrize("N,V,D,dtype", [(2048, 30011, 24, FP32), (4096, 40011, 8, BF16)])
+def test_several_pieces_in_planes_and_of_narrow_rows(ews, N, V, D, dtype):
+    """Three planes of G in pieces, and rows narrower than a tile."""
+    h, w, ids, t, dloss = inputs(dtype, N, V, D, 16)
+    ids[:, 0] = torch.randint(V - 300, V, (N,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(9))
+    got = run(ews, h, w, ids, t, 0.7, dloss)
+    total = None
+    for a in range(0, N, 1024):
+        want, bound = reference(h[a : a + 1024], w, ids[a : a + 1024], t[a : a + 1024], 0.7, dloss[a : a + 1024])
+        check(got[0][a : a + 1024], want[0], bound[0], "loss")
+        check(got[1][a : a + 1024], want[1], bound[1], "dh")
+        total = (want[2], bound[2]) if total is None else (total[0] + want[2], total[1] + bound[2])
+    check(got[2], *total, "dw")
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_rows_of_wider_matrices(ews, dtype):
+    """Strided rows, at offsets that TMA can and cannot start at, with their gradients."""
+    h, w, ids, t, dloss = inputs(dtype, 150, 300, 40, 9)
+    want, bound = reference(h, w, ids, t, 2.0, dloss)
+    for at in (0, 3, 8):
+        wide = [torch.full((x.shape[0], 40 + 16), float("nan"), dtype=dtype, device="cuda") for x in (h, w)]
+        for big, x in zip(wide, (h, w)):
+            big[:, at : at + 40] = x
+        leaves = [big.requires_grad_() for big in wide]
+        loss = ews.distill_loss(*(big[:, at : at + 40] for big in leaves), ids, t, temperature=2.0)
+        grads = torch.autograd.grad(loss, leaves, dloss)
+        check(loss.detach(), want[0], bound[0], ("loss", at))
+        for k in range(2):
+            check(grads[k][:, at : at + 40], want[1 + k], bound[1 + k], ("grad", k, at))
+            assert (grads[k][:, :at] == 0).all() and (grads[k][:, at + 40 :] == 0).all()

@@ -296,3 +296,18 @@ def test_float32_values_that_planes_cannot_hold(ews, N, kept):
     assert torch.equal(got[huge & ~want.isnan()], torch.copysign(torch.full_like(want, float("inf")), want)[huge & ~want.isnan()])
     rest = ~huge & ~want.isnan()
     assert ((got - want).abs()[rest] <= bound[rest] * 1.001 + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype,N,D,F", [(BF16, 48, 2048, 5632), (BF16, 1000, 512, 1032), (BF16, 700, 64, 40000), (FP32, 500, 128, 341)])
+def test_runs_repeat_bit_for_bit(ews, dtype, N, D, F):
+    """Whatever the workspaces and outputs held before."""
+    x, wg, wu, dh = inputs(dtype, N, D, F)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    first = None
+    for fill in (0.0, float("nan"), 1e30, float("inf")):
+        junk = [torch.full((16 << 20,), fill, device="cuda") for _ in range(4)]
+        del junk
+        h = ews.gated_linear(*leaves)
+        got = [h.detach(), *torch.autograd.grad(h, leaves, dh)]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))

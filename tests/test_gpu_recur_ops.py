@@ -439,3 +439,37 @@ def test_what_a_shut_decay_gate_hides(ews, dtype, B, T, C, top):
         assert torch.equal(a, b)
     assert all((g[shut] == 0).all() for g in results[1][2:5])
     assert torch.equal(results[1][8], s0)
+
+
+MANY = [(FP32, 4, 300, 96), (BF16, 4, 300, 192), (BF16, 75, 140, 192), (BF16, 3, 70, 130), (FP32, 2, 200, 33), (FP32, 40, 300, 256), (BF16, 6, 3000, 192)]
+
+
+@pytest.mark.parametrize("top", [1.39, None])
+@pytest.mark.parametrize("dtype,B,T,C", MANY)
+def test_rates_on_either_side(ews, dtype, B, T, C, top):
+    """Rates of up to 1.39, all of them where decays are formed without the exponent unit, and a few beyond, where a warp forms them with
+    it. In float32 more tiles than the GPU holds CTAs, so that their stages go round; in bfloat16 the same with fewer chains than
+    multiprocessors (backward in tiles of 64 tokens) and with more (32)."""
+    x, decay, gate, rate, s0, do, ds = inputs(dtype, B, T, C, seed=T + B)
+    rate = rate.clamp(max=1.39) if top else rate
+    ln = (T - (torch.arange(B, device="cuda", dtype=torch.int32) * 61) % (T // 2)).int()
+    leaves = [t.clone().requires_grad_() for t in (x, decay, gate, rate, s0)]
+    out = ews.gated_recurrence(*leaves[:4], initial_state=leaves[4], lengths=ln, return_state=True)
+    grads = torch.autograd.grad(out, leaves, (do, ds))
+    args = (x, decay, gate, rate, s0, ln, do, ds)
+    want, ab = reference(*args), reference(*args, absolute=True)
+    for k, (name, got) in enumerate(zip(("h", "state", "dx", "ddecay", "dgate", "drate", "dstate"), (out[0].detach(), out[1].detach(), *grads))):
+        check(got, want[k], ab[k], T if k < 2 else 2 * T, name)
+
+
+@pytest.mark.parametrize("dtype,B,C", [(BF16, 2, 64), (BF16, 75, 192), (BF16, 2, 65), (FP32, 2, 64), (FP32, 3, 33)])
+def test_gradients_of_the_end_state_alone(ews, dtype, B, C):
+    """No cotangent for the outputs, on states kept every 64 and every 32 tokens."""
+    x, decay, gate, rate, s0, do, ds = inputs(dtype, B, 140, C)
+    leaves = [t.clone().requires_grad_() for t in (x, decay, gate, rate, s0)]
+    _, end = ews.gated_recurrence(*leaves[:4], initial_state=leaves[4], return_state=True)
+    grads = torch.autograd.grad(end, leaves, ds)
+    args = (x, decay, gate, rate, s0, None, torch.zeros_like(do), ds)
+    want, ab = reference(*args), reference(*args, absolute=True)
+    for name, a, b, c in zip(("dx", "ddecay", "dgate", "drate", "dstate"), grads, want[2:], ab[2:]):
+        check(a, b, c, 280, name)
