@@ -29,7 +29,8 @@
 // operands without activation and product; 8,192 rows, 1,024 x 4,096: 102 us (97), 124 us where G and U are kept, the backward 298
 // us: 63 to 79 for its operands, 208 for 8 N D F at 1.32 PFLOP/s, 11 to join pieces. What bounds them is the tensor pipe, under the
 // power cap in a long run. Up to 64 rows, 5,632 x 2,048: 15 us (3.2 TB/s; 46 MB take 7), 11,008 x 4,096: 38 us (4.8 TB/s; 28): a CTA's
-// start, first bytes and epilogue beside its share of the weights; 4,096 x 1,024: 9 us, the same. float32, 16 rows, 1,024 x 4,096: 20.
+// start, first bytes and epilogue beside its share of the weights, and with 5,632 and 4,096 of them 88 and 64 CTAs for 148 SMs;
+// 4,096 x 1,024: 9 us. float32, 16 rows, 1,024 x 4,096: 20.
 #include "ews_tc.cuh"
 
 namespace ews {
@@ -43,7 +44,7 @@ constexpr int EPW = 8;              // epilogue warps
 constexpr int NTH = 64 + EPW * 32;  // and one each for TMA and MMA
 constexpr int SMS = 148;
 constexpr int kRun = 2;             // float32: k blocks of 64 in one accumulator
-// Rows up to which served_kernel runs (bfloat16; 100 rows, 5,632 x 2,048: 20 us there, 26 as tiles; 4,096 x 1,024: 14, 13), and up
+// Rows up to which served_kernel runs (bfloat16; 100 rows, 5,632 x 2,048: 20 us there, 26 as tiles; 4,096 x 1,024: 14, 13: the weights cold), and up
 // to which few_f32_kernel does (32 rows, 5,632 x 2,048: 88 us there, 109 as tiles of three planes; 64 rows: 139, 111).
 constexpr int kServed = 128, kFewF32 = 32;
 // Rounded to bfloat16 once, dG and dU take the gradients from 1.7e-3 of the exact ones, which is their own rounding, to 2.3e-3. Up to this many
@@ -825,7 +826,9 @@ __global__ void __launch_bounds__(128) few_f32_kernel(const __grid_constant__ Fe
 
 // Up to 128 rows: the weights as the wide operand, 64 rows of Wg above the same of Wu a CTA (their partners in lanes 64
 // apart), the rows of X as the narrow one (BN of them). One tile a CTA, whatever K; what counts is how many bytes of the
-// weights are in flight: eight stages of 16 KB and X's rows where one CTA an SM is enough, four where there are more tiles.
+// weights are in flight: eight stages of 16 KB and X's rows where one CTA an SM is enough, four where there are more tiles. BN is the rows
+// rounded up to 16, above 64 to 32: a row that is not there costs its share of the products and the epilogue (5,632 x 2,048, back to back:
+// 48 rows 12.1 us, 12.6 at BN = 64; 65 rows 13.6 at 96, 14.8 at 128; 80 and 112 would take another 0.4 and 0.6 off, and two more kernels).
 struct Served {
     int rows, inner, act, blocks, stages;  // k blocks of 64
     bf16* out;

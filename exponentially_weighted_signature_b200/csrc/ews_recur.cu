@@ -17,12 +17,14 @@
 // leaves one for each of its tiles (float32), from which the tile runs the recurrence again. So the gradient of the rates, a
 // float32 sum over all tokens, does not see the rounding of the stored states, and a stream less is read.
 //
-// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 76 us forwards (four streams, 3.5 TB/s) and 131 back (seven, 3.6),
-// float32 107 and 173 us (5.0 and 5.4 TB/s). bfloat16 is bound by the gates, of which the SM issues at half its rate at best:
-// with the exponent unit for every decay 81 and 153 us (backward tiles of 64 tokens), without the gates' arithmetic 60 and 134,
-// without the look-back too 56 and 116. One sample of 17,984 tokens: 111 and 181 us, 79 and 146 without the look-back: 32
-// chains of tiles, 18 of each in work at a time, wait for one another's maps and states (folding 12 or 16 tiles at once instead
-// of 4 changed nothing).
+// Measured, 8 x 2,048 tokens of 2,048 channels: bfloat16 77 us forwards (four streams, 3.5 TB/s) and 137 back (seven, 3.4),
+// float32 108 and 175 us (5.0 and 5.4 TB/s); with rates up to 4, so that decays take the exponent unit, 83 and 147 us, and 106 and 177.
+// bfloat16 is bound by latency, no unit is saturated: four warps a scheduler (128 registers)
+// issue in 46 % of the cycles forwards and 54 % back, the exponent unit works in 49 and 32 %, DRAM at a third of its rate, and a warp waits
+// for the tile's barriers, for what it loads and for its own arithmetic about as long each. (Of an earlier build: without the gates'
+// arithmetic 60 and 134 us, without the look-back too 56 and 116.) One sample of 17,984 tokens: 112 and 187 us; an earlier build's 111
+// and 181 were 79 and 146 without the look-back: 32 chains of tiles, 18 of each in work at a time, wait for one another's maps
+// and states (folding 12 or 16 tiles at once instead of 4 changed nothing).
 #include <float.h>
 
 #include <type_traits>
@@ -53,7 +55,8 @@ constexpr int PL = 16, PW = TILE / PL, PCTAS = 4;  // the same where TMA brings 
 // more tiles are in work and fewer threads wait at a barrier; a chain of few passes through twice as many states. Tiles of 64
 // tokens and of 32, 2,048 channels, us: 256 chains x 2,048 tokens 140 and 132, 160 x 2,048 99 and 93, 128 x 4,096 144 and 147,
 // 64 x 8,192 151 and 163, 32 x 16,384 167 and 192. One tile is better than two: 8,192 chains x 40 tokens 121 and 126.
-// (float32 has a token's 32 channels a tile, and enough tiles: 8 x 2,048 x 1,024 95 and 105.)
+// (float32 has a token's 32 channels a tile, and enough tiles: 8 x 2,048 x 1,024 95 and 105. All before the choices of `open`, which added
+// two or three to either.)
 template <int V, int ROWS>
 struct Back {
     static constexpr int QL = V == 1 ? 16 : 8, QW = ROWS / QL, QCTAS = V == 1 ? 3 : ROWS == TILE ? 2 : 4;
@@ -171,7 +174,8 @@ struct Word<bf16, 2> {
 };
 
 // The exponent unit's own instructions; what lies below the normal range counts as zero (a sigmoid of less than -87, say),
-// which spares their corrections, a third of the kernels' instructions.
+// which spares their corrections, a third of the kernels' instructions. A sigmoid's exponent is rounded before it: 2^-24 of |x| log2(e) comes
+// to 1e-6 of a sigmoid at x = -20 and 5e-6 at -87, in float32 too, where the states' own roundings are of that size over some ten tokens.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

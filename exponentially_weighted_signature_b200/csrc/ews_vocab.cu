@@ -925,7 +925,8 @@ void pick_pieces(Plan* p, long n, long v, long d, bool bwd) {
 }
 
 // K splits of the gradients where one has few tiles and long sums: as many as bring a unit down to an SM's share of both products
-// (96 rows, V = 8,548, D = 800, float32: 524 -> 78 us for both gradients), at least eight k blocks and at most 48 to a sum.
+// (96 rows, V = 8,548, D = 800, float32: 524 -> 78 us for both gradients), at least eight k blocks and at most 48 to a sum. For a teacher's
+// loss alone: the loss against single targets keeps its splits, and with them the order of its sums and its results to the last bit.
 void even_splits(Plan* p, long n, long d) {
     const long td = (d + tile_n(d) - 1) / tile_n(d), th = (n + BM - 1) / BM * td, tw = (p->piece + BM - 1) / BM * td;
     const long kh = (p->piece + BK - 1) / BK, kw = (n + BK - 1) / BK, all = th * kh + tw * kw;

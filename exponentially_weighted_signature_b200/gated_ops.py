@@ -87,7 +87,8 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
 
     x (..., D); gate_weight and up_weight (F, D), all float32 or all bfloat16 (rows of any stride). activation: "silu",
     ``g sigmoid(g)``, or "gelu", ``g Phi(g)``. Returns (..., F). Sums are float32; the product is formed from them and rounded
-    once. Differentiable in x and both weights (the two projections are kept for it, 6 bytes a pair for bfloat16, 8 for float32)."""
+    once. Differentiable in x and both weights (the two projections are kept for it, 6 bytes a pair for bfloat16, 8 for float32); in
+    float32, gradients are NaN where an infinity, or a value that bfloat16 rounds to one, enters them."""
     inner = gate_weight.shape
     if len(inner) != 2 or up_weight.shape != inner or 0 in inner:
         raise ValueError(f"gate_weight and up_weight must be (F, D) with F, D > 0, got {tuple(inner)} and {tuple(up_weight.shape)}")

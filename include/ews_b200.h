@@ -432,7 +432,8 @@ int ews_recur_step(const ews_recur_args* args, const int* slots, int pool, float
  * `up_stride` elements apart), out (rows, inner) contiguous; activation EWS_ACT_SILU, g sigmoid(g), or EWS_ACT_GELU, g Phi(g).
  * kept: ews_gated_kept_size(args) bytes, the two projections for the backward, or NULL.
  *   ews_gated_bwd: from dout (rows, inner; rows `dout_stride` apart) and kept the gradients dx (rows, dim), dw_gate and dw_up
- *   (inner, dim), contiguous; any may be NULL.
+ *   (inner, dim), contiguous; any may be NULL. In float32 they are NaN where an infinity, or a value that bfloat16 rounds to one,
+ *   enters them.
  * status as above. `work`: ews_gated_work_size(args, backward) bytes; the size also depends on which of dx, dw_gate and dw_up
  * are asked for, and on the matrices' strides and on their addresses modulo 16. */
 #define EWS_ACT_SILU 0
