@@ -116,12 +116,21 @@ struct Maps {
     CUtensorMap a[2], b[2], g;
 };
 
-// GRAD's epilogue stages its output, a box of 64 columns a warp at a time; OUT's passes rows that start on no vector through 16
-// columns at a time, so that a store has neighbours of a row instead of 32 rows' single elements (dW of 123,911 x 158: 205 -> 90 us).
+// OUT: whether what a warp has goes to memory by way of shared memory: rows that start on no vector.
+__host__ __device__ inline bool exchanged(const Job& j) {
+    return j.n % (j.acc ? 4 : 8) || (!j.acc && ((uintptr_t)j.out & 15u));
+}
+
+// GRAD's epilogue stages its output, a box of 64 columns a warp at a time; OUT's passes what is exchanged through 16
+// columns at a time, so that a store has neighbours of a row instead of 32 rows' single elements (dW of 123,911 x 158: 205 -> 90 us), with
+// eight rows' partial sums in flight (both gradients of 3,000 rows, V = 5,001, D = 333, float32: 1,131 us one after the other, 503 so).
+// A launch that exchanges nothing leaves that memory to the first-level cache, through which the partial sums are added to: taken from it,
+// both gradients of 96 rows, V = 8,548, D = 800, float32, went from 613 to 685 us.
 template <int EPI, int BN>
 struct Tile {
     static constexpr int A = BM * BK * 2, B = BN * BK * 2, STAGE = A + B;
-    static constexpr int OUTW = EPI == GRAD ? 4096 : EPI == OUT ? 32 * 17 * 4 : 0;  // bytes a warp: 32 rows of 64 columns; of 16 and a pad
+    static constexpr int OUTW = EPI == GRAD ? 4096 : 0;  // bytes a warp: 32 rows of 64 columns
+    static constexpr int SHARE = 32 * 17 * 4;            // and behind all else where a launch needs it: of 16 columns and a pad
     static constexpr int STAGES = BN == 256 ? 4 : EPI == GRAD ? 5 : 6;
     static constexpr size_t bytes = (size_t)STAGES * STAGE + EPW * OUTW + 1024 + 256;
 };
@@ -460,8 +469,8 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] *= factor;
                         }
-                        if (w < 32 || (job.n & (job.acc ? 3 : 7)) || (!job.acc && !aligned16_dev(job.out))) {
-                            float* share = reinterpret_cast<float*>(tiles + S * TL::STAGE + (warp - 2) * TL::OUTW);
+                        if (exchanged(job)) {
+                            float* share = reinterpret_cast<float*>(tiles + S * TL::STAGE + 256 + (warp - 2) * TL::SHARE);
                             const int first = r.tm * BM + quarter * 32, there = min((r.job ? job.m : m0) - first, 32);
 #pragma unroll
                             for (int h = 0; h < 32; h += 16) {
@@ -470,33 +479,43 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
 #pragma unroll
                                 for (int j = 0; j < 16; ++j) share[lane * 17 + j] = v[h + j];
                                 __syncwarp();
-                                const int k = h + (lane & 15);
-                                for (int q = lane >> 4; q < there && k < w; q += 2) {
-                                    const float x = share[q * 17 + (lane & 15)];
-                                    if (job.acc) {
-                                        float* p = job.acc + ((long)r.sp * job.m + first + q) * job.n + col + k;
-                                        *p = add ? *p + x : x;
-                                    } else {
-                                        job.out[(long)(first + q) * job.n + col + k] = from_f<bf16>(x);
+                                const int k = h + (lane & 15), rows = k < w ? there : 0;
+                                if (job.acc) {  // eight rows' sums in flight
+                                    for (int q0 = lane >> 4; q0 < rows; q0 += 16) {
+                                        float* p = job.acc + ((long)r.sp * job.m + first + q0) * job.n + col + k;
+                                        float o[8];
+#pragma unroll
+                                        for (int i = 0; i < 8; ++i) o[i] = add && q0 + 2 * i < rows ? p[(long)(2 * i) * job.n] : 0.f;
+#pragma unroll
+                                        for (int i = 0; i < 8; ++i) {
+                                            const float x = share[(q0 + 2 * i) * 17 + (lane & 15)];
+                                            if (q0 + 2 * i < rows) p[(long)(2 * i) * job.n] = add ? o[i] + x : x;
+                                        }
                                     }
+                                } else {
+                                    for (int q = lane >> 4; q < rows; q += 2)
+                                        job.out[(long)(first + q) * job.n + col + k] = from_f<bf16>(share[q * 17 + (lane & 15)]);
                                 }
                             }
                         } else if (!in) {
                         } else if (job.acc) {
                             float* p = job.acc + ((long)r.sp * job.m + row) * job.n + col;
+                            if (add) {
+                                float4 o[8];
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                float4 q = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                                if (add) {
-                                    const float4 o = *reinterpret_cast<const float4*>(p + j);
-                                    q.x += o.x, q.y += o.y, q.z += o.z, q.w += o.w;
-                                }
-                                *reinterpret_cast<float4*>(p + j) = q;
+                                for (int j = 0; j < 32; j += 4)
+                                    if (j < w) o[j / 4] = *reinterpret_cast<const float4*>(p + j);
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) v[j] += o[j / 4].x, v[j + 1] += o[j / 4].y, v[j + 2] += o[j / 4].z, v[j + 3] += o[j / 4].w;
                             }
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                if (j < w) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                         } else {
                             bf16* p = job.out + (long)row * job.n + col;
 #pragma unroll
-                            for (int j = 0; j < 32; j += 8) Vec<bf16, true>::store(p + j, v + j);
+                            for (int j = 0; j < 32; j += 8)
+                                if (j < w) Vec<bf16, true>::store(p + j, v + j);
                         }
                     }
                 }
@@ -786,7 +805,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ a
             if (at >= 0) {
                 const float* p = acc + at * n + c * W;
                 Vec<float, VEC>::load(p, s);
-                constexpr int AT_ONCE = VEC ? 2 : 8;  // in flight, added in order
+                constexpr int AT_ONCE = VEC ? 4 : 8;  // in flight, added in order
                 for (int k0 = 1; k0 < splits; k0 += AT_ONCE) {
                     float v[AT_ONCE][W];
 #pragma unroll
@@ -850,9 +869,12 @@ Job job_of(long m, long n, long k, int splits) {
 template <int EPI, int BN, bool TOP>
 int gemm_bn(const Maps& maps, const Gemm& g, cudaStream_t s) {
     auto* kern = gemm_kernel<EPI, BN, TOP>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<EPI, BN>::bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
+    size_t bytes = Tile<EPI, BN>::bytes;
+    for (const Job& j : g.job)
+        if (EPI == OUT && j.units && exchanged(j)) bytes = Tile<EPI, BN>::bytes + EPW * Tile<EPI, BN>::SHARE;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return EWS_ERR_LAUNCH;
     const long units = g.job[0].units + g.job[1].units;
-    kern<<<(unsigned)(units < SMS ? units : SMS), NTH, Tile<EPI, BN>::bytes, s>>>(maps, g);
+    kern<<<(unsigned)(units < SMS ? units : SMS), NTH, bytes, s>>>(maps, g);
     return cudaGetLastError() == cudaSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
