@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(NTH) gemm_kernel(const __grid_constant__ Maps 
                                 for (int j = 0; j < 32; j += 4)
                                     if (j < w) o[j / 4] = *reinterpret_cast<const float4*>(p + j);
 #pragma unroll
-                                for (int j = 0; j < 32; j += 4) v[j] += o[j / 4].x, v[j + 1] += o[j / 4].y, v[j + 2] += o[j / 4].z, v[j + 3] += o[j / 4].w;
+                                for (int j = 0; j < 32; j += 4)
+                                    if (j < w) v[j] += o[j / 4].x, v[j + 1] += o[j / 4].y, v[j + 2] += o[j / 4].z, v[j + 3] += o[j / 4].w;
                             }
 #pragma unroll
                             for (int j = 0; j < 32; j += 4)
